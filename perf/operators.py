@@ -1,0 +1,404 @@
+"""Differential attention and layer norm: the calls whose speed counts, and their plain forms.
+
+Kinds of cases and what a program uses them for:
+
+* ``attend``: ``differential_attention`` of whole sequences without gradients,
+  on the strided head views of a projection: prompts, encoder inference;
+* ``train``: the same with the gradients of q, k, v and the second map's weight;
+* ``cached``: ``differential_attention_cached``, one or a few new tokens of each
+  sequence against its key and value cache;
+* ``norm``: ``layer_norm`` without gradients;
+* ``norm_train``: the same with the gradients of the rows, weight and bias.
+
+Head ``h`` of differential attention is ``(P_0 - lam P_1) V`` with ``P_m`` the
+softmax of ``scale q_{2h+m} k_{2h+m}^T``. With ``own`` false, ``run`` computes
+the operators in float32 from elementary torch operations; ``exact`` restates
+them in float64.
+"""
+
+import math
+
+import torch
+
+own = False
+
+DTYPES = {"fp32": torch.float32, "fp16": torch.float16, "bf16": torch.bfloat16}
+
+
+def listed():
+    return [
+        # One layer of the smallest encoder, a padded batch of two: launches count.
+        {"name": "attend_short", "kind": "attend", "batch": 2, "heads": 4, "kv_heads": 4, "seq": 128, "dim": 32,
+         "dim_v": 64, "dtype": "fp32", "causal": True, "padded": True, "shared": True},
+        # One layer over two long documents (d_model 1024 in eight pairs of heads).
+        {"name": "attend_long", "kind": "attend", "batch": 2, "heads": 8, "kv_heads": 8, "seq": 8192, "dim": 64,
+         "dim_v": 128, "dtype": "bf16", "causal": True, "padded": False, "shared": True},
+        # Bidirectional encoding of a padded batch whose lengths fit no tile; wide heads, shared keys.
+        {"name": "attend_padded_odd", "kind": "attend", "batch": 5, "heads": 6, "kv_heads": 2, "seq": 1237, "dim": 128,
+         "dim_v": 256, "dtype": "fp16", "causal": False, "padded": True, "shared": False},
+        # A training step's attention in the smallest encoder, float32 throughout.
+        {"name": "train_short", "kind": "train", "batch": 2, "heads": 4, "kv_heads": 4, "seq": 128, "dim": 32,
+         "dim_v": 64, "dtype": "fp32", "causal": True, "padded": True, "shared": True},
+        # A training step's attention in the ordinary encoder (d_model 512), padded sequences.
+        {"name": "train_ordinary", "kind": "train", "batch": 8, "heads": 4, "kv_heads": 4, "seq": 1024, "dim": 64,
+         "dim_v": 128, "dtype": "fp16", "causal": True, "padded": True, "shared": True},
+        # A training step's attention over long sequences, pairs of query heads on shared keys.
+        {"name": "train_long", "kind": "train", "batch": 2, "heads": 8, "kv_heads": 4, "seq": 4096, "dim": 64,
+         "dim_v": 128, "dtype": "bf16", "causal": True, "padded": False, "shared": False},
+        # The next token of one short sequence: latency.
+        {"name": "cached_one", "kind": "cached", "batch": 1, "heads": 8, "kv_heads": 8, "new": 1, "capacity": 1024,
+         "dim": 64, "dim_v": 128, "dtype": "fp16", "shared": True},
+        # The next tokens of sixteen long conversations of different lengths, shared keys.
+        {"name": "cached_batch", "kind": "cached", "batch": 16, "heads": 16, "kv_heads": 4, "new": 1,
+         "capacity": 65536, "dim": 64, "dim_v": 128, "dtype": "bf16", "shared": True},
+        # The norm before a layer of the smallest encoder.
+        {"name": "norm_short", "kind": "norm", "rows": 256, "width": 256, "dtype": "fp32", "params": "fp32"},
+        # A training step's norm in the ordinary encoder.
+        {"name": "norm_train_ordinary", "kind": "norm_train", "rows": 8192, "width": 512, "dtype": "fp32",
+         "params": "fp32"},
+        # A training step's norm over a large batch of a wide model, float32 parameters.
+        {"name": "norm_train_large", "kind": "norm_train", "rows": 65536, "width": 2048, "dtype": "bf16",
+         "params": "fp32"},
+        # The norm of each head's attention output in a training step (rows of one head).
+        {"name": "norm_train_heads", "kind": "norm_train", "rows": 131072, "width": 128, "dtype": "fp16",
+         "params": "fp32"},
+    ]
+
+
+def _log_int(rng, low, high):
+    return int(round(math.exp(rng.uniform(math.log(low), math.log(high)))))
+
+
+def _draw_heads(rng):
+    dim = rng.choice((32, 32, 64, 64, 64, 128, 128, 40, 16))
+    kv_heads = rng.choice((1, 2, 3, 4, 8))
+    return {"heads": kv_heads * rng.choice((1, 1, 1, 2, 3, 4)), "kv_heads": kv_heads, "dim": dim, "dim_v": 2 * dim,
+            "dtype": rng.choice(("fp32", "fp16", "fp16", "bf16", "bf16")), "shared": rng.random() < 0.5}
+
+
+def draw(rng):
+    kind = rng.choice(("attend", "attend", "train", "train", "train", "cached", "cached", "norm", "norm_train",
+                       "norm_train"))
+    if kind in ("norm", "norm_train"):
+        while True:
+            width = rng.choice((_log_int(rng, 16, 8192), 64 * _log_int(rng, 1, 128), 2 ** rng.randint(5, 13)))
+            case = {"kind": kind, "rows": _log_int(rng, 1, 131072), "width": width,
+                    "dtype": rng.choice(("fp32", "fp16", "bf16")), "params": rng.choice(("fp32", "same", "none"))}
+            if case["rows"] * case["width"] <= 65536 * 2048:
+                return case
+    limit = max(work(c)["flops"] for c in listed() if c["kind"] == kind)
+    while True:
+        case = {"kind": kind, "batch": _log_int(rng, 1, 32), **_draw_heads(rng)}
+        if kind == "cached":
+            case.update(capacity=_log_int(rng, 16, 65536), new=rng.choice((1, 1, 1, 2, 5, 16)))
+            # Cache bytes bound these calls.
+            rows = case["batch"] * case["kv_heads"] * case["capacity"]
+            if rows * 4 * case["dim"] <= 16 * 4 * 65536 * 256:
+                return case
+            continue
+        case.update(seq=_log_int(rng, 16, 8192), causal=rng.random() < 0.7, padded=rng.random() < 0.5)
+        # float32 products run at a sixteenth of the 16-bit rate.
+        if work(case)["flops"] * (16 if case["dtype"] == "fp32" else 1) <= limit:
+            return case
+
+
+# -- what a program has in hand ---------------------------------------------
+
+def _lengths(case):
+    """The valid lengths of a padded batch, from the whole sequence down to a quarter, or None."""
+    b = case["batch"]
+    longest = case["capacity"] if case["kind"] == "cached" else case["seq"]
+    if case["kind"] != "cached" and not case["padded"]:
+        return None
+    if case["kind"] == "cached":
+        # Room for the new tokens at the least.
+        return [max(case["new"], longest - (longest - longest // 4) * i // b) for i in range(b)]
+    lengths = [longest - (longest - longest // 4) * i // b for i in range(b)]
+    if b > 6:
+        lengths[-1] = 0  # a filler row of a batch of fixed size
+    return lengths
+
+
+def _heads(g, batch, heads, seq, dim, dtype, std):
+    """A [B, H, S, D] view of [B, S, H, D] storage, as a projection gives it."""
+    x = torch.randn(batch, seq, heads, dim, generator=g, device="cuda")
+    return (x * std).to(dtype).transpose(1, 2)
+
+
+def prepare(case, seed):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    kind, dtype = case["kind"], DTYPES[case["dtype"]]
+    state = {"case": case}
+    if kind in ("norm", "norm_train"):
+        rows, width = case["rows"], case["width"]
+        # A residual stream: channels of different size and offset.
+        size = torch.exp(0.5 * torch.randn(width, generator=g, device="cuda"))
+        offset = 0.5 * torch.randn(width, generator=g, device="cuda")
+        state["x"] = (torch.randn(rows, width, generator=g, device="cuda") * size + offset).to(dtype)
+        state["weight"] = state["bias"] = None
+        if case["params"] != "none":
+            params = torch.float32 if case["params"] == "fp32" else dtype
+            state["weight"] = (1 + 0.2 * torch.randn(width, generator=g, device="cuda")).to(params)
+            state["bias"] = (0.1 * torch.randn(width, generator=g, device="cuda")).to(params)
+        if kind == "norm_train":
+            state["dout"] = (0.1 * torch.randn(rows, width, generator=g, device="cuda")).to(dtype)
+            for name in ("x", "weight", "bias"):
+                if state[name] is not None:
+                    state[name].requires_grad_()
+        return state
+    b, h, hk, d, dv = (case[n] for n in ("batch", "heads", "kv_heads", "dim", "dim_v"))
+    n = 1 if case["shared"] else h
+    lam = 0.2 + 0.6 * torch.rand(n, generator=g, device="cuda")
+    state["lam"] = lam.reshape(()) if case["shared"] else lam
+    lengths = _lengths(case)
+    state["lengths"] = None
+    if lengths is not None:
+        order = torch.randperm(b, generator=torch.Generator().manual_seed(seed))
+        state["lengths"] = torch.tensor(lengths, dtype=torch.int32)[order].cuda()
+    if kind == "cached":
+        cap = case["capacity"]
+        state["q"] = _heads(g, b, 2 * h, case["new"], d, dtype, 1.5)
+        state["k"] = torch.empty(b, 2 * hk, cap, d, dtype=dtype, device="cuda").normal_(generator=g)
+        state["v"] = torch.empty(b, hk, cap, dv, dtype=dtype, device="cuda").normal_(generator=g)
+        return state
+    s = case["seq"]
+    state["q"] = _heads(g, b, 2 * h, s, d, dtype, 1.5)
+    state["k"] = _heads(g, b, 2 * hk, s, d, dtype, 1.0)
+    state["v"] = _heads(g, b, hk, s, dv, dtype, 1.0)
+    if kind == "train":
+        state["dout"] = _heads(g, b, h, s, dv, dtype, 0.1)
+        for name in ("q", "k", "v", "lam"):
+            state[name] = state[name].detach().requires_grad_()
+    return state
+
+
+# -- one pass -----------------------------------------------------------------
+
+def run(state):
+    if own:
+        return _run_own(state)
+    case = state["case"]
+    with torch.no_grad():
+        if case["kind"] == "norm":
+            return _plain_norm(state["x"], state["weight"], state["bias"])[0]
+        if case["kind"] == "norm_train":
+            return _plain_norm_train(state)
+        return _plain_attention(state)
+
+
+def _run_own(state):
+    from techjam_amd.kernels import differential_attention, differential_attention_cached, layer_norm
+
+    case = state["case"]
+    kind = case["kind"]
+    if kind == "norm":
+        with torch.no_grad():
+            return layer_norm(state["x"], state["weight"], state["bias"])
+    if kind == "norm_train":
+        leaves = [state[n] for n in ("x", "weight", "bias") if state[n] is not None]
+        out = layer_norm(state["x"], state["weight"], state["bias"])
+        return [out.detach(), *torch.autograd.grad(out, leaves, state["dout"])]
+    q, k, v, lam, lengths = (state[n] for n in ("q", "k", "v", "lam", "lengths"))
+    if kind == "cached":
+        with torch.no_grad():
+            return differential_attention_cached(q, k, v, lam, lengths)
+    if kind == "attend":
+        with torch.no_grad():
+            return differential_attention(q, k, v, lam, is_causal=case["causal"], valid_len=lengths)
+    out = differential_attention(q, k, v, lam, is_causal=case["causal"], valid_len=lengths)
+    return [out.detach(), *torch.autograd.grad(out, (q, k, v, lam), state["dout"])]
+
+
+def _plain_norm(x, weight, bias, eps=1e-5):
+    x = x.float()
+    centred = x - x.mean(-1, keepdim=True)
+    rstd = torch.rsqrt((centred * centred).mean(-1, keepdim=True) + eps)
+    normed = centred * rstd
+    y = normed if weight is None else normed * weight.float() + bias.float()
+    return y, normed, rstd
+
+
+def _plain_norm_train(state):
+    x, weight, bias = state["x"], state["weight"], state["bias"]
+    y, normed, rstd = _plain_norm(x, weight, bias)
+    dy = state["dout"].float()
+    g = dy if weight is None else dy * weight.float()
+    dx = rstd * (g - g.mean(-1, keepdim=True) - normed * (g * normed).mean(-1, keepdim=True))
+    out = [y.to(x.dtype), dx.to(x.dtype)]
+    if weight is not None:
+        out += [(dy * normed).sum(0).to(weight.dtype), dy.sum(0).to(bias.dtype)]
+    return out
+
+
+def _visible(case, lengths, b, device):
+    """Truth values [rows, keys] of one sequence: which keys each row's softmax runs over."""
+    if case["kind"] == "cached":
+        n = lengths[b]
+        pos = n - case["new"] + torch.arange(case["new"], device=device)
+        return torch.arange(case["capacity"], device=device)[None, :] <= pos[:, None]
+    i = torch.arange(case["seq"], device=device)
+    seen = (i[None, :] <= i[:, None]) if case["causal"] else torch.ones(case["seq"], case["seq"], dtype=torch.bool,
+                                                                        device=device)
+    if lengths is not None:
+        seen = seen & (i[None, :] < lengths[b]) & (i[:, None] < lengths[b])
+    return seen
+
+
+def _plain_softmax(scores, seen):
+    scores = torch.where(seen, scores, torch.full_like(scores, -math.inf))
+    top = scores.max(-1, keepdim=True).values
+    e = torch.exp(scores - torch.where(torch.isinf(top), torch.zeros_like(top), top))
+    total = e.sum(-1, keepdim=True)
+    return e / torch.where(total == 0, torch.ones_like(total), total)
+
+
+def _plain_attention(state):
+    """One sequence at a time, its heads together: products, exponentials and sums in float32."""
+    case = state["case"]
+    q, k, v, lam, lengths = (state[n] for n in ("q", "k", "v", "lam", "lengths"))
+    b_all, h2, rows, d = q.shape
+    h, hk = h2 // 2, k.shape[1] // 2
+    g, dv, keys = h // hk, v.shape[-1], k.shape[2]
+    scale = d ** -0.5
+    train = case["kind"] == "train"
+    out = torch.empty(b_all, h, rows, dv, dtype=q.dtype, device=q.device)
+    if train:
+        dq, dk, dvv = (torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k, v))
+        dlam = torch.zeros(h, device=q.device)
+    weight = lam.expand(h).reshape(hk, g, 1, 1)
+    for b in range(b_all):
+        seen = _visible(case, lengths, b, q.device)
+        # [kv head, map, group, row, dim]
+        qb = q[b].float().reshape(hk, g, 2, rows, d).transpose(1, 2)
+        kb = k[b].float().reshape(hk, 2, 1, keys, d)
+        vb = v[b].float().reshape(hk, 1, keys, dv)
+        if case["kind"] == "cached":  # whatever lies behind a sequence's end takes no part
+            live = seen.any(0)
+            kb = torch.where(live[:, None], kb, torch.zeros_like(kb))
+            vb = torch.where(live[:, None], vb, torch.zeros_like(vb))
+        p = _plain_softmax(torch.matmul(qb, kb.transpose(-1, -2)) * scale, seen)
+        p0, p1 = p[:, 0], p[:, 1]
+        mixed = p0 - weight * p1
+        out[b] = torch.matmul(mixed, vb).reshape(h, rows, dv).to(out.dtype)
+        if not train:
+            continue
+        do = state["dout"][b].float().reshape(hk, g, rows, dv)
+        if lengths is not None:
+            do = torch.where((torch.arange(rows, device=q.device) < lengths[b])[:, None], do, torch.zeros_like(do))
+        dvv[b] = torch.matmul(mixed.transpose(-1, -2), do).sum(1).to(dvv.dtype)
+        del mixed
+        dp = torch.matmul(do, vb.transpose(-1, -2))
+        total = (p * dp[:, None]).sum(-1, keepdim=True)
+        dlam -= total[:, 1].sum((-1, -2)).reshape(h)
+        ds = p * (dp[:, None] - total)
+        del p, p0, p1, dp
+        ds[:, 1] *= -weight
+        ds *= scale
+        dq[b] = torch.matmul(ds, kb).transpose(1, 2).reshape(h2, rows, d).to(dq.dtype)
+        dk[b] = torch.matmul(ds.transpose(-1, -2), qb).sum(2).reshape(2 * hk, keys, d).to(dk.dtype)
+    if not train:
+        return out
+    return [out, dq, dk, dvv, dlam.sum() if lam.ndim == 0 else dlam]
+
+
+# -- what a pass cannot do without --------------------------------------------
+
+def _pairs(case):
+    """(rows, keys) pairs of one head over the batch, and valid tokens."""
+    lengths = _lengths(case)
+    if case["kind"] == "cached":
+        t = case["new"]
+        return sum(t * n - t * (t - 1) // 2 for n in lengths), sum(lengths)
+    if lengths is None:
+        lengths = [case["seq"]] * case["batch"]
+    return sum(n * (n + 1) // 2 if case["causal"] else n * n for n in lengths), sum(lengths)
+
+
+def work(case):
+    size = 4 if case["dtype"] == "fp32" else 2
+    if case["kind"] in ("norm", "norm_train"):
+        n, train = case["rows"] * case["width"], case["kind"] == "norm_train"
+        params = 0 if case["params"] == "none" else 2 * case["width"] * (4 if case["params"] == "fp32" else size)
+        # Forward: mean, variance, scale and shift. Backward: two row sums, two column sums, the row's gradient.
+        return {"bytes": float(n * size * (4 if train else 2) + params * (2 if train else 1)),
+                "flops": float(n * (8 + (14 if train else 0)))}
+    pairs, tokens = _pairs(case)
+    h, hk, d, dv = (case[n] for n in ("heads", "kv_heads", "dim", "dim_v"))
+    keys = tokens * hk * (2 * d + dv)
+    if case["kind"] == "cached":
+        rows = case["batch"] * case["new"]
+        return {"bytes": float(size * (keys + rows * h * (2 * d + dv))), "flops": float(pairs * h * (4 * d + 2 * dv))}
+    rows = tokens * h
+    written = case["batch"] * case["seq"] * h * dv
+    bytes_ = size * (keys + rows * 2 * d + written)
+    flops = pairs * h * (4 * d + 2 * dv)
+    if case["kind"] == "train":
+        bytes_ += size * (rows * dv + case["batch"] * case["seq"] * (2 * h * d + hk * (2 * d + dv)))
+        flops += pairs * h * (8 * d + 4 * dv)
+    return {"bytes": float(bytes_), "flops": float(flops)}
+
+
+# -- the definition in 64 bits --------------------------------------------------
+
+def exact(case, seed):
+    state = prepare(case, seed)
+    if case["kind"] in ("norm", "norm_train"):
+        return _exact_norm(state)
+    return _exact_attention(state)
+
+
+def _exact_norm(state):
+    train = state["case"]["kind"] == "norm_train"
+    leaves = [state[n].detach().double() for n in ("x", "weight", "bias") if state[n] is not None]
+    if train:
+        leaves = [t.requires_grad_() for t in leaves]
+    var, mean = torch.var_mean(leaves[0], -1, correction=0, keepdim=True)
+    y = (leaves[0] - mean) / torch.sqrt(var + 1e-5)
+    if len(leaves) == 3:
+        y = y * leaves[1] + leaves[2]
+    if not train:
+        return y
+    return [y.detach(), *torch.autograd.grad(y, leaves, state["dout"].double())]
+
+
+def _exact_attention(state):
+    """One head of one sequence at a time, over its own keys alone, with torch's own gradients."""
+    case, lengths = state["case"], state["lengths"]
+    train = case["kind"] == "train"
+    q, k, v, lam = (state[n].detach() for n in ("q", "k", "v", "lam"))
+    b_all, h2, rows, d = q.shape
+    h, hk, dv = h2 // 2, k.shape[1] // 2, v.shape[-1]
+    f64 = dict(dtype=torch.float64, device=q.device)
+    out = torch.zeros(b_all, h, rows, dv, **f64)
+    grads = [torch.zeros(t.shape, **f64) for t in (q, k, v)] + [torch.zeros(h, **f64)]
+    for b in range(b_all):
+        n = k.shape[2] if lengths is None else int(lengths[b])
+        first = n - case["new"] if case["kind"] == "cached" else 0
+        m = min(rows, n - first)
+        if m <= 0:
+            continue
+        for head in range(h):
+            kv = head // (h // hk)
+            leaves = [q[b, 2 * head:2 * head + 2, :m].double(), k[b, 2 * kv:2 * kv + 2, :n].double(),
+                      v[b, kv, :n].double(), lam.reshape(-1)[head if lam.ndim else 0].double()]
+            if train:
+                leaves = [t.requires_grad_() for t in leaves]
+            qs, ks, vs, weight = leaves
+            scores = qs @ ks.mT / math.sqrt(d)
+            if case["kind"] == "cached" or case["causal"]:
+                later = torch.ones(m, n, dtype=torch.bool, device=q.device).triu(first + 1)
+                scores = scores.masked_fill(later, -math.inf)
+            maps = torch.softmax(scores, -1)
+            del scores
+            o = (maps[0] - weight * maps[1]) @ vs
+            out[b, head, :m] = o.detach()
+            if train:
+                dq, dk, dvv, dl = torch.autograd.grad(o, leaves, state["dout"][b, head, :m].double())
+                grads[0][b, 2 * head:2 * head + 2, :m] += dq
+                grads[1][b, 2 * kv:2 * kv + 2, :n] += dk
+                grads[2][b, kv, :n] += dvv
+                grads[3][head] += dl
+            del maps, o
+    if not train:
+        return out
+    return [out, *grads[:3], grads[3].sum() if lam.ndim == 0 else grads[3]]
