@@ -44,6 +44,7 @@ extern "C" {
 /* Element types of the tensor arguments. */
 #define TJ_F32 0
 #define TJ_F16 1
+#define TJ_BF16 2 /* differential attention and layer norm only */
 
 /* ABI version, bumped on any signature or semantic change. */
 int tj_abi_version(void);
@@ -374,6 +375,90 @@ int tj_narrow_ffn_norm(const float* x, const float* w_in, const float* bias_in, 
                        const float* bias, const float* resid, float* out, int64_t M, int64_t seq_len,
                        const int32_t* valid_len, int mode, const float* gamma, const float* beta,
                        float* ln_out, float eps, int zero_ln_padded, hipStream_t stream);
+
+/*
+ * Differential attention, forward. No counterpart in the reference; it stands
+ * beside tj_attn_fwd. Head h of H is the difference of two softmax maps,
+ *
+ *   o[b,h,i,:] = sum_j (P_0[i,j] - lam[h] P_1[i,j]) v[b,h',j,:]
+ *   P_m[i,j]   = softmax_j(scale * q[b,2h+m,i,:] . k[b,2h'+m,j,:]),   h' = h / (H / Hk)
+ *
+ * q [B, 2H, Sq, D], k [B, 2Hk, Sk, D], v [B, Hk, Sk, Dv], o [B, H, Sq, Dv];
+ * H a multiple of Hk. lam: device fp32, one weight per head (lam_step 1) or
+ * one for all (lam_step 0).
+ *
+ * cached 0: whole sequences, Sq == Sk. Keys j < lengths[b] (all when lengths is
+ * NULL) and, when `causal`, j <= i; rows i >= lengths[b] are written as zeros.
+ * cached 1: the Sq last tokens of sequences whose keys and values lie in a cache
+ * of capacity Sk: lengths[b] counts the keys, these tokens' own among them, and
+ * token i sees the keys up to its position lengths[b] - Sq + i. Tokens at a
+ * negative position are written as zeros. Lengths are clipped to 0 .. Sk; what
+ * lies behind them is not read, whatever it holds.
+ *
+ * dtype: TJ_F32, TJ_F16 or TJ_BF16, shared by q, k, v and o. Products of 16-bit
+ * inputs run on MFMAs of that type with fp32 accumulation (probabilities are
+ * rounded to it for the product with v), those of fp32 inputs in fp32; the
+ * softmax runs in fp32. D <= 128, Dv <= 256, both multiples of 16 bytes.
+ *
+ * lse and maps, both or neither: what tj_diff_attn_bwd reads again, contiguous
+ * fp32: with R = Sq * H / Hk rows i * H / Hk + h % (H / Hk) per key head, the
+ * rows' softmax sums [B, Hk, 2, R] and the two maps' outputs [B, Hk, R, 2, Dv].
+ *
+ * workspace: tj_diff_attn_workspace_bytes bytes, 16-byte aligned, contents
+ * irrelevant, calls sharing one ordered on one stream: where few rows sweep many
+ * keys, the keys are cut into parts whose sums a second kernel joins. With 0
+ * bytes, or whole sequences, it may be NULL (every sweep then runs whole).
+ */
+size_t tj_diff_attn_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t Sq, int64_t Sk, int64_t Dv, int cached);
+int tj_diff_attn_fwd(const void* q, const void* k, const void* v, void* o, int dtype,
+                     int64_t B, int64_t H, int64_t Hk, int64_t Sq, int64_t Sk, int64_t D, int64_t Dv,
+                     const int64_t q_strides[4], const int64_t k_strides[4],
+                     const int64_t v_strides[4], const int64_t o_strides[4],
+                     float scale, int causal, int cached, const float* lam, int64_t lam_step,
+                     const int32_t* lengths, float* lse, float* maps,
+                     void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/*
+ * The gradients of tj_diff_attn_fwd (cached 0, Sq == Sk == S) for the output
+ * gradient dout [B, H, S, Dv]: dq, dk, dv (shaped and typed like q, k, v) and
+ * dlam, fp32 [H] or [1] as lam_step says, summed over what shares a weight.
+ * maps and lse come from the forward call. Rows at or past lengths[b] get zeros
+ * and their dout is not read. The sums' order is fixed: the same call gives the
+ * same bits. workspace as above, tj_diff_attn_bwd_workspace_bytes bytes, needed.
+ */
+size_t tj_diff_attn_bwd_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t S);
+int tj_diff_attn_bwd(const void* q, const void* k, const void* v, const float* maps, const float* lse,
+                     const void* dout, void* dq, void* dk, void* dv, float* dlam, int dtype,
+                     int64_t B, int64_t H, int64_t Hk, int64_t S, int64_t D, int64_t Dv,
+                     const int64_t q_strides[4], const int64_t k_strides[4],
+                     const int64_t v_strides[4], const int64_t do_strides[4],
+                     const int64_t dq_strides[4], const int64_t dk_strides[4], const int64_t dv_strides[4],
+                     float scale, int causal, const float* lam, int64_t lam_step, const int32_t* lengths,
+                     void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/*
+ * Layer norm of rows, forward and backward (torch.nn.LayerNorm's formula over
+ * the last dimension, torch_transformer_benchmark.py:125-172, where the norms
+ * are torch's):
+ *   y = (x - mean) * rstd * weight + bias,  rstd = 1 / sqrt(var + eps)
+ * x, y, dy, dx: [rows, cols] of dtype (TJ_F32, TJ_F16 or TJ_BF16), unit column
+ * stride, any row stride (in elements), aligned to one element. weight, bias
+ * and their gradients: [cols] of w_dtype, TJ_F32 or dtype; each may be NULL
+ * (weight 1, bias 0). Sums are fp32. cols at most 16384.
+ * mean, rstd: fp32 [rows], both or neither in the forward call, what the
+ * backward call reads. In the backward call dx, dweight and dbias may each be
+ * NULL; with either of the latter it needs tj_layer_norm_bwd_workspace_bytes
+ * bytes of workspace (4-byte aligned, contents irrelevant). With no rows nothing
+ * is written. y may not overlap x, nor dx any input.
+ */
+int tj_layer_norm_fwd(const void* x, const void* weight, const void* bias, void* y, int dtype, int w_dtype,
+                      int64_t rows, int64_t cols, int64_t x_stride, int64_t y_stride, float eps,
+                      float* mean, float* rstd, hipStream_t stream);
+size_t tj_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t cols);
+int tj_layer_norm_bwd(const void* dy, const void* x, const void* weight, const float* mean, const float* rstd,
+                      void* dx, void* dweight, void* dbias, int dtype, int w_dtype, int64_t rows, int64_t cols,
+                      int64_t dy_stride, int64_t x_stride, int64_t dx_stride,
+                      void* workspace, size_t workspace_bytes, hipStream_t stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,300 @@
+// Differential attention for gfx950: shared by its forward, backward and
+// cached kernels (diff_attn_fwd.hip, diff_attn_bwd_kv.hip, diff_attn_bwd_q.hip,
+// diff_attn.hip).
+//
+// Head h of H is the difference of two softmax maps over one value head,
+//
+//   O_h = (P_0 - lam_h P_1) V,   P_m = softmax(scale Q_{2h+m} K_{2h'+m}^T),
+//
+// with h' = h / G the key head that G = H / Hk query heads share. The G heads
+// of one key head are handled together: their query rows are numbered
+// r = i G + g (token i, head g of the group), so that neighbouring rows see
+// nearly the same keys, one sweep over K and V serves the whole group, and the
+// sums over the group in dK and dV are sums over rows.
+//
+// Element types: fp16 and bf16 run 32x32x16 MFMAs, fp32 runs 32x32x2 fp32
+// MFMAs (1/16 of the rate; nothing is rounded to fewer bits). The three share
+// every kernel: an operand fragment is 8 consecutive k of one row or column
+// per lane, and fp32 contracts it with eight MFMAs, one k of each lane half
+// at a time, which only reorders the sum.
+#pragma once
+
+#include "tj_common.h"
+
+typedef __bf16 bf16_t;
+typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+
+namespace tj {
+
+struct DiffArgs {
+  const void *q, *k, *v;
+  void* o;
+  float* maps;             // [B, Hk, R, 2, Dv] P_0 V and P_1 V for the backward pass, or null
+  View4 vq, vk, vv, vo;
+  int B, H, Hk, G, D, Dv;
+  int Sq, Sk;              // query tokens, key tokens (capacity of a cache)
+  int R;                   // rows of one key head: Sq * G
+  float scale;
+  int causal;
+  int cached;              // token i stands at position len - Sq + i instead of i
+  const float* lam;
+  int lam_step;            // elements between the weights of two heads: 0 or 1
+  const int32_t* len;      // [B] or null
+  float* lse;              // [B, Hk, 2, R] log2 of a row's sum of 2^(score log2 e), +inf for empty rows; or null
+  int n_mtiles;
+  // Key parts: part p covers keys p part_keys .. (p + 1) part_keys - 1 and leaves unnormalised sums
+  // [n_parts, B, Hk, R, 2, Dv] and (maximum, sum) pairs [n_parts, B, Hk, R, 2, 2].
+  int part_keys, n_parts;
+  float *part_o, *part_ml;
+  // Backward.
+  const void* dout;
+  View4 vdo, vdq, vdk, vdv;
+  void *dq, *dk, *dv;
+  float* dlam;             // [H], or [1] when lam_step is 0
+  int n_lam;
+  float* delta;            // [B, Hk, 2, R] rowsum(dO o O_m)
+  float* gsum;             // [B, Hk, R] rowsum(P_1 o dP), the row's part of -dlam
+  float* peak;             // [B, Hk, 2, kPeakParts] largest norms of dO and V rows (fp16 operands)
+  int n_peaks;
+};
+
+constexpr int kPeakParts = 64;
+constexpr int kDiffThreads = 256;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kDiffBufferFlags = 0x00020000;  // raw buffer resource word 3 on gfx950
+
+template <typename T>
+struct Elem;
+
+template <>
+struct Elem<half_t> {
+  typedef half8_t frag;
+  static constexpr bool kWide = false;
+  // 2^6: unnormalised probabilities reach 2^(6+8) with the lazy maximum, below
+  // fp16's largest value, and keep 11 bits down to 2^-20 of the row's maximum.
+  static constexpr float kLift = 6.f;
+  __device__ __forceinline__ static float16_t mma(frag a, frag b, float16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+  }
+};
+
+template <>
+struct Elem<bf16_t> {
+  typedef bf16x8_t frag;
+  static constexpr bool kWide = false;
+  static constexpr float kLift = 0.f;
+  __device__ __forceinline__ static float16_t mma(frag a, frag b, float16_t c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+  }
+};
+
+template <>
+struct Elem<float> {
+  typedef float8_t frag;
+  static constexpr bool kWide = true;
+  static constexpr float kLift = 0.f;
+  __device__ __forceinline__ static float16_t mma(frag a, frag b, float16_t c) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], b[e], c, 0, 0, 0);
+    return c;
+  }
+};
+
+template <typename T>
+using frag_t = typename Elem<T>::frag;
+
+__device__ __forceinline__ float16_t zero16() {
+  float16_t z;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) z[r] = 0.f;
+  return z;
+}
+
+// Accumulator row of register r in lane half hl (see mfma32 in tj_common.h).
+__device__ __forceinline__ constexpr int acc_row(int r, int hl) { return 8 * (r / 4) + 4 * hl + r % 4; }
+
+// Registers 8s .. 8s+7 of an accumulator as the operand fragment that
+// contracts its rows 16s .. 16s+15: k-slot (hl, j) stands for accumulator row
+// acc_row(8s + j, hl). Rounded to T.
+template <typename T>
+__device__ __forceinline__ frag_t<T> acc_frag(const float16_t& c, int s) {
+  frag_t<T> f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) f[j] = (T)c[8 * s + j];
+  return f;
+}
+
+// An LDS tile: rows of W elements, 16 bytes of padding after each.
+template <typename T, int W>
+struct LdsRows {
+  static constexpr int kVec = 16 / (int)sizeof(T);
+  static constexpr int kStride = W + kVec;
+  static constexpr int kChunks = W / kVec;
+
+  // The fragment of eight consecutive elements of one row.
+  __device__ __forceinline__ static frag_t<T> row_frag(const T* t, int row, int k) {
+    const T* p = t + row * kStride + k;
+    if constexpr (sizeof(T) == 4) {
+      const float4_t a = *reinterpret_cast<const float4_t*>(p), b = *reinterpret_cast<const float4_t*>(p + 4);
+      return frag_t<T>{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    } else {
+      return *reinterpret_cast<const frag_t<T>*>(p);
+    }
+  }
+
+  // The fragment that contracts rows row0 .. row0+15 in acc_frag's order, for
+  // column col0 + lane % 32. 16-bit elements come through the transposing LDS
+  // read: sixteen lanes name 4 rows x 16 columns, lane j of them gets column j.
+  __device__ __forceinline__ static frag_t<T> col_frag(const T* t, int row0, int col0, int lane) {
+    const int hl = lane / 32;
+    if constexpr (sizeof(T) == 4) {
+      const float* p = t + (row0 + 4 * hl) * kStride + col0 + lane % 32;
+      frag_t<T> f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = p[(j / 4 * 8 + j % 4) * kStride];
+      return f;
+    } else {
+      typedef short short4_t __attribute__((ext_vector_type(4)));
+      typedef short short8_t __attribute__((ext_vector_type(8)));
+      typedef __attribute__((address_space(3))) short4_t lds_short4;
+      const T* p = t + (row0 + 4 * hl + (lane & 15) / 4) * kStride + col0 + (lane & 16) + 4 * (lane & 3);
+      const short4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)p);
+      const short4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(p + 8 * kStride));
+      return __builtin_bit_cast(frag_t<T>, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
+    }
+  }
+
+  // Rows 0 .. ROWS-1 from memory: row_ptr(row) is the row's address, null for
+  // one that reads as zeros; elements at or past `width` read as zeros too.
+  template <int ROWS, int THREADS = kDiffThreads, typename F>
+  __device__ __forceinline__ static void fill(T* t, int tid, int width, F&& row_ptr) {
+#pragma unroll
+    for (int u = 0; u < ROWS * kChunks; u += THREADS) {
+      const int e = u + tid;
+      if (ROWS * kChunks % THREADS == 0 || e < ROWS * kChunks) {
+        const int row = e / kChunks, c = e % kChunks * kVec;
+        const T* p = row_ptr(row);
+        float4_t x = {0.f, 0.f, 0.f, 0.f};
+        if (p != nullptr && c < width) x = *reinterpret_cast<const float4_t*>(p + c);
+        *reinterpret_cast<float4_t*>(t + row * kStride + c) = x;
+      }
+    }
+  }
+};
+
+// Eight consecutive elements of a row in memory, zeros at or past `width`.
+template <typename T>
+__device__ __forceinline__ frag_t<T> load_frag(const T* p, int k, int width) {
+  frag_t<T> f;
+  if constexpr (sizeof(T) == 4) {
+    float4_t a = {0.f, 0.f, 0.f, 0.f}, b = a;
+    if (p != nullptr && k < width) a = *reinterpret_cast<const float4_t*>(p + k);
+    if (p != nullptr && k + 4 < width) b = *reinterpret_cast<const float4_t*>(p + k + 4);
+    f = frag_t<T>{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) f[j] = (T)0.f;
+    if (p != nullptr && k < width) f = *reinterpret_cast<const frag_t<T>*>(p + k);
+  }
+  return f;
+}
+
+// Four consecutive values, rounded to T.
+template <typename T>
+__device__ __forceinline__ void store4t(T* p, float a, float b, float c, float d) {
+  if constexpr (sizeof(T) == 4) {
+    *reinterpret_cast<float4_t*>(p) = float4_t{a, b, c, d};
+  } else {
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    *reinterpret_cast<t4*>(p) = t4{(T)a, (T)b, (T)c, (T)d};
+  }
+}
+
+// Keys of sequence b, clipped to what is there; the same in every lane.
+__device__ __forceinline__ int diff_len(const DiffArgs& a, int b) {
+  const int n = a.len == nullptr ? a.Sk : min(a.Sk, max(0, a.len[b]));
+  return __builtin_amdgcn_readfirstlane(n);
+}
+
+// Products with fp16 operands: the power of two that brings the largest
+// possible |dS| (2 |dO_i| |V_j| max(1, |lam|) scale) near 2^15, so that small
+// gradients and small probabilities keep fp16's bits. 1 for the other types.
+template <typename T>
+__device__ __forceinline__ float ds_lift(const DiffArgs& a, int bh, int hk, int lane) {
+  if constexpr (!std::is_same<T, half_t>::value) {
+    return 1.f;
+  } else {
+    const float* pk = a.peak + (int64_t)bh * 2 * kPeakParts;
+    float x = lane < a.n_peaks ? pk[lane] : 0.f, y = lane < a.n_peaks ? pk[kPeakParts + lane] : 0.f;
+#pragma unroll
+    for (int m = 32; m > 0; m >>= 1) {
+      x = fmaxf(x, __shfl_xor(x, m));
+      y = fmaxf(y, __shfl_xor(y, m));
+    }
+    float w = 1.f;
+    for (int g = 0; g < a.G; ++g) {
+      const float l = fabsf(a.lam[(hk * a.G + g) * a.lam_step]);
+      if (l < 3e38f) w = fmaxf(w, l);
+    }
+    // Exponents rather than products: the norms' product may leave fp32.
+    int ex, ey, ew;
+    frexpf(x, &ex);
+    frexpf(y, &ey);
+    frexpf(w, &ew);
+    if (!(x > 0.f) || !(y > 0.f)) return 1.f;
+    return ldexpf(1.f, min(max(14 - ex - ey - ew, -100), 100));
+  }
+}
+
+// The same for P_0 - lam P_1 (at most 1 + |lam|).
+template <typename T>
+__device__ __forceinline__ float p_lift(float lam_max) {
+  if constexpr (!std::is_same<T, half_t>::value) {
+    return 1.f;
+  } else {
+    int e;
+    frexpf(1.f + lam_max, &e);
+    return ldexpf(1.f, min(max(15 - e, -100), 14));
+  }
+}
+
+// A workgroup's tile and (b, key head). Consecutive ids run on the XCDs in
+// turn, so the (b, key head) index varies fastest: with a multiple of eight of
+// them the tiles that share K and V also share an XCD's L2. Tiles with the
+// most keys come first.
+struct DiffTile {
+  int b, hk, bh, tile;
+};
+__device__ __forceinline__ DiffTile diff_tile(const DiffArgs& a, int id, int tiles) {
+  const int bhn = a.B * a.Hk;
+  DiffTile t;
+  t.bh = id % bhn;
+  t.tile = id / bhn;
+  t.b = t.bh / a.Hk;
+  t.hk = t.bh % a.Hk;
+  return t;
+}
+
+int diff_fwd(const DiffArgs& a, int dtype, hipStream_t stream);
+int diff_few_rows(const DiffArgs& a, int dtype, hipStream_t stream);
+int diff_bwd_kv(const DiffArgs& a, int dtype, hipStream_t stream);
+int diff_bwd_q(const DiffArgs& a, int dtype, hipStream_t stream);
+
+// f.operator()<T, HD, DVP>() for the smallest instance that holds D and Dv:
+// head dims up to 32, 64 or 128 with values up to twice as wide.
+template <typename F>
+int diff_dispatch(const DiffArgs& a, int dtype, F&& f) {
+  const int need = a.D > (a.Dv + 1) / 2 ? a.D : (a.Dv + 1) / 2;
+  auto by_dim = [&](auto t) {
+    using T = decltype(t);
+    if (need <= 32) return f(t, std::integral_constant<int, 32>{});
+    if (need <= 64) return f(t, std::integral_constant<int, 64>{});
+    return f(t, std::integral_constant<int, 128>{});
+  };
+  if (dtype == TJ_F32) return by_dim(float{});
+  if (dtype == TJ_F16) return by_dim(half_t{});
+  return by_dim(bf16_t{});
+}
+
+}  // namespace tj

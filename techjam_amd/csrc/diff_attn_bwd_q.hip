@@ -1,0 +1,257 @@
+// Differential attention, backward: the rows' sums delta_m = rowsum(dO o O_m)
+// beforehand, dQ, and the gradient of the second map's weight (the mathematics
+// and the row numbering are in diff_attn.h and diff_attn_bwd_kv.hip).
+//
+//   dQ_m = scale dS_m K_m,  dS_m = c_m P_m (dP - delta_m)
+//   dlam = - sum over rows of sum_j P_1 dP
+//
+// delta_m comes from the maps' outputs, which the forward pass keeps in fp32:
+// rounded to 16 bits they cost dQ and dK a twentieth of their accuracy (bf16,
+// causal, 1024 tokens, 64 dims: 2.56e-3 instead of 2.40e-3, relative 2-norm; the
+// rounding of dS and of the result is 2.38e-3). What is left of its error is the
+// rounding of P in the forward product: the sum of P_1 (dP - delta_1) over the
+// keys (P_1 sums to 1), which dlam adds back and so is as exact as fp32 sums are.
+#include "diff_attn.h"
+
+namespace tj {
+namespace {
+
+// One group of `lpr` lanes per row: 16-byte chunks of dO and the same columns of the maps' outputs. n_peaks
+// blocks share the rows, then the keys, of one (b, key head).
+template <typename T>
+__global__ __launch_bounds__(kDiffThreads) void diff_delta_kernel(DiffArgs a, int lpr) {
+  constexpr int VEC = Vec16<float>::N * (4 / (int)sizeof(T));
+  typedef T vec_t __attribute__((ext_vector_type(VEC)));
+  __shared__ float red[2][kDiffThreads / kWave];
+  const int tid = threadIdx.x, block = blockIdx.x % a.n_peaks, bh = blockIdx.x / a.n_peaks, b = bh / a.Hk, hk = bh % a.Hk;
+  const int L = diff_len(a, b);
+  const int lane = tid % lpr, per_block = kDiffThreads / lpr;
+  const bool on = lane * VEC < a.Dv;
+  float peak_o = 0.f, peak_v = 0.f;
+  for (int r = block * per_block + tid / lpr; r < a.R; r += a.n_peaks * per_block) {
+    const int i = r / a.G, head = hk * a.G + r % a.G;
+    float d0 = 0.f, d1 = 0.f, n = 0.f;
+    if (i < L && on) {
+      const vec_t x = *reinterpret_cast<const vec_t*>(reinterpret_cast<const T*>(a.dout) + a.vdo.row(b, head, i) + lane * VEC);
+      const float* mp = a.maps + ((int64_t)bh * a.R + r) * 2 * a.Dv + lane * VEC;
+#pragma unroll
+      for (int e = 0; e < VEC; e += 4) {
+        const float4_t y = *reinterpret_cast<const float4_t*>(mp + e), z = *reinterpret_cast<const float4_t*>(mp + a.Dv + e);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float g = (float)x[e + j];
+          d0 = fmaf(g, y[j], d0);
+          d1 = fmaf(g, z[j], d1);
+          n = fmaf(g, g, n);
+        }
+      }
+    }
+    for (int s = lpr / 2; s > 0; s >>= 1) {
+      d0 += __shfl_xor(d0, s);
+      d1 += __shfl_xor(d1, s);
+      n += __shfl_xor(n, s);
+    }
+    if (lane == 0) {
+      float* del = a.delta + (int64_t)bh * 2 * a.R + r;
+      del[0] = d0;
+      del[a.R] = d1;
+    }
+    if (n < 3e38f) peak_o = fmaxf(peak_o, n);  // not those that are not finite: they spoil their own row only
+  }
+  if constexpr (std::is_same<T, half_t>::value) {
+    for (int j = block * per_block + tid / lpr; j < L; j += a.n_peaks * per_block) {
+      float n = 0.f;
+      if (on) {
+        const vec_t x = *reinterpret_cast<const vec_t*>(reinterpret_cast<const T*>(a.v) + a.vv.row(b, hk, j) + lane * VEC);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) n = fmaf((float)x[e], (float)x[e], n);
+      }
+      for (int s = lpr / 2; s > 0; s >>= 1) n += __shfl_xor(n, s);
+      if (n < 3e38f) peak_v = fmaxf(peak_v, n);
+    }
+    for (int s = kWave / 2; s > 0; s >>= 1) {
+      peak_o = fmaxf(peak_o, __shfl_xor(peak_o, s));
+      peak_v = fmaxf(peak_v, __shfl_xor(peak_v, s));
+    }
+    if (tid % kWave == 0) {
+      red[0][tid / kWave] = peak_o;
+      red[1][tid / kWave] = peak_v;
+    }
+    __syncthreads();
+    if (tid < 2) {
+      float x = red[tid][0];
+      for (int w = 1; w < kDiffThreads / kWave; ++w) x = fmaxf(x, red[tid][w]);
+      a.peak[((int64_t)bh * 2 + tid) * kPeakParts + block] = sqrtf(x);
+    }
+  }
+}
+
+// 4 waves x 32 rows, keys through LDS in tiles of 32. Scores transposed as in
+// the forward kernel: a row's sums are its lane's own numbers, and dS turns into
+// the B operand of dQ^T = K^T dS^T.
+template <typename T, int HD>
+__global__ __launch_bounds__(kDiffThreads, 1) void diff_bwd_q_kernel(DiffArgs a) {
+  constexpr int DVP = 2 * HD, KS = HD / 16, VS = DVP / 16, KB = HD / 32, BN = 32;
+  using KT = LdsRows<T, HD>;
+  using VT = LdsRows<T, DVP>;
+  __shared__ __attribute__((aligned(16))) T sk[2][BN * KT::kStride];
+  __shared__ __attribute__((aligned(16))) T sv[BN * VT::kStride];
+  const int tid = threadIdx.x, w = tid / kWave, lane = tid % kWave, hl = lane / 32, ln = lane % 32;
+  const DiffTile t = diff_tile(a, blockIdx.x, a.n_mtiles);
+  const int mt = a.n_mtiles - 1 - t.tile;
+  const int L = diff_len(a, t.b);
+  const int r0 = mt * 128, rw0 = r0 + 32 * w, r = rw0 + ln;
+  const int i = r / a.G, head = t.hk * a.G + r % a.G;
+  const bool live = r < a.R && i < L;
+  const int limit = a.causal ? i : L - 1;
+  const int kv_end = r0 / a.G >= L ? 0 : (a.causal ? min(L, min(r0 + 127, a.R - 1) / a.G + 1) : L);
+  const int own_end = rw0 >= a.R || rw0 / a.G >= L ? 0 : (a.causal ? min(L, min(rw0 + 31, a.R - 1) / a.G + 1) : L);
+  const int free = a.causal ? rw0 / a.G : L - 1;
+
+  frag_t<T> qf[2][KS], of[VS];
+  {
+    const T* qp = reinterpret_cast<const T*>(a.q) + (live ? a.vq.row(t.b, 2 * head, i) : 0);
+    const T* op = reinterpret_cast<const T*>(a.dout) + (live ? a.vdo.row(t.b, head, i) : 0);
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int s = 0; s < KS; ++s) qf[c][s] = load_frag<T>(live ? qp + c * a.vq.sh : nullptr, 16 * s + 8 * hl, a.D);
+#pragma unroll
+    for (int s = 0; s < VS; ++s) of[s] = load_frag<T>(live ? op : nullptr, 16 * s + 8 * hl, a.Dv);
+  }
+  float16_t dq[2][KB];
+#pragma unroll
+  for (int c = 0; c < 2; ++c)
+#pragma unroll
+    for (int d = 0; d < KB; ++d) dq[c][d] = zero16();
+  const float lift = ds_lift<T>(a, t.bh, t.hk, lane);
+  const float c2 = a.scale * kLog2e;
+  const float lam = live ? a.lam[head * a.lam_step] : 0.f;
+  float lse[2], del[2];
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    lse[c] = live ? a.lse[((int64_t)t.bh * 2 + c) * a.R + r] : __builtin_inff();
+    del[c] = live ? a.delta[((int64_t)t.bh * 2 + c) * a.R + r] : 0.f;
+  }
+  const float d0 = -del[0] * lift, nl = -lam * lift;
+  float rest = 0.f;
+
+  const T* kp = reinterpret_cast<const T*>(a.k) + a.vk.row(t.b, 2 * t.hk, 0);
+  const T* vp = reinterpret_cast<const T*>(a.v) + a.vv.row(t.b, t.hk, 0);
+  for (int kv0 = 0; kv0 < kv_end; kv0 += BN) {
+    __syncthreads();
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+      KT::template fill<BN>(sk[c], tid, a.D, [&](int row) {
+        return kv0 + row < L ? kp + c * a.vk.sh + (kv0 + row) * a.vk.ss : nullptr;
+      });
+    VT::template fill<BN>(sv, tid, a.Dv, [&](int row) {
+      return kv0 + row < L ? vp + (kv0 + row) * a.vv.ss : nullptr;
+    });
+    __syncthreads();
+    if (kv0 >= own_end) continue;
+    float16_t p[2], dp = zero16();
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      p[c] = zero16();
+#pragma unroll
+      for (int s = 0; s < KS; ++s) p[c] = Elem<T>::mma(KT::row_frag(sk[c], ln, 16 * s + 8 * hl), qf[c][s], p[c]);
+    }
+#pragma unroll
+    for (int s = 0; s < VS; ++s) dp = Elem<T>::mma(VT::row_frag(sv, ln, 16 * s + 8 * hl), of[s], dp);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+#pragma unroll
+      for (int e = 0; e < 16; ++e) p[c][e] = fast_exp2(fmaf(p[c][e], c2, -lse[c]));
+      if (kv0 + BN - 1 > free) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (kv0 + acc_row(e, hl) > limit) p[c][e] = 0.f;
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      p[0][e] *= fmaf(dp[e], lift, d0);
+      const float u = p[1][e] * (dp[e] - del[1]);
+      rest += u;
+      p[1][e] = u * nl;
+    }
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const frag_t<T> f = acc_frag<T>(p[c], s);
+#pragma unroll
+        for (int d = 0; d < KB; ++d) dq[c][d] = Elem<T>::mma(KT::col_frag(sk[c], 16 * s, 32 * d, lane), f, dq[c][d]);
+      }
+  }
+
+  rest = pair_sum(rest);
+  if (r >= a.R) return;
+  if (hl == 0) a.gsum[(int64_t)t.bh * a.R + r] = live ? del[1] + rest : 0.f;
+  const float out = a.scale / lift;
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    T* p = reinterpret_cast<T*>(a.dq) + a.vdq.row(t.b, 2 * head + c, i);
+#pragma unroll
+    for (int d = 0; d < KB; ++d)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int col = 32 * d + 8 * e + 4 * hl;
+        float y[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = live ? dq[c][d][4 * e + j] * out : 0.f;
+        if (col < a.D) store4t<T>(p + col, y[0], y[1], y[2], y[3]);
+      }
+  }
+}
+
+// dlam: one workgroup per weight, its rows in a fixed order, in 64 bits.
+__global__ __launch_bounds__(1024) void diff_dlam_kernel(DiffArgs a) {
+  __shared__ double red[1024 / kWave];
+  const int tid = threadIdx.x, n = blockIdx.x;
+  double s = 0.;
+  for (int h = (a.lam_step ? n : 0); h < (a.lam_step ? n + 1 : a.H); ++h)
+    for (int b = 0; b < a.B; ++b) {
+      const float* p = a.gsum + ((int64_t)b * a.Hk + h / a.G) * a.R + h % a.G;
+      for (int i = tid; i < a.Sq; i += 1024) s += p[(int64_t)i * a.G];
+    }
+  for (int m = kWave / 2; m > 0; m >>= 1) s += __shfl_xor(s, m);
+  if (tid % kWave == 0) red[tid / kWave] = s;
+  __syncthreads();
+  if (tid == 0) {
+    for (int w = 1; w < 1024 / kWave; ++w) s += red[w];
+    a.dlam[n] = (float)-s;
+  }
+}
+
+template <typename T>
+int launch_delta(const DiffArgs& a, hipStream_t stream) {
+  const int chunks = (a.Dv * (int)sizeof(T) + 15) / 16;
+  int lpr = 1;
+  while (lpr < chunks) lpr *= 2;
+  hipLaunchKernelGGL((diff_delta_kernel<T>), dim3(uint32_t((int64_t)a.n_peaks * a.B * a.Hk)), dim3(kDiffThreads), 0, stream, a, lpr);
+  return tjh::launch_status();
+}
+
+}  // namespace
+
+int diff_delta(const DiffArgs& a, int dtype, hipStream_t stream) {
+  if (dtype == TJ_F32) return launch_delta<float>(a, stream);
+  return dtype == TJ_F16 ? launch_delta<half_t>(a, stream) : launch_delta<bf16_t>(a, stream);
+}
+
+int diff_bwd_q(const DiffArgs& args, int dtype, hipStream_t stream) {
+  const int rc = diff_dispatch(args, dtype, [&](auto t, auto hd) {
+    DiffArgs a = args;
+    a.n_mtiles = (a.R + 127) / 128;
+    hipLaunchKernelGGL((diff_bwd_q_kernel<decltype(t), decltype(hd)::value>),
+                       dim3(uint32_t((int64_t)a.B * a.Hk * a.n_mtiles)), dim3(kDiffThreads), 0, stream, a);
+    return tjh::launch_status();
+  });
+  if (rc != TJ_OK) return rc;
+  hipLaunchKernelGGL(diff_dlam_kernel, dim3(args.n_lam), dim3(1024), 0, stream, args);
+  return tjh::launch_status();
+}
+
+}  // namespace tj

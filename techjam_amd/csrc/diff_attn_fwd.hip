@@ -1,0 +1,368 @@
+// Differential attention, forward (the mathematics and the row numbering are
+// in diff_attn.h): whole sequences, and few new tokens against a cache.
+//
+// Scores are formed transposed, S^T = K Q^T, so that a lane holds scores of ONE
+// row: maximum and sum are per lane (the other half of the wave holds the
+// other keys), and the probabilities turn into the B operand of O^T = V^T P^T
+// where they stand. The two maps have their own running maximum, sum and
+// accumulator and share every V fragment.
+//
+// diff_fwd_kernel: a workgroup = 4 waves = 128 rows of one (b, key head), 32
+// rows a wave; keys stream through LDS in tiles. diff_few_kernel: a workgroup =
+// one wave = 32 rows and one part of the keys, with its own LDS tile. Sweeps
+// cut into parts are joined by diff_join_kernel.
+#include "diff_attn.h"
+
+namespace tj {
+namespace {
+
+constexpr float kLazy = 8.f;  // the running maximum moves when a row's maximum grows by more than 2^8
+
+template <typename T, int HD, int BNT>
+struct FwdShape {
+  static constexpr int DVP = 2 * HD;
+  static constexpr int BN = BNT;
+  using KT = LdsRows<T, HD>;
+  using VT = LdsRows<T, DVP>;
+  static constexpr int KS = HD / 16;   // k-steps over the head dim
+  static constexpr int NKB = BN / 32;  // score blocks per tile
+  static constexpr int NS = BN / 16;   // k-steps over the tile's keys
+  static constexpr int DB = DVP / 32;  // output blocks
+  static constexpr int kElems = BN * (2 * KT::kStride + VT::kStride);
+};
+
+// A lane's row: r of the (b, key head), its token, head and position, and the last key it sees.
+struct DiffRow {
+  int r, i, g, limit;
+  bool live;
+  __device__ __forceinline__ DiffRow(const DiffArgs& a, int row, int L) : r(row), i(row / a.G), g(row % a.G) {
+    const int pos = (a.cached ? L - a.Sq : 0) + i;
+    live = r < a.R && pos >= 0 && pos < L;
+    limit = a.causal ? pos : L - 1;
+  }
+};
+
+// Rows row0 .. row1 (clipped to R) of a wave or workgroup: keys needed, and the
+// last key that every one of them sees.
+struct DiffSpan {
+  int end, free;
+  __device__ __forceinline__ DiffSpan(const DiffArgs& a, int row0, int row1, int L) {
+    const int first = a.cached ? L - a.Sq : 0;
+    const int p0 = first + row0 / a.G, p1 = first + min(row1, a.R - 1) / a.G;
+    end = row0 >= a.R || p0 >= L || p1 < 0 ? 0 : (a.causal ? min(L, p1 + 1) : L);
+    free = a.causal ? p0 : L - 1;
+  }
+};
+
+// The running state of a wave's 32 rows.
+template <typename T, typename SH>
+struct FwdState {
+  frag_t<T> q[2][SH::KS];
+  float16_t o[2][SH::DB];
+  float m[2], l[2];  // maximum in log2 units, the lane's part of the sum
+  float c2;          // |scale| log2 e
+
+  __device__ __forceinline__ void init(const DiffArgs& a, int b, int hk, const DiffRow& row, int lane) {
+    const int hl = lane / 32;
+    const T* qp = reinterpret_cast<const T*>(a.q) + (row.live ? a.vq.row(b, 2 * (hk * a.G + row.g), row.i) : 0);
+    // A negative scale turns q's sign, so that the largest score is the largest
+    // product; a zero one becomes too small to matter, so that masked stays -inf.
+    c2 = fmaxf(fabsf(a.scale) * kLog2e, 1e-37f);
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+#pragma unroll
+      for (int ks = 0; ks < SH::KS; ++ks) {
+        q[c][ks] = load_frag<T>(row.live ? qp + c * a.vq.sh : nullptr, 16 * ks + 8 * hl, a.D);
+        if (a.scale < 0.f)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) q[c][ks][j] = -q[c][ks][j];
+      }
+      m[c] = -__builtin_inff();
+      l[c] = 0.f;
+#pragma unroll
+      for (int d = 0; d < SH::DB; ++d) o[c][d] = zero16();
+    }
+  }
+
+  // One key tile: keys kv0 + (0 .. BN-1), of which the row sees those <= limit.
+  __device__ __forceinline__ void tile(const T* kt, const T* vt, int kv0, int limit, bool masked, int lane) {
+    const int hl = lane / 32, ln = lane % 32;
+    frag_t<T> p[2][SH::NS];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const T* kc = kt + c * SH::BN * SH::KT::kStride;
+      float16_t s[SH::NKB];
+#pragma unroll
+      for (int kb = 0; kb < SH::NKB; ++kb) {
+        s[kb] = zero16();
+#pragma unroll
+        for (int ks = 0; ks < SH::KS; ++ks)
+          s[kb] = Elem<T>::mma(SH::KT::row_frag(kc, kb * 32 + ln, 16 * ks + 8 * hl), q[c][ks], s[kb]);
+      }
+      if (masked) {
+#pragma unroll
+        for (int kb = 0; kb < SH::NKB; ++kb)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (kv0 + kb * 32 + acc_row(r, hl) > limit) s[kb][r] = -__builtin_inff();
+      }
+      float top = s[0][0];
+#pragma unroll
+      for (int kb = 0; kb < SH::NKB; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[kb][r]);
+      top = pair_max(top) * c2;
+      // The maximum moves by the row's need; one decision for the wave.
+      const bool move = top > m[c] + kLazy;  // also from -inf
+      if (__any(move)) {
+        const float to = move ? top : m[c];
+        const float alpha = m[c] == -__builtin_inff() ? 0.f : fast_exp2(m[c] - to);
+        m[c] = to;
+        l[c] *= alpha;
+#pragma unroll
+        for (int d = 0; d < SH::DB; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[c][d][r] *= alpha;
+      }
+      // A row that has seen no key keeps its unset maximum out of the exponent.
+      const float off = m[c] == -__builtin_inff() ? 0.f : Elem<T>::kLift - m[c];
+      float sum = 0.f;
+#pragma unroll
+      for (int kb = 0; kb < SH::NKB; ++kb) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          s[kb][r] = fast_exp2(fmaf(s[kb][r], c2, off));
+          sum += s[kb][r];
+        }
+        p[c][2 * kb] = acc_frag<T>(s[kb], 0);
+        p[c][2 * kb + 1] = acc_frag<T>(s[kb], 1);
+      }
+      l[c] += sum;
+    }
+#pragma unroll
+    for (int st = 0; st < SH::NS; ++st)
+#pragma unroll
+      for (int d = 0; d < SH::DB; ++d) {
+        const frag_t<T> vf = SH::VT::col_frag(vt, 16 * st, 32 * d, lane);
+#pragma unroll
+        for (int c = 0; c < 2; ++c) o[c][d] = Elem<T>::mma(vf, p[c][st], o[c][d]);
+      }
+  }
+
+  // The rows' results, whole (part < 0) or those of a part of the keys.
+  __device__ __forceinline__ void finish(const DiffArgs& a, int b, int hk, const DiffRow& row, int part, int lane) {
+    const int hl = lane / 32;
+    const int bh = b * a.Hk + hk, head = hk * a.G + row.g;
+    if (part >= 0) {
+      const int64_t slot = ((int64_t)part * a.B * a.Hk + bh) * a.R + row.r;
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const float sum = pair_sum(l[c]);
+        if (!row.live) continue;
+        float* po = a.part_o + (slot * 2 + c) * a.Dv;
+#pragma unroll
+        for (int d = 0; d < SH::DB; ++d)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int col = 32 * d + 8 * e + 4 * hl;
+            if (col < a.Dv) store4t<float>(po + col, o[c][d][4 * e], o[c][d][4 * e + 1], o[c][d][4 * e + 2], o[c][d][4 * e + 3]);
+          }
+        if (hl == 0) {
+          a.part_ml[(slot * 2 + c) * 2] = m[c];
+          a.part_ml[(slot * 2 + c) * 2 + 1] = sum;
+        }
+      }
+      return;
+    }
+    float inv[2];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const float sum = pair_sum(l[c]);
+      inv[c] = 1.f / sum;
+      if (a.lse != nullptr && row.r < a.R && hl == 0)
+        a.lse[((int64_t)bh * 2 + c) * a.R + row.r] =
+            row.live ? m[c] - Elem<T>::kLift + log2f(sum) : __builtin_inff();
+    }
+    if (row.r >= a.R) return;
+    const float lam = a.lam[head * a.lam_step];
+    const int64_t at = a.vo.row(b, head, row.i);
+    T* op = reinterpret_cast<T*>(a.o) + at;
+    float* mp = a.maps + ((int64_t)bh * a.R + row.r) * 2 * a.Dv;
+#pragma unroll
+    for (int d = 0; d < SH::DB; ++d)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int col = 32 * d + 8 * e + 4 * hl;
+        if (col >= a.Dv) continue;
+        float4_t y = {0.f, 0.f, 0.f, 0.f}, z = y;
+        if (row.live)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            y[j] = o[0][d][4 * e + j] * inv[0];
+            z[j] = o[1][d][4 * e + j] * inv[1];
+          }
+        store4t<T>(op + col, fmaf(-lam, z[0], y[0]), fmaf(-lam, z[1], y[1]), fmaf(-lam, z[2], y[2]), fmaf(-lam, z[3], y[3]));
+        if (a.maps != nullptr) {
+          *reinterpret_cast<float4_t*>(mp + col) = y;
+          *reinterpret_cast<float4_t*>(mp + a.Dv + col) = z;
+        }
+      }
+  }
+};
+
+// Keys kv0 .. kv0 + BN - 1 of K's two heads and of V into LDS; keys at or past L read as zeros, whatever is there.
+template <typename T, typename SH, int THREADS>
+__device__ __forceinline__ void fill_keys(const DiffArgs& a, T* kt, T* vt, const T* kp, const T* vp, int kv0, int L,
+                                          int tid) {
+#pragma unroll
+  for (int c = 0; c < 2; ++c)
+    SH::KT::template fill<SH::BN, THREADS>(kt + c * SH::BN * SH::KT::kStride, tid, a.D, [&](int row) {
+      return kv0 + row < L ? kp + c * a.vk.sh + (kv0 + row) * a.vk.ss : nullptr;
+    });
+  SH::VT::template fill<SH::BN, THREADS>(vt, tid, a.Dv, [&](int row) {
+    return kv0 + row < L ? vp + (kv0 + row) * a.vv.ss : nullptr;
+  });
+}
+
+template <typename T, int HD, bool PART>
+__global__ __launch_bounds__(kDiffThreads, (sizeof(T) == 2 && HD <= 64 ? 2 : 1)) void diff_fwd_kernel(DiffArgs a) {
+  using SH = FwdShape<T, HD, (sizeof(T) == 4 ? 32 : 64)>;
+  __shared__ __attribute__((aligned(16))) T smem[SH::kElems];
+  T* kt = smem;
+  T* vt = kt + 2 * SH::BN * SH::KT::kStride;
+  const int tid = threadIdx.x, w = tid / kWave, lane = tid % kWave;
+  const DiffTile t = diff_tile(a, blockIdx.x, a.n_mtiles);
+  const int part = PART ? t.tile / a.n_mtiles : -1;
+  const int mt = a.n_mtiles - 1 - (PART ? t.tile % a.n_mtiles : t.tile);
+  const int L = diff_len(a, t.b);
+  const DiffSpan all(a, mt * 128, mt * 128 + 127, L), own(a, mt * 128 + 32 * w, mt * 128 + 32 * w + 31, L);
+  const DiffRow row(a, mt * 128 + 32 * w + lane % 32, L);
+  const int kv_begin = PART ? part * a.part_keys : 0;
+  const int kv_end = PART ? min(all.end, kv_begin + a.part_keys) : all.end;
+  if (PART && kv_begin >= kv_end) return;  // not read either (live parts are counted from the rows' last key)
+  FwdState<T, SH> st;
+  st.init(a, t.b, t.hk, row, lane);
+  const T* kp = reinterpret_cast<const T*>(a.k) + a.vk.row(t.b, 2 * t.hk, 0);
+  const T* vp = reinterpret_cast<const T*>(a.v) + a.vv.row(t.b, t.hk, 0);
+  for (int kv0 = kv_begin; kv0 < kv_end; kv0 += SH::BN) {
+    __syncthreads();
+    fill_keys<T, SH, kDiffThreads>(a, kt, vt, kp, vp, kv0, L, tid);
+    __syncthreads();
+    if (kv0 < own.end) st.tile(kt, vt, kv0, row.limit, kv0 + SH::BN - 1 > own.free, lane);
+  }
+  st.finish(a, t.b, t.hk, row, part, lane);
+}
+
+template <typename T, int HD>
+__global__ __launch_bounds__(kWave) void diff_few_kernel(DiffArgs a) {
+  using SH = FwdShape<T, HD, 32>;
+  __shared__ __attribute__((aligned(16))) T smem[SH::kElems];
+  T* kt = smem;
+  T* vt = kt + 2 * SH::BN * SH::KT::kStride;
+  const int lane = threadIdx.x;
+  const DiffTile t = diff_tile(a, blockIdx.x, a.n_mtiles * a.n_parts);
+  const int mt = t.tile % a.n_mtiles, part = t.tile / a.n_mtiles;
+  const int L = diff_len(a, t.b);
+  const DiffSpan own(a, mt * 32, mt * 32 + 31, L);
+  const DiffRow row(a, mt * 32 + lane % 32, L);
+  const int kv_begin = part * a.part_keys, kv_end = min(own.end, kv_begin + a.part_keys);
+  if (kv_begin >= kv_end) return;
+  FwdState<T, SH> st;
+  st.init(a, t.b, t.hk, row, lane);
+  const T* kp = reinterpret_cast<const T*>(a.k) + a.vk.row(t.b, 2 * t.hk, 0);
+  const T* vp = reinterpret_cast<const T*>(a.v) + a.vv.row(t.b, t.hk, 0);
+  for (int kv0 = kv_begin; kv0 < kv_end; kv0 += SH::BN) {
+    __syncthreads();
+    fill_keys<T, SH, kWave>(a, kt, vt, kp, vp, kv0, L, lane);
+    __syncthreads();
+    st.tile(kt, vt, kv0, row.limit, kv0 + SH::BN - 1 > own.free, lane);
+  }
+  st.finish(a, t.b, t.hk, row, part, lane);
+}
+
+// Joins the parts: O_m = sum_p 2^(max_p - M) o_p / sum_p 2^(max_p - M) sum_p,
+// then the difference. One row per workgroup quarter: a wave per row, lanes over
+// columns. A row's parts are those up to its last key.
+template <typename T>
+__global__ __launch_bounds__(kDiffThreads) void diff_join_kernel(DiffArgs a) {
+  const int lane = threadIdx.x % kWave;
+  const int64_t n_rows = (int64_t)a.B * a.Hk * a.R;
+  const int64_t id = (int64_t)blockIdx.x * (kDiffThreads / kWave) + threadIdx.x / kWave;
+  if (id >= n_rows) return;
+  const int bh = (int)(id / a.R), b = bh / a.Hk, hk = bh % a.Hk;
+  const int L = diff_len(a, b);
+  const DiffRow row(a, (int)(id % a.R), L);
+  const int np = row.live ? row.limit / a.part_keys + 1 : 0;
+  float m[2] = {-__builtin_inff(), -__builtin_inff()}, l[2] = {0.f, 0.f};
+  for (int c = 0; c < 2; ++c) {
+    for (int p = lane; p < np; p += kWave) {
+      const float* ml = a.part_ml + ((p * n_rows + id) * 2 + c) * 2;
+      m[c] = fmaxf(m[c], ml[0]);
+    }
+    for (int s = 32; s > 0; s >>= 1) m[c] = fmaxf(m[c], __shfl_xor(m[c], s));
+    for (int p = lane; p < np; p += kWave) {
+      const float* ml = a.part_ml + ((p * n_rows + id) * 2 + c) * 2;
+      l[c] += ml[0] == -__builtin_inff() ? ml[1] : fast_exp2(ml[0] - m[c]) * ml[1];
+    }
+    for (int s = 32; s > 0; s >>= 1) l[c] += __shfl_xor(l[c], s);
+    if (a.lse != nullptr && lane == 0)
+      a.lse[((int64_t)bh * 2 + c) * a.R + row.r] = row.live ? m[c] - Elem<T>::kLift + log2f(l[c]) : __builtin_inff();
+  }
+  const int head = hk * a.G + row.g;
+  const float lam = a.lam[head * a.lam_step];
+  const int64_t at = a.vo.row(b, head, row.i);
+  for (int col = lane; col < a.Dv; col += kWave) {
+    float y[2] = {0.f, 0.f};
+    for (int c = 0; c < 2; ++c) {
+      for (int p = 0; p < np; ++p) {
+        const int64_t slot = (p * n_rows + id) * 2 + c;
+        const float mp = a.part_ml[slot * 2];
+        const float o = a.part_o[slot * a.Dv + col];
+        y[c] += mp == -__builtin_inff() ? o : fast_exp2(mp - m[c]) * o;
+      }
+      y[c] = row.live ? y[c] / l[c] : 0.f;
+      if (a.maps != nullptr) a.maps[(id * 2 + c) * a.Dv + col] = y[c];
+    }
+    reinterpret_cast<T*>(a.o)[at + col] = (T)fmaf(-lam, y[1], y[0]);
+  }
+}
+
+template <typename T>
+int launch_join(const DiffArgs& a, hipStream_t stream) {
+  const int64_t n = ((int64_t)a.B * a.Hk * a.R + 3) / 4;
+  hipLaunchKernelGGL((diff_join_kernel<T>), dim3(uint32_t(n)), dim3(kDiffThreads), 0, stream, a);
+  return tjh::launch_status();
+}
+
+}  // namespace
+
+int diff_fwd(const DiffArgs& args, int dtype, hipStream_t stream) {
+  return diff_dispatch(args, dtype, [&](auto t, auto hd) {
+    using T = decltype(t);
+    constexpr int HD = decltype(hd)::value;
+    DiffArgs a = args;
+    a.n_mtiles = (a.R + 127) / 128;
+    const int64_t n = (int64_t)a.B * a.Hk * a.n_mtiles;
+    if (a.n_parts > 1) {
+      hipLaunchKernelGGL((diff_fwd_kernel<T, HD, true>), dim3(uint32_t(n * a.n_parts)), dim3(kDiffThreads), 0, stream, a);
+      const int rc = tjh::launch_status();
+      return rc != TJ_OK ? rc : launch_join<T>(a, stream);
+    }
+    hipLaunchKernelGGL((diff_fwd_kernel<T, HD, false>), dim3(uint32_t(n)), dim3(kDiffThreads), 0, stream, a);
+    return tjh::launch_status();
+  });
+}
+
+int diff_few_rows(const DiffArgs& args, int dtype, hipStream_t stream) {
+  return diff_dispatch(args, dtype, [&](auto t, auto hd) {
+    using T = decltype(t);
+    DiffArgs a = args;
+    a.n_mtiles = (a.R + 31) / 32;
+    hipLaunchKernelGGL((diff_few_kernel<T, decltype(hd)::value>),
+                       dim3(uint32_t((int64_t)a.B * a.Hk * a.n_mtiles * a.n_parts)), dim3(kWave), 0, stream, a);
+    const int rc = tjh::launch_status();
+    return rc != TJ_OK ? rc : launch_join<T>(a, stream);
+  });
+}
+
+}  // namespace tj

@@ -27,6 +27,7 @@ TJ_ERR_SCRATCH = 7
 
 TJ_F32 = 0
 TJ_F16 = 1
+TJ_BF16 = 2
 
 #: The C ABI these bindings describe (tj_abi_version); a library built from
 #: other sources is refused at load time.
@@ -101,6 +102,23 @@ SIGNATURES = {
         _int,
         [_vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i64p, _i64p, _i64p, _i64p, _i64, _vp],
     ),
+    "tj_diff_attn_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _i64, _i64, _i64, _i64, _int]),
+    "tj_diff_attn_fwd": (
+        _int,
+        [_vp, _vp, _vp, _vp, _int, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64p, _i64p, _i64p, _i64p,
+         _f32, _int, _int, _vp, _i64, _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp],
+    ),
+    "tj_diff_attn_bwd_workspace_bytes": (ctypes.c_size_t, [_i64, _i64, _i64, _i64]),
+    "tj_diff_attn_bwd": (
+        _int,
+        [_vp] * 10 + [_int] + [_i64] * 6 + [_i64p] * 7
+        + [_f32, _int, _vp, _i64, _vp, _vp, ctypes.c_size_t, _vp],
+    ),
+    "tj_layer_norm_fwd": (
+        _int, [_vp, _vp, _vp, _vp, _int, _int, _i64, _i64, _i64, _i64, _f32, _vp, _vp, _vp]),
+    "tj_layer_norm_bwd_workspace_bytes": (ctypes.c_size_t, [_i64, _i64]),
+    "tj_layer_norm_bwd": (
+        _int, [_vp] * 8 + [_int, _int, _i64, _i64, _i64, _i64, _i64, _vp, ctypes.c_size_t, _vp]),
 }
 
 _lock = threading.Lock()

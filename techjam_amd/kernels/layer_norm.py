@@ -1,0 +1,140 @@
+"""Layer norm on the HIP kernels, forward and backward.
+
+The reference's norms are ``torch.nn.LayerNorm``
+(``torch_transformer_benchmark.py:125-172``). ``elementwise.py`` has the norm
+that closes a residual pass in inference; ``layer_norm`` is the norm by itself,
+for every width up to ``MAX_WIDTH``, with gradients.
+"""
+
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from ..errors import UnsupportedCaseError
+from . import _lib
+from .attention import _ptr, _require_device, _stream_ptr
+from .differential import DTYPES, on_device
+
+#: Widest row the kernels take.
+MAX_WIDTH = 16384
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """``t`` as ``[rows, width]`` with unit column stride: a view where its
+    leading dimensions have one stride in common, else a copy."""
+    width = t.shape[-1]
+    if t.stride(-1) != 1 and width > 1:
+        return t.reshape(-1, width).contiguous()
+    return t.reshape(-1, width)
+
+
+def _forward(x, weight, bias, eps, stats):
+    rows2d = _rows(x)
+    rows, width = rows2d.shape
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    mean = rstd = None
+    if stats:
+        mean, rstd = torch.empty(2, rows, dtype=torch.float32, device=x.device)
+    w_dtype = next((DTYPES[p.dtype] for p in (weight, bias) if p is not None), _lib.TJ_F32)
+    with on_device(x.device):
+        code = _lib.lib().tj_layer_norm_fwd(
+            rows2d.data_ptr(), _ptr(weight), _ptr(bias), y.data_ptr(), DTYPES[x.dtype], w_dtype, rows, width,
+            rows2d.stride(0), width, eps, _ptr(mean), _ptr(rstd), _stream_ptr(x.device))
+    _lib.check(code, "tj_layer_norm_fwd")
+    return y, mean, rstd
+
+
+def _backward(ctx, dy):
+    x, weight, mean, rstd = ctx.saved_tensors
+    need_x, need_w, need_b, _ = ctx.needs_input_grad
+    dy2d, x2d = _rows(dy), _rows(x)
+    rows, width = x2d.shape
+    dev = x.device
+    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
+    w_torch = ctx.bias_dtype if weight is None else weight.dtype
+    make = torch.zeros if rows == 0 else torch.empty
+    dw = make(width, dtype=w_torch, device=dev) if need_w else None
+    db = make(width, dtype=w_torch, device=dev) if need_b else None
+    lib = _lib.lib()
+    with on_device(dev):
+        ws_bytes = lib.tj_layer_norm_bwd_workspace_bytes(rows, width) if need_w or need_b else 0
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
+        code = lib.tj_layer_norm_bwd(
+            dy2d.data_ptr(), x2d.data_ptr(), _ptr(weight), mean.data_ptr(), rstd.data_ptr(), _ptr(dx), _ptr(dw),
+            _ptr(db), DTYPES[x.dtype], _lib.TJ_F32 if w_torch is None else DTYPES[w_torch], rows, width,
+            dy2d.stride(0), x2d.stride(0), width, _ptr(ws), ws_bytes, _stream_ptr(dev))
+    _lib.check(code, "tj_layer_norm_bwd")
+    return dx, dw, db, None
+
+
+#: Under create_graph: the gradients, with an error for whoever differentiates
+#: them. Without it the plain function, whose call is leaner: 110 -> 66 us for
+#: the forward and backward pass of 256 rows of 256.
+_backward_once = once_differentiable(_backward)
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y, mean, rstd = _forward(x, weight, bias, eps, True)
+        ctx.save_for_backward(x, weight, mean, rstd)
+        ctx.bias_dtype = None if bias is None else bias.dtype
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        return _backward_once(ctx, dy) if torch.is_grad_enabled() else _backward(ctx, dy)
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+               eps: float = 1e-5) -> torch.Tensor:
+    """Layer norm over the last dimension of ``x``; differentiable in all three tensors.
+
+    ``x`` is float32, float16 or bfloat16 with a last dimension of at most
+    ``MAX_WIDTH``, of any shape and strides (read in place where the rows have
+    one common stride). ``weight`` and ``bias`` are contiguous ``[width]``, both
+    float32 or both of ``x``'s type, each optional; their gradients come in their
+    type. Statistics and sums are float32, the output is ``x``'s type and
+    contiguous. The gradients' sums over the rows have a fixed order, so equal
+    calls give equal bits. Second derivatives are not implemented.
+    """
+    if x.ndim == 0 or x.shape[-1] == 0:
+        raise ValueError("x must have a last dimension to normalise over")
+    if x.dtype not in DTYPES:
+        raise UnsupportedCaseError(f"dtype {x.dtype} is not supported (float32, float16 or bfloat16)")
+    width = x.shape[-1]
+    if width > MAX_WIDTH:
+        raise UnsupportedCaseError(f"width {width} is not supported (at most {MAX_WIDTH})")
+    _require_device(x)
+    for name, p in (("weight", weight), ("bias", bias)):
+        if p is None:
+            continue
+        if p.shape != (width,) or p.device != x.device or not p.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous tensor of {width} elements on {x.device}")
+        if p.dtype not in (torch.float32, x.dtype):
+            raise ValueError(f"{name} must be float32 or {x.dtype}, not {p.dtype}")
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise ValueError("weight and bias must share a dtype")
+    eps = float(eps)
+    if torch.is_grad_enabled() and (x.requires_grad or any(p is not None and p.requires_grad for p in (weight, bias))):
+        return _LayerNorm.apply(x, weight, bias, eps)
+    return _forward(x, weight, bias, eps, False)[0]
+
+
+class LayerNorm(torch.nn.LayerNorm):
+    """``torch.nn.LayerNorm`` over one dimension, same parameters and state-dict
+    names, whose forward is :func:`layer_norm`."""
+
+    def __init__(self, width: int, eps: float = 1e-5, elementwise_affine: bool = True, bias: bool = True,
+                 device=None, dtype=None) -> None:
+        super().__init__(width, eps, elementwise_affine, bias, device=device, dtype=dtype)
+        if len(self.normalized_shape) != 1:
+            raise ValueError("LayerNorm normalises over the last dimension alone")
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if x.ndim == 0 or x.shape[-1] != self.normalized_shape[0]:
+            raise ValueError(f"x must have a last dimension of {self.normalized_shape[0]}, not {tuple(x.shape)}")
+        return layer_norm(x, self.weight, self.bias, self.eps)

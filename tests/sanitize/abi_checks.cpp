@@ -156,6 +156,93 @@ int main() {
   expect("narrow ffn act", tj_narrow_ffn_norm(x, w, y, 0, w, y, out, out, 4, 4, nullptr, 0, y, y, ln, 1e-5f, 0, nullptr), TJ_ERR_SHAPE);
   expect("narrow ffn misaligned", tj_narrow_ffn_norm(x, w, (float*)at(16388), 1, w, y, out, out, 4, 4, nullptr, 0, y, y, ln, 1e-5f, 0, nullptr), TJ_ERR_ALIGN);
 
+  // tj_diff_attn_fwd(q, k, v, o, dtype, B, H, Hk, Sq, Sk, D, Dv, strides x4, scale, causal, cached, lam, lam_step,
+  // lengths, lse, maps, workspace, bytes, stream)
+  {
+    const float* lam = static_cast<const float*>(at(1024));
+    float* stats = static_cast<float*>(at(2048));
+    const int32_t* len = static_cast<const int32_t*>(at(4096));
+    auto fwd = [&](const void* fq, int dtype, int64_t B, int64_t H, int64_t Hk, int64_t Sq, int64_t Sk, int64_t D,
+                   int64_t Dv, const int64_t* fst, int cached, int64_t lam_step, const int32_t* lengths, float* lse,
+                   float* maps, void* ws, size_t bytes) {
+      return tj_diff_attn_fwd(fq, k, v, o, dtype, B, H, Hk, Sq, Sk, D, Dv, fst, st, st, st, 0.125f, 1, cached, lam,
+                              lam_step, lengths, lse, maps, ws, bytes, nullptr);
+    };
+    expect("diff dtype", fwd(q, 7, 1, 2, 2, 16, 16, 64, 128, st, 0, 1, nullptr, nullptr, nullptr, nullptr, 0), TJ_ERR_DTYPE);
+    expect("diff shared heads", fwd(q, TJ_F16, 1, 3, 2, 16, 16, 64, 128, st, 0, 1, nullptr, nullptr, nullptr, nullptr, 0), TJ_ERR_SHAPE);
+    expect("diff no heads", fwd(q, TJ_F16, 1, 0, 0, 16, 16, 64, 128, st, 0, 1, nullptr, nullptr, nullptr, nullptr, 0), TJ_ERR_SHAPE);
+    expect("diff negative S", fwd(q, TJ_F16, 1, 2, 2, -1, -1, 64, 128, st, 0, 1, nullptr, nullptr, nullptr, nullptr, 0), TJ_ERR_SHAPE);
+    expect("diff huge S", fwd(q, TJ_F16, 1, 2, 2, kBig, kBig, 64, 128, st, 0, 1, nullptr, nullptr, nullptr, nullptr, 0), TJ_ERR_SHAPE);
+    expect("diff huge B", fwd(q, TJ_F16, kBig, 2, 2, 16, 16, 64, 128, st, 0, 1, nullptr, nullptr, nullptr, nullptr, 0), TJ_ERR_SHAPE);
+    expect("diff Sq != Sk", fwd(q, TJ_F16, 1, 2, 2, 8, 16, 64, 128, st, 0, 1, nullptr, nullptr, nullptr, nullptr, 0), TJ_ERR_SHAPE);
+    expect("diff head dim", fwd(q, TJ_F16, 1, 2, 2, 16, 16, 136, 128, st, 0, 1, nullptr, nullptr, nullptr, nullptr, 0), TJ_ERR_UNSUPPORTED);
+    expect("diff value dim", fwd(q, TJ_F16, 1, 2, 2, 16, 16, 64, 264, st, 0, 1, nullptr, nullptr, nullptr, nullptr, 0), TJ_ERR_UNSUPPORTED);
+    expect("diff odd head dim", fwd(q, TJ_F16, 1, 2, 2, 16, 16, 20, 64, st, 0, 1, nullptr, nullptr, nullptr, nullptr, 0), TJ_ERR_ALIGN);
+    expect("diff lam step", fwd(q, TJ_F16, 1, 2, 2, 16, 16, 64, 128, st, 0, 2, nullptr, nullptr, nullptr, nullptr, 0), TJ_ERR_SHAPE);
+    expect("diff half the stats", fwd(q, TJ_F16, 1, 2, 2, 16, 16, 64, 128, st, 0, 1, nullptr, stats, nullptr, nullptr, 0), TJ_ERR_SHAPE);
+    expect("diff missing q", fwd(nullptr, TJ_F16, 1, 2, 2, 16, 16, 64, 128, st, 0, 1, nullptr, nullptr, nullptr, nullptr, 0), TJ_ERR_SHAPE);
+    expect("diff inner stride", fwd(q, TJ_F16, 1, 2, 2, 16, 16, 64, 128, st_bad_inner, 0, 1, nullptr, nullptr, nullptr, nullptr, 0), TJ_ERR_ALIGN);
+    expect("diff q alignment", fwd(at(4), TJ_F16, 1, 2, 2, 16, 16, 64, 128, st, 0, 1, nullptr, nullptr, nullptr, nullptr, 0), TJ_ERR_ALIGN);
+    expect("diff maps alignment", fwd(q, TJ_F16, 1, 2, 2, 16, 16, 64, 128, st, 0, 1, nullptr, stats, stats + 1, nullptr, 0), TJ_ERR_ALIGN);
+    expect("diff empty batch", fwd(nullptr, TJ_F16, 0, 2, 2, 16, 16, 64, 128, st, 0, 1, nullptr, nullptr, nullptr, nullptr, 0), TJ_OK);
+    expect("cached lengths", fwd(q, TJ_F16, 1, 2, 2, 1, 4096, 64, 128, st, 1, 1, nullptr, nullptr, nullptr, at(8192), 1 << 16), TJ_ERR_SHAPE);
+    expect("cached workspace", fwd(q, TJ_F16, 1, 2, 2, 1, 4096, 64, 128, st, 1, 1, len, nullptr, nullptr, nullptr, 0), TJ_ERR_WORKSPACE);
+    expect("cached small workspace", fwd(q, TJ_F16, 1, 2, 2, 1, 4096, 64, 128, st, 1, 1, len, nullptr, nullptr, at(8192), 64), TJ_ERR_WORKSPACE);
+    expect("cached workspace alignment", fwd(q, TJ_F16, 1, 2, 2, 1, 64, 64, 128, st, 1, 1, len, nullptr, nullptr, at(8196), 1 << 15), TJ_ERR_ALIGN);
+    expect_size("diff workspace of huge sizes", tj_diff_attn_workspace_bytes(kBig, 2, 2, 16, 16, 128, 0), 0);
+    expect_size("diff workspace of many heads", tj_diff_attn_workspace_bytes(1, kBig, 1, 16, 16, 128, 1), 0);
+    expect_size("diff workspace of no values", tj_diff_attn_workspace_bytes(1, 2, 2, 1, 4096, 0, 1), 0);
+    expect_size("diff bwd workspace of huge sizes", tj_diff_attn_bwd_workspace_bytes(1, 2, 2, kBig), 0);
+
+    auto bwd = [&](int dtype, int64_t H, int64_t Hk, int64_t S, int64_t D, int64_t Dv, const float* maps, float* dlam,
+                   const int64_t* dst, int64_t lam_step, void* ws, size_t bytes) {
+      return tj_diff_attn_bwd(q, k, v, maps, stats, o, at(5120), at(5376), at(5632), dlam, dtype, 1, H, Hk, S, D, Dv, st,
+                              st, st, dst, st, st, st, 0.125f, 1, lam, lam_step, nullptr, ws, bytes, nullptr);
+    };
+    float* dlam = static_cast<float*>(at(6144));
+    expect("diff bwd dtype", bwd(3, 2, 2, 16, 64, 128, stats, dlam, st, 1, at(8192), 1 << 15), TJ_ERR_DTYPE);
+    expect("diff bwd shared heads", bwd(TJ_F16, 3, 2, 16, 64, 128, stats, dlam, st, 1, at(8192), 1 << 15), TJ_ERR_SHAPE);
+    expect("diff bwd huge S", bwd(TJ_F16, 2, 2, kBig, 64, 128, stats, dlam, st, 1, at(8192), 1 << 15), TJ_ERR_SHAPE);
+    expect("diff bwd head dim", bwd(TJ_F16, 2, 2, 16, 256, 128, stats, dlam, st, 1, at(8192), 1 << 15), TJ_ERR_UNSUPPORTED);
+    expect("diff bwd no maps", bwd(TJ_F16, 2, 2, 16, 64, 128, nullptr, dlam, st, 1, at(8192), 1 << 15), TJ_ERR_SHAPE);
+    expect("diff bwd no dlam", bwd(TJ_F16, 2, 2, 16, 64, 128, stats, nullptr, st, 1, at(8192), 1 << 15), TJ_ERR_SHAPE);
+    expect("diff bwd lam step", bwd(TJ_F16, 2, 2, 16, 64, 128, stats, dlam, st, -1, at(8192), 1 << 15), TJ_ERR_SHAPE);
+    expect("diff bwd inner stride", bwd(TJ_F16, 2, 2, 16, 64, 128, stats, dlam, st_bad_inner, 1, at(8192), 1 << 15), TJ_ERR_ALIGN);
+    expect("diff bwd workspace", bwd(TJ_F16, 2, 2, 16, 64, 128, stats, dlam, st, 1, nullptr, 0), TJ_ERR_WORKSPACE);
+    expect("diff bwd small workspace", bwd(TJ_F16, 2, 2, 16, 64, 128, stats, dlam, st, 1, at(8192), 32), TJ_ERR_WORKSPACE);
+    expect("diff bwd empty", bwd(TJ_F16, 2, 2, 0, 64, 128, stats, dlam, st, 1, nullptr, 0), TJ_OK);
+
+    // tj_layer_norm_fwd(x, weight, bias, y, dtype, w_dtype, rows, cols, x_stride, y_stride, eps, mean, rstd, stream)
+    auto norm = [&](const void* x, const void* w, int dtype, int w_dtype, int64_t rows, int64_t cols, float* mean) {
+      return tj_layer_norm_fwd(x, w, nullptr, o, dtype, w_dtype, rows, cols, cols, cols, 1e-5f, mean, nullptr, nullptr);
+    };
+    expect("norm dtype", norm(q, k, 5, TJ_F32, 4, 64, nullptr), TJ_ERR_DTYPE);
+    expect("norm weight dtype", norm(q, k, TJ_F16, TJ_BF16, 4, 64, nullptr), TJ_ERR_DTYPE);
+    expect("norm rows", norm(q, k, TJ_F16, TJ_F32, -1, 64, nullptr), TJ_ERR_SHAPE);
+    expect("norm huge rows", norm(q, k, TJ_F16, TJ_F32, kBig, 64, nullptr), TJ_ERR_SHAPE);
+    expect("norm no columns", norm(q, k, TJ_F16, TJ_F32, 4, 0, nullptr), TJ_ERR_SHAPE);
+    expect("norm wide", norm(q, k, TJ_F16, TJ_F32, 4, 16385, nullptr), TJ_ERR_UNSUPPORTED);
+    expect("norm half the stats", norm(q, k, TJ_F16, TJ_F32, 4, 64, stats), TJ_ERR_SHAPE);
+    expect("norm missing x", norm(nullptr, k, TJ_F16, TJ_F32, 4, 64, nullptr), TJ_ERR_SHAPE);
+    expect("norm x alignment", norm(at(1), k, TJ_F16, TJ_F32, 4, 64, nullptr), TJ_ERR_ALIGN);
+    expect("norm weight alignment", norm(q, at(2), TJ_F16, TJ_F32, 4, 64, nullptr), TJ_ERR_ALIGN);
+    expect("norm eps", tj_layer_norm_fwd(q, k, nullptr, o, TJ_F16, TJ_F32, 4, 64, 64, 64, -1.f, nullptr, nullptr, nullptr), TJ_ERR_SHAPE);
+    expect("norm no rows", norm(nullptr, k, TJ_F16, TJ_F32, 0, 64, nullptr), TJ_OK);
+    expect_size("norm workspace of huge sizes", tj_layer_norm_bwd_workspace_bytes(kBig, kBig), 0);
+    auto norm_bwd = [&](const void* dy, const float* mean, int dtype, int64_t rows, int64_t cols, void* dw, size_t bytes) {
+      return tj_layer_norm_bwd(dy, q, k, mean, stats, o, dw, nullptr, dtype, TJ_F32, rows, cols, cols, cols, cols,
+                               at(8192), bytes, nullptr);
+    };
+    expect("norm bwd dtype", norm_bwd(v, stats, -1, 4, 64, at(5120), 1 << 15), TJ_ERR_DTYPE);
+    expect("norm bwd huge rows", norm_bwd(v, stats, TJ_F16, kBig, 64, at(5120), 1 << 15), TJ_ERR_SHAPE);
+    expect("norm bwd wide", norm_bwd(v, stats, TJ_F16, 4, kBig, at(5120), 1 << 15), TJ_ERR_UNSUPPORTED);
+    expect("norm bwd missing dy", norm_bwd(nullptr, stats, TJ_F16, 4, 64, at(5120), 1 << 15), TJ_ERR_SHAPE);
+    expect("norm bwd missing mean", norm_bwd(v, nullptr, TJ_F16, 4, 64, at(5120), 1 << 15), TJ_ERR_SHAPE);
+    expect("norm bwd alignment", norm_bwd(at(3), stats, TJ_F16, 4, 64, at(5120), 1 << 15), TJ_ERR_ALIGN);
+    expect("norm bwd workspace", norm_bwd(v, stats, TJ_F16, 4, 64, at(5120), 16), TJ_ERR_WORKSPACE);
+    expect("norm bwd no rows", norm_bwd(nullptr, stats, TJ_F16, 0, 64, at(5120), 16), TJ_OK);
+  }
+
   if (g_failures != 0) {
     std::printf("%d check(s) failed\n", g_failures);
     return 1;
