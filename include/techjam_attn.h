@@ -399,6 +399,8 @@ int tj_narrow_ffn_norm(const float* x, const float* w_in, const float* bias_in, 
  * inputs run on MFMAs of that type with fp32 accumulation (probabilities are
  * rounded to it for the product with v), those of fp32 inputs in fp32; the
  * softmax runs in fp32. D <= 128, Dv <= 256, both multiples of 16 bytes.
+ * Strides as everywhere here; the rows of q, k, v (and dout below) run forward
+ * in memory, 64 of them within 2 GiB (TJ_ERR_UNSUPPORTED otherwise).
  *
  * lse and maps, both or neither: what tj_diff_attn_bwd reads again, contiguous
  * fp32: with R = Sq * H / Hk rows i * H / Hk + h % (H / Hk) per key head, the

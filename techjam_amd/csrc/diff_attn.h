@@ -30,7 +30,7 @@ namespace tj {
 struct DiffArgs {
   const void *q, *k, *v;
   void* o;
-  float* maps;             // [B, Hk, R, 2, Dv] P_0 V and P_1 V for the backward pass, or null
+  float* maps;             // [B, H, Sq, 2, Dv] P_0 V and P_1 V for the backward pass, or null
   View4 vq, vk, vv, vo;
   int B, H, Hk, G, D, Dv;
   int Sq, Sk;              // query tokens, key tokens (capacity of a cache)
@@ -41,7 +41,7 @@ struct DiffArgs {
   const float* lam;
   int lam_step;            // elements between the weights of two heads: 0 or 1
   const int32_t* len;      // [B] or null
-  float* lse;              // [B, Hk, 2, R] log2 of a row's sum of 2^(score log2 e), +inf for empty rows; or null
+  float* lse;              // [B, H, 2, Sq] log2 of a row's sum of 2^(score log2 e), +inf for empty rows; or null
   int n_mtiles;
   // Key parts: part p covers keys p part_keys .. (p + 1) part_keys - 1 and leaves unnormalised sums
   // [n_parts, B, Hk, R, 2, Dv] and (maximum, sum) pairs [n_parts, B, Hk, R, 2, 2].
@@ -53,8 +53,8 @@ struct DiffArgs {
   void *dq, *dk, *dv;
   float* dlam;             // [H], or [1] when lam_step is 0
   int n_lam;
-  float* delta;            // [B, Hk, 2, R] rowsum(dO o O_m)
-  float* gsum;             // [B, Hk, R] rowsum(P_1 o dP), the row's part of -dlam
+  float* delta;            // [B, H, 2, Sq] rowsum(dO o O_m)
+  float* gsum;             // [B, H, Sq] rowsum(P_1 o dP), the row's part of -dlam
   float* peak;             // [B, Hk, 2, kPeakParts] largest norms of dO and V rows (fp16 operands)
   int n_peaks;
 };
@@ -125,21 +125,33 @@ __device__ __forceinline__ frag_t<T> acc_frag(const float16_t& c, int s) {
   return f;
 }
 
-// An LDS tile: rows of W elements, 16 bytes of padding after each.
+// An LDS tile of rows of W elements without padding. The 16-byte chunk c of a
+// row stands at position c ^ swizzle(row), so that both readers below touch
+// every bank as often as they must and no more: eight lanes taking one chunk of
+// eight rows, and sixteen lanes taking two chunks of four rows.
 template <typename T, int W>
 struct LdsRows {
   static constexpr int kVec = 16 / (int)sizeof(T);
-  static constexpr int kStride = W + kVec;
   static constexpr int kChunks = W / kVec;
+  static constexpr int kRowBytes = W * (int)sizeof(T);
 
-  // The fragment of eight consecutive elements of one row.
+  __device__ __forceinline__ static int swizzle(int row) {
+    if constexpr (kChunks == 4) return (row >> 1) & 3;
+    else if constexpr (kChunks == 8) return row & 7;
+    else return (2 * row) & 14;
+  }
+  __device__ __forceinline__ static const char* at(const T* t, int row, int chunk) {
+    return reinterpret_cast<const char*>(t) + row * kRowBytes + ((chunk ^ swizzle(row)) << 4);
+  }
+
+  // The fragment of eight consecutive elements (k a multiple of 8) of one row.
   __device__ __forceinline__ static frag_t<T> row_frag(const T* t, int row, int k) {
-    const T* p = t + row * kStride + k;
     if constexpr (sizeof(T) == 4) {
-      const float4_t a = *reinterpret_cast<const float4_t*>(p), b = *reinterpret_cast<const float4_t*>(p + 4);
+      const float4_t a = *reinterpret_cast<const float4_t*>(at(t, row, k / 4));
+      const float4_t b = *reinterpret_cast<const float4_t*>(at(t, row, k / 4 + 1));
       return frag_t<T>{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
     } else {
-      return *reinterpret_cast<const frag_t<T>*>(p);
+      return *reinterpret_cast<const frag_t<T>*>(at(t, row, k / 8));
     }
   }
 
@@ -149,39 +161,81 @@ struct LdsRows {
   __device__ __forceinline__ static frag_t<T> col_frag(const T* t, int row0, int col0, int lane) {
     const int hl = lane / 32;
     if constexpr (sizeof(T) == 4) {
-      const float* p = t + (row0 + 4 * hl) * kStride + col0 + lane % 32;
       frag_t<T> f;
+      const int col = col0 + lane % 32;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = p[(j / 4 * 8 + j % 4) * kStride];
+      for (int j = 0; j < 8; ++j)
+        f[j] = *reinterpret_cast<const float*>(at(t, row0 + 4 * hl + j / 4 * 8 + j % 4, col / 4) + 4 * (col % 4));
       return f;
     } else {
       typedef short short4_t __attribute__((ext_vector_type(4)));
-      typedef short short8_t __attribute__((ext_vector_type(8)));
       typedef __attribute__((address_space(3))) short4_t lds_short4;
-      const T* p = t + (row0 + 4 * hl + (lane & 15) / 4) * kStride + col0 + (lane & 16) + 4 * (lane & 3);
+      const int row = row0 + 4 * hl + (lane & 15) / 4;
+      const char* p = at(t, row, col0 / 8 + (lane & 16) / 8 + (lane & 3) / 2) + 8 * (lane & 1);
+      // Eight rows on, the swizzle is the same.
       const short4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)p);
-      const short4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(p + 8 * kStride));
+      const short4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(p + 8 * kRowBytes));
       return __builtin_bit_cast(frag_t<T>, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
     }
   }
+};
 
-  // Rows 0 .. ROWS-1 from memory: row_ptr(row) is the row's address, null for
-  // one that reads as zeros; elements at or past `width` read as zeros too.
-  template <int ROWS, int THREADS = kDiffThreads, typename F>
-  __device__ __forceinline__ static void fill(T* t, int tid, int width, F&& row_ptr) {
-#pragma unroll
-    for (int u = 0; u < ROWS * kChunks; u += THREADS) {
-      const int e = u + tid;
-      if (ROWS * kChunks % THREADS == 0 || e < ROWS * kChunks) {
-        const int row = e / kChunks, c = e % kChunks * kVec;
-        const T* p = row_ptr(row);
-        float4_t x = {0.f, 0.f, 0.f, 0.f};
-        if (p != nullptr && c < width) x = *reinterpret_cast<const float4_t*>(p + c);
-        *reinterpret_cast<float4_t*>(t + row * kStride + c) = x;
-      }
-    }
+// ROWS rows of memory into an LDS tile, by WAVES waves, without registers:
+// each instruction brings 64 chunks of 16 bytes to consecutive places, so a
+// lane asks for the chunk that belongs at its place. Bounds-checked buffer
+// loads: what lies outside the resource, and columns at or past the width, land
+// as zeros. The copies are in flight until the wave has waited for them
+// (wait_copies) and the workgroup has met.
+constexpr uint32_t kOutside = 0x80000000u;
+
+template <typename T, int W, int ROWS, int WAVES>
+struct TileCopy {
+  using L = LdsRows<T, W>;
+  static constexpr int kRowsPer = 64 / L::kChunks;             // rows of one instruction
+  static constexpr int kTotal = ROWS / kRowsPer;               // instructions of the tile
+  static constexpr int N = (kTotal + WAVES - 1) / WAVES;       // of one wave
+  static_assert(ROWS % kRowsPer == 0 && (kTotal % WAVES == 0 || kTotal < WAVES), "tile rows");
+
+  __device__ __forceinline__ static int row(int wave, int n, int lane) {
+    return (wave * N + n) * kRowsPer + lane / L::kChunks;
+  }
+  // Byte offset of the lane's chunk in its row, outside for columns past `width`.
+  __device__ __forceinline__ static uint32_t chunk(int row, int lane, int width) {
+    const int c = (lane % L::kChunks) ^ L::swizzle(row);
+    return c * L::kVec < width ? (uint32_t)c * 16 : kOutside;
+  }
+  __device__ __forceinline__ static void issue(__amdgpu_buffer_rsrc_t r, T* tile, int wave, int n, uint32_t voff) {
+    if (kTotal < WAVES && wave >= kTotal) return;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(
+        r, (__attribute__((address_space(3))) void*)(reinterpret_cast<char*>(tile) + (wave * N + n) * 1024), 16, voff, 0, 0, 0);
   }
 };
+
+// A tile of consecutive rows (keys), whose lanes' offsets never change: the
+// resource moves along.
+template <typename T, int W, int ROWS, int WAVES>
+struct KeyCopy : TileCopy<T, W, ROWS, WAVES> {
+  using C = TileCopy<T, W, ROWS, WAVES>;
+  uint32_t voff[C::N];
+  __device__ __forceinline__ void init(int64_t row_stride, int width, int wave, int lane) {
+#pragma unroll
+    for (int n = 0; n < C::N; ++n) {
+      const int r = C::row(wave, n, lane);
+      const uint32_t c = C::chunk(r, lane, width);
+      voff[n] = c == kOutside ? kOutside : (uint32_t)r * (uint32_t)(row_stride * (int64_t)sizeof(T)) + c;
+    }
+  }
+  // Rows 0 .. rows-1 from `p` on; further rows of the tile read as zeros.
+  __device__ __forceinline__ void issue(const T* p, int64_t row_stride, int rows, int width, T* tile, int wave) const {
+    const int64_t bytes = rows <= 0 ? 0 : ((int64_t)(min(rows, ROWS) - 1) * row_stride + width) * (int64_t)sizeof(T);
+    const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(p), (short)0, (int)bytes, kDiffBufferFlags);
+#pragma unroll
+    for (int n = 0; n < C::N; ++n) C::issue(r, tile, wave, n, voff[n]);
+  }
+};
+
+// This wave's copies (and loads) and LDS accesses are done.
+__device__ __forceinline__ void wait_copies() { __builtin_amdgcn_s_waitcnt(0x0070); }
 
 // Eight consecutive elements of a row in memory, zeros at or past `width`.
 template <typename T>
@@ -245,6 +299,15 @@ __device__ __forceinline__ float ds_lift(const DiffArgs& a, int bh, int hk, int 
     if (!(x > 0.f) || !(y > 0.f)) return 1.f;
     return ldexpf(1.f, min(max(14 - ex - ey - ew, -100), 100));
   }
+}
+
+// A row's place in the arrays [B, H, Sq].
+__device__ __forceinline__ int64_t row_at(const DiffArgs& a, int b, int head, int i) {
+  return ((int64_t)b * a.H + head) * a.Sq + i;
+}
+// Its place in the arrays [B, H, 2, Sq], for map c.
+__device__ __forceinline__ int64_t map_at(const DiffArgs& a, int b, int head, int c, int i) {
+  return (((int64_t)b * a.H + head) * 2 + c) * a.Sq + i;
 }
 
 // The same for P_0 - lam P_1 (at most 1 + |lam|).

@@ -70,6 +70,11 @@ bool view_ok(const void* p, const int64_t st[4], int dtype) {
   return st[0] % vec == 0 && st[1] % vec == 0 && st[2] % vec == 0;
 }
 
+// Rows that the tile copies reach by 31-bit byte offsets, up to 64 at a time.
+bool rows_ok(const int64_t st[4], int dtype) {
+  return st[2] >= 0 && st[2] < (int64_t(1) << 31) / (64 * elem_bytes(dtype));
+}
+
 View4 view(const int64_t st[4]) { return View4{st[0], st[1], st[2]}; }
 
 bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
@@ -102,6 +107,7 @@ extern "C" int tj_diff_attn_fwd(const void* q, const void* k, const void* v, voi
   if (!view_ok(q, q_strides, dtype) || !view_ok(k, k_strides, dtype) || !view_ok(v, v_strides, dtype) ||
       !view_ok(o, o_strides, dtype) || !tjh::aligned16(maps) || !aligned4(lam) || !aligned4(lengths) || !aligned4(lse))
     return TJ_ERR_ALIGN;
+  if (!rows_ok(k_strides, dtype) || !rows_ok(v_strides, dtype)) return TJ_ERR_UNSUPPORTED;
   DiffArgs a{};
   a.q = q; a.k = k; a.v = v; a.o = o; a.maps = maps;
   a.vq = view(q_strides); a.vk = view(k_strides); a.vv = view(v_strides); a.vo = view(o_strides);
@@ -152,6 +158,8 @@ extern "C" int tj_diff_attn_bwd(const void* q, const void* k, const void* v, con
       !view_ok(dq, dq_strides, dtype) || !view_ok(dk, dk_strides, dtype) || !view_ok(dv, dv_strides, dtype) ||
       !aligned4(lam) || !aligned4(dlam) || !aligned4(lengths) || !aligned4(lse))
     return TJ_ERR_ALIGN;
+  for (const int64_t* st : {q_strides, k_strides, v_strides, do_strides})
+    if (!rows_ok(st, dtype)) return TJ_ERR_UNSUPPORTED;
   if (workspace == nullptr || workspace_bytes < tj_diff_attn_bwd_workspace_bytes(B, H, Hk, S)) return TJ_ERR_WORKSPACE;
   if (!tjh::aligned16(workspace)) return TJ_ERR_ALIGN;
   DiffArgs a{};

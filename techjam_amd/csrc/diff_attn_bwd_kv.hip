@@ -6,10 +6,10 @@
 //   dS_m = c_m P_m (dP - delta_m)
 //   dV = sum over rows of (P_0 - lam P_1)^T dO,   dK_m = scale sum over rows of dS_m^T Q_m.
 //
-// One workgroup = 4 waves = 128 keys of one (b, key head), 32 keys a wave, all
-// the rows that see them in turn through LDS; the rows of the G heads that
-// share the keys are one list, so nothing is added up across workgroups and the
-// result does not depend on their order. Scores are formed with rows in the
+// One workgroup = 4 waves = 128 keys of one (b, key head), 32 keys a wave; the
+// tokens that see them come through LDS in tiles of 32, one query head of the
+// group after the other, so that nothing is added up across workgroups and the
+// result does not depend on their order. Scores are formed with tokens in the
 // registers and keys over the lanes, so that P and dS turn into the A operands
 // of dV and dK where they stand; Q and dO come back as B operands through the
 // transposing LDS read.
@@ -26,15 +26,36 @@ __global__ __launch_bounds__(kDiffThreads, 1) void diff_bwd_kv_kernel(DiffArgs a
   constexpr bool DO_DV = (WHAT & 1) != 0, DO_DK = (WHAT & 2) != 0;
   using QT = LdsRows<T, HD>;
   using OT = LdsRows<T, DVP>;
-  __shared__ __attribute__((aligned(16))) T sq[2][BM * QT::kStride];
-  __shared__ __attribute__((aligned(16))) T so[BM * OT::kStride];
-  // lse_0, lse_1, delta_0, lam delta_1 (lifted), -lam (lifted), -lam
-  __shared__ __attribute__((aligned(16))) float stat[6][BM];
-  const int tid = threadIdx.x, w = tid / kWave, lane = tid % kWave, hl = lane / 32, ln = lane % 32;
+  constexpr int kTile = BM * (2 * HD + DVP);  // Q's two heads and dO
+  __shared__ __attribute__((aligned(1024))) T smem[2][kTile];
+  // lse_0, lse_1 (with the lift), -delta_0 and lam delta_1 (lifted) of a tile's tokens
+  __shared__ __attribute__((aligned(16))) float stat[2][4][BM];
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave, hl = lane / 32,
+            ln = lane % 32;
   const DiffTile t = diff_tile(a, blockIdx.x, a.n_mtiles);
   const int L = diff_len(a, t.b);
   const int k0 = t.tile * 128, kw0 = k0 + 32 * w, key = kw0 + ln;
   const bool live = key < L;
+
+  const T* qp = reinterpret_cast<const T*>(a.q) + a.vq.row(t.b, 2 * t.hk * a.G, 0);
+  const T* op = reinterpret_cast<const T*>(a.dout) + a.vdo.row(t.b, t.hk * a.G, 0);
+  KeyCopy<T, HD, BM, 4> qcopy;
+  KeyCopy<T, DVP, BM, 4> ocopy;
+  qcopy.init(a.vq.ss, a.D, w, lane);
+  ocopy.init(a.vdo.ss, a.Dv, w, lane);
+  // Tiles of the group's heads: head g of it, tokens i0 .. i0 + 31.
+  auto issue = [&](int g, int i0, T* tile) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+      qcopy.issue(qp + (2 * g + c) * a.vq.sh + i0 * a.vq.ss, a.vq.ss, L - i0, a.D, tile + c * BM * HD, w);
+    ocopy.issue(op + g * a.vdo.sh + i0 * a.vdo.ss, a.vdo.ss, L - i0, a.Dv, tile + 2 * BM * HD, w);
+  };
+  // Thread tid < 128 carries number tid / 32 of token tid % 32.
+  const float* sp = tid < 64 ? a.lse : a.delta;
+  auto load_stat = [&](int g, int i0) {
+    const int i = i0 + tid % BM;
+    return tid < 128 && i < L ? sp[map_at(a, t.b, t.hk * a.G + g, (tid / BM) & 1, i)] : 0.f;
+  };
 
   frag_t<T> kf[2][KS], vf[DO_DK ? VS : 1];
   {
@@ -65,96 +86,90 @@ __global__ __launch_bounds__(kDiffThreads, 1) void diff_bwd_kv_kernel(DiffArgs a
   const float pl = p_lift<T>(lam_max), dl = ds_lift<T>(a, t.bh, t.hk, lane), log_pl = log2f(pl);
   const float lift = dl / pl;
   const float c2 = a.scale * kLog2e;
-  const int r_end = k0 < L ? min(a.R, L * a.G) : 0;
-  const int r_begin = a.causal ? k0 * a.G / BM * BM : 0;
-  const T* qp = reinterpret_cast<const T*>(a.q);
-  const T* op = reinterpret_cast<const T*>(a.dout);
-  const float* lse = a.lse + (int64_t)t.bh * 2 * a.R;
-  const float* del = a.delta + (int64_t)t.bh * 2 * a.R;
-  for (int r0 = r_begin; r0 < r_end; r0 += BM) {
-    __syncthreads();
-#pragma unroll
-    for (int c = 0; c < 2; ++c)
-      QT::template fill<BM>(sq[c], tid, a.D, [&](int row) {
-        const int r = r0 + row;
-        return r < r_end ? qp + a.vq.row(t.b, 2 * (t.hk * a.G + r % a.G) + c, r / a.G) : nullptr;
-      });
-    OT::template fill<BM>(so, tid, a.Dv, [&](int row) {
-      const int r = r0 + row;
-      return r < r_end ? op + a.vdo.row(t.b, t.hk * a.G + r % a.G, r / a.G) : nullptr;
-    });
-    if (tid < BM) {
-      const int r = r0 + tid;
-      const bool in = r < r_end;
-      const float lam = a.lam[(t.hk * a.G + (in ? r % a.G : 0)) * a.lam_step];
-      // A row that is not there weighs nothing: P = 2^(0 - inf).
-      stat[0][tid] = in ? lse[r] - log_pl : __builtin_inff();
-      stat[1][tid] = in ? lse[a.R + r] - log_pl : __builtin_inff();
-      stat[2][tid] = in ? -del[r] * lift : 0.f;
-      stat[3][tid] = in ? lam * del[a.R + r] * lift : 0.f;
-      stat[4][tid] = in ? -lam * lift : 0.f;
-      stat[5][tid] = in ? -lam : 0.f;
-    }
-    __syncthreads();
-    if (a.causal && min(r0 + BM, r_end) - 1 < kw0 * a.G) continue;  // every row stands before the wave's keys
-
-    float16_t p[2];
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      p[c] = zero16();
-#pragma unroll
-      for (int s = 0; s < KS; ++s) p[c] = Elem<T>::mma(QT::row_frag(sq[c], ln, 16 * s + 8 * hl), kf[c][s], p[c]);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float4_t ls = *reinterpret_cast<const float4_t*>(&stat[c][8 * q + 4 * hl]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) p[c][4 * q + j] = fast_exp2(fmaf(p[c][4 * q + j], c2, -ls[j]));
+  const int i_begin = a.causal ? k0 : 0;
+  if (i_begin < L) {
+    issue(0, i_begin, smem[0]);
+    float next = load_stat(0, i_begin);
+    int cur = 0;
+    for (int g = 0, i0 = i_begin; g < a.G; cur ^= 1) {
+      const float lam = a.lam[(t.hk * a.G + g) * a.lam_step];
+      wait_copies();
+      if (tid < 128) {
+        const int n = tid / BM;
+        // A token that is not there weighs nothing: P = 2^(0 - inf).
+        const bool in = i0 + tid % BM < L;
+        stat[cur][n][tid % BM] = n < 2 ? (in ? next - log_pl : __builtin_inff()) : next * (n == 2 ? -lift : lam * lift);
       }
-      if (a.causal && r0 < (kw0 + 31) * a.G) {
-#pragma unroll
-        for (int r = 0; r < 16; ++r)
-          if (r0 + acc_row(r, hl) < key * a.G) p[c][r] = 0.f;
+      wait_lds();
+      lds_barrier();
+      int g1 = g, i1 = i0 + BM;
+      if (i1 >= L) {
+        i1 = i_begin;
+        ++g1;
       }
-    }
-    if constexpr (DO_DV) {
-      float16_t mix;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float4_t nl = *reinterpret_cast<const float4_t*>(&stat[5][8 * q + 4 * hl]);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) mix[4 * q + j] = fmaf(nl[j], p[1][4 * q + j], p[0][4 * q + j]);
+      if (g1 < a.G) {
+        issue(g1, i1, smem[cur ^ 1]);
+        next = load_stat(g1, i1);
       }
+      const T *sq[2] = {smem[cur], smem[cur] + BM * HD}, *so = smem[cur] + 2 * BM * HD;
+      if (!a.causal || i0 + BM > kw0) {  // else every token stands before the wave's keys
+        float16_t p[2];
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const frag_t<T> f = acc_frag<T>(mix, s);
+        for (int c = 0; c < 2; ++c) {
+          p[c] = zero16();
 #pragma unroll
-        for (int d = 0; d < VB; ++d) dv[d] = Elem<T>::mma(f, OT::col_frag(so, 16 * s, 32 * d, lane), dv[d]);
-      }
-    }
-    if constexpr (DO_DK) {
-      float16_t dp = zero16();
+          for (int s = 0; s < KS; ++s) p[c] = Elem<T>::mma(QT::row_frag(sq[c], ln, 16 * s + 8 * hl), kf[c][s], p[c]);
 #pragma unroll
-      for (int s = 0; s < VS; ++s) dp = Elem<T>::mma(OT::row_frag(so, ln, 16 * s + 8 * hl), vf[s], dp);
+          for (int q = 0; q < 4; ++q) {
+            const float4_t ls = *reinterpret_cast<const float4_t*>(&stat[cur][c][8 * q + 4 * hl]);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float4_t d0 = *reinterpret_cast<const float4_t*>(&stat[2][8 * q + 4 * hl]);
-        const float4_t d1 = *reinterpret_cast<const float4_t*>(&stat[3][8 * q + 4 * hl]);
-        const float4_t nl = *reinterpret_cast<const float4_t*>(&stat[4][8 * q + 4 * hl]);
+            for (int j = 0; j < 4; ++j) p[c][4 * q + j] = fast_exp2(fmaf(p[c][4 * q + j], c2, -ls[j]));
+          }
+          if (a.causal && i0 < kw0 + 31) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float x = dp[4 * q + j];
-          p[0][4 * q + j] *= fmaf(x, lift, d0[j]);
-          p[1][4 * q + j] *= fmaf(x, nl[j], d1[j]);
+            for (int r = 0; r < 16; ++r)
+              if (i0 + acc_row(r, hl) < key) p[c][r] = 0.f;
+          }
+        }
+        if constexpr (DO_DV) {
+          float16_t mix;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) mix[r] = fmaf(-lam, p[1][r], p[0][r]);
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            const frag_t<T> f = acc_frag<T>(mix, s);
+#pragma unroll
+            for (int d = 0; d < VB; ++d) dv[d] = Elem<T>::mma(f, OT::col_frag(so, 16 * s, 32 * d, lane), dv[d]);
+          }
+        }
+        if constexpr (DO_DK) {
+          float16_t dp = zero16();
+#pragma unroll
+          for (int s = 0; s < VS; ++s) dp = Elem<T>::mma(OT::row_frag(so, ln, 16 * s + 8 * hl), vf[s], dp);
+          const float nl = -lam * lift;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float4_t d0 = *reinterpret_cast<const float4_t*>(&stat[cur][2][8 * q + 4 * hl]);
+            const float4_t d1 = *reinterpret_cast<const float4_t*>(&stat[cur][3][8 * q + 4 * hl]);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float x = dp[4 * q + j];
+              p[0][4 * q + j] *= fmaf(x, lift, d0[j]);
+              p[1][4 * q + j] *= fmaf(x, nl, d1[j]);
+            }
+          }
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+              const frag_t<T> f = acc_frag<T>(p[c], s);
+#pragma unroll
+              for (int d = 0; d < KB; ++d) dk[c][d] = Elem<T>::mma(f, QT::col_frag(sq[c], 16 * s, 32 * d, lane), dk[c][d]);
+            }
         }
       }
-#pragma unroll
-      for (int c = 0; c < 2; ++c)
-#pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          const frag_t<T> f = acc_frag<T>(p[c], s);
-#pragma unroll
-          for (int d = 0; d < KB; ++d) dk[c][d] = Elem<T>::mma(f, QT::col_frag(sq[c], 16 * s, 32 * d, lane), dk[c][d]);
-        }
+      g = g1;
+      i0 = i1;
     }
   }
 

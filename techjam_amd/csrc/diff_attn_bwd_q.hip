@@ -33,7 +33,7 @@ __global__ __launch_bounds__(kDiffThreads) void diff_delta_kernel(DiffArgs a, in
     float d0 = 0.f, d1 = 0.f, n = 0.f;
     if (i < L && on) {
       const vec_t x = *reinterpret_cast<const vec_t*>(reinterpret_cast<const T*>(a.dout) + a.vdo.row(b, head, i) + lane * VEC);
-      const float* mp = a.maps + ((int64_t)bh * a.R + r) * 2 * a.Dv + lane * VEC;
+      const float* mp = a.maps + row_at(a, b, head, i) * 2 * a.Dv + lane * VEC;
 #pragma unroll
       for (int e = 0; e < VEC; e += 4) {
         const float4_t y = *reinterpret_cast<const float4_t*>(mp + e), z = *reinterpret_cast<const float4_t*>(mp + a.Dv + e);
@@ -52,9 +52,8 @@ __global__ __launch_bounds__(kDiffThreads) void diff_delta_kernel(DiffArgs a, in
       n += __shfl_xor(n, s);
     }
     if (lane == 0) {
-      float* del = a.delta + (int64_t)bh * 2 * a.R + r;
-      del[0] = d0;
-      del[a.R] = d1;
+      a.delta[map_at(a, b, head, 0, i)] = d0;
+      a.delta[map_at(a, b, head, 1, i)] = d1;
     }
     if (n < 3e38f) peak_o = fmaxf(peak_o, n);  // not those that are not finite: they spoil their own row only
   }
@@ -94,9 +93,9 @@ __global__ __launch_bounds__(kDiffThreads, 1) void diff_bwd_q_kernel(DiffArgs a)
   constexpr int DVP = 2 * HD, KS = HD / 16, VS = DVP / 16, KB = HD / 32, BN = 32;
   using KT = LdsRows<T, HD>;
   using VT = LdsRows<T, DVP>;
-  __shared__ __attribute__((aligned(16))) T sk[2][BN * KT::kStride];
-  __shared__ __attribute__((aligned(16))) T sv[BN * VT::kStride];
-  const int tid = threadIdx.x, w = tid / kWave, lane = tid % kWave, hl = lane / 32, ln = lane % 32;
+  constexpr int kTile = BN * (2 * HD + DVP);  // K's two heads and V
+  __shared__ __attribute__((aligned(1024))) T smem[2][kTile];
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave, hl = lane / 32, ln = lane % 32;
   const DiffTile t = diff_tile(a, blockIdx.x, a.n_mtiles);
   const int mt = a.n_mtiles - 1 - t.tile;
   const int L = diff_len(a, t.b);
@@ -130,26 +129,32 @@ __global__ __launch_bounds__(kDiffThreads, 1) void diff_bwd_q_kernel(DiffArgs a)
   float lse[2], del[2];
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
-    lse[c] = live ? a.lse[((int64_t)t.bh * 2 + c) * a.R + r] : __builtin_inff();
-    del[c] = live ? a.delta[((int64_t)t.bh * 2 + c) * a.R + r] : 0.f;
+    lse[c] = live ? a.lse[map_at(a, t.b, head, c, i)] : __builtin_inff();
+    del[c] = live ? a.delta[map_at(a, t.b, head, c, i)] : 0.f;
   }
   const float d0 = -del[0] * lift, nl = -lam * lift;
   float rest = 0.f;
 
   const T* kp = reinterpret_cast<const T*>(a.k) + a.vk.row(t.b, 2 * t.hk, 0);
   const T* vp = reinterpret_cast<const T*>(a.v) + a.vv.row(t.b, t.hk, 0);
-  for (int kv0 = 0; kv0 < kv_end; kv0 += BN) {
-    __syncthreads();
+  KeyCopy<T, HD, BN, 4> kcopy;
+  KeyCopy<T, DVP, BN, 4> vcopy;
+  kcopy.init(a.vk.ss, a.D, w, lane);
+  vcopy.init(a.vv.ss, a.Dv, w, lane);
+  auto issue = [&](int kv0, T* tile) {
 #pragma unroll
     for (int c = 0; c < 2; ++c)
-      KT::template fill<BN>(sk[c], tid, a.D, [&](int row) {
-        return kv0 + row < L ? kp + c * a.vk.sh + (kv0 + row) * a.vk.ss : nullptr;
-      });
-    VT::template fill<BN>(sv, tid, a.Dv, [&](int row) {
-      return kv0 + row < L ? vp + (kv0 + row) * a.vv.ss : nullptr;
-    });
-    __syncthreads();
+      kcopy.issue(kp + c * a.vk.sh + kv0 * a.vk.ss, a.vk.ss, L - kv0, a.D, tile + c * BN * HD, w);
+    vcopy.issue(vp + kv0 * a.vv.ss, a.vv.ss, L - kv0, a.Dv, tile + 2 * BN * HD, w);
+  };
+  if (kv_end > 0) issue(0, smem[0]);
+  int cur = 0;
+  for (int kv0 = 0; kv0 < kv_end; kv0 += BN, cur ^= 1) {
+    wait_copies();
+    lds_barrier();
+    if (kv0 + BN < kv_end) issue(kv0 + BN, smem[cur ^ 1]);
     if (kv0 >= own_end) continue;
+    const T *sk[2] = {smem[cur], smem[cur] + BN * HD}, *sv = smem[cur] + 2 * BN * HD;
     float16_t p[2], dp = zero16();
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
@@ -188,7 +193,7 @@ __global__ __launch_bounds__(kDiffThreads, 1) void diff_bwd_q_kernel(DiffArgs a)
 
   rest = pair_sum(rest);
   if (r >= a.R) return;
-  if (hl == 0) a.gsum[(int64_t)t.bh * a.R + r] = live ? del[1] + rest : 0.f;
+  if (hl == 0) a.gsum[row_at(a, t.b, head, i)] = live ? del[1] + rest : 0.f;
   const float out = a.scale / lift;
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
@@ -213,8 +218,8 @@ __global__ __launch_bounds__(1024) void diff_dlam_kernel(DiffArgs a) {
   double s = 0.;
   for (int h = (a.lam_step ? n : 0); h < (a.lam_step ? n + 1 : a.H); ++h)
     for (int b = 0; b < a.B; ++b) {
-      const float* p = a.gsum + ((int64_t)b * a.Hk + h / a.G) * a.R + h % a.G;
-      for (int i = tid; i < a.Sq; i += 1024) s += p[(int64_t)i * a.G];
+      const float* p = a.gsum + row_at(a, b, h, 0);
+      for (int i = tid; i < a.Sq; i += 1024) s += p[i];
     }
   for (int m = kWave / 2; m > 0; m >>= 1) s += __shfl_xor(s, m);
   if (tid % kWave == 0) red[tid / kWave] = s;

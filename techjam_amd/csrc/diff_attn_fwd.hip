@@ -28,7 +28,7 @@ struct FwdShape {
   static constexpr int NKB = BN / 32;  // score blocks per tile
   static constexpr int NS = BN / 16;   // k-steps over the tile's keys
   static constexpr int DB = DVP / 32;  // output blocks
-  static constexpr int kElems = BN * (2 * KT::kStride + VT::kStride);
+  static constexpr int kElems = BN * (2 * HD + DVP);  // one tile of both key heads and of V
 };
 
 // A lane's row: r of the (b, key head), its token, head and position, and the last key it sees.
@@ -55,8 +55,9 @@ struct DiffSpan {
 };
 
 // The running state of a wave's 32 rows.
-template <typename T, typename SH>
+template <typename T, int HD, int BN>
 struct FwdState {
+  using SH = FwdShape<T, HD, BN>;
   frag_t<T> q[2][SH::KS];
   float16_t o[2][SH::DB];
   float m[2], l[2];  // maximum in log2 units, the lane's part of the sum
@@ -90,7 +91,7 @@ struct FwdState {
     frag_t<T> p[2][SH::NS];
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      const T* kc = kt + c * SH::BN * SH::KT::kStride;
+      const T* kc = kt + c * SH::BN * HD;
       float16_t s[SH::NKB];
 #pragma unroll
       for (int kb = 0; kb < SH::NKB; ++kb) {
@@ -180,14 +181,14 @@ struct FwdState {
       const float sum = pair_sum(l[c]);
       inv[c] = 1.f / sum;
       if (a.lse != nullptr && row.r < a.R && hl == 0)
-        a.lse[((int64_t)bh * 2 + c) * a.R + row.r] =
+        a.lse[map_at(a, b, head, c, row.i)] =
             row.live ? m[c] - Elem<T>::kLift + log2f(sum) : __builtin_inff();
     }
     if (row.r >= a.R) return;
     const float lam = a.lam[head * a.lam_step];
     const int64_t at = a.vo.row(b, head, row.i);
     T* op = reinterpret_cast<T*>(a.o) + at;
-    float* mp = a.maps + ((int64_t)bh * a.R + row.r) * 2 * a.Dv;
+    float* mp = a.maps + row_at(a, b, head, row.i) * 2 * a.Dv;
 #pragma unroll
     for (int d = 0; d < SH::DB; ++d)
 #pragma unroll
@@ -210,27 +211,33 @@ struct FwdState {
   }
 };
 
-// Keys kv0 .. kv0 + BN - 1 of K's two heads and of V into LDS; keys at or past L read as zeros, whatever is there.
-template <typename T, typename SH, int THREADS>
-__device__ __forceinline__ void fill_keys(const DiffArgs& a, T* kt, T* vt, const T* kp, const T* vp, int kv0, int L,
-                                          int tid) {
+// The key tiles of one (b, key head), by WAVES waves into LDS.
+template <typename T, typename SH, int HD, int WAVES>
+struct KeyTiles {
+  KeyCopy<T, HD, SH::BN, WAVES> k;
+  KeyCopy<T, 2 * HD, SH::BN, WAVES> v;
+  const T *kp, *vp;
+  __device__ __forceinline__ void init(const DiffArgs& a, int b, int hk, int wave, int lane) {
+    kp = reinterpret_cast<const T*>(a.k) + a.vk.row(b, 2 * hk, 0);
+    vp = reinterpret_cast<const T*>(a.v) + a.vv.row(b, hk, 0);
+    k.init(a.vk.ss, a.D, wave, lane);
+    v.init(a.vv.ss, a.Dv, wave, lane);
+  }
+  // Keys kv0 .. kv0 + BN - 1; those at or past L land as zeros, whatever is there.
+  __device__ __forceinline__ void issue(const DiffArgs& a, int kv0, int L, T* tile, int wave) const {
 #pragma unroll
-  for (int c = 0; c < 2; ++c)
-    SH::KT::template fill<SH::BN, THREADS>(kt + c * SH::BN * SH::KT::kStride, tid, a.D, [&](int row) {
-      return kv0 + row < L ? kp + c * a.vk.sh + (kv0 + row) * a.vk.ss : nullptr;
-    });
-  SH::VT::template fill<SH::BN, THREADS>(vt, tid, a.Dv, [&](int row) {
-    return kv0 + row < L ? vp + (kv0 + row) * a.vv.ss : nullptr;
-  });
-}
+    for (int c = 0; c < 2; ++c)
+      k.issue(kp + c * a.vk.sh + kv0 * a.vk.ss, a.vk.ss, L - kv0, a.D, tile + c * SH::BN * HD, wave);
+    v.issue(vp + kv0 * a.vv.ss, a.vv.ss, L - kv0, a.Dv, tile + 2 * SH::BN * HD, wave);
+  }
+};
 
 template <typename T, int HD, bool PART>
 __global__ __launch_bounds__(kDiffThreads, (sizeof(T) == 2 && HD <= 64 ? 2 : 1)) void diff_fwd_kernel(DiffArgs a) {
-  using SH = FwdShape<T, HD, (sizeof(T) == 4 ? 32 : 64)>;
-  __shared__ __attribute__((aligned(16))) T smem[SH::kElems];
-  T* kt = smem;
-  T* vt = kt + 2 * SH::BN * SH::KT::kStride;
-  const int tid = threadIdx.x, w = tid / kWave, lane = tid % kWave;
+  constexpr int BN = sizeof(T) == 4 ? 32 : 64;
+  using SH = FwdShape<T, HD, BN>;
+  __shared__ __attribute__((aligned(1024))) T smem[2][SH::kElems];
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
   const DiffTile t = diff_tile(a, blockIdx.x, a.n_mtiles);
   const int part = PART ? t.tile / a.n_mtiles : -1;
   const int mt = a.n_mtiles - 1 - (PART ? t.tile % a.n_mtiles : t.tile);
@@ -240,25 +247,28 @@ __global__ __launch_bounds__(kDiffThreads, (sizeof(T) == 2 && HD <= 64 ? 2 : 1))
   const int kv_begin = PART ? part * a.part_keys : 0;
   const int kv_end = PART ? min(all.end, kv_begin + a.part_keys) : all.end;
   if (PART && kv_begin >= kv_end) return;  // not read either (live parts are counted from the rows' last key)
-  FwdState<T, SH> st;
+  KeyTiles<T, SH, HD, 4> keys;
+  keys.init(a, t.b, t.hk, w, lane);
+  if (kv_begin < kv_end) keys.issue(a, kv_begin, L, smem[0], w);
+  FwdState<T, HD, BN> st;
   st.init(a, t.b, t.hk, row, lane);
-  const T* kp = reinterpret_cast<const T*>(a.k) + a.vk.row(t.b, 2 * t.hk, 0);
-  const T* vp = reinterpret_cast<const T*>(a.v) + a.vv.row(t.b, t.hk, 0);
-  for (int kv0 = kv_begin; kv0 < kv_end; kv0 += SH::BN) {
-    __syncthreads();
-    fill_keys<T, SH, kDiffThreads>(a, kt, vt, kp, vp, kv0, L, tid);
-    __syncthreads();
-    if (kv0 < own.end) st.tile(kt, vt, kv0, row.limit, kv0 + SH::BN - 1 > own.free, lane);
+  int cur = 0;
+  for (int kv0 = kv_begin; kv0 < kv_end; kv0 += BN, cur ^= 1) {
+    // The tile is there, and the other one has been read by every wave.
+    wait_copies();
+    lds_barrier();
+    if (kv0 + BN < kv_end) keys.issue(a, kv0 + BN, L, smem[cur ^ 1], w);
+    if (kv0 < own.end)
+      st.tile(smem[cur], smem[cur] + 2 * BN * HD, kv0, row.limit, kv0 + BN - 1 > own.free, lane);
   }
   st.finish(a, t.b, t.hk, row, part, lane);
 }
 
 template <typename T, int HD>
 __global__ __launch_bounds__(kWave) void diff_few_kernel(DiffArgs a) {
-  using SH = FwdShape<T, HD, 32>;
-  __shared__ __attribute__((aligned(16))) T smem[SH::kElems];
-  T* kt = smem;
-  T* vt = kt + 2 * SH::BN * SH::KT::kStride;
+  constexpr int BN = 32;
+  using SH = FwdShape<T, HD, BN>;
+  __shared__ __attribute__((aligned(1024))) T smem[2][SH::kElems];
   const int lane = threadIdx.x;
   const DiffTile t = diff_tile(a, blockIdx.x, a.n_mtiles * a.n_parts);
   const int mt = t.tile % a.n_mtiles, part = t.tile / a.n_mtiles;
@@ -267,15 +277,17 @@ __global__ __launch_bounds__(kWave) void diff_few_kernel(DiffArgs a) {
   const DiffRow row(a, mt * 32 + lane % 32, L);
   const int kv_begin = part * a.part_keys, kv_end = min(own.end, kv_begin + a.part_keys);
   if (kv_begin >= kv_end) return;
-  FwdState<T, SH> st;
+  KeyTiles<T, SH, HD, 1> keys;
+  keys.init(a, t.b, t.hk, 0, lane);
+  keys.issue(a, kv_begin, L, smem[0], 0);
+  FwdState<T, HD, BN> st;
   st.init(a, t.b, t.hk, row, lane);
-  const T* kp = reinterpret_cast<const T*>(a.k) + a.vk.row(t.b, 2 * t.hk, 0);
-  const T* vp = reinterpret_cast<const T*>(a.v) + a.vv.row(t.b, t.hk, 0);
-  for (int kv0 = kv_begin; kv0 < kv_end; kv0 += SH::BN) {
-    __syncthreads();
-    fill_keys<T, SH, kWave>(a, kt, vt, kp, vp, kv0, L, lane);
-    __syncthreads();
-    st.tile(kt, vt, kv0, row.limit, kv0 + SH::BN - 1 > own.free, lane);
+  int cur = 0;
+  for (int kv0 = kv_begin; kv0 < kv_end; kv0 += BN, cur ^= 1) {
+    wait_copies();
+    lds_barrier();
+    if (kv0 + BN < kv_end) keys.issue(a, kv0 + BN, L, smem[cur ^ 1], 0);
+    st.tile(smem[cur], smem[cur] + 2 * BN * HD, kv0, row.limit, kv0 + BN - 1 > own.free, lane);
   }
   st.finish(a, t.b, t.hk, row, part, lane);
 }
@@ -306,7 +318,7 @@ __global__ __launch_bounds__(kDiffThreads) void diff_join_kernel(DiffArgs a) {
     }
     for (int s = 32; s > 0; s >>= 1) l[c] += __shfl_xor(l[c], s);
     if (a.lse != nullptr && lane == 0)
-      a.lse[((int64_t)bh * 2 + c) * a.R + row.r] = row.live ? m[c] - Elem<T>::kLift + log2f(l[c]) : __builtin_inff();
+      a.lse[map_at(a, b, hk * a.G + row.g, c, row.i)] = row.live ? m[c] - Elem<T>::kLift + log2f(l[c]) : __builtin_inff();
   }
   const int head = hk * a.G + row.g;
   const float lam = a.lam[head * a.lam_step];
@@ -321,7 +333,7 @@ __global__ __launch_bounds__(kDiffThreads) void diff_join_kernel(DiffArgs a) {
         y[c] += mp == -__builtin_inff() ? o : fast_exp2(mp - m[c]) * o;
       }
       y[c] = row.live ? y[c] / l[c] : 0.f;
-      if (a.maps != nullptr) a.maps[(id * 2 + c) * a.Dv + col] = y[c];
+      if (a.maps != nullptr) a.maps[(row_at(a, b, head, row.i) * 2 + c) * a.Dv + col] = y[c];
     }
     reinterpret_cast<T*>(a.o)[at + col] = (T)fmaf(-lam, y[1], y[0]);
   }

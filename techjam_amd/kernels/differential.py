@@ -38,9 +38,11 @@ def on_device(device: torch.device):
 
 def _rows_view(t: torch.Tensor) -> torch.Tensor:
     """``t`` itself when the kernels can read it in place (unit innermost
-    stride, rows and base aligned to 16 bytes), else a contiguous copy."""
+    stride, rows and base aligned to 16 bytes, 64 rows within 2 GiB), else a
+    contiguous copy."""
     sb, sh, ss, sd = t.stride()
-    if (sd == 1 or t.shape[-1] == 1) and not (sb | sh | ss) & (16 // t.element_size() - 1) and not t.data_ptr() & 15:
+    size = t.element_size()
+    if sd == 1 and not (sb | sh | ss) & (16 // size - 1) and not t.data_ptr() & 15 and ss * 64 * size < 1 << 31:
         return t
     t = t.contiguous()
     return t.clone() if t.data_ptr() & 15 else t
