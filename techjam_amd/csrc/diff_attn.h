@@ -62,7 +62,7 @@ struct DiffArgs {
 constexpr int kPeakParts = 64;
 constexpr int kDiffThreads = 256;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr int kDiffBufferFlags = 0x00020000;  // raw buffer resource word 3 on gfx950
+constexpr uint32_t kDiffBufferFlags = 0x00020000;  // raw buffer resource word 3 on gfx950
 
 template <typename T>
 struct Elem;
@@ -186,7 +186,31 @@ struct LdsRows {
 // loads: what lies outside the resource, and columns at or past the width, land
 // as zeros. The copies are in flight until the wave has waited for them
 // (wait_copies) and the workgroup has met.
+//
+// The copy is an asm statement because the compiler, where it knows of one in
+// flight, waits for it before every transposing LDS read, whatever that reads.
+// It has no register results, so nothing can be reused too early, and loads the
+// compiler does not count only make its own waits stricter (they end in order).
+// The wait state between m0's write and its use is in the statement.
 constexpr uint32_t kOutside = 0x80000000u;
+typedef uint32_t rsrc_t __attribute__((ext_vector_type(4)));
+
+// Raw buffer resource of `bytes` bytes at p (the same in every lane).
+__device__ __forceinline__ rsrc_t make_rsrc(const void* p, uint32_t bytes) {
+  const uint64_t u = reinterpret_cast<uint64_t>(p);
+  return rsrc_t{(uint32_t)u, (uint32_t)(u >> 32) & 0xffffu, bytes, kDiffBufferFlags};
+}
+
+__device__ __forceinline__ uint32_t lds_offset(const void* p) {
+  return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)p;
+}
+
+__device__ __forceinline__ void copy_16(rsrc_t r, uint32_t lds, uint32_t voff) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
+               :
+               : "s"(lds), "v"(voff), "s"(r)
+               : "memory", "m0");
+}
 
 template <typename T, int W, int ROWS, int WAVES>
 struct TileCopy {
@@ -204,10 +228,9 @@ struct TileCopy {
     const int c = (lane % L::kChunks) ^ L::swizzle(row);
     return c * L::kVec < width ? (uint32_t)c * 16 : kOutside;
   }
-  __device__ __forceinline__ static void issue(__amdgpu_buffer_rsrc_t r, T* tile, int wave, int n, uint32_t voff) {
+  __device__ __forceinline__ static void issue(rsrc_t r, T* tile, int wave, int n, uint32_t voff) {
     if (kTotal < WAVES && wave >= kTotal) return;
-    __builtin_amdgcn_raw_ptr_buffer_load_lds(
-        r, (__attribute__((address_space(3))) void*)(reinterpret_cast<char*>(tile) + (wave * N + n) * 1024), 16, voff, 0, 0, 0);
+    copy_16(r, lds_offset(tile) + (wave * N + n) * 1024, voff);
   }
 };
 
@@ -228,14 +251,33 @@ struct KeyCopy : TileCopy<T, W, ROWS, WAVES> {
   // Rows 0 .. rows-1 from `p` on; further rows of the tile read as zeros.
   __device__ __forceinline__ void issue(const T* p, int64_t row_stride, int rows, int width, T* tile, int wave) const {
     const int64_t bytes = rows <= 0 ? 0 : ((int64_t)(min(rows, ROWS) - 1) * row_stride + width) * (int64_t)sizeof(T);
-    const auto r = __builtin_amdgcn_make_buffer_rsrc(const_cast<T*>(p), (short)0, (int)bytes, kDiffBufferFlags);
+    const rsrc_t r = make_rsrc(p, (uint32_t)bytes);
 #pragma unroll
     for (int n = 0; n < C::N; ++n) C::issue(r, tile, wave, n, voff[n]);
   }
 };
 
 // This wave's copies (and loads) and LDS accesses are done.
-__device__ __forceinline__ void wait_copies() { __builtin_amdgcn_s_waitcnt(0x0070); }
+__device__ __forceinline__ void wait_copies() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
+
+// x plus the sum of a fragment's values.
+__device__ __forceinline__ float frag_sum(half8_t f, float x) {
+#pragma unroll
+  for (int j = 0; j < 8; j += 2) x = __builtin_amdgcn_fdot2(half2_t{f[j], f[j + 1]}, half2_t{1, 1}, x, false);
+  return x;
+}
+__device__ __forceinline__ float frag_sum(bf16x8_t f, float x) {
+  typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+#pragma unroll
+  for (int j = 0; j < 8; j += 2)
+    x = __builtin_amdgcn_fdot2_f32_bf16(bf16x2_t{f[j], f[j + 1]}, bf16x2_t{(__bf16)1.f, (__bf16)1.f}, x, false);
+  return x;
+}
+__device__ __forceinline__ float frag_sum(float8_t f, float x) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) x += f[j];
+  return x;
+}
 
 // Eight consecutive elements of a row in memory, zeros at or past `width`.
 template <typename T>

@@ -18,16 +18,20 @@
 namespace tj {
 namespace {
 
-// WHAT: 1 dV, 2 dK, 3 both. fp32 heads past 64 dims do not have the registers
-// for both and form the scores twice.
+// WHAT: 1 dV, 2 dK, 3 both. Heads past 64 dims do not have the registers for
+// both and form the scores twice.
 template <typename T, int HD, int WHAT>
-__global__ __launch_bounds__(kDiffThreads, 1) void diff_bwd_kv_kernel(DiffArgs a) {
+__global__ __launch_bounds__(kDiffThreads, (sizeof(T) == 2 && (HD <= 64 || WHAT == 1) ? 2 : 1)) void diff_bwd_kv_kernel(DiffArgs a) {
   constexpr int DVP = 2 * HD, KS = HD / 16, VS = DVP / 16, KB = HD / 32, VB = DVP / 32, BM = 32;
   constexpr bool DO_DV = (WHAT & 1) != 0, DO_DK = (WHAT & 2) != 0;
   using QT = LdsRows<T, HD>;
   using OT = LdsRows<T, DVP>;
   constexpr int kTile = BM * (2 * HD + DVP);  // Q's two heads and dO
+  // V's rows of the workgroup's keys stay in LDS where their fragments would
+  // take a wave's registers past what two waves per SIMD have.
+  constexpr bool kVInLds = DO_DK && sizeof(T) == 2 && HD == 64;
   __shared__ __attribute__((aligned(1024))) T smem[2][kTile];
+  __shared__ __attribute__((aligned(1024))) T sv[kVInLds ? 128 * DVP : 8];
   // lse_0, lse_1 (with the lift), -delta_0 and lam delta_1 (lifted) of a tile's tokens
   __shared__ __attribute__((aligned(16))) float stat[2][4][BM];
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave, hl = lane / 32,
@@ -57,7 +61,7 @@ __global__ __launch_bounds__(kDiffThreads, 1) void diff_bwd_kv_kernel(DiffArgs a
     return tid < 128 && i < L ? sp[map_at(a, t.b, t.hk * a.G + g, (tid / BM) & 1, i)] : 0.f;
   };
 
-  frag_t<T> kf[2][KS], vf[DO_DK ? VS : 1];
+  frag_t<T> kf[2][KS], vf[DO_DK && !kVInLds ? VS : 1];
   {
     const T* kp = reinterpret_cast<const T*>(a.k) + a.vk.row(t.b, 2 * t.hk, live ? key : 0);
     const T* vp = reinterpret_cast<const T*>(a.v) + a.vv.row(t.b, t.hk, live ? key : 0);
@@ -65,7 +69,11 @@ __global__ __launch_bounds__(kDiffThreads, 1) void diff_bwd_kv_kernel(DiffArgs a
     for (int c = 0; c < 2; ++c)
 #pragma unroll
       for (int s = 0; s < KS; ++s) kf[c][s] = load_frag<T>(live ? kp + c * a.vk.sh : nullptr, 16 * s + 8 * hl, a.D);
-    if constexpr (DO_DK)
+    if constexpr (kVInLds) {
+      KeyCopy<T, DVP, 128, 4> vcopy;
+      vcopy.init(a.vv.ss, a.Dv, w, lane);
+      vcopy.issue(reinterpret_cast<const T*>(a.v) + a.vv.row(t.b, t.hk, k0), a.vv.ss, L - k0, a.Dv, sv, w);
+    } else if constexpr (DO_DK)
 #pragma unroll
       for (int s = 0; s < VS; ++s) vf[s] = load_frag<T>(live ? vp : nullptr, 16 * s + 8 * hl, a.Dv);
   }
@@ -145,7 +153,10 @@ __global__ __launch_bounds__(kDiffThreads, 1) void diff_bwd_kv_kernel(DiffArgs a
         if constexpr (DO_DK) {
           float16_t dp = zero16();
 #pragma unroll
-          for (int s = 0; s < VS; ++s) dp = Elem<T>::mma(OT::row_frag(so, ln, 16 * s + 8 * hl), vf[s], dp);
+          for (int s = 0; s < VS; ++s) {
+            const frag_t<T> v = kVInLds ? OT::row_frag(sv, 32 * w + ln, 16 * s + 8 * hl) : vf[kVInLds ? 0 : s];
+            dp = Elem<T>::mma(OT::row_frag(so, ln, 16 * s + 8 * hl), v, dp);
+          }
           const float nl = -lam * lift;
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
@@ -213,7 +224,7 @@ int diff_bwd_kv(const DiffArgs& args, int dtype, hipStream_t stream) {
     constexpr int HD = decltype(hd)::value;
     DiffArgs a = args;
     a.n_mtiles = (a.Sk + 127) / 128;
-    if constexpr (sizeof(T) == 4 && HD == 128) {
+    if constexpr (HD == 128) {
       const int rc = launch<T, HD, 1>(a, stream);
       return rc != TJ_OK ? rc : launch<T, HD, 2>(a, stream);
     } else {

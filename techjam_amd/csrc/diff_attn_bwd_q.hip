@@ -89,7 +89,7 @@ __global__ __launch_bounds__(kDiffThreads) void diff_delta_kernel(DiffArgs a, in
 // the forward kernel: a row's sums are its lane's own numbers, and dS turns into
 // the B operand of dQ^T = K^T dS^T.
 template <typename T, int HD>
-__global__ __launch_bounds__(kDiffThreads, 1) void diff_bwd_q_kernel(DiffArgs a) {
+__global__ __launch_bounds__(kDiffThreads, (sizeof(T) == 2 && HD <= 64 ? 2 : 1)) void diff_bwd_q_kernel(DiffArgs a) {
   constexpr int DVP = 2 * HD, KS = HD / 16, VS = DVP / 16, KB = HD / 32, BN = 32;
   using KT = LdsRows<T, HD>;
   using VT = LdsRows<T, DVP>;

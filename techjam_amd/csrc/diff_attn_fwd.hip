@@ -25,8 +25,6 @@ struct FwdShape {
   using KT = LdsRows<T, HD>;
   using VT = LdsRows<T, DVP>;
   static constexpr int KS = HD / 16;   // k-steps over the head dim
-  static constexpr int NKB = BN / 32;  // score blocks per tile
-  static constexpr int NS = BN / 16;   // k-steps over the tile's keys
   static constexpr int DB = DVP / 32;  // output blocks
   static constexpr int kElems = BN * (2 * HD + DVP);  // one tile of both key heads and of V
 };
@@ -54,26 +52,30 @@ struct DiffSpan {
   }
 };
 
-// The running state of a wave's 32 rows.
-template <typename T, int HD, int BN>
+// The running state of a wave's 32 rows, for NM maps from map `first` on: both,
+// or one where two accumulators of the width exceed a wave's registers (a pair
+// of waves then shares the rows and the key tiles).
+template <typename T, int HD, int BN, int NM>
 struct FwdState {
   using SH = FwdShape<T, HD, BN>;
-  frag_t<T> q[2][SH::KS];
-  float16_t o[2][SH::DB];
-  float m[2], l[2];  // maximum in log2 units, the lane's part of the sum
-  float c2;          // |scale| log2 e
+  frag_t<T> q[NM][SH::KS];
+  float16_t o[NM][SH::DB];
+  float m[NM], l[NM];  // maximum in log2 units, the lane's part of the sum
+  float c2;            // |scale| log2 e
+  int first;
 
-  __device__ __forceinline__ void init(const DiffArgs& a, int b, int hk, const DiffRow& row, int lane) {
+  __device__ __forceinline__ void init(const DiffArgs& a, int b, int hk, const DiffRow& row, int first_map, int lane) {
     const int hl = lane / 32;
+    first = first_map;
     const T* qp = reinterpret_cast<const T*>(a.q) + (row.live ? a.vq.row(b, 2 * (hk * a.G + row.g), row.i) : 0);
     // A negative scale turns q's sign, so that the largest score is the largest
     // product; a zero one becomes too small to matter, so that masked stays -inf.
     c2 = fmaxf(fabsf(a.scale) * kLog2e, 1e-37f);
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
+    for (int c = 0; c < NM; ++c) {
 #pragma unroll
       for (int ks = 0; ks < SH::KS; ++ks) {
-        q[c][ks] = load_frag<T>(row.live ? qp + c * a.vq.sh : nullptr, 16 * ks + 8 * hl, a.D);
+        q[c][ks] = load_frag<T>(row.live ? qp + (first + c) * a.vq.sh : nullptr, 16 * ks + 8 * hl, a.D);
         if (a.scale < 0.f)
 #pragma unroll
           for (int j = 0; j < 8; ++j) q[c][ks][j] = -q[c][ks][j];
@@ -85,33 +87,27 @@ struct FwdState {
     }
   }
 
-  // One key tile: keys kv0 + (0 .. BN-1), of which the row sees those <= limit.
-  __device__ __forceinline__ void tile(const T* kt, const T* vt, int kv0, int limit, bool masked, int lane) {
+  // 32 keys of a tile, kb 32 .. kb 32 + 31 of it, kv0 on in the sequence, of
+  // which the row sees those <= limit. Small steps: scores and probabilities of
+  // 64 keys at once exceed the registers of two waves per SIMD, and a reload
+  // waits for the copies in flight too.
+  __device__ __forceinline__ void step(const T* tile, int kb, int kv0, int limit, bool masked, int lane) {
     const int hl = lane / 32, ln = lane % 32;
-    frag_t<T> p[2][SH::NS];
+    frag_t<T> p[NM][2];
 #pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const T* kc = kt + c * SH::BN * HD;
-      float16_t s[SH::NKB];
+    for (int c = 0; c < NM; ++c) {
+      float16_t s = zero16();
 #pragma unroll
-      for (int kb = 0; kb < SH::NKB; ++kb) {
-        s[kb] = zero16();
-#pragma unroll
-        for (int ks = 0; ks < SH::KS; ++ks)
-          s[kb] = Elem<T>::mma(SH::KT::row_frag(kc, kb * 32 + ln, 16 * ks + 8 * hl), q[c][ks], s[kb]);
-      }
+      for (int ks = 0; ks < SH::KS; ++ks)
+        s = Elem<T>::mma(SH::KT::row_frag(tile + (first + c) * BN * HD, kb * 32 + ln, 16 * ks + 8 * hl), q[c][ks], s);
       if (masked) {
 #pragma unroll
-        for (int kb = 0; kb < SH::NKB; ++kb)
-#pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (kv0 + kb * 32 + acc_row(r, hl) > limit) s[kb][r] = -__builtin_inff();
+        for (int r = 0; r < 16; ++r)
+          if (kv0 + acc_row(r, hl) > limit) s[r] = -__builtin_inff();
       }
-      float top = s[0][0];
+      float top = s[0];
 #pragma unroll
-      for (int kb = 0; kb < SH::NKB; ++kb)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[kb][r]);
+      for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
       top = pair_max(top) * c2;
       // The maximum moves by the row's need; one decision for the wave.
       const bool move = top > m[c] + kLazy;  // also from -inf
@@ -127,86 +123,96 @@ struct FwdState {
       }
       // A row that has seen no key keeps its unset maximum out of the exponent.
       const float off = m[c] == -__builtin_inff() ? 0.f : Elem<T>::kLift - m[c];
-      float sum = 0.f;
 #pragma unroll
-      for (int kb = 0; kb < SH::NKB; ++kb) {
+      for (int r = 0; r < 16; ++r) s[r] = fast_exp2(fmaf(s[r], c2, off));
+      // The sum takes the rounded values, as the product does: a dominant key's
+      // rounding cancels, and two values go into one instruction.
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          s[kb][r] = fast_exp2(fmaf(s[kb][r], c2, off));
-          sum += s[kb][r];
-        }
-        p[c][2 * kb] = acc_frag<T>(s[kb], 0);
-        p[c][2 * kb + 1] = acc_frag<T>(s[kb], 1);
+      for (int st = 0; st < 2; ++st) {
+        p[c][st] = acc_frag<T>(s, st);
+        l[c] = frag_sum(p[c][st], l[c]);
       }
-      l[c] += sum;
     }
 #pragma unroll
-    for (int st = 0; st < SH::NS; ++st)
+    for (int st = 0; st < 2; ++st)
 #pragma unroll
       for (int d = 0; d < SH::DB; ++d) {
-        const frag_t<T> vf = SH::VT::col_frag(vt, 16 * st, 32 * d, lane);
+        const frag_t<T> vf = SH::VT::col_frag(tile + 2 * BN * HD, kb * 32 + 16 * st, 32 * d, lane);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) o[c][d] = Elem<T>::mma(vf, p[c][st], o[c][d]);
+        for (int c = 0; c < NM; ++c) o[c][d] = Elem<T>::mma(vf, p[c][st], o[c][d]);
       }
   }
 
-  // The rows' results, whole (part < 0) or those of a part of the keys.
-  __device__ __forceinline__ void finish(const DiffArgs& a, int b, int hk, const DiffRow& row, int part, int lane) {
+  // The results of a part of the keys.
+  __device__ __forceinline__ void finish_part(const DiffArgs& a, int bh, const DiffRow& row, int part, int lane) {
     const int hl = lane / 32;
-    const int bh = b * a.Hk + hk, head = hk * a.G + row.g;
-    if (part >= 0) {
-      const int64_t slot = ((int64_t)part * a.B * a.Hk + bh) * a.R + row.r;
+    const int64_t slot = ((int64_t)part * a.B * a.Hk + bh) * a.R + row.r;
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        const float sum = pair_sum(l[c]);
-        if (!row.live) continue;
-        float* po = a.part_o + (slot * 2 + c) * a.Dv;
+    for (int c = 0; c < NM; ++c) {
+      const float sum = pair_sum(l[c]);
+      if (!row.live) continue;
+      float* po = a.part_o + (slot * 2 + first + c) * a.Dv;
+#pragma unroll
+      for (int d = 0; d < SH::DB; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int col = 32 * d + 8 * e + 4 * hl;
+          if (col < a.Dv) store4t<float>(po + col, o[c][d][4 * e], o[c][d][4 * e + 1], o[c][d][4 * e + 2], o[c][d][4 * e + 3]);
+        }
+      if (hl == 0) {
+        a.part_ml[(slot * 2 + first + c) * 2] = m[c];
+        a.part_ml[(slot * 2 + first + c) * 2 + 1] = sum;
+      }
+    }
+  }
+
+  // The rows' results. With one map a wave, the second map's waves hand theirs
+  // to the first's through `swap` (64 lanes x DB x 16 floats a pair of waves).
+  __device__ __forceinline__ void finish(const DiffArgs& a, int b, int hk, const DiffRow& row, float4_t* swap, int lane) {
+    const int hl = lane / 32, head = hk * a.G + row.g;
+    const bool in = row.r < a.R;
+    float* mp = a.maps != nullptr && in ? a.maps + row_at(a, b, head, row.i) * 2 * a.Dv : nullptr;
+#pragma unroll
+    for (int c = 0; c < NM; ++c) {
+      const float sum = pair_sum(l[c]), inv = 1.f / sum;
+      if (a.lse != nullptr && in && hl == 0)
+        a.lse[map_at(a, b, head, first + c, row.i)] = row.live ? m[c] - Elem<T>::kLift + log2f(sum) : __builtin_inff();
+#pragma unroll
+      for (int d = 0; d < SH::DB; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int col = 32 * d + 8 * e + 4 * hl;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[c][d][4 * e + j] = row.live ? o[c][d][4 * e + j] * inv : 0.f;
+          if (mp != nullptr && col < a.Dv)
+            store4t<float>(mp + (first + c) * a.Dv + col, o[c][d][4 * e], o[c][d][4 * e + 1], o[c][d][4 * e + 2], o[c][d][4 * e + 3]);
+        }
+    }
+    if constexpr (NM == 1) {
+      __syncthreads();  // the key tiles, in whose place `swap` lies, have been read
+      if (first == 1)
 #pragma unroll
         for (int d = 0; d < SH::DB; ++d)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int col = 32 * d + 8 * e + 4 * hl;
-            if (col < a.Dv) store4t<float>(po + col, o[c][d][4 * e], o[c][d][4 * e + 1], o[c][d][4 * e + 2], o[c][d][4 * e + 3]);
-          }
-        if (hl == 0) {
-          a.part_ml[(slot * 2 + c) * 2] = m[c];
-          a.part_ml[(slot * 2 + c) * 2 + 1] = sum;
-        }
-      }
-      return;
+          for (int e = 0; e < 4; ++e)
+            swap[(d * 4 + e) * kWave + lane] = float4_t{o[0][d][4 * e], o[0][d][4 * e + 1], o[0][d][4 * e + 2], o[0][d][4 * e + 3]};
+      __syncthreads();
+      if (first == 1) return;
     }
-    float inv[2];
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      const float sum = pair_sum(l[c]);
-      inv[c] = 1.f / sum;
-      if (a.lse != nullptr && row.r < a.R && hl == 0)
-        a.lse[map_at(a, b, head, c, row.i)] =
-            row.live ? m[c] - Elem<T>::kLift + log2f(sum) : __builtin_inff();
-    }
-    if (row.r >= a.R) return;
+    if (!in) return;
     const float lam = a.lam[head * a.lam_step];
-    const int64_t at = a.vo.row(b, head, row.i);
-    T* op = reinterpret_cast<T*>(a.o) + at;
-    float* mp = a.maps + row_at(a, b, head, row.i) * 2 * a.Dv;
+    T* op = reinterpret_cast<T*>(a.o) + a.vo.row(b, head, row.i);
 #pragma unroll
     for (int d = 0; d < SH::DB; ++d)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int col = 32 * d + 8 * e + 4 * hl;
         if (col >= a.Dv) continue;
-        float4_t y = {0.f, 0.f, 0.f, 0.f}, z = y;
-        if (row.live)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            y[j] = o[0][d][4 * e + j] * inv[0];
-            z[j] = o[1][d][4 * e + j] * inv[1];
-          }
-        store4t<T>(op + col, fmaf(-lam, z[0], y[0]), fmaf(-lam, z[1], y[1]), fmaf(-lam, z[2], y[2]), fmaf(-lam, z[3], y[3]));
-        if (a.maps != nullptr) {
-          *reinterpret_cast<float4_t*>(mp + col) = y;
-          *reinterpret_cast<float4_t*>(mp + a.Dv + col) = z;
-        }
+        float4_t z;
+        if constexpr (NM == 1) z = swap[(d * 4 + e) * kWave + lane];
+        else z = float4_t{o[1][d][4 * e], o[1][d][4 * e + 1], o[1][d][4 * e + 2], o[1][d][4 * e + 3]};
+        store4t<T>(op + col, fmaf(-lam, z[0], o[0][d][4 * e]), fmaf(-lam, z[1], o[0][d][4 * e + 1]),
+                   fmaf(-lam, z[2], o[0][d][4 * e + 2]), fmaf(-lam, z[3], o[0][d][4 * e + 3]));
       }
   }
 };
@@ -232,44 +238,53 @@ struct KeyTiles {
   }
 };
 
+// Maps a wave computes: accumulators of both take 4 HD registers.
+template <int HD>
+constexpr int kMaps = HD <= 64 ? 2 : 1;
+
 template <typename T, int HD, bool PART>
-__global__ __launch_bounds__(kDiffThreads, (sizeof(T) == 2 && HD <= 64 ? 2 : 1)) void diff_fwd_kernel(DiffArgs a) {
-  constexpr int BN = sizeof(T) == 4 ? 32 : 64;
+__global__ __launch_bounds__(512 / kMaps<HD>, (sizeof(T) == 4 && HD == 64 ? 1 : 2)) void diff_fwd_kernel(DiffArgs a) {
+  constexpr int BN = sizeof(T) == 4 ? 32 : 64, NM = kMaps<HD>;
   using SH = FwdShape<T, HD, BN>;
   __shared__ __attribute__((aligned(1024))) T smem[2][SH::kElems];
-  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
+  static_assert(NM == 2 || sizeof(smem) >= 4 * 64 * SH::DB * 64, "room for the second map's results");
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave, rw = w % 4;
   const DiffTile t = diff_tile(a, blockIdx.x, a.n_mtiles);
   const int part = PART ? t.tile / a.n_mtiles : -1;
   const int mt = a.n_mtiles - 1 - (PART ? t.tile % a.n_mtiles : t.tile);
   const int L = diff_len(a, t.b);
-  const DiffSpan all(a, mt * 128, mt * 128 + 127, L), own(a, mt * 128 + 32 * w, mt * 128 + 32 * w + 31, L);
-  const DiffRow row(a, mt * 128 + 32 * w + lane % 32, L);
+  const DiffSpan all(a, mt * 128, mt * 128 + 127, L), own(a, mt * 128 + 32 * rw, mt * 128 + 32 * rw + 31, L);
+  const DiffRow row(a, mt * 128 + 32 * rw + lane % 32, L);
   const int kv_begin = PART ? part * a.part_keys : 0;
   const int kv_end = PART ? min(all.end, kv_begin + a.part_keys) : all.end;
   if (PART && kv_begin >= kv_end) return;  // not read either (live parts are counted from the rows' last key)
-  KeyTiles<T, SH, HD, 4> keys;
+  KeyTiles<T, SH, HD, 8 / NM> keys;
   keys.init(a, t.b, t.hk, w, lane);
   if (kv_begin < kv_end) keys.issue(a, kv_begin, L, smem[0], w);
-  FwdState<T, HD, BN> st;
-  st.init(a, t.b, t.hk, row, lane);
+  FwdState<T, HD, BN, NM> st;
+  st.init(a, t.b, t.hk, row, w / 4, lane);
   int cur = 0;
   for (int kv0 = kv_begin; kv0 < kv_end; kv0 += BN, cur ^= 1) {
     // The tile is there, and the other one has been read by every wave.
     wait_copies();
     lds_barrier();
     if (kv0 + BN < kv_end) keys.issue(a, kv0 + BN, L, smem[cur ^ 1], w);
-    if (kv0 < own.end)
-      st.tile(smem[cur], smem[cur] + 2 * BN * HD, kv0, row.limit, kv0 + BN - 1 > own.free, lane);
+#pragma unroll
+    for (int kb = 0; kb < BN / 32; ++kb) {
+      const int k0 = kv0 + 32 * kb;
+      if (k0 < own.end) st.step(smem[cur], kb, k0, row.limit, k0 + 31 > own.free, lane);
+    }
   }
-  st.finish(a, t.b, t.hk, row, part, lane);
+  if constexpr (PART) st.finish_part(a, t.bh, row, part, lane);
+  else st.finish(a, t.b, t.hk, row, reinterpret_cast<float4_t*>(smem) + rw * SH::DB * 4 * kWave, lane);
 }
 
 template <typename T, int HD>
-__global__ __launch_bounds__(kWave) void diff_few_kernel(DiffArgs a) {
-  constexpr int BN = 32;
+__global__ __launch_bounds__(2 * kWave / kMaps<HD>) void diff_few_kernel(DiffArgs a) {
+  constexpr int BN = 32, NM = kMaps<HD>;
   using SH = FwdShape<T, HD, BN>;
   __shared__ __attribute__((aligned(1024))) T smem[2][SH::kElems];
-  const int lane = threadIdx.x;
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
   const DiffTile t = diff_tile(a, blockIdx.x, a.n_mtiles * a.n_parts);
   const int mt = t.tile % a.n_mtiles, part = t.tile / a.n_mtiles;
   const int L = diff_len(a, t.b);
@@ -277,19 +292,19 @@ __global__ __launch_bounds__(kWave) void diff_few_kernel(DiffArgs a) {
   const DiffRow row(a, mt * 32 + lane % 32, L);
   const int kv_begin = part * a.part_keys, kv_end = min(own.end, kv_begin + a.part_keys);
   if (kv_begin >= kv_end) return;
-  KeyTiles<T, SH, HD, 1> keys;
-  keys.init(a, t.b, t.hk, 0, lane);
-  keys.issue(a, kv_begin, L, smem[0], 0);
-  FwdState<T, HD, BN> st;
-  st.init(a, t.b, t.hk, row, lane);
+  KeyTiles<T, SH, HD, 2 / NM> keys;
+  keys.init(a, t.b, t.hk, w, lane);
+  keys.issue(a, kv_begin, L, smem[0], w);
+  FwdState<T, HD, BN, NM> st;
+  st.init(a, t.b, t.hk, row, w, lane);
   int cur = 0;
   for (int kv0 = kv_begin; kv0 < kv_end; kv0 += BN, cur ^= 1) {
     wait_copies();
     lds_barrier();
-    if (kv0 + BN < kv_end) keys.issue(a, kv0 + BN, L, smem[cur ^ 1], 0);
-    st.tile(smem[cur], smem[cur] + 2 * BN * HD, kv0, row.limit, kv0 + BN - 1 > own.free, lane);
+    if (kv0 + BN < kv_end) keys.issue(a, kv0 + BN, L, smem[cur ^ 1], w);
+    st.step(smem[cur], 0, kv0, row.limit, kv0 + BN - 1 > own.free, lane);
   }
-  st.finish(a, t.b, t.hk, row, part, lane);
+  st.finish_part(a, t.bh, row, part, lane);
 }
 
 // Joins the parts: O_m = sum_p 2^(max_p - M) o_p / sum_p 2^(max_p - M) sum_p,
@@ -356,11 +371,11 @@ int diff_fwd(const DiffArgs& args, int dtype, hipStream_t stream) {
     a.n_mtiles = (a.R + 127) / 128;
     const int64_t n = (int64_t)a.B * a.Hk * a.n_mtiles;
     if (a.n_parts > 1) {
-      hipLaunchKernelGGL((diff_fwd_kernel<T, HD, true>), dim3(uint32_t(n * a.n_parts)), dim3(kDiffThreads), 0, stream, a);
+      hipLaunchKernelGGL((diff_fwd_kernel<T, HD, true>), dim3(uint32_t(n * a.n_parts)), dim3(512 / kMaps<HD>), 0, stream, a);
       const int rc = tjh::launch_status();
       return rc != TJ_OK ? rc : launch_join<T>(a, stream);
     }
-    hipLaunchKernelGGL((diff_fwd_kernel<T, HD, false>), dim3(uint32_t(n)), dim3(kDiffThreads), 0, stream, a);
+    hipLaunchKernelGGL((diff_fwd_kernel<T, HD, false>), dim3(uint32_t(n)), dim3(512 / kMaps<HD>), 0, stream, a);
     return tjh::launch_status();
   });
 }
@@ -368,10 +383,11 @@ int diff_fwd(const DiffArgs& args, int dtype, hipStream_t stream) {
 int diff_few_rows(const DiffArgs& args, int dtype, hipStream_t stream) {
   return diff_dispatch(args, dtype, [&](auto t, auto hd) {
     using T = decltype(t);
+    constexpr int HD = decltype(hd)::value;
     DiffArgs a = args;
     a.n_mtiles = (a.R + 31) / 32;
-    hipLaunchKernelGGL((diff_few_kernel<T, decltype(hd)::value>),
-                       dim3(uint32_t((int64_t)a.B * a.Hk * a.n_mtiles * a.n_parts)), dim3(kWave), 0, stream, a);
+    hipLaunchKernelGGL((diff_few_kernel<T, HD>), dim3(uint32_t((int64_t)a.B * a.Hk * a.n_mtiles * a.n_parts)),
+                       dim3(2 * kWave / kMaps<HD>), 0, stream, a);
     const int rc = tjh::launch_status();
     return rc != TJ_OK ? rc : launch_join<T>(a, stream);
   });
