@@ -125,10 +125,18 @@ __device__ __forceinline__ frag_t<T> acc_frag(const float16_t& c, int s) {
   return f;
 }
 
+__device__ __forceinline__ uint32_t lds_offset(const void* p) {
+  return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)p;
+}
+template <typename V>
+__device__ __forceinline__ V lds_at(uint32_t at) {
+  return *(const __attribute__((address_space(3))) V*)(uintptr_t)at;
+}
+
 // An LDS tile of rows of W elements without padding. The 16-byte chunk c of a
-// row stands at position c ^ swizzle(row), so that both readers below touch
-// every bank as often as they must and no more: eight lanes taking one chunk of
-// eight rows, and sixteen lanes taking two chunks of four rows.
+// row stands at position c ^ swizzle(row), so that what both readers below take
+// at a time covers the 64 banks (256 bytes) once: sixteen lanes one chunk of
+// sixteen rows, and thirty-two lanes four chunks of four rows.
 template <typename T, int W>
 struct LdsRows {
   static constexpr int kVec = 16 / (int)sizeof(T);
@@ -136,45 +144,60 @@ struct LdsRows {
   static constexpr int kRowBytes = W * (int)sizeof(T);
 
   __device__ __forceinline__ static int swizzle(int row) {
-    if constexpr (kChunks == 4) return (row >> 1) & 3;
-    else if constexpr (kChunks == 8) return row & 7;
-    else return (2 * row) & 14;
-  }
-  __device__ __forceinline__ static const char* at(const T* t, int row, int chunk) {
-    return reinterpret_cast<const char*>(t) + row * kRowBytes + ((chunk ^ swizzle(row)) << 4);
+    if constexpr (kChunks == 4) return (row >> 2) & 3;
+    else if constexpr (kChunks == 8) return ((row & 2) << 1) | ((row >> 2) & 3);
+    else return ((row & 3) << 2) | ((row >> 2) & 3);
   }
 
-  // The fragment of eight consecutive elements (k a multiple of 8) of one row.
-  __device__ __forceinline__ static frag_t<T> row_frag(const T* t, int row, int k) {
+  // Lane addresses in a tile. A fragment's place is the lane's address with some
+  // bits turned (the tile's offset is a multiple of 1024) plus a constant: one
+  // register a tile, and one instruction a fragment.
+  __device__ __forceinline__ static uint32_t lane_row(int lane) {
+    const int row = lane % 32, chunk = (sizeof(T) == 4 ? 2 : 1) * (lane / 32);
+    return row * kRowBytes + ((chunk ^ swizzle(row)) << 4);
+  }
+  __device__ __forceinline__ static uint32_t lane_col(int lane) {
+    const int hl = lane / 32;
     if constexpr (sizeof(T) == 4) {
-      const float4_t a = *reinterpret_cast<const float4_t*>(at(t, row, k / 4));
-      const float4_t b = *reinterpret_cast<const float4_t*>(at(t, row, k / 4 + 1));
-      return frag_t<T>{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+      const int row = 4 * hl, col = lane % 32;
+      return row * kRowBytes + (((col / 4) ^ swizzle(row)) << 4) + 4 * (col % 4);
     } else {
-      return *reinterpret_cast<const frag_t<T>*>(at(t, row, k / 8));
+      const int row = 4 * hl + (lane & 15) / 4, chunk = (lane & 16) / 8 + (lane & 3) / 2;
+      return row * kRowBytes + ((chunk ^ swizzle(row)) << 4) + 8 * (lane & 1);
     }
   }
 
-  // The fragment that contracts rows row0 .. row0+15 in acc_frag's order, for
-  // column col0 + lane % 32. 16-bit elements come through the transposing LDS
-  // read: sixteen lanes name 4 rows x 16 columns, lane j of them gets column j.
-  __device__ __forceinline__ static frag_t<T> col_frag(const T* t, int row0, int col0, int lane) {
-    const int hl = lane / 32;
+  // Elements 16 ks + 8 (lane / 32) .. + 7 of row (lane % 32); base: tile +
+  // lane_row, offset: rows further on.
+  __device__ __forceinline__ static frag_t<T> row_frag(uint32_t base, int ks, int offset) {
+    if constexpr (sizeof(T) == 4) {
+      const float4_t a = lds_at<float4_t>((base ^ (ks << 6)) + offset);
+      const float4_t b = lds_at<float4_t>((base ^ (ks << 6 | 16)) + offset);
+      return frag_t<T>{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+    } else {
+      return lds_at<frag_t<T>>((base ^ (ks << 5)) + offset);
+    }
+  }
+
+  // The fragment that contracts 16 rows in acc_frag's order, for column 32 d +
+  // lane % 32; base: tile + lane_col, offset: where the rows start. 16-bit
+  // elements come through the transposing LDS read: sixteen lanes name 4 rows x
+  // 16 columns, lane j of them gets column j.
+  __device__ __forceinline__ static frag_t<T> col_frag(uint32_t base, int d, int offset) {
     if constexpr (sizeof(T) == 4) {
       frag_t<T> f;
-      const int col = col0 + lane % 32;
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        f[j] = *reinterpret_cast<const float*>(at(t, row0 + 4 * hl + j / 4 * 8 + j % 4, col / 4) + 4 * (col % 4));
+      for (int j = 0; j < 8; ++j) {
+        const int row = j / 4 * 8 + j % 4;  // beyond the lane's first
+        f[j] = lds_at<float>((base ^ (d << 7) ^ (swizzle(row) << 4)) + offset + row * kRowBytes);
+      }
       return f;
     } else {
       typedef short short4_t __attribute__((ext_vector_type(4)));
       typedef __attribute__((address_space(3))) short4_t lds_short4;
-      const int row = row0 + 4 * hl + (lane & 15) / 4;
-      const char* p = at(t, row, col0 / 8 + (lane & 16) / 8 + (lane & 3) / 2) + 8 * (lane & 1);
-      // Eight rows on, the swizzle is the same.
-      const short4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)p);
-      const short4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(p + 8 * kRowBytes));
+      const short4_t a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_short4*)(uintptr_t)((base ^ (d << 6)) + offset));
+      const short4_t b = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+          (lds_short4*)(uintptr_t)((base ^ (d << 6) ^ (swizzle(8) << 4)) + offset + 8 * kRowBytes));
       return __builtin_bit_cast(frag_t<T>, __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7));
     }
   }
@@ -201,10 +224,6 @@ __device__ __forceinline__ rsrc_t make_rsrc(const void* p, uint32_t bytes) {
   return rsrc_t{(uint32_t)u, (uint32_t)(u >> 32) & 0xffffu, bytes, kDiffBufferFlags};
 }
 
-__device__ __forceinline__ uint32_t lds_offset(const void* p) {
-  return (uint32_t)(uintptr_t)(const __attribute__((address_space(3))) char*)p;
-}
-
 __device__ __forceinline__ void copy_16(rsrc_t r, uint32_t lds, uint32_t voff) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds"
                :
@@ -228,9 +247,9 @@ struct TileCopy {
     const int c = (lane % L::kChunks) ^ L::swizzle(row);
     return c * L::kVec < width ? (uint32_t)c * 16 : kOutside;
   }
-  __device__ __forceinline__ static void issue(rsrc_t r, T* tile, int wave, int n, uint32_t voff) {
+  __device__ __forceinline__ static void issue(rsrc_t r, uint32_t tile, int wave, int n, uint32_t voff) {
     if (kTotal < WAVES && wave >= kTotal) return;
-    copy_16(r, lds_offset(tile) + (wave * N + n) * 1024, voff);
+    copy_16(r, tile + (wave * N + n) * 1024, voff);
   }
 };
 
@@ -248,8 +267,8 @@ struct KeyCopy : TileCopy<T, W, ROWS, WAVES> {
       voff[n] = c == kOutside ? kOutside : (uint32_t)r * (uint32_t)(row_stride * (int64_t)sizeof(T)) + c;
     }
   }
-  // Rows 0 .. rows-1 from `p` on; further rows of the tile read as zeros.
-  __device__ __forceinline__ void issue(const T* p, int64_t row_stride, int rows, int width, T* tile, int wave) const {
+  // Rows 0 .. rows-1 from `p` on to LDS offset `tile`; further rows of the tile read as zeros.
+  __device__ __forceinline__ void issue(const T* p, int64_t row_stride, int rows, int width, uint32_t tile, int wave) const {
     const int64_t bytes = rows <= 0 ? 0 : ((int64_t)(min(rows, ROWS) - 1) * row_stride + width) * (int64_t)sizeof(T);
     const rsrc_t r = make_rsrc(p, (uint32_t)bytes);
 #pragma unroll

@@ -94,6 +94,7 @@ __global__ __launch_bounds__(kDiffThreads, (sizeof(T) == 2 && HD <= 64 ? 2 : 1))
   using KT = LdsRows<T, HD>;
   using VT = LdsRows<T, DVP>;
   constexpr int kTile = BN * (2 * HD + DVP);  // K's two heads and V
+  constexpr int kBytes = kTile * (int)sizeof(T), kHead = BN * HD * (int)sizeof(T);
   __shared__ __attribute__((aligned(1024))) T smem[2][kTile];
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave, hl = lane / 32, ln = lane % 32;
   const DiffTile t = diff_tile(a, blockIdx.x, a.n_mtiles);
@@ -141,29 +142,31 @@ __global__ __launch_bounds__(kDiffThreads, (sizeof(T) == 2 && HD <= 64 ? 2 : 1))
   KeyCopy<T, DVP, BN, 4> vcopy;
   kcopy.init(a.vk.ss, a.D, w, lane);
   vcopy.init(a.vv.ss, a.Dv, w, lane);
-  auto issue = [&](int kv0, T* tile) {
+  const uint32_t tiles = lds_offset(smem);
+  const uint32_t krow = KT::lane_row(lane), kcol = KT::lane_col(lane), vrow = VT::lane_row(lane) + 2 * kHead;
+  auto issue = [&](int kv0, uint32_t tile) {
 #pragma unroll
     for (int c = 0; c < 2; ++c)
-      kcopy.issue(kp + c * a.vk.sh + kv0 * a.vk.ss, a.vk.ss, L - kv0, a.D, tile + c * BN * HD, w);
-    vcopy.issue(vp + kv0 * a.vv.ss, a.vv.ss, L - kv0, a.Dv, tile + 2 * BN * HD, w);
+      kcopy.issue(kp + c * a.vk.sh + kv0 * a.vk.ss, a.vk.ss, L - kv0, a.D, tile + c * kHead, w);
+    vcopy.issue(vp + kv0 * a.vv.ss, a.vv.ss, L - kv0, a.Dv, tile + 2 * kHead, w);
   };
-  if (kv_end > 0) issue(0, smem[0]);
+  if (kv_end > 0) issue(0, tiles);
   int cur = 0;
   for (int kv0 = 0; kv0 < kv_end; kv0 += BN, cur ^= 1) {
     wait_copies();
     lds_barrier();
-    if (kv0 + BN < kv_end) issue(kv0 + BN, smem[cur ^ 1]);
+    if (kv0 + BN < kv_end) issue(kv0 + BN, tiles + (cur ^ 1) * kBytes);
     if (kv0 >= own_end) continue;
-    const T *sk[2] = {smem[cur], smem[cur] + BN * HD}, *sv = smem[cur] + 2 * BN * HD;
+    const uint32_t tile = tiles + cur * kBytes;
     float16_t p[2], dp = zero16();
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       p[c] = zero16();
 #pragma unroll
-      for (int s = 0; s < KS; ++s) p[c] = Elem<T>::mma(KT::row_frag(sk[c], ln, 16 * s + 8 * hl), qf[c][s], p[c]);
+      for (int s = 0; s < KS; ++s) p[c] = Elem<T>::mma(KT::row_frag(tile + krow, s, c * kHead), qf[c][s], p[c]);
     }
 #pragma unroll
-    for (int s = 0; s < VS; ++s) dp = Elem<T>::mma(VT::row_frag(sv, ln, 16 * s + 8 * hl), of[s], dp);
+    for (int s = 0; s < VS; ++s) dp = Elem<T>::mma(VT::row_frag(tile + vrow, s, 0), of[s], dp);
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
 #pragma unroll
@@ -187,7 +190,7 @@ __global__ __launch_bounds__(kDiffThreads, (sizeof(T) == 2 && HD <= 64 ? 2 : 1))
       for (int s = 0; s < 2; ++s) {
         const frag_t<T> f = acc_frag<T>(p[c], s);
 #pragma unroll
-        for (int d = 0; d < KB; ++d) dq[c][d] = Elem<T>::mma(KT::col_frag(sk[c], 16 * s, 32 * d, lane), f, dq[c][d]);
+        for (int d = 0; d < KB; ++d) dq[c][d] = Elem<T>::mma(KT::col_frag(tile + kcol, d, c * kHead + 16 * s * KT::kRowBytes), f, dq[c][d]);
       }
   }
 

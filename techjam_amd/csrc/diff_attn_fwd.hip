@@ -27,6 +27,7 @@ struct FwdShape {
   static constexpr int KS = HD / 16;   // k-steps over the head dim
   static constexpr int DB = DVP / 32;  // output blocks
   static constexpr int kElems = BN * (2 * HD + DVP);  // one tile of both key heads and of V
+  static constexpr int kBytes = kElems * (int)sizeof(T), kHead = BN * HD * (int)sizeof(T);
 };
 
 // A lane's row: r of the (b, key head), its token, head and position, and the last key it sees.
@@ -63,10 +64,13 @@ struct FwdState {
   float m[NM], l[NM];  // maximum in log2 units, the lane's part of the sum
   float c2;            // |scale| log2 e
   int first;
+  uint32_t kbase, vbase;  // the lane's places in a key tile
 
   __device__ __forceinline__ void init(const DiffArgs& a, int b, int hk, const DiffRow& row, int first_map, int lane) {
     const int hl = lane / 32;
     first = first_map;
+    kbase = SH::KT::lane_row(lane) + first * SH::kHead;
+    vbase = SH::VT::lane_col(lane) + 2 * SH::kHead;
     const T* qp = reinterpret_cast<const T*>(a.q) + (row.live ? a.vq.row(b, 2 * (hk * a.G + row.g), row.i) : 0);
     // A negative scale turns q's sign, so that the largest score is the largest
     // product; a zero one becomes too small to matter, so that masked stays -inf.
@@ -91,15 +95,16 @@ struct FwdState {
   // which the row sees those <= limit. Small steps: scores and probabilities of
   // 64 keys at once exceed the registers of two waves per SIMD, and a reload
   // waits for the copies in flight too.
-  __device__ __forceinline__ void step(const T* tile, int kb, int kv0, int limit, bool masked, int lane) {
-    const int hl = lane / 32, ln = lane % 32;
+  __device__ __forceinline__ void step(uint32_t tile, int kb, int kv0, int limit, bool masked, int lane) {
+    const int hl = lane / 32;
+    const uint32_t kt = tile + kbase, vt = tile + vbase;
     frag_t<T> p[NM][2];
 #pragma unroll
     for (int c = 0; c < NM; ++c) {
       float16_t s = zero16();
 #pragma unroll
       for (int ks = 0; ks < SH::KS; ++ks)
-        s = Elem<T>::mma(SH::KT::row_frag(tile + (first + c) * BN * HD, kb * 32 + ln, 16 * ks + 8 * hl), q[c][ks], s);
+        s = Elem<T>::mma(SH::KT::row_frag(kt, ks, c * SH::kHead + kb * 32 * SH::KT::kRowBytes), q[c][ks], s);
       if (masked) {
 #pragma unroll
         for (int r = 0; r < 16; ++r)
@@ -137,7 +142,7 @@ struct FwdState {
     for (int st = 0; st < 2; ++st)
 #pragma unroll
       for (int d = 0; d < SH::DB; ++d) {
-        const frag_t<T> vf = SH::VT::col_frag(tile + 2 * BN * HD, kb * 32 + 16 * st, 32 * d, lane);
+        const frag_t<T> vf = SH::VT::col_frag(vt, d, (kb * 32 + 16 * st) * SH::VT::kRowBytes);
 #pragma unroll
         for (int c = 0; c < NM; ++c) o[c][d] = Elem<T>::mma(vf, p[c][st], o[c][d]);
       }
@@ -230,11 +235,11 @@ struct KeyTiles {
     v.init(a.vv.ss, a.Dv, wave, lane);
   }
   // Keys kv0 .. kv0 + BN - 1; those at or past L land as zeros, whatever is there.
-  __device__ __forceinline__ void issue(const DiffArgs& a, int kv0, int L, T* tile, int wave) const {
+  __device__ __forceinline__ void issue(const DiffArgs& a, int kv0, int L, uint32_t tile, int wave) const {
 #pragma unroll
     for (int c = 0; c < 2; ++c)
-      k.issue(kp + c * a.vk.sh + kv0 * a.vk.ss, a.vk.ss, L - kv0, a.D, tile + c * SH::BN * HD, wave);
-    v.issue(vp + kv0 * a.vv.ss, a.vv.ss, L - kv0, a.Dv, tile + 2 * SH::BN * HD, wave);
+      k.issue(kp + c * a.vk.sh + kv0 * a.vk.ss, a.vk.ss, L - kv0, a.D, tile + c * SH::kHead, wave);
+    v.issue(vp + kv0 * a.vv.ss, a.vv.ss, L - kv0, a.Dv, tile + 2 * SH::kHead, wave);
   }
 };
 
@@ -258,9 +263,10 @@ __global__ __launch_bounds__(512 / kMaps<HD>, (sizeof(T) == 4 && HD == 64 ? 1 : 
   const int kv_begin = PART ? part * a.part_keys : 0;
   const int kv_end = PART ? min(all.end, kv_begin + a.part_keys) : all.end;
   if (PART && kv_begin >= kv_end) return;  // not read either (live parts are counted from the rows' last key)
+  const uint32_t tiles = lds_offset(smem);
   KeyTiles<T, SH, HD, 8 / NM> keys;
   keys.init(a, t.b, t.hk, w, lane);
-  if (kv_begin < kv_end) keys.issue(a, kv_begin, L, smem[0], w);
+  if (kv_begin < kv_end) keys.issue(a, kv_begin, L, tiles, w);
   FwdState<T, HD, BN, NM> st;
   st.init(a, t.b, t.hk, row, w / 4, lane);
   int cur = 0;
@@ -268,11 +274,11 @@ __global__ __launch_bounds__(512 / kMaps<HD>, (sizeof(T) == 4 && HD == 64 ? 1 : 
     // The tile is there, and the other one has been read by every wave.
     wait_copies();
     lds_barrier();
-    if (kv0 + BN < kv_end) keys.issue(a, kv0 + BN, L, smem[cur ^ 1], w);
+    if (kv0 + BN < kv_end) keys.issue(a, kv0 + BN, L, tiles + (cur ^ 1) * SH::kBytes, w);
 #pragma unroll
     for (int kb = 0; kb < BN / 32; ++kb) {
       const int k0 = kv0 + 32 * kb;
-      if (k0 < own.end) st.step(smem[cur], kb, k0, row.limit, k0 + 31 > own.free, lane);
+      if (k0 < own.end) st.step(tiles + cur * SH::kBytes, kb, k0, row.limit, k0 + 31 > own.free, lane);
     }
   }
   if constexpr (PART) st.finish_part(a, t.bh, row, part, lane);
@@ -292,17 +298,18 @@ __global__ __launch_bounds__(2 * kWave / kMaps<HD>) void diff_few_kernel(DiffArg
   const DiffRow row(a, mt * 32 + lane % 32, L);
   const int kv_begin = part * a.part_keys, kv_end = min(own.end, kv_begin + a.part_keys);
   if (kv_begin >= kv_end) return;
+  const uint32_t tiles = lds_offset(smem);
   KeyTiles<T, SH, HD, 2 / NM> keys;
   keys.init(a, t.b, t.hk, w, lane);
-  keys.issue(a, kv_begin, L, smem[0], w);
+  keys.issue(a, kv_begin, L, tiles, w);
   FwdState<T, HD, BN, NM> st;
   st.init(a, t.b, t.hk, row, w, lane);
   int cur = 0;
   for (int kv0 = kv_begin; kv0 < kv_end; kv0 += BN, cur ^= 1) {
     wait_copies();
     lds_barrier();
-    if (kv0 + BN < kv_end) keys.issue(a, kv0 + BN, L, smem[cur ^ 1], w);
-    st.step(smem[cur], 0, kv0, row.limit, kv0 + BN - 1 > own.free, lane);
+    if (kv0 + BN < kv_end) keys.issue(a, kv0 + BN, L, tiles + (cur ^ 1) * SH::kBytes, w);
+    st.step(tiles + cur * SH::kBytes, 0, kv0, row.limit, kv0 + BN - 1 > own.free, lane);
   }
   st.finish_part(a, t.bh, row, part, lane);
 }
