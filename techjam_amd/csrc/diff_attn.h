@@ -400,6 +400,9 @@ __device__ __forceinline__ DiffTile diff_tile(const DiffArgs& a, int id, int til
   return t;
 }
 
+// Whether there are 128-row tiles enough for workgroups to take them rather than 64-row ones.
+inline bool wide_tiles(const DiffArgs& a) { return (int64_t)a.B * a.Hk * ((a.R + 127) / 128) >= 1024; }
+
 int diff_fwd(const DiffArgs& a, int dtype, hipStream_t stream);
 int diff_few_rows(const DiffArgs& a, int dtype, hipStream_t stream);
 int diff_bwd_kv(const DiffArgs& a, int dtype, hipStream_t stream);

@@ -71,8 +71,15 @@ __global__ __launch_bounds__((64 * KvShape<T, HD, WHAT>::WAVES), (KvShape<T, HD,
   // Tile n: head n / tiles of the group, tokens i_begin + 32 (n % tiles) on.
   const int i_begin = a.causal ? k0 : 0;
   const int tiles = k0 < L ? (L - i_begin + BM - 1) / BM : 0, n_end = tiles * a.G;
-  auto issue = [&](int n, uint32_t tile) {
-    const int g = n / tiles, i0 = i_begin + BM * (n % tiles);
+  // `n` tiles further on: the head and the token (no division in the loop).
+  auto advance = [&](int& g, int& i0, int n) {
+    i0 += BM * n;
+    while (i0 >= i_begin + BM * tiles) {
+      i0 -= BM * tiles;
+      ++g;
+    }
+  };
+  auto issue = [&](int g, int i0, uint32_t tile) {
 #pragma unroll
     for (int c = 0; c < 2; ++c)
       qcopy.issue(qp + (2 * g + c) * a.vq.sh + i0 * a.vq.ss, a.vq.ss, L - i0, a.D, tile + c * SH::kHead, kb);
@@ -81,9 +88,8 @@ __global__ __launch_bounds__((64 * KvShape<T, HD, WHAT>::WAVES), (KvShape<T, HD,
   // Every lane carries two of a token's four numbers: lse_0 and delta_0 in the
   // lower half of the wave, lse_1 and delta_1 in the upper one.
   float next[2] = {0.f, 0.f};
-  auto load_stat = [&](int n) {
-    const int g = n / tiles, i = i_begin + BM * (n % tiles) + ln;
-    const int64_t at = map_at(a, t.b, t.hk * a.G + g, hl, min(i, L - 1));
+  auto load_stat = [&](int g, int i0) {
+    const int64_t at = map_at(a, t.b, t.hk * a.G + g, hl, min(i0 + ln, L - 1));
     next[0] = a.lse[at];
     next[1] = a.delta[at];
   };
@@ -124,16 +130,17 @@ __global__ __launch_bounds__((64 * KvShape<T, HD, WHAT>::WAVES), (KvShape<T, HD,
   const float pl = p_lift<T>(lam_max), dl = ds_lift<T>(a, t.bh, t.hk, lane), log_pl = log2f(pl);
   const float lift = dl / pl;
   const float c2 = a.scale * kLog2e;
+  int g = 0, i0 = i_begin;  // this round's tile
   if (rg < n_end) {
-    issue(rg, group);
-    load_stat(rg);
+    advance(g, i0, rg);
+    issue(g, i0, group);
+    load_stat(g, i0);
   }
   // The workgroup goes round together, the last round maybe without a tile for every group.
   const int rounds = (n_end + RG - 1) / RG;
   for (int round = 0, n = rg, cur = 0; round < rounds; ++round, n += RG, cur ^= 1) {
     const bool on = n < n_end;
-    const int g = on ? n / tiles : 0, i0 = on ? i_begin + BM * (n % tiles) : 0;
-    const float lam = a.lam[(t.hk * a.G + g) * a.lam_step];
+    const float lam = on ? a.lam[(t.hk * a.G + g) * a.lam_step] : 0.f;
     wait_copies();
     if (on && kb == 0) {
       // A token that is not there weighs nothing: P = 2^(0 - inf).
@@ -155,9 +162,11 @@ __global__ __launch_bounds__((64 * KvShape<T, HD, WHAT>::WAVES), (KvShape<T, HD,
       }
     }
     // Only now: a spilled K fragment, read again above, would wait for the copies.
+    int g1 = g, i1 = i0;
     if (n + RG < n_end) {
-      issue(n + RG, group + (cur ^ 1) * SH::kBytes);
-      load_stat(n + RG);
+      advance(g1, i1, RG);
+      issue(g1, i1, group + (cur ^ 1) * SH::kBytes);
+      load_stat(g1, i1);
     }
     if (busy) {
 #pragma unroll
@@ -215,6 +224,8 @@ __global__ __launch_bounds__((64 * KvShape<T, HD, WHAT>::WAVES), (KvShape<T, HD,
           }
       }
     }
+    g = g1;
+    i0 = i1;
   }
 
   // The groups' sums, the upper half's added to the lower half's.

@@ -85,28 +85,61 @@ __global__ __launch_bounds__(kDiffThreads) void diff_delta_kernel(DiffArgs a, in
   }
 }
 
-// 4 waves x 32 rows, keys through LDS in tiles of 32. Scores transposed as in
-// the forward kernel: a row's sums are its lane's own numbers, and dS turns into
-// the B operand of dQ^T = K^T dS^T.
-template <typename T, int HD>
-__global__ __launch_bounds__(kDiffThreads, (sizeof(T) == 2 && HD <= 64 ? 2 : 1)) void diff_bwd_q_kernel(DiffArgs a) {
-  constexpr int DVP = 2 * HD, KS = HD / 16, VS = DVP / 16, KB = HD / 32, BN = 32;
+// A workgroup = RB blocks of 32 rows times KG groups, a wave each, keys through
+// LDS in tiles of 32 dealt to the groups in turn, whose sums meet in LDS at the
+// end. Scores transposed as in the forward kernel: a row's sums are its lane's
+// own numbers, and dS turns into the B operand of dQ^T = K^T dS^T. Four waves;
+// 128 rows where those fill the chip, 64 (WIDE false) with two groups otherwise,
+// if two tiles for each fit.
+template <typename T, int HD, bool WIDE>
+struct QShape {
+  static constexpr int DVP = 2 * HD;
+  static constexpr int WAVES = 4;
+  static constexpr int KG = !WIDE && HD * (int)sizeof(T) < 512 ? 2 : 1;
+  static constexpr int RB = WAVES / KG;
+  static constexpr int kBytes = 32 * (2 * HD + DVP) * (int)sizeof(T), kHead = 32 * HD * (int)sizeof(T);
+};
+
+template <typename T, int HD, bool WIDE>
+__global__ __launch_bounds__((64 * QShape<T, HD, WIDE>::WAVES), (HD == 32 || (sizeof(T) == 2 && HD == 64) ? 2 : 1)) void
+diff_bwd_q_kernel(DiffArgs a) {
+  using SH = QShape<T, HD, WIDE>;
+  constexpr int DVP = SH::DVP, KS = HD / 16, VS = DVP / 16, DB = HD / 32, BN = 32, RB = SH::RB, KG = SH::KG, ROWS = 32 * RB;
+  constexpr int kBytes = SH::kBytes, kHead = SH::kHead;
   using KT = LdsRows<T, HD>;
   using VT = LdsRows<T, DVP>;
-  constexpr int kTile = BN * (2 * HD + DVP);  // K's two heads and V
-  constexpr int kBytes = kTile * (int)sizeof(T), kHead = BN * HD * (int)sizeof(T);
-  __shared__ __attribute__((aligned(1024))) T smem[2][kTile];
-  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave, hl = lane / 32, ln = lane % 32;
+  constexpr int kSums = KG > 1 ? KG / 2 * RB * (2 * DB * 16 + 1) * kWave * 4 : 0;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[KG * 2 * kBytes > kSums ? KG * 2 * kBytes : kSums];
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave, hl = lane / 32,
+            ln = lane % 32;
+  const int kg = w / RB, rb = w % RB;
   const DiffTile t = diff_tile(a, blockIdx.x, a.n_mtiles);
   const int mt = a.n_mtiles - 1 - t.tile;
   const int L = diff_len(a, t.b);
-  const int r0 = mt * 128, rw0 = r0 + 32 * w, r = rw0 + ln;
+  const int r0 = mt * ROWS, rw0 = r0 + 32 * rb, r = rw0 + ln;
   const int i = r / a.G, head = t.hk * a.G + r % a.G;
   const bool live = r < a.R && i < L;
   const int limit = a.causal ? i : L - 1;
-  const int kv_end = r0 / a.G >= L ? 0 : (a.causal ? min(L, min(r0 + 127, a.R - 1) / a.G + 1) : L);
+  const int kv_end = r0 / a.G >= L ? 0 : (a.causal ? min(L, min(r0 + ROWS - 1, a.R - 1) / a.G + 1) : L);
   const int own_end = rw0 >= a.R || rw0 / a.G >= L ? 0 : (a.causal ? min(L, min(rw0 + 31, a.R - 1) / a.G + 1) : L);
   const int free = a.causal ? rw0 / a.G : L - 1;
+
+  const T* kp = reinterpret_cast<const T*>(a.k) + a.vk.row(t.b, 2 * t.hk, 0);
+  const T* vp = reinterpret_cast<const T*>(a.v) + a.vv.row(t.b, t.hk, 0);
+  KeyCopy<T, HD, BN, RB> kcopy;
+  KeyCopy<T, DVP, BN, RB> vcopy;
+  kcopy.init(a.vk.ss, a.D, rb, lane);
+  vcopy.init(a.vv.ss, a.Dv, rb, lane);
+  const uint32_t tiles = lds_offset(smem) + kg * 2 * kBytes;
+  const uint32_t krow = KT::lane_row(lane), kcol = KT::lane_col(lane), vrow = VT::lane_row(lane) + 2 * kHead;
+  auto issue = [&](int kv0, uint32_t tile) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c)
+      kcopy.issue(kp + c * a.vk.sh + kv0 * a.vk.ss, a.vk.ss, L - kv0, a.D, tile + c * kHead, rb);
+    vcopy.issue(vp + kv0 * a.vv.ss, a.vv.ss, L - kv0, a.Dv, tile + 2 * kHead, rb);
+  };
+  int kv0 = BN * kg;
+  if (kv0 < kv_end) issue(kv0, tiles);
 
   frag_t<T> qf[2][KS], of[VS];
   {
@@ -119,11 +152,11 @@ __global__ __launch_bounds__(kDiffThreads, (sizeof(T) == 2 && HD <= 64 ? 2 : 1))
 #pragma unroll
     for (int s = 0; s < VS; ++s) of[s] = load_frag<T>(live ? op : nullptr, 16 * s + 8 * hl, a.Dv);
   }
-  float16_t dq[2][KB];
+  float16_t dq[2][DB];
 #pragma unroll
   for (int c = 0; c < 2; ++c)
 #pragma unroll
-    for (int d = 0; d < KB; ++d) dq[c][d] = zero16();
+    for (int d = 0; d < DB; ++d) dq[c][d] = zero16();
   const float lift = ds_lift<T>(a, t.bh, t.hk, lane);
   const float c2 = a.scale * kLog2e;
   const float lam = live ? a.lam[head * a.lam_step] : 0.f;
@@ -136,26 +169,11 @@ __global__ __launch_bounds__(kDiffThreads, (sizeof(T) == 2 && HD <= 64 ? 2 : 1))
   const float d0 = -del[0] * lift, nl = -lam * lift;
   float rest = 0.f;
 
-  const T* kp = reinterpret_cast<const T*>(a.k) + a.vk.row(t.b, 2 * t.hk, 0);
-  const T* vp = reinterpret_cast<const T*>(a.v) + a.vv.row(t.b, t.hk, 0);
-  KeyCopy<T, HD, BN, 4> kcopy;
-  KeyCopy<T, DVP, BN, 4> vcopy;
-  kcopy.init(a.vk.ss, a.D, w, lane);
-  vcopy.init(a.vv.ss, a.Dv, w, lane);
-  const uint32_t tiles = lds_offset(smem);
-  const uint32_t krow = KT::lane_row(lane), kcol = KT::lane_col(lane), vrow = VT::lane_row(lane) + 2 * kHead;
-  auto issue = [&](int kv0, uint32_t tile) {
-#pragma unroll
-    for (int c = 0; c < 2; ++c)
-      kcopy.issue(kp + c * a.vk.sh + kv0 * a.vk.ss, a.vk.ss, L - kv0, a.D, tile + c * kHead, w);
-    vcopy.issue(vp + kv0 * a.vv.ss, a.vv.ss, L - kv0, a.Dv, tile + 2 * kHead, w);
-  };
-  if (kv_end > 0) issue(0, tiles);
-  int cur = 0;
-  for (int kv0 = 0; kv0 < kv_end; kv0 += BN, cur ^= 1) {
+  // The workgroup goes round together, the last round maybe without a tile for every group.
+  for (int first = 0, cur = 0; first < kv_end; first += KG * BN, kv0 += KG * BN, cur ^= 1) {
     wait_copies();
     lds_barrier();
-    if (kv0 + BN < kv_end) issue(kv0 + BN, tiles + (cur ^ 1) * kBytes);
+    if (kv0 + KG * BN < kv_end) issue(kv0 + KG * BN, tiles + (cur ^ 1) * kBytes);
     if (kv0 >= own_end) continue;
     const uint32_t tile = tiles + cur * kBytes;
     float16_t p[2], dp = zero16();
@@ -190,9 +208,45 @@ __global__ __launch_bounds__(kDiffThreads, (sizeof(T) == 2 && HD <= 64 ? 2 : 1))
       for (int s = 0; s < 2; ++s) {
         const frag_t<T> f = acc_frag<T>(p[c], s);
 #pragma unroll
-        for (int d = 0; d < KB; ++d) dq[c][d] = Elem<T>::mma(KT::col_frag(tile + kcol, d, c * kHead + 16 * s * KT::kRowBytes), f, dq[c][d]);
+        for (int d = 0; d < DB; ++d)
+          dq[c][d] = Elem<T>::mma(KT::col_frag(tile + kcol, d, c * kHead + 16 * s * KT::kRowBytes), f, dq[c][d]);
       }
   }
+
+  // The groups' sums, the upper half's added to the lower half's.
+#pragma unroll
+  for (int half = KG / 2; half > 0; half /= 2) {
+    const int at = (kg % half) * RB + rb;
+    float4_t* x = reinterpret_cast<float4_t*>(smem) + at * 2 * DB * 4 * kWave;
+    float* y = reinterpret_cast<float*>(smem) + half * RB * 2 * DB * 16 * kWave + at * kWave;
+    __syncthreads();
+    if (kg >= half && kg < 2 * half) {
+      y[lane] = rest;
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            x[((c * DB + d) * 4 + e) * kWave + lane] =
+                float4_t{dq[c][d][4 * e], dq[c][d][4 * e + 1], dq[c][d][4 * e + 2], dq[c][d][4 * e + 3]};
+    }
+    __syncthreads();
+    if (kg < half) {
+      rest += y[lane];
+#pragma unroll
+      for (int c = 0; c < 2; ++c)
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float4_t z = x[((c * DB + d) * 4 + e) * kWave + lane];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) dq[c][d][4 * e + j] += z[j];
+          }
+    }
+  }
+  if (kg != 0) return;
 
   rest = pair_sum(rest);
   if (r >= a.R) return;
@@ -202,7 +256,7 @@ __global__ __launch_bounds__(kDiffThreads, (sizeof(T) == 2 && HD <= 64 ? 2 : 1))
   for (int c = 0; c < 2; ++c) {
     T* p = reinterpret_cast<T*>(a.dq) + a.vdq.row(t.b, 2 * head + c, i);
 #pragma unroll
-    for (int d = 0; d < KB; ++d)
+    for (int d = 0; d < DB; ++d)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int col = 32 * d + 8 * e + 4 * hl;
@@ -212,6 +266,15 @@ __global__ __launch_bounds__(kDiffThreads, (sizeof(T) == 2 && HD <= 64 ? 2 : 1))
         if (col < a.D) store4t<T>(p + col, y[0], y[1], y[2], y[3]);
       }
   }
+}
+
+template <typename T, int HD, bool WIDE>
+int launch_q(DiffArgs a, hipStream_t stream) {
+  using SH = QShape<T, HD, WIDE>;
+  a.n_mtiles = (a.R + 32 * SH::RB - 1) / (32 * SH::RB);
+  hipLaunchKernelGGL((diff_bwd_q_kernel<T, HD, WIDE>), dim3(uint32_t((int64_t)a.B * a.Hk * a.n_mtiles)),
+                     dim3(64 * SH::WAVES), 0, stream, a);
+  return tjh::launch_status();
 }
 
 // dlam: one workgroup per weight, its rows in a fixed order, in 64 bits.
@@ -249,16 +312,17 @@ int diff_delta(const DiffArgs& a, int dtype, hipStream_t stream) {
   return dtype == TJ_F16 ? launch_delta<half_t>(a, stream) : launch_delta<bf16_t>(a, stream);
 }
 
-int diff_bwd_q(const DiffArgs& args, int dtype, hipStream_t stream) {
-  const int rc = diff_dispatch(args, dtype, [&](auto t, auto hd) {
-    DiffArgs a = args;
-    a.n_mtiles = (a.R + 127) / 128;
-    hipLaunchKernelGGL((diff_bwd_q_kernel<decltype(t), decltype(hd)::value>),
-                       dim3(uint32_t((int64_t)a.B * a.Hk * a.n_mtiles)), dim3(kDiffThreads), 0, stream, a);
-    return tjh::launch_status();
+int diff_bwd_q(const DiffArgs& a, int dtype, hipStream_t stream) {
+  const bool wide = wide_tiles(a);
+  const int rc = diff_dispatch(a, dtype, [&](auto t, auto hd) {
+    using T = decltype(t);
+    constexpr int HD = decltype(hd)::value;
+    if constexpr (QShape<T, HD, true>::RB != QShape<T, HD, false>::RB)
+      if (!wide) return launch_q<T, HD, false>(a, stream);
+    return launch_q<T, HD, true>(a, stream);
   });
   if (rc != TJ_OK) return rc;
-  hipLaunchKernelGGL(diff_dlam_kernel, dim3(args.n_lam), dim3(1024), 0, stream, args);
+  hipLaunchKernelGGL(diff_dlam_kernel, dim3(a.n_lam), dim3(1024), 0, stream, a);
   return tjh::launch_status();
 }
 

@@ -7,10 +7,11 @@
 // where they stand. The two maps have their own running maximum, sum and
 // accumulator and share every V fragment.
 //
-// diff_fwd_kernel: a workgroup = 4 waves = 128 rows of one (b, key head), 32
-// rows a wave; keys stream through LDS in tiles. diff_few_kernel: a workgroup =
-// one wave = 32 rows and one part of the keys, with its own LDS tile. Sweeps
-// cut into parts are joined by diff_join_kernel.
+// diff_fwd_kernel: a workgroup = RB blocks of 32 rows of one (b, key head) times
+// KG groups, a wave each; key tiles of 32 stream through LDS, dealt to the groups
+// in turn, and the groups' sums meet in LDS at the end. diff_few_kernel: a
+// workgroup = one wave = 32 rows and one part of the keys, with its own LDS tile.
+// Sweeps cut into parts are joined by diff_join_kernel.
 #include "diff_attn.h"
 
 namespace tj {
@@ -21,7 +22,7 @@ constexpr float kLazy = 8.f;  // the running maximum moves when a row's maximum 
 template <typename T, int HD, int BNT>
 struct FwdShape {
   static constexpr int DVP = 2 * HD;
-  static constexpr int BN = BNT;
+  static constexpr int BN = BNT;  // keys of a tile
   using KT = LdsRows<T, HD>;
   using VT = LdsRows<T, DVP>;
   static constexpr int KS = HD / 16;   // k-steps over the head dim
@@ -91,10 +92,10 @@ struct FwdState {
     }
   }
 
-  // 32 keys of a tile, kb 32 .. kb 32 + 31 of it, kv0 on in the sequence, of
-  // which the row sees those <= limit. Small steps: scores and probabilities of
-  // 64 keys at once exceed the registers of two waves per SIMD, and a reload
-  // waits for the copies in flight too.
+  // 32 keys of a tile, from its key 32 kb on, kv0 in the sequence, of which the
+  // row sees those <= limit. (Scores and probabilities of 64 keys at once exceed
+  // the registers of two waves per SIMD, and a spilled value's reload waits for
+  // the copies in flight too.)
   __device__ __forceinline__ void step(uint32_t tile, int kb, int kv0, int limit, bool masked, int lane) {
     const int hl = lane / 32;
     const uint32_t kt = tile + kbase, vt = tile + vbase;
@@ -148,6 +149,42 @@ struct FwdState {
       }
   }
 
+  // Adds the state of another group's wave over the same rows and other keys,
+  // which that wave has left in LDS (give).
+  static constexpr int kGive = SH::DB * 4 * kWave;  // float4 per map
+  __device__ __forceinline__ void give(float4_t* x, float* ml, int lane) {
+#pragma unroll
+    for (int c = 0; c < NM; ++c) {
+      ml[(2 * c) * kWave + lane] = m[c];
+      ml[(2 * c + 1) * kWave + lane] = l[c];
+#pragma unroll
+      for (int d = 0; d < SH::DB; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          x[c * kGive + (d * 4 + e) * kWave + lane] =
+              float4_t{o[c][d][4 * e], o[c][d][4 * e + 1], o[c][d][4 * e + 2], o[c][d][4 * e + 3]};
+    }
+  }
+  __device__ __forceinline__ void take(const float4_t* x, const float* ml, int lane) {
+#pragma unroll
+    for (int c = 0; c < NM; ++c) {
+      const float m1 = ml[(2 * c) * kWave + lane], to = fmaxf(m[c], m1);
+      // An unset maximum (-inf) goes with sums that are zero, or NaN and kept.
+      const float w0 = m[c] == -__builtin_inff() ? 1.f : fast_exp2(m[c] - to);
+      const float w1 = m1 == -__builtin_inff() ? 1.f : fast_exp2(m1 - to);
+      m[c] = to;
+      l[c] = fmaf(l[c], w0, ml[(2 * c + 1) * kWave + lane] * w1);
+#pragma unroll
+      for (int d = 0; d < SH::DB; ++d)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float4_t y = x[c * kGive + (d * 4 + e) * kWave + lane];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[c][d][4 * e + j] = fmaf(o[c][d][4 * e + j], w0, y[j] * w1);
+        }
+    }
+  }
+
   // The results of a part of the keys.
   __device__ __forceinline__ void finish_part(const DiffArgs& a, int bh, const DiffRow& row, int part, int lane) {
     const int hl = lane / 32;
@@ -172,10 +209,11 @@ struct FwdState {
   }
 
   // The rows' results. With one map a wave, the second map's waves hand theirs
-  // to the first's through `swap` (64 lanes x DB x 16 floats a pair of waves).
-  __device__ __forceinline__ void finish(const DiffArgs& a, int b, int hk, const DiffRow& row, float4_t* swap, int lane) {
+  // to the first's through `swap` (64 lanes x DB x 16 floats a pair of waves);
+  // waves whose rows are not theirs to write (`mine` false) come along.
+  __device__ __forceinline__ void finish(const DiffArgs& a, int b, int hk, const DiffRow& row, float4_t* swap, int lane, bool mine) {
     const int hl = lane / 32, head = hk * a.G + row.g;
-    const bool in = row.r < a.R;
+    const bool in = mine && row.r < a.R;
     float* mp = a.maps != nullptr && in ? a.maps + row_at(a, b, head, row.i) * 2 * a.Dv : nullptr;
 #pragma unroll
     for (int c = 0; c < NM; ++c) {
@@ -195,7 +233,7 @@ struct FwdState {
     }
     if constexpr (NM == 1) {
       __syncthreads();  // the key tiles, in whose place `swap` lies, have been read
-      if (first == 1)
+      if (first == 1 && mine)
 #pragma unroll
         for (int d = 0; d < SH::DB; ++d)
 #pragma unroll
@@ -247,42 +285,82 @@ struct KeyTiles {
 template <int HD>
 constexpr int kMaps = HD <= 64 ? 2 : 1;
 
-template <typename T, int HD, bool PART>
-__global__ __launch_bounds__(512 / kMaps<HD>, (sizeof(T) == 4 && HD == 64 ? 1 : 2)) void diff_fwd_kernel(DiffArgs a) {
-  constexpr int BN = sizeof(T) == 4 ? 32 : 64, NM = kMaps<HD>;
+// A workgroup's waves: row blocks times key groups times the waves that share the
+// maps. Four (eight of one map), so that two workgroups share a CU where the
+// registers allow it, and one's products run beside the other's exponentials:
+// eight waves meeting at one barrier were 15 % slower on the long bf16 case. 128
+// rows where those fill the chip, 64 (WIDE false) with two groups otherwise,
+// if two tiles for each fit.
+template <typename T, int HD, bool WIDE>
+struct FwdGroups {
+  static constexpr int kPairs = 2 / kMaps<HD>;
+  static constexpr int KG = !WIDE && HD * (int)sizeof(T) < 512 ? 2 : 1;
+  static constexpr int RB = 4 / KG;
+  static constexpr int WAVES = 4 * kPairs;
+  static constexpr int BN = KG == 1 && HD * (int)sizeof(T) <= 256 ? 64 : 32;
+};
+
+template <typename T, int HD, bool WIDE, bool PART>
+__global__ __launch_bounds__((64 * FwdGroups<T, HD, WIDE>::WAVES), (sizeof(T) == 4 && HD == 64 ? 1 : 2)) void
+diff_fwd_kernel(DiffArgs a) {
+  using GR = FwdGroups<T, HD, WIDE>;
+  constexpr int BN = GR::BN;
   using SH = FwdShape<T, HD, BN>;
-  __shared__ __attribute__((aligned(1024))) T smem[2][SH::kElems];
-  static_assert(NM == 2 || sizeof(smem) >= 4 * 64 * SH::DB * 64, "room for the second map's results");
-  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave, rw = w % 4;
+  using State = FwdState<T, HD, BN, kMaps<HD>>;
+  constexpr int NM = kMaps<HD>, RB = GR::RB, KG = GR::KG, ROWS = 32 * RB;
+  // Two tiles a group; afterwards the groups' results, then the second map's.
+  constexpr int kSums = 16 * State::kGive * RB * (KG > 1 && KG * GR::kPairs * NM / 2 > 1 ? KG * GR::kPairs * NM / 2 : 1);
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[KG * 2 * SH::kBytes > kSums ? KG * 2 * SH::kBytes : kSums];
+  __shared__ float ml[KG > 1 ? KG / 2 * RB * GR::kPairs * NM * 2 * kWave : 1];
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
+  const int kg = w / (RB * GR::kPairs), in_group = w % (RB * GR::kPairs), rb = in_group % RB, map = in_group / RB;
   const DiffTile t = diff_tile(a, blockIdx.x, a.n_mtiles);
   const int part = PART ? t.tile / a.n_mtiles : -1;
   const int mt = a.n_mtiles - 1 - (PART ? t.tile % a.n_mtiles : t.tile);
   const int L = diff_len(a, t.b);
-  const DiffSpan all(a, mt * 128, mt * 128 + 127, L), own(a, mt * 128 + 32 * rw, mt * 128 + 32 * rw + 31, L);
-  const DiffRow row(a, mt * 128 + 32 * rw + lane % 32, L);
+  const int r0 = mt * ROWS, rw0 = r0 + 32 * rb;
+  const DiffSpan all(a, r0, r0 + ROWS - 1, L), own(a, rw0, rw0 + 31, L);
+  const DiffRow row(a, rw0 + lane % 32, L);
   const int kv_begin = PART ? part * a.part_keys : 0;
   const int kv_end = PART ? min(all.end, kv_begin + a.part_keys) : all.end;
   if (PART && kv_begin >= kv_end) return;  // not read either (live parts are counted from the rows' last key)
-  const uint32_t tiles = lds_offset(smem);
-  KeyTiles<T, SH, HD, 8 / NM> keys;
-  keys.init(a, t.b, t.hk, w, lane);
-  if (kv_begin < kv_end) keys.issue(a, kv_begin, L, tiles, w);
-  FwdState<T, HD, BN, NM> st;
-  st.init(a, t.b, t.hk, row, w / 4, lane);
-  int cur = 0;
-  for (int kv0 = kv_begin; kv0 < kv_end; kv0 += BN, cur ^= 1) {
-    // The tile is there, and the other one has been read by every wave.
+  const uint32_t tiles = lds_offset(smem) + kg * 2 * SH::kBytes;
+  KeyTiles<T, SH, HD, RB * GR::kPairs> keys;
+  keys.init(a, t.b, t.hk, in_group, lane);
+  int kv0 = kv_begin + BN * kg;
+  if (kv0 < kv_end) keys.issue(a, kv0, L, tiles, in_group);
+  State st;
+  st.init(a, t.b, t.hk, row, map, lane);
+  // The workgroup goes round together, the last round maybe without a tile for every group.
+  for (int first = kv_begin, cur = 0; first < kv_end; first += KG * BN, kv0 += KG * BN, cur ^= 1) {
+    // The tile is there, and the group's other one has been read by its waves.
     wait_copies();
     lds_barrier();
-    if (kv0 + BN < kv_end) keys.issue(a, kv0 + BN, L, tiles + (cur ^ 1) * SH::kBytes, w);
+    if (kv0 + KG * BN < kv_end) keys.issue(a, kv0 + KG * BN, L, tiles + (cur ^ 1) * SH::kBytes, in_group);
 #pragma unroll
     for (int kb = 0; kb < BN / 32; ++kb) {
-      const int k0 = kv0 + 32 * kb;
-      if (k0 < own.end) st.step(tiles + cur * SH::kBytes, kb, k0, row.limit, k0 + 31 > own.free, lane);
+      const int at = kv0 + 32 * kb;
+      if (at < min(own.end, kv_end)) st.step(tiles + cur * SH::kBytes, kb, at, row.limit, at + 31 > own.free, lane);
     }
   }
-  if constexpr (PART) st.finish_part(a, t.bh, row, part, lane);
-  else st.finish(a, t.b, t.hk, row, reinterpret_cast<float4_t*>(smem) + rw * SH::DB * 4 * kWave, lane);
+  // The groups' states, the upper half's joined to the lower half's.
+#pragma unroll
+  for (int half = KG / 2; half > 0; half /= 2) {
+    float4_t* x = reinterpret_cast<float4_t*>(smem);
+    const int at = (kg % half) * RB * GR::kPairs + in_group;
+    __syncthreads();
+    if (kg >= half && kg < 2 * half) st.give(x + at * NM * State::kGive, ml + at * NM * 2 * kWave, lane);
+    __syncthreads();
+    if (kg < half) st.take(x + at * NM * State::kGive, ml + at * NM * 2 * kWave, lane);
+  }
+  if constexpr (NM == 2) {
+    if (kg != 0) return;
+  }
+  if constexpr (PART) {
+    if (kg == 0) st.finish_part(a, t.bh, row, part, lane);
+  } else {
+    st.finish(a, t.b, t.hk, row, reinterpret_cast<float4_t*>(smem) + rb * State::kGive, lane, kg == 0);
+  }
 }
 
 template <typename T, int HD>
@@ -370,20 +448,30 @@ int launch_join(const DiffArgs& a, hipStream_t stream) {
 
 }  // namespace
 
-int diff_fwd(const DiffArgs& args, int dtype, hipStream_t stream) {
-  return diff_dispatch(args, dtype, [&](auto t, auto hd) {
+namespace {
+template <typename T, int HD, bool WIDE>
+int launch_fwd(DiffArgs a, hipStream_t stream) {
+  using GR = FwdGroups<T, HD, WIDE>;
+  a.n_mtiles = (a.R + 32 * GR::RB - 1) / (32 * GR::RB);
+  const int64_t n = (int64_t)a.B * a.Hk * a.n_mtiles;
+  if (a.n_parts > 1) {
+    hipLaunchKernelGGL((diff_fwd_kernel<T, HD, WIDE, true>), dim3(uint32_t(n * a.n_parts)), dim3(64 * GR::WAVES), 0, stream, a);
+    const int rc = tjh::launch_status();
+    return rc != TJ_OK ? rc : launch_join<T>(a, stream);
+  }
+  hipLaunchKernelGGL((diff_fwd_kernel<T, HD, WIDE, false>), dim3(uint32_t(n)), dim3(64 * GR::WAVES), 0, stream, a);
+  return tjh::launch_status();
+}
+}  // namespace
+
+int diff_fwd(const DiffArgs& a, int dtype, hipStream_t stream) {
+  const bool wide = wide_tiles(a);
+  return diff_dispatch(a, dtype, [&](auto t, auto hd) {
     using T = decltype(t);
     constexpr int HD = decltype(hd)::value;
-    DiffArgs a = args;
-    a.n_mtiles = (a.R + 127) / 128;
-    const int64_t n = (int64_t)a.B * a.Hk * a.n_mtiles;
-    if (a.n_parts > 1) {
-      hipLaunchKernelGGL((diff_fwd_kernel<T, HD, true>), dim3(uint32_t(n * a.n_parts)), dim3(512 / kMaps<HD>), 0, stream, a);
-      const int rc = tjh::launch_status();
-      return rc != TJ_OK ? rc : launch_join<T>(a, stream);
-    }
-    hipLaunchKernelGGL((diff_fwd_kernel<T, HD, false>), dim3(uint32_t(n)), dim3(512 / kMaps<HD>), 0, stream, a);
-    return tjh::launch_status();
+    if constexpr (FwdGroups<T, HD, true>::RB != FwdGroups<T, HD, false>::RB)
+      if (!wide) return launch_fwd<T, HD, false>(a, stream);
+    return launch_fwd<T, HD, true>(a, stream);
   });
 }
 
