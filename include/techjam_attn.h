@@ -444,7 +444,8 @@ int tj_diff_attn_bwd(const void* q, const void* k, const void* v, const float* m
  * are torch's):
  *   y = (x - mean) * rstd * weight + bias,  rstd = 1 / sqrt(var + eps)
  * x, y, dy, dx: [rows, cols] of dtype (TJ_F32, TJ_F16 or TJ_BF16), unit column
- * stride, any row stride (in elements), aligned to one element. weight, bias
+ * stride, aligned to one element, any row stride >= 0 (in elements; 32 rows
+ * within 2 GiB, TJ_ERR_UNSUPPORTED otherwise). weight, bias
  * and their gradients: [cols] of w_dtype, TJ_F32 or dtype; each may be NULL
  * (weight 1, bias 0). Sums are fp32. cols at most 16384.
  * mean, rstd: fp32 [rows], both or neither in the forward call, what the

@@ -277,22 +277,30 @@ int launch_q(DiffArgs a, hipStream_t stream) {
   return tjh::launch_status();
 }
 
-// dlam: one workgroup per weight, its rows in a fixed order, in 64 bits.
+// dlam: one workgroup per weight, its rows in a fixed order, in 64 bits. A
+// weight for all heads sums [B, H, Sq] from end to end, a head's own B runs of Sq.
 __global__ __launch_bounds__(1024) void diff_dlam_kernel(DiffArgs a) {
   __shared__ double red[1024 / kWave];
-  const int tid = threadIdx.x, n = blockIdx.x;
+  const int tid = threadIdx.x, h = blockIdx.x;
+  const int64_t run = a.lam_step ? a.Sq : (int64_t)a.B * a.H * a.Sq;
+  const int runs = a.lam_step ? a.B : 1;
   double s = 0.;
-  for (int h = (a.lam_step ? n : 0); h < (a.lam_step ? n + 1 : a.H); ++h)
-    for (int b = 0; b < a.B; ++b) {
-      const float* p = a.gsum + row_at(a, b, h, 0);
-      for (int i = tid; i < a.Sq; i += 1024) s += p[i];
+  for (int b = 0; b < runs; ++b) {
+    const float* p = a.gsum + row_at(a, b, h, 0);
+    for (int64_t i0 = tid; i0 < run; i0 += 8 * 1024) {
+      float x[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] = p[min(i0 + 1024 * k, run - 1)];  // no branches: eight loads in flight
+#pragma unroll
+      for (int k = 0; k < 8; ++k) s += i0 + 1024 * k < run ? x[k] : 0.f;
     }
+  }
   for (int m = kWave / 2; m > 0; m >>= 1) s += __shfl_xor(s, m);
   if (tid % kWave == 0) red[tid / kWave] = s;
   __syncthreads();
   if (tid == 0) {
     for (int w = 1; w < 1024 / kWave; ++w) s += red[w];
-    a.dlam[n] = (float)-s;
+    a.dlam[h] = (float)-s;
   }
 }
 
@@ -313,12 +321,11 @@ int diff_delta(const DiffArgs& a, int dtype, hipStream_t stream) {
 }
 
 int diff_bwd_q(const DiffArgs& a, int dtype, hipStream_t stream) {
-  const bool wide = wide_tiles(a);
   const int rc = diff_dispatch(a, dtype, [&](auto t, auto hd) {
     using T = decltype(t);
     constexpr int HD = decltype(hd)::value;
     if constexpr (QShape<T, HD, true>::RB != QShape<T, HD, false>::RB)
-      if (!wide) return launch_q<T, HD, false>(a, stream);
+      if (!wide_tiles(a, HD)) return launch_q<T, HD, false>(a, stream);
     return launch_q<T, HD, true>(a, stream);
   });
   if (rc != TJ_OK) return rc;

@@ -51,7 +51,7 @@ def _rows_view(t: torch.Tensor) -> torch.Tensor:
 def _empty_heads(b: int, h: int, s: int, d: int, like: torch.Tensor) -> torch.Tensor:
     """A ``[B, H, S, D]`` tensor whose storage is ``[B, S, H, D]``, what
     merging the heads or splitting a projection views for free."""
-    return torch.empty(b, s, h, d, dtype=like.dtype, device=like.device).transpose(1, 2)
+    return like.new_empty_strided((b, h, s, d), (s * h * d, d, h * d, 1))
 
 
 def _check(q, k, v, lam, lengths, what: str, cached: bool) -> None:

@@ -24,49 +24,59 @@ MAX_WIDTH = 16384
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """``t`` as ``[rows, width]`` with unit column stride: a view where its
-    leading dimensions have one stride in common, else a copy."""
+    leading dimensions have one stride in common (below 2^23 elements), else a
+    copy."""
     width = t.shape[-1]
-    if t.stride(-1) != 1 and width > 1:
-        return t.reshape(-1, width).contiguous()
-    return t.reshape(-1, width)
+    t = t.reshape(-1, width)
+    if (t.stride(1) != 1 and width > 1) or t.stride(0) >= 1 << 23:
+        return t.contiguous()
+    return t
 
 
 def _forward(x, weight, bias, eps, stats):
     rows2d = _rows(x)
     rows, width = rows2d.shape
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    mean = rstd = None
-    if stats:
-        mean, rstd = torch.empty(2, rows, dtype=torch.float32, device=x.device)
-    w_dtype = next((DTYPES[p.dtype] for p in (weight, bias) if p is not None), _lib.TJ_F32)
-    with on_device(x.device):
+    dev = x.device
+    y = x.new_empty(x.shape)
+    # mean [rows], then 1 / sqrt(var + eps) [rows], in one tensor.
+    moments = torch.empty(2 * rows, dtype=torch.float32, device=dev) if stats else None
+    mean = moments.data_ptr() if stats and rows else None
+    w_dtype = _lib.TJ_F32
+    if weight is not None or bias is not None:
+        w_dtype = DTYPES[(bias if weight is None else weight).dtype]
+    with on_device(dev):
         code = _lib.lib().tj_layer_norm_fwd(
             rows2d.data_ptr(), _ptr(weight), _ptr(bias), y.data_ptr(), DTYPES[x.dtype], w_dtype, rows, width,
-            rows2d.stride(0), width, eps, _ptr(mean), _ptr(rstd), _stream_ptr(x.device))
-    _lib.check(code, "tj_layer_norm_fwd")
-    return y, mean, rstd
+            rows2d.stride(0), width, eps, mean, mean and mean + 4 * rows, _stream_ptr(dev))
+    if code:
+        _lib.check(code, "tj_layer_norm_fwd")
+    return y, moments
 
 
 def _backward(ctx, dy):
-    x, weight, mean, rstd = ctx.saved_tensors
+    x, weight, moments = ctx.saved_tensors
     need_x, need_w, need_b, _ = ctx.needs_input_grad
     dy2d, x2d = _rows(dy), _rows(x)
     rows, width = x2d.shape
     dev = x.device
-    dx = torch.empty(x.shape, dtype=x.dtype, device=dev) if need_x else None
+    dx = x.new_empty(x.shape) if need_x else None
     w_torch = ctx.bias_dtype if weight is None else weight.dtype
     make = torch.zeros if rows == 0 else torch.empty
     dw = make(width, dtype=w_torch, device=dev) if need_w else None
     db = make(width, dtype=w_torch, device=dev) if need_b else None
+    if rows == 0:
+        return dx, dw, db, None
     lib = _lib.lib()
+    mean = moments.data_ptr()
     with on_device(dev):
         ws_bytes = lib.tj_layer_norm_bwd_workspace_bytes(rows, width) if need_w or need_b else 0
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
         code = lib.tj_layer_norm_bwd(
-            dy2d.data_ptr(), x2d.data_ptr(), _ptr(weight), mean.data_ptr(), rstd.data_ptr(), _ptr(dx), _ptr(dw),
-            _ptr(db), DTYPES[x.dtype], _lib.TJ_F32 if w_torch is None else DTYPES[w_torch], rows, width,
-            dy2d.stride(0), x2d.stride(0), width, _ptr(ws), ws_bytes, _stream_ptr(dev))
-    _lib.check(code, "tj_layer_norm_bwd")
+            dy2d.data_ptr(), x2d.data_ptr(), _ptr(weight), mean, mean + 4 * rows, _ptr(dx), _ptr(dw), _ptr(db),
+            DTYPES[x.dtype], _lib.TJ_F32 if w_torch is None else DTYPES[w_torch], rows, width, dy2d.stride(0),
+            x2d.stride(0), width, _ptr(ws), ws_bytes, _stream_ptr(dev))
+    if code:
+        _lib.check(code, "tj_layer_norm_bwd")
     return dx, dw, db, None
 
 
@@ -79,8 +89,8 @@ _backward_once = once_differentiable(_backward)
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        y, mean, rstd = _forward(x, weight, bias, eps, True)
-        ctx.save_for_backward(x, weight, mean, rstd)
+        y, moments = _forward(x, weight, bias, eps, True)
+        ctx.save_for_backward(x, weight, moments)
         ctx.bias_dtype = None if bias is None else bias.dtype
         return y
 
