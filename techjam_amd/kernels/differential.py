@@ -192,6 +192,10 @@ def differential_attention(
     what those rows and keys hold is not read, and their gradients are zero.
     ``scale`` defaults to ``D ** -0.5``.
 
+    A NaN or an infinity among the valid inputs spoils what depends on it; one in
+    ``v`` under ``is_causal`` also the up to 31 rows before it in its tile of 32
+    tokens, as 0 times NaN.
+
     The output's storage is ``[B, S, H, Dv]``, so that merging the heads is a
     view. Gradients come for q, k, v and lam (summed over what shares a weight);
     their sums have a fixed order, so equal calls give equal bits. Second

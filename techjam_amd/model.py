@@ -22,10 +22,14 @@ import torch.nn.functional as F
 
 from .kernels.attention import scaled_dot_product_attention
 from .kernels.elementwise import NORM_WIDTHS
+from .kernels.layer_norm import LayerNorm
 from .kernels.linear import ffn_norm, projections, residual_norm, split_products_allowed
 
 
 ACTIVATIONS = ("gelu", "relu")
+ATTENTIONS = ("softmax", "differential")
+#: The norms whose parameters the fused inference kernels read.
+NORM_TYPES = (nn.LayerNorm, LayerNorm)
 
 
 @dataclass(frozen=True)
@@ -36,8 +40,12 @@ class TransformerConfig:
     pre-norm with exact GELU (the defaults); ``norm_first=False,
     activation="relu"`` is the post-norm / ReLU block of
     ``torch.nn.TransformerEncoderLayer(norm_first=False, activation="relu")``,
-    the wording some benchmark configurations are stated in. Config objects
-    without these fields (the reference harness's own) mean the defaults.
+    the wording some benchmark configurations are stated in.
+    ``attention="differential"`` puts differential attention
+    (``implementations/differential.py``) in the place of softmax attention:
+    an encoder that can also be trained on the kernels and, when it is causal
+    and pre-norm, run token by token (``TransformerEncoder.step``). Config
+    objects without these fields (the reference harness's own) mean the defaults.
     """
 
     batch_size: int
@@ -49,6 +57,7 @@ class TransformerConfig:
     causal: bool
     norm_first: bool = True
     activation: str = "gelu"
+    attention: str = "softmax"
 
     def validate(self) -> None:
         for name in ("batch_size", "seq_len", "d_model", "num_heads", "ffn_dim", "num_layers"):
@@ -60,6 +69,17 @@ class TransformerConfig:
             )
         if self.activation not in ACTIVATIONS:
             raise ValueError(f"activation must be one of {ACTIVATIONS}, not {self.activation!r}")
+        if attention_variant(self) == "differential" and self.d_model % (2 * self.num_heads):
+            raise ValueError(f"d_model ({self.d_model}) must be divisible by 2 * num_heads ({2 * self.num_heads}) "
+                             "for differential attention")
+
+
+def attention_variant(config) -> str:
+    """``"softmax"`` (also of configs that do not say) or ``"differential"``."""
+    attention = getattr(config, "attention", "softmax")
+    if attention not in ATTENTIONS:
+        raise ValueError(f"attention must be one of {ATTENTIONS}, not {attention!r}")
+    return attention
 
 
 def block_variant(config) -> Tuple[bool, str]:
@@ -219,15 +239,24 @@ class EncoderBlock(nn.Module):
     """
 
     def __init__(self, d_model: int, num_heads: int, ffn_dim: int, norm_first: bool = True,
-                 activation: str = "gelu") -> None:
+                 activation: str = "gelu", attention: str = "softmax", depth: int = 0) -> None:
         super().__init__()
         if activation not in ACTIVATIONS:
             raise ValueError(f"activation must be one of {ACTIVATIONS}, not {activation!r}")
         self.norm_first = norm_first
         self.activation = activation
-        self.norm1 = nn.LayerNorm(d_model)
-        self.attention = HipSelfAttention(d_model, num_heads)
-        self.norm2 = nn.LayerNorm(d_model)
+        #: Whether every operator of the block has gradients: with them enabled
+        #: it then runs unfused.
+        self.differentiable = attention == "differential"
+        norm = LayerNorm if self.differentiable else nn.LayerNorm
+        self.norm1 = norm(d_model)
+        if self.differentiable:
+            from .implementations.differential import DifferentialSelfAttention
+
+            self.attention = DifferentialSelfAttention(d_model, num_heads, depth)
+        else:
+            self.attention = HipSelfAttention(d_model, num_heads)
+        self.norm2 = norm(d_model)
         self.ffn_in = Linear(d_model, ffn_dim)
         self.ffn_out = Linear(ffn_dim, d_model)
 
@@ -239,7 +268,7 @@ class EncoderBlock(nn.Module):
             return self._forward_fused(x, valid_token_mask, causal, valid_len)
         if self.norm_first:
             x = x + self.attention(self.norm1(x), valid_token_mask, causal, valid_len=valid_len)
-            x = x + self.ffn_out(self._act(self.ffn_in(self.norm2(x))))
+            x = self.ffn(x)
         else:
             x = self.norm1(x + self.attention(x, valid_token_mask, causal, valid_len=valid_len))
             x = self.norm2(x + self.ffn_out(self._act(self.ffn_in(x))))
@@ -247,7 +276,13 @@ class EncoderBlock(nn.Module):
             x = x.masked_fill(~valid_token_mask[..., None], 0)
         return x
 
+    def ffn(self, x):
+        """The pre-norm block's second half."""
+        return x + self.ffn_out(self._act(self.ffn_in(self.norm2(x))))
+
     def _can_fuse(self, x, valid_token_mask, valid_len) -> bool:
+        if self.differentiable and (torch.is_grad_enabled() or self.ffn_in.weight.dtype != torch.float32):
+            return False
         return (x.is_cuda and x.dtype == torch.float32 and x.ndim == 3 and x.is_contiguous()
                 and x.data_ptr() % 16 == 0 and x.shape[-1] % 4 == 0 and self.ffn_in.out_features % 4 == 0
                 and (valid_token_mask is None or valid_len is not None)
@@ -258,7 +293,7 @@ class EncoderBlock(nn.Module):
     def _post_norms_fusable(self, x) -> bool:
         c = x.shape[-1]
         return (c in NORM_WIDTHS
-                and all(type(n) is nn.LayerNorm and n.elementwise_affine and n.bias is not None
+                and all(type(n) in NORM_TYPES and n.elementwise_affine and n.bias is not None
                         and n.weight.dtype == torch.float32 for n in (self.norm1, self.norm2)))
 
     def _hidden(self, a, act, allowed):
@@ -374,6 +409,14 @@ class EncoderBlock(nn.Module):
                                              norm_dtype=f16 if fp16_operands and not last else f32))
 
 
+def _not_captured() -> None:
+    """A replay would not count its tokens against the caches' capacity."""
+    if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
+        from .errors import UnsupportedCaseError
+
+        raise UnsupportedCaseError("prefill and step keep count on the host and cannot be captured into a graph")
+
+
 def _must(t):
     if t is None:
         raise RuntimeError("the fused block kernels rejected a layout the block checked beforehand")
@@ -392,13 +435,16 @@ class TransformerEncoder(nn.Module):
         super().__init__()
         self.config = config
         self.norm_first, self.activation = block_variant(config)
+        self.attention = attention_variant(config)
         self.layers = nn.ModuleList(
-            EncoderBlock(config.d_model, config.num_heads, config.ffn_dim, self.norm_first, self.activation)
-            for _ in range(config.num_layers)
+            EncoderBlock(config.d_model, config.num_heads, config.ffn_dim, self.norm_first, self.activation,
+                         self.attention, depth)
+            for depth in range(config.num_layers)
         )
         # A post-norm stack ends in its last block's norm (torch.nn.TransformerEncoder
         # with norm=None); only the pre-norm stack has a final LayerNorm.
-        self.final_norm = nn.LayerNorm(config.d_model) if self.norm_first else nn.Identity()
+        norm = LayerNorm if self.attention == "differential" else nn.LayerNorm
+        self.final_norm = norm(config.d_model) if self.norm_first else nn.Identity()
 
     def forward_layers(self, x, valid_token_mask=None, valid_len=None, gemm_operands=None):
         """The layer stack and final norm; ``gemm_operands`` overrides the
@@ -406,6 +452,10 @@ class TransformerEncoder(nn.Module):
         operands = self.gemm_operands if gemm_operands is None else gemm_operands
         if operands not in ("fp32", "fp16"):
             raise ValueError(f"gemm_operands must be 'fp32' or 'fp16', not {operands!r}")
+        if operands == "fp16" and self.attention == "differential":
+            from .errors import UnsupportedCaseError
+
+            raise UnsupportedCaseError("fp16 GEMM operands are not implemented for differential attention")
         if self._can_fuse_norms(x, valid_token_mask, valid_len):
             return self._forward_layers_fused(x, valid_token_mask, valid_len, operands)
         if operands == "fp16":
@@ -421,6 +471,55 @@ class TransformerEncoder(nn.Module):
             x.masked_fill_(~valid_token_mask[..., None], 0)  # x is the norm's fresh output
         return x
 
+    # -- token by token (causal differential attention) ----------------------
+    def new_state(self, batch: int, capacity: int, dtype: Optional[torch.dtype] = None):
+        """Empty caches for ``batch`` sequences of up to ``capacity`` tokens, in
+        the parameters' type unless ``dtype`` says otherwise."""
+        from .errors import UnsupportedCaseError
+        from .implementations.differential import DifferentialState
+
+        if self.attention != "differential" or not self.norm_first or not self.config.causal:
+            raise UnsupportedCaseError("token by token: causal, pre-norm encoders of differential attention only")
+        weight = self.layers[0].ffn_in.weight if len(self.layers) else self.final_norm.weight
+        return DifferentialState(self.config, batch, capacity, weight.dtype if dtype is None else dtype, weight.device)
+
+    @torch.no_grad()
+    def prefill(self, x, state, valid_token_mask: Optional[torch.Tensor] = None):
+        """The forward pass of each sequence's first tokens (``x`` ``[B, S, D]``,
+        right-padded by the mask) that leaves their keys and values in ``state``."""
+        _not_captured()
+        state.longest = 0
+        state.reserve(x.shape[1])
+        lengths = None if valid_token_mask is None else prefix_lengths(valid_token_mask)
+        for layer, cache in zip(self.layers, state.layers):
+            x = x + layer.attention(layer.norm1(x), valid_token_mask, True, lengths, cache)
+            x = layer.ffn(x)
+        x = self.final_norm(x)
+        if valid_token_mask is not None:
+            x = x.masked_fill(~valid_token_mask[..., None], 0)
+            state.lengths.copy_(lengths)
+        else:
+            state.lengths.fill_(x.shape[1])
+        state.longest = x.shape[1]
+        return x
+
+    @torch.no_grad()
+    def step(self, x, state):
+        """The next ``T`` tokens of every sequence (``x`` ``[B, T, D]``): the
+        encoder's output for them, their keys and values added to ``state``."""
+        _not_captured()
+        if x.ndim != 3 or x.shape[0] != state.lengths.shape[0] or x.shape[1] == 0:
+            raise ValueError(f"x must be [{state.lengths.shape[0]}, T, {self.config.d_model}], not {tuple(x.shape)}")
+        tokens = x.shape[1]
+        state.reserve(tokens)
+        place = state.lengths[:, None].long() + torch.arange(tokens, device=x.device)
+        state.lengths += tokens
+        state.longest += tokens
+        for layer, cache in zip(self.layers, state.layers):
+            x = x + layer.attention.step(layer.norm1(x), cache, state.lengths, place)
+            x = layer.ffn(x)
+        return self.final_norm(x)
+
     def _can_fuse_norms(self, x, valid_token_mask, valid_len) -> bool:
         d = x.shape[-1] if x.ndim == 3 else 0
         if not self.norm_first:
@@ -428,7 +527,7 @@ class TransformerEncoder(nn.Module):
         norms = [m for layer in self.layers for m in (layer.norm1, layer.norm2)] + [self.final_norm]
         return (len(self.layers) > 0 and d in NORM_WIDTHS
                 and all(layer._can_fuse(x, valid_token_mask, valid_len) for layer in self.layers)
-                and all(type(n) is nn.LayerNorm and n.elementwise_affine and n.bias is not None
+                and all(type(n) in NORM_TYPES and n.elementwise_affine and n.bias is not None
                         and n.weight.dtype == torch.float32 for n in norms))
 
     def _forward_layers_fused(self, x, valid_token_mask, valid_len, operands="fp32"):

@@ -1,0 +1,371 @@
+"""Differential attention as programs call it: strides, streams, graphs, odd numbers (GPU)."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from differential_reference import assert_within, attention
+from test_differential_gpu import FLOOR, TYPES, heads, inputs, lengths_of
+
+pytestmark = pytest.mark.gpu
+
+
+def test_any_strides_give_the_same_bits(cuda):
+    """Head-major, token-major, misaligned and gapped tensors of the same values."""
+    from techjam_amd.kernels import differential_attention
+
+    q, k, v, lam, dout = inputs(torch.float16, 2, 2, 1, 100, 64, 128)
+
+    def run(*ts):
+        leaves = [t.detach().requires_grad_() for t in ts[:3]]
+        out = differential_attention(*leaves, lam, is_causal=True)
+        return (out, *torch.autograd.grad(out, leaves, ts[3]))
+
+    def shifted(t):  # rows that start 2 bytes past an aligned address
+        flat = torch.zeros(t.numel() + 1, dtype=t.dtype, device=t.device)
+        flat[1:] = t.reshape(-1)
+        return flat[1:].view(t.shape)
+
+    def gapped(t):
+        wide = torch.full((*t.shape[:3], t.shape[3] + 24), float("nan"), dtype=t.dtype, device=t.device)
+        wide[..., :t.shape[3]] = t
+        return wide[..., :t.shape[3]]
+
+    def by_column(t):  # innermost stride other than 1
+        return t.transpose(2, 3).contiguous().transpose(2, 3)
+
+    want = run(q, k, v, dout)
+    for change in (torch.Tensor.contiguous, shifted, gapped, by_column):
+        for got, w in zip(run(*(change(t) for t in (q, k, v, dout))), want):
+            assert torch.equal(got, w), change
+
+
+def test_broadcast_inputs_and_gradients(cuda):
+    """Keys shared by the batch through expand, and a gradient of one value."""
+    from techjam_amd.kernels import differential_attention
+
+    q, k, v, lam, _ = inputs(torch.float32, 3, 2, 2, 40, 32, 64)
+    k1, v1 = k[:1], v[:1]
+    leaves = [t.detach().requires_grad_() for t in (q, k1, v1, lam)]
+    out = differential_attention(leaves[0], leaves[1].expand(3, -1, -1, -1), leaves[2].expand(3, -1, -1, -1), leaves[3])
+    grads = torch.autograd.grad(out.sum(), leaves)
+    want = attention(q, k1.expand(3, -1, -1, -1), v1.expand(3, -1, -1, -1), lam, causal=False, dout=torch.ones_like(out))
+    assert_within(grads[0], want["dq"], "dq", 1e-40)
+    # The sum over the batch adds three rounded gradients.
+    for got, name in ((grads[1], "dk"), (grads[2], "dv")):
+        value, bound = (x.sum(0, keepdim=True) for x in want[name])
+        assert_within(got, (value, bound + 3 * 2.0 ** -24 * want[name][0].abs().sum(0, keepdim=True)), name)
+    assert_within(grads[3], want["dlam"], "dlam", 1e-40)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("scale", [0.0, -0.3, 1.7])
+def test_scales(cuda, scale, dtype):
+    from techjam_amd.kernels import differential_attention
+
+    q, k, v, lam, dout = inputs(TYPES[dtype], 1, 2, 1, 70, 32, 64, seed=5)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v, lam)]
+    out = differential_attention(*leaves, is_causal=True, scale=scale)
+    grads = torch.autograd.grad(out, leaves, dout)
+    want = attention(q, k, v, lam, causal=True, scale=scale, dout=dout)
+    for name, got in zip(("out", "dq", "dk", "dv", "dlam"), (out, *grads)):
+        assert_within(got, want[name], name, FLOOR[q.dtype] if name != "dlam" else 1e-30)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("weights", [(0.0, 1.0), (-2.5, 40.0)])
+def test_weights_of_any_size(cuda, weights, dtype):
+    from techjam_amd.kernels import differential_attention
+
+    q, k, v, _, dout = inputs(TYPES[dtype], 1, 2, 1, 70, 32, 64, seed=6)
+    lam = torch.tensor(weights, device="cuda")
+    leaves = [t.detach().requires_grad_() for t in (q, k, v, lam)]
+    out = differential_attention(*leaves)
+    grads = torch.autograd.grad(out, leaves, dout)
+    want = attention(q, k, v, lam, causal=False, dout=dout)
+    for name, got in zip(("out", "dq", "dk", "dv", "dlam"), (out, *grads)):
+        assert_within(got, want[name], name, FLOOR[q.dtype] if name != "dlam" else 1e-30)
+
+
+@pytest.mark.parametrize("size", [1e-6, 3e3])
+def test_small_and_large_fp16_gradients(cuda, size):
+    """dS of long rows lies below fp16's normal numbers, or above its largest, unless it is lifted."""
+    from techjam_amd.kernels import differential_attention
+
+    q, k, v, lam, dout = inputs(torch.float16, 1, 1, 1, 600, 64, 128, seed=7)
+    dout = (dout.float() * size).half()
+    leaves = [t.detach().requires_grad_() for t in (q, k, v, lam)]
+    out = differential_attention(*leaves)
+    grads = torch.autograd.grad(out, leaves, dout)
+    want = attention(q, k, v, lam, causal=False, dout=dout)
+    for name, got in zip(("dq", "dk", "dv", "dlam"), grads):
+        assert_within(got, want[name], name, 2.0 ** -25 if name != "dlam" else 1e-30)
+
+
+def test_sharp_rows(cuda):
+    """Scores of hundreds: one key takes a row, and the maximum moves many times."""
+    from techjam_amd.kernels import differential_attention
+
+    g = torch.Generator().manual_seed(8)
+    for dtype in TYPES.values():
+        q, k, v = heads(g, 1, 2, 300, 64, dtype, 8.0), heads(g, 1, 2, 300, 64, dtype, 8.0), heads(g, 1, 1, 300, 128, dtype)
+        k = (k.float() * torch.linspace(0.1, 2, 300, device="cuda")[:, None]).to(dtype)
+        lam = torch.tensor([0.5], device="cuda")
+        with torch.no_grad():
+            out = differential_attention(q, k, v, lam, is_causal=True)
+        assert_within(out, attention(q, k, v, lam, causal=True)["out"], "out", FLOOR[dtype])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_not_a_number_stays_in_its_rows(cuda, dtype):
+    """A NaN query spoils its row; a NaN value spoils the rows that see it and, as 0
+    times NaN, those before it in its tile of 32 tokens (the plain product of a
+    masked map spoils every row); other rows and heads keep their bits."""
+    from techjam_amd.kernels import differential_attention
+
+    q, k, v, lam, dout = inputs(TYPES[dtype], 1, 2, 2, 100, 32, 64, seed=9)
+    with torch.no_grad():
+        clean = differential_attention(q, k, v, lam, is_causal=True)
+    bad = q.clone()
+    bad[0, 1, 40, 3] = float("nan")
+    leaves = [t.detach().requires_grad_() for t in (bad, k, v, lam)]
+    out = differential_attention(*leaves, is_causal=True)
+    assert bool(out[0, 0, 40].isnan().all())
+    keep = torch.ones(1, 2, 100, dtype=torch.bool, device="cuda")
+    keep[0, 0, 40] = False
+    assert torch.equal(out[keep], clean[keep])
+    dq = torch.autograd.grad(out, leaves, dout)[0]
+    assert bool(dq[0, 1, 40].isnan().any()) and bool(dq[0, 2:].isfinite().all())
+    assert bool(dq[0, :2, :40].isfinite().all()) and bool(dq[0, :2, 41:].isfinite().all())
+    bad = v.clone()
+    bad[0, 1, 60] = float("nan")
+    with torch.no_grad():
+        out = differential_attention(q, k, bad, lam, is_causal=True)
+    assert torch.equal(out[0, 0], clean[0, 0]) and torch.equal(out[0, 1, :32], clean[0, 1, :32])
+    assert bool(out[0, 1, 60:].isnan().all())
+
+
+def test_equal_calls_give_equal_bits(cuda):
+    from techjam_amd.kernels import differential_attention
+
+    q, k, v, lam, dout = inputs(torch.bfloat16, 2, 6, 2, 333, 64, 128, seed=10, shared=True)
+
+    def run():
+        leaves = [t.detach().requires_grad_() for t in (q, k, v, lam)]
+        out = differential_attention(*leaves, is_causal=True)
+        return (out, *torch.autograd.grad(out, leaves, dout))
+
+    first = run()
+    for _ in range(3):
+        for a, b in zip(run(), first):
+            assert torch.equal(a, b)
+
+
+def test_two_streams_at_once(cuda):
+    from techjam_amd.kernels import differential_attention, differential_attention_cached
+
+    cases = [inputs(torch.float16, 2, 4, 2, 500, 64, 128, seed=s) for s in (11, 12)]
+    lengths = lengths_of(500, 123)
+
+    def run(q, k, v, lam, dout):
+        leaves = [t.detach().requires_grad_() for t in (q, k, v, lam)]
+        out = differential_attention(*leaves, is_causal=True, valid_len=lengths)
+        new = differential_attention_cached(q[:, :, -1:], k, v, lam, lengths)
+        return (out, new, *torch.autograd.grad(out, leaves, dout))
+
+    want = [run(*c) for c in cases]
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(3):
+        torch.cuda.synchronize()
+        got = []
+        for c, s in zip(cases, streams):
+            with torch.cuda.stream(s):
+                got.append(run(*c))
+        torch.cuda.synchronize()
+        for a, b in zip(got, want):
+            for x, y in zip(a, b):
+                assert torch.equal(x, y)
+
+
+def test_forward_and_cached_replay_in_graphs(cuda):
+    """Two captured graphs with other work between the replays, new inputs each time."""
+    from techjam_amd.kernels import differential_attention, differential_attention_cached
+
+    q, k, v, lam, _ = inputs(torch.bfloat16, 2, 4, 2, 700, 64, 128, seed=13)
+    lengths = lengths_of(700, 80)
+    q1 = q[:, :, :1].contiguous()
+    calls = (lambda: differential_attention(q, k, v, lam, is_causal=True, valid_len=lengths),
+             lambda: differential_attention_cached(q1, k, v, lam, lengths))
+    graphs = []
+    with torch.no_grad():
+        for call in calls:
+            side = torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):
+                call()
+            torch.cuda.current_stream().wait_stream(side)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                out = call()
+            graphs.append((graph, out))
+        for i in range(4):
+            g = torch.Generator(device="cuda").manual_seed(20 + i)
+            for t in (q, k, v, q1):
+                t.normal_(generator=g)
+            lengths.copy_(lengths_of(700 - 100 * i, 80 + 7 * i))
+            for graph, _ in graphs:
+                graph.replay()
+            got = [out.clone() for _, out in graphs]
+            for x, call in zip(got, calls):
+                assert torch.equal(x, call())
+            torch.cuda.synchronize()
+
+
+def test_training_step_replays_in_a_graph(cuda):
+    from techjam_amd.kernels import differential_attention
+
+    q, k, v, lam, dout = inputs(torch.float16, 2, 2, 1, 150, 64, 128, seed=14)
+    leaves = [t.detach().clone().requires_grad_() for t in (q, k, v, lam)]
+
+    def step():
+        out = differential_attention(*leaves, is_causal=True)
+        return (out.detach(), *torch.autograd.grad(out, leaves, dout))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for i in range(4):
+        g = torch.Generator(device="cuda").manual_seed(30 + i)
+        with torch.no_grad():
+            for t in (*leaves[:3], dout):
+                t.normal_(generator=g)
+        graph.replay()
+        got = [t.clone() for t in held]
+        for a, b in zip(got, step()):
+            assert torch.equal(a, b)
+        torch.cuda.synchronize()
+
+
+def test_rows_past_four_gibibytes(cuda):
+    """Keys whose rows are 32 KiB apart: 64-bit offsets, the same bits as a compact copy."""
+    from techjam_amd.kernels import differential_attention_cached
+
+    tokens, row = 140000, 16384
+    store = torch.empty(tokens, row, dtype=torch.bfloat16, device="cuda")
+    g = torch.Generator(device="cuda").manual_seed(15)
+    store[:, :256] = torch.randn(tokens, 256, generator=g, device="cuda").bfloat16()
+    k = store[:, :128].view(1, tokens, 2, 64).transpose(1, 2)
+    v = store[:, 128:256].view(1, tokens, 1, 128).transpose(1, 2)
+    assert (tokens - 1) * row * 2 > 1 << 32
+    q = torch.randn(1, 2, 1, 64, generator=g, device="cuda").bfloat16()
+    lam = torch.tensor([0.4], device="cuda")
+    lengths = lengths_of(tokens - 3)
+    got = differential_attention_cached(q, k, v, lam, lengths)
+    assert torch.equal(got, differential_attention_cached(q, k.contiguous(), v.contiguous(), lam, lengths))
+
+
+def test_cached_follows_the_whole_sequence(cuda):
+    """Each new token's output is its row of the whole causal sequence's."""
+    from techjam_amd.kernels import differential_attention, differential_attention_cached
+
+    for dtype in TYPES.values():
+        q, k, v, lam, _ = inputs(dtype, 2, 4, 2, 96, 64, 128, seed=16)
+        want = attention(q, k, v, lam, causal=True)["out"]
+        with torch.no_grad():
+            whole = differential_attention(q, k, v, lam, is_causal=True)
+        assert_within(whole, want, "whole", FLOOR[dtype])
+        for n, new in ((1, 1), (33, 1), (64, 3), (96, 96)):
+            got = differential_attention_cached(q[:, :, n - new:n], k, v, lam, lengths_of(n, n))
+            at = slice(n - new, n)
+            assert_within(got, (want[0][:, :, at], want[1][:, :, at]), f"{new} at {n}", FLOOR[dtype])
+
+
+def test_gradient_is_the_slope(cuda):
+    """Central differences of the float32 kernel along random directions."""
+    from techjam_amd.kernels import differential_attention
+
+    q, k, v, lam, dout = inputs(torch.float32, 1, 2, 1, 40, 32, 64, seed=17)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v, lam)]
+    out = differential_attention(*leaves, is_causal=True)
+    grads = torch.autograd.grad(out, leaves, dout)
+    eps = 2.0 ** -6
+    g = torch.Generator(device="cuda").manual_seed(18)
+    for i, name in enumerate(("q", "k", "v", "lam")):
+        d = torch.randn(leaves[i].shape, generator=g, device="cuda")
+
+        def value(sign, exact):
+            moved = [t.detach() for t in leaves]
+            moved[i] = moved[i] + sign * eps * d
+            if exact:
+                val, bound = attention(*moved, causal=True)["out"]
+            else:
+                with torch.no_grad():
+                    val, bound = differential_attention(*moved, is_causal=True).cpu().double(), torch.zeros(())
+            w = dout.cpu().double()
+            return (val * w).sum(), (bound * w.abs()).sum()
+
+        up, down = value(1, False)[0], value(-1, False)[0]
+        (eu, bu), (ed, bd) = value(1, True), value(-1, True)
+        slope = float((grads[i].double() * d.double()).sum())
+        # What the difference of the exact values misses of the slope, twice (the
+        # kernel's inputs are the same), and both values' rounding bounds.
+        exact_grad = attention(*leaves, causal=True, dout=dout)["d" + name]
+        want = float((exact_grad[0] * d.cpu().double()).sum())
+        missed = abs(float((eu - ed) / (2 * eps)) - want)
+        allowed = missed + float((bu + bd) / (2 * eps)) + float((exact_grad[1] * d.cpu().double().abs()).sum())
+        assert abs(float((up - down) / (2 * eps)) - slope) <= allowed, name
+        assert missed < 0.05 * abs(want) + 0.05, name  # the check says something
+
+
+def test_gradients_of_some_inputs_and_second_derivatives(cuda):
+    from techjam_amd.kernels import differential_attention
+
+    q, k, v, lam, dout = inputs(torch.float32, 1, 2, 1, 20, 32, 64, seed=19)
+    qr = q.detach().requires_grad_()
+    out = differential_attention(qr, k, v, lam, is_causal=True)
+    (dq,) = torch.autograd.grad(out, qr, dout, create_graph=True)
+    assert_within(dq, attention(q, k, v, lam, causal=True, dout=dout)["dq"], "dq", 1e-40)
+    with pytest.raises(RuntimeError):
+        dq.sum().backward()
+
+
+def test_refusals_on_the_gpu(cuda):
+    from techjam_amd import UnsupportedCaseError
+    from techjam_amd.kernels import differential_attention, differential_attention_cached
+
+    q, k, v, lam, _ = inputs(torch.float32, 2, 2, 1, 20, 32, 64)
+    lens = lengths_of(20, 20)
+    for bad in (lens.long(), lens[:1], lens.cpu(), torch.stack([lens, lens], 1)[:, 0]):
+        with pytest.raises(ValueError):
+            differential_attention(q, k, v, lam, valid_len=bad)
+        with pytest.raises(ValueError):
+            differential_attention_cached(q, k, v, lam, bad)
+    with pytest.raises(ValueError):
+        differential_attention(q, k, v, lam.cpu())
+    with pytest.raises(ValueError):
+        differential_attention(q, k, v, lam, scale=float("nan"))
+    with pytest.raises(UnsupportedCaseError):
+        differential_attention_cached(q.requires_grad_(), k, v, lam, lens)
+
+
+def test_empty_batches(cuda):
+    from techjam_amd.kernels import differential_attention, differential_attention_cached
+
+    lam = torch.ones(2, device="cuda", requires_grad=True)
+    for b, s in ((0, 8), (2, 0)):
+        q, k, v = (torch.zeros(b, h, s, d, device="cuda", requires_grad=True) for h, d in ((4, 32), (4, 32), (2, 64)))
+        out = differential_attention(q, k, v, lam)
+        assert out.shape == (b, 2, s, 64)
+        grads = torch.autograd.grad(out.sum(), (q, k, v, lam))
+        assert float(grads[3].abs().sum()) == 0
+    with torch.no_grad():
+        out = differential_attention_cached(torch.zeros(1, 4, 1, 32, device="cuda"), torch.zeros(1, 4, 0, 32, device="cuda"),
+                                            torch.zeros(1, 2, 0, 64, device="cuda"), lam, lengths_of(0))
+    assert out.shape == (1, 2, 1, 64) and float(out.abs().sum()) == 0
