@@ -193,7 +193,7 @@ def _run_own(state):
     kind = case["kind"]
     if kind == "norm":
         with torch.no_grad():
-            return layer_norm(state["x"], state["weight"], state["bias"])
+            return layer_norm(state["x"], state["weight"], state["bias"], norm_dtype=torch.float32)
     if kind == "norm_train":
         leaves = [state[n] for n in ("x", "weight", "bias") if state[n] is not None]
         out = layer_norm(state["x"], state["weight"], state["bias"])
