@@ -443,7 +443,8 @@ int tj_diff_attn_bwd(const void* q, const void* k, const void* v, const float* m
  * the last dimension, torch_transformer_benchmark.py:125-172, where the norms
  * are torch's):
  *   y = (x - mean) * rstd * weight + bias,  rstd = 1 / sqrt(var + eps)
- * x, y, dy, dx: [rows, cols] of dtype (TJ_F32, TJ_F16 or TJ_BF16), unit column
+ * x, dx: [rows, cols] of dtype (TJ_F32, TJ_F16 or TJ_BF16), y, dy of y_dtype
+ * (dtype or TJ_F32: the norm not rounded to 16 bits), unit column
  * stride, aligned to one element, any row stride >= 0 (in elements; 32 rows
  * within 2 GiB, TJ_ERR_UNSUPPORTED otherwise). weight, bias
  * and their gradients: [cols] of w_dtype, TJ_F32 or dtype; each may be NULL
@@ -454,12 +455,13 @@ int tj_diff_attn_bwd(const void* q, const void* k, const void* v, const float* m
  * bytes of workspace (4-byte aligned, contents irrelevant). With no rows nothing
  * is written. y may not overlap x, nor dx any input.
  */
-int tj_layer_norm_fwd(const void* x, const void* weight, const void* bias, void* y, int dtype, int w_dtype,
-                      int64_t rows, int64_t cols, int64_t x_stride, int64_t y_stride, float eps,
+int tj_layer_norm_fwd(const void* x, const void* weight, const void* bias, void* y, int dtype, int y_dtype,
+                      int w_dtype, int64_t rows, int64_t cols, int64_t x_stride, int64_t y_stride, float eps,
                       float* mean, float* rstd, hipStream_t stream);
 size_t tj_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t cols);
 int tj_layer_norm_bwd(const void* dy, const void* x, const void* weight, const float* mean, const float* rstd,
-                      void* dx, void* dweight, void* dbias, int dtype, int w_dtype, int64_t rows, int64_t cols,
+                      void* dx, void* dweight, void* dbias, int dtype, int y_dtype, int w_dtype,
+                      int64_t rows, int64_t cols,
                       int64_t dy_stride, int64_t x_stride, int64_t dx_stride,
                       void* workspace, size_t workspace_bytes, hipStream_t stream);
 

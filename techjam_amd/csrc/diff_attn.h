@@ -23,7 +23,6 @@
 
 typedef __bf16 bf16_t;
 typedef __bf16 bf16x4_t __attribute__((ext_vector_type(4)));
-typedef float float2_t __attribute__((ext_vector_type(2)));
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 
 namespace tj {
@@ -45,7 +44,7 @@ struct DiffArgs {
   float* lse;              // [B, H, 2, Sq] log2 of a row's sum of 2^(score log2 e), +inf for empty rows; or null
   int n_mtiles;
   // Key parts: part p covers keys p part_keys .. (p + 1) part_keys - 1 and leaves unnormalised sums
-  // [n_parts, B, Hk, R, 2, Dv] and (maximum, sum) pairs [n_parts, B, Hk, R, 2, 2].
+  // [n_parts, B, Hk, R, 2, Dv] and (maximum, sum, sum before rounding, -) [n_parts, B, Hk, R, 2, 4].
   int part_keys, n_parts;
   float *part_o, *part_ml;
   // Backward.

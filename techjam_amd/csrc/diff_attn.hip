@@ -46,7 +46,7 @@ DiffPlan plan(int64_t B, int64_t Hk, int64_t R, int64_t Sk, bool cached) {
 size_t part_bytes(const DiffPlan& p, int64_t B, int64_t Hk, int64_t R, int64_t Dv) {
   if (!p.few && p.n_parts <= 1) return 0;
   const size_t rows = size_t(p.n_parts) * size_t(B) * size_t(Hk) * size_t(R) * 2;
-  return (rows * size_t(Dv) + rows * 2) * sizeof(float);
+  return (rows * size_t(Dv) + rows * 4) * sizeof(float);
 }
 
 // Sizes that the kernels' 32-bit row and key numbers and the grids hold.
@@ -183,6 +183,7 @@ extern "C" int tj_diff_attn_bwd(const void* q, const void* k, const void* v, con
   const int64_t blocks = ((int64_t)a.R + 63) / 64;
   a.n_peaks = (int)(blocks < kPeakParts ? blocks : kPeakParts);
   if (const int rc = diff_delta(a, dtype, stream)) return rc;
-  if (const int rc = diff_bwd_kv(a, dtype, stream)) return rc;
-  return diff_bwd_q(a, dtype, stream);
+  // dQ first: it leaves the exact delta for dK.
+  if (const int rc = diff_bwd_q(a, dtype, stream)) return rc;
+  return diff_bwd_kv(a, dtype, stream);
 }

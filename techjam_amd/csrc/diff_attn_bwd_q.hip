@@ -9,8 +9,9 @@
 // rounded to 16 bits they cost dQ and dK a twentieth of their accuracy (bf16,
 // causal, 1024 tokens, 64 dims: 2.56e-3 instead of 2.40e-3, relative 2-norm; the
 // rounding of dS and of the result is 2.38e-3). What is left of its error is the
-// rounding of P in the forward product: the sum of P_1 (dP - delta_1) over the
-// keys (P_1 sums to 1), which dlam adds back and so is as exact as fp32 sums are.
+// rounding of P in the forward product: the sum of P_m (dP - delta_m) over the
+// keys (P_m sums to 1). The dQ kernel adds it back to delta, exact then to what
+// fp32 sums are, for dlam and for dK, which come after it.
 #include "diff_attn.h"
 
 namespace tj {
@@ -108,7 +109,7 @@ diff_bwd_q_kernel(DiffArgs a) {
   constexpr int kBytes = SH::kBytes, kHead = SH::kHead;
   using KT = LdsRows<T, HD>;
   using VT = LdsRows<T, DVP>;
-  constexpr int kSums = KG > 1 ? KG / 2 * RB * (2 * DB * 16 + 1) * kWave * 4 : 0;
+  constexpr int kSums = KG > 1 ? KG / 2 * RB * (2 * DB * 16 + 2) * kWave * 4 : 0;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[KG * 2 * kBytes > kSums ? KG * 2 * kBytes : kSums];
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave, hl = lane / 32,
             ln = lane % 32;
@@ -167,7 +168,7 @@ diff_bwd_q_kernel(DiffArgs a) {
     del[c] = live ? a.delta[map_at(a, t.b, head, c, i)] : 0.f;
   }
   const float d0 = -del[0] * lift, nl = -lam * lift;
-  float rest = 0.f;
+  float rest[2] = {0.f, 0.f};
 
   // The workgroup goes round together, the last round maybe without a tile for every group.
   for (int first = 0, cur = 0; first < kv_end; first += KG * BN, kv0 += KG * BN, cur ^= 1) {
@@ -198,8 +199,9 @@ diff_bwd_q_kernel(DiffArgs a) {
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
       p[0][e] *= fmaf(dp[e], lift, d0);
+      rest[0] += p[0][e];
       const float u = p[1][e] * (dp[e] - del[1]);
-      rest += u;
+      rest[1] += u;
       p[1][e] = u * nl;
     }
 #pragma unroll
@@ -218,10 +220,11 @@ diff_bwd_q_kernel(DiffArgs a) {
   for (int half = KG / 2; half > 0; half /= 2) {
     const int at = (kg % half) * RB + rb;
     float4_t* x = reinterpret_cast<float4_t*>(smem) + at * 2 * DB * 4 * kWave;
-    float* y = reinterpret_cast<float*>(smem) + half * RB * 2 * DB * 16 * kWave + at * kWave;
+    float* y = reinterpret_cast<float*>(smem) + half * RB * 2 * DB * 16 * kWave + at * 2 * kWave;
     __syncthreads();
     if (kg >= half && kg < 2 * half) {
-      y[lane] = rest;
+      y[lane] = rest[0];
+      y[kWave + lane] = rest[1];
 #pragma unroll
       for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -233,7 +236,8 @@ diff_bwd_q_kernel(DiffArgs a) {
     }
     __syncthreads();
     if (kg < half) {
-      rest += y[lane];
+      rest[0] += y[lane];
+      rest[1] += y[kWave + lane];
 #pragma unroll
       for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -248,9 +252,14 @@ diff_bwd_q_kernel(DiffArgs a) {
   }
   if (kg != 0) return;
 
-  rest = pair_sum(rest);
+  rest[0] = pair_sum(rest[0]) / lift;
+  rest[1] = pair_sum(rest[1]);
   if (r >= a.R) return;
-  if (hl == 0) a.gsum[row_at(a, t.b, head, i)] = live ? del[1] + rest : 0.f;
+  if (hl == 0) {
+    a.gsum[row_at(a, t.b, head, i)] = live ? del[1] + rest[1] : 0.f;
+#pragma unroll
+    for (int c = 0; c < 2; ++c) a.delta[map_at(a, t.b, head, c, i)] = live ? del[c] + rest[c] : 0.f;
+  }
   const float out = a.scale / lift;
 #pragma unroll
   for (int c = 0; c < 2; ++c) {

@@ -57,12 +57,17 @@ struct DiffSpan {
 // The running state of a wave's 32 rows, for NM maps from map `first` on: both,
 // or one where two accumulators of the width exceed a wave's registers (a pair
 // of waves then shares the rows and the key tiles).
-template <typename T, int HD, int BN, int NM>
+// The output is divided by the sum of the probabilities as they were rounded for
+// its product: a dominant key's rounding cancels, and two go into one
+// instruction. What the backward pass gets (STATS) is the sum of the unrounded
+// ones, so that its P sums to 1 as exactly as fp32 does.
+template <typename T, int HD, int BN, int NM, bool STATS>
 struct FwdState {
   using SH = FwdShape<T, HD, BN>;
   frag_t<T> q[NM][SH::KS];
   float16_t o[NM][SH::DB];
   float m[NM], l[NM];  // maximum in log2 units, the lane's part of the sum
+  float e[STATS ? NM : 1];
   float c2;            // |scale| log2 e
   int first;
   uint32_t kbase, vbase;  // the lane's places in a key tile
@@ -87,6 +92,7 @@ struct FwdState {
       }
       m[c] = -__builtin_inff();
       l[c] = 0.f;
+      if constexpr (STATS) e[c] = 0.f;
 #pragma unroll
       for (int d = 0; d < SH::DB; ++d) o[c][d] = zero16();
     }
@@ -122,6 +128,7 @@ struct FwdState {
         const float alpha = m[c] == -__builtin_inff() ? 0.f : fast_exp2(m[c] - to);
         m[c] = to;
         l[c] *= alpha;
+        if constexpr (STATS) e[c] *= alpha;
 #pragma unroll
         for (int d = 0; d < SH::DB; ++d)
 #pragma unroll
@@ -130,9 +137,10 @@ struct FwdState {
       // A row that has seen no key keeps its unset maximum out of the exponent.
       const float off = m[c] == -__builtin_inff() ? 0.f : Elem<T>::kLift - m[c];
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = fast_exp2(fmaf(s[r], c2, off));
-      // The sum takes the rounded values, as the product does: a dominant key's
-      // rounding cancels, and two values go into one instruction.
+      for (int r = 0; r < 16; ++r) {
+        s[r] = fast_exp2(fmaf(s[r], c2, off));
+        if constexpr (STATS) e[c] += s[r];
+      }
 #pragma unroll
       for (int st = 0; st < 2; ++st) {
         p[c][st] = acc_frag<T>(s, st);
@@ -152,11 +160,13 @@ struct FwdState {
   // Adds the state of another group's wave over the same rows and other keys,
   // which that wave has left in LDS (give).
   static constexpr int kGive = SH::DB * 4 * kWave;  // float4 per map
+  static constexpr int kMl = STATS ? 3 : 2;         // numbers of a lane and map beside them
   __device__ __forceinline__ void give(float4_t* x, float* ml, int lane) {
 #pragma unroll
     for (int c = 0; c < NM; ++c) {
-      ml[(2 * c) * kWave + lane] = m[c];
-      ml[(2 * c + 1) * kWave + lane] = l[c];
+      ml[(kMl * c) * kWave + lane] = m[c];
+      ml[(kMl * c + 1) * kWave + lane] = l[c];
+      if constexpr (STATS) ml[(kMl * c + 2) * kWave + lane] = e[c];
 #pragma unroll
       for (int d = 0; d < SH::DB; ++d)
 #pragma unroll
@@ -168,12 +178,13 @@ struct FwdState {
   __device__ __forceinline__ void take(const float4_t* x, const float* ml, int lane) {
 #pragma unroll
     for (int c = 0; c < NM; ++c) {
-      const float m1 = ml[(2 * c) * kWave + lane], to = fmaxf(m[c], m1);
+      const float m1 = ml[(kMl * c) * kWave + lane], to = fmaxf(m[c], m1);
       // An unset maximum (-inf) goes with sums that are zero, or NaN and kept.
       const float w0 = m[c] == -__builtin_inff() ? 1.f : fast_exp2(m[c] - to);
       const float w1 = m1 == -__builtin_inff() ? 1.f : fast_exp2(m1 - to);
       m[c] = to;
-      l[c] = fmaf(l[c], w0, ml[(2 * c + 1) * kWave + lane] * w1);
+      l[c] = fmaf(l[c], w0, ml[(kMl * c + 1) * kWave + lane] * w1);
+      if constexpr (STATS) e[c] = fmaf(e[c], w0, ml[(kMl * c + 2) * kWave + lane] * w1);
 #pragma unroll
       for (int d = 0; d < SH::DB; ++d)
 #pragma unroll
@@ -191,7 +202,7 @@ struct FwdState {
     const int64_t slot = ((int64_t)part * a.B * a.Hk + bh) * a.R + row.r;
 #pragma unroll
     for (int c = 0; c < NM; ++c) {
-      const float sum = pair_sum(l[c]);
+      const float sum = pair_sum(l[c]), exact = STATS ? pair_sum(e[STATS ? c : 0]) : 0.f;
       if (!row.live) continue;
       float* po = a.part_o + (slot * 2 + first + c) * a.Dv;
 #pragma unroll
@@ -202,8 +213,7 @@ struct FwdState {
           if (col < a.Dv) store4t<float>(po + col, o[c][d][4 * e], o[c][d][4 * e + 1], o[c][d][4 * e + 2], o[c][d][4 * e + 3]);
         }
       if (hl == 0) {
-        a.part_ml[(slot * 2 + first + c) * 2] = m[c];
-        a.part_ml[(slot * 2 + first + c) * 2 + 1] = sum;
+        *reinterpret_cast<float4_t*>(a.part_ml + (slot * 2 + first + c) * 4) = float4_t{m[c], sum, exact, 0.f};
       }
     }
   }
@@ -214,12 +224,15 @@ struct FwdState {
   __device__ __forceinline__ void finish(const DiffArgs& a, int b, int hk, const DiffRow& row, float4_t* swap, int lane, bool mine) {
     const int hl = lane / 32, head = hk * a.G + row.g;
     const bool in = mine && row.r < a.R;
-    float* mp = a.maps != nullptr && in ? a.maps + row_at(a, b, head, row.i) * 2 * a.Dv : nullptr;
+    float* mp = STATS && a.maps != nullptr && in ? a.maps + row_at(a, b, head, row.i) * 2 * a.Dv : nullptr;
 #pragma unroll
     for (int c = 0; c < NM; ++c) {
       const float sum = pair_sum(l[c]), inv = 1.f / sum;
-      if (a.lse != nullptr && in && hl == 0)
-        a.lse[map_at(a, b, head, first + c, row.i)] = row.live ? m[c] - Elem<T>::kLift + log2f(sum) : __builtin_inff();
+      if constexpr (STATS) {
+        const float exact = pair_sum(e[c]);
+        if (a.lse != nullptr && in && hl == 0)
+          a.lse[map_at(a, b, head, first + c, row.i)] = row.live ? m[c] - Elem<T>::kLift + log2f(exact) : __builtin_inff();
+      }
 #pragma unroll
       for (int d = 0; d < SH::DB; ++d)
 #pragma unroll
@@ -300,18 +313,18 @@ struct FwdGroups {
   static constexpr int BN = KG == 1 && HD * (int)sizeof(T) <= 256 ? 64 : 32;
 };
 
-template <typename T, int HD, bool WIDE, bool PART>
+template <typename T, int HD, bool WIDE, bool PART, bool STATS>
 __global__ __launch_bounds__((64 * FwdGroups<T, HD, WIDE>::WAVES), (sizeof(T) == 4 && HD == 64 ? 1 : 2)) void
 diff_fwd_kernel(DiffArgs a) {
   using GR = FwdGroups<T, HD, WIDE>;
   constexpr int BN = GR::BN;
   using SH = FwdShape<T, HD, BN>;
-  using State = FwdState<T, HD, BN, kMaps<HD>>;
+  using State = FwdState<T, HD, BN, kMaps<HD>, STATS>;
   constexpr int NM = kMaps<HD>, RB = GR::RB, KG = GR::KG, ROWS = 32 * RB;
   // Two tiles a group; afterwards the groups' results, then the second map's.
   constexpr int kSums = 16 * State::kGive * RB * (KG > 1 && KG * GR::kPairs * NM / 2 > 1 ? KG * GR::kPairs * NM / 2 : 1);
   __shared__ __attribute__((aligned(1024))) unsigned char smem[KG * 2 * SH::kBytes > kSums ? KG * 2 * SH::kBytes : kSums];
-  __shared__ float ml[KG > 1 ? KG / 2 * RB * GR::kPairs * NM * 2 * kWave : 1];
+  __shared__ float ml[KG > 1 ? KG / 2 * RB * GR::kPairs * NM * State::kMl * kWave : 1];
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
   const int kg = w / (RB * GR::kPairs), in_group = w % (RB * GR::kPairs), rb = in_group % RB, map = in_group / RB;
   const DiffTile t = diff_tile(a, blockIdx.x, a.n_mtiles);
@@ -349,9 +362,9 @@ diff_fwd_kernel(DiffArgs a) {
     float4_t* x = reinterpret_cast<float4_t*>(smem);
     const int at = (kg % half) * RB * GR::kPairs + in_group;
     __syncthreads();
-    if (kg >= half && kg < 2 * half) st.give(x + at * NM * State::kGive, ml + at * NM * 2 * kWave, lane);
+    if (kg >= half && kg < 2 * half) st.give(x + at * NM * State::kGive, ml + at * NM * State::kMl * kWave, lane);
     __syncthreads();
-    if (kg < half) st.take(x + at * NM * State::kGive, ml + at * NM * 2 * kWave, lane);
+    if (kg < half) st.take(x + at * NM * State::kGive, ml + at * NM * State::kMl * kWave, lane);
   }
   if constexpr (NM == 2) {
     if (kg != 0) return;
@@ -380,7 +393,7 @@ __global__ __launch_bounds__(2 * kWave / kMaps<HD>) void diff_few_kernel(DiffArg
   KeyTiles<T, SH, HD, 2 / NM> keys;
   keys.init(a, t.b, t.hk, w, lane);
   keys.issue(a, kv_begin, L, tiles, w);
-  FwdState<T, HD, BN, NM> st;
+  FwdState<T, HD, BN, NM, false> st;
   st.init(a, t.b, t.hk, row, w, lane);
   int cur = 0;
   for (int kv0 = kv_begin; kv0 < kv_end; kv0 += BN, cur ^= 1) {
@@ -401,14 +414,14 @@ __global__ __launch_bounds__(2 * kWave / kMaps<HD>) void diff_few_kernel(DiffArg
 template <typename T>
 __global__ __launch_bounds__(kDiffThreads) void diff_join_kernel(DiffArgs a, int lanes) {
   __shared__ float4_t sum[kDiffThreads];
-  __shared__ float top[2][kDiffThreads / kWave], total[kDiffThreads];
+  __shared__ float top[2][kDiffThreads / kWave], total[2][kDiffThreads];
   const int tid = threadIdx.x;
   const int64_t n_rows = (int64_t)a.B * a.Hk * a.R, id = blockIdx.x;
   const int bh = (int)(id / a.R), b = bh / a.Hk, hk = bh % a.Hk;
   const int L = diff_len(a, b);
   const DiffRow row(a, (int)(id % a.R), L);
   const int np = row.live ? row.limit / a.part_keys + 1 : 0;
-  const float2_t* ml = reinterpret_cast<const float2_t*>(a.part_ml) + id * 2;  // part p, map c: [p * n_rows * 2 + c]
+  const float4_t* ml = reinterpret_cast<const float4_t*>(a.part_ml) + id * 2;  // part p, map c: [p * n_rows * 2 + c]
   float m[2] = {-__builtin_inff(), -__builtin_inff()};
   for (int p = tid; p < np; p += kDiffThreads)
 #pragma unroll
@@ -431,24 +444,27 @@ __global__ __launch_bounds__(kDiffThreads) void diff_join_kernel(DiffArgs a, int
   const float* po = a.part_o + id * 2 * a.Dv + (on ? chunk : 0) * 4;
   const int64_t step = n_rows * 2 * a.Dv;
   float4_t y = {0.f, 0.f, 0.f, 0.f};
-  float l = 0.f;
+  float l = 0.f, exact = 0.f;
 #pragma unroll 4
   for (int p = tid / lanes; p < np; p += kDiffThreads / lanes) {
-    const float2_t x = ml[p * n_rows * 2 + c];
+    const float4_t x = ml[p * n_rows * 2 + c];
     const float4_t o = *reinterpret_cast<const float4_t*>(po + p * step);
     // An unset maximum (-inf) goes with sums that are zero, or NaN and kept.
     const float w = x[0] == -__builtin_inff() ? 1.f : fast_exp2(x[0] - m[c]);
     l = fmaf(w, x[1], l);
+    exact = fmaf(w, x[2], exact);
 #pragma unroll
     for (int j = 0; j < 4; ++j) y[j] = fmaf(w, o[j], y[j]);
   }
   sum[tid] = y;
-  total[tid] = l;
+  total[0][tid] = l;
+  total[1][tid] = exact;
   __syncthreads();
   if (tid < lanes) {
     for (int s = tid + lanes; s < kDiffThreads; s += lanes) {
       y += sum[s];
-      l += total[s];
+      l += total[0][s];
+      exact += total[1][s];
     }
     const float inv = 1.f / l;
 #pragma unroll
@@ -457,7 +473,7 @@ __global__ __launch_bounds__(kDiffThreads) void diff_join_kernel(DiffArgs a, int
     const int head = hk * a.G + row.g;
     if (on && a.maps != nullptr) *reinterpret_cast<float4_t*>(a.maps + row_at(a, b, head, row.i) * 2 * a.Dv + chunk * 4) = y;
     if (a.lse != nullptr && (chunk == 0 || chunk == per_map))
-      a.lse[map_at(a, b, head, c, row.i)] = row.live ? m[c] - Elem<T>::kLift + log2f(l) : __builtin_inff();
+      a.lse[map_at(a, b, head, c, row.i)] = row.live ? m[c] - Elem<T>::kLift + log2f(exact) : __builtin_inff();
   }
   __syncthreads();
   if (tid < per_map) {
@@ -486,11 +502,19 @@ int launch_fwd(DiffArgs a, hipStream_t stream) {
   a.n_mtiles = (a.R + 32 * GR::RB - 1) / (32 * GR::RB);
   const int64_t n = (int64_t)a.B * a.Hk * a.n_mtiles;
   if (a.n_parts > 1) {
-    hipLaunchKernelGGL((diff_fwd_kernel<T, HD, WIDE, true>), dim3(uint32_t(n * a.n_parts)), dim3(64 * GR::WAVES), 0, stream, a);
+    hipLaunchKernelGGL((diff_fwd_kernel<T, HD, WIDE, true, true>), dim3(uint32_t(n * a.n_parts)), dim3(64 * GR::WAVES), 0,
+                       stream, a);
     const int rc = tjh::launch_status();
     return rc != TJ_OK ? rc : launch_join<T>(a, stream);
   }
-  hipLaunchKernelGGL((diff_fwd_kernel<T, HD, WIDE, false>), dim3(uint32_t(n)), dim3(64 * GR::WAVES), 0, stream, a);
+  // Without statistics the long sweeps of 128-row workgroups save the second sum.
+  if constexpr (WIDE) {
+    if (a.lse == nullptr) {
+      hipLaunchKernelGGL((diff_fwd_kernel<T, HD, WIDE, false, false>), dim3(uint32_t(n)), dim3(64 * GR::WAVES), 0, stream, a);
+      return tjh::launch_status();
+    }
+  }
+  hipLaunchKernelGGL((diff_fwd_kernel<T, HD, WIDE, false, true>), dim3(uint32_t(n)), dim3(64 * GR::WAVES), 0, stream, a);
   return tjh::launch_status();
 }
 }  // namespace

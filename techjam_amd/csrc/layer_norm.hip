@@ -43,11 +43,15 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_at(const void* p, int64_t
 // N elements of T at byte offset `at`, as fp32; zeros outside.
 template <typename T, int N>
 __device__ __forceinline__ void load_n(float (&f)[N], __amdgpu_buffer_rsrc_t r, uint32_t at) {
-  if constexpr (N * sizeof(T) == 16) {
-    typedef T vec __attribute__((ext_vector_type(N)));
-    const vec v = __builtin_bit_cast(vec, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, 0));
+  if constexpr (N * sizeof(T) >= 16) {
+    constexpr int M = 16 / (int)sizeof(T);
+    typedef T vec __attribute__((ext_vector_type(M)));
 #pragma unroll
-    for (int j = 0; j < N; ++j) f[j] = (float)v[j];
+    for (int i = 0; i < N; i += M) {
+      const vec v = __builtin_bit_cast(vec, __builtin_amdgcn_raw_buffer_load_b128(r, at + i * (uint32_t)sizeof(T), 0, 0));
+#pragma unroll
+      for (int j = 0; j < M; ++j) f[i + j] = (float)v[j];
+    }
   } else if constexpr (sizeof(T) == 4) {
     f[0] = __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(r, at, 0, 0));
   } else {
@@ -57,13 +61,17 @@ __device__ __forceinline__ void load_n(float (&f)[N], __amdgpu_buffer_rsrc_t r, 
 // The same stored, rounded to T; nothing outside.
 template <typename T, int N>
 __device__ __forceinline__ void store_n(const float (&f)[N], __amdgpu_buffer_rsrc_t r, uint32_t at) {
-  if constexpr (N * sizeof(T) == 16) {
-    typedef T vec __attribute__((ext_vector_type(N)));
+  if constexpr (N * sizeof(T) >= 16) {
+    constexpr int M = 16 / (int)sizeof(T);
+    typedef T vec __attribute__((ext_vector_type(M)));
     typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-    vec v;
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = (T)f[j];
-    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, at, 0, 0);
+    for (int i = 0; i < N; i += M) {
+      vec v;
+#pragma unroll
+      for (int j = 0; j < M; ++j) v[j] = (T)f[i + j];
+      __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, at + i * (uint32_t)sizeof(T), 0, 0);
+    }
   } else if constexpr (sizeof(T) == 4) {
     __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, f[0]), r, at, 0, 0);
   } else {
@@ -78,18 +86,8 @@ __device__ __forceinline__ void load_param(float (&f)[N], const void* p, int is_
   for (int j = 0; j < N; ++j) f[j] = none;
   if (p == nullptr) return;
   const auto r = rows_at(p, 0);
-  if (!is_f32) {
-    load_n<T, N>(f, r, col < cols ? (uint32_t)col * (uint32_t)sizeof(T) : kOutside);
-    return;
-  }
-  constexpr int M = N < 4 ? N : 4;
-#pragma unroll
-  for (int j = 0; j < N; j += M) {
-    float g[M];
-    load_n<float, M>(g, r, col < cols ? (uint32_t)(col + j) * 4u : kOutside);
-#pragma unroll
-    for (int i = 0; i < M; ++i) f[j + i] = g[i];
-  }
+  if (is_f32) load_n<float, N>(f, r, col < cols ? (uint32_t)col * 4u : kOutside);
+  else load_n<T, N>(f, r, col < cols ? (uint32_t)col * (uint32_t)sizeof(T) : kOutside);
 }
 
 // Sum over the LPR lanes of a row; every lane gets it. Rows of a whole
@@ -122,7 +120,8 @@ __device__ __forceinline__ void row_sums(float (&s)[NS], float* red, int& parity
 template <int LPR>
 constexpr int norm_threads() { return LPR > 256 ? LPR : 256; }
 
-template <typename T, int N, int LPR, int NV>
+// Y: the output's type, T or fp32.
+template <typename T, typename Y, int N, int LPR, int NV>
 __global__ __launch_bounds__(norm_threads<LPR>()) void norm_fwd_kernel(NormArgs a) {
   constexpr int THREADS = norm_threads<LPR>(), RPB = THREADS / LPR;
   __shared__ float red[4 * (LPR > kWave ? LPR / kWave : 1)];
@@ -136,11 +135,11 @@ __global__ __launch_bounds__(norm_threads<LPR>()) void norm_fwd_kernel(NormArgs 
     load_param<T, N>(b[v], a.b, a.w_is_f32, col, a.cols, 0.f);
   }
   const float inv_n = 1.f / (float)a.cols;
-  const uint32_t x_row = sub * (uint32_t)(a.x_stride * (int64_t)sizeof(T)), y_row = sub * (uint32_t)(a.y_stride * (int64_t)sizeof(T));
+  const uint32_t x_row = sub * (uint32_t)(a.x_stride * (int64_t)sizeof(T)), y_row = sub * (uint32_t)(a.y_stride * (int64_t)sizeof(Y));
   for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.rows; r0 += (int64_t)gridDim.x * RPB) {
     const bool on = sub < a.rows - r0;
     const auto xr = rows_at(a.x, r0 * a.x_stride * (int64_t)sizeof(T));
-    const auto yr = rows_at(a.y, r0 * a.y_stride * (int64_t)sizeof(T));
+    const auto yr = rows_at(a.y, r0 * a.y_stride * (int64_t)sizeof(Y));
     float x[NV][N], s[1] = {0.f};
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
@@ -170,7 +169,7 @@ __global__ __launch_bounds__(norm_threads<LPR>()) void norm_fwd_kernel(NormArgs 
       const int col = (lane + v * LPR) * N;
 #pragma unroll
       for (int j = 0; j < N; ++j) x[v][j] = fmaf(x[v][j] * rstd, w[v][j], b[v][j]);
-      store_n<T, N>(x[v], yr, on && col < a.cols ? y_row + col * (int)sizeof(T) : kOutside);
+      store_n<Y, N>(x[v], yr, on && col < a.cols ? y_row + col * (int)sizeof(Y) : kOutside);
     }
     if (a.mean != nullptr && on && lane == 0) {
       a.mean[r0 + sub] = mean;
@@ -179,7 +178,8 @@ __global__ __launch_bounds__(norm_threads<LPR>()) void norm_fwd_kernel(NormArgs 
   }
 }
 
-template <typename T, int N, int LPR, int NV>
+// Y: the type of the output and so of its gradient.
+template <typename T, typename Y, int N, int LPR, int NV>
 __global__ __launch_bounds__(norm_threads<LPR>()) void norm_bwd_kernel(NormArgs a) {
   constexpr int THREADS = norm_threads<LPR>(), RPB = THREADS / LPR;
   __shared__ float red[4 * (LPR > kWave ? LPR / kWave : 1)];
@@ -194,19 +194,19 @@ __global__ __launch_bounds__(norm_threads<LPR>()) void norm_bwd_kernel(NormArgs 
     for (int j = 0; j < N; ++j) dw[v][j] = db[v][j] = 0.f;
   }
   const float inv_n = 1.f / (float)a.cols;
-  const uint32_t x_row = sub * (uint32_t)(a.x_stride * (int64_t)sizeof(T)), g_row = sub * (uint32_t)(a.dy_stride * (int64_t)sizeof(T)),
+  const uint32_t x_row = sub * (uint32_t)(a.x_stride * (int64_t)sizeof(T)), g_row = sub * (uint32_t)(a.dy_stride * (int64_t)sizeof(Y)),
                  d_row = sub * (uint32_t)(a.dx_stride * (int64_t)sizeof(T));
   for (int64_t r0 = (int64_t)blockIdx.x * RPB; r0 < a.rows; r0 += (int64_t)gridDim.x * RPB) {
     const bool on = sub < a.rows - r0;
     const auto xr = rows_at(a.x, r0 * a.x_stride * (int64_t)sizeof(T));
-    const auto gr = rows_at(a.dy, r0 * a.dy_stride * (int64_t)sizeof(T));
+    const auto gr = rows_at(a.dy, r0 * a.dy_stride * (int64_t)sizeof(Y));
     float x[NV][N], g[NV][N], s[2] = {0.f, 0.f};
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
       const int col = (lane + v * LPR) * N;
       const bool in = on && col < a.cols;
       load_n<T, N>(x[v], xr, in ? x_row + col * (int)sizeof(T) : kOutside);
-      load_n<T, N>(g[v], gr, in ? g_row + col * (int)sizeof(T) : kOutside);
+      load_n<Y, N>(g[v], gr, in ? g_row + col * (int)sizeof(Y) : kOutside);
     }
     const float mean = on ? a.mean[r0 + sub] : 0.f, rstd = on ? a.rstd[r0 + sub] : 0.f;
 #pragma unroll
@@ -290,15 +290,15 @@ __global__ __launch_bounds__(1024) void norm_columns_kernel(NormArgs a) {
 
 constexpr int64_t kNormCols = 16384;  // what 1024 threads' registers hold
 
-// f.operator()<T, N, LPR, NV>() for rows of `cols` elements, whose chunks are 16
-// bytes (`whole`) or single elements.
+// f.operator()<T, Y, N, LPR, NV>() for rows of `cols` elements, whose chunks are
+// 16 bytes (`whole`) or single elements; y_dtype is T's or fp32.
 template <typename F>
-int norm_dispatch(int dtype, int64_t cols, bool whole, F&& f) {
-  auto by_width = [&](auto t) {
+int norm_dispatch(int dtype, int y_dtype, int64_t cols, bool whole, F&& f) {
+  auto by_width = [&](auto t, auto y) {
     using T = decltype(t);
     constexpr int VEC = 16 / (int)sizeof(T);
 #define TJ_NORM(N, L, V) \
-  return f(t, std::integral_constant<int, N>{}, std::integral_constant<int, L>{}, std::integral_constant<int, V>{})
+  return f(t, y, std::integral_constant<int, N>{}, std::integral_constant<int, L>{}, std::integral_constant<int, V>{})
     if (!whole) {
       if (cols <= 256) TJ_NORM(1, 64, 4);
       if (cols <= 1024) TJ_NORM(1, 64, 16);
@@ -319,9 +319,9 @@ int norm_dispatch(int dtype, int64_t cols, bool whole, F&& f) {
     TJ_NORM(VEC, 1024, 2);
 #undef TJ_NORM
   };
-  if (dtype == TJ_F32) return by_width(float{});
-  if (dtype == TJ_F16) return by_width(half_t{});
-  return by_width(bf16_t{});
+  if (dtype == TJ_F32) return by_width(float{}, float{});
+  if (dtype == TJ_F16) return y_dtype == TJ_F32 ? by_width(half_t{}, float{}) : by_width(half_t{}, half_t{});
+  return y_dtype == TJ_F32 ? by_width(bf16_t{}, float{}) : by_width(bf16_t{}, bf16_t{});
 }
 
 int norm_elem_bytes(int dtype) { return dtype == TJ_F32 ? 4 : (dtype == TJ_F16 || dtype == TJ_BF16 ? 2 : 0); }
@@ -337,8 +337,8 @@ int64_t norm_grid(int64_t rows, int rows_per_block, int64_t most) {
 }
 constexpr int64_t kFwdGroups = 1024, kBwdGroupsNarrow = 1024, kBwdGroups = 512;  // narrow: rows of less than a wave
 
-int norm_checks(int dtype, int w_dtype, int64_t rows, int64_t cols, const void* w, const void* b) {
-  if (norm_elem_bytes(dtype) == 0) return TJ_ERR_DTYPE;
+int norm_checks(int dtype, int y_dtype, int w_dtype, int64_t rows, int64_t cols, const void* w, const void* b) {
+  if (norm_elem_bytes(dtype) == 0 || (y_dtype != TJ_F32 && y_dtype != dtype)) return TJ_ERR_DTYPE;
   if ((w != nullptr || b != nullptr) && w_dtype != TJ_F32 && w_dtype != dtype) return TJ_ERR_DTYPE;
   if (rows < 0 || cols <= 0 || rows >= (int64_t(1) << 40)) return TJ_ERR_SHAPE;
   if (cols > kNormCols) return TJ_ERR_UNSUPPORTED;
@@ -368,27 +368,27 @@ bool element_aligned(const void* p, int dtype) {
 
 using namespace tj;
 
-extern "C" int tj_layer_norm_fwd(const void* x, const void* weight, const void* bias, void* y, int dtype, int w_dtype,
+extern "C" int tj_layer_norm_fwd(const void* x, const void* weight, const void* bias, void* y, int dtype, int y_dtype, int w_dtype,
                                  int64_t rows, int64_t cols, int64_t x_stride, int64_t y_stride, float eps, float* mean,
                                  float* rstd, hipStream_t stream) {
-  if (const int rc = norm_checks(dtype, w_dtype, rows, cols, weight, bias)) return rc;
+  if (const int rc = norm_checks(dtype, y_dtype, w_dtype, rows, cols, weight, bias)) return rc;
   if ((mean == nullptr) != (rstd == nullptr) || !(eps >= 0.f)) return TJ_ERR_SHAPE;
   if (rows == 0) return TJ_OK;
   if (x == nullptr || y == nullptr) return TJ_ERR_SHAPE;
-  if (!element_aligned(x, dtype) || !element_aligned(y, dtype) || !element_aligned(weight, w_dtype == TJ_F32 ? TJ_F32 : dtype) ||
+  if (!element_aligned(x, dtype) || !element_aligned(y, y_dtype) || !element_aligned(weight, w_dtype == TJ_F32 ? TJ_F32 : dtype) ||
       !element_aligned(bias, w_dtype == TJ_F32 ? TJ_F32 : dtype) || !element_aligned(mean, TJ_F32) || !element_aligned(rstd, TJ_F32))
     return TJ_ERR_ALIGN;
-  if (!row_stride_ok(x_stride, dtype) || !row_stride_ok(y_stride, dtype)) return TJ_ERR_UNSUPPORTED;
+  if (!row_stride_ok(x_stride, dtype) || !row_stride_ok(y_stride, y_dtype)) return TJ_ERR_UNSUPPORTED;
   NormArgs a{};
   a.x = x; a.w = weight; a.b = bias; a.y = y; a.mean = mean; a.rstd = rstd;
   a.rows = rows; a.cols = cols; a.x_stride = x_stride; a.y_stride = y_stride; a.eps = eps;
   a.w_is_f32 = w_dtype == TJ_F32;
   const bool whole = whole_chunks(dtype, cols, {x, y, weight, bias}, {x_stride, y_stride});
-  return norm_dispatch(dtype, cols, whole, [&](auto t, auto n, auto lpr, auto nv) {
+  return norm_dispatch(dtype, y_dtype, cols, whole, [&](auto t, auto y, auto n, auto lpr, auto nv) {
     constexpr int LPR = decltype(lpr)::value, THREADS = norm_threads<LPR>();
     const int64_t grid = norm_grid(rows, THREADS / LPR, kFwdGroups);
-    hipLaunchKernelGGL((norm_fwd_kernel<decltype(t), decltype(n)::value, LPR, decltype(nv)::value>), dim3(uint32_t(grid)),
-                       dim3(THREADS), 0, stream, a);
+    hipLaunchKernelGGL((norm_fwd_kernel<decltype(t), decltype(y), decltype(n)::value, LPR, decltype(nv)::value>),
+                       dim3(uint32_t(grid)), dim3(THREADS), 0, stream, a);
     return tjh::launch_status();
   });
 }
@@ -399,18 +399,18 @@ extern "C" size_t tj_layer_norm_bwd_workspace_bytes(int64_t rows, int64_t cols) 
 }
 
 extern "C" int tj_layer_norm_bwd(const void* dy, const void* x, const void* weight, const float* mean, const float* rstd,
-                                 void* dx, void* dweight, void* dbias, int dtype, int w_dtype, int64_t rows, int64_t cols,
+                                 void* dx, void* dweight, void* dbias, int dtype, int y_dtype, int w_dtype, int64_t rows, int64_t cols,
                                  int64_t dy_stride, int64_t x_stride, int64_t dx_stride, void* workspace,
                                  size_t workspace_bytes, hipStream_t stream) {
-  if (const int rc = norm_checks(dtype, w_dtype, rows, cols, weight, dweight != nullptr ? dweight : dbias)) return rc;
+  if (const int rc = norm_checks(dtype, y_dtype, w_dtype, rows, cols, weight, dweight != nullptr ? dweight : dbias)) return rc;
   if (rows == 0) return TJ_OK;
   if (dy == nullptr || x == nullptr || mean == nullptr || rstd == nullptr) return TJ_ERR_SHAPE;
   const int wd = w_dtype == TJ_F32 ? TJ_F32 : dtype;
-  if (!element_aligned(dy, dtype) || !element_aligned(x, dtype) || !element_aligned(dx, dtype) ||
+  if (!element_aligned(dy, y_dtype) || !element_aligned(x, dtype) || !element_aligned(dx, dtype) ||
       !element_aligned(weight, wd) || !element_aligned(dweight, wd) || !element_aligned(dbias, wd) ||
       !element_aligned(mean, TJ_F32) || !element_aligned(rstd, TJ_F32) || !element_aligned(workspace, TJ_F32))
     return TJ_ERR_ALIGN;
-  if (!row_stride_ok(x_stride, dtype) || !row_stride_ok(dy_stride, dtype) || (dx != nullptr && !row_stride_ok(dx_stride, dtype)))
+  if (!row_stride_ok(x_stride, dtype) || !row_stride_ok(dy_stride, y_dtype) || (dx != nullptr && !row_stride_ok(dx_stride, dtype)))
     return TJ_ERR_UNSUPPORTED;
   const bool columns = dweight != nullptr || dbias != nullptr;
   if (columns && (workspace == nullptr || workspace_bytes < tj_layer_norm_bwd_workspace_bytes(rows, cols)))
@@ -421,11 +421,12 @@ extern "C" int tj_layer_norm_bwd(const void* dy, const void* x, const void* weig
   a.rows = rows; a.cols = cols; a.dy_stride = dy_stride; a.x_stride = x_stride; a.dx_stride = dx_stride;
   a.w_is_f32 = w_dtype == TJ_F32;
   const bool whole = whole_chunks(dtype, cols, {x, dy, dx, weight}, {x_stride, dy_stride, dx == nullptr ? 0 : dx_stride});
-  return norm_dispatch(dtype, cols, whole, [&](auto t, auto n, auto lpr, auto nv) {
+  return norm_dispatch(dtype, y_dtype, cols, whole, [&](auto t, auto y, auto n, auto lpr, auto nv) {
     using T = decltype(t);
     constexpr int LPR = decltype(lpr)::value, THREADS = norm_threads<LPR>();
     a.n_parts = (int)norm_grid(rows, THREADS / LPR, LPR < kWave ? kBwdGroupsNarrow : kBwdGroups);
-    hipLaunchKernelGGL((norm_bwd_kernel<T, decltype(n)::value, LPR, decltype(nv)::value>), dim3(uint32_t(a.n_parts)), dim3(THREADS), 0, stream, a);
+    hipLaunchKernelGGL((norm_bwd_kernel<T, decltype(y), decltype(n)::value, LPR, decltype(nv)::value>),
+                       dim3(uint32_t(a.n_parts)), dim3(THREADS), 0, stream, a);
     const int rc = tjh::launch_status();
     if (rc != TJ_OK || !columns) return rc;
     hipLaunchKernelGGL((norm_columns_kernel<T>), dim3(uint32_t((2 * cols + 31) / 32)), dim3(1024), 0, stream, a);

@@ -115,10 +115,10 @@ SIGNATURES = {
         + [_f32, _int, _vp, _i64, _vp, _vp, ctypes.c_size_t, _vp],
     ),
     "tj_layer_norm_fwd": (
-        _int, [_vp, _vp, _vp, _vp, _int, _int, _i64, _i64, _i64, _i64, _f32, _vp, _vp, _vp]),
+        _int, [_vp, _vp, _vp, _vp, _int, _int, _int, _i64, _i64, _i64, _i64, _f32, _vp, _vp, _vp]),
     "tj_layer_norm_bwd_workspace_bytes": (ctypes.c_size_t, [_i64, _i64]),
     "tj_layer_norm_bwd": (
-        _int, [_vp] * 8 + [_int, _int, _i64, _i64, _i64, _i64, _i64, _vp, ctypes.c_size_t, _vp]),
+        _int, [_vp] * 8 + [_int, _int, _int, _i64, _i64, _i64, _i64, _i64, _vp, ctypes.c_size_t, _vp]),
 }
 
 _lock = threading.Lock()

@@ -33,11 +33,11 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     return t
 
 
-def _forward(x, weight, bias, eps, stats):
+def _forward(x, weight, bias, eps, stats, y_dtype):
     rows2d = _rows(x)
     rows, width = rows2d.shape
     dev = x.device
-    y = x.new_empty(x.shape)
+    y = x.new_empty(x.shape, dtype=y_dtype)
     # mean [rows], then 1 / sqrt(var + eps) [rows], in one tensor.
     moments = torch.empty(2 * rows, dtype=torch.float32, device=dev) if stats else None
     mean = moments.data_ptr() if stats and rows else None
@@ -46,7 +46,7 @@ def _forward(x, weight, bias, eps, stats):
         w_dtype = DTYPES[(bias if weight is None else weight).dtype]
     with on_device(dev):
         code = _lib.lib().tj_layer_norm_fwd(
-            rows2d.data_ptr(), _ptr(weight), _ptr(bias), y.data_ptr(), DTYPES[x.dtype], w_dtype, rows, width,
+            rows2d.data_ptr(), _ptr(weight), _ptr(bias), y.data_ptr(), DTYPES[x.dtype], DTYPES[y_dtype], w_dtype, rows, width,
             rows2d.stride(0), width, eps, mean, mean and mean + 4 * rows, _stream_ptr(dev))
     if code:
         _lib.check(code, "tj_layer_norm_fwd")
@@ -55,7 +55,7 @@ def _forward(x, weight, bias, eps, stats):
 
 def _backward(ctx, dy):
     x, weight, moments = ctx.saved_tensors
-    need_x, need_w, need_b, _ = ctx.needs_input_grad
+    need_x, need_w, need_b = ctx.needs_input_grad[:3]
     dy2d, x2d = _rows(dy), _rows(x)
     rows, width = x2d.shape
     dev = x.device
@@ -65,7 +65,7 @@ def _backward(ctx, dy):
     dw = make(width, dtype=w_torch, device=dev) if need_w else None
     db = make(width, dtype=w_torch, device=dev) if need_b else None
     if rows == 0:
-        return dx, dw, db, None
+        return dx, dw, db, None, None
     lib = _lib.lib()
     mean = moments.data_ptr()
     with on_device(dev):
@@ -73,11 +73,11 @@ def _backward(ctx, dy):
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
         code = lib.tj_layer_norm_bwd(
             dy2d.data_ptr(), x2d.data_ptr(), _ptr(weight), mean, mean + 4 * rows, _ptr(dx), _ptr(dw), _ptr(db),
-            DTYPES[x.dtype], _lib.TJ_F32 if w_torch is None else DTYPES[w_torch], rows, width, dy2d.stride(0),
-            x2d.stride(0), width, _ptr(ws), ws_bytes, _stream_ptr(dev))
+            DTYPES[x.dtype], DTYPES[dy.dtype], _lib.TJ_F32 if w_torch is None else DTYPES[w_torch], rows, width,
+            dy2d.stride(0), x2d.stride(0), width, _ptr(ws), ws_bytes, _stream_ptr(dev))
     if code:
         _lib.check(code, "tj_layer_norm_bwd")
-    return dx, dw, db, None
+    return dx, dw, db, None, None
 
 
 #: Under create_graph: the gradients, with an error for whoever differentiates
@@ -88,8 +88,8 @@ _backward_once = once_differentiable(_backward)
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, eps):
-        y, moments = _forward(x, weight, bias, eps, True)
+    def forward(ctx, x, weight, bias, eps, y_dtype):
+        y, moments = _forward(x, weight, bias, eps, True, y_dtype)
         ctx.save_for_backward(x, weight, moments)
         ctx.bias_dtype = None if bias is None else bias.dtype
         return y
@@ -100,15 +100,16 @@ class _LayerNorm(torch.autograd.Function):
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
-               eps: float = 1e-5) -> torch.Tensor:
+               eps: float = 1e-5, *, norm_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """Layer norm over the last dimension of ``x``; differentiable in all three tensors.
 
     ``x`` is float32, float16 or bfloat16 with a last dimension of at most
     ``MAX_WIDTH``, of any shape and strides (read in place where the rows have
     one common stride). ``weight`` and ``bias`` are contiguous ``[width]``, both
     float32 or both of ``x``'s type, each optional; their gradients come in their
-    type. Statistics and sums are float32, the output is ``x``'s type and
-    contiguous. The gradients' sums over the rows have a fixed order, so equal
+    type. Statistics and sums are float32, the output is contiguous and of
+    ``x``'s type, or float32 with ``norm_dtype=torch.float32`` (the norm of
+    16-bit rows not rounded to 16 bits). The gradients' sums over the rows have a fixed order, so equal
     calls give equal bits. Second derivatives are not implemented.
     """
     if x.ndim == 0 or x.shape[-1] == 0:
@@ -128,10 +129,14 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
             raise ValueError(f"{name} must be float32 or {x.dtype}, not {p.dtype}")
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         raise ValueError("weight and bias must share a dtype")
+    if norm_dtype is None:
+        norm_dtype = x.dtype
+    elif norm_dtype not in (torch.float32, x.dtype):
+        raise ValueError(f"norm_dtype must be float32 or {x.dtype}, not {norm_dtype}")
     eps = float(eps)
     if torch.is_grad_enabled() and (x.requires_grad or any(p is not None and p.requires_grad for p in (weight, bias))):
-        return _LayerNorm.apply(x, weight, bias, eps)
-    return _forward(x, weight, bias, eps, False)[0]
+        return _LayerNorm.apply(x, weight, bias, eps, norm_dtype)
+    return _forward(x, weight, bias, eps, False, norm_dtype)[0]
 
 
 class LayerNorm(torch.nn.LayerNorm):

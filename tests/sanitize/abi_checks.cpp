@@ -214,7 +214,7 @@ int main() {
 
     // tj_layer_norm_fwd(x, weight, bias, y, dtype, w_dtype, rows, cols, x_stride, y_stride, eps, mean, rstd, stream)
     auto norm = [&](const void* x, const void* w, int dtype, int w_dtype, int64_t rows, int64_t cols, float* mean) {
-      return tj_layer_norm_fwd(x, w, nullptr, o, dtype, w_dtype, rows, cols, cols, cols, 1e-5f, mean, nullptr, nullptr);
+      return tj_layer_norm_fwd(x, w, nullptr, o, dtype, dtype, w_dtype, rows, cols, cols, cols, 1e-5f, mean, nullptr, nullptr);
     };
     expect("norm dtype", norm(q, k, 5, TJ_F32, 4, 64, nullptr), TJ_ERR_DTYPE);
     expect("norm weight dtype", norm(q, k, TJ_F16, TJ_BF16, 4, 64, nullptr), TJ_ERR_DTYPE);
@@ -226,11 +226,12 @@ int main() {
     expect("norm missing x", norm(nullptr, k, TJ_F16, TJ_F32, 4, 64, nullptr), TJ_ERR_SHAPE);
     expect("norm x alignment", norm(at(1), k, TJ_F16, TJ_F32, 4, 64, nullptr), TJ_ERR_ALIGN);
     expect("norm weight alignment", norm(q, at(2), TJ_F16, TJ_F32, 4, 64, nullptr), TJ_ERR_ALIGN);
-    expect("norm eps", tj_layer_norm_fwd(q, k, nullptr, o, TJ_F16, TJ_F32, 4, 64, 64, 64, -1.f, nullptr, nullptr, nullptr), TJ_ERR_SHAPE);
+    expect("norm eps", tj_layer_norm_fwd(q, k, nullptr, o, TJ_F16, TJ_F16, TJ_F32, 4, 64, 64, 64, -1.f, nullptr, nullptr, nullptr), TJ_ERR_SHAPE);
+    expect("norm y dtype", tj_layer_norm_fwd(q, k, nullptr, o, TJ_F16, TJ_BF16, TJ_F32, 4, 64, 64, 64, 1e-5f, nullptr, nullptr, nullptr), TJ_ERR_DTYPE);
     expect("norm no rows", norm(nullptr, k, TJ_F16, TJ_F32, 0, 64, nullptr), TJ_OK);
     expect_size("norm workspace of huge sizes", tj_layer_norm_bwd_workspace_bytes(kBig, kBig), 0);
     auto norm_bwd = [&](const void* dy, const float* mean, int dtype, int64_t rows, int64_t cols, void* dw, size_t bytes) {
-      return tj_layer_norm_bwd(dy, q, k, mean, stats, o, dw, nullptr, dtype, TJ_F32, rows, cols, cols, cols, cols,
+      return tj_layer_norm_bwd(dy, q, k, mean, stats, o, dw, nullptr, dtype, dtype, TJ_F32, rows, cols, cols, cols, cols,
                                at(8192), bytes, nullptr);
     };
     expect("norm bwd dtype", norm_bwd(v, stats, -1, 4, 64, at(5120), 1 << 15), TJ_ERR_DTYPE);

@@ -60,6 +60,8 @@ def test_norm_refuses():
     for bad in (torch.zeros(()), torch.zeros(2, 0)):
         with pytest.raises(ValueError):
             layer_norm(bad)
+    with pytest.raises(UnsupportedCaseError):  # the device comes first
+        layer_norm(x, norm_dtype=torch.float16)
     with pytest.raises(ValueError):
         LayerNorm((2, 8))
     with pytest.raises(ValueError):

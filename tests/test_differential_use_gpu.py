@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from differential_reference import assert_within, attention
+from graph_capture import captured, replay
 from test_differential_gpu import FLOOR, TYPES, heads, inputs, lengths_of
 
 pytestmark = pytest.mark.gpu
@@ -197,25 +198,15 @@ def test_forward_and_cached_replay_in_graphs(cuda):
     q1 = q[:, :, :1].contiguous()
     calls = (lambda: differential_attention(q, k, v, lam, is_causal=True, valid_len=lengths),
              lambda: differential_attention_cached(q1, k, v, lam, lengths))
-    graphs = []
     with torch.no_grad():
-        for call in calls:
-            side = torch.cuda.Stream()
-            side.wait_stream(torch.cuda.current_stream())
-            with torch.cuda.stream(side):
-                call()
-            torch.cuda.current_stream().wait_stream(side)
-            graph = torch.cuda.CUDAGraph()
-            with torch.cuda.graph(graph):
-                out = call()
-            graphs.append((graph, out))
+        graphs = [captured(call) for call in calls]
         for i in range(4):
             g = torch.Generator(device="cuda").manual_seed(20 + i)
             for t in (q, k, v, q1):
                 t.normal_(generator=g)
             lengths.copy_(lengths_of(700 - 100 * i, 80 + 7 * i))
             for graph, _ in graphs:
-                graph.replay()
+                replay(graph)
             got = [out.clone() for _, out in graphs]
             for x, call in zip(got, calls):
                 assert torch.equal(x, call())
@@ -232,21 +223,13 @@ def test_training_step_replays_in_a_graph(cuda):
         out = differential_attention(*leaves, is_causal=True)
         return (out.detach(), *torch.autograd.grad(out, leaves, dout))
 
-    side = torch.cuda.Stream()
-    side.wait_stream(torch.cuda.current_stream())
-    with torch.cuda.stream(side):
-        for _ in range(2):
-            step()
-    torch.cuda.current_stream().wait_stream(side)
-    graph = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(graph):
-        held = step()
+    graph, held = captured(step)
     for i in range(4):
         g = torch.Generator(device="cuda").manual_seed(30 + i)
         with torch.no_grad():
             for t in (*leaves[:3], dout):
                 t.normal_(generator=g)
-        graph.replay()
+        replay(graph)
         got = [t.clone() for t in held]
         for a, b in zip(got, step()):
             assert torch.equal(a, b)

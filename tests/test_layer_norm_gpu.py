@@ -10,6 +10,8 @@ from __future__ import annotations
 import pytest
 import torch
 
+from graph_capture import captured, replay
+
 pytestmark = pytest.mark.gpu
 
 TYPES = {"fp32": torch.float32, "fp16": torch.float16, "bf16": torch.bfloat16}
@@ -215,13 +217,11 @@ def test_replays_in_a_graph_and_on_another_stream(cuda):
     torch.cuda.current_stream().wait_stream(side)
     for a, c in zip(first, _grads(x, w, b, dy)):
         assert torch.equal(a, c)
-    graph = torch.cuda.CUDAGraph()
-    with torch.cuda.graph(graph):
-        held = _grads(x, w, b, dy)
+    graph, held = captured(lambda: _grads(x, w, b, dy))
     for i in range(4):
         x.normal_()
         dy.normal_()
-        graph.replay()
+        replay(graph)
         got = [t.detach().clone() for t in held]
         for a, c in zip(got, _grads(x, w, b, dy)):
             assert torch.equal(a, c)
@@ -256,3 +256,26 @@ def test_gradient_is_the_slope(cuda):
         slope = (grads[i].cpu().double() * d.cpu().double()).sum()
         assert float(((u - l) / (2 * eps) - slope).abs()) <= float(allowed), name
         assert float(missed) < 0.05 * float(want.abs()) + 0.05, name
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("rows,width", [(37, 128), (19, 1000), (5, 333), (3, 4096)])
+def test_float32_norms_of_sixteen_bit_rows(cuda, rows, width, dtype):
+    """norm_dtype: y and its gradient float32, everything else as before."""
+    from techjam_amd.kernels import layer_norm
+
+    t = TYPES[dtype]
+    g = torch.Generator().manual_seed(8)
+    x, w, b = rows_of(g, rows, width, t), torch.randn(width, generator=g).cuda(), torch.randn(width, generator=g).cuda()
+    dy = torch.randn(rows, width, generator=g).cuda()
+    want = reference(x, w, b, dy, 1e-5)
+    y32 = reference(x.float(), w, b, dy, 1e-5)["y"]
+    leaves = [p.detach().requires_grad_() for p in (x, w, b)]
+    y = layer_norm(*leaves, norm_dtype=torch.float32)
+    grads = torch.autograd.grad(y, leaves, dy)
+    assert y.dtype == torch.float32 and grads[0].dtype == t
+    check(y, y32, "y")
+    for name, got in zip(("dx", "dw", "db"), grads):
+        check(got, want[name], name)
+    with pytest.raises(ValueError):
+        layer_norm(x, norm_dtype=torch.float64)
