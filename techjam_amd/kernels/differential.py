@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import contextlib
 import math
+from functools import lru_cache
 from typing import Optional
 
 import torch
@@ -92,6 +93,16 @@ def _padded(q, k, v):
     return q, k, v
 
 
+@lru_cache(maxsize=256)
+def _workspace_floats(b: int, h: int, hk: int, sq: int, sk: int, dv: int, cached: int) -> int:
+    return _lib.lib().tj_diff_attn_workspace_bytes(b, h, hk, sq, sk, dv, cached) // 4
+
+
+@lru_cache(maxsize=256)
+def _backward_floats(b: int, h: int, hk: int, s: int) -> int:
+    return _lib.lib().tj_diff_attn_bwd_workspace_bytes(b, h, hk, s) // 4
+
+
 def _forward(q, k, v, lam, lengths, scale, causal, cached, stats):
     """One kernel call on padded inputs: ``(out, maps, lse)``, the last two None without ``stats``."""
     b, h2, sq, d = q.shape
@@ -102,16 +113,14 @@ def _forward(q, k, v, lam, lengths, scale, causal, cached, stats):
     out = _empty_heads(b, h, sq, dv, q)
     maps = lse = None
     if stats:
-        maps = torch.empty(b, hk, sq * (h // hk), 2, dv, dtype=torch.float32, device=dev)
-        lse = torch.empty(b, hk, 2, sq * (h // hk), dtype=torch.float32, device=dev)
-    lib = _lib.lib()
+        maps, lse = lam.new_empty((b, h, sq, 2, dv)), lam.new_empty((b, h, 2, sq))
+    floats = _workspace_floats(b, h, hk, sq, sk, dv, int(cached))
+    ws = lam.new_empty(floats) if floats else None
     with on_device(dev):
-        ws_bytes = lib.tj_diff_attn_workspace_bytes(b, h, hk, sq, sk, dv, int(cached))
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
-        code = lib.tj_diff_attn_fwd(
+        code = _lib.lib().tj_diff_attn_fwd(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), DTYPES[q.dtype], b, h, hk, sq, sk, d, dv,
             _lib.strides4(q), _lib.strides4(k), _lib.strides4(v), _lib.strides4(out), scale, int(causal), int(cached),
-            lam.data_ptr(), int(lam.numel() > 1), _ptr(lengths), _ptr(lse), _ptr(maps), _ptr(ws), ws_bytes,
+            lam.data_ptr(), int(lam.numel() > 1), _ptr(lengths), _ptr(lse), _ptr(maps), _ptr(ws), 4 * floats,
             _stream_ptr(dev))
     _lib.check(code, "tj_diff_attn_fwd")
     return out, maps, lse
@@ -126,18 +135,17 @@ def _backward(ctx, dout):
     dev = q.device
     dq, dk = _empty_heads(b, h2, s, d, q), _empty_heads(b, 2 * hk, s, d, q)
     dvv = _empty_heads(b, hk, s, dv, q)
-    dlam = torch.empty(lam.shape, dtype=torch.float32, device=dev)
+    dlam = lam.new_empty(lam.shape)
     if b == 0 or s == 0:
         return dq, dk, dvv, dlam.zero_(), None, None, None
-    lib = _lib.lib()
+    floats = _backward_floats(b, h, hk, s)
+    ws = lam.new_empty(floats)
     with on_device(dev):
-        ws_bytes = lib.tj_diff_attn_bwd_workspace_bytes(b, h, hk, s)
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-        code = lib.tj_diff_attn_bwd(
+        code = _lib.lib().tj_diff_attn_bwd(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), maps.data_ptr(), lse.data_ptr(),
             dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dvv.data_ptr(), dlam.data_ptr(), DTYPES[q.dtype],
             b, h, hk, s, d, dv, *map(_lib.strides4, (q, k, v, dout, dq, dk, dvv)), ctx.scale, int(ctx.causal),
-            lam.data_ptr(), int(lam.numel() > 1), _ptr(lengths), ws.data_ptr(), ws_bytes, _stream_ptr(dev))
+            lam.data_ptr(), int(lam.numel() > 1), _ptr(lengths), ws.data_ptr(), 4 * floats, _stream_ptr(dev))
     _lib.check(code, "tj_diff_attn_bwd")
     return dq, dk, dvv, dlam, None, None, None
 

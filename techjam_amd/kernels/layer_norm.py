@@ -8,6 +8,7 @@ for every width up to ``MAX_WIDTH``, with gradients.
 
 from __future__ import annotations
 
+from functools import lru_cache
 from typing import Optional
 
 import torch
@@ -22,11 +23,18 @@ from .differential import DTYPES, on_device
 MAX_WIDTH = 16384
 
 
+@lru_cache(maxsize=256)
+def _workspace_floats(rows: int, width: int) -> int:
+    return _lib.lib().tj_layer_norm_bwd_workspace_bytes(rows, width) // 4
+
+
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """``t`` as ``[rows, width]`` with unit column stride: a view where its
     leading dimensions have one stride in common (below 2^23 elements), else a
     copy."""
     width = t.shape[-1]
+    if t.is_contiguous():
+        return t if t.ndim == 2 else t.view(-1, width)
     t = t.reshape(-1, width)
     if (t.stride(1) != 1 and width > 1) or t.stride(0) >= 1 << 23:
         return t.contiguous()
@@ -37,9 +45,9 @@ def _forward(x, weight, bias, eps, stats, y_dtype):
     rows2d = _rows(x)
     rows, width = rows2d.shape
     dev = x.device
-    y = x.new_empty(x.shape, dtype=y_dtype)
+    y = torch.empty_like(x, dtype=y_dtype, memory_format=torch.contiguous_format)
     # mean [rows], then 1 / sqrt(var + eps) [rows], in one tensor.
-    moments = torch.empty(2 * rows, dtype=torch.float32, device=dev) if stats else None
+    moments = x.new_empty(2 * rows, dtype=torch.float32) if stats else None
     mean = moments.data_ptr() if stats and rows else None
     w_dtype = _lib.TJ_F32
     if weight is not None or bias is not None:
@@ -59,22 +67,19 @@ def _backward(ctx, dy):
     dy2d, x2d = _rows(dy), _rows(x)
     rows, width = x2d.shape
     dev = x.device
-    dx = x.new_empty(x.shape) if need_x else None
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format) if need_x else None
     w_torch = ctx.bias_dtype if weight is None else weight.dtype
-    make = torch.zeros if rows == 0 else torch.empty
-    dw = make(width, dtype=w_torch, device=dev) if need_w else None
-    db = make(width, dtype=w_torch, device=dev) if need_b else None
+    dw = moments.new_empty(width, dtype=w_torch) if need_w else None
+    db = moments.new_empty(width, dtype=w_torch) if need_b else None
     if rows == 0:
-        return dx, dw, db, None, None
-    lib = _lib.lib()
+        return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_(), None, None
     mean = moments.data_ptr()
+    ws = moments.new_empty(_workspace_floats(rows, width)) if need_w or need_b else None
     with on_device(dev):
-        ws_bytes = lib.tj_layer_norm_bwd_workspace_bytes(rows, width) if need_w or need_b else 0
-        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=dev) if ws_bytes else None
-        code = lib.tj_layer_norm_bwd(
+        code = _lib.lib().tj_layer_norm_bwd(
             dy2d.data_ptr(), x2d.data_ptr(), _ptr(weight), mean, mean + 4 * rows, _ptr(dx), _ptr(dw), _ptr(db),
             DTYPES[x.dtype], DTYPES[dy.dtype], _lib.TJ_F32 if w_torch is None else DTYPES[w_torch], rows, width,
-            dy2d.stride(0), x2d.stride(0), width, _ptr(ws), ws_bytes, _stream_ptr(dev))
+            dy2d.stride(0), x2d.stride(0), width, _ptr(ws), 0 if ws is None else 4 * ws.numel(), _stream_ptr(dev))
     if code:
         _lib.check(code, "tj_layer_norm_bwd")
     return dx, dw, db, None, None
@@ -99,6 +104,13 @@ class _LayerNorm(torch.autograd.Function):
         return _backward_once(ctx, dy) if torch.is_grad_enabled() else _backward(ctx, dy)
 
 
+def _check_param(name, p, width, dtype, dev) -> None:
+    if p.shape != (width,) or p.device != dev or not p.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous tensor of {width} elements on {dev}")
+    if p.dtype != torch.float32 and p.dtype != dtype:
+        raise ValueError(f"{name} must be float32 or {dtype}, not {p.dtype}")
+
+
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
                eps: float = 1e-5, *, norm_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """Layer norm over the last dimension of ``x``; differentiable in all three tensors.
@@ -119,22 +131,20 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     width = x.shape[-1]
     if width > MAX_WIDTH:
         raise UnsupportedCaseError(f"width {width} is not supported (at most {MAX_WIDTH})")
-    _require_device(x)
-    for name, p in (("weight", weight), ("bias", bias)):
-        if p is None:
-            continue
-        if p.shape != (width,) or p.device != x.device or not p.is_contiguous():
-            raise ValueError(f"{name} must be a contiguous tensor of {width} elements on {x.device}")
-        if p.dtype not in (torch.float32, x.dtype):
-            raise ValueError(f"{name} must be float32 or {x.dtype}, not {p.dtype}")
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise ValueError("weight and bias must share a dtype")
+    dev = _require_device(x)
+    if weight is not None:
+        _check_param("weight", weight, width, x.dtype, dev)
+    if bias is not None:
+        _check_param("bias", bias, width, x.dtype, dev)
+        if weight is not None and weight.dtype != bias.dtype:
+            raise ValueError("weight and bias must share a dtype")
     if norm_dtype is None:
         norm_dtype = x.dtype
     elif norm_dtype not in (torch.float32, x.dtype):
         raise ValueError(f"norm_dtype must be float32 or {x.dtype}, not {norm_dtype}")
     eps = float(eps)
-    if torch.is_grad_enabled() and (x.requires_grad or any(p is not None and p.requires_grad for p in (weight, bias))):
+    if torch.is_grad_enabled() and (x.requires_grad or (weight is not None and weight.requires_grad)
+                                    or (bias is not None and bias.requires_grad)):
         return _LayerNorm.apply(x, weight, bias, eps, norm_dtype)
     return _forward(x, weight, bias, eps, False, norm_dtype)[0]
 
