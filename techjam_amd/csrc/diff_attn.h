@@ -55,6 +55,7 @@ struct DiffArgs {
   int n_lam;
   float* delta;            // [B, H, 2, Sq] rowsum(dO o O_m)
   float* gsum;             // [B, H, Sq] rowsum(P_1 o dP), the row's part of -dlam
+  float* stat;             // [B, H, stat_rows(Sq) / 32, 4, 32] what the dK, dV kernel reads of a row
   float* peak;             // [B, Hk, 2, kPeakParts] largest norms of dO and V rows (fp16 operands)
   int n_peaks;
 };
@@ -276,6 +277,31 @@ struct KeyCopy : TileCopy<T, W, ROWS, WAVES> {
   }
 };
 
+// 64 single floats the same way: lane l's from byte offset voff to lds + 4 l.
+__device__ __forceinline__ void copy_4(rsrc_t r, uint32_t lds, uint32_t voff) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dword %1, %2, 0 offen lds"
+               :
+               : "s"(lds), "v"(voff), "s"(r)
+               : "memory", "m0");
+}
+
+// N products, the operands of each read from LDS DEPTH products before it. The
+// compiler, left to itself, reads right before the use and waits; that is as
+// good where other waves fill the gap and the registers are needed (DEPTH 0).
+template <int N, int DEPTH, typename Read, typename Use>
+__device__ __forceinline__ void read_ahead(Read&& read, Use&& use) {
+  decltype(read(0)) f[N];
+#pragma unroll
+  for (int i = 0; i < DEPTH && i < N; ++i) f[i] = read(i);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (i + DEPTH < N) f[i + DEPTH] = read(i + DEPTH);
+    if constexpr (DEPTH > 0) __builtin_amdgcn_sched_barrier(0);
+    use(i, f[i]);
+    if constexpr (DEPTH > 0) __builtin_amdgcn_sched_barrier(0);
+  }
+}
+
 // This wave's copies (and loads) and LDS accesses are done.
 __device__ __forceinline__ void wait_copies() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
 
@@ -371,12 +397,25 @@ __device__ __forceinline__ int64_t map_at(const DiffArgs& a, int b, int head, in
   return (((int64_t)b * a.H + head) * 2 + c) * a.Sq + i;
 }
 
+// A row's numbers in `stat`: log2 of P_0's and P_1's factor (minus lse, plus the
+// lift), -delta_0 and lam delta_1 (lifted). Rows that are not there, up to the
+// next multiple of 32, have -inf, -inf, 0, 0: P is 0.
+__host__ __device__ __forceinline__ int64_t stat_rows(int64_t S) { return (S + 31) / 32 * 32; }
+__device__ __forceinline__ float* stat_at(const DiffArgs& a, int b, int head, int i, int which) {
+  return a.stat + (((int64_t)b * a.H + head) * stat_rows(a.Sq) + i / 32 * 32) * 4 + which * 32 + i % 32;
+}
+
 // The same for P_0 - lam P_1 (at most 1 + |lam|).
 template <typename T>
-__device__ __forceinline__ float p_lift(float lam_max) {
+__device__ __forceinline__ float p_lift(const DiffArgs& a, int hk) {
   if constexpr (!std::is_same<T, half_t>::value) {
     return 1.f;
   } else {
+    float lam_max = 0.f;
+    for (int g = 0; g < a.G; ++g) {
+      const float l = fabsf(a.lam[(hk * a.G + g) * a.lam_step]);
+      if (l < 3e38f) lam_max = fmaxf(lam_max, l);
+    }
     int e;
     frexpf(1.f + lam_max, &e);
     return ldexpf(1.f, min(max(15 - e, -100), 14));

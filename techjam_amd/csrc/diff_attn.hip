@@ -139,7 +139,8 @@ extern "C" int tj_diff_attn_fwd(const void* q, const void* k, const void* v, voi
 
 extern "C" size_t tj_diff_attn_bwd_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t S) {
   if (!sizes_ok(B, H, Hk, S, S)) return 0;
-  return (size_t(B) * size_t(H) * size_t(S) * 3 + size_t(B) * size_t(Hk) * 2 * kPeakParts) * sizeof(float);
+  return (size_t(B) * size_t(H) * (size_t(S) * 3 + size_t(stat_rows(S)) * 4) + size_t(B) * size_t(Hk) * 2 * kPeakParts) *
+         sizeof(float);
 }
 
 extern "C" int tj_diff_attn_bwd(const void* q, const void* k, const void* v, const float* maps, const float* lse,
@@ -179,7 +180,8 @@ extern "C" int tj_diff_attn_bwd(const void* q, const void* k, const void* v, con
   a.n_lam = lam_step ? (int)H : 1;
   a.delta = static_cast<float*>(workspace);
   a.gsum = a.delta + 2 * B * H * S;
-  a.peak = a.gsum + B * H * S;
+  a.stat = a.gsum + B * H * S;
+  a.peak = a.stat + B * H * 4 * stat_rows(S);
   const int64_t blocks = ((int64_t)a.R + 63) / 64;
   a.n_peaks = (int)(blocks < kPeakParts ? blocks : kPeakParts);
   if (const int rc = diff_delta(a, dtype, stream)) return rc;

@@ -20,17 +20,23 @@
 namespace tj {
 namespace {
 
-// WHAT: 1 dV, 2 dK, 3 both. Heads past 64 dims do not have the registers for
-// both and form the scores twice. Eight waves, two a SIMD, where their
-// registers allow it, else four; as many groups as have room for two tiles each
-// (at most 128 KB of LDS), so that a tile is on its way while one is worked on.
+// WHAT: 1 dV, 2 dK, 3 both; fp32 heads past 64 dims do not have the registers for
+// both and form the scores twice. (16-bit ones of 128 dims do, in all 512 registers
+// of one wave a SIMD with operands read ahead: 229 us instead of 228 + 217 at b2 h4
+// s4096 bf16.) Eight waves, two a SIMD, where their registers allow it, else four;
+// as many groups as have room for two tiles each (at most 128 KB of LDS), so that a
+// tile is on its way while one is worked on.
 template <typename T, int HD, int WHAT>
 struct KvShape {
   static constexpr int DVP = 2 * HD;
-  static constexpr int WAVES = (sizeof(T) == 2 && (HD <= 64 || WHAT == 1)) || HD == 32 ? 8 : 4;
+  static constexpr int WAVES = (sizeof(T) == 2 && HD <= 64) || HD == 32 ? 8 : 4;
   static constexpr int RG = 512 / (HD * (int)sizeof(T)) < WAVES / 2 ? 512 / (HD * (int)sizeof(T)) : WAVES / 2;
   static constexpr int KB = WAVES / RG;
+  // What of the keys' rows stays in LDS, as the registers have no room for it.
+  static constexpr bool kK1InLds = WHAT == 3 && HD == 128;
   static constexpr bool kVInLds = (WHAT & 2) != 0 && sizeof(T) == 2 && HD == 64;
+  // bf16, two deep: 354 -> 337 us (fp32 d64, one deep), 214 -> 209 (bf16 d64), none at d32 (319).
+  static constexpr int kDepth = HD == 32 ? 0 : sizeof(T) == 2 ? 2 : 1;
   static constexpr int kTile = 32 * (2 * HD + DVP);  // Q's two heads and dO, of 32 tokens
   static constexpr int kBytes = kTile * (int)sizeof(T), kHead = 32 * HD * (int)sizeof(T);
 };
@@ -44,11 +50,9 @@ __global__ __launch_bounds__((64 * KvShape<T, HD, WHAT>::WAVES), (KvShape<T, HD,
   using QT = LdsRows<T, HD>;
   using OT = LdsRows<T, DVP>;
   __shared__ __attribute__((aligned(1024))) T smem[RG][2][SH::kTile];
-  // V's rows stay in LDS where their fragments would take a wave's registers
-  // past what two waves per SIMD have.
   __shared__ __attribute__((aligned(1024))) T sv[SH::kVInLds ? 32 * KB * DVP : 8];
-  // lse_0, lse_1 (with the lift), -delta_0 and lam delta_1 (lifted) of a tile's tokens
-  __shared__ __attribute__((aligned(16))) float stat[RG][2][4][BM];
+  __shared__ __attribute__((aligned(1024))) T sk[SH::kK1InLds ? 32 * KB * HD : 8];
+  __shared__ __attribute__((aligned(1024))) float stat[RG][2][4][BM];  // of a tile's tokens
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave, hl = lane / 32,
             ln = lane % 32;
   const int kb = w % KB, rg = w / KB;
@@ -67,6 +71,7 @@ __global__ __launch_bounds__((64 * KvShape<T, HD, WHAT>::WAVES), (KvShape<T, HD,
   const uint32_t group = lds_offset(smem[rg]);
   const uint32_t qrow = QT::lane_row(lane), qcol = QT::lane_col(lane), orow = OT::lane_row(lane) + 2 * SH::kHead,
                  ocol = OT::lane_col(lane) + 2 * SH::kHead;
+  const uint32_t krow = lds_offset(sk) + QT::lane_row(lane) + 32 * kb * QT::kRowBytes;
   const uint32_t vrow = lds_offset(sv) + OT::lane_row(lane) + 32 * kb * OT::kRowBytes;
   // Tile n: head n / tiles of the group, tokens i_begin + 32 (n % tiles) on.
   const int i_begin = a.causal ? k0 : 0;
@@ -85,23 +90,31 @@ __global__ __launch_bounds__((64 * KvShape<T, HD, WHAT>::WAVES), (KvShape<T, HD,
       qcopy.issue(qp + (2 * g + c) * a.vq.sh + i0 * a.vq.ss, a.vq.ss, L - i0, a.D, tile + c * SH::kHead, kb);
     ocopy.issue(op + g * a.vdo.sh + i0 * a.vdo.ss, a.vdo.ss, L - i0, a.Dv, tile + 2 * SH::kHead, kb);
   };
-  // Every lane carries two of a token's four numbers: lse_0 and delta_0 in the
-  // lower half of the wave, lse_1 and delta_1 in the upper one.
-  float next[2] = {0.f, 0.f};
-  auto load_stat = [&](int g, int i0) {
-    const int64_t at = map_at(a, t.b, t.hk * a.G + g, hl, min(i0 + ln, L - 1));
-    next[0] = a.lse[at];
-    next[1] = a.delta[at];
+  // The tokens' numbers by the same way (a load into registers would have to be
+  // waited for, and every copy issued before with it), two rows of 32 an instruction.
+  const uint32_t stat0 = lds_offset(stat[rg]);
+  auto issue_stat = [&](int g, int i0, int buf) {
+#pragma unroll
+    for (int pair = 0; pair < 2; ++pair)
+      if (kb == pair % KB)
+        copy_4(make_rsrc(stat_at(a, t.b, t.hk * a.G + g, i0, 2 * pair), 256), stat0 + (buf * 2 + pair) * 256, 4 * lane);
   };
 
-  frag_t<T> kf[2][KS], vf[DO_DK && !SH::kVInLds ? VS : 1];
+  frag_t<T> kf[SH::kK1InLds ? 1 : 2][KS], vf[DO_DK && !SH::kVInLds ? VS : 1];
   {
     const T* kp = reinterpret_cast<const T*>(a.k) + a.vk.row(t.b, 2 * t.hk, live ? key : 0);
     const T* vp = reinterpret_cast<const T*>(a.v) + a.vv.row(t.b, t.hk, live ? key : 0);
 #pragma unroll
-    for (int c = 0; c < 2; ++c)
+    for (int c = 0; c < (SH::kK1InLds ? 1 : 2); ++c)
 #pragma unroll
       for (int s = 0; s < KS; ++s) kf[c][s] = load_frag<T>(live ? kp + c * a.vk.sh : nullptr, 16 * s + 8 * hl, a.D);
+    if constexpr (SH::kK1InLds) {
+      KeyCopy<T, HD, 32 * KB, WAVES> kcopy;
+      kcopy.init(a.vk.ss, a.D, w, lane);
+      kcopy.issue(reinterpret_cast<const T*>(a.k) + a.vk.row(t.b, 2 * t.hk + 1, k0), a.vk.ss, L - k0, a.D, lds_offset(sk), w);
+      wait_copies();
+      __syncthreads();
+    }
     if constexpr (SH::kVInLds) {
       KeyCopy<T, DVP, 32 * KB, WAVES> vcopy;
       vcopy.init(a.vv.ss, a.Dv, w, lane);
@@ -121,61 +134,59 @@ __global__ __launch_bounds__((64 * KvShape<T, HD, WHAT>::WAVES), (KvShape<T, HD,
 #pragma unroll
   for (auto& x : dk[1]) x = zero16();
 
-  float lam_max = 0.f;
-  for (int g = 0; g < a.G; ++g) {
-    const float l = fabsf(a.lam[(t.hk * a.G + g) * a.lam_step]);
-    if (l < 3e38f) lam_max = fmaxf(lam_max, l);
-  }
-  // P is lifted by pl in its exponent; what multiplies P to dS takes that out again.
-  const float pl = p_lift<T>(lam_max), dl = ds_lift<T>(a, t.bh, t.hk, lane), log_pl = log2f(pl);
-  const float lift = dl / pl;
+  const float pl = p_lift<T>(a, t.hk), dl = ds_lift<T>(a, t.bh, t.hk, lane), lift = dl / pl;
   const float c2 = a.scale * kLog2e;
+  const auto lams = (const __attribute__((address_space(4))) float*)a.lam;
   int g = 0, i0 = i_begin;  // this round's tile
   if (rg < n_end) {
     advance(g, i0, rg);
     issue(g, i0, group);
-    load_stat(g, i0);
+    issue_stat(g, i0, 0);
   }
   // The workgroup goes round together, the last round maybe without a tile for every group.
   const int rounds = (n_end + RG - 1) / RG;
   for (int round = 0, n = rg, cur = 0; round < rounds; ++round, n += RG, cur ^= 1) {
     const bool on = n < n_end;
-    const float lam = on ? a.lam[(t.hk * a.G + g) * a.lam_step] : 0.f;
-    wait_copies();
-    if (on && kb == 0) {
-      // A token that is not there weighs nothing: P = 2^(0 - inf).
-      stat[rg][cur][hl][ln] = i0 + ln < L ? next[0] - log_pl : __builtin_inff();
-      stat[rg][cur][2 + hl][ln] = next[1] * (hl == 0 ? -lift : lam * lift);
-    }
+    // A scalar load (nothing here writes lam): it does not wait for the copies.
+    const float lam = on ? lams[(t.hk * a.G + g) * a.lam_step] : 0.f;
     // The tile is there, and the group's other one has been read by its waves.
-    wait_lds();
+    wait_copies();
     lds_barrier();
-    const uint32_t tile = group + cur * SH::kBytes;
+    const uint32_t tile = group + cur * SH::kBytes, srow = stat0 + cur * 512 + 16 * hl;
     const bool busy = on && (!a.causal || i0 + BM > kw0);  // else every token stands before the wave's keys
-    float16_t p[2];
-    if (busy) {
-#pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        p[c] = zero16();
-#pragma unroll
-        for (int s = 0; s < KS; ++s) p[c] = Elem<T>::mma(QT::row_frag(tile + qrow, s, c * SH::kHead), kf[c][s], p[c]);
-      }
-    }
-    // Only now: a spilled K fragment, read again above, would wait for the copies.
     int g1 = g, i1 = i0;
-    if (n + RG < n_end) {
+    // Called after the scores: a spilled K fragment, read again for them, would wait for
+    // the copies. In both branches rather than between two, where p would be merged.
+    auto issue_next = [&] {
+      if (n + RG >= n_end) return;
       advance(g1, i1, RG);
       issue(g1, i1, group + (cur ^ 1) * SH::kBytes);
-      load_stat(g1, i1);
-    }
+      issue_stat(g1, i1, cur ^ 1);
+    };
+    if (!busy) issue_next();
     if (busy) {
+      float16_t p[2], dp = zero16();
+p[0] = p[1] = zero16();
+      struct Two { frag_t<T> o, v; };
+      read_ahead<2 * KS, SH::kDepth>(
+          [&](int i) {
+            const int c = i / KS, s = i % KS;
+            return Two{QT::row_frag(tile + qrow, s, c * SH::kHead), SH::kK1InLds && c == 1 ? QT::row_frag(krow, s, 0) : kf[SH::kK1InLds ? 0 : c][s]};
+          },
+          [&](int i, Two f) { p[i / KS] = Elem<T>::mma(f.o, f.v, p[i / KS]); });
+      if constexpr (DO_DK) {
+        read_ahead<VS, SH::kDepth>(
+            [&](int s) { return Two{OT::row_frag(tile + orow, s, 0), SH::kVInLds ? OT::row_frag(vrow, s, 0) : vf[SH::kVInLds ? 0 : s]}; },
+            [&](int, Two f) { dp = Elem<T>::mma(f.o, f.v, dp); });
+      }
+      issue_next();
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const float4_t ls = *reinterpret_cast<const float4_t*>(&stat[rg][cur][c][8 * q + 4 * hl]);
+          const float4_t ls = lds_at<float4_t>(srow + c * 128 + q * 32);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) p[c][4 * q + j] = fast_exp2(fmaf(p[c][4 * q + j], c2, -ls[j]));
+          for (int j = 0; j < 4; ++j) p[c][4 * q + j] = fast_exp2(fmaf(p[c][4 * q + j], c2, ls[j]));
         }
         if (a.causal && i0 < kw0 + 31) {
 #pragma unroll
@@ -183,29 +194,20 @@ __global__ __launch_bounds__((64 * KvShape<T, HD, WHAT>::WAVES), (KvShape<T, HD,
             if (i0 + acc_row(r, hl) < key) p[c][r] = 0.f;
         }
       }
+      frag_t<T> fm[2], fs[2][2];
       if constexpr (DO_DV) {
         float16_t mix;
 #pragma unroll
         for (int r = 0; r < 16; ++r) mix[r] = fmaf(-lam, p[1][r], p[0][r]);
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          const frag_t<T> f = acc_frag<T>(mix, s);
-#pragma unroll
-          for (int d = 0; d < VB; ++d) dv[d] = Elem<T>::mma(f, OT::col_frag(tile + ocol, d, 16 * s * OT::kRowBytes), dv[d]);
-        }
+        for (int s = 0; s < 2; ++s) fm[s] = acc_frag<T>(mix, s);
       }
       if constexpr (DO_DK) {
-        float16_t dp = zero16();
-#pragma unroll
-        for (int s = 0; s < VS; ++s) {
-          const frag_t<T> v = SH::kVInLds ? OT::row_frag(vrow, s, 0) : vf[SH::kVInLds ? 0 : s];
-          dp = Elem<T>::mma(OT::row_frag(tile + orow, s, 0), v, dp);
-        }
         const float nl = -lam * lift;
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-          const float4_t d0 = *reinterpret_cast<const float4_t*>(&stat[rg][cur][2][8 * q + 4 * hl]);
-          const float4_t d1 = *reinterpret_cast<const float4_t*>(&stat[rg][cur][3][8 * q + 4 * hl]);
+          const float4_t d0 = lds_at<float4_t>(srow + 256 + q * 32);
+          const float4_t d1 = lds_at<float4_t>(srow + 384 + q * 32);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             const float x = dp[4 * q + j];
@@ -216,13 +218,19 @@ __global__ __launch_bounds__((64 * KvShape<T, HD, WHAT>::WAVES), (KvShape<T, HD,
 #pragma unroll
         for (int c = 0; c < 2; ++c)
 #pragma unroll
-          for (int s = 0; s < 2; ++s) {
-            const frag_t<T> f = acc_frag<T>(p[c], s);
-#pragma unroll
-            for (int d = 0; d < DB; ++d)
-              dk[c][d] = Elem<T>::mma(f, QT::col_frag(tile + qcol, d, c * SH::kHead + 16 * s * QT::kRowBytes), dk[c][d]);
-          }
+          for (int s = 0; s < 2; ++s) fs[c][s] = acc_frag<T>(p[c], s);
       }
+      if constexpr (SH::kDepth > 0) __builtin_amdgcn_sched_barrier(0);
+      if constexpr (DO_DV)
+        read_ahead<2 * VB, SH::kDepth>([&](int i) { return OT::col_frag(tile + ocol, i % VB, 16 * (i / VB) * OT::kRowBytes); },
+                                       [&](int i, frag_t<T> f) { dv[i % VB] = Elem<T>::mma(fm[i / VB], f, dv[i % VB]); });
+      if constexpr (DO_DK)
+        read_ahead<4 * DB, SH::kDepth>(
+            [&](int i) { return QT::col_frag(tile + qcol, i % DB, i / (2 * DB) * SH::kHead + 16 * (i / DB % 2) * QT::kRowBytes); },
+            [&](int i, frag_t<T> f) {
+              const int c = i / (2 * DB), s = i / DB % 2, d = i % DB;
+              dk[c][d] = Elem<T>::mma(fs[c][s], f, dk[c][d]);
+            });
     }
     g = g1;
     i0 = i1;
@@ -308,7 +316,7 @@ int diff_bwd_kv(const DiffArgs& args, int dtype, hipStream_t stream) {
     using T = decltype(t);
     constexpr int HD = decltype(hd)::value;
     const DiffArgs& a = args;
-    if constexpr (HD == 128) {
+    if constexpr (HD == 128 && sizeof(T) == 4) {
       const int rc = launch<T, HD, 1>(a, stream);
       return rc != TJ_OK ? rc : launch<T, HD, 2>(a, stream);
     } else {

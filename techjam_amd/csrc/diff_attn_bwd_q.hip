@@ -11,7 +11,8 @@
 // rounding of dS and of the result is 2.38e-3). What is left of its error is the
 // rounding of P in the forward product: the sum of P_m (dP - delta_m) over the
 // keys (P_m sums to 1). The dQ kernel adds it back to delta, exact then to what
-// fp32 sums are, for dlam and for dK, which come after it.
+// fp32 sums are, for dlam and for dK, which come after it, and leaves the rows'
+// numbers as the dK, dV kernel wants them.
 #include "diff_attn.h"
 
 namespace tj {
@@ -55,6 +56,10 @@ __global__ __launch_bounds__(kDiffThreads) void diff_delta_kernel(DiffArgs a, in
     if (lane == 0) {
       a.delta[map_at(a, b, head, 0, i)] = d0;
       a.delta[map_at(a, b, head, 1, i)] = d1;
+      if (i == a.Sq - 1)
+        for (int j = a.Sq; j < (int)stat_rows(a.Sq); ++j)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) *stat_at(a, b, head, j, c) = c < 2 ? -__builtin_inff() : 0.f;
     }
     if (n < 3e38f) peak_o = fmaxf(peak_o, n);  // not those that are not finite: they spoil their own row only
   }
@@ -257,8 +262,13 @@ diff_bwd_q_kernel(DiffArgs a) {
   if (r >= a.R) return;
   if (hl == 0) {
     a.gsum[row_at(a, t.b, head, i)] = live ? del[1] + rest[1] : 0.f;
+    // P is lifted by pl in its exponent; what multiplies P to dS takes that out again.
+    const float pl = p_lift<T>(a, t.hk), dl = lift / pl;
 #pragma unroll
-    for (int c = 0; c < 2; ++c) a.delta[map_at(a, t.b, head, c, i)] = live ? del[c] + rest[c] : 0.f;
+    for (int c = 0; c < 2; ++c) {
+      *stat_at(a, t.b, head, i, c) = live ? log2f(pl) - lse[c] : -__builtin_inff();
+      *stat_at(a, t.b, head, i, 2 + c) = live ? (del[c] + rest[c]) * (c == 0 ? -dl : lam * dl) : 0.f;
+    }
   }
   const float out = a.scale / lift;
 #pragma unroll
