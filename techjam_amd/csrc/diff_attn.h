@@ -439,12 +439,13 @@ __device__ __forceinline__ DiffTile diff_tile(const DiffArgs& a, int id, int til
   return t;
 }
 
-// Whether there are 128-row tiles enough for workgroups to take them rather than 64-row ones
-// (two rounds of them where two fit a CU, one where one does). Forward passes,
-// 128 / 64 rows: 64 dims bf16, 1024 tiles 436 / 453 us, 512 tiles of a causal
-// training step 520 / 466 us (whole step); 128 dims fp16, 290 tiles 68 / 81 us.
+// Whether there are 128-row tiles enough for workgroups to take them rather than 64-row ones:
+// two rounds of them where two fit a CU; where one does, one, and two of causal ones,
+// whose lengths differ. Forward passes, us with 128 / 64 rows: 64 dims bf16, 1024
+// tiles 436 / 453, 512 tiles of a causal training step 520 / 466 (whole step); 32 dims,
+// 1024 tiles 157 / 182; 128 dims, 290 tiles 68 / 81, causal 256 tiles 174 / 141, 512 tiles 227 / 280.
 inline bool wide_tiles(const DiffArgs& a, int hd) {
-  return (int64_t)a.B * a.Hk * ((a.R + 127) / 128) >= (hd == 128 ? 256 : 1024);
+  return (int64_t)a.B * a.Hk * ((a.R + 127) / 128) >= (hd == 128 ? (a.causal ? 512 : 256) : 1024);
 }
 
 int diff_fwd(const DiffArgs& a, int dtype, hipStream_t stream);

@@ -103,6 +103,7 @@ struct QShape {
   static constexpr int WAVES = 4;
   static constexpr int KG = !WIDE && HD * (int)sizeof(T) < 512 ? 2 : 1;
   static constexpr int RB = WAVES / KG;
+  static constexpr int kDepth = HD == 32 ? 0 : 2;  // fp32 d64: 281 -> 271 us (b2 h8 s2048); 16 bits: equal
   static constexpr int kBytes = 32 * (2 * HD + DVP) * (int)sizeof(T), kHead = 32 * HD * (int)sizeof(T);
 };
 
@@ -183,14 +184,11 @@ diff_bwd_q_kernel(DiffArgs a) {
     if (kv0 >= own_end) continue;
     const uint32_t tile = tiles + cur * kBytes;
     float16_t p[2], dp = zero16();
-#pragma unroll
-    for (int c = 0; c < 2; ++c) {
-      p[c] = zero16();
-#pragma unroll
-      for (int s = 0; s < KS; ++s) p[c] = Elem<T>::mma(KT::row_frag(tile + krow, s, c * kHead), qf[c][s], p[c]);
-    }
-#pragma unroll
-    for (int s = 0; s < VS; ++s) dp = Elem<T>::mma(VT::row_frag(tile + vrow, s, 0), of[s], dp);
+    p[0] = p[1] = zero16();
+    read_ahead<2 * KS, SH::kDepth>([&](int j) { return KT::row_frag(tile + krow, j % KS, j / KS * kHead); },
+                                   [&](int j, frag_t<T> f) { p[j / KS] = Elem<T>::mma(f, qf[j / KS][j % KS], p[j / KS]); });
+    read_ahead<VS, SH::kDepth>([&](int s) { return VT::row_frag(tile + vrow, s, 0); },
+                               [&](int s, frag_t<T> f) { dp = Elem<T>::mma(f, of[s], dp); });
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
 #pragma unroll
@@ -209,15 +207,18 @@ diff_bwd_q_kernel(DiffArgs a) {
       rest[1] += u;
       p[1][e] = u * nl;
     }
+    frag_t<T> fs[2][2];
 #pragma unroll
     for (int c = 0; c < 2; ++c)
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const frag_t<T> f = acc_frag<T>(p[c], s);
-#pragma unroll
-        for (int d = 0; d < DB; ++d)
-          dq[c][d] = Elem<T>::mma(KT::col_frag(tile + kcol, d, c * kHead + 16 * s * KT::kRowBytes), f, dq[c][d]);
-      }
+      for (int s = 0; s < 2; ++s) fs[c][s] = acc_frag<T>(p[c], s);
+    if constexpr (SH::kDepth > 0) __builtin_amdgcn_sched_barrier(0);
+    read_ahead<4 * DB, SH::kDepth>(
+        [&](int j) { return KT::col_frag(tile + kcol, j % DB, j / (2 * DB) * kHead + 16 * (j / DB % 2) * KT::kRowBytes); },
+        [&](int j, frag_t<T> f) {
+          const int c = j / (2 * DB), d = j % DB;
+          dq[c][d] = Elem<T>::mma(f, fs[c][j / DB % 2], dq[c][d]);
+        });
   }
 
   // The groups' sums, the upper half's added to the lower half's.
@@ -343,9 +344,12 @@ int diff_bwd_q(const DiffArgs& a, int dtype, hipStream_t stream) {
   const int rc = diff_dispatch(a, dtype, [&](auto t, auto hd) {
     using T = decltype(t);
     constexpr int HD = decltype(hd)::value;
-    if constexpr (QShape<T, HD, true>::RB != QShape<T, HD, false>::RB)
-      if (!wide_tiles(a, HD)) return launch_q<T, HD, false>(a, stream);
-    return launch_q<T, HD, true>(a, stream);
+    // 128-row tiles where two workgroups fit a CU: 320 / 360 us (b8 h16 s2048 d64 bf16,
+    // 2048 of them). Else 64 rows: 32 dims 184 / 183 us (1024 tiles), 128 dims
+    // 329 / 194, 405 / 365, 787 / 725 us (256, 512, 1024 tiles, causal).
+    if constexpr (HD == 64 && sizeof(T) == 2)
+      if (wide_tiles(a, HD)) return launch_q<T, HD, true>(a, stream);
+    return launch_q<T, HD, false>(a, stream);
   });
   if (rc != TJ_OK) return rc;
   hipLaunchKernelGGL(diff_dlam_kernel, dim3(a.n_lam), dim3(1024), 0, stream, a);

@@ -27,6 +27,11 @@ struct FwdShape {
   using VT = LdsRows<T, DVP>;
   static constexpr int KS = HD / 16;   // k-steps over the head dim
   static constexpr int DB = DVP / 32;  // output blocks
+  // Operands read ahead where the registers have room (us without / with): 128 dims,
+  // 186 / 174 and 154 / 141 (b2 h4 s4096 causal bf16, 128- and 64-row tiles), 64 dims in
+  // tiles of 64 keys 515 / 502 (b4 h16 s4096); in those of 32 it costs,
+  // 168 / 175, and so it does in fp32, 452 / 475 (b2 h4 s2048 d128).
+  static constexpr int kDepth = sizeof(T) == 2 && (HD == 128 || (HD == 64 && BN > 32)) ? 2 : 0;
   static constexpr int kElems = BN * (2 * HD + DVP);  // one tile of both key heads and of V
   static constexpr int kBytes = kElems * (int)sizeof(T), kHead = BN * HD * (int)sizeof(T);
 };
@@ -109,9 +114,8 @@ struct FwdState {
 #pragma unroll
     for (int c = 0; c < NM; ++c) {
       float16_t s = zero16();
-#pragma unroll
-      for (int ks = 0; ks < SH::KS; ++ks)
-        s = Elem<T>::mma(SH::KT::row_frag(kt, ks, c * SH::kHead + kb * 32 * SH::KT::kRowBytes), q[c][ks], s);
+      read_ahead<SH::KS, SH::kDepth>([&](int ks) { return SH::KT::row_frag(kt, ks, c * SH::kHead + kb * 32 * SH::KT::kRowBytes); },
+                                     [&](int ks, frag_t<T> f) { s = Elem<T>::mma(f, q[c][ks], s); });
       if (masked) {
 #pragma unroll
         for (int r = 0; r < 16; ++r)
@@ -147,14 +151,12 @@ struct FwdState {
         l[c] = frag_sum(p[c][st], l[c]);
       }
     }
+    read_ahead<2 * SH::DB, SH::kDepth>(
+        [&](int j) { return SH::VT::col_frag(vt, j % SH::DB, (kb * 32 + 16 * (j / SH::DB)) * SH::VT::kRowBytes); },
+        [&](int j, frag_t<T> f) {
 #pragma unroll
-    for (int st = 0; st < 2; ++st)
-#pragma unroll
-      for (int d = 0; d < SH::DB; ++d) {
-        const frag_t<T> vf = SH::VT::col_frag(vt, d, (kb * 32 + 16 * st) * SH::VT::kRowBytes);
-#pragma unroll
-        for (int c = 0; c < NM; ++c) o[c][d] = Elem<T>::mma(vf, p[c][st], o[c][d]);
-      }
+          for (int c = 0; c < NM; ++c) o[c][j % SH::DB] = Elem<T>::mma(f, p[c][j / SH::DB], o[c][j % SH::DB]);
+        });
   }
 
   // Adds the state of another group's wave over the same rows and other keys,
