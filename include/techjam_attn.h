@@ -403,8 +403,8 @@ int tj_narrow_ffn_norm(const float* x, const float* w_in, const float* bias_in, 
  * in memory, 64 of them within 2 GiB (TJ_ERR_UNSUPPORTED otherwise).
  *
  * lse and maps, both or neither: what tj_diff_attn_bwd reads again, contiguous
- * fp32: with R = Sq * H / Hk rows i * H / Hk + h % (H / Hk) per key head, the
- * rows' softmax sums [B, Hk, 2, R] and the two maps' outputs [B, Hk, R, 2, Dv].
+ * fp32: log2 of the rows' softmax sums [B, H, 2, Sq] and the two maps' outputs
+ * [B, H, Sq, 2, Dv], unrounded.
  *
  * workspace: tj_diff_attn_workspace_bytes bytes, 16-byte aligned, contents
  * irrelevant, calls sharing one ordered on one stream: where few rows sweep many
@@ -425,7 +425,7 @@ int tj_diff_attn_fwd(const void* q, const void* k, const void* v, void* o, int d
  * gradient dout [B, H, S, Dv]: dq, dk, dv (shaped and typed like q, k, v) and
  * dlam, fp32 [H] or [1] as lam_step says, summed over what shares a weight.
  * maps and lse come from the forward call. Rows at or past lengths[b] get zeros
- * and their dout is not read. The sums' order is fixed: the same call gives the
+ * and their dout is not read; with no rows at all nothing is written, dlam neither. The sums' order is fixed: the same call gives the
  * same bits. workspace as above, tj_diff_attn_bwd_workspace_bytes bytes, needed.
  */
 size_t tj_diff_attn_bwd_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t S);

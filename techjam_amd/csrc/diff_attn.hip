@@ -123,7 +123,7 @@ extern "C" int tj_diff_attn_fwd(const void* q, const void* k, const void* v, voi
   const DiffPlan p = plan(B, Hk, a.R, Sk, a.cached);
   const size_t need = part_bytes(p, B, Hk, a.R, Dv);
   // diff_join_kernel: a workgroup per row.
-  if (need != 0 && B * Hk * a.R >= (int64_t(1) << 24)) return TJ_ERR_SHAPE;
+  if ((p.few || need != 0) && B * Hk * a.R >= (int64_t(1) << 24)) return TJ_ERR_SHAPE;
   a.n_parts = 1;
   a.part_keys = (int)Sk;
   if (need != 0 && (p.few || workspace != nullptr)) {

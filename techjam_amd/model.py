@@ -488,9 +488,12 @@ class TransformerEncoder(nn.Module):
         """The forward pass of each sequence's first tokens (``x`` ``[B, S, D]``,
         right-padded by the mask) that leaves their keys and values in ``state``."""
         _not_captured()
-        state.longest = 0
-        state.reserve(x.shape[1])
+        self._check_state(x, state)
+        if x.shape[1] > state.capacity:
+            raise ValueError(f"{x.shape[1]} tokens exceed the cache's capacity of {state.capacity}")
         lengths = None if valid_token_mask is None else prefix_lengths(valid_token_mask)
+        state.lengths.zero_()  # a call that fails on its way leaves an empty state
+        state.longest = 0
         for layer, cache in zip(self.layers, state.layers):
             x = x + layer.attention(layer.norm1(x), valid_token_mask, True, lengths, cache)
             x = layer.ffn(x)
@@ -508,17 +511,30 @@ class TransformerEncoder(nn.Module):
         """The next ``T`` tokens of every sequence (``x`` ``[B, T, D]``): the
         encoder's output for them, their keys and values added to ``state``."""
         _not_captured()
-        if x.ndim != 3 or x.shape[0] != state.lengths.shape[0] or x.shape[1] == 0:
-            raise ValueError(f"x must be [{state.lengths.shape[0]}, T, {self.config.d_model}], not {tuple(x.shape)}")
+        self._check_state(x, state)
         tokens = x.shape[1]
+        if tokens == 0:
+            raise ValueError("a step has at least one token")
         state.reserve(tokens)
         place = state.lengths[:, None].long() + torch.arange(tokens, device=x.device)
-        state.lengths += tokens
-        state.longest += tokens
+        # The state counts the tokens when all layers have them: a refused call
+        # leaves it as it was.
+        lengths = state.lengths + tokens
         for layer, cache in zip(self.layers, state.layers):
-            x = x + layer.attention.step(layer.norm1(x), cache, state.lengths, place)
+            x = x + layer.attention.step(layer.norm1(x), cache, lengths, place)
             x = layer.ffn(x)
-        return self.final_norm(x)
+        x = self.final_norm(x)
+        state.lengths.copy_(lengths)
+        state.longest += tokens
+        return x
+
+    def _check_state(self, x, state) -> None:
+        b, d = state.lengths.shape[0], self.config.d_model
+        if x.ndim != 3 or x.shape[0] != b or x.shape[2] != d:
+            raise ValueError(f"x must be [{b}, T, {d}], not {tuple(x.shape)}")
+        head = (2 * self.config.num_heads, d // self.config.num_heads // 2)
+        if len(state.layers) != len(self.layers) or any((c.k.shape[1], c.k.shape[3]) != head for c in state.layers):
+            raise ValueError("the state is another model's")
 
     def _can_fuse_norms(self, x, valid_token_mask, valid_len) -> bool:
         d = x.shape[-1] if x.ndim == 3 else 0

@@ -98,3 +98,42 @@ def test_entry_points_refuse_before_launching():
     assert L.tj_diff_attn_workspace_bytes(64, 16, 16, 4096, 4096, 128, 0) == 0
     # existing entry points do not take bfloat16
     assert L.tj_attn_fwd(p, p, p, p, _lib.TJ_BF16, 1, 4, 128, 64, st, st, st, st, 0.125, 1, None, None, None, None) == _lib.TJ_ERR_DTYPE
+
+
+def test_refused_steps_leave_the_state_as_it_was():
+    from techjam_amd.model import TransformerConfig, TransformerEncoder
+
+    def model(layers=2, heads=2):
+        return TransformerEncoder(TransformerConfig(2, 8, 16, heads, 32, layers, True, attention="differential"))
+
+    m = model()
+    state = m.new_state(2, 8)
+    state.lengths.fill_(6)
+    state.longest = 6
+    for x in (torch.zeros(1, 9, 16), torch.zeros(1, 1, 16), torch.zeros(2, 9, 16), torch.zeros(2, 1, 8), torch.zeros(2, 16)):
+        with pytest.raises(ValueError):  # another batch would spread over the caches' rows; 9 exceed the capacity
+            m.prefill(x, state)
+    for x in (torch.zeros(1, 1, 16), torch.zeros(2, 3, 16), torch.zeros(2, 0, 16)):
+        with pytest.raises(ValueError):
+            m.step(x, state)
+    for other in (model(layers=3), model(heads=4)):
+        with pytest.raises(ValueError):
+            m.step(torch.zeros(2, 1, 16), other.new_state(2, 8))
+    # A call that is refused on its way (here: no kernels for CPU tensors) counts no tokens.
+    with pytest.raises(UnsupportedCaseError):
+        m.step(torch.zeros(2, 1, 16), state)
+    assert state.lengths.tolist() == [6, 6] and state.longest == 6
+    with pytest.raises(UnsupportedCaseError):
+        m.prefill(torch.zeros(2, 8, 16), state)
+    assert state.lengths.tolist() == [0, 0] and state.longest == 0
+
+
+def test_cache_without_room_is_refused_past_the_grid():
+    from techjam_amd.kernels import _lib
+
+    L = _lib.lib()
+    st = (_lib.ctypes.c_int64 * 4)(64, 64, 64, 1)
+    p, rows = 4096, 1 << 20
+    # 2^20 sequences of 16 tokens against caches of no capacity: a workgroup per row, 2^24 of them.
+    assert L.tj_diff_attn_fwd(p, p, p, p, _lib.TJ_F16, rows, 1, 1, 16, 0, 64, 64, st, st, st, st, 0.125, 1, 1, p, 1, p,
+                              None, None, None, 0, None) == _lib.TJ_ERR_SHAPE
