@@ -43,9 +43,11 @@ struct DiffArgs {
   const int32_t* len;      // [B] or null
   float* lse;              // [B, H, 2, Sq] log2 of a row's sum of 2^(score log2 e), +inf for empty rows; or null
   int n_mtiles;
-  // Key parts: part p covers keys p part_keys .. (p + 1) part_keys - 1 and leaves unnormalised sums
-  // [n_parts, B, Hk, R, 2, Dv] and (maximum, sum, sum before rounding, -) [n_parts, B, Hk, R, 2, 4].
-  int part_keys, n_parts;
+  // Key parts: n_parts of every sequence (part_keys), which leave unnormalised sums
+  // [n_parts, B, Hk, R, 2, Dv] and (maximum, sum, sum before rounding, -) [n_parts, B, Hk, R, 2, 4];
+  // or, for few rows, as many of each sequence as its length asks for (FewParts),
+  // n_parts in all, [n_parts, Hk, R, ...]. part_o null: sweeps run whole.
+  int n_parts, few_slots;
   float *part_o, *part_ml;
   // Backward.
   const void* dout;
@@ -358,6 +360,89 @@ __device__ __forceinline__ int diff_len(const DiffArgs& a, int b) {
   return __builtin_amdgcn_readfirstlane(n);
 }
 
+// Keys of one of n_parts parts of a sequence of L: they share the sequence, not
+// the capacity, so that a short sequence in a long cache is swept by as many.
+constexpr int kPartKeys = 512;
+__device__ __forceinline__ int part_keys(const DiffArgs& a, int L) {
+  return max(kPartKeys, ((L + a.n_parts - 1) / a.n_parts + 63) / 64 * 64);
+}
+
+// The parts of few-row sweeps: of at most `per` blocks of 32 keys, in the order of
+// the sequences, the same `per` for all of them, so that the waves of a ragged
+// batch end together (sixteen sequences of 16384 .. 65536 keys: 254 us, with as
+// many parts for each 284). few_slots times `per` cover all blocks for certain,
+// and with a part begun by every sequence that is few_slots + B = n_parts of them
+// at most; a smaller `per` is taken where its parts, counted, are no more. A whole
+// wave calls these.
+struct FewParts {
+  int b, first;   // sequence, its first part
+  int n, keys;    // its parts, and the keys of each
+  __device__ __forceinline__ static uint32_t blocks(const DiffArgs& a, int b) {
+    return b < a.B ? (uint32_t)(min(a.Sk, max(0, a.len[b])) + 31) / 32 : 0;
+  }
+  __device__ __forceinline__ static uint32_t wave_sum(uint32_t x) {
+#pragma unroll
+    for (int s = kWave / 2; s > 0; s >>= 1) x += __shfl_xor(x, s);
+    return x;
+  }
+  __device__ __forceinline__ static uint32_t blocks_per_part(const DiffArgs& a, int lane) {
+    if (a.B == 1) return max(1u, (blocks(a, 0) + a.n_parts - 1) / a.n_parts);
+    uint32_t sum = 0;
+    for (int b = lane; b < a.B; b += kWave) sum += blocks(a, b);
+    sum = wave_sum(sum);
+    for (uint32_t begun = a.B; begun > 0; begun = begun == (uint32_t)a.B ? begun / 2 : 0) {
+      const uint32_t per = max(1u, (sum + a.few_slots + begun - 1) / (a.few_slots + begun));
+      uint32_t n = 0;
+      for (int b = lane; b < a.B; b += kWave) n += (blocks(a, b) + per - 1) / per;
+      if (wave_sum(n) <= (uint32_t)a.n_parts) return per;
+    }
+    return max(1u, (sum + a.few_slots - 1) / a.few_slots);
+  }
+  __device__ __forceinline__ void take(const DiffArgs& a, uint32_t per) {
+    const uint32_t k = blocks(a, b);
+    n = (int)((k + per - 1) / per);
+    keys = n == 0 ? 0 : (int)((k + n - 1) / n) * 32;
+  }
+  // The sequence that `part` belongs to; false for none.
+  __device__ __forceinline__ bool find(const DiffArgs& a, int part, int lane) {
+    const uint32_t per = blocks_per_part(a, lane);
+    if (a.B == 1) {
+      b = first = 0;
+      take(a, per);
+      return part < n;
+    }
+    uint32_t before = 0;
+    for (int b0 = 0; b0 < a.B; b0 += kWave) {
+      const uint32_t own = (blocks(a, b0 + lane) + per - 1) / per;
+      uint32_t upto = own;
+#pragma unroll
+      for (int s = 1; s < kWave; s <<= 1) {
+        const uint32_t x = __shfl_up(upto, s);
+        if (lane >= s) upto += x;
+      }
+      const uint64_t past = __ballot((uint32_t)part < before + upto);
+      if (past != 0) {
+        const int at = __builtin_ctzll(past);
+        b = b0 + at;
+        first = (int)(before + __shfl(upto - own, at));
+        take(a, per);
+        return true;
+      }
+      before += __shfl(upto, kWave - 1);
+    }
+    return false;
+  }
+  // Sequence `seq`'s parts.
+  __device__ __forceinline__ void of(const DiffArgs& a, int seq, int lane) {
+    const uint32_t per = blocks_per_part(a, lane);
+    uint32_t before = 0;
+    for (int x = lane; x < seq; x += kWave) before += (blocks(a, x) + per - 1) / per;
+    b = seq;
+    first = (int)wave_sum(before);
+    take(a, per);
+  }
+};
+
 // Products with fp16 operands: the power of two that brings the largest
 // possible |dS| (2 |dO_i| |V_j| max(1, |lam|) scale) near 2^15, so that small
 // gradients and small probabilities keep fp16's bits. 1 for the other types.
@@ -437,6 +522,18 @@ __device__ __forceinline__ DiffTile diff_tile(const DiffArgs& a, int id, int til
   t.b = t.bh / a.Hk;
   t.hk = t.bh % a.Hk;
   return t;
+}
+
+// Parts (less one a sequence, FewParts) for `groups` workgroups of few rows in
+// all, as many as run at once: with more, one sequence of 65536 keys takes 49 us
+// instead of 38 (twice as many) and sixteen of them 382 instead of 364. At least
+// one more part per sequence, for long ones among short; none below 32 keys.
+constexpr int kCus = 256, kMostGroups = 8 * kCus;
+inline int few_slots(int64_t B, int64_t Hk, int64_t mtiles, int64_t Sk, int64_t groups) {
+  int64_t n = groups / (Hk * mtiles) - B;
+  if (n < B) n = B;
+  const int64_t most = B * (Sk > 0 ? (Sk + 31) / 32 : 1);
+  return (int)(n < most ? n : most);
 }
 
 // Whether there are 128-row tiles enough for workgroups to take them rather than 64-row ones:

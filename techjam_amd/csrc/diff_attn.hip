@@ -11,41 +11,28 @@ namespace {
 
 int elem_bytes(int dtype) { return dtype == TJ_F32 ? 4 : (dtype == TJ_F16 || dtype == TJ_BF16 ? 2 : 0); }
 
-// How a forward call runs: 32-row waves on their own (few rows) or 128-row
-// workgroups, the keys in n_parts parts.
+// How a forward call runs: 32-row waves on their own (few rows) or workgroups of
+// 64 or 128 rows; n_parts as in DiffArgs, the most a few-row kernel asks for.
 struct DiffPlan {
   bool few;
-  int64_t part_keys, n_parts;
+  int64_t n_parts;
 };
 
 // Rows of one key head up to which every wave works by itself.
 constexpr int64_t kFewRows = 64;
 
-// Few rows: 2048 waves (two rounds of the chip at 64 dims) or parts of 32 keys,
-// whichever is fewer. 2048 / 4096 / 8192 waves, sixteen sequences of up to 65536
-// keys: 288 / 306 / 318 us with the join; shortest part of 32 / 64 / 128 keys, one
-// sequence of 1024: 12.6 / 13.6 / 16 us. Else as many parts as fill 512
-// workgroups, of at least 512 keys.
+// More rows than few: as many parts as fill 512 workgroups, of at least kPartKeys keys.
 DiffPlan plan(int64_t B, int64_t Hk, int64_t R, int64_t Sk, bool cached) {
-  DiffPlan p{cached && R <= kFewRows, Sk, 1};
-  if (p.few) {
-    const int64_t tiles = B * Hk * ((R + 31) / 32), want = (2048 + tiles - 1) / tiles;
-    p.part_keys = ((Sk + want - 1) / want + 31) / 32 * 32;
-    if (p.part_keys < 32) p.part_keys = 32;
-  } else {
-    const int64_t tiles = B * Hk * ((R + 127) / 128);
-    if (tiles >= 256) return p;
-    const int64_t want = (512 + tiles - 1) / tiles;
-    p.part_keys = ((Sk + want - 1) / want + 63) / 64 * 64;
-    if (p.part_keys < 512) p.part_keys = 512;
-  }
-  p.n_parts = (Sk + p.part_keys - 1) / p.part_keys;
-  return p;
+  if (cached && R <= kFewRows) return {true, few_slots(B, Hk, (R + 31) / 32, Sk, kMostGroups) + B};
+  const int64_t tiles = B * Hk * ((R + 127) / 128);
+  if (tiles >= 256) return {false, 1};
+  const int64_t want = (512 + tiles - 1) / tiles, most = (Sk + kPartKeys - 1) / kPartKeys;
+  return {false, want < most ? want : most};
 }
 
 size_t part_bytes(const DiffPlan& p, int64_t B, int64_t Hk, int64_t R, int64_t Dv) {
   if (!p.few && p.n_parts <= 1) return 0;
-  const size_t rows = size_t(p.n_parts) * size_t(B) * size_t(Hk) * size_t(R) * 2;
+  const size_t rows = size_t(p.n_parts) * size_t(p.few ? 1 : B) * size_t(Hk) * size_t(R) * 2;
   return (rows * size_t(Dv) + rows * 4) * sizeof(float);
 }
 
@@ -91,7 +78,7 @@ using namespace tj;
 
 extern "C" size_t tj_diff_attn_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t Sq, int64_t Sk, int64_t Dv,
                                                int cached) {
-  if (!sizes_ok(B, H, Hk, Sq, Sk) || Dv <= 0 || Dv > 256 || B == 0 || Sq == 0 || Sk == 0) return 0;
+  if (!sizes_ok(B, H, Hk, Sq, Sk) || Dv <= 0 || Dv > 256 || B == 0 || Sq == 0) return 0;
   const int64_t R = Sq * (H / Hk);
   return part_bytes(plan(B, Hk, R, Sk, cached != 0), B, Hk, R, Dv);
 }
@@ -122,17 +109,15 @@ extern "C" int tj_diff_attn_fwd(const void* q, const void* k, const void* v, voi
   a.lam = lam; a.lam_step = (int)lam_step; a.len = lengths; a.lse = lse;
   const DiffPlan p = plan(B, Hk, a.R, Sk, a.cached);
   const size_t need = part_bytes(p, B, Hk, a.R, Dv);
-  // diff_join_kernel: a workgroup per row.
+  // diff_join_kernel: a workgroup per row. (A cache of no capacity still has rows to clear.)
   if ((p.few || need != 0) && B * Hk * a.R >= (int64_t(1) << 24)) return TJ_ERR_SHAPE;
   a.n_parts = 1;
-  a.part_keys = (int)Sk;
   if (need != 0 && (p.few || workspace != nullptr)) {
     if (workspace == nullptr || workspace_bytes < need) return TJ_ERR_WORKSPACE;
     if (!tjh::aligned16(workspace)) return TJ_ERR_ALIGN;
     a.n_parts = (int)p.n_parts;
-    a.part_keys = (int)p.part_keys;
     a.part_o = static_cast<float*>(workspace);
-    a.part_ml = a.part_o + p.n_parts * B * Hk * a.R * 2 * Dv;
+    a.part_ml = a.part_o + need / sizeof(float) / (Dv + 4) * Dv;
   }
   return p.few ? diff_few_rows(a, dtype, stream) : diff_fwd(a, dtype, stream);
 }

@@ -12,7 +12,13 @@
 // rounding of P in the forward product: the sum of P_m (dP - delta_m) over the
 // keys (P_m sums to 1). The dQ kernel adds it back to delta, exact then to what
 // fp32 sums are, for dlam and for dK, which come after it, and leaves the rows'
-// numbers as the dK, dV kernel wants them.
+// numbers as the dK, dV kernel wants them. dS itself is rounded to the operands'
+// type for the product, as is the result, two roundings where fp32 products
+// have one: the error of dQ is 1.45 times theirs at 64 dims and 1.6 at 16, where
+// the sum of dS K cancels more (fp32 MFMAs would take 16 times as long).
+//
+// b2 h8 key heads 4 s4096 d64 bf16 causal: dQ 139 us, 740 TFLOP/s of its 8D + 2Dv
+// operations a pair, matrix units busy 39 %, vector units 57 %; delta 14 us, 6 TB/s.
 #include "diff_attn.h"
 
 namespace tj {

@@ -8,10 +8,17 @@
 // accumulator and share every V fragment.
 //
 // diff_fwd_kernel: a workgroup = RB blocks of 32 rows of one (b, key head) times
-// KG groups, a wave each; key tiles of 32 stream through LDS, dealt to the groups
-// in turn, and the groups' sums meet in LDS at the end. diff_few_kernel: a
+// KG groups, a wave each; key tiles of 32 or 64 stream through LDS, dealt to the
+// groups in turn, and the groups' sums meet in LDS at the end. diff_few_kernel: a
 // workgroup = one wave = 32 rows and one part of the keys, with its own LDS tile.
 // Sweeps cut into parts are joined by diff_join_kernel.
+//
+// Long sequences are bound by the matrix and vector units together: b2 h8 s8192
+// d64 bf16 causal takes 425 us, 970 TFLOP/s of its own 4D + 4Dv operations a pair
+// (a large library product of that type runs at 1144), matrix units busy 53 % and
+// vector units 58 % of the time, no LDS bank conflicts. Few rows are bound by the
+// cache's bytes: 16 sequences of 16384 to 65536 keys, 4 key heads, d64 bf16, one
+// token: 240 us + 7 us of joining, 5.6 TB/s (a copy of 1 GiB: 5.1).
 #include "diff_attn.h"
 
 namespace tj {
@@ -198,10 +205,10 @@ struct FwdState {
     }
   }
 
-  // The results of a part of the keys.
-  __device__ __forceinline__ void finish_part(const DiffArgs& a, int bh, const DiffRow& row, int part, int lane) {
+  // The results of a part of the keys, whose row 0 has number `rows` of all.
+  __device__ __forceinline__ void finish_part(const DiffArgs& a, int64_t rows, const DiffRow& row, int lane) {
     const int hl = lane / 32;
-    const int64_t slot = ((int64_t)part * a.B * a.Hk + bh) * a.R + row.r;
+    const int64_t slot = rows + row.r;
 #pragma unroll
     for (int c = 0; c < NM; ++c) {
       const float sum = pair_sum(l[c]), exact = STATS ? pair_sum(e[STATS ? c : 0]) : 0.f;
@@ -336,8 +343,8 @@ diff_fwd_kernel(DiffArgs a) {
   const int r0 = mt * ROWS, rw0 = r0 + 32 * rb;
   const DiffSpan all(a, r0, r0 + ROWS - 1, L), own(a, rw0, rw0 + 31, L);
   const DiffRow row(a, rw0 + lane % 32, L);
-  const int kv_begin = PART ? part * a.part_keys : 0;
-  const int kv_end = PART ? min(all.end, kv_begin + a.part_keys) : all.end;
+  const int n_keys = PART ? part_keys(a, L) : 0, kv_begin = PART ? part * n_keys : 0;
+  const int kv_end = PART ? min(all.end, kv_begin + n_keys) : all.end;
   if (PART && kv_begin >= kv_end) return;  // not read either (live parts are counted from the rows' last key)
   const uint32_t tiles = lds_offset(smem) + kg * 2 * SH::kBytes;
   KeyTiles<T, SH, HD, RB * GR::kPairs> keys;
@@ -372,7 +379,7 @@ diff_fwd_kernel(DiffArgs a) {
     if (kg != 0) return;
   }
   if constexpr (PART) {
-    if (kg == 0) st.finish_part(a, t.bh, row, part, lane);
+    if (kg == 0) st.finish_part(a, ((int64_t)part * a.B * a.Hk + t.bh) * a.R, row, lane);
   } else {
     st.finish(a, t.b, t.hk, row, reinterpret_cast<float4_t*>(smem) + rb * State::kGive, lane, kg == 0);
   }
@@ -384,19 +391,22 @@ __global__ __launch_bounds__(2 * kWave / kMaps<HD>) void diff_few_kernel(DiffArg
   using SH = FwdShape<T, HD, BN>;
   __shared__ __attribute__((aligned(1024))) T smem[2][SH::kElems];
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
-  const DiffTile t = diff_tile(a, blockIdx.x, a.n_mtiles * a.n_parts);
-  const int mt = t.tile % a.n_mtiles, part = t.tile / a.n_mtiles;
-  const int L = diff_len(a, t.b);
+  const int mt = blockIdx.x % a.n_mtiles, hk = blockIdx.x / a.n_mtiles % a.Hk, part = blockIdx.x / a.n_mtiles / a.Hk;
+  FewParts f;
+  if (!f.find(a, part, lane)) return;
+  const int b = __builtin_amdgcn_readfirstlane(f.b);
+  const int L = diff_len(a, b);
   const DiffSpan own(a, mt * 32, mt * 32 + 31, L);
   const DiffRow row(a, mt * 32 + lane % 32, L);
-  const int kv_begin = part * a.part_keys, kv_end = min(own.end, kv_begin + a.part_keys);
+  const int kv_begin = __builtin_amdgcn_readfirstlane((part - f.first) * f.keys);
+  const int kv_end = min(own.end, kv_begin + __builtin_amdgcn_readfirstlane(f.keys));
   if (kv_begin >= kv_end) return;
   const uint32_t tiles = lds_offset(smem);
   KeyTiles<T, SH, HD, 2 / NM> keys;
-  keys.init(a, t.b, t.hk, w, lane);
+  keys.init(a, b, hk, w, lane);
   keys.issue(a, kv_begin, L, tiles, w);
   FwdState<T, HD, BN, NM, false> st;
-  st.init(a, t.b, t.hk, row, w, lane);
+  st.init(a, b, hk, row, w, lane);
   int cur = 0;
   for (int kv0 = kv_begin; kv0 < kv_end; kv0 += BN, cur ^= 1) {
     wait_copies();
@@ -404,7 +414,7 @@ __global__ __launch_bounds__(2 * kWave / kMaps<HD>) void diff_few_kernel(DiffArg
     if (kv0 + BN < kv_end) keys.issue(a, kv0 + BN, L, tiles + (cur ^ 1) * SH::kBytes, w);
     st.step(tiles + cur * SH::kBytes, 0, kv0, row.limit, kv0 + BN - 1 > own.free, lane);
   }
-  st.finish_part(a, t.bh, row, part, lane);
+  st.finish_part(a, ((int64_t)part * a.Hk + hk) * a.R, row, lane);
 }
 
 // Joins the parts: O_m = sum_p 2^(max_p - M) o_p / sum_p 2^(max_p - M) sum_p,
@@ -418,11 +428,22 @@ __global__ __launch_bounds__(kDiffThreads) void diff_join_kernel(DiffArgs a, int
   __shared__ float4_t sum[kDiffThreads];
   __shared__ float top[2][kDiffThreads / kWave], total[2][kDiffThreads];
   const int tid = threadIdx.x;
-  const int64_t n_rows = (int64_t)a.B * a.Hk * a.R, id = blockIdx.x;
-  const int bh = (int)(id / a.R), b = bh / a.Hk, hk = bh % a.Hk;
+  const int bh = blockIdx.x / a.R, b = bh / a.Hk, hk = bh % a.Hk;
   const int L = diff_len(a, b);
-  const DiffRow row(a, (int)(id % a.R), L);
-  const int np = row.live ? row.limit / a.part_keys + 1 : 0;
+  const DiffRow row(a, blockIdx.x % a.R, L);
+  // The row's number in the first part, and from one part to the next.
+  int64_t id = blockIdx.x, n_rows = (int64_t)a.B * a.Hk * a.R;
+  int n_keys;
+  if (a.few_slots != 0) {
+    FewParts f;
+    f.of(a, b, tid % kWave);
+    id = ((int64_t)f.first * a.Hk + hk) * a.R + row.r;
+    n_rows = (int64_t)a.Hk * a.R;
+    n_keys = f.keys;
+  } else {
+    n_keys = part_keys(a, L);
+  }
+  const int np = row.live ? row.limit / n_keys + 1 : 0;
   const float4_t* ml = reinterpret_cast<const float4_t*>(a.part_ml) + id * 2;  // part p, map c: [p * n_rows * 2 + c]
   float m[2] = {-__builtin_inff(), -__builtin_inff()};
   for (int p = tid; p < np; p += kDiffThreads)
@@ -536,9 +557,14 @@ int diff_few_rows(const DiffArgs& args, int dtype, hipStream_t stream) {
     using T = decltype(t);
     constexpr int HD = decltype(hd)::value;
     DiffArgs a = args;
+    constexpr int kWaves = 2 / kMaps<HD>, kLds = 2 * FwdShape<T, HD, 32>::kBytes;
+    // What the LDS and the registers hold at once: two waves a SIMD at 32 dims, else one.
+    constexpr int kByLds = 160 * 1024 / kLds, kByRegs = (HD == 32 ? 8 : 4) / kWaves;
     a.n_mtiles = (a.R + 31) / 32;
-    hipLaunchKernelGGL((diff_few_kernel<T, HD>), dim3(uint32_t((int64_t)a.B * a.Hk * a.n_mtiles * a.n_parts)),
-                       dim3(2 * kWave / kMaps<HD>), 0, stream, a);
+    a.few_slots = few_slots(a.B, a.Hk, a.n_mtiles, a.Sk, kCus * (kByLds < kByRegs ? kByLds : kByRegs));
+    a.n_parts = a.few_slots + a.B;
+    hipLaunchKernelGGL((diff_few_kernel<T, HD>), dim3(uint32_t((int64_t)a.n_parts * a.Hk * a.n_mtiles)), dim3(kWave * kWaves), 0,
+                       stream, a);
     const int rc = tjh::launch_status();
     return rc != TJ_OK ? rc : launch_join<T>(a, stream);
   });

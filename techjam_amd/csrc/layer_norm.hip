@@ -13,7 +13,9 @@
 // bases are multiples of that, one element otherwise. Loads and stores go through
 // bounds-checked buffers with an offset outside for what is not there, so that a
 // row's accesses are all in flight at once (with a branch around each, 65536 rows
-// of 2048 bf16 took 204 us forward and 226 us backward).
+// of 2048 bf16 took 204 us forward and 226 us backward). Now 88 us forward, 6.1 TB/s,
+// and 155 us backward, 5.2 TB/s (a copy of 1
+// GiB: 5.1); 131072 rows of 128 fp16: 13 and 22 us.
 #include "tj_common.h"
 
 typedef __bf16 bf16_t;

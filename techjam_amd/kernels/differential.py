@@ -240,6 +240,10 @@ def differential_attention_cached(
     (a sequence shorter than ``T``, an empty slot of the batch) get zeros. Lengths
     are clipped to ``C``, and what the caches hold behind them is not read.
 
+    How the keys are shared among the GPU's units follows the batch's lengths, so
+    a sequence's last bits may differ beside other sequences; equal calls give
+    equal bits.
+
     Layouts, types and ``lam`` as in :func:`differential_attention`. No
     gradients: inputs that require them are refused while they are enabled.
     """
