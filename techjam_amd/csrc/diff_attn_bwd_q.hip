@@ -17,7 +17,7 @@
 // have one: the error of dQ is 1.45 times theirs at 64 dims and 1.6 at 16, where
 // the sum of dS K cancels more (fp32 MFMAs would take 16 times as long).
 //
-// b2 h8 key heads 4 s4096 d64 bf16 causal: dQ 139 us, 740 TFLOP/s of its 8D + 2Dv
+// b2 h8 key heads 4 s4096 d64 bf16 causal: dQ 144 us, 716 TFLOP/s of its 8D + 2Dv
 // operations a pair, matrix units busy 39 %, vector units 57 %; delta 14 us, 6 TB/s.
 #include "diff_attn.h"
 
@@ -154,6 +154,11 @@ diff_bwd_q_kernel(DiffArgs a) {
   int kv0 = BN * kg;
   if (kv0 < kv_end) issue(kv0, tiles);
 
+  // Every other token works with -dO and -dP: the matrix unit's sums lean to minus
+  // infinity, which dlam, the sum of all rows, would keep (b8 h4 s1024 d64 fp16: its
+  // error 3.0e-5 in every one of eight draws, now 0 to 7e-6 of either sign).
+  const bool odd = i % 2 != 0;
+  const float sign = odd ? -1.f : 1.f;
   frag_t<T> qf[2][KS], of[VS];
   {
     const T* qp = reinterpret_cast<const T*>(a.q) + (live ? a.vq.row(t.b, 2 * head, i) : 0);
@@ -163,7 +168,12 @@ diff_bwd_q_kernel(DiffArgs a) {
 #pragma unroll
       for (int s = 0; s < KS; ++s) qf[c][s] = load_frag<T>(live ? qp + c * a.vq.sh : nullptr, 16 * s + 8 * hl, a.D);
 #pragma unroll
-    for (int s = 0; s < VS; ++s) of[s] = load_frag<T>(live ? op : nullptr, 16 * s + 8 * hl, a.Dv);
+    for (int s = 0; s < VS; ++s) {
+      of[s] = load_frag<T>(live ? op : nullptr, 16 * s + 8 * hl, a.Dv);
+      if (odd)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) of[s][j] = -of[s][j];
+    }
   }
   float16_t dq[2][DB];
 #pragma unroll
@@ -179,8 +189,10 @@ diff_bwd_q_kernel(DiffArgs a) {
     lse[c] = live ? a.lse[map_at(a, t.b, head, c, i)] : __builtin_inff();
     del[c] = live ? a.delta[map_at(a, t.b, head, c, i)] : 0.f;
   }
-  const float d0 = -del[0] * lift, nl = -lam * lift;
-  float rest[2] = {0.f, 0.f};
+  const float d0 = -del[0] * lift, nl = -lam * lift, signed_lift = sign * lift;
+  // With what the additions lost: a row's terms one after another would leave some
+  // 1e-6 of the sum of thousands. Both together cost 140 -> 144 us (b2 h8 s4096).
+  float rest[2] = {0.f, 0.f}, lost[2] = {0.f, 0.f};
 
   // The workgroup goes round together, the last round maybe without a tile for every group.
   for (int first = 0, cur = 0; first < kv_end; first += KG * BN, kv0 += KG * BN, cur ^= 1) {
@@ -205,13 +217,20 @@ diff_bwd_q_kernel(DiffArgs a) {
           if (kv0 + acc_row(e, hl) > limit) p[c][e] = 0.f;
       }
     }
+    float sum[2] = {0.f, 0.f};
 #pragma unroll
     for (int e = 0; e < 16; ++e) {
-      p[0][e] *= fmaf(dp[e], lift, d0);
-      rest[0] += p[0][e];
-      const float u = p[1][e] * (dp[e] - del[1]);
-      rest[1] += u;
+      p[0][e] *= fmaf(dp[e], signed_lift, d0);
+      sum[0] += p[0][e];
+      const float u = p[1][e] * fmaf(dp[e], sign, -del[1]);
+      sum[1] += u;
       p[1][e] = u * nl;
+    }
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const float y = sum[c] - lost[c], x = rest[c] + y;
+      lost[c] = (x - rest[c]) - y;
+      rest[c] = x;
     }
     frag_t<T> fs[2][2];
 #pragma unroll
