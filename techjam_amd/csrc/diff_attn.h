@@ -545,6 +545,11 @@ inline bool wide_tiles(const DiffArgs& a, int hd) {
   return (int64_t)a.B * a.Hk * ((a.R + 127) / 128) >= (hd == 128 ? (a.causal ? 512 : 256) : 1024);
 }
 
+// Workgroups of four waves have `blocks` blocks of 32 rows (4, 2 or 1) times 4 / blocks
+// groups of key tiles. Whether two tiles for each of those groups fit the LDS.
+template <typename T, int HD>
+constexpr bool row_blocks_fit(int blocks) { return 4 / blocks * HD * (int)sizeof(T) <= 512; }
+
 int diff_fwd(const DiffArgs& a, int dtype, hipStream_t stream);
 int diff_few_rows(const DiffArgs& a, int dtype, hipStream_t stream);
 int diff_bwd_kv(const DiffArgs& a, int dtype, hipStream_t stream);

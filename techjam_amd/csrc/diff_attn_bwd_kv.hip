@@ -32,11 +32,12 @@ namespace {
 // s4096 bf16.) Eight waves, two a SIMD, where their registers allow it, else four;
 // as many groups as have room for two tiles each (at most 128 KB of LDS), so that a
 // tile is on its way while one is worked on.
-template <typename T, int HD, int WHAT>
+// HALF: half of the key blocks, and so of the waves, a workgroup.
+template <typename T, int HD, int WHAT, bool HALF>
 struct KvShape {
   static constexpr int DVP = 2 * HD;
-  static constexpr int WAVES = (sizeof(T) == 2 && HD <= 64) || HD == 32 ? 8 : 4;
-  static constexpr int RG = 512 / (HD * (int)sizeof(T)) < WAVES / 2 ? 512 / (HD * (int)sizeof(T)) : WAVES / 2;
+  static constexpr int kWhole = (sizeof(T) == 2 && HD <= 64) || HD == 32 ? 8 : 4, WAVES = HALF ? kWhole / 2 : kWhole;
+  static constexpr int RG = 512 / (HD * (int)sizeof(T)) < kWhole / 2 ? 512 / (HD * (int)sizeof(T)) : kWhole / 2;
   static constexpr int KB = WAVES / RG;
   // What of the keys' rows stays in LDS, as the registers have no room for it.
   static constexpr bool kK1InLds = WHAT == 3 && HD == 128;
@@ -47,9 +48,9 @@ struct KvShape {
   static constexpr int kBytes = kTile * (int)sizeof(T), kHead = 32 * HD * (int)sizeof(T);
 };
 
-template <typename T, int HD, int WHAT>
-__global__ __launch_bounds__((64 * KvShape<T, HD, WHAT>::WAVES), (KvShape<T, HD, WHAT>::WAVES / 4)) void diff_bwd_kv_kernel(DiffArgs a) {
-  using SH = KvShape<T, HD, WHAT>;
+template <typename T, int HD, int WHAT, bool HALF>
+__global__ __launch_bounds__((64 * KvShape<T, HD, WHAT, HALF>::WAVES), (KvShape<T, HD, WHAT, HALF>::WAVES / 4)) void diff_bwd_kv_kernel(DiffArgs a) {
+  using SH = KvShape<T, HD, WHAT, HALF>;
   constexpr int DVP = SH::DVP, KS = HD / 16, VS = DVP / 16, DB = HD / 32, VB = DVP / 32, BM = 32;
   constexpr int KB = SH::KB, RG = SH::RG, WAVES = SH::WAVES;
   constexpr bool DO_DV = (WHAT & 1) != 0, DO_DK = (WHAT & 2) != 0;
@@ -306,12 +307,17 @@ p[0] = p[1] = zero16();
   }
 }
 
-template <typename T, int HD, int WHAT>
+template <typename T, int HD, int WHAT, bool HALF = false>
 int launch(DiffArgs a, hipStream_t stream) {
-  constexpr int kKeys = 32 * KvShape<T, HD, WHAT>::KB;
+  using SH = KvShape<T, HD, WHAT, HALF>;
+  constexpr int kKeys = 32 * SH::KB;
   a.n_mtiles = (a.Sk + kKeys - 1) / kKeys;
-  hipLaunchKernelGGL((diff_bwd_kv_kernel<T, HD, WHAT>), dim3(uint32_t((int64_t)a.B * a.Hk * a.n_mtiles)),
-                     dim3(64 * KvShape<T, HD, WHAT>::WAVES), 0, stream, a);
+  // Where half of the CUs would have no work, us with 64 keys a workgroup / 32: b1 h1 s8192
+  // d64 bf16 163 / 138, h2 s4096 87 / 74, h8 s1024 d32 fp32 80 / 53; 192 workgroups of 64: 32 / 36.
+  if constexpr (!HALF && SH::WAVES == 8)
+    if ((int64_t)a.B * a.Hk * a.n_mtiles <= kCus / 2) return launch<T, HD, WHAT, true>(a, stream);
+  hipLaunchKernelGGL((diff_bwd_kv_kernel<T, HD, WHAT, HALF>), dim3(uint32_t((int64_t)a.B * a.Hk * a.n_mtiles)),
+                     dim3(64 * SH::WAVES), 0, stream, a);
   return tjh::launch_status();
 }
 

@@ -101,22 +101,21 @@ __global__ __launch_bounds__(kDiffThreads) void diff_delta_kernel(DiffArgs a, in
 // LDS in tiles of 32 dealt to the groups in turn, whose sums meet in LDS at the
 // end. Scores transposed as in the forward kernel: a row's sums are its lane's
 // own numbers, and dS turns into the B operand of dQ^T = K^T dS^T. Four waves;
-// 128 rows where those fill the chip, 64 (WIDE false) with two groups otherwise,
-// if two tiles for each fit.
-template <typename T, int HD, bool WIDE>
+// 128 rows, or 64 with two groups, or 32 with four, if two tiles for each fit.
+template <typename T, int HD, int BLOCKS>
 struct QShape {
   static constexpr int DVP = 2 * HD;
   static constexpr int WAVES = 4;
-  static constexpr int KG = !WIDE && HD * (int)sizeof(T) < 512 ? 2 : 1;
-  static constexpr int RB = WAVES / KG;
+  static constexpr int RB = BLOCKS, KG = WAVES / RB;
+  static_assert(row_blocks_fit<T, HD>(BLOCKS), "two tiles a group");
   static constexpr int kDepth = HD == 32 ? 0 : 2;  // fp32 d64: 281 -> 271 us (b2 h8 s2048); 16 bits: equal
   static constexpr int kBytes = 32 * (2 * HD + DVP) * (int)sizeof(T), kHead = 32 * HD * (int)sizeof(T);
 };
 
-template <typename T, int HD, bool WIDE>
-__global__ __launch_bounds__((64 * QShape<T, HD, WIDE>::WAVES), (HD == 32 || (sizeof(T) == 2 && HD == 64) ? 2 : 1)) void
+template <typename T, int HD, int BLOCKS>
+__global__ __launch_bounds__((64 * QShape<T, HD, BLOCKS>::WAVES), (HD == 32 || (sizeof(T) == 2 && HD == 64) ? 2 : 1)) void
 diff_bwd_q_kernel(DiffArgs a) {
-  using SH = QShape<T, HD, WIDE>;
+  using SH = QShape<T, HD, BLOCKS>;
   constexpr int DVP = SH::DVP, KS = HD / 16, VS = DVP / 16, DB = HD / 32, BN = 32, RB = SH::RB, KG = SH::KG, ROWS = 32 * RB;
   constexpr int kBytes = SH::kBytes, kHead = SH::kHead;
   using KT = LdsRows<T, HD>;
@@ -313,11 +312,11 @@ diff_bwd_q_kernel(DiffArgs a) {
   }
 }
 
-template <typename T, int HD, bool WIDE>
+template <typename T, int HD, int BLOCKS>
 int launch_q(DiffArgs a, hipStream_t stream) {
-  using SH = QShape<T, HD, WIDE>;
+  using SH = QShape<T, HD, BLOCKS>;
   a.n_mtiles = (a.R + 32 * SH::RB - 1) / (32 * SH::RB);
-  hipLaunchKernelGGL((diff_bwd_q_kernel<T, HD, WIDE>), dim3(uint32_t((int64_t)a.B * a.Hk * a.n_mtiles)),
+  hipLaunchKernelGGL((diff_bwd_q_kernel<T, HD, BLOCKS>), dim3(uint32_t((int64_t)a.B * a.Hk * a.n_mtiles)),
                      dim3(64 * SH::WAVES), 0, stream, a);
   return tjh::launch_status();
 }
@@ -373,8 +372,13 @@ int diff_bwd_q(const DiffArgs& a, int dtype, hipStream_t stream) {
     // 2048 of them). Else 64 rows: 32 dims 184 / 183 us (1024 tiles), 128 dims
     // 329 / 194, 405 / 365, 787 / 725 us (256, 512, 1024 tiles, causal).
     if constexpr (HD == 64 && sizeof(T) == 2)
-      if (wide_tiles(a, HD)) return launch_q<T, HD, true>(a, stream);
-    return launch_q<T, HD, false>(a, stream);
+      if (wide_tiles(a, HD)) return launch_q<T, HD, 4>(a, stream);
+    // 32 rows where 64 leave half of the CUs without work, us with 64 / 32: b1 h1 s8192
+    // d64 bf16 (128 tiles of 64) 146 / 103, h2 s4096 77 / 56, h8 s1024 25 / 20 (d32: 18 / 12),
+    // h12 s1024 (192 tiles) 24.8 / 25.1.
+    if constexpr (row_blocks_fit<T, HD>(1))
+      if ((int64_t)a.B * a.Hk * ((a.R + 63) / 64) <= kCus / 2) return launch_q<T, HD, 1>(a, stream);
+    return launch_q<T, HD, row_blocks_fit<T, HD>(2) ? 2 : 4>(a, stream);
   });
   if (rc != TJ_OK) return rc;
   hipLaunchKernelGGL(diff_dlam_kernel, dim3(a.n_lam), dim3(1024), 0, stream, a);

@@ -311,21 +311,22 @@ constexpr int kMaps = HD <= 64 ? 2 : 1;
 // maps. Four (eight of one map), so that two workgroups share a CU where the
 // registers allow it, and one's products run beside the other's exponentials:
 // eight waves meeting at one barrier were 15 % slower on the long bf16 case. 128
-// rows where those fill the chip, 64 (WIDE false) with two groups otherwise,
-// if two tiles for each fit.
-template <typename T, int HD, bool WIDE>
+// rows where those fill the chip, else 64 with two groups, if two tiles for each
+// fit. (32 rows with four: b1 h4 s512 20.3 against 19.7 us, and twice the time where
+// the keys are in parts.)
+template <typename T, int HD, int BLOCKS>
 struct FwdGroups {
   static constexpr int kPairs = 2 / kMaps<HD>;
-  static constexpr int KG = !WIDE && HD * (int)sizeof(T) < 512 ? 2 : 1;
-  static constexpr int RB = 4 / KG;
+  static constexpr int RB = BLOCKS, KG = 4 / RB;
+  static_assert(row_blocks_fit<T, HD>(BLOCKS), "two tiles a group");
   static constexpr int WAVES = 4 * kPairs;
   static constexpr int BN = KG == 1 && HD * (int)sizeof(T) <= 256 ? 64 : 32;
 };
 
-template <typename T, int HD, bool WIDE, bool PART, bool STATS>
-__global__ __launch_bounds__((64 * FwdGroups<T, HD, WIDE>::WAVES), (sizeof(T) == 4 && HD == 64 ? 1 : 2)) void
+template <typename T, int HD, int BLOCKS, bool PART, bool STATS>
+__global__ __launch_bounds__((64 * FwdGroups<T, HD, BLOCKS>::WAVES), (sizeof(T) == 4 && HD == 64 ? 1 : 2)) void
 diff_fwd_kernel(DiffArgs a) {
-  using GR = FwdGroups<T, HD, WIDE>;
+  using GR = FwdGroups<T, HD, BLOCKS>;
   constexpr int BN = GR::BN;
   using SH = FwdShape<T, HD, BN>;
   using State = FwdState<T, HD, BN, kMaps<HD>, STATS>;
@@ -519,25 +520,25 @@ int launch_join(const DiffArgs& a, hipStream_t stream) {
 }  // namespace
 
 namespace {
-template <typename T, int HD, bool WIDE>
+template <typename T, int HD, int BLOCKS>
 int launch_fwd(DiffArgs a, hipStream_t stream) {
-  using GR = FwdGroups<T, HD, WIDE>;
+  using GR = FwdGroups<T, HD, BLOCKS>;
   a.n_mtiles = (a.R + 32 * GR::RB - 1) / (32 * GR::RB);
   const int64_t n = (int64_t)a.B * a.Hk * a.n_mtiles;
   if (a.n_parts > 1) {
-    hipLaunchKernelGGL((diff_fwd_kernel<T, HD, WIDE, true, true>), dim3(uint32_t(n * a.n_parts)), dim3(64 * GR::WAVES), 0,
+    hipLaunchKernelGGL((diff_fwd_kernel<T, HD, BLOCKS, true, true>), dim3(uint32_t(n * a.n_parts)), dim3(64 * GR::WAVES), 0,
                        stream, a);
     const int rc = tjh::launch_status();
     return rc != TJ_OK ? rc : launch_join<T>(a, stream);
   }
   // Without statistics the long sweeps of 128-row workgroups save the second sum.
-  if constexpr (WIDE) {
+  if constexpr (BLOCKS == 4) {
     if (a.lse == nullptr) {
-      hipLaunchKernelGGL((diff_fwd_kernel<T, HD, WIDE, false, false>), dim3(uint32_t(n)), dim3(64 * GR::WAVES), 0, stream, a);
+      hipLaunchKernelGGL((diff_fwd_kernel<T, HD, BLOCKS, false, false>), dim3(uint32_t(n)), dim3(64 * GR::WAVES), 0, stream, a);
       return tjh::launch_status();
     }
   }
-  hipLaunchKernelGGL((diff_fwd_kernel<T, HD, WIDE, false, true>), dim3(uint32_t(n)), dim3(64 * GR::WAVES), 0, stream, a);
+  hipLaunchKernelGGL((diff_fwd_kernel<T, HD, BLOCKS, false, true>), dim3(uint32_t(n)), dim3(64 * GR::WAVES), 0, stream, a);
   return tjh::launch_status();
 }
 }  // namespace
@@ -546,9 +547,9 @@ int diff_fwd(const DiffArgs& a, int dtype, hipStream_t stream) {
   return diff_dispatch(a, dtype, [&](auto t, auto hd) {
     using T = decltype(t);
     constexpr int HD = decltype(hd)::value;
-    if constexpr (FwdGroups<T, HD, true>::RB != FwdGroups<T, HD, false>::RB)
-      if (!wide_tiles(a, HD)) return launch_fwd<T, HD, false>(a, stream);
-    return launch_fwd<T, HD, true>(a, stream);
+    if constexpr (row_blocks_fit<T, HD>(2))
+      if (!wide_tiles(a, HD)) return launch_fwd<T, HD, 2>(a, stream);
+    return launch_fwd<T, HD, 4>(a, stream);
   });
 }
 

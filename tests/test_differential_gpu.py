@@ -184,3 +184,45 @@ def test_cached_batches(cuda, shape, dtype):
     out = differential_attention_cached(q, k, v, lam, lengths)
     assert_within(out, want, "out", FLOOR[t])
     assert torch.equal(out, differential_attention_cached(q, k, v, lam, lengths))
+
+
+# Launches that fill the chip run other workgroups than those above. Heads are
+# independent: the first, a middle and the last key head are compared.
+# b, h, hk, s, d, dv, causal, lengths
+MANY_HEADS = {
+    "64_rows_d64": (3, 44, 44, 70, 64, 128, True, (70, 33, 0)),
+    "64_rows_d32": (2, 80, 40, 66, 32, 64, False, None),
+    "64_rows_d128": (2, 90, 90, 70, 128, 256, True, (70, 65)),
+    "128_rows_d64": (8, 64, 64, 130, 64, 128, True, None),
+    "128_rows_d64_shared": (8, 128, 64, 70, 64, 128, False, (70, 1, 33, 64, 65, 0, 69, 70)),
+    "128_rows_d32": (8, 64, 64, 130, 32, 64, True, (130, 129, 128, 97, 96, 1, 0, 64)),
+    "128_rows_d128": (4, 32, 32, 130, 128, 256, False, (130, 129, 0, 33)),
+    "128_rows_d128_causal": (4, 64, 64, 130, 128, 256, True, None),
+}
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("shape", MANY_HEADS)
+def test_many_heads(cuda, shape, dtype):
+    from techjam_amd.kernels import differential_attention
+
+    b, h, hk, s, d, dv, causal, lens = MANY_HEADS[shape]
+    q, k, v, lam, dout = inputs(TYPES[dtype], b, h, hk, s, d, dv, seed=8)
+    lengths = None if lens is None else lengths_of(*lens)
+    leaves = [t.detach().requires_grad_() for t in (q, k, v, lam)]
+    out = differential_attention(*leaves, is_causal=causal, valid_len=lengths)
+    dq, dk, dvv, dlam = torch.autograd.grad(out, leaves, dout)
+    with torch.no_grad():
+        plain = differential_attention(q, k, v, lam, is_causal=causal, valid_len=lengths)
+    for kv in (0, hk // 2, hk - 1):
+        g = h // hk
+        heads_of = slice(kv * g, (kv + 1) * g)
+        pairs, key_pair = slice(2 * kv * g, 2 * (kv + 1) * g), slice(2 * kv, 2 * kv + 2)
+        want = attention(q[:, pairs], k[:, key_pair], v[:, kv:kv + 1], lam[heads_of], causal=causal, lengths=lengths,
+                         dout=dout[:, heads_of])
+        assert_within(out[:, heads_of], want["out"], "out", FLOOR[q.dtype])
+        assert_within(plain[:, heads_of], want["out"], "out without gradients", FLOOR[q.dtype])
+        assert_within(dq[:, pairs], want["dq"], "dq", FLOOR[q.dtype])
+        assert_within(dk[:, key_pair], want["dk"], "dk", FLOOR[q.dtype])
+        assert_within(dvv[:, kv:kv + 1], want["dv"], "dv", FLOOR[q.dtype])
+        assert_within(dlam[heads_of], want["dlam"], "dlam", 1e-40)
