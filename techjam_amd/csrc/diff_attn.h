@@ -47,7 +47,7 @@ struct DiffArgs {
   // [n_parts, B, Hk, R, 2, Dv] and (maximum, sum, sum before rounding, -) [n_parts, B, Hk, R, 2, 4];
   // or, for few rows, as many of each sequence as its length asks for (FewParts),
   // n_parts in all, [n_parts, Hk, R, ...]. part_o null: sweeps run whole.
-  int n_parts, few_slots;
+  int n_parts, few_slots, few_each;
   float *part_o, *part_ml;
   // Backward.
   const void* dout;
@@ -372,8 +372,9 @@ __device__ __forceinline__ int part_keys(const DiffArgs& a, int L) {
 // batch end together (sixteen sequences of 16384 .. 65536 keys: 254 us, with as
 // many parts for each 284). few_slots times `per` cover all blocks for certain,
 // and with a part begun by every sequence that is few_slots + B = n_parts of them
-// at most; a smaller `per` is taken where its parts, counted, are no more. A whole
-// wave calls these.
+// at most; a smaller `per` is taken where its parts, counted, are no more. With
+// few_each, that many parts of every sequence, without a look at the others. A
+// whole wave calls these.
 struct FewParts {
   int b, first;   // sequence, its first part
   int n, keys;    // its parts, and the keys of each
@@ -400,11 +401,17 @@ struct FewParts {
   }
   __device__ __forceinline__ void take(const DiffArgs& a, uint32_t per) {
     const uint32_t k = blocks(a, b);
-    n = (int)((k + per - 1) / per);
+    n = a.few_each != 0 ? min(a.few_each, (int)k) : (int)((k + per - 1) / per);
     keys = n == 0 ? 0 : (int)((k + n - 1) / n) * 32;
   }
   // The sequence that `part` belongs to; false for none.
   __device__ __forceinline__ bool find(const DiffArgs& a, int part, int lane) {
+    if (a.few_each != 0) {
+      b = part / a.few_each;
+      first = b * a.few_each;
+      take(a, 1);
+      return part - first < n;
+    }
     const uint32_t per = blocks_per_part(a, lane);
     if (a.B == 1) {
       b = first = 0;
@@ -434,6 +441,11 @@ struct FewParts {
   }
   // Sequence `seq`'s parts.
   __device__ __forceinline__ void of(const DiffArgs& a, int seq, int lane) {
+    if (a.few_each != 0) {
+      b = seq;
+      first = b * a.few_each;
+      return take(a, 1);
+    }
     const uint32_t per = blocks_per_part(a, lane);
     uint32_t before = 0;
     for (int x = lane; x < seq; x += kWave) before += (blocks(a, x) + per - 1) / per;
@@ -524,16 +536,28 @@ __device__ __forceinline__ DiffTile diff_tile(const DiffArgs& a, int id, int til
   return t;
 }
 
-// Parts (less one a sequence, FewParts) for `groups` workgroups of few rows in
-// all, as many as run at once: with more, one sequence of 65536 keys takes 49 us
-// instead of 38 (twice as many) and sixteen of them 382 instead of 364. At least
-// one more part per sequence, for long ones among short; none below 32 keys.
+// The parts (FewParts) for `groups` workgroups of few rows in all, as many as run
+// at once: with more, one sequence of 65536 keys takes 49 us instead of 38 (twice
+// as many) and sixteen of them 382 instead of 364. At least one more part than
+// sequences, for long ones among short; none below 32 keys. Sequences that fill
+// the chip by themselves, or too many to look at in every workgroup, get as many
+// parts each as they are.
 constexpr int kCus = 256, kMostGroups = 8 * kCus;
-inline int few_slots(int64_t B, int64_t Hk, int64_t mtiles, int64_t Sk, int64_t groups) {
-  int64_t n = groups / (Hk * mtiles) - B;
-  if (n < B) n = B;
-  const int64_t most = B * (Sk > 0 ? (Sk + 31) / 32 : 1);
-  return (int)(n < most ? n : most);
+struct FewPlan {
+  int64_t slots, each, total;
+};
+inline FewPlan few_plan(int64_t B, int64_t Hk, int64_t mtiles, int64_t Sk, int64_t groups) {
+  const int64_t tiles = B * Hk * mtiles, blocks = Sk > 0 ? (Sk + 31) / 32 : 1;
+  if (B > 2 * kWave || tiles >= groups) {
+    int64_t each = groups / tiles;
+    if (each < 1) each = 1;
+    if (each > blocks) each = blocks;
+    return {0, each, B * each};
+  }
+  int64_t slots = groups / (Hk * mtiles) - B;
+  if (slots < B) slots = B;
+  if (slots > B * blocks) slots = B * blocks;
+  return {slots, 0, slots + B};
 }
 
 // Whether there are 128-row tiles enough for workgroups to take them rather than 64-row ones:

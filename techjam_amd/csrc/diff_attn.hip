@@ -23,7 +23,7 @@ constexpr int64_t kFewRows = 64;
 
 // More rows than few: as many parts as fill 512 workgroups, of at least kPartKeys keys.
 DiffPlan plan(int64_t B, int64_t Hk, int64_t R, int64_t Sk, bool cached) {
-  if (cached && R <= kFewRows) return {true, few_slots(B, Hk, (R + 31) / 32, Sk, kMostGroups) + B};
+  if (cached && R <= kFewRows) return {true, few_plan(B, Hk, (R + 31) / 32, Sk, kMostGroups).total};
   const int64_t tiles = B * Hk * ((R + 127) / 128);
   if (tiles >= 256) return {false, 1};
   const int64_t want = (512 + tiles - 1) / tiles, most = (Sk + kPartKeys - 1) / kPartKeys;

@@ -435,7 +435,7 @@ __global__ __launch_bounds__(kDiffThreads) void diff_join_kernel(DiffArgs a, int
   // The row's number in the first part, and from one part to the next.
   int64_t id = blockIdx.x, n_rows = (int64_t)a.B * a.Hk * a.R;
   int n_keys;
-  if (a.few_slots != 0) {
+  if (a.few_slots + a.few_each != 0) {
     FewParts f;
     f.of(a, b, tid % kWave);
     id = ((int64_t)f.first * a.Hk + hk) * a.R + row.r;
@@ -562,8 +562,10 @@ int diff_few_rows(const DiffArgs& args, int dtype, hipStream_t stream) {
     // What the LDS and the registers hold at once: two waves a SIMD at 32 dims, else one.
     constexpr int kByLds = 160 * 1024 / kLds, kByRegs = (HD == 32 ? 8 : 4) / kWaves;
     a.n_mtiles = (a.R + 31) / 32;
-    a.few_slots = few_slots(a.B, a.Hk, a.n_mtiles, a.Sk, kCus * (kByLds < kByRegs ? kByLds : kByRegs));
-    a.n_parts = a.few_slots + a.B;
+    const FewPlan p = few_plan(a.B, a.Hk, a.n_mtiles, a.Sk, kCus * (kByLds < kByRegs ? kByLds : kByRegs));
+    a.few_slots = (int)p.slots;
+    a.few_each = (int)p.each;
+    a.n_parts = (int)p.total;
     hipLaunchKernelGGL((diff_few_kernel<T, HD>), dim3(uint32_t((int64_t)a.n_parts * a.Hk * a.n_mtiles)), dim3(kWave * kWaves), 0,
                        stream, a);
     const int rc = tjh::launch_status();

@@ -158,6 +158,8 @@ BATCHES = {
     "last_alone": (70, 1, 1, 300, [0] * 69 + [300]),
     "equal": (16, 4, 1, 2048, [2048] * 16),
     "short_in_a_long_cache": (3, 4, 2, 40000, [700, 701, 40]),
+    "more_than_run_at_once": (40, 32, 32, 70, [(13 * i) % 71 for i in range(40)]),
+    "two_waves_of_sequences": (128, 1, 1, 200, [(53 * i) % 201 for i in range(128)]),
     "all_empty": (3, 2, 1, 64, [0, 0, 0]),
     "no_capacity": (2, 2, 1, 0, [0, 5]),
 }
