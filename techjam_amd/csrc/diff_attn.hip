@@ -21,12 +21,17 @@ struct DiffPlan {
 // Rows of one key head up to which every wave works by itself.
 constexpr int64_t kFewRows = 64;
 
-// More rows than few: as many parts as fill 512 workgroups, of at least kPartKeys keys.
-DiffPlan plan(int64_t B, int64_t Hk, int64_t R, int64_t Sk, bool cached) {
+// More rows than few: parts of at least kPartKeys keys where workgroups of 64 rows
+// leave half of the CUs idle, as many as fill them (twice where two fit a CU). They cost
+// the join of every row, so only from kPartsFrom keys on. Forward, us with parts / without:
+// b1 h2 s4096 d64 bf16 57 / 81, h1 s8192 79 / 153, h4 s2048 49 / 47, fp32 142 / 225; 512 new
+// rows a key head against 4096 keys 32 / 82; with 256 workgroups already, h8 s2048 75 / 48.
+constexpr int64_t kPartsFrom = 2048;
+DiffPlan plan(int64_t B, int64_t Hk, int64_t R, int64_t Sk, int64_t Dv, bool cached) {
   if (cached && R <= kFewRows) return {true, few_plan(B, Hk, (R + 31) / 32, Sk, kMostGroups).total};
-  const int64_t tiles = B * Hk * ((R + 127) / 128);
-  if (tiles >= 256) return {false, 1};
-  const int64_t want = (512 + tiles - 1) / tiles, most = (Sk + kPartKeys - 1) / kPartKeys;
+  const int64_t tiles = B * Hk * ((R + 63) / 64);
+  if (tiles > kCus / 2 || Sk < kPartsFrom) return {false, 1};
+  const int64_t fill = Dv > 128 ? kCus : 2 * kCus, want = (fill + tiles - 1) / tiles, most = (Sk + kPartKeys - 1) / kPartKeys;
   return {false, want < most ? want : most};
 }
 
@@ -80,7 +85,7 @@ extern "C" size_t tj_diff_attn_workspace_bytes(int64_t B, int64_t H, int64_t Hk,
                                                int cached) {
   if (!sizes_ok(B, H, Hk, Sq, Sk) || Dv <= 0 || Dv > 256 || B == 0 || Sq == 0) return 0;
   const int64_t R = Sq * (H / Hk);
-  return part_bytes(plan(B, Hk, R, Sk, cached != 0), B, Hk, R, Dv);
+  return part_bytes(plan(B, Hk, R, Sk, Dv, cached != 0), B, Hk, R, Dv);
 }
 
 extern "C" int tj_diff_attn_fwd(const void* q, const void* k, const void* v, void* o, int dtype, int64_t B, int64_t H,
@@ -107,7 +112,7 @@ extern "C" int tj_diff_attn_fwd(const void* q, const void* k, const void* v, voi
   a.Sq = (int)Sq; a.Sk = (int)Sk; a.R = (int)(Sq * a.G);
   a.scale = scale; a.causal = causal != 0 || cached != 0; a.cached = cached != 0;
   a.lam = lam; a.lam_step = (int)lam_step; a.len = lengths; a.lse = lse;
-  const DiffPlan p = plan(B, Hk, a.R, Sk, a.cached);
+  const DiffPlan p = plan(B, Hk, a.R, Sk, Dv, a.cached);
   const size_t need = part_bytes(p, B, Hk, a.R, Dv);
   // diff_join_kernel: a workgroup per row. (A cache of no capacity still has rows to clear.)
   if ((p.few || need != 0) && B * Hk * a.R >= (int64_t(1) << 24)) return TJ_ERR_SHAPE;

@@ -312,8 +312,8 @@ constexpr int kMaps = HD <= 64 ? 2 : 1;
 // registers allow it, and one's products run beside the other's exponentials:
 // eight waves meeting at one barrier were 15 % slower on the long bf16 case. 128
 // rows where those fill the chip, else 64 with two groups, if two tiles for each
-// fit. (32 rows with four: b1 h4 s512 20.3 against 19.7 us, and twice the time where
-// the keys are in parts.)
+// fit. (32 rows with four, bf16: b1 h4 s512 20.3 against 19.7 us, and twice the time
+// where the keys are in parts.)
 template <typename T, int HD, int BLOCKS>
 struct FwdGroups {
   static constexpr int kPairs = 2 / kMaps<HD>;
@@ -547,6 +547,10 @@ int diff_fwd(const DiffArgs& a, int dtype, hipStream_t stream) {
   return diff_dispatch(a, dtype, [&](auto t, auto hd) {
     using T = decltype(t);
     constexpr int HD = decltype(hd)::value;
+    // Four groups: fp32 d32 (bound by its products) from 128 keys on, with two / four: b1 h1 s128 12.9 / 11.8
+    // us, s512 33.7 / 23.2, but s64 9.4 / 11.4.
+    if constexpr (sizeof(T) == 4 && row_blocks_fit<T, HD>(1))
+      if (a.Sk >= 128 && (int64_t)a.B * a.Hk * ((a.R + 63) / 64) * a.n_parts <= kCus / 2) return launch_fwd<T, HD, 1>(a, stream);
     if constexpr (row_blocks_fit<T, HD>(2))
       if (!wide_tiles(a, HD)) return launch_fwd<T, HD, 2>(a, stream);
     return launch_fwd<T, HD, 4>(a, stream);

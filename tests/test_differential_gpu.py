@@ -49,6 +49,9 @@ SHAPES = {
     "tiny_dims": (1, 1, 1, 33, 3, 5, True, None),
     "keys_shared_by_five": (1, 10, 2, 77, 32, 64, True, None),
     "long": (1, 1, 1, 1100, 64, 128, True, None),
+    "keys_in_parts": (1, 1, 1, 2300, 64, 128, True, None),
+    "keys_in_parts_padded": (2, 2, 1, 2090, 32, 64, False, (2090, 700)),
+    "keys_in_parts_wide": (1, 1, 1, 2049, 128, 256, True, None),
 }
 
 
@@ -107,6 +110,8 @@ CACHES = {
     "wide": (1, 4, 1, 2, 200, 128, 256, (199,)),
     "rows_of_two_tiles": (2, 4, 1, 16, 270, 64, 128, (270, 40)),
     "a_chunk": (2, 2, 1, 90, 700, 64, 128, (700, 95)),
+    "a_chunk_in_parts": (2, 4, 2, 90, 4500, 64, 128, (4500, 600)),
+    "a_chunk_in_a_long_cache": (3, 2, 1, 70, 3000, 128, 256, (90, 0, 2999)),
     "odd_dims": (2, 2, 2, 1, 130, 40, 80, (130, 99)),
 }
 
