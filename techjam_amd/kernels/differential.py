@@ -16,6 +16,7 @@ from typing import Optional
 
 import torch
 import torch.nn.functional as F
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from ..errors import UnsupportedCaseError
@@ -35,6 +36,16 @@ def on_device(device: torch.device):
     if device.index == torch.cuda.current_device():
         return contextlib.nullcontext()
     return torch.cuda.device(device)
+
+
+def refuse_tangents(*tensors: Optional[torch.Tensor]) -> None:
+    """Forward-mode derivatives are not implemented. A dual tensor need not
+    require grad, so without a look at it a call outside of autograd would
+    return its output without the tangent, which torch takes as zero."""
+    if forward_ad._current_level < 0 or not torch._C._is_fwd_grad_enabled():
+        return
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise UnsupportedCaseError("forward-mode derivatives are not implemented")
 
 
 def _rows_view(t: torch.Tensor) -> torch.Tensor:
@@ -75,6 +86,7 @@ def _check(q, k, v, lam, lengths, what: str, cached: bool) -> None:
                                    f"{MAX_VALUE_DIM})")
     if not isinstance(lam, torch.Tensor) or not lam.is_floating_point() or lam.shape not in ((), (1,), (h2 // 2,)):
         raise ValueError(f"lam must be a floating-point tensor of one or {h2 // 2} elements")
+    refuse_tangents(q, k, v, lam)
     dev = _require_device(q, k, v, lam)
     if lengths is not None and (lengths.dtype != torch.int32 or lengths.device != dev or lengths.shape != (b,)
                                 or not lengths.is_contiguous()):
@@ -207,7 +219,8 @@ def differential_attention(
     The output's storage is ``[B, S, H, Dv]``, so that merging the heads is a
     view. Gradients come for q, k, v and lam (summed over what shares a weight);
     their sums have a fixed order, so equal calls give equal bits. Second
-    derivatives are not implemented.
+    derivatives and forward-mode ones (``torch.autograd.forward_ad``) are not
+    implemented and refused.
     """
     _check(q, k, v, lam, valid_len, "valid_len", False)
     scale = _scale(scale, q.shape[-1])
@@ -245,7 +258,8 @@ def differential_attention_cached(
     equal bits.
 
     Layouts, types and ``lam`` as in :func:`differential_attention`. No
-    gradients: inputs that require them are refused while they are enabled.
+    gradients: inputs that require them are refused while they are enabled, as
+    are forward-mode tangents.
     """
     if lengths is None:
         raise ValueError("lengths must be given: a cache's capacity is not its sequences' length")

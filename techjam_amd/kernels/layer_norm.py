@@ -17,7 +17,7 @@ from torch.autograd.function import once_differentiable
 from ..errors import UnsupportedCaseError
 from . import _lib
 from .attention import _ptr, _require_device, _stream_ptr
-from .differential import DTYPES, on_device
+from .differential import DTYPES, on_device, refuse_tangents
 
 #: Widest row the kernels take.
 MAX_WIDTH = 16384
@@ -121,8 +121,10 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     float32 or both of ``x``'s type, each optional; their gradients come in their
     type. Statistics and sums are float32, the output is contiguous and of
     ``x``'s type, or float32 with ``norm_dtype=torch.float32`` (the norm of
-    16-bit rows not rounded to 16 bits). The gradients' sums over the rows have a fixed order, so equal
-    calls give equal bits. Second derivatives are not implemented.
+    16-bit rows not rounded to 16 bits). The gradients' sums over the rows have
+    a fixed order, so equal calls give equal bits. Second derivatives and
+    forward-mode ones (``torch.autograd.forward_ad``) are not implemented and
+    refused.
     """
     if x.ndim == 0 or x.shape[-1] == 0:
         raise ValueError("x must have a last dimension to normalise over")
@@ -131,6 +133,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     width = x.shape[-1]
     if width > MAX_WIDTH:
         raise UnsupportedCaseError(f"width {width} is not supported (at most {MAX_WIDTH})")
+    refuse_tangents(x, weight, bias)
     dev = _require_device(x)
     if weight is not None:
         _check_param("weight", weight, width, x.dtype, dev)
