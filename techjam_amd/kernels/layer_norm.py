@@ -34,7 +34,10 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     copy."""
     width = t.shape[-1]
     if t.is_contiguous():
-        return t if t.ndim == 2 else t.view(-1, width)
+        if t.ndim != 2:
+            t = t.view(-1, width)
+        # A single row is contiguous whatever its row stride is.
+        return t if t.shape[0] != 1 or t.stride(0) == width else t.as_strided((1, width), (width, 1))
     t = t.reshape(-1, width)
     if (t.stride(1) != 1 and width > 1) or t.stride(0) >= 1 << 23:
         return t.contiguous()

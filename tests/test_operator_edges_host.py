@@ -2,12 +2,16 @@
 
 from __future__ import annotations
 
+import sys
+
 import pytest
 import torch
 from torch.autograd import forward_ad
 
 from techjam_amd import UnsupportedCaseError
 from techjam_amd.kernels import LayerNorm, differential_attention, differential_attention_cached, layer_norm
+
+norm_kernels = sys.modules["techjam_amd.kernels.layer_norm"]  # the package's attribute is the function
 
 
 def attention_inputs(sq=4, sk=4):
@@ -33,3 +37,23 @@ def test_tangents_are_refused_and_not_dropped(grad):
                     call(*inputs[:i], dual, *inputs[i + 1:])  # no derivatives there: the device is what is refused
             with pytest.raises(UnsupportedCaseError, match="GPU"):
                 call(*inputs)
+
+
+@pytest.mark.parametrize("width,row_stride", [(2048, 8192 * 2048), (96, 1 << 40), (8, 3), (1, 1 << 30), (7, 0)])
+@pytest.mark.parametrize("ndim", [1, 2, 3])
+def test_a_single_row_has_no_row_stride(width, row_stride, ndim):
+    """One row counts as contiguous whatever its stride, and the kernels take strides below 2^23."""
+    t = torch.arange(width, dtype=torch.float32).as_strided((1,) * (ndim - 1) + (width,), (row_stride,) * (ndim - 1) + (1,))
+    rows = norm_kernels._rows(t)
+    assert rows.shape == (1, width) and rows.stride() == (width, 1) and rows.data_ptr() == t.data_ptr()
+    assert torch.equal(rows[0], torch.arange(width))
+
+
+def test_rows_far_apart_are_copied():
+    two = torch.zeros(2).as_strided((2, 1), (1, 5)).expand(2, 4)
+    assert norm_kernels._rows(two).stride() == (4, 1)
+    far = torch.empty(1, device="meta").as_strided((2, 4), (1 << 23, 1))
+    near = torch.empty(1, device="meta").as_strided((2, 4), ((1 << 23) - 1, 1))
+    assert norm_kernels._rows(far).stride() == (4, 1)
+    assert norm_kernels._rows(near).stride() == ((1 << 23) - 1, 1)
+    assert norm_kernels._rows(torch.zeros(0, 4)).shape == (0, 4)
