@@ -48,14 +48,23 @@ def refuse_tangents(*tensors: Optional[torch.Tensor]) -> None:
         raise UnsupportedCaseError("forward-mode derivatives are not implemented")
 
 
-def _rows_view(t: torch.Tensor) -> torch.Tensor:
-    """``t`` itself when the kernels can read it in place (unit innermost
-    stride, rows and base aligned to 16 bytes, 64 rows within 2 GiB), else a
-    contiguous copy."""
+def _readable(t: torch.Tensor) -> bool:
+    """Unit innermost stride, rows and base aligned to 16 bytes, 64 rows within 2 GiB."""
     sb, sh, ss, sd = t.stride()
     size = t.element_size()
-    if sd == 1 and not (sb | sh | ss) & (16 // size - 1) and not t.data_ptr() & 15 and ss * 64 * size < 1 << 31:
+    return sd == 1 and not (sb | sh | ss) & (16 // size - 1) and not t.data_ptr() & 15 and ss * 64 * size < 1 << 31
+
+
+def _rows_view(t: torch.Tensor) -> torch.Tensor:
+    """``t`` itself when the kernels can read it in place, else a contiguous copy."""
+    if _readable(t):
         return t
+    if min(t.shape[:3]) <= 1:
+        # The stride of a dimension of at most one is never used, may be anything,
+        # and stays what it is in contiguous(): 0 instead.
+        t = t.as_strided(t.shape, [0 if n <= 1 else st for n, st in zip(t.shape[:3], t.stride())] + [t.stride(3)])
+        if _readable(t):
+            return t
     t = t.contiguous()
     return t.clone() if t.data_ptr() & 15 else t
 

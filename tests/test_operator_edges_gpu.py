@@ -27,3 +27,37 @@ def test_norm_of_the_last_token_of_a_long_sequence(cuda, dtype):
 
     for got, want in zip(run(x, dy), run(x.clone(memory_format=torch.contiguous_format), dy.clone())):
         assert torch.equal(got, want)
+
+
+def test_strides_of_dimensions_of_one(cuda):
+    """Batch, key heads or tokens of one with odd strides: the bits of compact tensors."""
+    from techjam_amd.kernels import differential_attention, differential_attention_cached
+
+    g = torch.Generator(device="cuda").manual_seed(2)
+    lam = torch.rand(1, generator=g, device="cuda")
+
+    def odd(shape, strides):
+        n = sum((a - 1) * b for a, b in zip(shape, strides)) + 1
+        return torch.randn(n, generator=g, device="cuda").half().as_strided(shape, strides)
+
+    for sq, sk in ((7, 7), (1, 1), (1, 9)):
+        q = odd((1, 2, sq, 64), (897, 64 * sq, 64 if sq > 1 else 1027, 1))
+        k = odd((1, 2, sk, 64), (3, 64 * sk, 64 if sk > 1 else 5, 1))
+        v = odd((1, 1, sk, 128), (3, 1025, 128 if sk > 1 else 1027, 1))
+        dout = odd((1, 1, sq, 128), (1, 1, 128 if sq > 1 else 3, 1))
+
+        def run(q, k, v, dout):
+            lengths = torch.full((1,), sk, dtype=torch.int32, device="cuda")
+            with torch.no_grad():
+                new = differential_attention_cached(q, k, v, lam, lengths)
+            if sq != sk:
+                return (new,)
+            leaves = [t.detach().requires_grad_() for t in (q, k, v)]
+            out = differential_attention(*leaves, lam, is_causal=True)
+            return (new, out, *torch.autograd.grad(out, leaves, dout))
+
+        def compact(t):
+            return t.new_empty(t.shape).copy_(t)
+
+        for got, want in zip(run(q, k, v, dout), run(*map(compact, (q, k, v, dout)))):
+            assert torch.equal(got, want)

@@ -11,6 +11,7 @@ from torch.autograd import forward_ad
 from techjam_amd import UnsupportedCaseError
 from techjam_amd.kernels import LayerNorm, differential_attention, differential_attention_cached, layer_norm
 
+attention_kernels = sys.modules["techjam_amd.kernels.differential"]
 norm_kernels = sys.modules["techjam_amd.kernels.layer_norm"]  # the package's attribute is the function
 
 
@@ -57,3 +58,39 @@ def test_rows_far_apart_are_copied():
     assert norm_kernels._rows(far).stride() == (4, 1)
     assert norm_kernels._rows(near).stride() == ((1 << 23) - 1, 1)
     assert norm_kernels._rows(torch.zeros(0, 4)).shape == (0, 4)
+
+
+def _view(shape, strides, offset=0):
+    n = offset + sum((a - 1) * b for a, b in zip(shape, strides)) + 1
+    return torch.randn(n).half().as_strided(shape, strides, offset)
+
+
+@pytest.mark.parametrize("shape,strides,in_place", [
+    ((1, 1, 1, 64), (1027, 1027, 1027, 1), True),     # one token's value in a projection of odd width
+    ((1, 2, 7, 64), (897, 448, 64, 1), True),         # a batch of one
+    ((1, 2, 7, 64), (5, 64, 128, 1), True),           # the same, token by token in memory
+    ((2, 1, 7, 64), (448, 3, 64, 1), True),           # one key head
+    ((2, 2, 1, 64), (128, 64, 1 << 40, 1), True),     # one token
+    ((1, 2, 7, 64), (897, 455, 65, 1), False),        # odd rows
+    ((1, 1, 2, 64), (1, 1, 65, 1), False),
+    ((1, 1, 1, 64), (1, 1, 1, 1), True),
+    ((1, 1, 2, 64), (7, 7, 1 << 26, 1), False),       # rows too far apart
+    ((0, 2, 1, 64), (3, 64, 7, 1), True),
+    ((2, 2, 0, 64), (64, 128, 7, 1), True),           # a cache of no capacity
+])
+def test_strides_of_dimensions_of_one_do_not_count(shape, strides, in_place):
+    if strides[2] == 1 << 26:
+        t = torch.empty(1, device="meta").half().as_strided(shape, strides)
+    else:
+        t = _view(shape, strides) if 0 not in shape else torch.empty(1).half().as_strided(shape, strides)
+    got = attention_kernels._rows_view(t)
+    assert attention_kernels._readable(got) and got.shape == t.shape
+    if t.device.type == "cpu":
+        assert torch.equal(got, t)
+        assert (got.data_ptr() == t.data_ptr()) == in_place or 0 in shape
+
+
+def test_misaligned_single_tokens_are_copied():
+    t = _view((1, 2, 1, 64), (1, 64, 1, 1), offset=1)
+    got = attention_kernels._rows_view(t)
+    assert attention_kernels._readable(got) and torch.equal(got, t)
