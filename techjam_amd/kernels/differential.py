@@ -10,7 +10,6 @@ views the same way, and have gradients.
 from __future__ import annotations
 
 import contextlib
-import math
 from functools import lru_cache
 from typing import Optional
 
@@ -26,6 +25,8 @@ from .attention import _ptr, _require_device, _stream_ptr
 #: Largest head dim of q and k, and of v.
 MAX_HEAD_DIM = 128
 MAX_VALUE_DIM = 256
+#: Largest scale whose product with log2 e is a float32.
+MAX_SCALE = 2.0 ** 127
 
 DTYPES = {torch.float32: _lib.TJ_F32, torch.float16: _lib.TJ_F16, torch.bfloat16: _lib.TJ_BF16}
 
@@ -191,8 +192,8 @@ class _DifferentialAttention(torch.autograd.Function):
 
 def _scale(scale: Optional[float], d: int) -> float:
     scale = d ** -0.5 if scale is None else float(scale)
-    if not math.isfinite(scale):
-        raise ValueError(f"scale must be finite, not {scale}")
+    if not abs(scale) <= MAX_SCALE:
+        raise ValueError(f"scale must be at most 2^127 in magnitude, not {scale}")
     return scale
 
 
@@ -219,7 +220,7 @@ def differential_attention(
     ``valid_len`` (int32 ``[B]`` on the device) masks keys ``j >= valid_len[b]``
     and zeroes rows ``i >= valid_len[b]``, as in ``scaled_dot_product_attention``;
     what those rows and keys hold is not read, and their gradients are zero.
-    ``scale`` defaults to ``D ** -0.5``.
+    ``scale`` defaults to ``D ** -0.5``; its magnitude is at most 2^127.
 
     A NaN or an infinity among the valid inputs spoils what depends on it; one in
     ``v`` under ``is_causal`` also the up to 31 rows before it in its tile of 32

@@ -94,3 +94,15 @@ def test_misaligned_single_tokens_are_copied():
     t = _view((1, 2, 1, 64), (1, 64, 1, 1), offset=1)
     got = attention_kernels._rows_view(t)
     assert attention_kernels._readable(got) and torch.equal(got, t)
+
+
+@pytest.mark.parametrize("scale", [1e300, -3.5e38, 2.0 ** 127.5, float("inf"), float("nan")])
+def test_scales_past_float32_are_refused(scale):
+    """Handed on as a float32, 1e300 would be an infinity and every output NaN."""
+    with pytest.raises(ValueError):
+        attention_kernels._scale(scale, 64)
+
+
+@pytest.mark.parametrize("scale", [0.0, -2.0 ** 127, 2.0 ** 127, 1e-300])
+def test_scales_of_float32_are_taken(scale):
+    assert attention_kernels._scale(scale, 64) == scale
