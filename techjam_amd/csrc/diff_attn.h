@@ -455,35 +455,48 @@ struct FewParts {
   }
 };
 
-// Products with fp16 operands: the power of two that brings the largest
-// possible |dS| (2 |dO_i| |V_j| max(1, |lam|) scale) near 2^15, so that small
-// gradients and small probabilities keep fp16's bits. 1 for the other types.
+// Products with fp16 operands: powers of two that bring the largest possible |dS|,
+// 2 |dO_i| |V_j| max(1, |lam|), near 2^15, so that small gradients and small
+// probabilities keep fp16's bits. dQ is a sum over keys, so there every row has
+// its own, by its dO (of): a row's bits do not depend on how large others are.
+// dK sums over rows and has one for all of a (b, key head), by the largest dO
+// row: dS of a row r times smaller keeps 11 bits down to P of about 2^-26 r, and
+// what lies below is off by at most 2^-37 of the largest possible |dS|. 1 for the
+// other types.
 template <typename T>
-__device__ __forceinline__ float ds_lift(const DiffArgs& a, int bh, int hk, int lane) {
-  if constexpr (!std::is_same<T, half_t>::value) {
-    return 1.f;
-  } else {
-    const float* pk = a.peak + (int64_t)bh * 2 * kPeakParts;
-    float x = lane < a.n_peaks ? pk[lane] : 0.f, y = lane < a.n_peaks ? pk[kPeakParts + lane] : 0.f;
+struct DsLift {
+  float o = 1.f, v = 1.f;  // the largest norms of dO and V rows
+  int ew = 0;              // exponent of the heads' largest max(1, |lam|)
+  __device__ __forceinline__ DsLift(const DiffArgs& a, int bh, int hk, int lane) {
+    if constexpr (std::is_same<T, half_t>::value) {
+      const float* pk = a.peak + (int64_t)bh * 2 * kPeakParts;
+      o = lane < a.n_peaks ? pk[lane] : 0.f;
+      v = lane < a.n_peaks ? pk[kPeakParts + lane] : 0.f;
 #pragma unroll
-    for (int m = 32; m > 0; m >>= 1) {
-      x = fmaxf(x, __shfl_xor(x, m));
-      y = fmaxf(y, __shfl_xor(y, m));
+      for (int m = 32; m > 0; m >>= 1) {
+        o = fmaxf(o, __shfl_xor(o, m));
+        v = fmaxf(v, __shfl_xor(v, m));
+      }
+      float w = 1.f;
+      for (int g = 0; g < a.G; ++g) {
+        const float l = fabsf(a.lam[(hk * a.G + g) * a.lam_step]);
+        if (l < 3e38f) w = fmaxf(w, l);
+      }
+      frexpf(w, &ew);
     }
-    float w = 1.f;
-    for (int g = 0; g < a.G; ++g) {
-      const float l = fabsf(a.lam[(hk * a.G + g) * a.lam_step]);
-      if (l < 3e38f) w = fmaxf(w, l);
-    }
+  }
+  // For rows whose dO has at most this norm.
+  __device__ __forceinline__ float of(float norm) const {
+    if constexpr (!std::is_same<T, half_t>::value) return 1.f;
     // Exponents rather than products: the norms' product may leave fp32.
-    int ex, ey, ew;
-    frexpf(x, &ex);
-    frexpf(y, &ey);
-    frexpf(w, &ew);
-    if (!(x > 0.f) || !(y > 0.f)) return 1.f;
+    int ex, ey;
+    frexpf(norm, &ex);
+    frexpf(v, &ey);
+    if (!(norm > 0.f) || !(norm < 3e38f) || !(v > 0.f)) return 1.f;  // a row that is not finite is lost anyway
     return ldexpf(1.f, min(max(14 - ex - ey - ew, -100), 100));
   }
-}
+  __device__ __forceinline__ float all() const { return of(o); }
+};
 
 // A row's place in the arrays [B, H, Sq].
 __device__ __forceinline__ int64_t row_at(const DiffArgs& a, int b, int head, int i) {

@@ -141,7 +141,7 @@ __global__ __launch_bounds__((64 * KvShape<T, HD, WHAT, HALF>::WAVES), (KvShape<
 #pragma unroll
   for (auto& x : dk[1]) x = zero16();
 
-  const float pl = p_lift<T>(a, t.hk), dl = ds_lift<T>(a, t.bh, t.hk, lane), lift = dl / pl;
+  const float pl = p_lift<T>(a, t.hk), dl = DsLift<T>(a, t.bh, t.hk, lane).all(), lift = dl / pl;
   const float c2 = a.scale * kLog2e;
   const auto lams = (const __attribute__((address_space(4))) float*)a.lam;
   int g = 0, i0 = i_begin;  // this round's tile

@@ -179,7 +179,16 @@ diff_bwd_q_kernel(DiffArgs a) {
   for (int c = 0; c < 2; ++c)
 #pragma unroll
     for (int d = 0; d < DB; ++d) dq[c][d] = zero16();
-  const float lift = ds_lift<T>(a, t.bh, t.hk, lane);
+  // The row's own lift: its lane (and the one of the other half) has all of its dO.
+  float norm = 0.f;
+  if constexpr (std::is_same<T, half_t>::value) {
+#pragma unroll
+    for (int s = 0; s < VS; ++s)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) norm = fmaf((float)of[s][j], (float)of[s][j], norm);
+    norm = sqrtf(pair_sum(norm));
+  }
+  const float lift = DsLift<T>(a, t.bh, t.hk, lane).of(norm);
   const float c2 = a.scale * kLog2e;
   const float lam = live ? a.lam[head * a.lam_step] : 0.f;
   float lse[2], del[2];
@@ -284,11 +293,12 @@ diff_bwd_q_kernel(DiffArgs a) {
 
   rest[0] = pair_sum(rest[0]) / lift;
   rest[1] = pair_sum(rest[1]);
+  // P is lifted by pl in its exponent in the dK, dV kernel, and dS by one lift for all
+  // rows; what multiplies P to dS takes the former out again.
+  const float pl = p_lift<T>(a, t.hk), dl = DsLift<T>(a, t.bh, t.hk, lane).all() / pl;
   if (r >= a.R) return;
   if (hl == 0) {
     a.gsum[row_at(a, t.b, head, i)] = live ? del[1] + rest[1] : 0.f;
-    // P is lifted by pl in its exponent; what multiplies P to dS takes that out again.
-    const float pl = p_lift<T>(a, t.hk), dl = lift / pl;
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
       *stat_at(a, t.b, head, i, c) = live ? log2f(pl) - lse[c] : -__builtin_inff();
