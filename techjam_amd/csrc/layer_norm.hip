@@ -213,10 +213,12 @@ __global__ __launch_bounds__(norm_threads<LPR>()) void norm_bwd_kernel(NormArgs 
     const float mean = on ? a.mean[r0 + sub] : 0.f, rstd = on ? a.rstd[r0 + sub] : 0.f;
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
+      // Past the row's end dy and x read as zero, and with no mean there xh is too:
+      // -mean rstd may be an infinity, which times zero would spoil the row's sums.
+      const float centre = (lane + v * LPR) * N < a.cols ? mean : 0.f;
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        // Past the row's end dy reads as zero, so whatever xh is there adds nothing.
-        x[v][j] = (x[v][j] - mean) * rstd;
+        x[v][j] = (x[v][j] - centre) * rstd;
         dw[v][j] = fmaf(g[v][j], x[v][j], dw[v][j]);
         db[v][j] += g[v][j];
         g[v][j] *= w[v][j];

@@ -94,3 +94,26 @@ def test_fp16_gradients_beside_one_large_row(cuda, shape):
     assert_within(dk, (value, bound + 2.0 ** -36 * x * y * w * d ** -0.5 * mass), "dk", FLOOR[torch.float16])
     assert_within(dvv, want["dv"], "dv", FLOOR[torch.float16])
     assert_within(dlam, want["dlam"], "dlam", 1e-40)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("width", [1, 2, 8, 32, 128, 512, 8192])
+def test_norm_gradients_of_huge_constant_rows(cuda, width, dtype):
+    """x = 2^108, whose sum of up to 8192 and mean are exact: xh is 0, dx = rstd (g - mean(g)).
+
+    What lanes past the row's end hold is -mean rstd in size, an infinity for eps
+    of 1e-30. dy is 1 or 2 in equal parts (1 alone in a row of one), so its mean is
+    exact too, and dx is rstd times 0, -1/2 or 1/2 with rstd = 1 / sqrt(1e-30 in float32),
+    two roundings of 2^-24 and the result's own.
+    """
+    x = torch.full((3, width), 2.0 ** 108, dtype=dtype, device="cuda").requires_grad_()
+    w, b = (torch.ones(width, device="cuda").requires_grad_() for _ in range(2))
+    dy = (1.0 + torch.arange(width, device="cuda") % 2).expand(3, width).to(dtype).contiguous()
+    y = layer_norm(x, w, b, 1e-30)
+    dx, dw, db = torch.autograd.grad(y, (x, w, b), dy)
+    assert torch.equal(y, torch.ones_like(y))
+    rstd = float(torch.tensor(1e-30, dtype=torch.float32).double() ** -0.5)
+    want = rstd * (dy.double() - dy.double().mean(-1, keepdim=True))
+    allowed = (torch.finfo(dtype).eps / 2 + 4 * 2.0 ** -24) * want.abs()
+    assert bool(((dx.double() - want).abs() <= allowed).all())
+    assert torch.equal(dw, torch.zeros_like(dw)) and torch.equal(db, 3 * dy[0].float())
