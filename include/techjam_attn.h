@@ -394,6 +394,9 @@ int tj_narrow_ffn_norm(const float* x, const float* w_in, const float* bias_in, 
  * token i sees the keys up to its position lengths[b] - Sq + i. Tokens at a
  * negative position are written as zeros. Lengths are clipped to 0 .. Sk; what
  * lies behind them is not read, whatever it holds.
+ * Sizes (TJ_ERR_SHAPE past them): B Hk ((Sq / 128 + 1) H / Hk + Sk / 128 + 2) below
+ * 2^22, without Sk for cached ones, of which those cut into parts (few tokens) have
+ * B H Sq below 2^24; B H, Sq H / Hk and Sk H / Hk below 2^30; B Sk below 2^35.
  *
  * dtype: TJ_F32, TJ_F16 or TJ_BF16, shared by q, k, v and o. Products of 16-bit
  * inputs run on MFMAs of that type with fp32 accumulation (probabilities are

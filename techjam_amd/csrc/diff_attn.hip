@@ -41,15 +41,17 @@ size_t part_bytes(const DiffPlan& p, int64_t B, int64_t Hk, int64_t R, int64_t D
   return (rows * size_t(Dv) + rows * 4) * sizeof(float);
 }
 
-// Sizes that the kernels' 32-bit row and key numbers and the grids hold.
-bool sizes_ok(int64_t B, int64_t H, int64_t Hk, int64_t Sq, int64_t Sk) {
+// Sizes that the kernels' 32-bit row and key numbers and the grids hold. A cache's
+// capacity is no part of a grid (the rows say how many parts there are), but FewParts
+// counts all of its blocks of 32 keys.
+bool sizes_ok(int64_t B, int64_t H, int64_t Hk, int64_t Sq, int64_t Sk, bool cached) {
   if (B < 0 || H <= 0 || Hk <= 0 || H % Hk != 0 || Sq < 0 || Sk < 0) return false;
   const int64_t lim = int64_t(1) << 30;
   return B < lim && H < lim && Sq < lim && Sk < lim && tjh::product_below(lim, {Sq, H / Hk}) &&
          tjh::product_below(lim, {Sk, H / Hk}) && tjh::product_below(lim, {B, H}) &&
-         tjh::product_below(int64_t(1) << 56, {B, H, Sq + 128, 1024}) &&
+         tjh::product_below(int64_t(1) << 56, {B, H, Sq + 128, 1024}) && tjh::product_below(int64_t(1) << 35, {B, Sk}) &&
          // workgroups of 256 threads: one for every 128 rows or keys, and up to 512 more in parts
-         tjh::product_below(int64_t(1) << 22, {B, Hk, (Sq / 128 + 1) * (H / Hk) + Sk / 128 + 2});
+         tjh::product_below(int64_t(1) << 22, {B, Hk, (Sq / 128 + 1) * (H / Hk) + (cached ? 0 : Sk / 128) + 2});
 }
 
 int check_dims(int dtype, int64_t D, int64_t Dv) {
@@ -83,7 +85,7 @@ using namespace tj;
 
 extern "C" size_t tj_diff_attn_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t Sq, int64_t Sk, int64_t Dv,
                                                int cached) {
-  if (!sizes_ok(B, H, Hk, Sq, Sk) || Dv <= 0 || Dv > 256 || B == 0 || Sq == 0) return 0;
+  if (!sizes_ok(B, H, Hk, Sq, Sk, cached != 0) || Dv <= 0 || Dv > 256 || B == 0 || Sq == 0) return 0;
   const int64_t R = Sq * (H / Hk);
   return part_bytes(plan(B, Hk, R, Sk, Dv, cached != 0), B, Hk, R, Dv);
 }
@@ -95,7 +97,7 @@ extern "C" int tj_diff_attn_fwd(const void* q, const void* k, const void* v, voi
                                 const int32_t* lengths, float* lse, float* maps, void* workspace, size_t workspace_bytes,
                                 hipStream_t stream) {
   if (elem_bytes(dtype) == 0) return TJ_ERR_DTYPE;
-  if (!sizes_ok(B, H, Hk, Sq, Sk)) return TJ_ERR_SHAPE;
+  if (!sizes_ok(B, H, Hk, Sq, Sk, cached != 0)) return TJ_ERR_SHAPE;
   if (const int rc = check_dims(dtype, D, Dv)) return rc;
   if (cached ? lengths == nullptr : Sq != Sk) return TJ_ERR_SHAPE;
   if ((lam_step != 0 && lam_step != 1) || (lse == nullptr) != (maps == nullptr)) return TJ_ERR_SHAPE;
@@ -128,7 +130,7 @@ extern "C" int tj_diff_attn_fwd(const void* q, const void* k, const void* v, voi
 }
 
 extern "C" size_t tj_diff_attn_bwd_workspace_bytes(int64_t B, int64_t H, int64_t Hk, int64_t S) {
-  if (!sizes_ok(B, H, Hk, S, S)) return 0;
+  if (!sizes_ok(B, H, Hk, S, S, false)) return 0;
   return (size_t(B) * size_t(H) * (size_t(S) * 3 + size_t(stat_rows(S)) * 4) + size_t(B) * size_t(Hk) * 2 * kPeakParts) *
          sizeof(float);
 }
@@ -142,7 +144,7 @@ extern "C" int tj_diff_attn_bwd(const void* q, const void* k, const void* v, con
                                 const float* lam, int64_t lam_step, const int32_t* lengths, void* workspace,
                                 size_t workspace_bytes, hipStream_t stream) {
   if (elem_bytes(dtype) == 0) return TJ_ERR_DTYPE;
-  if (!sizes_ok(B, H, Hk, S, S)) return TJ_ERR_SHAPE;
+  if (!sizes_ok(B, H, Hk, S, S, false)) return TJ_ERR_SHAPE;
   if (const int rc = check_dims(dtype, D, Dv)) return rc;
   if (lam_step != 0 && lam_step != 1) return TJ_ERR_SHAPE;
   if (lam == nullptr || dlam == nullptr) return TJ_ERR_SHAPE;

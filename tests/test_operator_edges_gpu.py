@@ -117,3 +117,23 @@ def test_norm_gradients_of_huge_constant_rows(cuda, width, dtype):
     allowed = (torch.finfo(dtype).eps / 2 + 4 * 2.0 ** -24) * want.abs()
     assert bool(((dx.double() - want).abs() <= allowed).all())
     assert torch.equal(dw, torch.zeros_like(dw)) and torch.equal(db, 3 * dy[0].float())
+
+
+def test_many_sequences_of_a_large_capacity(cuda):
+    """2^30 places for keys over 512 sequences and 32 key heads (one row repeated: strides of 0)."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    b, hk, cap = 512, 32, 65536
+    q = torch.randn(b, 2 * hk, 1, 32, generator=g, device="cuda").half()
+    k = torch.randn(1, 2 * hk, 1, 32, generator=g, device="cuda").half().expand(b, -1, cap, -1)
+    v = torch.randn(1, hk, 1, 64, generator=g, device="cuda").half().expand(b, -1, cap, -1)
+    lam = torch.full((1,), 0.25, device="cuda")
+    lengths = torch.randint(0, 100, (b,), generator=g, device="cuda", dtype=torch.int32)
+    lengths[0], lengths[-1] = cap, 1
+    out = differential_attention_cached(q, k, v, lam, lengths)
+    # Equal keys share a row's probability evenly: both maps give v, whatever the scores are. A
+    # key's probability and the sums are rounded alike, so v comes out to float32 sums of n terms.
+    want = torch.where(lengths[:, None, None, None] > 0, 0.75 * v[:, :, :1].double(), 0.0)
+    allowed = (2.0 ** -11 + 4 * (cap + 8) * 2.0 ** -24) * want.abs() + 2.0 ** -25
+    assert bool(((out.double() - want).abs() <= allowed).all())
+    short = differential_attention_cached(q[1:], k[1:, :, :100], v[1:, :, :100], lam, lengths[1:])
+    assert bool(((short.double() - want[1:]).abs() <= allowed[1:]).all())

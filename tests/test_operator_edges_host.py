@@ -9,7 +9,7 @@ import torch
 from torch.autograd import forward_ad
 
 from techjam_amd import UnsupportedCaseError
-from techjam_amd.kernels import LayerNorm, differential_attention, differential_attention_cached, layer_norm
+from techjam_amd.kernels import LayerNorm, _lib, differential_attention, differential_attention_cached, layer_norm
 
 attention_kernels = sys.modules["techjam_amd.kernels.differential"]
 norm_kernels = sys.modules["techjam_amd.kernels.layer_norm"]  # the package's attribute is the function
@@ -106,3 +106,24 @@ def test_scales_past_float32_are_refused(scale):
 @pytest.mark.parametrize("scale", [0.0, -2.0 ** 127, 2.0 ** 127, 1e-300])
 def test_scales_of_float32_are_taken(scale):
     assert attention_kernels._scale(scale, 64) == scale
+
+
+@pytest.mark.parametrize("b,h,hk,sq,sk,fits", [
+    (512, 32, 32, 1, 65536, True),       # 137 GB of keys and values at 32 dims in 16 bits
+    (1, 64, 64, 1, 1 << 24, True),
+    (2048, 8, 1, 1, 1 << 20, True),
+    (128, 1, 1, 1, 1 << 29, False),      # more blocks of keys than are counted in 32 bits
+    (1, 1, 1, 1, 1 << 30, False),
+    (1 << 20, 16, 1, 1, 16, False),      # a workgroup per row: 2^24 of them
+])
+def test_how_large_caches_may_be(b, h, hk, sq, sk, fits):
+    """What a call within the limits lacks here is its workspace; nothing is launched."""
+    L = _lib.lib()
+    st = (_lib.ctypes.c_int64 * 4)(64, 64, 64, 1)
+    p = 4096  # never dereferenced
+    code = L.tj_diff_attn_fwd(p, p, p, p, _lib.TJ_F16, b, h, hk, sq, sk, 32, 64, st, st, st, st, 0.125, 1, 1, p, 1, p,
+                              None, None, None, 0, None)
+    assert code == (_lib.TJ_ERR_WORKSPACE if fits else _lib.TJ_ERR_SHAPE)
+    if fits:
+        floats = L.tj_diff_attn_workspace_bytes(b, h, hk, sq, sk, 64, 1) // 4
+        assert 0 < floats < 1 << 28
