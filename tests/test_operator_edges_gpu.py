@@ -137,3 +137,64 @@ def test_many_sequences_of_a_large_capacity(cuda):
     assert bool(((out.double() - want).abs() <= allowed).all())
     short = differential_attention_cached(q[1:], k[1:, :, :100], v[1:, :, :100], lam, lengths[1:])
     assert bool(((short.double() - want[1:]).abs() <= allowed[1:]).all())
+
+
+# b, h, hk, s, d, dv, causal, lengths: float32 of up to 32 dims, 128 tokens and more, at most
+# 128 workgroups of 64 rows times parts. These run 32-row workgroups of four key groups.
+FOUR_GROUPS = {
+    "one_tile_each": (1, 1, 1, 128, 32, 64, True, None),
+    "one_key_more": (1, 1, 1, 129, 32, 64, False, None),
+    "ragged": (3, 2, 1, 201, 32, 64, True, (201, 0, 33)),
+    "shorter_than_the_groups": (3, 2, 2, 150, 16, 32, False, (1, 96, 97)),
+    "odd_dims": (2, 3, 1, 333, 20, 36, True, (333, 200)),
+    "in_parts": (1, 1, 1, 2048, 32, 64, True, None),
+    "in_parts_padded": (1, 1, 1, 2048, 8, 64, False, (1500,)),
+    "in_parts_of_few_keys": (1, 1, 1, 2048, 32, 32, True, (513,)),
+    # Past that bound, the neighbours in parts: 64 rows and two groups.
+    "two_groups_padded": (1, 2, 2, 2049, 8, 64, False, (1500,)),
+    "two_groups_of_few_keys": (1, 1, 1, 2100, 32, 32, True, (513,)),
+}
+
+
+def _four_groups(b, hk, rows, keys, parts):
+    return keys >= 128 and b * hk * -(-rows // 64) * parts <= 128
+
+
+@pytest.mark.parametrize("shape", FOUR_GROUPS)
+def test_small_float32_launches(cuda, shape):
+    b, h, hk, s, d, dv, causal, lens = FOUR_GROUPS[shape]
+    rows = s * (h // hk)
+    tiles = b * hk * -(-rows // 64)
+    parts = min(-(-512 // tiles), -(-s // 512)) if s >= 2048 else 1
+    assert _four_groups(b, hk, rows, s, parts) != shape.startswith("two_groups")
+    assert (parts > 1) == shape.startswith(("in_parts", "two_groups"))
+    q, k, v, lam, dout = inputs(torch.float32, b, h, hk, s, d, dv, seed=22)
+    lengths = None if lens is None else torch.tensor(lens, dtype=torch.int32, device="cuda")
+    leaves = [t.detach().requires_grad_() for t in (q, k, v, lam)]
+    out = differential_attention(*leaves, is_causal=causal, valid_len=lengths)
+    grads = torch.autograd.grad(out, leaves, dout)
+    with torch.no_grad():
+        plain = differential_attention(q, k, v, lam, is_causal=causal, valid_len=lengths)
+    want = attention(q, k, v, lam, causal=causal, lengths=lengths, dout=dout)
+    assert_within(out, want["out"], "out", 1e-40)
+    assert_within(plain, want["out"], "out without gradients", 1e-40)
+    for name, got in zip(("dq", "dk", "dv", "dlam"), grads):
+        assert_within(got, want[name], name, 1e-40)
+
+
+@pytest.mark.parametrize("new,capacity,lens", [(70, 300, (300, 71, 10)), (90, 4500, (4500, 600)), (65, 2048, (0, 2048))])
+def test_small_float32_chunks_against_a_cache(cuda, new, capacity, lens):
+    b, h, hk, d, dv = len(lens), 2, 1, 32, 64
+    rows = new * (h // hk)
+    tiles = b * hk * -(-rows // 64)
+    parts = min(-(-512 // tiles), -(-capacity // 512)) if capacity >= 2048 else 1
+    assert rows > 64 and _four_groups(b, hk, rows, capacity, parts)
+    q = inputs(torch.float32, b, h, hk, new, d, dv, seed=23)[0]
+    _, k, v, lam, _ = inputs(torch.float32, b, h, hk, capacity, d, dv, seed=24)
+    k, v = k.clone(), v.clone()
+    lengths = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    want = attention(q, k, v, lam, causal=True, lengths=lengths, cached=True)["out"]
+    for i, n in enumerate(lens):  # what lies behind a sequence's end is not read
+        k[i, :, n:] = float("nan")
+        v[i, :, n:] = float("inf")
+    assert_within(differential_attention_cached(q, k, v, lam, lengths), want, "out", 1e-40)
