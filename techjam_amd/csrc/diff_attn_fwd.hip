@@ -525,11 +525,14 @@ int launch_fwd(DiffArgs a, hipStream_t stream) {
   using GR = FwdGroups<T, HD, BLOCKS>;
   a.n_mtiles = (a.R + 32 * GR::RB - 1) / (32 * GR::RB);
   const int64_t n = (int64_t)a.B * a.Hk * a.n_mtiles;
-  if (a.n_parts > 1) {
-    hipLaunchKernelGGL((diff_fwd_kernel<T, HD, BLOCKS, true, true>), dim3(uint32_t(n * a.n_parts)), dim3(64 * GR::WAVES), 0,
-                       stream, a);
-    const int rc = tjh::launch_status();
-    return rc != TJ_OK ? rc : launch_join<T>(a, stream);
+  // Parts are for launches that 64-row workgroups do not fill, never for 128-row ones beside them.
+  if constexpr (BLOCKS != 4 || !row_blocks_fit<T, HD>(2)) {
+    if (a.n_parts > 1) {
+      hipLaunchKernelGGL((diff_fwd_kernel<T, HD, BLOCKS, true, true>), dim3(uint32_t(n * a.n_parts)), dim3(64 * GR::WAVES), 0,
+                         stream, a);
+      const int rc = tjh::launch_status();
+      return rc != TJ_OK ? rc : launch_join<T>(a, stream);
+    }
   }
   // Without statistics the long sweeps of 128-row workgroups save the second sum.
   if constexpr (BLOCKS == 4) {
