@@ -6,7 +6,8 @@ import pytest
 import torch
 
 from differential_reference import assert_within, attention
-from test_differential_gpu import FLOOR, inputs
+from test_differential_gpu import FLOOR, TYPES, inputs
+from test_layer_norm_gpu import check as norm_check, reference as norm_reference, rows_of as norm_rows
 from techjam_amd.kernels import differential_attention, differential_attention_cached, layer_norm
 
 pytestmark = pytest.mark.gpu
@@ -198,3 +199,53 @@ def test_small_float32_chunks_against_a_cache(cuda, new, capacity, lens):
         k[i, :, n:] = float("nan")
         v[i, :, n:] = float("inf")
     assert_within(differential_attention_cached(q, k, v, lam, lengths), want, "out", 1e-40)
+
+
+# b, h, hk, s, d, dv, causal, lengths: parts of narrow heads in 16 bits (at most 128 workgroups of 64 rows)
+NARROW_PARTS = {
+    "causal": (1, 2, 2, 2050, 32, 64, True, None),
+    "shared_padded": (1, 2, 1, 2048, 32, 64, False, (777,)),
+    "odd_dims": (1, 1, 1, 2777, 11, 21, True, (2600,)),
+}
+
+
+@pytest.mark.parametrize("dtype", ["fp16", "bf16"])
+@pytest.mark.parametrize("shape", NARROW_PARTS)
+def test_key_parts_of_narrow_heads(cuda, shape, dtype):
+    b, h, hk, s, d, dv, causal, lens = NARROW_PARTS[shape]
+    assert s >= 2048 and b * hk * -(-s * (h // hk) // 64) <= 128
+    q, k, v, lam, dout = inputs(TYPES[dtype], b, h, hk, s, d, dv, seed=25)
+    lengths = None if lens is None else torch.tensor(lens, dtype=torch.int32, device="cuda")
+    leaves = [t.detach().requires_grad_() for t in (q, k, v, lam)]
+    out = differential_attention(*leaves, is_causal=causal, valid_len=lengths)
+    grads = torch.autograd.grad(out, leaves, dout)
+    with torch.no_grad():
+        plain = differential_attention(q, k, v, lam, is_causal=causal, valid_len=lengths)
+    want = attention(q, k, v, lam, causal=causal, lengths=lengths, dout=dout)
+    assert_within(out, want["out"], "out", FLOOR[q.dtype])
+    assert_within(plain, want["out"], "out without gradients", FLOOR[q.dtype])
+    for name, got in zip(("dq", "dk", "dv", "dlam"), grads):
+        assert_within(got, want[name], name, FLOOR[q.dtype] if name != "dlam" else 1e-40)
+
+
+# One width for every span of columns a lane, wave or workgroup holds, in 16-byte chunks and in
+# single elements (odd widths).
+NORM_SPANS = (60, 64, 128, 256, 512, 1024, 2048, 4096, 8192, 16384, 101, 777, 2001, 9999)
+
+
+@pytest.mark.parametrize("dtype,norm_dtype", [("fp32", "fp32"), ("fp16", "fp16"), ("bf16", "bf16"), ("fp16", "fp32"), ("bf16", "fp32")])
+@pytest.mark.parametrize("width", NORM_SPANS)
+def test_norms_of_every_span(cuda, width, dtype, norm_dtype):
+    g = torch.Generator().manual_seed(width)
+    rows = 9
+    x = norm_rows(g, rows, width, TYPES[dtype])
+    dy = (0.3 * torch.randn(rows, width, generator=g)).to(TYPES[norm_dtype]).cuda()
+    w, b = (1 + 0.2 * torch.randn(width, generator=g)).cuda(), (0.1 * torch.randn(width, generator=g)).cuda()
+    want = norm_reference(x, w, b, dy, 1e-5)
+    if dtype != norm_dtype:
+        want["y"] = norm_reference(x.float(), w, b, dy, 1e-5)["y"]
+    leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+    y = layer_norm(*leaves, norm_dtype=TYPES[norm_dtype])
+    grads = torch.autograd.grad(y, leaves, dy)
+    for name, got in zip(("y", "dx", "dw", "db"), (y, *grads)):
+        norm_check(got, want[name], name)
