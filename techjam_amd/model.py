@@ -281,7 +281,9 @@ class EncoderBlock(nn.Module):
         return x + self.ffn_out(self._act(self.ffn_in(self.norm2(x))))
 
     def _can_fuse(self, x, valid_token_mask, valid_len) -> bool:
-        if self.differentiable and (torch.is_grad_enabled() or self.ffn_in.weight.dtype != torch.float32):
+        # The fused passes take float32 products, which autocast's are not.
+        if self.differentiable and (torch.is_grad_enabled() or self.ffn_in.weight.dtype != torch.float32
+                                    or torch.is_autocast_enabled("cuda")):
             return False
         return (x.is_cuda and x.dtype == torch.float32 and x.ndim == 3 and x.is_contiguous()
                 and x.data_ptr() % 16 == 0 and x.shape[-1] % 4 == 0 and self.ffn_in.out_features % 4 == 0

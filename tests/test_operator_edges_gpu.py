@@ -7,6 +7,7 @@ import torch
 
 from differential_reference import assert_within, attention
 from test_differential_gpu import FLOOR, TYPES, inputs
+from test_differential_model_gpu import encoder
 from test_layer_norm_gpu import check as norm_check, reference as norm_reference, rows_of as norm_rows
 from techjam_amd.kernels import differential_attention, differential_attention_cached, layer_norm
 
@@ -249,3 +250,17 @@ def test_norms_of_every_span(cuda, width, dtype, norm_dtype):
     grads = torch.autograd.grad(y, leaves, dy)
     for name, got in zip(("y", "dx", "dw", "db"), (y, *grads)):
         norm_check(got, want[name], name)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("variant", [dict(), dict(d=96, heads=3, seq=33), dict(norm_first=False, activation="relu")])
+def test_autocast_gives_evaluation_what_it_gives_training(cuda, variant, dtype):
+    """The encoder's forward pass under autocast, with and without gradients: the same operators, the same bits."""
+    model, x, _, mask = encoder(**variant)
+    model, x, mask = model.cuda(), x.cuda(), mask.cuda()
+    with torch.autocast("cuda", dtype):
+        want = model(x, mask)
+        assert want.requires_grad
+        for mode in (torch.no_grad, torch.inference_mode):
+            with mode():
+                assert torch.equal(model(x, mask), want)
