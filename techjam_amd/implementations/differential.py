@@ -122,6 +122,9 @@ class DifferentialSelfAttention(nn.Module):
         of ``lengths`` (these included), whose places in the cache are ``place``
         (int64 ``[B, T]``)."""
         q, k, v = self.qkv(x)
+        if k.dtype != cache.k.dtype:
+            raise ValueError(f"the cache holds {cache.k.dtype}, the step's keys and values are {k.dtype}: "
+                             "create the state in that dtype")
         rows = torch.arange(x.shape[0], device=x.device)[:, None]
         cache.k[rows, :, place] = k.transpose(1, 2)
         cache.v[rows, :, place] = v.transpose(1, 2)

@@ -475,8 +475,9 @@ class TransformerEncoder(nn.Module):
 
     # -- token by token (causal differential attention) ----------------------
     def new_state(self, batch: int, capacity: int, dtype: Optional[torch.dtype] = None):
-        """Empty caches for ``batch`` sequences of up to ``capacity`` tokens, in
-        the parameters' type unless ``dtype`` says otherwise."""
+        """Empty caches for ``batch`` sequences of up to ``capacity`` tokens. Their
+        type is that of the steps' projections: the parameters' (the default),
+        or autocast's for steps under it; a step whose type differs is refused."""
         from .errors import UnsupportedCaseError
         from .implementations.differential import DifferentialState
 
