@@ -407,7 +407,7 @@ int tj_narrow_ffn_norm(const float* x, const float* w_in, const float* bias_in, 
  *
  * lse and maps, both or neither: what tj_diff_attn_bwd reads again, contiguous
  * fp32: log2 of the rows' softmax sums [B, H, 2, Sq] and the two maps' outputs
- * [B, H, Sq, 2, Dv], unrounded.
+ * [B, H, Sq, 2, Dv], unrounded (8 Dv bytes a row and head, four times a 16-bit o).
  *
  * workspace: tj_diff_attn_workspace_bytes bytes, 16-byte aligned, contents
  * irrelevant, calls sharing one ordered on one stream: where few rows sweep many

@@ -458,7 +458,8 @@ struct FewParts {
 // Products with fp16 operands: powers of two that bring the largest possible |dS|,
 // 2 |dO_i| |V_j| max(1, |lam|), near 2^15, so that small gradients and small
 // probabilities keep fp16's bits. dQ is a sum over keys, so there every row has
-// its own, by its dO (of): a row's bits do not depend on how large others are.
+// its own, by its dO (of) and the largest V row: a row's bits do not depend on
+// how large the gradients of others are.
 // dK sums over rows and has one for all of a (b, key head), by the largest dO
 // row: dS of a row r times smaller keeps 11 bits down to P of about 2^-26 r, and
 // what lies below is off by at most 2^-37 of the largest possible |dS|. 1 for the
@@ -575,9 +576,13 @@ inline FewPlan few_plan(int64_t B, int64_t Hk, int64_t mtiles, int64_t Sk, int64
 
 // Whether there are 128-row tiles enough for workgroups to take them rather than 64-row ones:
 // two rounds of them where two fit a CU; where one does, one, and two of causal ones,
-// whose lengths differ. Forward passes, us with 128 / 64 rows: 64 dims bf16, 1024
-// tiles 436 / 453, 512 tiles of a causal training step 520 / 466 (whole step); 32 dims,
-// 1024 tiles 157 / 182; 128 dims, 290 tiles 68 / 81, causal 256 tiles 174 / 141, 512 tiles 227 / 280.
+// whose lengths differ. us with 128 / 64 rows, bf16, 4096 tokens. 64 dims, causal: forward
+// with sums 512 tiles 164 / 156, 640 tiles 175 / 186, 768 tiles 201 / 212, 1024 tiles 245 / 263, dQ
+// 172 / 146, 178 / 174, 196 / 199, 257 / 255; not causal, forward 226 / 247, 333 / 309, 343 / 365,
+// 437 / 481, dQ 233 / 246, 344 / 309, 354 / 366, 455 / 484. So 1024 is where both gain whatever the
+// mask; the causal forward alone would from 640 on. 32 dims, causal forward: 512 tiles 107 / 90, 768
+// tiles 130 / 123, 1024 tiles 154 / 161. 128 dims forward, 290 tiles 68 / 81, causal 256 tiles
+// 174 / 141, 512 tiles 227 / 280.
 inline bool wide_tiles(const DiffArgs& a, int hd) {
   return (int64_t)a.B * a.Hk * ((a.R + 127) / 128) >= (hd == 128 ? (a.causal ? 512 : 256) : 1024);
 }

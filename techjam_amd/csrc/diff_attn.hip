@@ -18,7 +18,13 @@ struct DiffPlan {
   int64_t n_parts;
 };
 
-// Rows of one key head up to which every wave works by itself.
+// Rows of one key head up to which every wave works by itself, so that the parts of the
+// keys follow the batch's lengths. us by waves / by workgroups, 16 sequences against caches
+// of 65536, 4 key heads, d64 bf16: lengths spread over a factor of four, 4 rows 249 / 270, 32
+// rows 265 / 286, 64 rows 455 / 320; one long sequence among short ones 40 / 153, 45 / 156,
+// 70 / 216. Past 64 rows the waves read the keys too often: spread to 16384, 80 rows 188 / 140,
+// 256 rows 520 / 300. (Even lengths alone would have the border lower: 64 sequences of 2048
+// and fewer, 8 key heads, 16 rows 104 / 71.)
 constexpr int64_t kFewRows = 64;
 
 // More rows than few: parts of at least kPartKeys keys where workgroups of 64 rows

@@ -230,7 +230,12 @@ def differential_attention(
     view. Gradients come for q, k, v and lam (summed over what shares a weight);
     their sums have a fixed order, so equal calls give equal bits. Second
     derivatives and forward-mode ones (``torch.autograd.forward_ad``) are not
-    implemented and refused.
+    implemented and refused. For the backward pass a call keeps its inputs and
+    both maps' outputs in float32, ``8 * B * H * S * (Dv + 1)`` bytes.
+
+    A training step can be captured into a graph as any of torch's: while it is
+    captured, no graph of an earlier eager call on the same leaves may be alive
+    (delete its outputs first).
     """
     _check(q, k, v, lam, valid_len, "valid_len", False)
     scale = _scale(scale, q.shape[-1])
@@ -261,7 +266,8 @@ def differential_attention_cached(
     ``lengths`` (int32 ``[B]`` on the device) counts them. Token ``t`` sees the
     keys up to its position ``lengths[b] - T + t``; tokens at a negative position
     (a sequence shorter than ``T``, an empty slot of the batch) get zeros. Lengths
-    are clipped to ``C``, and what the caches hold behind them is not read.
+    are clipped to ``C``, and what the caches hold behind them is not read. ``B *
+    H * T`` is below 2^24 where ``T * H / Hk`` is at most 64.
 
     How the keys are shared among the GPU's units follows the batch's lengths, so
     a sequence's last bits may differ beside other sequences; equal calls give
