@@ -39,13 +39,16 @@ def on_device(device: torch.device):
     return torch.cuda.device(device)
 
 
+def tangents_enabled() -> bool:
+    """Whether tensors may carry forward-mode tangents that operators have to hand on."""
+    return forward_ad._current_level >= 0 and torch._C._is_fwd_grad_enabled()
+
+
 def refuse_tangents(*tensors: Optional[torch.Tensor]) -> None:
     """Forward-mode derivatives are not implemented. A dual tensor need not
     require grad, so without a look at it a call outside of autograd would
     return its output without the tangent, which torch takes as zero."""
-    if forward_ad._current_level < 0 or not torch._C._is_fwd_grad_enabled():
-        return
-    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+    if tangents_enabled() and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise UnsupportedCaseError("forward-mode derivatives are not implemented")
 
 

@@ -21,6 +21,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from .kernels.attention import scaled_dot_product_attention
+from .kernels.differential import tangents_enabled
 from .kernels.elementwise import NORM_WIDTHS
 from .kernels.layer_norm import LayerNorm
 from .kernels.linear import ffn_norm, projections, residual_norm, split_products_allowed
@@ -281,9 +282,10 @@ class EncoderBlock(nn.Module):
         return x + self.ffn_out(self._act(self.ffn_in(self.norm2(x))))
 
     def _can_fuse(self, x, valid_token_mask, valid_len) -> bool:
-        # The fused passes take float32 products, which autocast's are not.
+        # The fused passes have no derivatives of either mode, and take float32
+        # products, which autocast's are not.
         if self.differentiable and (torch.is_grad_enabled() or self.ffn_in.weight.dtype != torch.float32
-                                    or torch.is_autocast_enabled("cuda")):
+                                    or torch.is_autocast_enabled("cuda") or tangents_enabled()):
             return False
         return (x.is_cuda and x.dtype == torch.float32 and x.ndim == 3 and x.is_contiguous()
                 and x.data_ptr() % 16 == 0 and x.shape[-1] % 4 == 0 and self.ffn_in.out_features % 4 == 0

@@ -4,11 +4,13 @@ from __future__ import annotations
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 from differential_reference import assert_within, attention
 from test_differential_gpu import FLOOR, TYPES, inputs
-from test_differential_model_gpu import encoder
+from test_differential_model_gpu import TOLERANCE, close, encoder
 from test_layer_norm_gpu import check as norm_check, reference as norm_reference, rows_of as norm_rows
+from techjam_amd import UnsupportedCaseError
 from techjam_amd.kernels import differential_attention, differential_attention_cached, layer_norm
 
 pytestmark = pytest.mark.gpu
@@ -264,3 +266,22 @@ def test_autocast_gives_evaluation_what_it_gives_training(cuda, variant, dtype):
         for mode in (torch.no_grad, torch.inference_mode):
             with mode():
                 assert torch.equal(model(x, mask), want)
+
+
+@pytest.mark.parametrize("grad", [True, False])
+@pytest.mark.parametrize("variant", [dict(), dict(d=96, heads=3, seq=33), dict(norm_first=False, activation="relu")])
+def test_encoders_do_not_drop_tangents(cuda, variant, grad):
+    """A parameter with a tangent: the norm after it refuses, instead of a fused pass that ignores it."""
+    model, x, _, mask = encoder(**variant)
+    model, x, mask = model.cuda(), x.cuda(), mask.cuda()
+    ffn = model.layers[-1].ffn_out
+    with torch.no_grad():
+        want = model(x, mask)
+    with torch.set_grad_enabled(grad), forward_ad.dual_level():
+        # A level without tangents: both forms are within TOLERANCE of the exact result.
+        close(model(x, mask), want.cpu(), "no tangents", 2 * TOLERANCE)
+        weight = ffn.weight.detach()
+        del ffn.weight
+        ffn.weight = forward_ad.make_dual(weight, torch.ones_like(weight))
+        with pytest.raises(UnsupportedCaseError, match="forward-mode"):
+            model(x, mask)
