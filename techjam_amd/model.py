@@ -244,6 +244,8 @@ class EncoderBlock(nn.Module):
         super().__init__()
         if activation not in ACTIVATIONS:
             raise ValueError(f"activation must be one of {ACTIVATIONS}, not {activation!r}")
+        if attention not in ATTENTIONS:
+            raise ValueError(f"attention must be one of {ATTENTIONS}, not {attention!r}")
         self.norm_first = norm_first
         self.activation = activation
         #: Whether every operator of the block has gradients: with them enabled

@@ -10,7 +10,7 @@ from torch.autograd import forward_ad
 
 from techjam_amd import UnsupportedCaseError
 from techjam_amd.kernels import LayerNorm, _lib, differential_attention, differential_attention_cached, layer_norm
-from techjam_amd.model import TransformerConfig, TransformerEncoder
+from techjam_amd.model import EncoderBlock, TransformerConfig, TransformerEncoder
 
 attention_kernels = sys.modules["techjam_amd.kernels.differential"]
 norm_kernels = sys.modules["techjam_amd.kernels.layer_norm"]  # the package's attribute is the function
@@ -142,3 +142,11 @@ def test_steps_of_another_type_than_the_cache_are_refused(dtype):
     assert not bool(cache.k.any())
     with torch.autocast("cpu", dtype), pytest.raises(UnsupportedCaseError, match="GPU"):
         attention.step(x, cache, lengths, place)  # autocast's type is the cache's
+
+
+def test_blocks_of_unknown_attention_are_refused():
+    """Any word but "differential" would have built softmax attention."""
+    with pytest.raises(ValueError, match="attention must be one of"):
+        EncoderBlock(16, 2, 32, attention="differental")
+    with pytest.raises(ValueError, match="attention must be one of"):
+        TransformerEncoder(TransformerConfig(2, 8, 16, 2, 32, 1, True, attention="differental"))
