@@ -188,7 +188,10 @@ diff_bwd_q_kernel(DiffArgs a) {
       for (int j = 0; j < 8; ++j) norm = fmaf((float)of[s][j], (float)of[s][j], norm);
     norm = sqrtf(pair_sum(norm));
   }
-  const float lift = DsLift<T>(a, t.bh, t.hk, lane).of(norm);
+  const DsLift<T> lifts(a, t.bh, t.hk, lane);
+  const float lift = lifts.of(norm);
+  // The rows' common one, for `stat`: the same in every lane, so a scalar register holds it through the sweep.
+  const float lift_all = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(lifts.all())));
   const float c2 = a.scale * kLog2e;
   const float lam = live ? a.lam[head * a.lam_step] : 0.f;
   float lse[2], del[2];
@@ -295,7 +298,7 @@ diff_bwd_q_kernel(DiffArgs a) {
   rest[1] = pair_sum(rest[1]);
   // P is lifted by pl in its exponent in the dK, dV kernel, and dS by one lift for all
   // rows; what multiplies P to dS takes the former out again.
-  const float pl = p_lift<T>(a, t.hk), dl = DsLift<T>(a, t.bh, t.hk, lane).all() / pl;
+  const float pl = p_lift<T>(a, t.hk), dl = lift_all / pl;
   if (r >= a.R) return;
   if (hl == 0) {
     a.gsum[row_at(a, t.b, head, i)] = live ? del[1] + rest[1] : 0.f;

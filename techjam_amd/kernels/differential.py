@@ -231,7 +231,9 @@ def differential_attention(
 
     The output's storage is ``[B, S, H, Dv]``, so that merging the heads is a
     view. Gradients come for q, k, v and lam (summed over what shares a weight);
-    their sums have a fixed order, so equal calls give equal bits. Second
+    their sums have a fixed order, so equal calls give equal bits. In float16 the
+    gradient of ``k`` sums its rows at one scale: beside an output gradient 1e6
+    times larger in the same sequence and key head, a row's share loses bits. Second
     derivatives and forward-mode ones (``torch.autograd.forward_ad``) are not
     implemented and refused. For the backward pass a call keeps its inputs and
     both maps' outputs in float32, ``8 * B * H * S * (Dv + 1)`` bytes.
