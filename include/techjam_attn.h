@@ -442,6 +442,79 @@ int tj_diff_attn_bwd(const void* q, const void* k, const void* v, const float* m
                      void* workspace, size_t workspace_bytes, hipStream_t stream);
 
 /*
+ * Softmax attention of packed sequences with grouped heads, forward. It stands
+ * beside tj_attn_fwd (F.scaled_dot_product_attention at
+ * src/implementations/sdpa.py:65-73 in the reference, which pads its batches).
+ *
+ *   o[t,h,:] = sum_u P[t,u] v[u,h',:],  P[t,.] = softmax(scale * q[t,h,:] . k[u,h',:]),  h' = h / (H / Hk)
+ *
+ * over the tokens u of t's own sequence (u <= t when `causal`). q [T, H, D],
+ * k [T, Hk, D], v [T, Hk, Dv], o [T, H, Dv]; H a multiple of Hk. Sequence n of N has the
+ * rows offsets[n] .. offsets[n + 1] - 1 (int32 on the device, N + 1 of them, none below
+ * the one before, none below 0 or above T), of which the first lengths[n] hold tokens
+ * (all of them when lengths is NULL; clipped to what is there). All other rows, before the first
+ * and behind the last sequence too, are written as zeros; what they hold is not
+ * read. Offsets out of order give wrong rows, but no access outside of the tensors.
+ * Sizes (TJ_ERR_SHAPE past them): H (T + 64) below 2^30, Hk ((T / 32 + 1) H / Hk + N + 4) below 2^23.
+ *
+ * dtype: TJ_F32, TJ_F16 or TJ_BF16, shared by q, k, v and o, with the products of
+ * tj_diff_attn_fwd. D and Dv <= 128, both multiples of 16 bytes. Strides in
+ * elements, the innermost 1, the others multiples of 16 bytes; 64 rows of k and v (and
+ * of q and dout below) within 2 GiB (TJ_ERR_UNSUPPORTED otherwise).
+ *
+ * lse: fp32 [T, H], what tj_packed_attn_bwd reads again, or NULL: log2 of the rows'
+ * softmax sums (rows without a token are not written).
+ */
+int tj_packed_attn_fwd(const void* q, const void* k, const void* v, void* o, int dtype,
+                       int64_t T, int64_t N, int64_t H, int64_t Hk, int64_t D, int64_t Dv,
+                       const int64_t q_strides[3], const int64_t k_strides[3],
+                       const int64_t v_strides[3], const int64_t o_strides[3],
+                       float scale, int causal, const int32_t* offsets, const int32_t* lengths,
+                       float* lse, hipStream_t stream);
+
+/*
+ * The gradients of tj_packed_attn_fwd for the output gradient dout [T, H, Dv]: dq, dk, dv
+ * (shaped and typed like q, k, v). o and lse come from the forward call. Rows without a token
+ * get zeros and their dout is not read. The sums' order is fixed: the same call gives the
+ * same bits. workspace: tj_packed_attn_bwd_workspace_bytes bytes, 16-byte aligned, contents
+ * irrelevant, calls sharing one ordered on one stream.
+ */
+size_t tj_packed_attn_bwd_workspace_bytes(int64_t T, int64_t N, int64_t H, int64_t Hk);
+int tj_packed_attn_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse,
+                       const void* dout, void* dq, void* dk, void* dv, int dtype,
+                       int64_t T, int64_t N, int64_t H, int64_t Hk, int64_t D, int64_t Dv,
+                       const int64_t q_strides[3], const int64_t k_strides[3], const int64_t v_strides[3],
+                       const int64_t o_strides[3], const int64_t do_strides[3], const int64_t dq_strides[3],
+                       const int64_t dk_strides[3], const int64_t dv_strides[3],
+                       float scale, int causal, const int32_t* offsets, const int32_t* lengths,
+                       void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/*
+ * Softmax attention of the Sq newest tokens of each sequence against its cache, with grouped
+ * heads: q [B, H, Sq, D], k [B, Hk, Sk, D], v [B, Hk, Sk, Dv], o [B, H, Sq, Dv]. lengths[b]
+ * (int32 on the device, clipped to 0 .. Sk) counts the keys in the cache, these tokens' own among
+ * them: token i stands at position lengths[b] - Sq + i.
+ * parents NULL: token i sees the keys up to its position. Else (int32 [B, Sq] on the
+ * device, contiguous, Sq <= 64, TJ_ERR_UNSUPPORTED otherwise) the tokens are drafts that
+ * form trees: token i sees the keys before the drafts, its own, and those of the drafts on its
+ * line of parents, parents[b][i] < i, which ends at -1.
+ * A token whose parent is neither -1 nor one of those before it is not there, nor are those
+ * on whose line it stands and those at a negative position: their rows are written as zeros, and
+ * what the cache holds in their place may be anything. What it holds behind lengths[b] is not read.
+ * Sizes (TJ_ERR_SHAPE past them): B H Sq below 2^23 - 2^16, B Hk below 2^22, B Sk below 2^35.
+ * Types, dims and strides as in tj_packed_attn_fwd (four strides). workspace:
+ * tj_tree_attn_workspace_bytes bytes, as above; NULL where that is 0.
+ */
+size_t tj_tree_attn_workspace_bytes(int dtype, int64_t B, int64_t H, int64_t Hk, int64_t Sq, int64_t Sk,
+                                    int64_t D, int64_t Dv);
+int tj_tree_attn_fwd(const void* q, const void* k, const void* v, void* o, int dtype,
+                     int64_t B, int64_t H, int64_t Hk, int64_t Sq, int64_t Sk, int64_t D, int64_t Dv,
+                     const int64_t q_strides[4], const int64_t k_strides[4],
+                     const int64_t v_strides[4], const int64_t o_strides[4],
+                     float scale, const int32_t* lengths, const int32_t* parents,
+                     void* workspace, size_t workspace_bytes, hipStream_t stream);
+
+/*
  * Layer norm of rows, forward and backward (torch.nn.LayerNorm's formula over
  * the last dimension, torch_transformer_benchmark.py:125-172, where the norms
  * are torch's):

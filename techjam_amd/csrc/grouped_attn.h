@@ -1,0 +1,333 @@
+// Softmax attention with grouped heads for gfx950: shared by the kernels of
+// packed sequences (packed_attn_fwd.hip, packed_attn_bwd.hip), of drafted tokens
+// against a cache (tree_attn.hip) and their entry points (grouped_attn.hip).
+//
+//   O_h = softmax(scale Q_h K_{h'}^T) V_{h'},   h' = h / G,  G = H / Hk.
+//
+// The G query heads of one key head are handled together: their query rows are
+// numbered r = i G + g (token i, head g of the group), so that neighbouring rows
+// see nearly the same keys, one sweep over K and V serves the whole group, and
+// the sums over the group in dK and dV are sums over rows.
+#pragma once
+
+#include "attn_tiles.h"
+
+namespace tj {
+
+// Strided [rows, heads, dim] view with unit dim stride.
+struct View3 {
+  int64_t st, sh;
+  __device__ __forceinline__ int64_t row(int64_t t, int h) const { return t * st + h * sh; }
+};
+
+struct PackedArgs {
+  const void *q, *k, *v;
+  void* o;
+  View3 vq, vk, vv, vo;
+  int T, N;                // tokens in all, sequences
+  int H, Hk, G, D, Dv;
+  float scale;
+  int causal;
+  const int32_t* off;      // [N + 1]
+  const int32_t* len;      // [N] valid tokens of each sequence's rows, or null: all
+  float* lse;              // [T, H] log2 of a row's sum of 2^(score log2 e); or null
+  int n_slots;             // of the launch, see Region
+  // Backward.
+  const void *out, *dout;
+  View3 vdo, vdq, vdk, vdv;
+  void *dq, *dk, *dv;
+  float* stat;             // [slots of 32 tokens, H, 2, 32] what the dK, dV kernel reads of a row
+  float* peak;             // [slots of 64 tokens, Hk, 2] largest norms of dO and V rows (fp16 operands)
+};
+
+// The rows fall into regions: what lies before the first sequence, the sequences,
+// and what lies behind the last, whose rows are written as zeros. Region j of
+// regions() starts at token edge(j).
+//
+// Where a tile of `unit` rows belongs is found without a list of tiles, which would
+// cost a launch, and without the lengths on the host, which would cost a wait: region
+// j's tiles have the slots from slot(j) = edge(j) per / unit + j on, rows counted
+// `per` a token. A region of n rows has at most slot(j + 1) - slot(j) tiles, so the
+// slots do not overlap, and at most one a region is left over. Offsets
+// are clipped to 0 .. T, and offsets out of order give wrong rows, but none outside.
+struct Region {
+  int index, start, rows, len, tile;
+
+  __device__ __forceinline__ static int regions(const PackedArgs& a) { return a.N + 2; }
+  __device__ __forceinline__ static int edge(const PackedArgs& a, int j) {
+    if (j <= 0) return 0;
+    return j > a.N + 1 ? a.T : min(a.T, max(0, a.off[j - 1]));
+  }
+  __device__ __forceinline__ static int slot(int edge, int j, int per, int unit) { return (int)((int64_t)edge * per / unit) + j; }
+
+  // The region and tile of `at`, in every lane of the wave that asks; false for a slot left
+  // over. Sixty-four regions are looked at at a time.
+  __device__ __forceinline__ bool find(const PackedArgs& a, int at, int per, int unit, int lane) {
+    int lo = 0, n = regions(a), first = 0;
+    while (n > 1) {
+      const int step = (n + kWave - 1) / kWave, j = lo + lane * step;
+      const bool in = lane * step < n;
+      const int s = in ? slot(edge(a, j), j, per, unit) : 0;
+      const int before = max(1, (int)__popcll(__ballot(in && s <= at)));
+      lo += (before - 1) * step;
+      n = min(step, n - (before - 1) * step);
+    }
+    index = __builtin_amdgcn_readfirstlane(lo);
+    start = __builtin_amdgcn_readfirstlane(edge(a, index));
+    rows = max(0, __builtin_amdgcn_readfirstlane(edge(a, index + 1)) - start);
+    first = slot(start, index, per, unit);
+    tile = at - first;
+    const bool sequence = index > 0 && index <= a.N;
+    len = !sequence ? 0 : (a.len == nullptr ? rows : min(rows, max(0, __builtin_amdgcn_readfirstlane(a.len[index - 1]))));
+    return tile >= 0 && (int64_t)tile * unit < (int64_t)rows * per;
+  }
+};
+
+struct TreeArgs {
+  const void *q, *k, *v;
+  void* o;
+  View4 vq, vk, vv, vo;
+  int B, H, Hk, G, D, Dv;
+  int Sq, Sk;              // drafted tokens, capacity of the cache
+  int R;                   // rows of one key head: Sq * G
+  float scale;
+  const int32_t* len;      // [B]
+  const int32_t* parents;  // [B, Sq], or null: a chain
+  int n_mtiles;
+  // Parts of the keys (FewParts), n_parts in all, which leave unnormalised sums [n_parts, Hk, R, Dv] and
+  // (maximum, sum, whether the row is there, -) [n_parts, Hk, R, 4]. part_o null: sweeps run whole.
+  int n_parts, few_slots, few_each;
+  float *part_o, *part_ml;
+};
+
+inline int64_t region_slots(int64_t T, int64_t N, int64_t per, int64_t unit) { return T * per / unit + N + 2; }
+
+constexpr float kLazy = 8.f;  // the running maximum moves when a row's maximum grows by more than 2^8
+
+// HD: head dim computed, 32, 64, 96 or 128; a row of an LDS tile holds the next power of two.
+template <typename T, int HD, int BNT>
+struct SweepShape {
+  static constexpr int W = HD <= 32 ? 32 : (HD <= 64 ? 64 : 128);
+  static constexpr int BN = BNT;       // keys of a tile
+  using Rows = LdsRows<T, W>;
+  static constexpr int KS = HD / 16;   // k-steps over the head dim
+  static constexpr int DB = HD / 32;   // output blocks
+  static constexpr int kDepth = sizeof(T) == 2 && HD > 32 ? 2 : 0;
+  static constexpr int kTensor = BN * W * (int)sizeof(T), kBytes = 2 * kTensor;  // K's tile, then V's
+};
+
+// A lane's row: r of the tile's (region or sequence, key head): its token, head, and
+// the last key it sees.
+struct SweepRow {
+  int r, i, g, limit;
+  bool live;
+};
+
+// The running state of a wave's NB blocks of 32 rows. Scores are formed transposed,
+// S^T = K Q^T, so that a lane holds scores of ONE row of a block: maximum and sum are
+// per lane (the other half of the wave holds the other keys), and the probabilities
+// turn into the B operand of O^T = V^T P^T where they stand. Every K and V fragment
+// read from LDS serves all NB blocks.
+//
+// The output is divided by the sum of the probabilities as they were rounded for its
+// product (to the inputs' type: fp32 MFMAs would take 16 times as long): a dominant
+// key's rounding cancels, and two go into one instruction. What the backward pass
+// gets (STATS) is the sum of the unrounded ones, so that its P sums to 1 as exactly
+// as fp32 does.
+template <typename T, int HD, int BN, int NB, bool STATS>
+struct SweepState {
+  using SH = SweepShape<T, HD, BN>;
+  frag_t<T> q[NB][SH::KS];
+  float16_t o[NB][SH::DB];
+  float m[NB], l[NB];  // maximum in log2 units, the lane's part of the sum
+  float e[STATS ? NB : 1];
+  float c2;            // |scale| log2 e
+  uint32_t kbase, vbase;  // the lane's places in a tile
+
+  __device__ __forceinline__ void init(float scale, int lane) {
+    kbase = SH::Rows::lane_row(lane);
+    vbase = SH::Rows::lane_col(lane) + SH::kTensor;
+    // A negative scale turns q's sign, so that the largest score is the largest
+    // product; a zero one becomes too small to matter, so that masked stays -inf.
+    c2 = fmaxf(fabsf(scale) * kLog2e, 1e-37f);
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      m[n] = -__builtin_inff();
+      l[n] = 0.f;
+      if constexpr (STATS) e[n] = 0.f;
+#pragma unroll
+      for (int d = 0; d < SH::DB; ++d) o[n][d] = zero16();
+    }
+  }
+  // Block n's rows of q; null: a row that is not there.
+  __device__ __forceinline__ void load_q(int n, const T* p, float scale, int width, int lane) {
+#pragma unroll
+    for (int ks = 0; ks < SH::KS; ++ks) {
+      q[n][ks] = load_frag<T>(p, 16 * ks + 8 * (lane / 32), width);
+      if (scale < 0.f)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) q[n][ks][j] = -q[n][ks][j];
+    }
+  }
+
+  // 32 keys of a tile, from its key 32 kb on. mask(n, s): sets block n's scores of keys that the
+  // lane's row does not see to -inf.
+  template <typename Mask>
+  __device__ __forceinline__ void step(uint32_t tile, int kb, Mask&& mask) {
+    const uint32_t kt = tile + kbase, vt = tile + vbase;
+    frag_t<T> p[NB][2];
+    float16_t s[NB];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) s[n] = zero16();
+    read_ahead<SH::KS, SH::kDepth>([&](int ks) { return SH::Rows::row_frag(kt, ks, kb * 32 * SH::Rows::kRowBytes); },
+                                   [&](int ks, frag_t<T> f) {
+#pragma unroll
+                                     for (int n = 0; n < NB; ++n) s[n] = Elem<T>::mma(f, q[n][ks], s[n]);
+                                   });
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      mask(n, s[n]);
+      float top = s[n][0];
+#pragma unroll
+      for (int r = 1; r < 16; ++r) top = fmaxf(top, s[n][r]);
+      top = pair_max(top) * c2;
+      // The maximum moves by the row's need; one decision for the wave.
+      const bool move = top > m[n] + kLazy;  // also from -inf
+      if (__any(move)) {
+        const float to = move ? top : m[n];
+        const float alpha = m[n] == -__builtin_inff() ? 0.f : fast_exp2(m[n] - to);
+        m[n] = to;
+        l[n] *= alpha;
+        if constexpr (STATS) e[n] *= alpha;
+#pragma unroll
+        for (int d = 0; d < SH::DB; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[n][d][r] *= alpha;
+      }
+      // A row that has seen no key keeps its unset maximum out of the exponent.
+      const float off = m[n] == -__builtin_inff() ? 0.f : Elem<T>::kLift - m[n];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[n][r] = fast_exp2(fmaf(s[n][r], c2, off));
+        if constexpr (STATS) e[n] += s[n][r];
+      }
+#pragma unroll
+      for (int st = 0; st < 2; ++st) {
+        p[n][st] = acc_frag<T>(s[n], st);
+        l[n] = frag_sum(p[n][st], l[n]);
+      }
+    }
+    read_ahead<2 * SH::DB, SH::kDepth>(
+        [&](int j) { return SH::Rows::col_frag(vt, j % SH::DB, (kb * 32 + 16 * (j / SH::DB)) * SH::Rows::kRowBytes); },
+        [&](int j, frag_t<T> f) {
+#pragma unroll
+          for (int n = 0; n < NB; ++n) o[n][j % SH::DB] = Elem<T>::mma(f, p[n][j / SH::DB], o[n][j % SH::DB]);
+        });
+  }
+
+  // Adds the state of another wave over the same rows and other keys, which that wave has left
+  // in LDS (give).
+  static constexpr int kGive = SH::DB * 4 * kWave;  // float4 per block
+  static constexpr int kMl = STATS ? 3 : 2;         // numbers of a lane and block beside them
+  __device__ __forceinline__ void give(float4_t* x, float* ml, int lane) {
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      ml[(kMl * n) * kWave + lane] = m[n];
+      ml[(kMl * n + 1) * kWave + lane] = l[n];
+      if constexpr (STATS) ml[(kMl * n + 2) * kWave + lane] = e[n];
+#pragma unroll
+      for (int d = 0; d < SH::DB; ++d)
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+          x[n * kGive + (d * 4 + c) * kWave + lane] =
+              float4_t{o[n][d][4 * c], o[n][d][4 * c + 1], o[n][d][4 * c + 2], o[n][d][4 * c + 3]};
+    }
+  }
+  __device__ __forceinline__ void take(const float4_t* x, const float* ml, int lane) {
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      const float m1 = ml[(kMl * n) * kWave + lane], to = fmaxf(m[n], m1);
+      // An unset maximum (-inf) goes with sums that are zero, or NaN and kept.
+      const float w0 = m[n] == -__builtin_inff() ? 1.f : fast_exp2(m[n] - to);
+      const float w1 = m1 == -__builtin_inff() ? 1.f : fast_exp2(m1 - to);
+      m[n] = to;
+      l[n] = fmaf(l[n], w0, ml[(kMl * n + 1) * kWave + lane] * w1);
+      if constexpr (STATS) e[n] = fmaf(e[n], w0, ml[(kMl * n + 2) * kWave + lane] * w1);
+#pragma unroll
+      for (int d = 0; d < SH::DB; ++d)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          const float4_t y = x[n * kGive + (d * 4 + c) * kWave + lane];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) o[n][d][4 * c + j] = fmaf(o[n][d][4 * c + j], w0, y[j] * w1);
+        }
+    }
+  }
+
+  // f(column, four values of block n's row from that column on), for the columns below `width`.
+  template <typename F>
+  __device__ __forceinline__ void columns(int n, int width, int lane, F&& f) const {
+#pragma unroll
+    for (int d = 0; d < SH::DB; ++d)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int col = 32 * d + 8 * c + 4 * (lane / 32);
+        if (col < width) f(col, float4_t{o[n][d][4 * c], o[n][d][4 * c + 1], o[n][d][4 * c + 2], o[n][d][4 * c + 3]});
+      }
+  }
+};
+
+// The key tiles of one key head, by WAVES waves into LDS.
+template <typename T, typename SH, int WAVES>
+struct SweepTiles {
+  using Copy = KeyCopy<T, SH::W, SH::BN, WAVES>;
+  Copy k, v;
+  const T *kp, *vp;
+  int64_t ks, vs;
+  int D, Dv;
+  // k0, v0: the first key; rows `ks_`, `vs_` elements apart.
+  __device__ __forceinline__ void init(const T* k0, const T* v0, int64_t ks_, int64_t vs_, int d, int dv, int wave, int lane) {
+    kp = k0;
+    vp = v0;
+    ks = ks_;
+    vs = vs_;
+    D = d;
+    Dv = dv;
+    k.init(ks, D, wave, lane);
+    v.init(vs, Dv, wave, lane);
+  }
+  // Keys kv0 .. kv0 + BN - 1; those at or past `end` land as zeros, whatever is there.
+  __device__ __forceinline__ void issue(int kv0, int end, uint32_t tile, int wave) const {
+    k.issue(kp + kv0 * ks, ks, end - kv0, D, tile, wave);
+    v.issue(vp + kv0 * vs, vs, end - kv0, Dv, tile + SH::kTensor, wave);
+  }
+};
+
+// f(T{}, integral_constant<HD>) for the smallest instance that holds D and Dv.
+template <typename F>
+int grouped_dispatch(int D, int Dv, int dtype, F&& f) {
+  const int need = D > Dv ? D : Dv;
+  auto by_dim = [&](auto t) {
+    if (need <= 32) return f(t, std::integral_constant<int, 32>{});
+    if (need <= 64) return f(t, std::integral_constant<int, 64>{});
+    if (need <= 96) return f(t, std::integral_constant<int, 96>{});
+    return f(t, std::integral_constant<int, 128>{});
+  };
+  if (dtype == TJ_F32) return by_dim(float{});
+  if (dtype == TJ_F16) return by_dim(half_t{});
+  return by_dim(bf16_t{});
+}
+
+// How a call on drafted tokens runs: workgroups of `blocks` blocks of 32 rows, and the parts of the keys.
+struct TreePlan {
+  int blocks;
+  FewPlan parts;
+  bool whole() const { return parts.each == 1; }
+};
+TreePlan tree_plan(const TreeArgs& a, int dtype);
+int tree_fwd(const TreeArgs& a, const TreePlan& p, int dtype, hipStream_t stream);
+
+int packed_fwd(const PackedArgs& a, int dtype, hipStream_t stream);
+int packed_bwd(const PackedArgs& a, int dtype, hipStream_t stream);
+
+}  // namespace tj

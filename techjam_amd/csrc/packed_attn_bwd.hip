@@ -1,0 +1,517 @@
+// Attention of packed sequences with grouped heads, backward (the mathematics, the
+// row numbering and the regions are in grouped_attn.h). With the saved row sums,
+// P = 2^(scale log2 e S - lse),
+//
+//   delta = rowsum(dO o O),  dP = dO V^T,  dS = P (dP - delta),
+//   dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T dO,
+//
+// the last two summed over the group's rows. delta comes from the output as it was
+// returned, rounded to the inputs' type. 16-bit inputs have P and dS rounded to
+// their type for these products, one rounding more than the result's own (fp32
+// MFMAs would take 16 times as long); fp32 inputs have none.
+//
+// The dQ kernel goes over the keys of its rows and leaves each row's lse and delta
+// as the dK, dV kernel wants them; that one goes over the rows of its keys. So
+// nothing is added up across workgroups, and the result does not depend on their order.
+#include "grouped_attn.h"
+
+namespace tj {
+namespace {
+
+constexpr int kThreads = 256;
+constexpr int kPeakTokens = 64;
+
+// Products with fp16 operands: powers of two that bring the largest possible |dS|,
+// 2 |dO_i| |V_j|, near 2^15, so that small gradients and small probabilities keep
+// fp16's bits. dQ is a sum over keys, so there every row has its own, by its dO
+// (of) and the largest V row of its sequence and key head: a row's bits do not depend on how large the
+// gradients of others are. dK sums over rows and has one for all of a (sequence,
+// key head), by the largest dO row: dS of a row r times smaller keeps 11 bits down
+// to P of about 2^-26 r, and what lies below is off by at most 2^-37 of the largest
+// possible |dS|. P itself is lifted by 2^14. 1 for the other types.
+template <typename T>
+struct DsLift {
+  static constexpr bool kOn = std::is_same<T, half_t>::value;
+  static constexpr float kP = kOn ? 16384.f : 1.f, kLogP = kOn ? 14.f : 0.f;
+  float o = 1.f, v = 1.f;  // the largest norms of dO and V rows
+  __device__ __forceinline__ DsLift(const PackedArgs& a, const Region& g, int hk, int lane) {
+    if constexpr (kOn) {
+      const float* pk = a.peak + ((int64_t)Region::slot(g.start, g.index, 1, kPeakTokens) * a.Hk + hk) * 2;
+      o = v = 0.f;
+      for (int s = lane; s * kPeakTokens < g.len; s += kWave) {
+        o = fmaxf(o, pk[(int64_t)s * a.Hk * 2]);
+        v = fmaxf(v, pk[(int64_t)s * a.Hk * 2 + 1]);
+      }
+#pragma unroll
+      for (int m = 32; m > 0; m >>= 1) {
+        o = fmaxf(o, __shfl_xor(o, m));
+        v = fmaxf(v, __shfl_xor(v, m));
+      }
+    }
+  }
+  // For rows whose dO has at most this norm.
+  __device__ __forceinline__ float of(float norm) const {
+    if constexpr (!kOn) return 1.f;
+    // Exponents rather than products: the norms' product may leave fp32.
+    int ex, ey;
+    frexpf(norm, &ex);
+    frexpf(v, &ey);
+    if (!(norm > 0.f) || !(norm < 3e38f) || !(v > 0.f)) return 1.f;  // a row that is not finite is lost anyway
+    return ldexpf(1.f, min(max(14 - ex - ey, -100), 100));
+  }
+  // Of all rows: the same in every lane, so a scalar register holds it.
+  __device__ __forceinline__ float all() const {
+    return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(of(o))));
+  }
+};
+
+// The largest norms of 64 tokens' dO rows (all heads of the group) and V rows, those that are finite: others
+// spoil their own row only. A group of `lpr` lanes a row, 16-byte chunks.
+__global__ __launch_bounds__(kThreads) void packed_peak_kernel(PackedArgs a, int lpr) {
+  __shared__ float red[2][kThreads / kWave];
+  const int tid = threadIdx.x, hk = blockIdx.x % a.Hk, at = blockIdx.x / a.Hk;
+  Region g;
+  if (!g.find(a, at, 1, kPeakTokens, tid % kWave)) return;
+  const int lane = tid % lpr, per_block = kThreads / lpr, first = g.tile * kPeakTokens;
+  const int tokens = min(kPeakTokens, g.len - first);
+  const bool on = lane * 8 < a.Dv;
+  auto norm2 = [&](const half_t* p) {
+    float n = 0.f;
+    if (on) {
+      const half8_t x = *reinterpret_cast<const half8_t*>(p + lane * 8);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) n = fmaf((float)x[e], (float)x[e], n);
+    }
+    for (int s = lpr / 2; s > 0; s >>= 1) n += __shfl_xor(n, s);
+    return n < 3e38f ? n : 0.f;
+  };
+  float peak[2] = {0.f, 0.f};
+  for (int r = tid / lpr; r < tokens * a.G; r += per_block)
+    peak[0] = fmaxf(peak[0], norm2(reinterpret_cast<const half_t*>(a.dout) +
+                                   a.vdo.row(g.start + first + r / a.G, hk * a.G + r % a.G)));
+  for (int j = tid / lpr; j < tokens; j += per_block)
+    peak[1] = fmaxf(peak[1], norm2(reinterpret_cast<const half_t*>(a.v) + a.vv.row(g.start + first + j, hk)));
+#pragma unroll
+  for (int c = 0; c < 2; ++c) {
+    for (int s = kWave / 2; s > 0; s >>= 1) peak[c] = fmaxf(peak[c], __shfl_xor(peak[c], s));
+    if (tid % kWave == 0) red[c][tid / kWave] = peak[c];
+  }
+  __syncthreads();
+  if (tid < 2) {
+    float x = red[tid][0];
+    for (int w = 1; w < kThreads / kWave; ++w) x = fmaxf(x, red[tid][w]);
+    a.peak[((int64_t)at * a.Hk + hk) * 2 + tid] = sqrtf(x);
+  }
+}
+
+// The numbers of 32 tokens of a head: 32 of log2(lift of P) - lse, 32 of -delta, lifted.
+__device__ __forceinline__ float* stat_at(const PackedArgs& a, const Region& g, int head, int i) {
+  return a.stat + (((int64_t)Region::slot(g.start, g.index, 1, 32) + i / 32) * a.H + head) * 64 + i % 32;
+}
+
+// A workgroup = RB waves of NB blocks of 32 rows times KG groups, keys through LDS in
+// tiles of 32 dealt to the groups in turn, whose sums meet in LDS at the end. Scores
+// transposed as in the forward kernel: a row's sums are its lane's own numbers, and
+// dS turns into the B operand of dQ^T = K^T dS^T.
+template <typename T, int HD, int BLOCKS, int NBT>
+struct QShape {
+  static constexpr int NB = NBT, RB = BLOCKS, KG = 4 / RB, ROWS = 32 * RB * NB;
+  using SH = SweepShape<T, HD, 32>;
+};
+template <typename T, int HD>
+constexpr bool groups_fit(int groups) { return groups * SweepShape<T, HD, 32>::W * (int)sizeof(T) <= 1024; }
+
+template <typename T, int HD, int BLOCKS, int NB>
+__global__ __launch_bounds__(kThreads, (HD * (int)sizeof(T) <= 128 ? 2 : 1)) void packed_bwd_q_kernel(PackedArgs a) {
+  using QS = QShape<T, HD, BLOCKS, NB>;
+  using SH = typename QS::SH;
+  using Rows = typename SH::Rows;
+  constexpr int KS = SH::KS, DB = SH::DB, BN = 32, RB = QS::RB, KG = QS::KG, ROWS = QS::ROWS, kDepth = SH::kDepth;
+  constexpr int kSums = KG > 1 ? KG / 2 * RB * NB * DB * 16 * kWave * 4 : 0;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[KG * 2 * SH::kBytes > kSums ? KG * 2 * SH::kBytes : kSums];
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave, hl = lane / 32,
+            ln = lane % 32;
+  const int kg = w / RB, rb = w % RB, hk = blockIdx.x % a.Hk;
+  Region g;
+  if (!g.find(a, a.n_slots - 1 - (int)(blockIdx.x / a.Hk), a.G, ROWS, lane)) return;
+  const int L = g.len, R = g.rows * a.G, r0 = g.tile * ROWS, rw0 = r0 + 32 * NB * rb;
+  auto span = [&](int row, int last) {
+    return row >= R || row / a.G >= L ? 0 : (a.causal ? min(L, min(last, R - 1) / a.G + 1) : L);
+  };
+  const int kv_end = span(r0, r0 + ROWS - 1), own_end = span(rw0, rw0 + 32 * NB - 1);
+  const uint32_t tiles = lds_offset(smem) + kg * 2 * SH::kBytes;
+  const uint32_t krow = Rows::lane_row(lane), kcol = Rows::lane_col(lane), vrow = krow + SH::kTensor;
+  SweepTiles<T, SH, RB> keys;
+  keys.init(reinterpret_cast<const T*>(a.k) + a.vk.row(g.start, hk), reinterpret_cast<const T*>(a.v) + a.vv.row(g.start, hk),
+            a.vk.st, a.vv.st, a.D, a.Dv, rb, lane);
+  int kv0 = BN * kg;
+  if (kv0 < kv_end) keys.issue(kv0, L, tiles, rb);
+
+  const DsLift<T> lifts(a, g, hk, lane);
+  const float c2 = a.scale * kLog2e;
+  SweepRow row[NB];
+  int free[NB];
+  frag_t<T> qf[NB][KS], of[NB][KS];
+  float lse[NB], del[NB], lift[NB];
+  float16_t dq[NB][DB];
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    const int first = rw0 + 32 * n, r = first + ln;
+    row[n] = SweepRow{r, r / a.G, r % a.G, 0, r < R && r / a.G < L};
+    row[n].limit = a.causal ? row[n].i : L - 1;
+    free[n] = a.causal ? first / a.G : L - 1;
+    const int64_t token = g.start + row[n].i;
+    const int head = hk * a.G + row[n].g;
+    const T* qp = reinterpret_cast<const T*>(a.q) + a.vq.row(token, head);
+    const T* op = reinterpret_cast<const T*>(a.dout) + a.vdo.row(token, head);
+    const T* yp = reinterpret_cast<const T*>(a.out) + a.vo.row(token, head);
+    float sum = 0.f, norm = 0.f;
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      qf[n][s] = load_frag<T>(row[n].live ? qp : nullptr, 16 * s + 8 * hl, a.D);
+      of[n][s] = load_frag<T>(row[n].live ? op : nullptr, 16 * s + 8 * hl, a.Dv);
+      const frag_t<T> y = load_frag<T>(row[n].live ? yp : nullptr, 16 * s + 8 * hl, a.Dv);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        sum = fmaf((float)of[n][s][j], (float)y[j], sum);
+        if constexpr (DsLift<T>::kOn) norm = fmaf((float)of[n][s][j], (float)of[n][s][j], norm);
+      }
+    }
+    del[n] = pair_sum(sum);
+    lse[n] = row[n].live ? a.lse[token * a.H + head] : __builtin_inff();
+    // The row's own lift: its lane (and the one of the other half) has all of its dO.
+    lift[n] = DsLift<T>::kOn ? lifts.of(sqrtf(pair_sum(norm))) : 1.f;
+#pragma unroll
+    for (int d = 0; d < DB; ++d) dq[n][d] = zero16();
+  }
+  const float common = lifts.all() / DsLift<T>::kP;
+
+  // The workgroup goes round together, the last round maybe without a tile for every group.
+  for (int first = 0, cur = 0; first < kv_end; first += KG * BN, kv0 += KG * BN, cur ^= 1) {
+    wait_copies();
+    lds_barrier();
+    if (kv0 + KG * BN < kv_end) keys.issue(kv0 + KG * BN, L, tiles + (cur ^ 1) * SH::kBytes, rb);
+    if (kv0 >= own_end) continue;
+    const uint32_t tile = tiles + cur * SH::kBytes;
+    float16_t p[NB], dp[NB];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) p[n] = dp[n] = zero16();
+    read_ahead<KS, kDepth>([&](int s) { return Rows::row_frag(tile + krow, s, 0); },
+                           [&](int s, frag_t<T> f) {
+#pragma unroll
+                             for (int n = 0; n < NB; ++n) p[n] = Elem<T>::mma(f, qf[n][s], p[n]);
+                           });
+    read_ahead<KS, kDepth>([&](int s) { return Rows::row_frag(tile + vrow, s, 0); },
+                           [&](int s, frag_t<T> f) {
+#pragma unroll
+                             for (int n = 0; n < NB; ++n) dp[n] = Elem<T>::mma(f, of[n][s], dp[n]);
+                           });
+    frag_t<T> fs[NB][2];
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      const float d0 = -del[n] * lift[n];
+#pragma unroll
+      for (int e = 0; e < 16; ++e) p[n][e] = fast_exp2(fmaf(p[n][e], c2, -lse[n])) * fmaf(dp[n][e], lift[n], d0);
+      // Selected, not multiplied: what a masked key holds does not matter.
+      if (kv0 + BN - 1 > free[n]) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (kv0 + acc_row(e, hl) > row[n].limit) p[n][e] = 0.f;
+      }
+#pragma unroll
+      for (int s = 0; s < 2; ++s) fs[n][s] = acc_frag<T>(p[n], s);
+    }
+    if constexpr (kDepth > 0) __builtin_amdgcn_sched_barrier(0);
+    read_ahead<2 * DB, kDepth>([&](int j) { return Rows::col_frag(tile + kcol, j % DB, 16 * (j / DB) * Rows::kRowBytes); },
+                               [&](int j, frag_t<T> f) {
+#pragma unroll
+                                 for (int n = 0; n < NB; ++n) dq[n][j % DB] = Elem<T>::mma(f, fs[n][j / DB], dq[n][j % DB]);
+                               });
+  }
+
+  // The groups' sums, the upper half's added to the lower half's.
+#pragma unroll
+  for (int half = KG / 2; half > 0; half /= 2) {
+    float4_t* x = reinterpret_cast<float4_t*>(smem) + ((kg % half) * RB + rb) * NB * DB * 4 * kWave;
+    __syncthreads();
+    if (kg >= half && kg < 2 * half) {
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            x[((n * DB + d) * 4 + e) * kWave + lane] =
+                float4_t{dq[n][d][4 * e], dq[n][d][4 * e + 1], dq[n][d][4 * e + 2], dq[n][d][4 * e + 3]};
+    }
+    __syncthreads();
+    if (kg < half) {
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float4_t z = x[((n * DB + d) * 4 + e) * kWave + lane];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) dq[n][d][4 * e + j] += z[j];
+          }
+    }
+  }
+  if (kg != 0) return;
+
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    if (row[n].r >= R) continue;
+    const int head = hk * a.G + row[n].g;
+    if (row[n].live && hl == 0) {
+      float* st = stat_at(a, g, head, row[n].i);
+      st[0] = DsLift<T>::kLogP - lse[n];
+      st[32] = -del[n] * common;
+    }
+    const float out = a.scale / lift[n];
+    T* p = reinterpret_cast<T*>(a.dq) + a.vdq.row(g.start + row[n].i, head);
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int col = 32 * d + 8 * e + 4 * hl;
+        float y[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = row[n].live ? dq[n][d][4 * e + j] * out : 0.f;
+        if (col < a.D) store4t<T>(p + col, y[0], y[1], y[2], y[3]);
+      }
+  }
+}
+
+// A workgroup = KB blocks of 32 keys of one (sequence, key head) times RG groups of
+// token tiles, a wave each: the tiles of 32 tokens that see the keys, of one query
+// head of the group after the other, are dealt to the groups in turn, and the
+// groups' sums meet in LDS at the end. Scores are formed with tokens in the
+// registers and keys over the lanes, so that P and dS turn into the A operands of dV
+// and dK where they stand; Q and dO come back as B operands through the transposing
+// LDS read.
+template <typename T, int HD, bool HALF>
+struct KvShape {
+  using SH = SweepShape<T, HD, 32>;
+  static constexpr int kWhole = (sizeof(T) == 2 && HD <= 64) || HD == 32 ? 8 : 4, WAVES = HALF ? kWhole / 2 : kWhole;
+  static constexpr int kFit = 1024 / (SH::W * (int)sizeof(T));
+  static constexpr int RG = kFit < kWhole / 2 ? kFit : kWhole / 2;
+  static constexpr int KB = WAVES / RG;
+  static constexpr int kDepth = HD == 32 ? 0 : sizeof(T) == 2 ? 2 : 1;
+};
+
+template <typename T, int HD, bool HALF>
+__global__ __launch_bounds__((64 * KvShape<T, HD, HALF>::WAVES), (KvShape<T, HD, HALF>::kWhole / 4)) void
+packed_bwd_kv_kernel(PackedArgs a) {
+  using KV = KvShape<T, HD, HALF>;
+  using SH = typename KV::SH;
+  using Rows = typename SH::Rows;
+  constexpr int KS = SH::KS, DB = SH::DB, BM = 32, KB = KV::KB, RG = KV::RG, kDepth = KV::kDepth;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[RG * 2 * SH::kBytes];  // Q's tile, then dO's
+  __shared__ __attribute__((aligned(1024))) float stat[RG][2][64];                    // of a tile's tokens
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave, hl = lane / 32,
+            ln = lane % 32;
+  const int kb = w % KB, rg = w / KB, hk = blockIdx.x % a.Hk;
+  Region g;
+  if (!g.find(a, blockIdx.x / a.Hk, 1, 32 * KB, lane)) return;
+  const int L = g.len, k0 = g.tile * 32 * KB, kw0 = k0 + 32 * kb, key = kw0 + ln;
+  const bool live = key < L;
+
+  // The group's KB waves bring its tiles.
+  SweepTiles<T, SH, KB> rows;
+  rows.init(nullptr, nullptr, a.vq.st, a.vdo.st, a.D, a.Dv, kb, lane);
+  const T* qp = reinterpret_cast<const T*>(a.q) + a.vq.row(g.start, hk * a.G);
+  const T* op = reinterpret_cast<const T*>(a.dout) + a.vdo.row(g.start, hk * a.G);
+  const uint32_t group = lds_offset(smem) + rg * 2 * SH::kBytes, stat0 = lds_offset(stat[rg]);
+  const uint32_t qrow = Rows::lane_row(lane), qcol = Rows::lane_col(lane), orow = qrow + SH::kTensor, ocol = qcol + SH::kTensor;
+  // Tile n: head n / tiles of the group, tokens i_begin + 32 (n % tiles) on.
+  const int i_begin = a.causal ? k0 : 0;
+  const int tiles = k0 < L ? (L - i_begin + BM - 1) / BM : 0, n_end = tiles * a.G;
+  // `n` tiles further on: the head and the token (no division in the loop).
+  auto advance = [&](int& h, int& i0, int n) {
+    i0 += BM * n;
+    while (i0 >= i_begin + BM * tiles) {
+      i0 -= BM * tiles;
+      ++h;
+    }
+  };
+  auto issue = [&](int h, int i0, int buf) {
+    rows.kp = qp + h * a.vq.sh;
+    rows.vp = op + h * a.vdo.sh;
+    rows.issue(i0, L, group + buf * SH::kBytes, kb);
+    // The tokens' numbers by the same way: a load into registers would have to be waited for,
+    // and every copy issued before with it.
+    if (kb == 0) copy_4(make_rsrc(stat_at(a, g, hk * a.G + h, i0), 256), stat0 + buf * 256, 4 * lane);
+  };
+
+  frag_t<T> kf[KS], vf[KS];
+  {
+    const T* kp = reinterpret_cast<const T*>(a.k) + a.vk.row(g.start + key, hk);
+    const T* vp = reinterpret_cast<const T*>(a.v) + a.vv.row(g.start + key, hk);
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+      kf[s] = load_frag<T>(live ? kp : nullptr, 16 * s + 8 * hl, a.D);
+      vf[s] = load_frag<T>(live ? vp : nullptr, 16 * s + 8 * hl, a.Dv);
+    }
+  }
+  float16_t dv[DB], dk[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d) dv[d] = dk[d] = zero16();
+
+  const float dl = DsLift<T>(a, g, hk, lane).all(), lift = dl / DsLift<T>::kP, c2 = a.scale * kLog2e;
+  int h = 0, i0 = i_begin;  // this round's tile
+  if (rg < n_end) {
+    advance(h, i0, rg);
+    issue(h, i0, 0);
+  }
+  // The workgroup goes round together, the last round maybe without a tile for every group.
+  const int rounds = (n_end + RG - 1) / RG;
+  for (int round = 0, n = rg, cur = 0; round < rounds; ++round, n += RG, cur ^= 1) {
+    // The tile is there, and the group's other one has been read by its waves.
+    wait_copies();
+    lds_barrier();
+    const uint32_t tile = group + cur * SH::kBytes, srow = stat0 + cur * 256 + 16 * hl;
+    // Else there is no tile, or every token stands before the wave's keys.
+    const bool busy = n < n_end && (!a.causal || i0 + BM > kw0);
+    const int at = i0;
+    if (n + RG < n_end) {
+      advance(h, i0, RG);
+      issue(h, i0, cur ^ 1);
+    }
+    if (!busy) continue;
+    float16_t p = zero16(), dp = zero16();
+    read_ahead<KS, kDepth>([&](int s) { return Rows::row_frag(tile + qrow, s, 0); },
+                           [&](int s, frag_t<T> f) { p = Elem<T>::mma(f, kf[s], p); });
+    read_ahead<KS, kDepth>([&](int s) { return Rows::row_frag(tile + orow, s, 0); },
+                           [&](int s, frag_t<T> f) { dp = Elem<T>::mma(f, vf[s], dp); });
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const float4_t ls = lds_at<float4_t>(srow + q * 32), d0 = lds_at<float4_t>(srow + 128 + q * 32);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float e = fast_exp2(fmaf(p[4 * q + j], c2, ls[j]));
+        p[4 * q + j] = e;
+        dp[4 * q + j] = e * fmaf(dp[4 * q + j], lift, d0[j]);
+      }
+    }
+    // Selected, not multiplied: tokens past the length have no numbers at all.
+    if ((a.causal && at < kw0 + 31) || at + BM > L) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int i = at + acc_row(r, hl);
+        if ((a.causal && i < key) || i >= L) p[r] = dp[r] = 0.f;
+      }
+    }
+    frag_t<T> fp[2], fs[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      fp[s] = acc_frag<T>(p, s);
+      fs[s] = acc_frag<T>(dp, s);
+    }
+    if constexpr (kDepth > 0) __builtin_amdgcn_sched_barrier(0);
+    read_ahead<2 * DB, kDepth>([&](int j) { return Rows::col_frag(tile + ocol, j % DB, 16 * (j / DB) * Rows::kRowBytes); },
+                               [&](int j, frag_t<T> f) { dv[j % DB] = Elem<T>::mma(fp[j / DB], f, dv[j % DB]); });
+    read_ahead<2 * DB, kDepth>([&](int j) { return Rows::col_frag(tile + qcol, j % DB, 16 * (j / DB) * Rows::kRowBytes); },
+                               [&](int j, frag_t<T> f) { dk[j % DB] = Elem<T>::mma(fs[j / DB], f, dk[j % DB]); });
+  }
+
+  // The groups' sums, the upper half's added to the lower half's.
+  if constexpr (RG > 1) {
+    static_assert(sizeof(smem) >= (RG / 2) * KB * 2 * DB * 16 * kWave * sizeof(float), "room for the groups' sums");
+    float4_t* x = reinterpret_cast<float4_t*>(smem);
+#pragma unroll
+    for (int half = RG / 2; half > 0; half /= 2) {
+      float4_t* y = x + ((rg % half) * KB + kb) * 2 * DB * 4 * kWave + lane;
+      __syncthreads();
+      if (rg >= half && rg < 2 * half) {
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            y[(2 * d * 4 + q) * kWave] = float4_t{dv[d][4 * q], dv[d][4 * q + 1], dv[d][4 * q + 2], dv[d][4 * q + 3]};
+            y[((2 * d + 1) * 4 + q) * kWave] = float4_t{dk[d][4 * q], dk[d][4 * q + 1], dk[d][4 * q + 2], dk[d][4 * q + 3]};
+          }
+      }
+      __syncthreads();
+      if (rg < half) {
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const float4_t u = y[(2 * d * 4 + q) * kWave], z = y[((2 * d + 1) * 4 + q) * kWave];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              dv[d][4 * q + j] += u[j];
+              dk[d][4 * q + j] += z[j];
+            }
+          }
+      }
+    }
+    if (rg != 0) return;
+  }
+
+  // Keys at or past the length have no gradient: zeros, whatever their scores were.
+  const float dv_scale = 1.f / DsLift<T>::kP, dk_scale = a.scale / dl;
+#pragma unroll
+  for (int r = 0; r < 16; ++r) {
+    const int j = kw0 + acc_row(r, hl);
+    if (j >= g.rows) continue;
+    const bool in = j < L;
+    T* pv = reinterpret_cast<T*>(a.dv) + a.vdv.row(g.start + j, hk);
+    T* pk = reinterpret_cast<T*>(a.dk) + a.vdk.row(g.start + j, hk);
+#pragma unroll
+    for (int d = 0; d < DB; ++d) {
+      if (32 * d + ln < a.Dv) pv[32 * d + ln] = (T)(in ? dv[d][r] * dv_scale : 0.f);
+      if (32 * d + ln < a.D) pk[32 * d + ln] = (T)(in ? dk[d][r] * dk_scale : 0.f);
+    }
+  }
+}
+
+template <typename T, int HD, int BLOCKS, int NB>
+int launch_q(PackedArgs a, hipStream_t stream) {
+  const int64_t slots = region_slots(a.T, a.N, a.G, QShape<T, HD, BLOCKS, NB>::ROWS);
+  a.n_slots = (int)slots;
+  hipLaunchKernelGGL((packed_bwd_q_kernel<T, HD, BLOCKS, NB>), dim3(uint32_t(slots * a.Hk)), dim3(kThreads), 0, stream, a);
+  return tjh::launch_status();
+}
+
+template <typename T, int HD, bool HALF>
+int launch_kv(PackedArgs a, hipStream_t stream) {
+  using KV = KvShape<T, HD, HALF>;
+  const int64_t slots = region_slots(a.T, a.N, 1, 32 * KV::KB);
+  a.n_slots = (int)slots;
+  hipLaunchKernelGGL((packed_bwd_kv_kernel<T, HD, HALF>), dim3(uint32_t(slots * a.Hk)), dim3(64 * KV::WAVES), 0, stream, a);
+  return tjh::launch_status();
+}
+
+}  // namespace
+
+int packed_bwd(const PackedArgs& a, int dtype, hipStream_t stream) {
+  if (dtype == TJ_F16) {
+    int lpr = 1;
+    while (lpr * 8 < a.Dv) lpr *= 2;
+    const int64_t slots = region_slots(a.T, a.N, 1, kPeakTokens);
+    hipLaunchKernelGGL(packed_peak_kernel, dim3(uint32_t(slots * a.Hk)), dim3(kThreads), 0, stream, a, lpr);
+    if (const int rc = tjh::launch_status()) return rc;
+  }
+  return grouped_dispatch(a.D, a.Dv, dtype, [&](auto t, auto hd) {
+    using T = decltype(t);
+    constexpr int HD = decltype(hd)::value;
+    const int64_t rows = (int64_t)a.T * a.G;  // of one key head
+    int rc;
+    if constexpr (groups_fit<T, HD>(4)) {
+      if ((rows + 63) / 64 * a.Hk <= kCus / 2) rc = launch_q<T, HD, 1, 1>(a, stream);
+      else if ((rows + 127) / 128 * a.Hk <= 2 * kCus) rc = launch_q<T, HD, 2, 1>(a, stream);
+      else rc = launch_q<T, HD, 4, 1>(a, stream);
+    } else {
+      if ((rows + 127) / 128 * a.Hk <= 2 * kCus) rc = launch_q<T, HD, 2, 1>(a, stream);
+      else rc = launch_q<T, HD, 4, 1>(a, stream);
+    }
+    if (rc != TJ_OK) return rc;
+    if ((int64_t)(a.T + 63) / 64 * a.Hk <= kCus / 2) return launch_kv<T, HD, true>(a, stream);
+    return launch_kv<T, HD, false>(a, stream);
+  });
+}
+
+}  // namespace tj

@@ -1,0 +1,262 @@
+// Attention of drafted tokens against a cache, with grouped heads (the mathematics
+// and the row numbering are in grouped_attn.h). The Sq drafted tokens of a sequence
+// stand in its cache behind what it has settled, at positions len - Sq on; token t sees
+// all settled keys, and of the drafted ones its own and those on its line of parents.
+//
+// A workgroup = RB waves of 32 rows of one (sequence, key head) and one part of the
+// keys, so that up to 256 rows read a key from memory once. Parts are joined by
+// tree_join_kernel.
+#include "grouped_attn.h"
+
+namespace tj {
+namespace {
+
+constexpr int kJoinThreads = 256;
+
+// The drafted tokens that each one sees, a bit each: the line of parents is followed in
+// steps of twice the length, token t in lane t, six times for up to 64 of them. A token
+// is not there when its parent does not stand before it, when its position is negative,
+// or when something on its line is not there.
+struct Lineage {
+  uint64_t seen;
+  bool gone;
+  __device__ __forceinline__ Lineage(const TreeArgs& a, int b, int ctx, int lane) {
+    const int p = lane < a.Sq ? a.parents[(int64_t)b * a.Sq + lane] : lane;
+    gone = p < -1 || p >= lane || ctx + lane < 0;
+    seen = uint64_t(1) << lane;
+    int up = gone ? -1 : p;
+#pragma unroll
+    for (int s = 0; s < 6; ++s) {
+      const int from = max(up, 0);
+      const uint32_t lo = __shfl((uint32_t)seen, from), hi = __shfl((uint32_t)(seen >> 32), from);
+      const int next = __shfl(up, from), lost = __shfl((int)gone, from);
+      if (up >= 0) {
+        seen |= (uint64_t)hi << 32 | lo;
+        gone |= lost != 0;
+        up = next;
+      }
+    }
+  }
+};
+
+template <typename T, int HD, int BLOCKS>
+struct TreeShape {
+  static constexpr int RB = BLOCKS, ROWS = 32 * RB, THREADS = kWave * RB;
+  using SH = SweepShape<T, HD, 32>;
+  // Waves of a SIMD by the registers, and workgroups that a CU holds.
+  static constexpr int kWaves = HD == 32 ? 3 : (sizeof(T) == 2 || HD == 64 ? 2 : 1);
+  static constexpr int kByLds = 160 * 1024 / (2 * SH::kBytes), kByRegs = kWaves * 4 / RB > 1 ? kWaves * 4 / RB : 1;
+  static constexpr int kPerCu = kByLds < kByRegs ? kByLds : kByRegs;
+};
+
+template <typename T, int HD, int BLOCKS>
+__global__ __launch_bounds__((TreeShape<T, HD, BLOCKS>::THREADS), (BLOCKS == 8 ? 2 : TreeShape<T, HD, BLOCKS>::kWaves)) void tree_kernel(TreeArgs a) {
+  using TS = TreeShape<T, HD, BLOCKS>;
+  using SH = typename TS::SH;
+  constexpr int RB = TS::RB, BN = SH::BN;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * SH::kBytes];
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
+  const int mt = blockIdx.x % a.n_mtiles, hk = blockIdx.x / a.n_mtiles % a.Hk, part = blockIdx.x / a.n_mtiles / a.Hk;
+  const bool whole = a.part_o == nullptr;
+  FewParts f;
+  if (whole) f.b = part;
+  else if (!f.find(a, part, lane)) return;
+  const int b = __builtin_amdgcn_readfirstlane(f.b);
+  const int L = __builtin_amdgcn_readfirstlane(min(a.Sk, max(0, a.len[b]))), ctx = L - a.Sq;
+  const int row0 = mt * TS::ROWS, rw0 = row0 + 32 * w;
+  // Keys that rows row .. last (clipped to R) need.
+  auto span = [&](int row, int last) { return row >= a.R ? 0 : max(0, ctx + min(last, a.R - 1) / a.G + 1); };
+  const int n_keys = whole ? L : __builtin_amdgcn_readfirstlane(f.keys);
+  const int kv_begin = whole ? 0 : __builtin_amdgcn_readfirstlane((part - f.first) * f.keys);
+  const int kv_end = min(span(row0, row0 + TS::ROWS - 1), kv_begin + n_keys), own_end = min(kv_end, span(rw0, rw0 + 31));
+  if (kv_begin >= kv_end && !whole) return;  // not read either
+  const uint32_t tiles = lds_offset(smem);
+  SweepTiles<T, SH, RB> keys;
+  keys.init(reinterpret_cast<const T*>(a.k) + a.vk.row(b, hk, 0), reinterpret_cast<const T*>(a.v) + a.vv.row(b, hk, 0),
+            a.vk.ss, a.vv.ss, a.D, a.Dv, w, lane);
+  if (kv_begin < kv_end) keys.issue(kv_begin, L, tiles, w);
+  const int r = rw0 + lane % 32;
+  SweepRow row{r, r / a.G, r % a.G, 0, false};
+  row.limit = ctx + row.i;
+  row.live = r < a.R && row.limit >= 0;
+  uint64_t seen = 0, gone = 0;
+  if (a.parents != nullptr) {
+    const Lineage line(a, b, ctx, lane);
+    const int t = min(row.i, kWave - 1);
+    seen = (uint64_t)__shfl((uint32_t)(line.seen >> 32), t) << 32 | (uint64_t)__shfl((uint32_t)line.seen, t);
+    gone = __ballot(line.gone && lane < a.Sq);
+    row.live = row.live && !(gone >> t & 1);
+  }
+  SweepState<T, HD, BN, 1, false> st;
+  st.init(a.scale, lane);
+  st.load_q(0, row.live ? reinterpret_cast<const T*>(a.q) + a.vq.row(b, hk * a.G + row.g, row.i) : nullptr, a.scale, a.D, lane);
+  for (int kv0 = kv_begin, cur = 0; kv0 < kv_end; kv0 += BN, cur ^= 1) {
+    // The tile is there, and the other one has been read.
+    wait_copies();
+    lds_barrier();
+    if (kv0 + BN < kv_end) keys.issue(kv0 + BN, L, tiles + (cur ^ 1) * SH::kBytes, w);
+    const uint32_t tile = tiles + cur * SH::kBytes;
+    if (gone != 0 && kv0 + BN > ctx) {
+      // What is not there may hold anything: its values are cleared, as 0 times NaN would spoil the others.
+      constexpr int kChunks = SH::Rows::kChunks;
+      for (int c = tid; c < BN * kChunks; c += TS::THREADS) {
+        const int t = kv0 + c / kChunks - ctx;
+        if (t >= 0 && t < kWave && (gone >> t & 1))
+          *(__attribute__((address_space(3))) float4_t*)(uintptr_t)(tile + SH::kTensor + c * 16) = float4_t{0.f, 0.f, 0.f, 0.f};
+      }
+      wait_lds();
+      lds_barrier();
+    }
+    if (kv0 >= own_end) continue;
+    st.step(tile, 0, [&](int, float16_t& s) {
+      const int hl = lane / 32;
+      if (kv0 + BN <= ctx) return;
+      if (a.parents == nullptr) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          if (kv0 + acc_row(e, hl) > row.limit) s[e] = -__builtin_inff();
+        return;
+      }
+      // The tile's keys that the row sees: settled ones, then its line.
+      const int t = kv0 - ctx;  // drafted token of the tile's first key
+      uint32_t word = t >= kWave ? 0 : (t >= 0 ? (uint32_t)(seen >> t) : (uint32_t)(seen << -t) | ((1u << -t) - 1));
+      word >>= 4 * hl;
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (!(word >> acc_row(e, 0) & 1)) s[e] = -__builtin_inff();
+    });
+  }
+  const float sum = pair_sum(st.l[0]);
+  if (r >= a.R) return;
+  if (whole) {
+    const float inv = 1.f / sum;
+    T* op = reinterpret_cast<T*>(a.o) + a.vo.row(b, hk * a.G + row.g, row.i);
+    st.columns(0, a.Dv, lane, [&](int col, float4_t y) {
+      if (!row.live) y = float4_t{0.f, 0.f, 0.f, 0.f};
+      else y *= inv;
+      store4t<T>(op + col, y[0], y[1], y[2], y[3]);
+    });
+    return;
+  }
+  const int64_t at = ((int64_t)part * a.Hk + hk) * a.R + r;
+  if (lane < 32) *reinterpret_cast<float4_t*>(a.part_ml + at * 4) = float4_t{st.m[0], sum, row.live ? 1.f : 0.f, 0.f};
+  if (row.live)
+    st.columns(0, a.Dv, lane, [&](int col, float4_t y) { *reinterpret_cast<float4_t*>(a.part_o + at * a.Dv + col) = y; });
+}
+
+// Joins the parts: O = sum_p 2^(max_p - M) o_p / sum_p 2^(max_p - M) sum_p. `lanes` threads take a row's
+// chunks of 4 columns, `sets` of them every so many-th part, the workgroup's 256 threads as many rows as
+// that leaves. A row's parts are those up to its last key.
+template <typename T>
+__global__ __launch_bounds__(kJoinThreads) void tree_join_kernel(TreeArgs a, int lanes, int sets) {
+  __shared__ float4_t part[kJoinThreads];
+  __shared__ float top[kJoinThreads], total[kJoinThreads];
+  const int tid = threadIdx.x, per_row = lanes * sets, rows = kJoinThreads / per_row;
+  const int chunk = tid % lanes, set = tid / lanes % sets;
+  const int tiles = (a.R + rows - 1) / rows;  // of one (sequence, key head)
+  const int bh = blockIdx.x / tiles, b = bh / a.Hk, hk = bh % a.Hk;
+  const int r = blockIdx.x % tiles * rows + tid / per_row, i = r / a.G;
+  const int L = min(a.Sk, max(0, a.len[b])), limit = L - a.Sq + i;
+  FewParts f;
+  f.of(a, b, tid % kWave);
+  const int np = r < a.R && limit >= 0 ? limit / f.keys + 1 : 0;
+  const int64_t first = ((int64_t)f.first * a.Hk + hk) * a.R + r, step = (int64_t)a.Hk * a.R;
+  const bool on = chunk * 4 < a.Dv;
+  float m = -__builtin_inff(), l = 0.f, live = 0.f;
+  float4_t y = {0.f, 0.f, 0.f, 0.f};
+  for (int p = set; p < np; p += sets) {
+    const float4_t x = *reinterpret_cast<const float4_t*>(a.part_ml + (first + p * step) * 4);
+    live = x[2];
+    if (live == 0.f) break;
+    const float4_t o = on ? *reinterpret_cast<const float4_t*>(a.part_o + (first + p * step) * a.Dv + chunk * 4) : y;
+    const float to = fmaxf(m, x[0]);
+    // An unset maximum (-inf) goes with sums that are zero, or NaN and kept.
+    const float w0 = m == -__builtin_inff() ? 1.f : fast_exp2(m - to), w1 = x[0] == -__builtin_inff() ? 1.f : fast_exp2(x[0] - to);
+    m = to;
+    l = fmaf(l, w0, x[1] * w1);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = fmaf(y[j], w0, o[j] * w1);
+  }
+  part[tid] = y;
+  top[tid] = m;
+  total[tid] = l;
+  __syncthreads();
+  if (set != 0 || r >= a.R || !on) return;
+  float most = m;
+  for (int s = 1; s < sets; ++s) most = fmaxf(most, top[tid + s * lanes]);
+  const float w0 = m == -__builtin_inff() ? 1.f : fast_exp2(m - most);
+  l *= w0;
+  y *= w0;
+  for (int s = 1; s < sets; ++s) {
+    const float x = top[tid + s * lanes], w = x == -__builtin_inff() ? 1.f : fast_exp2(x - most);
+    const float4_t o = part[tid + s * lanes];
+    l = fmaf(total[tid + s * lanes], w, l);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = fmaf(o[j], w, y[j]);
+  }
+  const float inv = 1.f / l;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) y[j] = live != 0.f ? y[j] * inv : 0.f;
+  store4t<T>(reinterpret_cast<T*>(a.o) + a.vo.row(b, hk * a.G + r % a.G, i) + chunk * 4, y[0], y[1], y[2], y[3]);
+}
+
+template <typename T>
+int launch_join(const TreeArgs& a, hipStream_t stream) {
+  int lanes = 1, sets = 1;
+  while (lanes * 4 < a.Dv) lanes *= 2;
+  // As many sets as leave each a part or two.
+  const int parts = a.few_each != 0 ? a.few_each : (a.n_parts + a.B - 1) / a.B;
+  while (2 * sets < parts && lanes * sets < kJoinThreads) sets *= 2;
+  const int rows = kJoinThreads / (lanes * sets), tiles = (a.R + rows - 1) / rows;
+  hipLaunchKernelGGL((tree_join_kernel<T>), dim3(uint32_t((int64_t)a.B * a.Hk * tiles)), dim3(kJoinThreads), 0, stream, a, lanes, sets);
+  return tjh::launch_status();
+}
+
+template <typename T, int HD, int BLOCKS>
+int launch(const TreeArgs& a, hipStream_t stream) {
+  using TS = TreeShape<T, HD, BLOCKS>;
+  const int64_t parts = a.part_o == nullptr ? a.B : a.n_parts;
+  hipLaunchKernelGGL((tree_kernel<T, HD, BLOCKS>), dim3(uint32_t(parts * a.Hk * a.n_mtiles)), dim3(TS::THREADS), 0, stream, a);
+  const int rc = tjh::launch_status();
+  return rc != TJ_OK || a.part_o == nullptr ? rc : launch_join<T>(a, stream);
+}
+
+// f(integral_constant<int, blocks of 32 rows a workgroup>).
+template <typename F>
+auto by_blocks(int R, F&& f) {
+  if (R <= 32) return f(std::integral_constant<int, 1>{});
+  if (R <= 64) return f(std::integral_constant<int, 2>{});
+  if (R <= 128) return f(std::integral_constant<int, 4>{});
+  return f(std::integral_constant<int, 8>{});
+}
+
+}  // namespace
+
+TreePlan tree_plan(const TreeArgs& a, int dtype) {
+  TreePlan p{};
+  grouped_dispatch(a.D, a.Dv, dtype, [&](auto t, auto hd) {
+    by_blocks(a.R, [&](auto blocks) {
+      using TS = TreeShape<decltype(t), decltype(hd)::value, decltype(blocks)::value>;
+      p.blocks = TS::RB;
+      p.parts = few_plan(a.B, a.Hk, (a.R + TS::ROWS - 1) / TS::ROWS, a.Sk, kCus * TS::kPerCu);
+      return 0;
+    });
+    return 0;
+  });
+  return p;
+}
+
+int tree_fwd(const TreeArgs& args, const TreePlan& p, int dtype, hipStream_t stream) {
+  TreeArgs a = args;
+  a.n_mtiles = (a.R + 32 * p.blocks - 1) / (32 * p.blocks);
+  a.few_slots = (int)p.parts.slots;
+  a.few_each = (int)p.parts.each;
+  a.n_parts = (int)p.parts.total;
+  return grouped_dispatch(a.D, a.Dv, dtype, [&](auto t, auto hd) {
+    return by_blocks(a.R, [&](auto blocks) {
+      return launch<decltype(t), decltype(hd)::value, decltype(blocks)::value>(a, stream);
+    });
+  });
+}
+
+}  // namespace tj

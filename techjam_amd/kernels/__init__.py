@@ -2,7 +2,8 @@
 
 from .attention import scaled_dot_product_attention, score_guard
 from .differential import differential_attention, differential_attention_cached
+from .grouped import packed_attention, tree_attention
 from .layer_norm import LayerNorm, layer_norm
 
-__all__ = ["LayerNorm", "differential_attention", "differential_attention_cached", "layer_norm",
-           "scaled_dot_product_attention", "score_guard"]
+__all__ = ["LayerNorm", "differential_attention", "differential_attention_cached", "layer_norm", "packed_attention",
+           "scaled_dot_product_attention", "score_guard", "tree_attention"]
