@@ -462,26 +462,27 @@ int tj_diff_attn_bwd(const void* q, const void* k, const void* v, const float* m
  * elements, the innermost 1, the others multiples of 16 bytes; 64 rows of k and v (and
  * of q and dout below) within 2 GiB (TJ_ERR_UNSUPPORTED otherwise).
  *
- * lse: fp32 [T, H], what tj_packed_attn_bwd reads again, or NULL: log2 of the rows'
- * softmax sums (rows without a token are not written).
+ * lse and, with 16-bit types, o_rest: what tj_packed_attn_bwd reads again, or NULL:
+ * fp32 [T, H], log2 of the rows' softmax sums (rows without a token are not written), and what
+ * rounding took from o, in o's type, shape and strides (NULL for fp32).
  */
 int tj_packed_attn_fwd(const void* q, const void* k, const void* v, void* o, int dtype,
                        int64_t T, int64_t N, int64_t H, int64_t Hk, int64_t D, int64_t Dv,
                        const int64_t q_strides[3], const int64_t k_strides[3],
                        const int64_t v_strides[3], const int64_t o_strides[3],
                        float scale, int causal, const int32_t* offsets, const int32_t* lengths,
-                       float* lse, hipStream_t stream);
+                       float* lse, void* o_rest, hipStream_t stream);
 
 /*
  * The gradients of tj_packed_attn_fwd for the output gradient dout [T, H, Dv]: dq, dk, dv
- * (shaped and typed like q, k, v). o and lse come from the forward call. Rows without a token
+ * (shaped and typed like q, k, v). o, o_rest and lse come from the forward call. Rows without a token
  * get zeros and their dout is not read. The sums' order is fixed: the same call gives the
  * same bits. workspace: tj_packed_attn_bwd_workspace_bytes bytes, 16-byte aligned, contents
  * irrelevant, calls sharing one ordered on one stream.
  */
 size_t tj_packed_attn_bwd_workspace_bytes(int64_t T, int64_t N, int64_t H, int64_t Hk);
-int tj_packed_attn_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse,
-                       const void* dout, void* dq, void* dk, void* dv, int dtype,
+int tj_packed_attn_bwd(const void* q, const void* k, const void* v, const void* o,
+                       const void* o_rest, const float* lse, const void* dout, void* dq, void* dk, void* dv, int dtype,
                        int64_t T, int64_t N, int64_t H, int64_t Hk, int64_t D, int64_t Dv,
                        const int64_t q_strides[3], const int64_t k_strides[3], const int64_t v_strides[3],
                        const int64_t o_strides[3], const int64_t do_strides[3], const int64_t dq_strides[3],

@@ -31,6 +31,7 @@ struct PackedArgs {
   const int32_t* off;      // [N + 1]
   const int32_t* len;      // [N] valid tokens of each sequence's rows, or null: all
   float* lse;              // [T, H] log2 of a row's sum of 2^(score log2 e); or null
+  void* rest;              // what rounding took from o, in o's type and layout (16-bit types); or null
   int n_slots;             // of the launch, see Region
   // Backward.
   const void *out, *dout;

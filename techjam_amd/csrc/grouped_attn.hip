@@ -85,21 +85,23 @@ extern "C" int tj_packed_attn_fwd(const void* q, const void* k, const void* v, v
                                   int64_t H, int64_t Hk, int64_t D, int64_t Dv, const int64_t q_strides[3],
                                   const int64_t k_strides[3], const int64_t v_strides[3], const int64_t o_strides[3],
                                   float scale, int causal, const int32_t* offsets, const int32_t* lengths, float* lse,
-                                  hipStream_t stream) {
+                                  void* o_rest, hipStream_t stream) {
   if (elem_bytes(dtype) == 0) return TJ_ERR_DTYPE;
   if (!packed_sizes_ok(T, N, H, Hk)) return TJ_ERR_SHAPE;
   if (const int rc = check_dims(dtype, D, Dv)) return rc;
   if (T == 0) return TJ_OK;
   for (const void* p : {q, k, v, (const void*)o, (const void*)offsets})
     if (p == nullptr) return TJ_ERR_SHAPE;
+  if ((o_rest != nullptr) != (lse != nullptr && dtype != TJ_F32)) return TJ_ERR_SHAPE;
   if (!view_ok(q, q_strides, 3, dtype) || !view_ok(k, k_strides, 3, dtype) || !view_ok(v, v_strides, 3, dtype) ||
-      !view_ok(o, o_strides, 3, dtype) || !aligned4(offsets) || !aligned4(lengths) || !aligned4(lse))
+      !view_ok(o, o_strides, 3, dtype) || !tjh::aligned16(o_rest) || !aligned4(offsets) || !aligned4(lengths) || !aligned4(lse))
     return TJ_ERR_ALIGN;
   if (!rows_ok(k_strides[0], dtype) || !rows_ok(v_strides[0], dtype)) return TJ_ERR_UNSUPPORTED;
   PackedArgs a = packed_args(q, k, v, T, N, H, Hk, D, Dv, q_strides, k_strides, v_strides, o_strides, scale, causal, offsets,
                              lengths);
   a.o = o;
   a.lse = lse;
+  a.rest = o_rest;
   return packed_fwd(a, dtype, stream);
 }
 
@@ -108,8 +110,8 @@ extern "C" size_t tj_packed_attn_bwd_workspace_bytes(int64_t T, int64_t N, int64
   return (stat_floats(T, N, H) + peak_floats(T, N, Hk)) * sizeof(float);
 }
 
-extern "C" int tj_packed_attn_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse,
-                                  const void* dout, void* dq, void* dk, void* dv, int dtype, int64_t T, int64_t N, int64_t H,
+extern "C" int tj_packed_attn_bwd(const void* q, const void* k, const void* v, const void* o,
+                                  const void* o_rest, const float* lse, const void* dout, void* dq, void* dk, void* dv, int dtype, int64_t T, int64_t N, int64_t H,
                                   int64_t Hk, int64_t D, int64_t Dv, const int64_t q_strides[3], const int64_t k_strides[3],
                                   const int64_t v_strides[3], const int64_t o_strides[3], const int64_t do_strides[3],
                                   const int64_t dq_strides[3], const int64_t dk_strides[3], const int64_t dv_strides[3],
@@ -122,8 +124,9 @@ extern "C" int tj_packed_attn_bwd(const void* q, const void* k, const void* v, c
   for (const void* p : {q, k, v, o, (const void*)lse, dout, (const void*)dq, (const void*)dk, (const void*)dv,
                         (const void*)offsets})
     if (p == nullptr) return TJ_ERR_SHAPE;
+  if ((o_rest != nullptr) != (dtype != TJ_F32)) return TJ_ERR_SHAPE;
   if (!view_ok(q, q_strides, 3, dtype) || !view_ok(k, k_strides, 3, dtype) || !view_ok(v, v_strides, 3, dtype) ||
-      !view_ok(o, o_strides, 3, dtype) || !view_ok(dout, do_strides, 3, dtype) || !view_ok(dq, dq_strides, 3, dtype) ||
+      !view_ok(o, o_strides, 3, dtype) || !tjh::aligned16(o_rest) || !view_ok(dout, do_strides, 3, dtype) || !view_ok(dq, dq_strides, 3, dtype) ||
       !view_ok(dk, dk_strides, 3, dtype) || !view_ok(dv, dv_strides, 3, dtype) || !aligned4(offsets) || !aligned4(lengths) ||
       !aligned4(lse))
     return TJ_ERR_ALIGN;
@@ -133,7 +136,7 @@ extern "C" int tj_packed_attn_bwd(const void* q, const void* k, const void* v, c
   if (!tjh::aligned16(workspace)) return TJ_ERR_ALIGN;
   PackedArgs a = packed_args(q, k, v, T, N, H, Hk, D, Dv, q_strides, k_strides, v_strides, o_strides, scale, causal, offsets,
                              lengths);
-  a.out = o; a.lse = const_cast<float*>(lse); a.dout = dout;
+  a.out = o; a.rest = const_cast<void*>(o_rest); a.lse = const_cast<float*>(lse); a.dout = dout;
   a.dq = dq; a.dk = dk; a.dv = dv;
   a.vdo = View3{do_strides[0], do_strides[1]}; a.vdq = View3{dq_strides[0], dq_strides[1]};
   a.vdk = View3{dk_strides[0], dk_strides[1]}; a.vdv = View3{dv_strides[0], dv_strides[1]};

@@ -6,7 +6,10 @@
 //   dQ = scale dS K,  dK = scale dS^T Q,  dV = P^T dO,
 //
 // the last two summed over the group's rows. delta comes from the output as it was
-// returned, rounded to the inputs' type. 16-bit inputs have P and dS rounded to
+// returned plus what its rounding took away, which the forward pass keeps (in bf16
+// and fp16; together the two have 16 and 22 bits): from the rounded output alone dQ and dK
+// are 1.55 to 2.4 times as far from 64 bits as one rounding of the result (the most
+// for sequences of a few tokens), so 1.45 times. 16-bit inputs have P and dS rounded to
 // their type for these products, one rounding more than the result's own (fp32
 // MFMAs would take 16 times as long); fp32 inputs have none.
 //
@@ -164,16 +167,19 @@ __global__ __launch_bounds__(kThreads, (HD * (int)sizeof(T) <= 128 ? 2 : 1)) voi
     const int head = hk * a.G + row[n].g;
     const T* qp = reinterpret_cast<const T*>(a.q) + a.vq.row(token, head);
     const T* op = reinterpret_cast<const T*>(a.dout) + a.vdo.row(token, head);
-    const T* yp = reinterpret_cast<const T*>(a.out) + a.vo.row(token, head);
+    const int64_t at = a.vo.row(token, head);
     float sum = 0.f, norm = 0.f;
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       qf[n][s] = load_frag<T>(row[n].live ? qp : nullptr, 16 * s + 8 * hl, a.D);
       of[n][s] = load_frag<T>(row[n].live ? op : nullptr, 16 * s + 8 * hl, a.Dv);
-      const frag_t<T> y = load_frag<T>(row[n].live ? yp : nullptr, 16 * s + 8 * hl, a.Dv);
+      const frag_t<T> y = load_frag<T>(row[n].live ? reinterpret_cast<const T*>(a.out) + at : nullptr, 16 * s + 8 * hl, a.Dv);
+      frag_t<T> z;
+      if constexpr (sizeof(T) == 2)
+        z = load_frag<T>(row[n].live ? reinterpret_cast<const T*>(a.rest) + at : nullptr, 16 * s + 8 * hl, a.Dv);
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        sum = fmaf((float)of[n][s][j], (float)y[j], sum);
+        sum = fmaf((float)of[n][s][j], (float)y[j] + (sizeof(T) == 2 ? (float)z[j] : 0.f), sum);
         if constexpr (DsLift<T>::kOn) norm = fmaf((float)of[n][s][j], (float)of[n][s][j], norm);
       }
     }

@@ -102,10 +102,13 @@ __global__ __launch_bounds__(kThreads, (NB == 1 && HD * (int)sizeof(T) <= 256 ? 
     const int head = hk * a.G + row[n].g;
     if (STATS && row[n].live && lane < 32) a.lse[token * a.H + head] = st.m[n] - Elem<T>::kLift + log2f(exact);
     T* op = reinterpret_cast<T*>(a.o) + a.vo.row(token, head);
+    T* rp = reinterpret_cast<T*>(a.rest) + a.vo.row(token, head);
     st.columns(n, a.Dv, lane, [&](int col, float4_t y) {
       if (!row[n].live) y = float4_t{0.f, 0.f, 0.f, 0.f};
       else y *= inv;
       store4t<T>(op + col, y[0], y[1], y[2], y[3]);
+      if constexpr (STATS && sizeof(T) == 2)
+        store4t<T>(rp + col, y[0] - (float)(T)y[0], y[1] - (float)(T)y[1], y[2] - (float)(T)y[2], y[3] - (float)(T)y[3]);
     });
   }
 }

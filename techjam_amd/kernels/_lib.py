@@ -115,11 +115,11 @@ SIGNATURES = {
         + [_f32, _int, _vp, _i64, _vp, _vp, ctypes.c_size_t, _vp],
     ),
     "tj_packed_attn_fwd": (
-        _int, [_vp] * 4 + [_int] + [_i64] * 6 + [_i64p] * 4 + [_f32, _int, _vp, _vp, _vp, _vp]),
+        _int, [_vp] * 4 + [_int] + [_i64] * 6 + [_i64p] * 4 + [_f32, _int, _vp, _vp, _vp, _vp, _vp]),
     "tj_packed_attn_bwd_workspace_bytes": (ctypes.c_size_t, [_i64] * 4),
     "tj_packed_attn_bwd": (
         _int,
-        [_vp] * 9 + [_int] + [_i64] * 6 + [_i64p] * 8 + [_f32, _int, _vp, _vp, _vp, ctypes.c_size_t, _vp],
+        [_vp] * 10 + [_int] + [_i64] * 6 + [_i64p] * 8 + [_f32, _int, _vp, _vp, _vp, ctypes.c_size_t, _vp],
     ),
     "tj_tree_attn_workspace_bytes": (ctypes.c_size_t, [_int] + [_i64] * 7),
     "tj_tree_attn_fwd": (

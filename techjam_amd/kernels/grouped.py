@@ -87,24 +87,26 @@ def _backward_floats(t: int, n: int, h: int, hk: int) -> int:
 
 
 def _forward(q, k, v, offsets, valid_len, scale, causal, stats):
-    """One kernel call on padded inputs: ``(out, lse)``, the latter None without ``stats``."""
+    """One kernel call on padded inputs: ``(out, rest, lse)``, the last two for the backward pass:
+    None without ``stats``, and no ``rest`` of float32."""
     t, h, d = q.shape
     _, hk, dv = v.shape
     q, k, v = _tokens_view(q), _tokens_view(k), _tokens_view(v)
     dev = q.device
     out = q.new_empty((t, h, dv))
     lse = q.new_empty((t, h), dtype=torch.float32) if stats else None
+    rest = torch.empty_like(out) if stats and q.dtype != torch.float32 else None
     with on_device(dev):
         code = _lib.lib().tj_packed_attn_fwd(
             q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), DTYPES[q.dtype], t, offsets.shape[0] - 1, h, hk, d, dv,
             _lib.strides3(q), _lib.strides3(k), _lib.strides3(v), _lib.strides3(out), scale, int(causal),
-            offsets.data_ptr(), _ptr(valid_len), _ptr(lse), _stream_ptr(dev))
+            offsets.data_ptr(), _ptr(valid_len), _ptr(lse), _ptr(rest), _stream_ptr(dev))
     _lib.check(code, "tj_packed_attn_fwd")
-    return out, lse
+    return out, rest, lse
 
 
 def _backward(ctx, dout):
-    q, k, v, out, lse, offsets, valid_len = ctx.saved_tensors
+    q, k, v, out, rest, lse, offsets, valid_len = ctx.saved_tensors
     t, h, d = q.shape
     _, hk, dv = v.shape
     n = offsets.shape[0] - 1
@@ -115,7 +117,7 @@ def _backward(ctx, dout):
     ws = lse.new_empty(floats)
     with on_device(dev):
         code = _lib.lib().tj_packed_attn_bwd(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), dout.data_ptr(),
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(rest), lse.data_ptr(), dout.data_ptr(),
             dq.data_ptr(), dk.data_ptr(), dvv.data_ptr(), DTYPES[q.dtype], t, n, h, hk, d, dv,
             *map(_lib.strides3, (q, k, v, out, dout, dq, dk, dvv)), ctx.scale, int(ctx.causal),
             offsets.data_ptr(), _ptr(valid_len), ws.data_ptr(), 4 * floats, _stream_ptr(dev))
@@ -131,8 +133,8 @@ _backward_once = once_differentiable(_backward)
 class _PackedAttention(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, offsets, valid_len, scale, causal):
-        out, lse = _forward(q, k, v, offsets, valid_len, scale, causal, True)
-        ctx.save_for_backward(q, k, v, out, lse, offsets, valid_len)
+        out, rest, lse = _forward(q, k, v, offsets, valid_len, scale, causal, True)
+        ctx.save_for_backward(q, k, v, out, rest, lse, offsets, valid_len)
         ctx.scale, ctx.causal = scale, causal
         return out
 
@@ -176,8 +178,8 @@ def packed_attention(
     bits. In float16 the gradient of ``k`` sums its rows at one scale: beside an output gradient 1e6
     times larger in the same sequence and key head, a row's share loses bits. Second
     derivatives and forward-mode ones (``torch.autograd.forward_ad``) are not implemented and
-    refused. For the backward pass a call keeps its inputs, its output and ``4 * T * H`` bytes; an
-    output that was changed in place is refused there, as everywhere in torch.
+    refused. For the backward pass a call keeps its inputs, its output, ``4 * T * H`` bytes and, of 16-bit
+    types, what rounding took from the output (``2 * T * H * Dv`` bytes); an output that was changed in place is refused there, as everywhere in torch.
 
     A training step can be captured into a graph as any of torch's: while it is captured, no
     graph of an earlier eager call on the same leaves may be alive (delete its outputs first).
