@@ -60,11 +60,16 @@ struct Region {
     return j > a.N + 1 ? a.T : min(a.T, max(0, a.off[j - 1]));
   }
   __device__ __forceinline__ static int slot(int edge, int j, int per, int unit) { return (int)((int64_t)edge * per / unit) + j; }
+  // Tokens among the first rows of region j.
+  __device__ __forceinline__ static int tokens(const PackedArgs& a, int j, int rows) {
+    if (j <= 0 || j > a.N) return 0;
+    return a.len == nullptr ? rows : min(rows, max(0, a.len[j - 1]));
+  }
 
-  // The region and tile of `at`, in every lane of the wave that asks; false for a slot left
+  // The region and tile of slot `at`, in every lane of the wave that asks; false for a slot left
   // over. Sixty-four regions are looked at at a time.
   __device__ __forceinline__ bool find(const PackedArgs& a, int at, int per, int unit, int lane) {
-    int lo = 0, n = regions(a), first = 0;
+    int lo = 0, n = regions(a);
     while (n > 1) {
       const int step = (n + kWave - 1) / kWave, j = lo + lane * step;
       const bool in = lane * step < n;
@@ -76,13 +81,117 @@ struct Region {
     index = __builtin_amdgcn_readfirstlane(lo);
     start = __builtin_amdgcn_readfirstlane(edge(a, index));
     rows = max(0, __builtin_amdgcn_readfirstlane(edge(a, index + 1)) - start);
-    first = slot(start, index, per, unit);
-    tile = at - first;
-    const bool sequence = index > 0 && index <= a.N;
-    len = !sequence ? 0 : (a.len == nullptr ? rows : min(rows, max(0, __builtin_amdgcn_readfirstlane(a.len[index - 1]))));
+    len = __builtin_amdgcn_readfirstlane(tokens(a, index, rows));
+    tile = at - slot(start, index, per, unit);
+    return there(per, unit);
+  }
+  // Offsets out of order may have led anywhere.
+  __device__ __forceinline__ bool there(int per, int unit) const {
     return tile >= 0 && (int64_t)tile * unit < (int64_t)rows * per;
   }
+
+  // Sums and maxima of non-negative numbers over a wave, by DPP: a shuffle through the LDS takes
+  // five times as long.
+  template <typename Op>
+  __device__ __forceinline__ static int over_wave(int x, Op&& op) {
+    x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false));  // row_shr:1, 2, 4, 8
+    x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false));
+    x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false));
+    x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false));
+    x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false));  // row_bcast:15, 31
+    x = op(x, __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false));
+    return __builtin_amdgcn_readlane(x, kWave - 1);
+  }
+
+  // The at-th tile of all when those that take longest come first, so that no long one is left
+  // for the end: a causal sequence of n tiles has one of each length from 1 to n (the
+  // last the longest, or with `down` the first), another n of length n. Tiles without tokens
+  // come last. Every wave counts for itself, by halving the range of lengths: half a
+  // microsecond, where a launch that sorts would take several. For up to kRanked regions.
+  static constexpr int kChunks = 4, kRanked = kChunks * kWave;
+  __device__ __forceinline__ bool ranked(const PackedArgs& a, int at, int per, int unit, bool down, int lane) {
+    int n[kChunks], all[kChunks], count = 0, top = 0;
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+      const int j = c * kWave + lane;
+      n[c] = all[c] = 0;
+      if (c * kWave < regions(a) && j < regions(a)) {
+        const int rows = max(0, edge(a, j + 1) - edge(a, j));
+        all[c] = (rows * per + unit - 1) / unit;
+        n[c] = (tokens(a, j, rows) * per + unit - 1) / unit;
+      }
+      count += n[c];
+      top = max(top, n[c]);
+    }
+    auto sum = [](int x, int y) { return x + y; };
+    count = over_wave(count, sum);
+    const bool live = at < count;
+    int lo = 0, rank;
+    if (live) {
+      int hi = over_wave(top, [](int x, int y) { return max(x, y); }), beyond = 0;  // more than `at` tiles are longer than lo, `beyond` <= at than hi
+      while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        int x = 0;
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) x += a.causal ? max(0, n[c] - mid) : (n[c] > mid ? n[c] : 0);
+        x = over_wave(x, sum);
+        if (x > at) lo = mid;
+        else {
+          hi = mid;
+          beyond = x;
+        }
+      }
+      rank = at - beyond;
+    } else {
+      rank = at - count;
+    }
+    // Which region: among those with a tile of this length the rank-th, or the rank-th of the tiles without tokens.
+    tile = a.causal ? lo : (live ? rank % (lo + 1) : 0);
+    if (live && !a.causal) rank /= lo + 1;
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+      if (c * kWave >= regions(a)) break;
+      uint64_t who;
+      if (live) {
+        const bool has = a.causal ? n[c] > lo : n[c] == lo + 1;
+        const uint64_t mask = __ballot(has);
+        const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+        who = __ballot(has && before == rank);
+        rank -= (int)__popcll(mask);
+      } else {
+        int upto = all[c] - n[c];
+        const int own = upto;
+#pragma unroll
+        for (int s = 1; s < kWave; s <<= 1) {
+          const int x = __shfl_up(upto, s);
+          if (lane >= s) upto += x;
+        }
+        who = __ballot(rank < upto && rank >= upto - own);
+        if (who != 0) tile = rank - __builtin_amdgcn_readlane(upto - own, __builtin_ctzll(who));
+        else rank -= __builtin_amdgcn_readlane(upto, kWave - 1);
+      }
+      if (who != 0) {
+        const int from = __builtin_ctzll(who), tiles = __builtin_amdgcn_readlane(n[c], from);
+        index = c * kWave + from;
+        if (!live) tile += tiles;
+        else if (a.causal && down) tile = tiles - 1 - tile;
+        start = __builtin_amdgcn_readfirstlane(edge(a, index));
+        rows = max(0, __builtin_amdgcn_readfirstlane(edge(a, index + 1)) - start);
+        len = __builtin_amdgcn_readfirstlane(tokens(a, index, rows));
+        return there(per, unit);
+      }
+    }
+    return false;
+  }
+
+  // The tile of workgroup `at`, of as many slots as the launch has.
+  __device__ __forceinline__ bool take(const PackedArgs& a, int at, int per, int unit, bool down, int lane) {
+    if (regions(a) <= kRanked) return ranked(a, at, per, unit, down, lane);
+    return find(a, down ? at : a.n_slots - 1 - at, per, unit, lane);
+  }
 };
+
+inline int64_t region_slots(int64_t T, int64_t N, int64_t per, int64_t unit) { return T * per / unit + N + 2; }
 
 struct TreeArgs {
   const void *q, *k, *v;
@@ -100,8 +209,6 @@ struct TreeArgs {
   int n_parts, few_slots, few_each;
   float *part_o, *part_ml;
 };
-
-inline int64_t region_slots(int64_t T, int64_t N, int64_t per, int64_t unit) { return T * per / unit + N + 2; }
 
 constexpr float kLazy = 8.f;  // the running maximum moves when a row's maximum grows by more than 2^8
 

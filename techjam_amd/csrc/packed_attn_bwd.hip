@@ -125,7 +125,7 @@ template <typename T, int HD>
 constexpr bool groups_fit(int groups) { return groups * SweepShape<T, HD, 32>::W * (int)sizeof(T) <= 1024; }
 
 template <typename T, int HD, int BLOCKS, int NB>
-__global__ __launch_bounds__(kThreads, (HD * (int)sizeof(T) <= 128 ? 2 : 1)) void packed_bwd_q_kernel(PackedArgs a) {
+__global__ __launch_bounds__(kThreads, (HD * (int)sizeof(T) <= 256 ? 2 : 1)) void packed_bwd_q_kernel(PackedArgs a) {
   using QS = QShape<T, HD, BLOCKS, NB>;
   using SH = typename QS::SH;
   using Rows = typename SH::Rows;
@@ -136,7 +136,7 @@ __global__ __launch_bounds__(kThreads, (HD * (int)sizeof(T) <= 128 ? 2 : 1)) voi
             ln = lane % 32;
   const int kg = w / RB, rb = w % RB, hk = blockIdx.x % a.Hk;
   Region g;
-  if (!g.find(a, a.n_slots - 1 - (int)(blockIdx.x / a.Hk), a.G, ROWS, lane)) return;
+  if (!g.take(a, blockIdx.x / a.Hk, a.G, ROWS, false, lane)) return;
   const int L = g.len, R = g.rows * a.G, r0 = g.tile * ROWS, rw0 = r0 + 32 * NB * rb;
   auto span = [&](int row, int last) {
     return row >= R || row / a.G >= L ? 0 : (a.causal ? min(L, min(last, R - 1) / a.G + 1) : L);
@@ -290,39 +290,38 @@ __global__ __launch_bounds__(kThreads, (HD * (int)sizeof(T) <= 128 ? 2 : 1)) voi
   }
 }
 
-// A workgroup = KB blocks of 32 keys of one (sequence, key head) times RG groups of
-// token tiles, a wave each: the tiles of 32 tokens that see the keys, of one query
+// A workgroup = KB waves of NB blocks of 32 keys of one (sequence, key head) times RG
+// groups of token tiles: the tiles of 32 tokens that see the keys, of one query
 // head of the group after the other, are dealt to the groups in turn, and the
 // groups' sums meet in LDS at the end. Scores are formed with tokens in the
 // registers and keys over the lanes, so that P and dS turn into the A operands of dV
 // and dK where they stand; Q and dO come back as B operands through the transposing
 // LDS read.
-template <typename T, int HD, bool HALF>
+template <typename T, int HD, int BLOCKS, int GROUPS, int NBT>
 struct KvShape {
   using SH = SweepShape<T, HD, 32>;
-  static constexpr int kWhole = (sizeof(T) == 2 && HD <= 64) || HD == 32 ? 8 : 4, WAVES = HALF ? kWhole / 2 : kWhole;
-  static constexpr int kFit = 1024 / (SH::W * (int)sizeof(T));
-  static constexpr int RG = kFit < kWhole / 2 ? kFit : kWhole / 2;
-  static constexpr int KB = WAVES / RG;
+  static constexpr int KB = BLOCKS, RG = GROUPS, NB = NBT, WAVES = KB * RG, KEYS = 32 * NB * KB;
   static constexpr int kDepth = HD == 32 ? 0 : sizeof(T) == 2 ? 2 : 1;
+  // Waves of a SIMD, by the registers.
+  static constexpr int kMin = sizeof(T) == 2 ? (HD <= 64 && KB > 1 ? 3 : 2) : (HD == 32 ? 2 : 1);
 };
 
-template <typename T, int HD, bool HALF>
-__global__ __launch_bounds__((64 * KvShape<T, HD, HALF>::WAVES), (KvShape<T, HD, HALF>::kWhole / 4)) void
+template <typename T, int HD, int BLOCKS, int GROUPS, int NB>
+__global__ __launch_bounds__((64 * BLOCKS * GROUPS), (KvShape<T, HD, BLOCKS, GROUPS, NB>::kMin)) void
 packed_bwd_kv_kernel(PackedArgs a) {
-  using KV = KvShape<T, HD, HALF>;
+  using KV = KvShape<T, HD, BLOCKS, GROUPS, NB>;
   using SH = typename KV::SH;
   using Rows = typename SH::Rows;
   constexpr int KS = SH::KS, DB = SH::DB, BM = 32, KB = KV::KB, RG = KV::RG, kDepth = KV::kDepth;
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[RG * 2 * SH::kBytes];  // Q's tile, then dO's
-  __shared__ __attribute__((aligned(1024))) float stat[RG][2][64];                    // of a tile's tokens
+  constexpr int kSums = RG / 2 * KB * NB * 2 * DB * 16 * kWave * 4;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[RG * 2 * SH::kBytes > kSums ? RG * 2 * SH::kBytes : kSums];  // Q's tile, then dO's
+  __shared__ __attribute__((aligned(1024))) float stat[RG][2][64];  // of a tile's tokens
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave, hl = lane / 32,
             ln = lane % 32;
   const int kb = w % KB, rg = w / KB, hk = blockIdx.x % a.Hk;
   Region g;
-  if (!g.find(a, blockIdx.x / a.Hk, 1, 32 * KB, lane)) return;
-  const int L = g.len, k0 = g.tile * 32 * KB, kw0 = k0 + 32 * kb, key = kw0 + ln;
-  const bool live = key < L;
+  if (!g.take(a, blockIdx.x / a.Hk, 1, KV::KEYS, true, lane)) return;
+  const int L = g.len, k0 = g.tile * KV::KEYS, kw0 = k0 + 32 * NB * kb;
 
   // The group's KB waves bring its tiles.
   SweepTiles<T, SH, KB> rows;
@@ -351,19 +350,21 @@ packed_bwd_kv_kernel(PackedArgs a) {
     if (kb == 0) copy_4(make_rsrc(stat_at(a, g, hk * a.G + h, i0), 256), stat0 + buf * 256, 4 * lane);
   };
 
-  frag_t<T> kf[KS], vf[KS];
-  {
+  frag_t<T> kf[NB][KS], vf[NB][KS];
+  float16_t dv[NB][DB], dk[NB][DB];
+#pragma unroll
+  for (int n = 0; n < NB; ++n) {
+    const int key = kw0 + 32 * n + ln;
     const T* kp = reinterpret_cast<const T*>(a.k) + a.vk.row(g.start + key, hk);
     const T* vp = reinterpret_cast<const T*>(a.v) + a.vv.row(g.start + key, hk);
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-      kf[s] = load_frag<T>(live ? kp : nullptr, 16 * s + 8 * hl, a.D);
-      vf[s] = load_frag<T>(live ? vp : nullptr, 16 * s + 8 * hl, a.Dv);
+      kf[n][s] = load_frag<T>(key < L ? kp : nullptr, 16 * s + 8 * hl, a.D);
+      vf[n][s] = load_frag<T>(key < L ? vp : nullptr, 16 * s + 8 * hl, a.Dv);
     }
-  }
-  float16_t dv[DB], dk[DB];
 #pragma unroll
-  for (int d = 0; d < DB; ++d) dv[d] = dk[d] = zero16();
+    for (int d = 0; d < DB; ++d) dv[n][d] = dk[n][d] = zero16();
+  }
 
   const float dl = DsLift<T>(a, g, hk, lane).all(), lift = dl / DsLift<T>::kP, c2 = a.scale * kLog2e;
   int h = 0, i0 = i_begin;  // this round's tile
@@ -386,73 +387,90 @@ packed_bwd_kv_kernel(PackedArgs a) {
       issue(h, i0, cur ^ 1);
     }
     if (!busy) continue;
-    float16_t p = zero16(), dp = zero16();
+    float16_t p[NB], dp[NB];
+#pragma unroll
+    for (int b = 0; b < NB; ++b) p[b] = dp[b] = zero16();
     read_ahead<KS, kDepth>([&](int s) { return Rows::row_frag(tile + qrow, s, 0); },
-                           [&](int s, frag_t<T> f) { p = Elem<T>::mma(f, kf[s], p); });
+                           [&](int s, frag_t<T> f) {
+#pragma unroll
+                             for (int b = 0; b < NB; ++b) p[b] = Elem<T>::mma(f, kf[b][s], p[b]);
+                           });
     read_ahead<KS, kDepth>([&](int s) { return Rows::row_frag(tile + orow, s, 0); },
-                           [&](int s, frag_t<T> f) { dp = Elem<T>::mma(f, vf[s], dp); });
+                           [&](int s, frag_t<T> f) {
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const float4_t ls = lds_at<float4_t>(srow + q * 32), d0 = lds_at<float4_t>(srow + 128 + q * 32);
+                             for (int b = 0; b < NB; ++b) dp[b] = Elem<T>::mma(f, vf[b][s], dp[b]);
+                           });
+    frag_t<T> fp[NB][2], fs[NB][2];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const float e = fast_exp2(fmaf(p[4 * q + j], c2, ls[j]));
-        p[4 * q + j] = e;
-        dp[4 * q + j] = e * fmaf(dp[4 * q + j], lift, d0[j]);
+    for (int b = 0; b < NB; ++b) {
+      const int first = kw0 + 32 * b;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const float4_t ls = lds_at<float4_t>(srow + q * 32), d0 = lds_at<float4_t>(srow + 128 + q * 32);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float e = fast_exp2(fmaf(p[b][4 * q + j], c2, ls[j]));
+          p[b][4 * q + j] = e;
+          dp[b][4 * q + j] = e * fmaf(dp[b][4 * q + j], lift, d0[j]);
+        }
       }
-    }
-    // Selected, not multiplied: tokens past the length have no numbers at all.
-    if ((a.causal && at < kw0 + 31) || at + BM > L) {
+      // Selected, not multiplied: tokens past the length have no numbers at all.
+      if ((a.causal && at < first + 31) || at + BM > L) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int i = at + acc_row(r, hl);
-        if ((a.causal && i < key) || i >= L) p[r] = dp[r] = 0.f;
+        for (int r = 0; r < 16; ++r) {
+          const int i = at + acc_row(r, hl);
+          if ((a.causal && i < first + ln) || i >= L) p[b][r] = dp[b][r] = 0.f;
+        }
       }
-    }
-    frag_t<T> fp[2], fs[2];
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      fp[s] = acc_frag<T>(p, s);
-      fs[s] = acc_frag<T>(dp, s);
+      for (int s = 0; s < 2; ++s) {
+        fp[b][s] = acc_frag<T>(p[b], s);
+        fs[b][s] = acc_frag<T>(dp[b], s);
+      }
     }
     if constexpr (kDepth > 0) __builtin_amdgcn_sched_barrier(0);
     read_ahead<2 * DB, kDepth>([&](int j) { return Rows::col_frag(tile + ocol, j % DB, 16 * (j / DB) * Rows::kRowBytes); },
-                               [&](int j, frag_t<T> f) { dv[j % DB] = Elem<T>::mma(fp[j / DB], f, dv[j % DB]); });
+                               [&](int j, frag_t<T> f) {
+#pragma unroll
+                                 for (int b = 0; b < NB; ++b) dv[b][j % DB] = Elem<T>::mma(fp[b][j / DB], f, dv[b][j % DB]);
+                               });
     read_ahead<2 * DB, kDepth>([&](int j) { return Rows::col_frag(tile + qcol, j % DB, 16 * (j / DB) * Rows::kRowBytes); },
-                               [&](int j, frag_t<T> f) { dk[j % DB] = Elem<T>::mma(fs[j / DB], f, dk[j % DB]); });
+                               [&](int j, frag_t<T> f) {
+#pragma unroll
+                                 for (int b = 0; b < NB; ++b) dk[b][j % DB] = Elem<T>::mma(fs[b][j / DB], f, dk[b][j % DB]);
+                               });
   }
 
   // The groups' sums, the upper half's added to the lower half's.
   if constexpr (RG > 1) {
-    static_assert(sizeof(smem) >= (RG / 2) * KB * 2 * DB * 16 * kWave * sizeof(float), "room for the groups' sums");
-    float4_t* x = reinterpret_cast<float4_t*>(smem);
+    auto each = [&](auto&& f) {
+#pragma unroll
+      for (int n = 0; n < NB; ++n)
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+          f(dv[n][d], 2 * (n * DB + d));
+          f(dk[n][d], 2 * (n * DB + d) + 1);
+        }
+    };
 #pragma unroll
     for (int half = RG / 2; half > 0; half /= 2) {
-      float4_t* y = x + ((rg % half) * KB + kb) * 2 * DB * 4 * kWave + lane;
+      float4_t* y = reinterpret_cast<float4_t*>(smem) + ((rg % half) * KB + kb) * NB * 2 * DB * 4 * kWave + lane;
       __syncthreads();
-      if (rg >= half && rg < 2 * half) {
+      if (rg >= half && rg < 2 * half)
+        each([&](float16_t& x, int i) {
 #pragma unroll
-        for (int d = 0; d < DB; ++d)
+          for (int q = 0; q < 4; ++q) y[(4 * i + q) * kWave] = float4_t{x[4 * q], x[4 * q + 1], x[4 * q + 2], x[4 * q + 3]};
+        });
+      __syncthreads();
+      if (rg < half)
+        each([&](float16_t& x, int i) {
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            y[(2 * d * 4 + q) * kWave] = float4_t{dv[d][4 * q], dv[d][4 * q + 1], dv[d][4 * q + 2], dv[d][4 * q + 3]};
-            y[((2 * d + 1) * 4 + q) * kWave] = float4_t{dk[d][4 * q], dk[d][4 * q + 1], dk[d][4 * q + 2], dk[d][4 * q + 3]};
+            const float4_t z = y[(4 * i + q) * kWave];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[4 * q + j] += z[j];
           }
-      }
-      __syncthreads();
-      if (rg < half) {
-#pragma unroll
-        for (int d = 0; d < DB; ++d)
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const float4_t u = y[(2 * d * 4 + q) * kWave], z = y[((2 * d + 1) * 4 + q) * kWave];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              dv[d][4 * q + j] += u[j];
-              dk[d][4 * q + j] += z[j];
-            }
-          }
-      }
+        });
     }
     if (rg != 0) return;
   }
@@ -460,18 +478,20 @@ packed_bwd_kv_kernel(PackedArgs a) {
   // Keys at or past the length have no gradient: zeros, whatever their scores were.
   const float dv_scale = 1.f / DsLift<T>::kP, dk_scale = a.scale / dl;
 #pragma unroll
-  for (int r = 0; r < 16; ++r) {
-    const int j = kw0 + acc_row(r, hl);
-    if (j >= g.rows) continue;
-    const bool in = j < L;
-    T* pv = reinterpret_cast<T*>(a.dv) + a.vdv.row(g.start + j, hk);
-    T* pk = reinterpret_cast<T*>(a.dk) + a.vdk.row(g.start + j, hk);
+  for (int n = 0; n < NB; ++n)
 #pragma unroll
-    for (int d = 0; d < DB; ++d) {
-      if (32 * d + ln < a.Dv) pv[32 * d + ln] = (T)(in ? dv[d][r] * dv_scale : 0.f);
-      if (32 * d + ln < a.D) pk[32 * d + ln] = (T)(in ? dk[d][r] * dk_scale : 0.f);
+    for (int r = 0; r < 16; ++r) {
+      const int j = kw0 + 32 * n + acc_row(r, hl);
+      if (j >= g.rows) continue;
+      const bool in = j < L;
+      T* pv = reinterpret_cast<T*>(a.dv) + a.vdv.row(g.start + j, hk);
+      T* pk = reinterpret_cast<T*>(a.dk) + a.vdk.row(g.start + j, hk);
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        if (32 * d + ln < a.Dv) pv[32 * d + ln] = (T)(in ? dv[n][d][r] * dv_scale : 0.f);
+        if (32 * d + ln < a.D) pk[32 * d + ln] = (T)(in ? dk[n][d][r] * dk_scale : 0.f);
+      }
     }
-  }
 }
 
 template <typename T, int HD, int BLOCKS, int NB>
@@ -482,12 +502,13 @@ int launch_q(PackedArgs a, hipStream_t stream) {
   return tjh::launch_status();
 }
 
-template <typename T, int HD, bool HALF>
+template <typename T, int HD, int BLOCKS, int GROUPS, int NB>
 int launch_kv(PackedArgs a, hipStream_t stream) {
-  using KV = KvShape<T, HD, HALF>;
-  const int64_t slots = region_slots(a.T, a.N, 1, 32 * KV::KB);
+  using KV = KvShape<T, HD, BLOCKS, GROUPS, NB>;
+  const int64_t slots = region_slots(a.T, a.N, 1, KV::KEYS);
   a.n_slots = (int)slots;
-  hipLaunchKernelGGL((packed_bwd_kv_kernel<T, HD, HALF>), dim3(uint32_t(slots * a.Hk)), dim3(64 * KV::WAVES), 0, stream, a);
+  hipLaunchKernelGGL((packed_bwd_kv_kernel<T, HD, BLOCKS, GROUPS, NB>), dim3(uint32_t(slots * a.Hk)), dim3(64 * KV::WAVES), 0,
+                     stream, a);
   return tjh::launch_status();
 }
 
@@ -515,8 +536,8 @@ int packed_bwd(const PackedArgs& a, int dtype, hipStream_t stream) {
       else rc = launch_q<T, HD, 4, 1>(a, stream);
     }
     if (rc != TJ_OK) return rc;
-    if ((int64_t)(a.T + 63) / 64 * a.Hk <= kCus / 2) return launch_kv<T, HD, true>(a, stream);
-    return launch_kv<T, HD, false>(a, stream);
+    if ((int64_t)(a.T + 63) / 64 * a.Hk <= kCus / 2) return launch_kv<T, HD, 1, HD == 32 || (HD == 64 && sizeof(T) == 2) ? 4 : 2, 1>(a, stream);
+    return launch_kv<T, HD, 2, 2, 1>(a, stream);
   });
 }
 

@@ -35,10 +35,10 @@ __global__ __launch_bounds__(kThreads, (NB == 1 && HD * (int)sizeof(T) <= 256 ? 
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
   const int kg = w / RB, rb = w % RB;
   // Consecutive ids run on the XCDs in turn, so the key head varies fastest: the tiles that share
-  // K and V also share an XCD's L2. The tiles with the most keys of a causal sequence come first.
+  // K and V also share an XCD's L2.
   const int hk = blockIdx.x % a.Hk;
   Region g;
-  if (!g.find(a, a.n_slots - 1 - (int)(blockIdx.x / a.Hk), a.G, ROWS, lane)) return;
+  if (!g.take(a, blockIdx.x / a.Hk, a.G, ROWS, false, lane)) return;
   const int L = g.len, R = g.rows * a.G, r0 = g.tile * ROWS, rw0 = r0 + 32 * NB * rb;
   // Keys needed by rows row .. last (clipped to the region's).
   auto span = [&](int row, int last) {
