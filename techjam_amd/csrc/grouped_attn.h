@@ -208,6 +208,7 @@ struct TreeArgs {
   // (maximum, sum, whether the row is there, -) [n_parts, Hk, R, 4]. part_o null: sweeps run whole.
   int n_parts, few_slots, few_each;
   float *part_o, *part_ml;
+  int32_t* plan;           // [B, 2] a sequence's first part, the keys of each
 };
 
 constexpr float kLazy = 8.f;  // the running maximum moves when a row's maximum grows by more than 2^8

@@ -72,8 +72,9 @@ TreeArgs tree_sizes(int64_t B, int64_t H, int64_t Hk, int64_t Sq, int64_t Sk, in
   return a;
 }
 
-size_t part_rows(const TreeArgs& a, const TreePlan& p) {
-  return p.whole() ? 0 : size_t(p.parts.total) * size_t(a.Hk) * size_t(a.R);
+size_t part_rows(const TreeArgs& a, const TreePlan& p) { return size_t(p.parts.total) * size_t(a.Hk) * size_t(a.R); }
+size_t part_bytes(const TreeArgs& a, const TreePlan& p) {
+  return p.whole() ? 0 : (part_rows(a, p) * size_t(a.Dv + 4) + size_t(a.B) * 2) * sizeof(float);
 }
 
 }  // namespace
@@ -149,7 +150,7 @@ extern "C" size_t tj_tree_attn_workspace_bytes(int dtype, int64_t B, int64_t H, 
                                                int64_t Dv) {
   if (!tree_sizes_ok(B, H, Hk, Sq, Sk) || check_dims(dtype, D, Dv) != TJ_OK || B == 0 || Sq == 0) return 0;
   const TreeArgs a = tree_sizes(B, H, Hk, Sq, Sk, D, Dv);
-  return part_rows(a, tree_plan(a, dtype)) * size_t(Dv + 4) * sizeof(float);
+  return part_bytes(a, tree_plan(a, dtype));
 }
 
 extern "C" int tj_tree_attn_fwd(const void* q, const void* k, const void* v, void* o, int dtype, int64_t B, int64_t H,
@@ -173,11 +174,12 @@ extern "C" int tj_tree_attn_fwd(const void* q, const void* k, const void* v, voi
   a.vv = View4{v_strides[0], v_strides[1], v_strides[2]}; a.vo = View4{o_strides[0], o_strides[1], o_strides[2]};
   a.scale = scale; a.len = lengths; a.parents = parents;
   const TreePlan p = tree_plan(a, dtype);
-  if (const size_t rows = part_rows(a, p)) {
-    if (workspace == nullptr || workspace_bytes < rows * size_t(Dv + 4) * sizeof(float)) return TJ_ERR_WORKSPACE;
+  if (const size_t bytes = part_bytes(a, p)) {
+    if (workspace == nullptr || workspace_bytes < bytes) return TJ_ERR_WORKSPACE;
     if (!tjh::aligned16(workspace)) return TJ_ERR_ALIGN;
     a.part_o = static_cast<float*>(workspace);
-    a.part_ml = a.part_o + rows * size_t(Dv);
+    a.part_ml = a.part_o + part_rows(a, p) * size_t(Dv);
+    a.plan = reinterpret_cast<int32_t*>(a.part_ml + part_rows(a, p) * 4);
   }
   return tree_fwd(a, p, dtype, stream);
 }

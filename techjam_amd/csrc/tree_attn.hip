@@ -3,9 +3,9 @@
 // stand in its cache behind what it has settled, at positions len - Sq on; token t sees
 // all settled keys, and of the drafted ones its own and those on its line of parents.
 //
-// A workgroup = RB waves of 32 rows of one (sequence, key head) and one part of the
-// keys, so that up to 256 rows read a key from memory once. Parts are joined by
-// tree_join_kernel.
+// A workgroup = RB waves of 32 rows of one (sequence, key head) times KG groups over one
+// part of the keys, so that up to 256 rows read a key from memory once; the tiles are dealt to the
+// groups, whose sums meet in LDS at the end. Parts are joined by tree_join_kernel.
 #include "grouped_attn.h"
 
 namespace tj {
@@ -39,42 +39,58 @@ struct Lineage {
   }
 };
 
+// Four waves of key groups for up to 64 rows, so that four parts meet in LDS rather than in memory; eight
+// waves in all at the most, and two tiles a group in at most 128 KB.
 template <typename T, int HD, int BLOCKS>
 struct TreeShape {
-  static constexpr int RB = BLOCKS, ROWS = 32 * RB, THREADS = kWave * RB;
-  using SH = SweepShape<T, HD, 32>;
+  static constexpr int RB = BLOCKS, ROWS = 32 * RB, BN = RB == 8 ? 64 : 32;
+  using SH = SweepShape<T, HD, BN>;
+  static constexpr int kFit = 128 * 1024 / (2 * SH::kBytes), kMost = RB <= 2 ? 4 : 8 / RB, KG = kFit < kMost ? kFit : kMost;
+  static constexpr int WAVES = RB * KG, THREADS = kWave * WAVES;
   // Waves of a SIMD by the registers, and workgroups that a CU holds.
-  static constexpr int kWaves = HD == 32 ? 3 : (sizeof(T) == 2 || HD == 64 ? 2 : 1);
-  static constexpr int kByLds = 160 * 1024 / (2 * SH::kBytes), kByRegs = kWaves * 4 / RB > 1 ? kWaves * 4 / RB : 1;
+  static constexpr int kWaves = HD == 32 ? 3 : (sizeof(T) == 2 || HD == 64 || WAVES > 4 ? 2 : 1);
+  static constexpr int kByLds = 160 * 1024 / (KG * 2 * SH::kBytes), kByRegs = kWaves * 4 / WAVES;
   static constexpr int kPerCu = kByLds < kByRegs ? kByLds : kByRegs;
+  static_assert(kPerCu >= 1, "a workgroup fits a CU");
 };
 
 template <typename T, int HD, int BLOCKS>
-__global__ __launch_bounds__((TreeShape<T, HD, BLOCKS>::THREADS), (BLOCKS == 8 ? 2 : TreeShape<T, HD, BLOCKS>::kWaves)) void tree_kernel(TreeArgs a) {
+__global__ __launch_bounds__((TreeShape<T, HD, BLOCKS>::THREADS), (TreeShape<T, HD, BLOCKS>::kWaves)) void tree_kernel(TreeArgs a) {
   using TS = TreeShape<T, HD, BLOCKS>;
   using SH = typename TS::SH;
-  constexpr int RB = TS::RB, BN = SH::BN;
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[2 * SH::kBytes];
+  using State = SweepState<T, HD, TS::BN, 1, false>;
+  constexpr int RB = TS::RB, KG = TS::KG, BN = TS::BN;
+  // Two tiles a group; afterwards the groups' results.
+  constexpr int kSums = KG > 1 ? 16 * State::kGive * RB * (KG / 2) : 0;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[KG * 2 * SH::kBytes > kSums ? KG * 2 * SH::kBytes : kSums];
+  __shared__ float ml[KG > 1 ? KG / 2 * RB * State::kMl * kWave : 1];
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
+  const int kg = w / RB, rb = w % RB;
   const int mt = blockIdx.x % a.n_mtiles, hk = blockIdx.x / a.n_mtiles % a.Hk, part = blockIdx.x / a.n_mtiles / a.Hk;
   const bool whole = a.part_o == nullptr;
   FewParts f;
   if (whole) f.b = part;
   else if (!f.find(a, part, lane)) return;
   const int b = __builtin_amdgcn_readfirstlane(f.b);
+  // For the join, which need not count parts again.
+  if (!whole && part == f.first && hk == 0 && mt == 0 && tid == 0) {
+    a.plan[2 * b] = f.first;
+    a.plan[2 * b + 1] = f.keys;
+  }
   const int L = __builtin_amdgcn_readfirstlane(min(a.Sk, max(0, a.len[b]))), ctx = L - a.Sq;
-  const int row0 = mt * TS::ROWS, rw0 = row0 + 32 * w;
+  const int row0 = mt * TS::ROWS, rw0 = row0 + 32 * rb;
   // Keys that rows row .. last (clipped to R) need.
   auto span = [&](int row, int last) { return row >= a.R ? 0 : max(0, ctx + min(last, a.R - 1) / a.G + 1); };
   const int n_keys = whole ? L : __builtin_amdgcn_readfirstlane(f.keys);
   const int kv_begin = whole ? 0 : __builtin_amdgcn_readfirstlane((part - f.first) * f.keys);
   const int kv_end = min(span(row0, row0 + TS::ROWS - 1), kv_begin + n_keys), own_end = min(kv_end, span(rw0, rw0 + 31));
   if (kv_begin >= kv_end && !whole) return;  // not read either
-  const uint32_t tiles = lds_offset(smem);
+  const uint32_t tiles = lds_offset(smem) + kg * 2 * SH::kBytes;
   SweepTiles<T, SH, RB> keys;
   keys.init(reinterpret_cast<const T*>(a.k) + a.vk.row(b, hk, 0), reinterpret_cast<const T*>(a.v) + a.vv.row(b, hk, 0),
-            a.vk.ss, a.vv.ss, a.D, a.Dv, w, lane);
-  if (kv_begin < kv_end) keys.issue(kv_begin, L, tiles, w);
+            a.vk.ss, a.vv.ss, a.D, a.Dv, rb, lane);
+  int kv0 = kv_begin + BN * kg;
+  if (kv0 < kv_end) keys.issue(kv0, L, tiles, rb);
   const int r = rw0 + lane % 32;
   SweepRow row{r, r / a.G, r % a.G, 0, false};
   row.limit = ctx + row.i;
@@ -87,47 +103,63 @@ __global__ __launch_bounds__((TreeShape<T, HD, BLOCKS>::THREADS), (BLOCKS == 8 ?
     gone = __ballot(line.gone && lane < a.Sq);
     row.live = row.live && !(gone >> t & 1);
   }
-  SweepState<T, HD, BN, 1, false> st;
+  State st;
   st.init(a.scale, lane);
   st.load_q(0, row.live ? reinterpret_cast<const T*>(a.q) + a.vq.row(b, hk * a.G + row.g, row.i) : nullptr, a.scale, a.D, lane);
-  for (int kv0 = kv_begin, cur = 0; kv0 < kv_end; kv0 += BN, cur ^= 1) {
-    // The tile is there, and the other one has been read.
+  // The workgroup goes round together, the last round maybe without a tile for every group.
+  for (int first = kv_begin, cur = 0; first < kv_end; first += KG * BN, kv0 += KG * BN, cur ^= 1) {
+    // The tile is there, and the group's other one has been read by its waves. (A group of one wave has waited for
+    // itself.)
     wait_copies();
-    lds_barrier();
-    if (kv0 + BN < kv_end) keys.issue(kv0 + BN, L, tiles + (cur ^ 1) * SH::kBytes, w);
+    if constexpr (RB > 1) lds_barrier();
+    if (kv0 + KG * BN < kv_end) keys.issue(kv0 + KG * BN, L, tiles + (cur ^ 1) * SH::kBytes, rb);
     const uint32_t tile = tiles + cur * SH::kBytes;
-    if (gone != 0 && kv0 + BN > ctx) {
+    if (gone != 0 && first + KG * BN > ctx) {
       // What is not there may hold anything: its values are cleared, as 0 times NaN would spoil the others.
       constexpr int kChunks = SH::Rows::kChunks;
-      for (int c = tid; c < BN * kChunks; c += TS::THREADS) {
+      for (int c = rb * kWave + lane; c < BN * kChunks; c += RB * kWave) {
         const int t = kv0 + c / kChunks - ctx;
         if (t >= 0 && t < kWave && (gone >> t & 1))
           *(__attribute__((address_space(3))) float4_t*)(uintptr_t)(tile + SH::kTensor + c * 16) = float4_t{0.f, 0.f, 0.f, 0.f};
       }
       wait_lds();
-      lds_barrier();
+      if constexpr (RB > 1) lds_barrier();
     }
-    if (kv0 >= own_end) continue;
-    st.step(tile, 0, [&](int, float16_t& s) {
-      const int hl = lane / 32;
-      if (kv0 + BN <= ctx) return;
-      if (a.parents == nullptr) {
+#pragma unroll
+    for (int kb = 0; kb < BN / 32; ++kb) {
+      const int at = kv0 + 32 * kb;
+      if (at >= own_end) continue;
+      st.step(tile, kb, [&](int, float16_t& s) {
+        const int hl = lane / 32;
+        if (at + 32 <= ctx) return;
+        if (a.parents == nullptr) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (at + acc_row(e, hl) > row.limit) s[e] = -__builtin_inff();
+          return;
+        }
+        // The 32 keys that the row sees: settled ones, then its line.
+        const int t = at - ctx;  // drafted token of the first key
+        uint32_t word = t >= kWave ? 0 : (t >= 0 ? (uint32_t)(seen >> t) : (uint32_t)(seen << -t) | ((1u << -t) - 1));
+        word >>= 4 * hl;
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          if (kv0 + acc_row(e, hl) > row.limit) s[e] = -__builtin_inff();
-        return;
-      }
-      // The tile's keys that the row sees: settled ones, then its line.
-      const int t = kv0 - ctx;  // drafted token of the tile's first key
-      uint32_t word = t >= kWave ? 0 : (t >= 0 ? (uint32_t)(seen >> t) : (uint32_t)(seen << -t) | ((1u << -t) - 1));
-      word >>= 4 * hl;
+          if (!(word >> acc_row(e, 0) & 1)) s[e] = -__builtin_inff();
+      });
+    }
+  }
+  // The groups' states, the upper half's joined to the lower half's.
 #pragma unroll
-      for (int e = 0; e < 16; ++e)
-        if (!(word >> acc_row(e, 0) & 1)) s[e] = -__builtin_inff();
-    });
+  for (int half = KG / 2; half > 0; half /= 2) {
+    float4_t* x = reinterpret_cast<float4_t*>(smem) + ((kg % half) * RB + rb) * State::kGive;
+    float* y = ml + ((kg % half) * RB + rb) * State::kMl * kWave;
+    __syncthreads();
+    if (kg >= half && kg < 2 * half) st.give(x, y, lane);
+    __syncthreads();
+    if (kg < half) st.take(x, y, lane);
   }
   const float sum = pair_sum(st.l[0]);
-  if (r >= a.R) return;
+  if (kg != 0 || r >= a.R) return;
   if (whole) {
     const float inv = 1.f / sum;
     T* op = reinterpret_cast<T*>(a.o) + a.vo.row(b, hk * a.G + row.g, row.i);
@@ -157,18 +189,21 @@ __global__ __launch_bounds__(kJoinThreads) void tree_join_kernel(TreeArgs a, int
   const int bh = blockIdx.x / tiles, b = bh / a.Hk, hk = bh % a.Hk;
   const int r = blockIdx.x % tiles * rows + tid / per_row, i = r / a.G;
   const int L = min(a.Sk, max(0, a.len[b])), limit = L - a.Sq + i;
-  FewParts f;
-  f.of(a, b, tid % kWave);
-  const int np = r < a.R && limit >= 0 ? limit / f.keys + 1 : 0;
-  const int64_t first = ((int64_t)f.first * a.Hk + hk) * a.R + r, step = (int64_t)a.Hk * a.R;
+  int np = 0;
+  int64_t at = 0;  // the row's number in its first part
+  if (r < a.R && limit >= 0) {
+    np = limit / a.plan[2 * b + 1] + 1;
+    at = ((int64_t)a.plan[2 * b] * a.Hk + hk) * a.R + r;
+  }
+  const int64_t step = (int64_t)a.Hk * a.R;
   const bool on = chunk * 4 < a.Dv;
   float m = -__builtin_inff(), l = 0.f, live = 0.f;
   float4_t y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
   for (int p = set; p < np; p += sets) {
-    const float4_t x = *reinterpret_cast<const float4_t*>(a.part_ml + (first + p * step) * 4);
+    const float4_t x = *reinterpret_cast<const float4_t*>(a.part_ml + (at + p * step) * 4);
+    const float4_t o = *reinterpret_cast<const float4_t*>(a.part_o + (at + p * step) * a.Dv + (on ? chunk : 0) * 4);
     live = x[2];
-    if (live == 0.f) break;
-    const float4_t o = on ? *reinterpret_cast<const float4_t*>(a.part_o + (first + p * step) * a.Dv + chunk * 4) : y;
     const float to = fmaxf(m, x[0]);
     // An unset maximum (-inf) goes with sums that are zero, or NaN and kept.
     const float w0 = m == -__builtin_inff() ? 1.f : fast_exp2(m - to), w1 = x[0] == -__builtin_inff() ? 1.f : fast_exp2(x[0] - to);
