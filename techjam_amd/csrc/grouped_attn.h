@@ -20,12 +20,27 @@ struct View3 {
   __device__ __forceinline__ int64_t row(int64_t t, int h) const { return t * st + h * sh; }
 };
 
+// Division of row numbers (below 2^31) by the group's size, by a product: with 2^shift >= n > 2^(shift - 1)
+// and mul = ceil(2^(31 + shift) / n), x mul / 2^(31 + shift) is off by less than x / 2^31 / n.
+struct Divisor {
+  uint32_t mul;
+  int shift, n;
+  static Divisor of(int n) {
+    int shift = 0;
+    while ((int64_t(1) << shift) < n) ++shift;
+    return Divisor{uint32_t(((uint64_t(1) << (31 + shift)) + n - 1) / n), shift, n};
+  }
+};
+__device__ __forceinline__ int operator/(int x, Divisor d) { return (int)(__umulhi((uint32_t)x * 2, d.mul) >> d.shift); }
+__device__ __forceinline__ int operator%(int x, Divisor d) { return x - x / d * d.n; }
+
 struct PackedArgs {
   const void *q, *k, *v;
   void* o;
   View3 vq, vk, vv, vo;
   int T, N;                // tokens in all, sequences
   int H, Hk, G, D, Dv;
+  Divisor by_group;        // G
   float scale;
   int causal;
   const int32_t* off;      // [N + 1]
@@ -110,15 +125,16 @@ struct Region {
   // microsecond, where a launch that sorts would take several. For up to kRanked regions.
   static constexpr int kChunks = 4, kRanked = kChunks * kWave;
   __device__ __forceinline__ bool ranked(const PackedArgs& a, int at, int per, int unit, bool down, int lane) {
-    int n[kChunks], all[kChunks], count = 0, top = 0;
+    int n[kChunks], from_[kChunks], rows_[kChunks], len_[kChunks], count = 0, top = 0;
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
       const int j = c * kWave + lane;
-      n[c] = all[c] = 0;
+      n[c] = from_[c] = rows_[c] = len_[c] = 0;
       if (c * kWave < regions(a) && j < regions(a)) {
-        const int rows = max(0, edge(a, j + 1) - edge(a, j));
-        all[c] = (rows * per + unit - 1) / unit;
-        n[c] = (tokens(a, j, rows) * per + unit - 1) / unit;
+        from_[c] = edge(a, j);
+        rows_[c] = max(0, edge(a, j + 1) - from_[c]);
+        len_[c] = tokens(a, j, rows_[c]);
+        n[c] = (len_[c] * per + unit - 1) / unit;
       }
       count += n[c];
       top = max(top, n[c]);
@@ -159,7 +175,7 @@ struct Region {
         who = __ballot(has && before == rank);
         rank -= (int)__popcll(mask);
       } else {
-        int upto = all[c] - n[c];
+        int upto = (rows_[c] * per + unit - 1) / unit - n[c];
         const int own = upto;
 #pragma unroll
         for (int s = 1; s < kWave; s <<= 1) {
@@ -171,13 +187,13 @@ struct Region {
         else rank -= __builtin_amdgcn_readlane(upto, kWave - 1);
       }
       if (who != 0) {
-        const int from = __builtin_ctzll(who), tiles = __builtin_amdgcn_readlane(n[c], from);
-        index = c * kWave + from;
+        const int at = __builtin_ctzll(who), tiles = __builtin_amdgcn_readlane(n[c], at);
+        index = c * kWave + at;
         if (!live) tile += tiles;
         else if (a.causal && down) tile = tiles - 1 - tile;
-        start = __builtin_amdgcn_readfirstlane(edge(a, index));
-        rows = max(0, __builtin_amdgcn_readfirstlane(edge(a, index + 1)) - start);
-        len = __builtin_amdgcn_readfirstlane(tokens(a, index, rows));
+        start = __builtin_amdgcn_readlane(from_[c], at);
+        rows = __builtin_amdgcn_readlane(rows_[c], at);
+        len = __builtin_amdgcn_readlane(len_[c], at);
         return there(per, unit);
       }
     }
@@ -200,6 +216,7 @@ struct TreeArgs {
   int B, H, Hk, G, D, Dv;
   int Sq, Sk;              // drafted tokens, capacity of the cache
   int R;                   // rows of one key head: Sq * G
+  Divisor by_group;        // G
   float scale;
   const int32_t* len;      // [B]
   const int32_t* parents;  // [B, Sq], or null: a chain
@@ -232,157 +249,189 @@ struct SweepRow {
   bool live;
 };
 
-// The running state of a wave's NB blocks of 32 rows. Scores are formed transposed,
-// S^T = K Q^T, so that a lane holds scores of ONE row of a block: maximum and sum are
-// per lane (the other half of the wave holds the other keys), and the probabilities
-// turn into the B operand of O^T = V^T P^T where they stand. Every K and V fragment
-// read from LDS serves all NB blocks.
+// The 32 rows of a wave between memory and registers, through an LDS tile of its own. A fragment
+// holds a row's elements lane by lane, so that one instruction would touch 32 rows, 32 or
+// 16 bytes of each; through the tile it moves whole rows.
+template <typename T, int HD>
+struct WaveRows {
+  using SH = SweepShape<T, HD, 32>;
+  using Rows = typename SH::Rows;
+  static constexpr int kBytes = 32 * Rows::kRowBytes;
+  static constexpr int kPer = kWave / Rows::kChunks, N = 32 / kPer;  // rows of an instruction, instructions
+  typedef T vec_t __attribute__((ext_vector_type(Rows::kVec)));
+  template <typename V>
+  __device__ __forceinline__ static void put(uint32_t at, V x) { *(__attribute__((address_space(3))) V*)(uintptr_t)at = x; }
+
+  // The lane's chunks of the rows; row(n): a pointer to row n's elements, or null where it is not there.
+  template <typename F>
+  __device__ __forceinline__ static void read(vec_t x[N], int width, int lane, F&& row) {
+    const int col = lane % Rows::kChunks * Rows::kVec;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const T* p = row(n * kPer + lane / Rows::kChunks);
+#pragma unroll
+      for (int j = 0; j < Rows::kVec; ++j) x[n][j] = (T)0.f;
+      if (p != nullptr && col < width) x[n] = *reinterpret_cast<const vec_t*>(p + col);
+    }
+  }
+  // They, as the wave's fragments.
+  __device__ __forceinline__ static void turn(const vec_t x[N], uint32_t tile, int lane, frag_t<T> f[SH::KS]) {
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int r = n * kPer + lane / Rows::kChunks;
+      put(tile + r * Rows::kRowBytes + (((lane % Rows::kChunks) ^ Rows::swizzle(r)) << 4), x[n]);
+    }
+    wait_lds();
+    const uint32_t base = tile + Rows::lane_row(lane);
+#pragma unroll
+    for (int ks = 0; ks < SH::KS; ++ks) f[ks] = Rows::row_frag(base, ks, 0);
+  }
+
+  // Accumulators of a transposed product to rows of memory: value(d, c): the four values of the lane's row from
+  // column 32 d + 8 c + 4 (lane / 32) on.
+  template <typename V, typename F>
+  __device__ __forceinline__ static void write(uint32_t tile, int width, int lane, V&& value, F&& row) {
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    const int r = lane % 32;
+#pragma unroll
+    for (int d = 0; d < SH::DB; ++d)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float4_t y = value(d, c);
+        const int col = 32 * d + 8 * c + 4 * (lane / 32);
+        put(tile + r * Rows::kRowBytes + (((col / Rows::kVec) ^ Rows::swizzle(r)) << 4) + (col % Rows::kVec) * (int)sizeof(T),
+            t4{(T)y[0], (T)y[1], (T)y[2], (T)y[3]});
+      }
+    wait_lds();
+    const int col = lane % Rows::kChunks * Rows::kVec;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const int r = n * kPer + lane / Rows::kChunks;
+      const vec_t x = lds_at<vec_t>(tile + r * Rows::kRowBytes + (((lane % Rows::kChunks) ^ Rows::swizzle(r)) << 4));
+      T* p = row(r);
+      if (p != nullptr && col < width) *reinterpret_cast<vec_t*>(p + col) = x;
+    }
+  }
+};
+
+// The running state of a wave's 32 rows. Scores are formed transposed, S^T = K Q^T,
+// so that a lane holds scores of ONE row: maximum and sum are per lane (the other
+// half of the wave holds the other keys), and the probabilities turn into the B
+// operand of O^T = V^T P^T where they stand. (Two blocks of 32 rows a wave read every fragment from LDS
+// half as often, but leave a SIMD one wave of 400 registers, whose products and exponentials take turns:
+// 1310 us instead of 857 for two sequences of 1904 and 14480 tokens, 16 heads on 8, 128 dims, bf16.)
 //
 // The output is divided by the sum of the probabilities as they were rounded for its
 // product (to the inputs' type: fp32 MFMAs would take 16 times as long): a dominant
 // key's rounding cancels, and two go into one instruction. What the backward pass
 // gets (STATS) is the sum of the unrounded ones, so that its P sums to 1 as exactly
 // as fp32 does.
-template <typename T, int HD, int BN, int NB, bool STATS>
+template <typename T, int HD, int BN, bool STATS>
 struct SweepState {
   using SH = SweepShape<T, HD, BN>;
-  frag_t<T> q[NB][SH::KS];
-  float16_t o[NB][SH::DB];
-  float m[NB], l[NB];  // maximum in log2 units, the lane's part of the sum
-  float e[STATS ? NB : 1];
+  frag_t<T> q[SH::KS];
+  float16_t o[SH::DB];
+  float m, l;          // maximum in log2 units, the lane's part of the sum
+  float e;             // of the unrounded ones
   float c2;            // |scale| log2 e
   uint32_t kbase, vbase;  // the lane's places in a tile
 
+  // With q's rows as they are in memory.
   __device__ __forceinline__ void init(float scale, int lane) {
     kbase = SH::Rows::lane_row(lane);
     vbase = SH::Rows::lane_col(lane) + SH::kTensor;
     // A negative scale turns q's sign, so that the largest score is the largest
     // product; a zero one becomes too small to matter, so that masked stays -inf.
     c2 = fmaxf(fabsf(scale) * kLog2e, 1e-37f);
+    if (scale < 0.f)
 #pragma unroll
-    for (int n = 0; n < NB; ++n) {
-      m[n] = -__builtin_inff();
-      l[n] = 0.f;
-      if constexpr (STATS) e[n] = 0.f;
+      for (int ks = 0; ks < SH::KS; ++ks)
 #pragma unroll
-      for (int d = 0; d < SH::DB; ++d) o[n][d] = zero16();
-    }
-  }
-  // Block n's rows of q; null: a row that is not there.
-  __device__ __forceinline__ void load_q(int n, const T* p, float scale, int width, int lane) {
+        for (int j = 0; j < 8; ++j) q[ks][j] = -q[ks][j];
+    m = -__builtin_inff();
+    l = e = 0.f;
 #pragma unroll
-    for (int ks = 0; ks < SH::KS; ++ks) {
-      q[n][ks] = load_frag<T>(p, 16 * ks + 8 * (lane / 32), width);
-      if (scale < 0.f)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) q[n][ks][j] = -q[n][ks][j];
-    }
+    for (int d = 0; d < SH::DB; ++d) o[d] = zero16();
   }
 
-  // 32 keys of a tile, from its key 32 kb on. mask(n, s): sets block n's scores of keys that the
-  // lane's row does not see to -inf.
+  // 32 keys of a tile, from its key 32 kb on. mask(s): sets the scores of keys that the lane's
+  // row does not see to -inf.
   template <typename Mask>
   __device__ __forceinline__ void step(uint32_t tile, int kb, Mask&& mask) {
     const uint32_t kt = tile + kbase, vt = tile + vbase;
-    frag_t<T> p[NB][2];
-    float16_t s[NB];
-#pragma unroll
-    for (int n = 0; n < NB; ++n) s[n] = zero16();
+    float16_t s = zero16();
     read_ahead<SH::KS, SH::kDepth>([&](int ks) { return SH::Rows::row_frag(kt, ks, kb * 32 * SH::Rows::kRowBytes); },
-                                   [&](int ks, frag_t<T> f) {
+                                   [&](int ks, frag_t<T> f) { s = Elem<T>::mma(f, q[ks], s); });
+    mask(s);
+    float top = s[0];
 #pragma unroll
-                                     for (int n = 0; n < NB; ++n) s[n] = Elem<T>::mma(f, q[n][ks], s[n]);
-                                   });
+    for (int r = 1; r < 16; ++r) top = fmaxf(top, s[r]);
+    top = pair_max(top) * c2;
+    // The maximum moves by the row's need; one decision for the wave.
+    const bool move = top > m + kLazy;  // also from -inf
+    if (__any(move)) {
+      const float to = move ? top : m;
+      const float alpha = m == -__builtin_inff() ? 0.f : fast_exp2(m - to);
+      m = to;
+      l *= alpha;
+      if constexpr (STATS) e *= alpha;
 #pragma unroll
-    for (int n = 0; n < NB; ++n) {
-      mask(n, s[n]);
-      float top = s[n][0];
+      for (int d = 0; d < SH::DB; ++d)
 #pragma unroll
-      for (int r = 1; r < 16; ++r) top = fmaxf(top, s[n][r]);
-      top = pair_max(top) * c2;
-      // The maximum moves by the row's need; one decision for the wave.
-      const bool move = top > m[n] + kLazy;  // also from -inf
-      if (__any(move)) {
-        const float to = move ? top : m[n];
-        const float alpha = m[n] == -__builtin_inff() ? 0.f : fast_exp2(m[n] - to);
-        m[n] = to;
-        l[n] *= alpha;
-        if constexpr (STATS) e[n] *= alpha;
+        for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
+    }
+    // A row that has seen no key keeps its unset maximum out of the exponent.
+    const float off = m == -__builtin_inff() ? 0.f : Elem<T>::kLift - m;
 #pragma unroll
-        for (int d = 0; d < SH::DB; ++d)
+    for (int r = 0; r < 16; ++r) {
+      s[r] = fast_exp2(fmaf(s[r], c2, off));
+      if constexpr (STATS) e += s[r];
+    }
+    frag_t<T> p[2];
 #pragma unroll
-          for (int r = 0; r < 16; ++r) o[n][d][r] *= alpha;
-      }
-      // A row that has seen no key keeps its unset maximum out of the exponent.
-      const float off = m[n] == -__builtin_inff() ? 0.f : Elem<T>::kLift - m[n];
-#pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        s[n][r] = fast_exp2(fmaf(s[n][r], c2, off));
-        if constexpr (STATS) e[n] += s[n][r];
-      }
-#pragma unroll
-      for (int st = 0; st < 2; ++st) {
-        p[n][st] = acc_frag<T>(s[n], st);
-        l[n] = frag_sum(p[n][st], l[n]);
-      }
+    for (int st = 0; st < 2; ++st) {
+      p[st] = acc_frag<T>(s, st);
+      l = frag_sum(p[st], l);
     }
     read_ahead<2 * SH::DB, SH::kDepth>(
         [&](int j) { return SH::Rows::col_frag(vt, j % SH::DB, (kb * 32 + 16 * (j / SH::DB)) * SH::Rows::kRowBytes); },
-        [&](int j, frag_t<T> f) {
-#pragma unroll
-          for (int n = 0; n < NB; ++n) o[n][j % SH::DB] = Elem<T>::mma(f, p[n][j / SH::DB], o[n][j % SH::DB]);
-        });
+        [&](int j, frag_t<T> f) { o[j % SH::DB] = Elem<T>::mma(f, p[j / SH::DB], o[j % SH::DB]); });
   }
 
   // Adds the state of another wave over the same rows and other keys, which that wave has left
   // in LDS (give).
-  static constexpr int kGive = SH::DB * 4 * kWave;  // float4 per block
-  static constexpr int kMl = STATS ? 3 : 2;         // numbers of a lane and block beside them
+  static constexpr int kGive = SH::DB * 4 * kWave;  // float4
+  static constexpr int kMl = STATS ? 3 : 2;         // numbers of a lane beside them
   __device__ __forceinline__ void give(float4_t* x, float* ml, int lane) {
+    ml[lane] = m;
+    ml[kWave + lane] = l;
+    if constexpr (STATS) ml[2 * kWave + lane] = e;
 #pragma unroll
-    for (int n = 0; n < NB; ++n) {
-      ml[(kMl * n) * kWave + lane] = m[n];
-      ml[(kMl * n + 1) * kWave + lane] = l[n];
-      if constexpr (STATS) ml[(kMl * n + 2) * kWave + lane] = e[n];
+    for (int d = 0; d < SH::DB; ++d)
 #pragma unroll
-      for (int d = 0; d < SH::DB; ++d)
-#pragma unroll
-        for (int c = 0; c < 4; ++c)
-          x[n * kGive + (d * 4 + c) * kWave + lane] =
-              float4_t{o[n][d][4 * c], o[n][d][4 * c + 1], o[n][d][4 * c + 2], o[n][d][4 * c + 3]};
-    }
+      for (int c = 0; c < 4; ++c) x[(d * 4 + c) * kWave + lane] = four(d, c);
   }
   __device__ __forceinline__ void take(const float4_t* x, const float* ml, int lane) {
-#pragma unroll
-    for (int n = 0; n < NB; ++n) {
-      const float m1 = ml[(kMl * n) * kWave + lane], to = fmaxf(m[n], m1);
-      // An unset maximum (-inf) goes with sums that are zero, or NaN and kept.
-      const float w0 = m[n] == -__builtin_inff() ? 1.f : fast_exp2(m[n] - to);
-      const float w1 = m1 == -__builtin_inff() ? 1.f : fast_exp2(m1 - to);
-      m[n] = to;
-      l[n] = fmaf(l[n], w0, ml[(kMl * n + 1) * kWave + lane] * w1);
-      if constexpr (STATS) e[n] = fmaf(e[n], w0, ml[(kMl * n + 2) * kWave + lane] * w1);
-#pragma unroll
-      for (int d = 0; d < SH::DB; ++d)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const float4_t y = x[n * kGive + (d * 4 + c) * kWave + lane];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) o[n][d][4 * c + j] = fmaf(o[n][d][4 * c + j], w0, y[j] * w1);
-        }
-    }
-  }
-
-  // f(column, four values of block n's row from that column on), for the columns below `width`.
-  template <typename F>
-  __device__ __forceinline__ void columns(int n, int width, int lane, F&& f) const {
+    const float m1 = ml[lane], to = fmaxf(m, m1);
+    // An unset maximum (-inf) goes with sums that are zero, or NaN and kept.
+    const float w0 = m == -__builtin_inff() ? 1.f : fast_exp2(m - to);
+    const float w1 = m1 == -__builtin_inff() ? 1.f : fast_exp2(m1 - to);
+    m = to;
+    l = fmaf(l, w0, ml[kWave + lane] * w1);
+    if constexpr (STATS) e = fmaf(e, w0, ml[2 * kWave + lane] * w1);
 #pragma unroll
     for (int d = 0; d < SH::DB; ++d)
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        const int col = 32 * d + 8 * c + 4 * (lane / 32);
-        if (col < width) f(col, float4_t{o[n][d][4 * c], o[n][d][4 * c + 1], o[n][d][4 * c + 2], o[n][d][4 * c + 3]});
+        const float4_t y = x[(d * 4 + c) * kWave + lane];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[d][4 * c + j] = fmaf(o[d][4 * c + j], w0, y[j] * w1);
       }
+  }
+
+  // The lane's four values from column 32 d + 8 c + 4 (lane / 32) on.
+  __device__ __forceinline__ float4_t four(int d, int c) const {
+    return float4_t{o[d][4 * c], o[d][4 * c + 1], o[d][4 * c + 2], o[d][4 * c + 3]};
   }
 };
 

@@ -46,7 +46,7 @@ PackedArgs packed_args(const void* q, const void* k, const void* v, int64_t T, i
   PackedArgs a{};
   a.q = q; a.k = k; a.v = v;
   a.vq = View3{qs[0], qs[1]}; a.vk = View3{ks[0], ks[1]}; a.vv = View3{vs[0], vs[1]}; a.vo = View3{os[0], os[1]};
-  a.T = (int)T; a.N = (int)N; a.H = (int)H; a.Hk = (int)Hk; a.G = (int)(H / Hk); a.D = (int)D; a.Dv = (int)Dv;
+  a.T = (int)T; a.N = (int)N; a.H = (int)H; a.Hk = (int)Hk; a.G = (int)(H / Hk); a.by_group = Divisor::of(a.G); a.D = (int)D; a.Dv = (int)Dv;
   a.scale = scale; a.causal = causal != 0; a.off = offsets; a.len = lengths;
   return a;
 }
@@ -67,7 +67,7 @@ bool tree_sizes_ok(int64_t B, int64_t H, int64_t Hk, int64_t Sq, int64_t Sk) {
 
 TreeArgs tree_sizes(int64_t B, int64_t H, int64_t Hk, int64_t Sq, int64_t Sk, int64_t D, int64_t Dv) {
   TreeArgs a{};
-  a.B = (int)B; a.H = (int)H; a.Hk = (int)Hk; a.G = (int)(H / Hk); a.D = (int)D; a.Dv = (int)Dv;
+  a.B = (int)B; a.H = (int)H; a.Hk = (int)Hk; a.G = (int)(H / Hk); a.by_group = Divisor::of(a.G); a.D = (int)D; a.Dv = (int)Dv;
   a.Sq = (int)Sq; a.Sk = (int)Sk; a.R = (int)(Sq * a.G);
   return a;
 }

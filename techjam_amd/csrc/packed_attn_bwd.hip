@@ -91,7 +91,7 @@ __global__ __launch_bounds__(kThreads) void packed_peak_kernel(PackedArgs a, int
   float peak[2] = {0.f, 0.f};
   for (int r = tid / lpr; r < tokens * a.G; r += per_block)
     peak[0] = fmaxf(peak[0], norm2(reinterpret_cast<const half_t*>(a.dout) +
-                                   a.vdo.row(g.start + first + r / a.G, hk * a.G + r % a.G)));
+                                   a.vdo.row(g.start + first + r / a.by_group, hk * a.G + r % a.by_group)));
   for (int j = tid / lpr; j < tokens; j += per_block)
     peak[1] = fmaxf(peak[1], norm2(reinterpret_cast<const half_t*>(a.v) + a.vv.row(g.start + first + j, hk)));
 #pragma unroll
@@ -112,36 +112,42 @@ __device__ __forceinline__ float* stat_at(const PackedArgs& a, const Region& g, 
   return a.stat + (((int64_t)Region::slot(g.start, g.index, 1, 32) + i / 32) * a.H + head) * 64 + i % 32;
 }
 
-// A workgroup = RB waves of NB blocks of 32 rows times KG groups, keys through LDS in
+// A workgroup = RB waves of 32 rows times KG groups, keys through LDS in
 // tiles of 32 dealt to the groups in turn, whose sums meet in LDS at the end. Scores
 // transposed as in the forward kernel: a row's sums are its lane's own numbers, and
 // dS turns into the B operand of dQ^T = K^T dS^T.
-template <typename T, int HD, int BLOCKS, int NBT>
+template <typename T, int HD, int BLOCKS>
 struct QShape {
-  static constexpr int NB = NBT, RB = BLOCKS, KG = 4 / RB, ROWS = 32 * RB * NB;
+  static constexpr int RB = BLOCKS, KG = 4 / RB, ROWS = 32 * RB;
   using SH = SweepShape<T, HD, 32>;
+  using Wave = WaveRows<T, HD>;
+  // Two tiles a group, afterwards the groups' sums. The rows come through the second tile while the first keys are on
+  // their way, or through a place of their own where it has no room for them.
+  static constexpr int kTiles = KG * 2 * SH::kBytes, kSums = KG > 1 ? KG / 2 * RB * SH::DB * 16 * kWave * 4 : 0;
+  static constexpr bool kOwn = RB * Wave::kBytes > SH::kBytes;
+  static constexpr int kWithRows = kTiles + (kOwn ? RB * Wave::kBytes : 0), kBytes = kWithRows > kSums ? kWithRows : kSums;
+  static_assert(!kOwn || KG == 1, "places are one group's");
 };
 template <typename T, int HD>
 constexpr bool groups_fit(int groups) { return groups * SweepShape<T, HD, 32>::W * (int)sizeof(T) <= 1024; }
 
-template <typename T, int HD, int BLOCKS, int NB>
+template <typename T, int HD, int BLOCKS>
 __global__ __launch_bounds__(kThreads, (HD * (int)sizeof(T) <= 256 ? 2 : 1)) void packed_bwd_q_kernel(PackedArgs a) {
-  using QS = QShape<T, HD, BLOCKS, NB>;
+  using QS = QShape<T, HD, BLOCKS>;
   using SH = typename QS::SH;
+  using Wave = typename QS::Wave;
   using Rows = typename SH::Rows;
   constexpr int KS = SH::KS, DB = SH::DB, BN = 32, RB = QS::RB, KG = QS::KG, ROWS = QS::ROWS, kDepth = SH::kDepth;
-  constexpr int kSums = KG > 1 ? KG / 2 * RB * NB * DB * 16 * kWave * 4 : 0;
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[KG * 2 * SH::kBytes > kSums ? KG * 2 * SH::kBytes : kSums];
-  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave, hl = lane / 32,
-            ln = lane % 32;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[QS::kBytes];
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave, hl = lane / 32;
   const int kg = w / RB, rb = w % RB, hk = blockIdx.x % a.Hk;
   Region g;
   if (!g.take(a, blockIdx.x / a.Hk, a.G, ROWS, false, lane)) return;
-  const int L = g.len, R = g.rows * a.G, r0 = g.tile * ROWS, rw0 = r0 + 32 * NB * rb;
+  const int L = g.len, R = g.rows * a.G, r0 = g.tile * ROWS, rw0 = r0 + 32 * rb;
   auto span = [&](int row, int last) {
-    return row >= R || row / a.G >= L ? 0 : (a.causal ? min(L, min(last, R - 1) / a.G + 1) : L);
+    return row >= R || row / a.by_group >= L ? 0 : (a.causal ? min(L, min(last, R - 1) / a.by_group + 1) : L);
   };
-  const int kv_end = span(r0, r0 + ROWS - 1), own_end = span(rw0, rw0 + 32 * NB - 1);
+  const int kv_end = span(r0, r0 + ROWS - 1), own_end = span(rw0, rw0 + 31);
   const uint32_t tiles = lds_offset(smem) + kg * 2 * SH::kBytes;
   const uint32_t krow = Rows::lane_row(lane), kcol = Rows::lane_col(lane), vrow = krow + SH::kTensor;
   SweepTiles<T, SH, RB> keys;
@@ -150,47 +156,57 @@ __global__ __launch_bounds__(kThreads, (HD * (int)sizeof(T) <= 256 ? 2 : 1)) voi
   int kv0 = BN * kg;
   if (kv0 < kv_end) keys.issue(kv0, L, tiles, rb);
 
-  const DsLift<T> lifts(a, g, hk, lane);
-  const float c2 = a.scale * kLog2e;
-  SweepRow row[NB];
-  int free[NB];
-  frag_t<T> qf[NB][KS], of[NB][KS];
-  float lse[NB], del[NB], lift[NB];
-  float16_t dq[NB][DB];
+  const int r = rw0 + lane % 32;
+  SweepRow row{r, r / a.by_group, r % a.by_group, 0, r < R && r / a.by_group < L};
+  row.limit = a.causal ? row.i : L - 1;
+  const int free = a.causal ? rw0 / a.by_group : L - 1;  // the last key that all of the wave's rows see
+  frag_t<T> qf[KS], of[KS];
+  float sum = 0.f, norm = 0.f;
+  {
+    typename Wave::vec_t xq[Wave::N], xo[Wave::N], xy[Wave::N], xz[Wave::N];
+    auto rows = [&](const void* p, const View3& v) {
+      return [&, p](int n) -> const T* {
+        const int r = rw0 + n, i = r / a.by_group;
+        return r < R && i < L ? reinterpret_cast<const T*>(p) + v.row(g.start + i, hk * a.G + r - i * a.G) : nullptr;
+      };
+    };
+    Wave::read(xq, a.D, lane, rows(a.q, a.vq));
+    Wave::read(xo, a.Dv, lane, rows(a.dout, a.vdo));
+    Wave::read(xy, a.Dv, lane, rows(a.out, a.vo));
+    if constexpr (sizeof(T) == 2) Wave::read(xz, a.Dv, lane, rows(a.rest, a.vo));
+    const uint32_t turn = QS::kOwn ? lds_offset(smem) + QS::kTiles + rb * Wave::kBytes : tiles + SH::kBytes + rb * Wave::kBytes;
+    frag_t<T> y[KS];
+    auto dot = [&] {
 #pragma unroll
-  for (int n = 0; n < NB; ++n) {
-    const int first = rw0 + 32 * n, r = first + ln;
-    row[n] = SweepRow{r, r / a.G, r % a.G, 0, r < R && r / a.G < L};
-    row[n].limit = a.causal ? row[n].i : L - 1;
-    free[n] = a.causal ? first / a.G : L - 1;
-    const int64_t token = g.start + row[n].i;
-    const int head = hk * a.G + row[n].g;
-    const T* qp = reinterpret_cast<const T*>(a.q) + a.vq.row(token, head);
-    const T* op = reinterpret_cast<const T*>(a.dout) + a.vdo.row(token, head);
-    const int64_t at = a.vo.row(token, head);
-    float sum = 0.f, norm = 0.f;
+      for (int s = 0; s < KS; ++s)
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      qf[n][s] = load_frag<T>(row[n].live ? qp : nullptr, 16 * s + 8 * hl, a.D);
-      of[n][s] = load_frag<T>(row[n].live ? op : nullptr, 16 * s + 8 * hl, a.Dv);
-      const frag_t<T> y = load_frag<T>(row[n].live ? reinterpret_cast<const T*>(a.out) + at : nullptr, 16 * s + 8 * hl, a.Dv);
-      frag_t<T> z;
-      if constexpr (sizeof(T) == 2)
-        z = load_frag<T>(row[n].live ? reinterpret_cast<const T*>(a.rest) + at : nullptr, 16 * s + 8 * hl, a.Dv);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        sum = fmaf((float)of[n][s][j], (float)y[j] + (sizeof(T) == 2 ? (float)z[j] : 0.f), sum);
-        if constexpr (DsLift<T>::kOn) norm = fmaf((float)of[n][s][j], (float)of[n][s][j], norm);
-      }
+        for (int j = 0; j < 8; ++j) sum = fmaf((float)of[s][j], (float)y[s][j], sum);
+    };
+    Wave::turn(xq, turn, lane, qf);
+    Wave::turn(xo, turn, lane, of);
+    Wave::turn(xy, turn, lane, y);
+    dot();
+    if constexpr (sizeof(T) == 2) {
+      Wave::turn(xz, turn, lane, y);
+      dot();
     }
-    del[n] = pair_sum(sum);
-    lse[n] = row[n].live ? a.lse[token * a.H + head] : __builtin_inff();
-    // The row's own lift: its lane (and the one of the other half) has all of its dO.
-    lift[n] = DsLift<T>::kOn ? lifts.of(sqrtf(pair_sum(norm))) : 1.f;
-#pragma unroll
-    for (int d = 0; d < DB; ++d) dq[n][d] = zero16();
   }
-  const float common = lifts.all() / DsLift<T>::kP;
+  const float del = pair_sum(sum);
+  const float lse = row.live ? a.lse[(int64_t)(g.start + row.i) * a.H + hk * a.G + row.g] : __builtin_inff();
+  // The row's own lift: its lane (and the one of the other half) has all of its dO.
+  const DsLift<T> lifts(a, g, hk, lane);
+  float lift = 1.f;
+  if constexpr (DsLift<T>::kOn) {
+#pragma unroll
+    for (int s = 0; s < KS; ++s)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) norm = fmaf((float)of[s][j], (float)of[s][j], norm);
+    lift = lifts.of(sqrtf(pair_sum(norm)));
+  }
+  const float common = lifts.all() / DsLift<T>::kP, c2 = a.scale * kLog2e, d0 = -del * lift;
+  float16_t dq[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d) dq[d] = zero16();
 
   // The workgroup goes round together, the last round maybe without a tile for every group.
   for (int first = 0, cur = 0; first < kv_end; first += KG * BN, kv0 += KG * BN, cur ^= 1) {
@@ -199,121 +215,96 @@ __global__ __launch_bounds__(kThreads, (HD * (int)sizeof(T) <= 256 ? 2 : 1)) voi
     if (kv0 + KG * BN < kv_end) keys.issue(kv0 + KG * BN, L, tiles + (cur ^ 1) * SH::kBytes, rb);
     if (kv0 >= own_end) continue;
     const uint32_t tile = tiles + cur * SH::kBytes;
-    float16_t p[NB], dp[NB];
-#pragma unroll
-    for (int n = 0; n < NB; ++n) p[n] = dp[n] = zero16();
+    float16_t p = zero16(), dp = zero16();
     read_ahead<KS, kDepth>([&](int s) { return Rows::row_frag(tile + krow, s, 0); },
-                           [&](int s, frag_t<T> f) {
-#pragma unroll
-                             for (int n = 0; n < NB; ++n) p[n] = Elem<T>::mma(f, qf[n][s], p[n]);
-                           });
+                           [&](int s, frag_t<T> f) { p = Elem<T>::mma(f, qf[s], p); });
     read_ahead<KS, kDepth>([&](int s) { return Rows::row_frag(tile + vrow, s, 0); },
-                           [&](int s, frag_t<T> f) {
+                           [&](int s, frag_t<T> f) { dp = Elem<T>::mma(f, of[s], dp); });
 #pragma unroll
-                             for (int n = 0; n < NB; ++n) dp[n] = Elem<T>::mma(f, of[n][s], dp[n]);
-                           });
-    frag_t<T> fs[NB][2];
+    for (int e = 0; e < 16; ++e) p[e] = fast_exp2(fmaf(p[e], c2, -lse)) * fmaf(dp[e], lift, d0);
+    // Selected, not multiplied: what a masked key holds does not matter.
+    if (kv0 + BN - 1 > free) {
 #pragma unroll
-    for (int n = 0; n < NB; ++n) {
-      const float d0 = -del[n] * lift[n];
-#pragma unroll
-      for (int e = 0; e < 16; ++e) p[n][e] = fast_exp2(fmaf(p[n][e], c2, -lse[n])) * fmaf(dp[n][e], lift[n], d0);
-      // Selected, not multiplied: what a masked key holds does not matter.
-      if (kv0 + BN - 1 > free[n]) {
-#pragma unroll
-        for (int e = 0; e < 16; ++e)
-          if (kv0 + acc_row(e, hl) > row[n].limit) p[n][e] = 0.f;
-      }
-#pragma unroll
-      for (int s = 0; s < 2; ++s) fs[n][s] = acc_frag<T>(p[n], s);
+      for (int e = 0; e < 16; ++e)
+        if (kv0 + acc_row(e, hl) > row.limit) p[e] = 0.f;
     }
+    frag_t<T> fs[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) fs[s] = acc_frag<T>(p, s);
     if constexpr (kDepth > 0) __builtin_amdgcn_sched_barrier(0);
     read_ahead<2 * DB, kDepth>([&](int j) { return Rows::col_frag(tile + kcol, j % DB, 16 * (j / DB) * Rows::kRowBytes); },
-                               [&](int j, frag_t<T> f) {
-#pragma unroll
-                                 for (int n = 0; n < NB; ++n) dq[n][j % DB] = Elem<T>::mma(f, fs[n][j / DB], dq[n][j % DB]);
-                               });
+                               [&](int j, frag_t<T> f) { dq[j % DB] = Elem<T>::mma(f, fs[j / DB], dq[j % DB]); });
   }
 
   // The groups' sums, the upper half's added to the lower half's.
 #pragma unroll
   for (int half = KG / 2; half > 0; half /= 2) {
-    float4_t* x = reinterpret_cast<float4_t*>(smem) + ((kg % half) * RB + rb) * NB * DB * 4 * kWave;
+    float4_t* x = reinterpret_cast<float4_t*>(smem) + ((kg % half) * RB + rb) * DB * 4 * kWave + lane;
     __syncthreads();
     if (kg >= half && kg < 2 * half) {
 #pragma unroll
-      for (int n = 0; n < NB; ++n)
+      for (int d = 0; d < DB; ++d)
 #pragma unroll
-        for (int d = 0; d < DB; ++d)
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            x[((n * DB + d) * 4 + e) * kWave + lane] =
-                float4_t{dq[n][d][4 * e], dq[n][d][4 * e + 1], dq[n][d][4 * e + 2], dq[n][d][4 * e + 3]};
+        for (int e = 0; e < 4; ++e)
+          x[(d * 4 + e) * kWave] = float4_t{dq[d][4 * e], dq[d][4 * e + 1], dq[d][4 * e + 2], dq[d][4 * e + 3]};
     }
     __syncthreads();
     if (kg < half) {
 #pragma unroll
-      for (int n = 0; n < NB; ++n)
+      for (int d = 0; d < DB; ++d)
 #pragma unroll
-        for (int d = 0; d < DB; ++d)
+        for (int e = 0; e < 4; ++e) {
+          const float4_t z = x[(d * 4 + e) * kWave];
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float4_t z = x[((n * DB + d) * 4 + e) * kWave + lane];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) dq[n][d][4 * e + j] += z[j];
-          }
+          for (int j = 0; j < 4; ++j) dq[d][4 * e + j] += z[j];
+        }
     }
   }
+  __syncthreads();  // the tiles, in whose place the rows are turned, have been read
   if (kg != 0) return;
 
-#pragma unroll
-  for (int n = 0; n < NB; ++n) {
-    if (row[n].r >= R) continue;
-    const int head = hk * a.G + row[n].g;
-    if (row[n].live && hl == 0) {
-      float* st = stat_at(a, g, head, row[n].i);
-      st[0] = DsLift<T>::kLogP - lse[n];
-      st[32] = -del[n] * common;
-    }
-    const float out = a.scale / lift[n];
-    T* p = reinterpret_cast<T*>(a.dq) + a.vdq.row(g.start + row[n].i, head);
-#pragma unroll
-    for (int d = 0; d < DB; ++d)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int col = 32 * d + 8 * e + 4 * hl;
-        float y[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) y[j] = row[n].live ? dq[n][d][4 * e + j] * out : 0.f;
-        if (col < a.D) store4t<T>(p + col, y[0], y[1], y[2], y[3]);
-      }
+  if (row.live && hl == 0) {
+    float* st = stat_at(a, g, hk * a.G + row.g, row.i);
+    st[0] = DsLift<T>::kLogP - lse;
+    st[32] = -del * common;
   }
+  const float out = a.scale / lift;
+  Wave::write(lds_offset(smem) + rb * Wave::kBytes, a.D, lane,
+              [&](int d, int c) {
+                float4_t y = {0.f, 0.f, 0.f, 0.f};
+                if (row.live) y = float4_t{dq[d][4 * c], dq[d][4 * c + 1], dq[d][4 * c + 2], dq[d][4 * c + 3]} * out;
+                return y;
+              },
+              [&](int n) -> T* {
+                const int r = rw0 + n, i = r / a.by_group;
+                return r < R ? reinterpret_cast<T*>(a.dq) + a.vdq.row(g.start + i, hk * a.G + r - i * a.G) : nullptr;
+              });
 }
 
-// A workgroup = KB waves of NB blocks of 32 keys of one (sequence, key head) times RG
+// A workgroup = KB waves of 32 keys of one (sequence, key head) times RG
 // groups of token tiles: the tiles of 32 tokens that see the keys, of one query
 // head of the group after the other, are dealt to the groups in turn, and the
 // groups' sums meet in LDS at the end. Scores are formed with tokens in the
 // registers and keys over the lanes, so that P and dS turn into the A operands of dV
 // and dK where they stand; Q and dO come back as B operands through the transposing
 // LDS read.
-template <typename T, int HD, int BLOCKS, int GROUPS, int NBT>
+template <typename T, int HD, int BLOCKS, int GROUPS>
 struct KvShape {
   using SH = SweepShape<T, HD, 32>;
-  static constexpr int KB = BLOCKS, RG = GROUPS, NB = NBT, WAVES = KB * RG, KEYS = 32 * NB * KB;
+  static constexpr int KB = BLOCKS, RG = GROUPS, WAVES = KB * RG, KEYS = 32 * KB;
   static constexpr int kDepth = HD == 32 ? 0 : sizeof(T) == 2 ? 2 : 1;
   // Waves of a SIMD, by the registers.
   static constexpr int kMin = sizeof(T) == 2 ? (HD <= 64 && KB > 1 ? 3 : 2) : (HD == 32 ? 2 : 1);
 };
 
-template <typename T, int HD, int BLOCKS, int GROUPS, int NB>
-__global__ __launch_bounds__((64 * BLOCKS * GROUPS), (KvShape<T, HD, BLOCKS, GROUPS, NB>::kMin)) void
+template <typename T, int HD, int BLOCKS, int GROUPS>
+__global__ __launch_bounds__((64 * BLOCKS * GROUPS), (KvShape<T, HD, BLOCKS, GROUPS>::kMin)) void
 packed_bwd_kv_kernel(PackedArgs a) {
-  using KV = KvShape<T, HD, BLOCKS, GROUPS, NB>;
+  using KV = KvShape<T, HD, BLOCKS, GROUPS>;
   using SH = typename KV::SH;
   using Rows = typename SH::Rows;
   constexpr int KS = SH::KS, DB = SH::DB, BM = 32, KB = KV::KB, RG = KV::RG, kDepth = KV::kDepth;
-  constexpr int kSums = RG / 2 * KB * NB * 2 * DB * 16 * kWave * 4;
+  constexpr int kSums = RG / 2 * KB * 2 * DB * 16 * kWave * 4;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[RG * 2 * SH::kBytes > kSums ? RG * 2 * SH::kBytes : kSums];  // Q's tile, then dO's
   __shared__ __attribute__((aligned(1024))) float stat[RG][2][64];  // of a tile's tokens
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave, hl = lane / 32,
@@ -321,7 +312,7 @@ packed_bwd_kv_kernel(PackedArgs a) {
   const int kb = w % KB, rg = w / KB, hk = blockIdx.x % a.Hk;
   Region g;
   if (!g.take(a, blockIdx.x / a.Hk, 1, KV::KEYS, true, lane)) return;
-  const int L = g.len, k0 = g.tile * KV::KEYS, kw0 = k0 + 32 * NB * kb;
+  const int L = g.len, k0 = g.tile * KV::KEYS, kw0 = k0 + 32 * kb, key = kw0 + ln;
 
   // The group's KB waves bring its tiles.
   SweepTiles<T, SH, KB> rows;
@@ -350,28 +341,31 @@ packed_bwd_kv_kernel(PackedArgs a) {
     if (kb == 0) copy_4(make_rsrc(stat_at(a, g, hk * a.G + h, i0), 256), stat0 + buf * 256, 4 * lane);
   };
 
-  frag_t<T> kf[NB][KS], vf[NB][KS];
-  float16_t dv[NB][DB], dk[NB][DB];
-#pragma unroll
-  for (int n = 0; n < NB; ++n) {
-    const int key = kw0 + 32 * n + ln;
-    const T* kp = reinterpret_cast<const T*>(a.k) + a.vk.row(g.start + key, hk);
-    const T* vp = reinterpret_cast<const T*>(a.v) + a.vv.row(g.start + key, hk);
-#pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      kf[n][s] = load_frag<T>(key < L ? kp : nullptr, 16 * s + 8 * hl, a.D);
-      vf[n][s] = load_frag<T>(key < L ? vp : nullptr, 16 * s + 8 * hl, a.Dv);
-    }
-#pragma unroll
-    for (int d = 0; d < DB; ++d) dv[n][d] = dk[n][d] = zero16();
-  }
-
-  const float dl = DsLift<T>(a, g, hk, lane).all(), lift = dl / DsLift<T>::kP, c2 = a.scale * kLog2e;
   int h = 0, i0 = i_begin;  // this round's tile
   if (rg < n_end) {
     advance(h, i0, rg);
     issue(h, i0, 0);
   }
+  frag_t<T> kf[KS], vf[KS];
+  {
+    // Through the second tile, while the first is on its way.
+    using Wave = WaveRows<T, HD>;
+    static_assert(KB * Wave::kBytes <= SH::kBytes, "room for the keys");
+    typename Wave::vec_t xk[Wave::N], xv[Wave::N];
+    Wave::read(xk, a.D, lane, [&](int n) -> const T* {
+      return kw0 + n < L ? reinterpret_cast<const T*>(a.k) + a.vk.row(g.start + kw0 + n, hk) : nullptr;
+    });
+    Wave::read(xv, a.Dv, lane, [&](int n) -> const T* {
+      return kw0 + n < L ? reinterpret_cast<const T*>(a.v) + a.vv.row(g.start + kw0 + n, hk) : nullptr;
+    });
+    Wave::turn(xk, group + SH::kBytes + kb * Wave::kBytes, lane, kf);
+    Wave::turn(xv, group + SH::kBytes + kb * Wave::kBytes, lane, vf);
+  }
+  float16_t dv[DB], dk[DB];
+#pragma unroll
+  for (int d = 0; d < DB; ++d) dv[d] = dk[d] = zero16();
+
+  const float dl = DsLift<T>(a, g, hk, lane).all(), lift = dl / DsLift<T>::kP, c2 = a.scale * kLog2e;
   // The workgroup goes round together, the last round maybe without a tile for every group.
   const int rounds = (n_end + RG - 1) / RG;
   for (int round = 0, n = rg, cur = 0; round < rounds; ++round, n += RG, cur ^= 1) {
@@ -387,74 +381,54 @@ packed_bwd_kv_kernel(PackedArgs a) {
       issue(h, i0, cur ^ 1);
     }
     if (!busy) continue;
-    float16_t p[NB], dp[NB];
-#pragma unroll
-    for (int b = 0; b < NB; ++b) p[b] = dp[b] = zero16();
+    float16_t p = zero16(), dp = zero16();
     read_ahead<KS, kDepth>([&](int s) { return Rows::row_frag(tile + qrow, s, 0); },
-                           [&](int s, frag_t<T> f) {
-#pragma unroll
-                             for (int b = 0; b < NB; ++b) p[b] = Elem<T>::mma(f, kf[b][s], p[b]);
-                           });
+                           [&](int s, frag_t<T> f) { p = Elem<T>::mma(f, kf[s], p); });
     read_ahead<KS, kDepth>([&](int s) { return Rows::row_frag(tile + orow, s, 0); },
-                           [&](int s, frag_t<T> f) {
+                           [&](int s, frag_t<T> f) { dp = Elem<T>::mma(f, vf[s], dp); });
 #pragma unroll
-                             for (int b = 0; b < NB; ++b) dp[b] = Elem<T>::mma(f, vf[b][s], dp[b]);
-                           });
-    frag_t<T> fp[NB][2], fs[NB][2];
+    for (int q = 0; q < 4; ++q) {
+      const float4_t ls = lds_at<float4_t>(srow + q * 32), d0 = lds_at<float4_t>(srow + 128 + q * 32);
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      const int first = kw0 + 32 * b;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float4_t ls = lds_at<float4_t>(srow + q * 32), d0 = lds_at<float4_t>(srow + 128 + q * 32);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float e = fast_exp2(fmaf(p[b][4 * q + j], c2, ls[j]));
-          p[b][4 * q + j] = e;
-          dp[b][4 * q + j] = e * fmaf(dp[b][4 * q + j], lift, d0[j]);
-        }
+      for (int j = 0; j < 4; ++j) {
+        const float e = fast_exp2(fmaf(p[4 * q + j], c2, ls[j]));
+        p[4 * q + j] = e;
+        dp[4 * q + j] = e * fmaf(dp[4 * q + j], lift, d0[j]);
       }
-      // Selected, not multiplied: tokens past the length have no numbers at all.
-      if ((a.causal && at < first + 31) || at + BM > L) {
+    }
+    // Selected, not multiplied: tokens past the length have no numbers at all.
+    if ((a.causal && at < kw0 + 31) || at + BM > L) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          const int i = at + acc_row(r, hl);
-          if ((a.causal && i < first + ln) || i >= L) p[b][r] = dp[b][r] = 0.f;
-        }
+      for (int r = 0; r < 16; ++r) {
+        const int i = at + acc_row(r, hl);
+        if ((a.causal && i < key) || i >= L) p[r] = dp[r] = 0.f;
       }
+    }
+    frag_t<T> fp[2], fs[2];
 #pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        fp[b][s] = acc_frag<T>(p[b], s);
-        fs[b][s] = acc_frag<T>(dp[b], s);
-      }
+    for (int s = 0; s < 2; ++s) {
+      fp[s] = acc_frag<T>(p, s);
+      fs[s] = acc_frag<T>(dp, s);
     }
     if constexpr (kDepth > 0) __builtin_amdgcn_sched_barrier(0);
     read_ahead<2 * DB, kDepth>([&](int j) { return Rows::col_frag(tile + ocol, j % DB, 16 * (j / DB) * Rows::kRowBytes); },
-                               [&](int j, frag_t<T> f) {
-#pragma unroll
-                                 for (int b = 0; b < NB; ++b) dv[b][j % DB] = Elem<T>::mma(fp[b][j / DB], f, dv[b][j % DB]);
-                               });
+                               [&](int j, frag_t<T> f) { dv[j % DB] = Elem<T>::mma(fp[j / DB], f, dv[j % DB]); });
     read_ahead<2 * DB, kDepth>([&](int j) { return Rows::col_frag(tile + qcol, j % DB, 16 * (j / DB) * Rows::kRowBytes); },
-                               [&](int j, frag_t<T> f) {
-#pragma unroll
-                                 for (int b = 0; b < NB; ++b) dk[b][j % DB] = Elem<T>::mma(fs[b][j / DB], f, dk[b][j % DB]);
-                               });
+                               [&](int j, frag_t<T> f) { dk[j % DB] = Elem<T>::mma(fs[j / DB], f, dk[j % DB]); });
   }
 
   // The groups' sums, the upper half's added to the lower half's.
   if constexpr (RG > 1) {
     auto each = [&](auto&& f) {
 #pragma unroll
-      for (int n = 0; n < NB; ++n)
-#pragma unroll
-        for (int d = 0; d < DB; ++d) {
-          f(dv[n][d], 2 * (n * DB + d));
-          f(dk[n][d], 2 * (n * DB + d) + 1);
-        }
+      for (int d = 0; d < DB; ++d) {
+        f(dv[d], 2 * d);
+        f(dk[d], 2 * d + 1);
+      }
     };
 #pragma unroll
     for (int half = RG / 2; half > 0; half /= 2) {
-      float4_t* y = reinterpret_cast<float4_t*>(smem) + ((rg % half) * KB + kb) * NB * 2 * DB * 4 * kWave + lane;
+      float4_t* y = reinterpret_cast<float4_t*>(smem) + ((rg % half) * KB + kb) * 2 * DB * 4 * kWave + lane;
       __syncthreads();
       if (rg >= half && rg < 2 * half)
         each([&](float16_t& x, int i) {
@@ -478,36 +452,34 @@ packed_bwd_kv_kernel(PackedArgs a) {
   // Keys at or past the length have no gradient: zeros, whatever their scores were.
   const float dv_scale = 1.f / DsLift<T>::kP, dk_scale = a.scale / dl;
 #pragma unroll
-  for (int n = 0; n < NB; ++n)
+  for (int r = 0; r < 16; ++r) {
+    const int j = kw0 + acc_row(r, hl);
+    if (j >= g.rows) continue;
+    const bool in = j < L;
+    T* pv = reinterpret_cast<T*>(a.dv) + a.vdv.row(g.start + j, hk);
+    T* pk = reinterpret_cast<T*>(a.dk) + a.vdk.row(g.start + j, hk);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-      const int j = kw0 + 32 * n + acc_row(r, hl);
-      if (j >= g.rows) continue;
-      const bool in = j < L;
-      T* pv = reinterpret_cast<T*>(a.dv) + a.vdv.row(g.start + j, hk);
-      T* pk = reinterpret_cast<T*>(a.dk) + a.vdk.row(g.start + j, hk);
-#pragma unroll
-      for (int d = 0; d < DB; ++d) {
-        if (32 * d + ln < a.Dv) pv[32 * d + ln] = (T)(in ? dv[n][d][r] * dv_scale : 0.f);
-        if (32 * d + ln < a.D) pk[32 * d + ln] = (T)(in ? dk[n][d][r] * dk_scale : 0.f);
-      }
+    for (int d = 0; d < DB; ++d) {
+      if (32 * d + ln < a.Dv) pv[32 * d + ln] = (T)(in ? dv[d][r] * dv_scale : 0.f);
+      if (32 * d + ln < a.D) pk[32 * d + ln] = (T)(in ? dk[d][r] * dk_scale : 0.f);
     }
+  }
 }
 
-template <typename T, int HD, int BLOCKS, int NB>
+template <typename T, int HD, int BLOCKS>
 int launch_q(PackedArgs a, hipStream_t stream) {
-  const int64_t slots = region_slots(a.T, a.N, a.G, QShape<T, HD, BLOCKS, NB>::ROWS);
+  const int64_t slots = region_slots(a.T, a.N, a.G, QShape<T, HD, BLOCKS>::ROWS);
   a.n_slots = (int)slots;
-  hipLaunchKernelGGL((packed_bwd_q_kernel<T, HD, BLOCKS, NB>), dim3(uint32_t(slots * a.Hk)), dim3(kThreads), 0, stream, a);
+  hipLaunchKernelGGL((packed_bwd_q_kernel<T, HD, BLOCKS>), dim3(uint32_t(slots * a.Hk)), dim3(kThreads), 0, stream, a);
   return tjh::launch_status();
 }
 
-template <typename T, int HD, int BLOCKS, int GROUPS, int NB>
+template <typename T, int HD, int BLOCKS, int GROUPS>
 int launch_kv(PackedArgs a, hipStream_t stream) {
-  using KV = KvShape<T, HD, BLOCKS, GROUPS, NB>;
+  using KV = KvShape<T, HD, BLOCKS, GROUPS>;
   const int64_t slots = region_slots(a.T, a.N, 1, KV::KEYS);
   a.n_slots = (int)slots;
-  hipLaunchKernelGGL((packed_bwd_kv_kernel<T, HD, BLOCKS, GROUPS, NB>), dim3(uint32_t(slots * a.Hk)), dim3(64 * KV::WAVES), 0,
+  hipLaunchKernelGGL((packed_bwd_kv_kernel<T, HD, BLOCKS, GROUPS>), dim3(uint32_t(slots * a.Hk)), dim3(64 * KV::WAVES), 0,
                      stream, a);
   return tjh::launch_status();
 }
@@ -528,16 +500,16 @@ int packed_bwd(const PackedArgs& a, int dtype, hipStream_t stream) {
     const int64_t rows = (int64_t)a.T * a.G;  // of one key head
     int rc;
     if constexpr (groups_fit<T, HD>(4)) {
-      if ((rows + 63) / 64 * a.Hk <= kCus / 2) rc = launch_q<T, HD, 1, 1>(a, stream);
-      else if ((rows + 127) / 128 * a.Hk <= 2 * kCus) rc = launch_q<T, HD, 2, 1>(a, stream);
-      else rc = launch_q<T, HD, 4, 1>(a, stream);
+      if ((rows + 63) / 64 * a.Hk <= kCus / 2) rc = launch_q<T, HD, 1>(a, stream);
+      else if ((rows + 127) / 128 * a.Hk <= 2 * kCus) rc = launch_q<T, HD, 2>(a, stream);
+      else rc = launch_q<T, HD, 4>(a, stream);
     } else {
-      if ((rows + 127) / 128 * a.Hk <= 2 * kCus) rc = launch_q<T, HD, 2, 1>(a, stream);
-      else rc = launch_q<T, HD, 4, 1>(a, stream);
+      if ((rows + 127) / 128 * a.Hk <= 2 * kCus) rc = launch_q<T, HD, 2>(a, stream);
+      else rc = launch_q<T, HD, 4>(a, stream);
     }
     if (rc != TJ_OK) return rc;
-    if ((int64_t)(a.T + 63) / 64 * a.Hk <= kCus / 2) return launch_kv<T, HD, 1, HD == 32 || (HD == 64 && sizeof(T) == 2) ? 4 : 2, 1>(a, stream);
-    return launch_kv<T, HD, 2, 2, 1>(a, stream);
+    if ((int64_t)(a.T + 63) / 64 * a.Hk <= kCus / 2) return launch_kv<T, HD, 1, groups_fit<T, HD>(4) ? 4 : 2>(a, stream);
+    return launch_kv<T, HD, 2, 2>(a, stream);
   });
 }
 

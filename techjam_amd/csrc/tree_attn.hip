@@ -47,9 +47,16 @@ struct TreeShape {
   using SH = SweepShape<T, HD, BN>;
   static constexpr int kFit = 128 * 1024 / (2 * SH::kBytes), kMost = RB <= 2 ? 4 : 8 / RB, KG = kFit < kMost ? kFit : kMost;
   static constexpr int WAVES = RB * KG, THREADS = kWave * WAVES;
+  using Wave = WaveRows<T, HD>;
+  // Two tiles a group, afterwards the groups' results.
+  static constexpr int kTiles = KG * 2 * SH::kBytes, kSums = KG > 1 ? 16 * SH::DB * 4 * kWave * RB * (KG / 2) : 0;
+  static constexpr int kBytes = kTiles > kSums ? kTiles : kSums;
+  // q comes through the second tile while the first keys are on their way, or before them where it needs both.
+  static constexpr bool kBefore = RB * Wave::kBytes > SH::kBytes;
+  static_assert(RB * Wave::kBytes <= 2 * SH::kBytes, "room for q");
   // Waves of a SIMD by the registers, and workgroups that a CU holds.
   static constexpr int kWaves = HD == 32 ? 3 : (sizeof(T) == 2 || HD == 64 || WAVES > 4 ? 2 : 1);
-  static constexpr int kByLds = 160 * 1024 / (KG * 2 * SH::kBytes), kByRegs = kWaves * 4 / WAVES;
+  static constexpr int kByLds = 160 * 1024 / kBytes, kByRegs = kWaves * 4 / WAVES;
   static constexpr int kPerCu = kByLds < kByRegs ? kByLds : kByRegs;
   static_assert(kPerCu >= 1, "a workgroup fits a CU");
 };
@@ -58,11 +65,10 @@ template <typename T, int HD, int BLOCKS>
 __global__ __launch_bounds__((TreeShape<T, HD, BLOCKS>::THREADS), (TreeShape<T, HD, BLOCKS>::kWaves)) void tree_kernel(TreeArgs a) {
   using TS = TreeShape<T, HD, BLOCKS>;
   using SH = typename TS::SH;
-  using State = SweepState<T, HD, TS::BN, 1, false>;
+  using State = SweepState<T, HD, TS::BN, false>;
   constexpr int RB = TS::RB, KG = TS::KG, BN = TS::BN;
-  // Two tiles a group; afterwards the groups' results.
-  constexpr int kSums = KG > 1 ? 16 * State::kGive * RB * (KG / 2) : 0;
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[KG * 2 * SH::kBytes > kSums ? KG * 2 * SH::kBytes : kSums];
+  using Wave = typename TS::Wave;
+  __shared__ __attribute__((aligned(1024))) unsigned char smem[TS::kBytes];
   __shared__ float ml[KG > 1 ? KG / 2 * RB * State::kMl * kWave : 1];
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave;
   const int kg = w / RB, rb = w % RB;
@@ -80,7 +86,7 @@ __global__ __launch_bounds__((TreeShape<T, HD, BLOCKS>::THREADS), (TreeShape<T, 
   const int L = __builtin_amdgcn_readfirstlane(min(a.Sk, max(0, a.len[b]))), ctx = L - a.Sq;
   const int row0 = mt * TS::ROWS, rw0 = row0 + 32 * rb;
   // Keys that rows row .. last (clipped to R) need.
-  auto span = [&](int row, int last) { return row >= a.R ? 0 : max(0, ctx + min(last, a.R - 1) / a.G + 1); };
+  auto span = [&](int row, int last) { return row >= a.R ? 0 : max(0, ctx + min(last, a.R - 1) / a.by_group + 1); };
   const int n_keys = whole ? L : __builtin_amdgcn_readfirstlane(f.keys);
   const int kv_begin = whole ? 0 : __builtin_amdgcn_readfirstlane((part - f.first) * f.keys);
   const int kv_end = min(span(row0, row0 + TS::ROWS - 1), kv_begin + n_keys), own_end = min(kv_end, span(rw0, rw0 + 31));
@@ -90,9 +96,9 @@ __global__ __launch_bounds__((TreeShape<T, HD, BLOCKS>::THREADS), (TreeShape<T, 
   keys.init(reinterpret_cast<const T*>(a.k) + a.vk.row(b, hk, 0), reinterpret_cast<const T*>(a.v) + a.vv.row(b, hk, 0),
             a.vk.ss, a.vv.ss, a.D, a.Dv, rb, lane);
   int kv0 = kv_begin + BN * kg;
-  if (kv0 < kv_end) keys.issue(kv0, L, tiles, rb);
+  if (!TS::kBefore && kv0 < kv_end) keys.issue(kv0, L, tiles, rb);
   const int r = rw0 + lane % 32;
-  SweepRow row{r, r / a.G, r % a.G, 0, false};
+  SweepRow row{r, r / a.by_group, r % a.by_group, 0, false};
   row.limit = ctx + row.i;
   row.live = r < a.R && row.limit >= 0;
   uint64_t seen = 0, gone = 0;
@@ -104,8 +110,19 @@ __global__ __launch_bounds__((TreeShape<T, HD, BLOCKS>::THREADS), (TreeShape<T, 
     row.live = row.live && !(gone >> t & 1);
   }
   State st;
+  {
+    typename Wave::vec_t x[Wave::N];
+    Wave::read(x, a.D, lane, [&](int n) -> const T* {
+      const int r = rw0 + n, i = r / a.by_group;
+      return r < a.R ? reinterpret_cast<const T*>(a.q) + a.vq.row(b, hk * a.G + r - i * a.G, i) : nullptr;
+    });
+    Wave::turn(x, tiles + (TS::kBefore ? 0 : SH::kBytes) + rb * Wave::kBytes, lane, st.q);
+  }
+  if constexpr (TS::kBefore) {
+    __syncthreads();
+    if (kv0 < kv_end) keys.issue(kv0, L, tiles, rb);
+  }
   st.init(a.scale, lane);
-  st.load_q(0, row.live ? reinterpret_cast<const T*>(a.q) + a.vq.row(b, hk * a.G + row.g, row.i) : nullptr, a.scale, a.D, lane);
   // The workgroup goes round together, the last round maybe without a tile for every group.
   for (int first = kv_begin, cur = 0; first < kv_end; first += KG * BN, kv0 += KG * BN, cur ^= 1) {
     // The tile is there, and the group's other one has been read by its waves. (A group of one wave has waited for
@@ -129,7 +146,7 @@ __global__ __launch_bounds__((TreeShape<T, HD, BLOCKS>::THREADS), (TreeShape<T, 
     for (int kb = 0; kb < BN / 32; ++kb) {
       const int at = kv0 + 32 * kb;
       if (at >= own_end) continue;
-      st.step(tile, kb, [&](int, float16_t& s) {
+      st.step(tile, kb, [&](float16_t& s) {
         const int hl = lane / 32;
         if (at + 32 <= ctx) return;
         if (a.parents == nullptr) {
@@ -158,22 +175,30 @@ __global__ __launch_bounds__((TreeShape<T, HD, BLOCKS>::THREADS), (TreeShape<T, 
     __syncthreads();
     if (kg < half) st.take(x, y, lane);
   }
-  const float sum = pair_sum(st.l[0]);
-  if (kg != 0 || r >= a.R) return;
+  __syncthreads();  // the tiles, in whose place the rows are turned, have been read
+  const float sum = pair_sum(st.l);
+  if (kg != 0) return;
   if (whole) {
     const float inv = 1.f / sum;
-    T* op = reinterpret_cast<T*>(a.o) + a.vo.row(b, hk * a.G + row.g, row.i);
-    st.columns(0, a.Dv, lane, [&](int col, float4_t y) {
-      if (!row.live) y = float4_t{0.f, 0.f, 0.f, 0.f};
-      else y *= inv;
-      store4t<T>(op + col, y[0], y[1], y[2], y[3]);
-    });
+    Wave::write(lds_offset(smem) + rb * Wave::kBytes, a.Dv, lane,
+                [&](int d, int c) { return row.live ? st.four(d, c) * inv : float4_t{0.f, 0.f, 0.f, 0.f}; },
+                [&](int n) -> T* {
+                  const int r = rw0 + n, i = r / a.by_group;
+                  return r < a.R ? reinterpret_cast<T*>(a.o) + a.vo.row(b, hk * a.G + r - i * a.G, i) : nullptr;
+                });
     return;
   }
+  if (r >= a.R) return;
   const int64_t at = ((int64_t)part * a.Hk + hk) * a.R + r;
-  if (lane < 32) *reinterpret_cast<float4_t*>(a.part_ml + at * 4) = float4_t{st.m[0], sum, row.live ? 1.f : 0.f, 0.f};
-  if (row.live)
-    st.columns(0, a.Dv, lane, [&](int col, float4_t y) { *reinterpret_cast<float4_t*>(a.part_o + at * a.Dv + col) = y; });
+  if (lane < 32) *reinterpret_cast<float4_t*>(a.part_ml + at * 4) = float4_t{st.m, sum, row.live ? 1.f : 0.f, 0.f};
+  if (!row.live) return;
+#pragma unroll
+  for (int d = 0; d < SH::DB; ++d)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int col = 32 * d + 8 * c + 4 * (lane / 32);
+      if (col < a.Dv) *reinterpret_cast<float4_t*>(a.part_o + at * a.Dv + col) = st.four(d, c);
+    }
 }
 
 // Joins the parts: O = sum_p 2^(max_p - M) o_p / sum_p 2^(max_p - M) sum_p. `lanes` threads take a row's
@@ -187,7 +212,7 @@ __global__ __launch_bounds__(kJoinThreads) void tree_join_kernel(TreeArgs a, int
   const int chunk = tid % lanes, set = tid / lanes % sets;
   const int tiles = (a.R + rows - 1) / rows;  // of one (sequence, key head)
   const int bh = blockIdx.x / tiles, b = bh / a.Hk, hk = bh % a.Hk;
-  const int r = blockIdx.x % tiles * rows + tid / per_row, i = r / a.G;
+  const int r = blockIdx.x % tiles * rows + tid / per_row, i = r / a.by_group;
   const int L = min(a.Sk, max(0, a.len[b])), limit = L - a.Sq + i;
   int np = 0;
   int64_t at = 0;  // the row's number in its first part
@@ -232,7 +257,7 @@ __global__ __launch_bounds__(kJoinThreads) void tree_join_kernel(TreeArgs a, int
   const float inv = 1.f / l;
 #pragma unroll
   for (int j = 0; j < 4; ++j) y[j] = live != 0.f ? y[j] * inv : 0.f;
-  store4t<T>(reinterpret_cast<T*>(a.o) + a.vo.row(b, hk * a.G + r % a.G, i) + chunk * 4, y[0], y[1], y[2], y[3]);
+  store4t<T>(reinterpret_cast<T*>(a.o) + a.vo.row(b, hk * a.G + r % a.by_group, i) + chunk * 4, y[0], y[1], y[2], y[3]);
 }
 
 template <typename T>
@@ -256,13 +281,14 @@ int launch(const TreeArgs& a, hipStream_t stream) {
   return rc != TJ_OK || a.part_o == nullptr ? rc : launch_join<T>(a, stream);
 }
 
-// f(integral_constant<int, blocks of 32 rows a workgroup>).
-template <typename F>
+// f(integral_constant<int, blocks of 32 rows a workgroup>); eight blocks of fp32 rows spill.
+template <typename T, typename F>
 auto by_blocks(int R, F&& f) {
   if (R <= 32) return f(std::integral_constant<int, 1>{});
   if (R <= 64) return f(std::integral_constant<int, 2>{});
-  if (R <= 128) return f(std::integral_constant<int, 4>{});
-  return f(std::integral_constant<int, 8>{});
+  if constexpr (sizeof(T) == 2)
+    if (R > 128) return f(std::integral_constant<int, 8>{});
+  return f(std::integral_constant<int, 4>{});
 }
 
 }  // namespace
@@ -270,7 +296,7 @@ auto by_blocks(int R, F&& f) {
 TreePlan tree_plan(const TreeArgs& a, int dtype) {
   TreePlan p{};
   grouped_dispatch(a.D, a.Dv, dtype, [&](auto t, auto hd) {
-    by_blocks(a.R, [&](auto blocks) {
+    by_blocks<decltype(t)>(a.R, [&](auto blocks) {
       using TS = TreeShape<decltype(t), decltype(hd)::value, decltype(blocks)::value>;
       p.blocks = TS::RB;
       p.parts = few_plan(a.B, a.Hk, (a.R + TS::ROWS - 1) / TS::ROWS, a.Sk, kCus * TS::kPerCu);
@@ -288,7 +314,7 @@ int tree_fwd(const TreeArgs& args, const TreePlan& p, int dtype, hipStream_t str
   a.few_each = (int)p.parts.each;
   a.n_parts = (int)p.parts.total;
   return grouped_dispatch(a.D, a.Dv, dtype, [&](auto t, auto hd) {
-    return by_blocks(a.R, [&](auto blocks) {
+    return by_blocks<decltype(t)>(a.R, [&](auto blocks) {
       return launch<decltype(t), decltype(hd)::value, decltype(blocks)::value>(a, stream);
     });
   });
