@@ -152,7 +152,7 @@ int packed_fwd(const PackedArgs& a, int dtype, hipStream_t stream) {
     if constexpr (groups_fit<T, HD>(4))
       if ((rows + 63) / 64 * a.Hk <= kCus / 2) return launch<T, HD, 1>(a, stream);
     if constexpr (groups_fit<T, HD>(2))
-      if ((rows + 127) / 128 * a.Hk <= kCus) return launch<T, HD, 2>(a, stream);
+      if ((rows + 127) / 128 * a.Hk <= (HD <= 64 ? 2 : 1) * kCus) return launch<T, HD, 2>(a, stream);
     return launch<T, HD, 4>(a, stream);
   });
 }
