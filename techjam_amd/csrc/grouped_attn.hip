@@ -36,7 +36,7 @@ bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0
 bool packed_sizes_ok(int64_t T, int64_t N, int64_t H, int64_t Hk) {
   if (T < 0 || N < 0 || H <= 0 || Hk <= 0 || H % Hk != 0) return false;
   const int64_t lim = int64_t(1) << 30;
-  return N < lim && H < lim && tjh::product_below(lim, {T + 64, H}) &&
+  return T < lim && N < lim && H < lim && tjh::product_below(lim, {T + 64, H}) &&
          tjh::product_below(int64_t(1) << 23, {Hk, (T / 32 + 1) * (H / Hk) + N + 4});
 }
 

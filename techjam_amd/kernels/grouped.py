@@ -15,7 +15,6 @@ from typing import Optional
 
 import torch
 import torch.nn.functional as F
-from torch.autograd.function import once_differentiable
 
 from ..errors import UnsupportedCaseError
 from . import _lib
@@ -125,9 +124,17 @@ def _backward(ctx, dout):
     return dq, dk, dvv, None, None, None, None
 
 
-#: Under create_graph: the gradients, with an error for whoever differentiates
-#: them. Without it the plain function, whose call is leaner.
-_backward_once = once_differentiable(_backward)
+class _OnceOnly(torch.autograd.Function):
+    """Hands gradients on as functions of what they were computed from, whose derivatives are refused. (They
+    depend on the inputs also where the output gradient requires none.)"""
+
+    @staticmethod
+    def forward(ctx, dq, dk, dv, *inputs):
+        return dq, dk, dv
+
+    @staticmethod
+    def backward(ctx, *grads):
+        raise UnsupportedCaseError("packed_attention is differentiable once: second derivatives are not implemented")
 
 
 class _PackedAttention(torch.autograd.Function):
@@ -140,7 +147,11 @@ class _PackedAttention(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, dout):
-        return _backward_once(ctx, dout) if torch.is_grad_enabled() else _backward(ctx, dout)
+        if not torch.is_grad_enabled():
+            return _backward(ctx, dout)
+        with torch.no_grad():  # under create_graph
+            grads = _backward(ctx, dout)
+        return *_OnceOnly.apply(*grads[:3], *ctx.saved_tensors[:3], dout), *grads[3:]
 
 
 def packed_attention(

@@ -28,7 +28,7 @@ from .kernels.linear import ffn_norm, projections, residual_norm, split_products
 
 
 ACTIVATIONS = ("gelu", "relu")
-ATTENTIONS = ("softmax", "differential")
+ATTENTIONS = ("softmax", "differential", "grouped")
 #: The norms whose parameters the fused inference kernels read.
 NORM_TYPES = (nn.LayerNorm, LayerNorm)
 
@@ -45,7 +45,11 @@ class TransformerConfig:
     ``attention="differential"`` puts differential attention
     (``implementations/differential.py``) in the place of softmax attention:
     an encoder that can also be trained on the kernels and, when it is causal
-    and pre-norm, run token by token (``TransformerEncoder.step``). Config
+    and pre-norm, run token by token (``TransformerEncoder.step``).
+    ``attention="grouped"`` is softmax attention whose query heads share ``kv_heads``
+    key heads (``implementations/grouped.py``; as many as there are query heads by
+    default), which trains, steps over single tokens and trees of drafts, and takes
+    sequences laid end to end (``TransformerEncoder.forward_packed``). Config
     objects without these fields (the reference harness's own) mean the defaults.
     """
 
@@ -59,6 +63,7 @@ class TransformerConfig:
     norm_first: bool = True
     activation: str = "gelu"
     attention: str = "softmax"
+    kv_heads: Optional[int] = None
 
     def validate(self) -> None:
         for name in ("batch_size", "seq_len", "d_model", "num_heads", "ffn_dim", "num_layers"):
@@ -73,10 +78,15 @@ class TransformerConfig:
         if attention_variant(self) == "differential" and self.d_model % (2 * self.num_heads):
             raise ValueError(f"d_model ({self.d_model}) must be divisible by 2 * num_heads ({2 * self.num_heads}) "
                              "for differential attention")
+        if self.kv_heads is not None:
+            if self.attention != "grouped":
+                raise ValueError(f"kv_heads belongs to grouped attention, not to {self.attention} attention")
+            if self.kv_heads <= 0 or self.num_heads % self.kv_heads:
+                raise ValueError(f"num_heads ({self.num_heads}) must be divisible by kv_heads ({self.kv_heads})")
 
 
 def attention_variant(config) -> str:
-    """``"softmax"`` (also of configs that do not say) or ``"differential"``."""
+    """``"softmax"`` (also of configs that do not say), ``"differential"`` or ``"grouped"``."""
     attention = getattr(config, "attention", "softmax")
     if attention not in ATTENTIONS:
         raise ValueError(f"attention must be one of {ATTENTIONS}, not {attention!r}")
@@ -240,7 +250,8 @@ class EncoderBlock(nn.Module):
     """
 
     def __init__(self, d_model: int, num_heads: int, ffn_dim: int, norm_first: bool = True,
-                 activation: str = "gelu", attention: str = "softmax", depth: int = 0) -> None:
+                 activation: str = "gelu", attention: str = "softmax", depth: int = 0,
+                 kv_heads: Optional[int] = None) -> None:
         super().__init__()
         if activation not in ACTIVATIONS:
             raise ValueError(f"activation must be one of {ACTIVATIONS}, not {activation!r}")
@@ -250,13 +261,17 @@ class EncoderBlock(nn.Module):
         self.activation = activation
         #: Whether every operator of the block has gradients: with them enabled
         #: it then runs unfused.
-        self.differentiable = attention == "differential"
+        self.differentiable = attention != "softmax"
         norm = LayerNorm if self.differentiable else nn.LayerNorm
         self.norm1 = norm(d_model)
-        if self.differentiable:
+        if attention == "differential":
             from .implementations.differential import DifferentialSelfAttention
 
             self.attention = DifferentialSelfAttention(d_model, num_heads, depth)
+        elif attention == "grouped":
+            from .implementations.grouped import GroupedSelfAttention
+
+            self.attention = GroupedSelfAttention(d_model, num_heads, kv_heads)
         else:
             self.attention = HipSelfAttention(d_model, num_heads)
         self.norm2 = norm(d_model)
@@ -278,6 +293,13 @@ class EncoderBlock(nn.Module):
         if valid_token_mask is not None:
             x = x.masked_fill(~valid_token_mask[..., None], 0)
         return x
+
+    def forward_packed(self, x, offsets, causal, keep=None):
+        """The block over sequences laid end to end (grouped attention), unfused."""
+        if self.norm_first:
+            return self.ffn(x + self.attention.packed(self.norm1(x), offsets, causal, keep))
+        x = self.norm1(x + self.attention.packed(x, offsets, causal, keep))
+        return self.norm2(x + self.ffn_out(self._act(self.ffn_in(x))))
 
     def ffn(self, x):
         """The pre-norm block's second half."""
@@ -444,12 +466,12 @@ class TransformerEncoder(nn.Module):
         self.attention = attention_variant(config)
         self.layers = nn.ModuleList(
             EncoderBlock(config.d_model, config.num_heads, config.ffn_dim, self.norm_first, self.activation,
-                         self.attention, depth)
+                         self.attention, depth, getattr(config, "kv_heads", None))
             for depth in range(config.num_layers)
         )
         # A post-norm stack ends in its last block's norm (torch.nn.TransformerEncoder
         # with norm=None); only the pre-norm stack has a final LayerNorm.
-        norm = LayerNorm if self.attention == "differential" else nn.LayerNorm
+        norm = LayerNorm if self.attention != "softmax" else nn.LayerNorm
         self.final_norm = norm(config.d_model) if self.norm_first else nn.Identity()
 
     def forward_layers(self, x, valid_token_mask=None, valid_len=None, gemm_operands=None):
@@ -458,10 +480,10 @@ class TransformerEncoder(nn.Module):
         operands = self.gemm_operands if gemm_operands is None else gemm_operands
         if operands not in ("fp32", "fp16"):
             raise ValueError(f"gemm_operands must be 'fp32' or 'fp16', not {operands!r}")
-        if operands == "fp16" and self.attention == "differential":
+        if operands == "fp16" and self.attention != "softmax":
             from .errors import UnsupportedCaseError
 
-            raise UnsupportedCaseError("fp16 GEMM operands are not implemented for differential attention")
+            raise UnsupportedCaseError(f"fp16 GEMM operands are not implemented for {self.attention} attention")
         if self._can_fuse_norms(x, valid_token_mask, valid_len):
             return self._forward_layers_fused(x, valid_token_mask, valid_len, operands)
         if operands == "fp16":
@@ -477,18 +499,40 @@ class TransformerEncoder(nn.Module):
             x.masked_fill_(~valid_token_mask[..., None], 0)  # x is the norm's fresh output
         return x
 
-    # -- token by token (causal differential attention) ----------------------
+    def forward_packed(self, x, offsets):
+        """Sequences laid end to end, ``x`` ``[T, D]`` (grouped attention): tokens ``offsets[n] .. offsets[n + 1] - 1``
+        (int32 ``[N + 1]`` on the device) are sequence ``n``. Rows before the first and behind the last sequence are not
+        read and come out as zeros. Runs unfused, with gradients where they are enabled."""
+        self._check_packed(x)
+        rows = torch.arange(x.shape[0], device=x.device)
+        outside = ((rows < offsets[0]) | (rows >= offsets[-1]))[:, None]
+        x = x.masked_fill(outside, 0)
+        for layer in self.layers:
+            x = layer.forward_packed(x, offsets, self.config.causal)
+        return self.final_norm(x).masked_fill(outside, 0)
+
+    def _check_packed(self, x) -> None:
+        from .errors import UnsupportedCaseError
+
+        if self.attention != "grouped":
+            raise UnsupportedCaseError("sequences laid end to end: encoders of grouped attention only")
+        if x.ndim != 2 or x.shape[1] != self.config.d_model:
+            raise ValueError(f"x must be [T, {self.config.d_model}], not {tuple(x.shape)}")
+
+    # -- token by token (causal differential or grouped attention) -----------
     def new_state(self, batch: int, capacity: int, dtype: Optional[torch.dtype] = None):
         """Empty caches for ``batch`` sequences of up to ``capacity`` tokens. Their
         type is that of the steps' projections: the parameters' (the default),
         or autocast's for steps under it; a step whose type differs is refused."""
         from .errors import UnsupportedCaseError
         from .implementations.differential import DifferentialState
+        from .implementations.grouped import GroupedState
 
-        if self.attention != "differential" or not self.norm_first or not self.config.causal:
-            raise UnsupportedCaseError("token by token: causal, pre-norm encoders of differential attention only")
+        if self.attention == "softmax" or not self.norm_first or not self.config.causal:
+            raise UnsupportedCaseError("token by token: causal, pre-norm encoders of differential or grouped attention only")
         weight = self.layers[0].ffn_in.weight if len(self.layers) else self.final_norm.weight
-        return DifferentialState(self.config, batch, capacity, weight.dtype if dtype is None else dtype, weight.device)
+        state = DifferentialState if self.attention == "differential" else GroupedState
+        return state(self.config, batch, capacity, weight.dtype if dtype is None else dtype, weight.device)
 
     @torch.no_grad()
     def prefill(self, x, state, valid_token_mask: Optional[torch.Tensor] = None):
@@ -499,8 +543,7 @@ class TransformerEncoder(nn.Module):
         if x.shape[1] > state.capacity:
             raise ValueError(f"{x.shape[1]} tokens exceed the cache's capacity of {state.capacity}")
         lengths = None if valid_token_mask is None else prefix_lengths(valid_token_mask)
-        state.lengths.zero_()  # a call that fails on its way leaves an empty state
-        state.longest = 0
+        self._empty(state)
         for layer, cache in zip(self.layers, state.layers):
             x = x + layer.attention(layer.norm1(x), valid_token_mask, True, lengths, cache)
             x = layer.ffn(x)
@@ -514,11 +557,65 @@ class TransformerEncoder(nn.Module):
         return x
 
     @torch.no_grad()
-    def step(self, x, state):
+    def prefill_packed(self, x, offsets, state):
+        """:meth:`prefill` of prompts laid end to end (grouped attention; ``x`` and ``offsets`` as in
+        :meth:`forward_packed`, one sequence for each of ``state``): their outputs, ``[T, D]``. Waits for the
+        device once, to look at the offsets."""
+        _not_captured()
+        self._check_packed(x)
+        batch = state.lengths.shape[0]
+        if offsets.shape != (batch + 1,):
+            raise ValueError(f"offsets must be [{batch + 1}], one sequence for each of the state, not {tuple(offsets.shape)}")
+        self._check_state(x.new_empty((batch, 0, x.shape[1])), state)
+        edges = offsets.tolist()
+        if edges[0] < 0 or edges[-1] > x.shape[0] or any(a > b for a, b in zip(edges, edges[1:])):
+            raise ValueError(f"offsets must not decrease and lie within 0 and {x.shape[0]}, not {edges}")
+        longest = max(b - a for a, b in zip(edges, edges[1:]))
+        if longest > state.capacity:
+            raise ValueError(f"{longest} tokens exceed the cache's capacity of {state.capacity}")
+        self._empty(state)
+        out = torch.zeros_like(x)
+        first, last = edges[0], edges[-1]
+        x, offsets = x[first:last], offsets - first
+        row = torch.arange(last - first, dtype=torch.int32, device=x.device)
+        sequence = torch.searchsorted(offsets[1:], row, right=True)
+        place = (row - offsets[sequence]).long()
+        for layer, cache in zip(self.layers, state.layers):
+            def keep(k, v):
+                if k.dtype != cache.k.dtype:
+                    raise ValueError(f"the cache holds {cache.k.dtype}, the prompts' keys and values are {k.dtype}: "
+                                     "create the state in that dtype")
+                cache.k[sequence, :, place] = k
+                cache.v[sequence, :, place] = v
+            x = layer.forward_packed(x, offsets, True, keep)
+        out[first:last] = self.final_norm(x)
+        state.lengths.copy_(offsets.diff())
+        state.longest = longest
+        return out
+
+    @staticmethod
+    def _empty(state) -> None:
+        """A call that fails on its way leaves an empty state."""
+        state.lengths.zero_()
+        state.longest = 0
+        if hasattr(state, "drafts"):
+            state.drafts = 0
+
+    @torch.no_grad()
+    def step(self, x, state, parents: Optional[torch.Tensor] = None):
         """The next ``T`` tokens of every sequence (``x`` ``[B, T, D]``): the
-        encoder's output for them, their keys and values added to ``state``."""
+        encoder's output for them, their keys and values added to ``state``.
+
+        With ``parents`` (grouped attention; int32 ``[B, T]`` on the device, as in
+        ``kernels.tree_attention``) the tokens are drafts that form trees: each sees the settled tokens
+        and its own line of parents. Nothing is settled by that: ``state.accept`` makes one line of them
+        the sequence's next tokens, and the next step drops the others."""
         _not_captured()
         self._check_state(x, state)
+        if parents is not None and self.attention != "grouped":
+            from .errors import UnsupportedCaseError
+
+            raise UnsupportedCaseError("trees of drafts: encoders of grouped attention only")
         tokens = x.shape[1]
         if tokens == 0:
             raise ValueError("a step has at least one token")
@@ -527,19 +624,28 @@ class TransformerEncoder(nn.Module):
         # The state counts the tokens when all layers have them: a refused call
         # leaves it as it was.
         lengths = state.lengths + tokens
+        drafts = () if parents is None else (parents,)
         for layer, cache in zip(self.layers, state.layers):
-            x = x + layer.attention.step(layer.norm1(x), cache, lengths, place)
+            x = x + layer.attention.step(layer.norm1(x), cache, lengths, place, *drafts)
             x = layer.ffn(x)
         x = self.final_norm(x)
-        state.lengths.copy_(lengths)
-        state.longest += tokens
+        if parents is None:
+            state.lengths.copy_(lengths)
+            state.longest += tokens
+        if hasattr(state, "drafts"):
+            state.drafts = 0 if parents is None else tokens
         return x
 
     def _check_state(self, x, state) -> None:
         b, d = state.lengths.shape[0], self.config.d_model
         if x.ndim != 3 or x.shape[0] != b or x.shape[2] != d:
             raise ValueError(f"x must be [{b}, T, {d}], not {tuple(x.shape)}")
-        head = (2 * self.config.num_heads, d // self.config.num_heads // 2)
+        if self.attention == "grouped":
+            from .implementations.grouped import grouped_heads
+
+            head = grouped_heads(self.config)
+        else:
+            head = (2 * self.config.num_heads, d // self.config.num_heads // 2)
         if len(state.layers) != len(self.layers) or any((c.k.shape[1], c.k.shape[3]) != head for c in state.layers):
             raise ValueError("the state is another model's")
 

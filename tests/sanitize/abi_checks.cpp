@@ -242,6 +242,69 @@ int main() {
     expect("norm bwd alignment", norm_bwd(at(3), stats, TJ_F16, 4, 64, at(5120), 1 << 15), TJ_ERR_ALIGN);
     expect("norm bwd workspace", norm_bwd(v, stats, TJ_F16, 4, 64, at(5120), 16), TJ_ERR_WORKSPACE);
     expect("norm bwd no rows", norm_bwd(nullptr, stats, TJ_F16, 0, 64, at(5120), 16), TJ_OK);
+
+    // tj_packed_attn_fwd(q, k, v, o, dtype, T, N, H, Hk, D, Dv, strides x4, scale, causal, offsets, lengths, lse, o_rest, stream)
+    const int64_t rows3[3] = {1024, 64, 1}, rows3_inner[3] = {1024, 64, 2}, rows3_far[3] = {int64_t(1) << 40, 64, 1};
+    auto packed = [&](const void* fq, int dtype, int64_t T, int64_t N, int64_t H, int64_t Hk, int64_t D, int64_t Dv,
+                      const int64_t* kst, const int32_t* offsets, float* lse, void* rest) {
+      return tj_packed_attn_fwd(fq, k, v, o, dtype, T, N, H, Hk, D, Dv, rows3, kst, rows3, rows3, 0.125f, 1, offsets, len, lse,
+                                rest, nullptr);
+    };
+    expect("packed dtype", packed(q, 9, 16, 1, 2, 2, 64, 64, rows3, len, nullptr, nullptr), TJ_ERR_DTYPE);
+    expect("packed shared heads", packed(q, TJ_F16, 16, 1, 3, 2, 64, 64, rows3, len, nullptr, nullptr), TJ_ERR_SHAPE);
+    expect("packed no heads", packed(q, TJ_F16, 16, 1, 0, 0, 64, 64, rows3, len, nullptr, nullptr), TJ_ERR_SHAPE);
+    expect("packed negative T", packed(q, TJ_F16, -1, 1, 2, 2, 64, 64, rows3, len, nullptr, nullptr), TJ_ERR_SHAPE);
+    expect("packed huge T", packed(q, TJ_F16, std::numeric_limits<int64_t>::max(), 1, 2, 2, 64, 64, rows3, len, nullptr, nullptr), TJ_ERR_SHAPE);
+    expect("packed huge N", packed(q, TJ_F16, 16, kBig, 2, 2, 64, 64, rows3, len, nullptr, nullptr), TJ_ERR_SHAPE);
+    expect("packed huge H", packed(q, TJ_F16, 16, 1, kBig, 1, 64, 64, rows3, len, nullptr, nullptr), TJ_ERR_SHAPE);
+    expect("packed head dim", packed(q, TJ_F16, 16, 1, 2, 2, 136, 64, rows3, len, nullptr, nullptr), TJ_ERR_UNSUPPORTED);
+    expect("packed odd dim", packed(q, TJ_F16, 16, 1, 2, 2, 64, 20, rows3, len, nullptr, nullptr), TJ_ERR_ALIGN);
+    expect("packed missing q", packed(nullptr, TJ_F16, 16, 1, 2, 2, 64, 64, rows3, len, nullptr, nullptr), TJ_ERR_SHAPE);
+    expect("packed missing offsets", packed(q, TJ_F16, 16, 1, 2, 2, 64, 64, rows3, nullptr, nullptr, nullptr), TJ_ERR_SHAPE);
+    expect("packed no rest", packed(q, TJ_F16, 16, 1, 2, 2, 64, 64, rows3, len, stats, nullptr), TJ_ERR_SHAPE);
+    expect("packed rest of fp32", packed(q, TJ_F32, 16, 1, 2, 2, 64, 64, rows3, len, stats, o), TJ_ERR_SHAPE);
+    expect("packed inner stride", packed(q, TJ_F16, 16, 1, 2, 2, 64, 64, rows3_inner, len, nullptr, nullptr), TJ_ERR_ALIGN);
+    expect("packed far rows", packed(q, TJ_F16, 16, 1, 2, 2, 64, 64, rows3_far, len, nullptr, nullptr), TJ_ERR_UNSUPPORTED);
+    expect("packed empty", packed(nullptr, TJ_F16, 0, 1, 2, 2, 64, 64, rows3, nullptr, nullptr, nullptr), TJ_OK);
+    expect_size("packed bwd workspace of huge sizes", tj_packed_attn_bwd_workspace_bytes(kBig, 1, 2, 2), 0);
+    auto packed_bwd = [&](int dtype, int64_t T, int64_t D, const void* rest, const float* lse, const int64_t* dst, void* ws,
+                          size_t bytes) {
+      return tj_packed_attn_bwd(q, k, v, o, rest, lse, at(5120), at(5376), at(5632), at(6144), dtype, T, 1, 2, 2, D, 64, rows3,
+                                rows3, rows3, rows3, dst, rows3, rows3, rows3, 0.125f, 1, len, nullptr, ws, bytes, nullptr);
+    };
+    expect("packed bwd dtype", packed_bwd(-1, 16, 64, o, stats, rows3, at(8192), 1 << 20), TJ_ERR_DTYPE);
+    expect("packed bwd huge T", packed_bwd(TJ_F16, kBig, 64, o, stats, rows3, at(8192), 1 << 20), TJ_ERR_SHAPE);
+    expect("packed bwd head dim", packed_bwd(TJ_F16, 16, 256, o, stats, rows3, at(8192), 1 << 20), TJ_ERR_UNSUPPORTED);
+    expect("packed bwd no lse", packed_bwd(TJ_F16, 16, 64, o, nullptr, rows3, at(8192), 1 << 20), TJ_ERR_SHAPE);
+    expect("packed bwd no rest", packed_bwd(TJ_F16, 16, 64, nullptr, stats, rows3, at(8192), 1 << 20), TJ_ERR_SHAPE);
+    expect("packed bwd inner stride", packed_bwd(TJ_F16, 16, 64, o, stats, rows3_inner, at(8192), 1 << 20), TJ_ERR_ALIGN);
+    expect("packed bwd far rows", packed_bwd(TJ_F16, 16, 64, o, stats, rows3_far, at(8192), 1 << 20), TJ_ERR_UNSUPPORTED);
+    expect("packed bwd workspace", packed_bwd(TJ_F16, 16, 64, o, stats, rows3, nullptr, 0), TJ_ERR_WORKSPACE);
+    expect("packed bwd small workspace", packed_bwd(TJ_F16, 16, 64, o, stats, rows3, at(8192), 32), TJ_ERR_WORKSPACE);
+    expect("packed bwd workspace alignment", packed_bwd(TJ_F16, 16, 64, o, stats, rows3, at(8196), 1 << 20), TJ_ERR_ALIGN);
+    expect("packed bwd empty", packed_bwd(TJ_F16, 0, 64, nullptr, nullptr, rows3, nullptr, 0), TJ_OK);
+
+    // tj_tree_attn_fwd(q, k, v, o, dtype, B, H, Hk, Sq, Sk, D, Dv, strides x4, scale, lengths, parents, workspace, bytes, stream)
+    auto tree = [&](const void* fq, int dtype, int64_t B, int64_t H, int64_t Hk, int64_t Sq, int64_t Sk, int64_t D,
+                    const int64_t* fst, const int32_t* lengths, const int32_t* parents, void* ws, size_t bytes) {
+      return tj_tree_attn_fwd(fq, k, v, o, dtype, B, H, Hk, Sq, Sk, D, 64, fst, st, st, st, 0.125f, lengths, parents, ws, bytes,
+                              nullptr);
+    };
+    expect("tree dtype", tree(q, 4, 1, 2, 2, 1, 64, 64, st, len, nullptr, at(8192), 1 << 20), TJ_ERR_DTYPE);
+    expect("tree shared heads", tree(q, TJ_F16, 1, 3, 2, 1, 64, 64, st, len, nullptr, at(8192), 1 << 20), TJ_ERR_SHAPE);
+    expect("tree huge B", tree(q, TJ_F16, kBig, 2, 2, 1, 64, 64, st, len, nullptr, at(8192), 1 << 20), TJ_ERR_SHAPE);
+    expect("tree huge Sq", tree(q, TJ_F16, 1, 2, 2, kBig, 64, 64, st, len, nullptr, at(8192), 1 << 20), TJ_ERR_SHAPE);
+    expect("tree huge Sk", tree(q, TJ_F16, 1, 2, 2, 1, kBig, 64, st, len, nullptr, at(8192), 1 << 20), TJ_ERR_SHAPE);
+    expect("tree head dim", tree(q, TJ_F16, 1, 2, 2, 1, 64, 136, st, len, nullptr, at(8192), 1 << 20), TJ_ERR_UNSUPPORTED);
+    expect("tree drafts", tree(q, TJ_F16, 1, 2, 2, 65, 64, 64, st, len, len, at(8192), 1 << 20), TJ_ERR_UNSUPPORTED);
+    expect("tree lengths", tree(q, TJ_F16, 1, 2, 2, 1, 64, 64, st, nullptr, nullptr, at(8192), 1 << 20), TJ_ERR_SHAPE);
+    expect("tree inner stride", tree(q, TJ_F16, 1, 2, 2, 1, 64, 64, st_bad_inner, len, nullptr, at(8192), 1 << 20), TJ_ERR_ALIGN);
+    expect("tree parents alignment", tree(q, TJ_F16, 1, 2, 2, 1, 64, 64, st, len, static_cast<const int32_t*>(at(4098)), at(8192), 1 << 20), TJ_ERR_ALIGN);
+    expect("tree workspace", tree(q, TJ_F16, 1, 2, 2, 1, 4096, 64, st, len, nullptr, nullptr, 0), TJ_ERR_WORKSPACE);
+    expect("tree workspace alignment", tree(q, TJ_F16, 1, 2, 2, 1, 64, 64, st, len, nullptr, at(8196), 1 << 20), TJ_ERR_ALIGN);
+    expect("tree empty", tree(nullptr, TJ_F16, 0, 2, 2, 1, 64, 64, st, nullptr, nullptr, nullptr, 0), TJ_OK);
+    expect_size("tree workspace of huge sizes", tj_tree_attn_workspace_bytes(TJ_F16, kBig, 2, 2, 1, 64, 64, 64), 0);
+    expect_size("tree workspace of no type", tj_tree_attn_workspace_bytes(9, 1, 2, 2, 1, 64, 64, 64), 0);
   }
 
   if (g_failures != 0) {

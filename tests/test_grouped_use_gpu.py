@@ -1,0 +1,573 @@
+"""Attention with grouped heads as programs use it: masks and rows at the edges, strides, streams, graphs, sizes (GPU)."""
+
+from __future__ import annotations
+
+import random
+
+import pytest
+import torch
+
+from graph_capture import captured, replay
+from grouped_reference import check, packed, tree
+from test_grouped_gpu import DTYPES, compare_packed, inputs, ints, norm_of, offsets_of, run_packed
+
+from techjam_amd import UnsupportedCaseError
+
+pytestmark = pytest.mark.gpu
+
+
+def same(a, b):
+    return all(torch.equal(x, y) for x, y in zip(a.values(), b.values()))
+
+
+# -- every kernel instance -------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [32, 64, 96, 128])
+@pytest.mark.parametrize("t,h,hk,longest", [
+    (700, 2, 1, 260),      # few tiles: 32 rows a workgroup
+    (4300, 4, 2, 420),     # more: 64 rows
+    (18500, 8, 2, 300),    # many: 128 rows
+])
+def test_launch_sizes(dtype, d, t, h, hk, longest):
+    """Ragged sequences in a buffer they do not fill; what fills the chip is made of many short ones."""
+    rng = random.Random(d)
+    lengths = []
+    while sum(lengths) < t - longest - 40:
+        lengths.append(rng.choice((longest, rng.randint(0, longest), rng.randint(0, 40))))
+    first = 17
+    q, k, v, dout = inputs(t, h, hk, d, d, dtype, seed=t + d)
+    offsets = offsets_of(lengths, first)
+    # The first and last few sequences in 64 bits, all of them against the same call on their own rows.
+    got = run_packed(q, k, v, offsets, True, dout)
+    some = sorted(set(range(min(4, len(lengths)))) | set(range(max(0, len(lengths) - 4), len(lengths))))
+    for n in some:
+        a, b = offsets[n], offsets[n + 1]
+        want = packed(q[a:b], k[a:b], v[a:b], [0, b - a], True, None, None, dout[a:b])
+        for name, (value, bound) in want.items():
+            check(f"{name} of sequence {n}", got[name][a:b], value, bound)
+    for name, x in got.items():
+        assert not x[:first].any() and not x[offsets[-1]:].any(), name
+    again = run_packed(q, k, v, offsets, True, dout)
+    assert same(got, again)
+    with torch.no_grad():
+        assert torch.equal(run_packed(q, k, v, offsets, True)["out"], got["out"])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_one_long_sequence(dtype):
+    """Whole tiles without a mask beside the diagonal's."""
+    q, k, v, dout = inputs(1500, 4, 2, 64, 64, dtype)
+    for causal in (True, False):
+        compare_packed(q, k, v, [0, 1500], causal, dout)
+
+
+@pytest.mark.parametrize("n", [252, 253, 254, 255, 300, 4200])
+@pytest.mark.parametrize("causal", [True, False])
+def test_many_sequences(n, causal):
+    """Tiles are found by counting all regions up to 256 of them, and by their slots beyond."""
+    rng = random.Random(n)
+    lengths = [rng.choice((0, 1, 2, 5)) for _ in range(n)]
+    lengths[n // 2] = 70
+    t = sum(lengths) + 3
+    q, k, v, dout = inputs(t, 2, 1, 32, 32, torch.float16, seed=n)
+    offsets = offsets_of(lengths, 2)
+    got = run_packed(q, k, v, offsets, causal, dout)
+    # Short sequences together, as one block of a mask.
+    owner = torch.full((t,), -1)
+    for i, (a, b) in enumerate(zip(offsets[:-1], offsets[1:])):
+        owner[a:b] = i
+    owner = owner.cuda()
+    for a in range(0, t, 512):
+        rows = slice(a, min(t, a + 512))
+        lo, hi = max(0, a - 100), min(t, a + 612)
+        seen = (owner[rows, None] == owner[None, lo:hi]) & (owner[rows, None] >= 0)
+        if causal:
+            i = torch.arange(t, device="cuda")
+            seen = seen & (i[None, lo:hi] <= i[rows, None])
+        from grouped_reference import Head
+
+        for head in range(2):
+            one = Head(q[rows, head], k[lo:hi, 0], v[lo:hi, 0], seen, 32 ** -0.5, q.dtype)
+            check("out", got["out"][rows, head], one.out, one.out_tol)
+    assert all(torch.isfinite(x).all() for x in got.values())
+    # The gradients, sequence by sequence where there are few rows.
+    for i in (n // 2, 0, n - 1):
+        a, b = offsets[i], offsets[i + 1]
+        if a == b:
+            continue
+        want = packed(q[a:b], k[a:b], v[a:b], [0, b - a], causal, None, None, dout[a:b])
+        for name, (value, bound) in want.items():
+            check(name, got[name][a:b], value, bound)
+
+
+# -- rows without tokens, values that are not finite -------------------------------
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("causal", [True, False])
+def test_padded_batch(dtype, causal):
+    b, s = 5, 77
+    valid = [77, 40, 0, 1, 90]  # the last clipped
+    q, k, v, dout = inputs(b * s, 4, 2, 64, 64, dtype)
+    hidden = torch.zeros(b * s, dtype=torch.bool, device="cuda")
+    for n, m in enumerate(valid):
+        hidden[n * s + min(m, s):(n + 1) * s] = True
+    for x in (q, k, v, dout):  # not read
+        x.masked_fill_(hidden[:, None, None], float("nan"))
+    got = run_packed(q, k, v, list(range(0, b * s + 1, s)), causal, dout, valid)
+    clean = [x.masked_fill(hidden[:, None, None], 0) for x in (q, k, v, dout)]
+    want = packed(*clean[:3], list(range(0, b * s + 1, s)), causal, None, valid, clean[3])
+    for name, (value, bound) in want.items():
+        check(name, got[name], value, bound, norm_of(dtype))
+        assert not got[name][hidden].any()
+
+
+def test_negative_valid_lengths_are_none():
+    q, k, v, dout = inputs(20, 2, 1, 32, 32, torch.float16)
+    got = run_packed(q, k, v, [0, 20], True, dout, [-3])
+    assert not any(x.any() for x in got.values())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_of_no_sequence_are_not_read(dtype):
+    t, lengths, first = 300, [100, 0, 60], 20
+    q, k, v, dout = inputs(t, 4, 2, 64, 64, dtype)
+    offsets = offsets_of(lengths, first)
+    for x in (q, k, v, dout):
+        x[:first] = float("nan")
+        x[offsets[-1]:] = float("inf")
+    got = run_packed(q, k, v, offsets, True, dout)
+    a, b = first, offsets[-1]
+    want = packed(q[a:b], k[a:b], v[a:b], [n - a for n in offsets], True, None, None, dout[a:b])
+    for name, (value, bound) in want.items():
+        check(name, got[name][a:b], value, bound, norm_of(dtype))
+        assert not got[name][:a].any() and not got[name][b:].any()
+
+
+@pytest.mark.parametrize("offsets", [[0], [5], [0, 0], [7, 7, 7], [0, 0, 9, 9]])
+def test_empty_sequences(offsets):
+    q, k, v, dout = inputs(9, 2, 1, 32, 32, torch.bfloat16)
+    compare_packed(q, k, v, offsets, True, dout, norm=False)
+
+
+def test_no_rows_at_all():
+    from techjam_amd.kernels import packed_attention, tree_attention
+
+    q, k, v, dout = inputs(0, 4, 2, 64, 32, torch.float32)
+    got = run_packed(q, k, v, [0, 0], True, dout)
+    assert got["out"].shape == (0, 4, 32) and got["dk"].shape == (0, 2, 64)
+    z = torch.zeros
+    with torch.no_grad():
+        for b, t, c in ((0, 1, 8), (2, 0, 8), (2, 1, 0)):
+            out = tree_attention(z(b, 4, t, 64, device="cuda"), z(b, 2, c, 64, device="cuda"), z(b, 2, c, 32, device="cuda"),
+                                 ints([3] * b))
+            assert out.shape == (b, 4, t, 32) and not out.any()
+    with pytest.raises(ValueError):
+        packed_attention(q, k, v, ints([0]).long())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_offsets_out_of_order_stay_inside(dtype):
+    """Wrong rows, as documented, but nothing outside of the tensors: the buffers around them stay as they were."""
+    t, h, hk, d = 200, 4, 2, 64
+    rng = random.Random(3)
+    for offsets in ([0, 500, 100, 200], [-50, 20, 10, 1 << 30], [150, 100, 50, 0], [200, 0, 200, 0, 200], [-5, -4],
+                    [rng.randint(-300, 500) for _ in range(40)], [(1 << 31) - 1, -(1 << 31), 7] * 30,
+                    [rng.randint(0, 200) for _ in range(400)]):
+        q, k, v, dout = inputs(t, h, hk, d, d, dtype)
+        got = run_packed(q, k, v, offsets, True, dout)
+        assert [tuple(x.shape) for x in got.values()] == [(t, h, d), (t, h, d), (t, hk, d), (t, hk, d)]
+    torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_spoiled_sequence_spoils_itself_only(dtype):
+    lengths = [60, 50, 70]
+    q, k, v, dout = inputs(sum(lengths), 2, 2, 64, 64, dtype)
+    want = run_packed(q, k, v, offsets_of(lengths), True, dout)
+    for x in (q, k, v, dout):
+        x[80, 0, 3] = float("nan")
+    got = run_packed(q, k, v, offsets_of(lengths), True, dout)
+    for name in got:
+        assert torch.equal(got[name][:60], want[name][:60]) and torch.equal(got[name][110:], want[name][110:]), name
+        assert torch.equal(got[name][:, 1], want[name][:, 1]), name  # the other head
+    assert torch.isnan(got["out"][80:110, 0]).all()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_keys_to_come_may_hold_anything_that_is_finite(dtype):
+    """The largest numbers of a type in masked places: their scores overflow and are not seen."""
+    q, k, v, _ = inputs(64, 2, 1, 64, 64, dtype)
+    k[40:] = torch.finfo(dtype).max
+    v[40:] = torch.finfo(dtype).max
+    got = run_packed(q, k, v, [0, 64], True)["out"][:40]
+    value, bound = packed(q[:40], k[:40], v[:40], [0, 40], True)["out"]
+    check("out", got, value, bound)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("scale", [0.0, -0.2, 1.0, 1e-30, 30.0])
+def test_scales(dtype, scale):
+    q, k, v, dout = inputs(150, 4, 2, 64, 64, dtype)
+    compare_packed(q, k, v, [0, 40, 150], True, dout, scale=scale, norm=False)
+
+
+@pytest.mark.parametrize("size", [1e-4, 1.0, 100.0])
+def test_small_and_large_gradients_of_fp16(size):
+    """dS is lifted to fp16's bits by powers of two; what is below 2^-24 in the result is rounded to its steps."""
+    lengths = [200, 300]
+    q, k, v, dout = inputs(500, 2, 1, 64, 64, torch.float16)
+    dout = (dout.float() * size).half()
+    dout[200:] /= 64  # another sequence's gradients do not take its bits
+    compare_packed(q, k, v, offsets_of(lengths), True, dout, norm=False)
+
+
+# -- strides, devices, streams, graphs ---------------------------------------------
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_layouts(dtype):
+    q, k, v, dout = inputs(90, 4, 2, 64, 64, dtype)
+    offsets = [0, 50, 90]
+    want = run_packed(q.contiguous(), k.contiguous(), v.contiguous(), offsets, True, dout)
+
+    def odd(x):  # rows that are not aligned
+        big = torch.empty(*x.shape[:2], x.shape[2] + 1, dtype=x.dtype, device="cuda")
+        big[..., 1:] = x
+        return big[..., 1:]
+
+    def heads_first(x):
+        return x.transpose(0, 1).contiguous().transpose(0, 1)
+
+    def columns_apart(x):
+        return torch.stack((x, x), -1).flatten(2)[..., ::2]
+
+    for view in (odd, heads_first, columns_apart):
+        assert same(run_packed(view(q), view(k), view(v), offsets, True, view(dout)), want), view.__name__
+    one = run_packed(q[:, :1].expand(-1, 4, -1), k, v, offsets, True, dout[:1, :1].expand(90, 4, -1))
+    assert same(one, run_packed(q[:, :1].repeat(1, 4, 1), k, v, offsets, True, dout[:1, :1].repeat(90, 4, 1)))
+
+
+def test_shared_leaves_sum_their_gradients():
+    """One tensor for k and v, and one head's query for all of them."""
+    from techjam_amd.kernels import packed_attention
+
+    _, k, _, dout = inputs(60, 4, 2, 64, 64, torch.float32)
+    q = torch.randn(60, 1, 64, device="cuda")
+    a, b = (x.detach().clone().requires_grad_() for x in (q, k))
+    out = packed_attention(a.expand(-1, 4, -1), b, b, ints([0, 25, 60]), is_causal=True)
+    da, db = torch.autograd.grad(out, (a, b), dout)
+    want = packed(q.expand(-1, 4, -1), k, k, [0, 25, 60], True, None, None, dout)
+    total = {"da": (want["dq"][0].sum(1, keepdim=True), want["dq"][1].sum(1, keepdim=True)),
+             "db": (want["dk"][0] + want["dv"][0], want["dk"][1] + want["dv"][1])}
+    for name, got in (("da", da), ("db", db)):
+        value, bound = total[name]
+        check(name, got, value, bound + 8 * 2.0 ** -24 * value.abs() + 1e-6 * bound)
+
+
+def test_gradients_against_differences():
+    """Central differences of a float32 sum: steps of 2^-6 leave their third-order term and rounding, both below 2%."""
+    q, k, v, dout = inputs(40, 2, 1, 32, 32, torch.float32)
+    dout = dout * 10
+    got = run_packed(q, k, v, [0, 13, 40], True, dout)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    for name, x in (("dq", q), ("dk", k), ("dv", v)):
+        for _ in range(3):
+            way = torch.randn(x.shape, generator=g, device="cuda")
+            step = 2.0 ** -6
+            ends = []
+            for sign in (1, -1):
+                moved = {"dq": q, "dk": k, "dv": v}
+                moved[name] = x + sign * step * way
+                ends.append((packed(moved["dq"], moved["dk"], moved["dv"], [0, 13, 40], True)["out"][0] * dout).sum())
+            slope = (ends[0] - ends[1]) / (2 * step)
+            assert abs((got[name] * way).sum() - slope) <= 0.02 * (got[name].norm() * way.norm()), name
+
+
+def test_derivatives_that_are_not_implemented():
+    from techjam_amd.kernels import packed_attention
+
+    q, k, v, dout = inputs(20, 2, 1, 32, 32, torch.float32)
+    a = q.detach().requires_grad_()
+    out = packed_attention(a, k, v, ints([0, 20]), is_causal=True)
+    (grad,) = torch.autograd.grad(out, a, dout, create_graph=True)
+    assert torch.equal(grad, run_packed(q, k, v, [0, 20], True, dout)["dq"])
+    with pytest.raises(UnsupportedCaseError, match="second derivatives"):
+        grad.sum().backward()
+    for again in (dout, dout.clone().requires_grad_()):
+        out = packed_attention(a, k, v, ints([0, 20]), is_causal=True)
+        (grad,) = torch.autograd.grad(out, a, again, create_graph=True)
+        with pytest.raises(UnsupportedCaseError, match="second derivatives"):
+            torch.autograd.grad(grad.square().sum() + a.sum(), a)
+    out = packed_attention(a, k, v, ints([0, 20]), is_causal=True)
+    out.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+
+
+def test_streams():
+    """Calls of two streams at once do not share anything."""
+    q, k, v, dout = inputs(900, 8, 2, 64, 64, torch.bfloat16)
+    offsets = [0, 100, 420, 900]
+    want = run_packed(q, k, v, offsets, True, dout)
+    want2 = run_packed(k.repeat(1, 4, 1), q[:, :2], v, offsets, False, dout)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    results = []
+    for _ in range(4):
+        for n, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                results.append((n, run_packed(q, k, v, offsets, True, dout) if n == 0 else
+                                run_packed(k.repeat(1, 4, 1), q[:, :2], v, offsets, False, dout)))
+    torch.cuda.synchronize()
+    assert all(same(r, want if n == 0 else want2) for n, r in results)
+
+
+def test_training_step_replays_in_a_graph():
+    """Two graphs, replayed in turn with new inputs and eager work between."""
+    from techjam_amd.kernels import packed_attention
+
+    def setup(dtype, seed):
+        q, k, v, dout = inputs(400, 4, 2, 64, 64, dtype, seed)
+        leaves = [x.detach().clone().requires_grad_() for x in (q, k, v)]
+        offsets, dout = ints([0, 150, 400]), dout.clone()
+
+        def call():
+            out = packed_attention(*leaves, offsets, is_causal=True)
+            return [out, *torch.autograd.grad(out, leaves, dout)]
+
+        return leaves, offsets, dout, call
+
+    programs = [setup(torch.float16, 1), setup(torch.bfloat16, 2)]
+    graphs = [captured(p[3]) for p in programs]
+    for n in range(4):
+        for (leaves, offsets, dout, call), (graph, held) in zip(programs, graphs):
+            with torch.no_grad():
+                for x in leaves:
+                    x.normal_()
+                dout.normal_()
+                offsets.copy_(ints([0, 20 + 90 * n, 400 - n]))
+            torch.cuda.synchronize()
+            replay(graph)
+            torch.cuda.synchronize()
+            got = [x.detach().clone() for x in held]
+            want = run_packed(*leaves, offsets.tolist(), True, dout)
+            assert same(dict(enumerate(got)), dict(enumerate(want.values())))
+
+
+# -- drafts ------------------------------------------------------------------------
+
+def draft_inputs(b, h, hk, t, c, d, dtype, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    q = (1.5 * torch.randn(b, t, h, d, generator=g, device="cuda")).to(dtype).transpose(1, 2)
+    return q, torch.randn(b, hk, c, d, generator=g, device="cuda").to(dtype), torch.randn(b, hk, c, d, generator=g, device="cuda").to(dtype)
+
+
+def run_tree(q, k, v, lengths, parents=None, **kw):
+    from techjam_amd.kernels import tree_attention
+
+    with torch.no_grad():
+        return tree_attention(q, k, v, ints(lengths), None if parents is None else ints(parents), **kw)
+
+
+def compare_tree(q, k, v, lengths, parents=None, **kw):
+    out = run_tree(q, k, v, lengths, parents, **kw)
+    value, bound = tree(q, k, v, lengths, parents, kw.get("scale"))
+    check("out", out, value, bound, None if "scale" in kw else norm_of(q.dtype))
+    return out
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [32, 64, 96, 128])
+@pytest.mark.parametrize("h,t", [(2, 3), (4, 12), (8, 15), (8, 40)])  # rows of a key head: 6, 48, 120, 320
+def test_draft_launches(dtype, d, h, t):
+    """Workgroups of 32, 64, 128 and 256 rows, keys in parts."""
+    rng = random.Random(h * t + d)
+    b, c = 3, 700
+    q, k, v = draft_inputs(b, h, 1, t, c, d, dtype, seed=d)
+    lengths = [700, 333, t]
+    parents = [[rng.randint(max(-1, i - 5), i - 1) for i in range(t)] for _ in range(b)]
+    compare_tree(q, k, v, lengths, parents)
+    compare_tree(q, k, v, lengths)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_sequences_that_fill_the_chip_are_swept_whole(dtype):
+    b = 300
+    q, k, v = draft_inputs(b, 4, 4, 2, 40, 32, dtype)
+    lengths = [(7 * n) % 42 for n in range(b)]
+    out = compare_tree(q, k, v, lengths)
+    assert not out[0].any() and not out[6].any()  # lengths 0
+    parents = [[-1, n % 3 - 1] for n in range(b)]  # -1, 0, or itself: not there
+    compare_tree(q, k, v, lengths, parents)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_many_sequences_of_few_rows(dtype):
+    """More sequences than a workgroup looks at: as many parts for each."""
+    b = 150
+    q, k, v = draft_inputs(b, 2, 1, 1, 300, 32, dtype)
+    compare_tree(q, k, v, [(37 * n) % 301 for n in range(b)])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_tree_that_is_a_chain_is_a_chain(dtype):
+    q, k, v = draft_inputs(2, 4, 2, 20, 150, 64, dtype)
+    chain = [[i - 1 for i in range(20)]] * 2
+    assert torch.equal(run_tree(q, k, v, [150, 77], chain), run_tree(q, k, v, [150, 77]))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_drafts_that_are_not_there_may_hold_anything(dtype):
+    """Slots behind the used ones, their descendants, and what stands behind the length: NaN in the cache and in q."""
+    b, t, c = 4, 12, 260
+    q, k, v = draft_inputs(b, 4, 2, t, c, 64, dtype)
+    parents = [[-1, 0, 1, 1, 0, 12, 5, 3, 12, 12, 12, 12],   # 5 is not there, and so is its child 6
+               [12] * 12,                                    # nothing is
+               [-1] * 6 + [99, -2, 8, 6, 1 << 30, -(1 << 31)],
+               list(range(-1, 11))]
+    lengths = [250, 40, 260, 7]                              # the last: five drafts at negative positions
+    gone = [{5, 6, 8, 9, 10, 11}, set(range(12)), {6, 7, 8, 9, 10, 11}, set(range(12))]
+    clean = tree(q, k, v, lengths, parents)
+    for n in range(b):
+        for i in gone[n]:
+            q[n, :, i] = float("nan")
+            at = lengths[n] - t + i
+            if at >= 0:
+                k[n, :, at] = float("nan")
+                v[n, :, at] = float("inf")
+        k[n, :, lengths[n]:] = float("nan")
+        v[n, :, lengths[n]:] = float("nan")
+    out = run_tree(q, k, v, lengths, parents)
+    check("out", out, *clean, norm_of(dtype))
+    for n in range(b):
+        assert not out[n][:, sorted(gone[n])].any()
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_a_draft_sees_its_line_only(dtype):
+    """Other branches' keys, however large, change nothing."""
+    q, k, v = draft_inputs(1, 2, 1, 6, 100, 64, dtype)
+    parents = [[-1, 0, 0, 1, 2, -1]]
+    before = run_tree(q, k, v, [100], parents)
+    k[0, :, 96] *= 50  # draft 2
+    v[0, :, 96] *= 50
+    after = run_tree(q, k, v, [100], parents)
+    assert torch.equal(before[0, :, [0, 1, 3, 5]], after[0, :, [0, 1, 3, 5]])
+    assert not torch.equal(before[0, :, 2], after[0, :, 2]) and not torch.equal(before[0, :, 4], after[0, :, 4])
+
+
+@pytest.mark.parametrize("t", [1, 2, 31, 32, 33, 63, 64])
+def test_numbers_of_drafts(t):
+    rng = random.Random(t)
+    q, k, v = draft_inputs(2, 2, 2, t, 64 + t, 32, torch.float16)
+    for lengths in ([t, t + 1], [64 + t, t + 31], [t + 33, t + 32]):
+        compare_tree(q, k, v, lengths, [[rng.randint(-1, i - 1) for i in range(t)] for _ in range(2)])
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.3, 1.0])
+def test_draft_scales(scale):
+    q, k, v = draft_inputs(2, 4, 2, 5, 90, 64, torch.bfloat16)
+    compare_tree(q, k, v, [90, 50], [[-1, 0, 0, 2, 1]] * 2, scale=scale)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_cache_layouts(dtype):
+    b, h, hk, t, c, d = 2, 4, 2, 3, 80, 64
+    q, k, v = draft_inputs(b, h, hk, t, c, d, dtype)
+    want = run_tree(q, k, v, [80, 33])
+
+    def tokens_first(x):  # [B, C, Hk, D] storage
+        return x.transpose(1, 2).contiguous().transpose(1, 2)
+
+    def longer(x):        # part of a larger cache
+        big = x.new_full((x.shape[0] + 1, x.shape[1], x.shape[2] + 7, x.shape[3]), float("nan"))
+        big[1:, :, :x.shape[2]] = x
+        return big[1:, :, :x.shape[2]]
+
+    def odd(x):
+        big = x.new_empty((*x.shape[:3], x.shape[3] + 1))
+        big[..., 1:] = x
+        return big[..., 1:]
+
+    for view in (tokens_first, longer, odd):
+        assert torch.equal(run_tree(view(q), view(k), view(v), [80, 33]), want), view.__name__
+    out = run_tree(q, k, v, [80, 33])
+    assert out.transpose(1, 2).is_contiguous()
+
+
+def test_a_cache_past_32_bits():
+    """A cache whose second sequence lies 2^31 elements behind its first."""
+    hk, c, d = 4, 65536, 128
+    big = torch.empty((1 << 31) + hk * c * d, dtype=torch.float16, device="cuda")
+    k = big.as_strided((2, hk, c, d), (1 << 31, c * d, d, 1)).normal_()
+    v = torch.randn(2, hk, c, d, device="cuda").half()
+    q = (1.5 * torch.randn(2, 8, 2, d, device="cuda")).half()
+    out = run_tree(q, k, v, [300, 65536])
+    for n, length in enumerate((300, 65536)):
+        check(f"sequence {n}", out[n:n + 1], *tree(q[n:n + 1], k[n:n + 1], v[n:n + 1], [length]), norm_of(torch.float16))
+
+
+def test_packed_rows_past_32_bits():
+    """Tokens of a wide projection whose last rows begin 2^31 elements behind the first."""
+    width, t = 1 << 18, (1 << 13) + 40
+    big = torch.empty(t * width, dtype=torch.float16, device="cuda")
+    q, k, v = (big.as_strided((t, 2, 64), (width, 64, 1), 128 * n) for n in range(3))
+    for x in (q, k, v):
+        x.normal_()
+    dout = torch.randn(t, 2, 64, device="cuda").half()
+    offsets = [0, 30, (1 << 13) - 1, t]
+    got = run_packed(q, k, v, offsets, True, dout)
+    a, b = offsets[-2], t
+    want = packed(q[a:b], k[a:b], v[a:b], [0, b - a], True, None, None, dout[a:b])
+    for name, (value, bound) in want.items():
+        check(name, got[name][a:b], value, bound, norm_of(torch.float16))
+
+
+def test_drafts_on_streams_and_in_graphs():
+    q, k, v = draft_inputs(3, 8, 2, 8, 500, 64, torch.float16)
+    from techjam_amd.kernels import tree_attention
+
+    lengths, parents = ints([500, 200, 8]), ints([[-1, 0, 1, 0, 3, 8, -1, 6]] * 3)
+    want = run_tree(q, k, v, lengths.tolist(), parents.tolist())
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        again = run_tree(q, k, v, lengths.tolist(), parents.tolist())
+    torch.cuda.synchronize()
+    assert torch.equal(again, want)
+
+    with torch.no_grad():
+        graphs = [captured(lambda: tree_attention(q, k, v, lengths, parents)), captured(lambda: tree_attention(q, k, v, lengths))]
+        for n in range(4):
+            lengths.copy_(ints([500 - 40 * n, 30 * n + 8, 8 + n]))
+            q.normal_()
+            for (graph, held), tree_of in zip(graphs, (parents.tolist(), None)):
+                replay(graph)
+                torch.cuda.synchronize()
+                assert torch.equal(held, run_tree(q, k, v, lengths.tolist(), tree_of))
+
+
+def test_refusals_on_the_gpu():
+    from techjam_amd.kernels import packed_attention, tree_attention
+
+    q, k, v, _ = inputs(8, 4, 2, 64, 64, torch.float16)
+    good = ints([0, 8])
+    for offsets in (good.cpu(), good.long(), good[None], ints([0, 4, 8, 9])[::2], None, [0, 8], good[:0]):
+        with pytest.raises(ValueError):
+            packed_attention(q, k, v, offsets)
+    for valid in (ints([8, 8]), ints([8]).cpu(), ints([8]).long(), ints(8)):
+        with pytest.raises(ValueError):
+            packed_attention(q, k, v, good, valid_len=valid)
+    with pytest.raises(ValueError):
+        packed_attention(q, k.cpu(), v, good)
+    q, k, v = draft_inputs(2, 4, 2, 3, 16, 64, torch.float16)
+    with torch.no_grad():
+        for parents in (ints([[-1, 0, 1]]), ints([[-1, 0]] * 2), ints([[-1, 0, 1]] * 2).long(), ints([[-1, 0, 1]] * 2).cpu(),
+                        ints([[-1] * 2] * 3).T, ints([-1, 0, 1])):
+            with pytest.raises(ValueError):
+                tree_attention(q, k, v, ints([5, 5]), parents)
+        for lengths in (ints([5]), ints([5, 5]).cpu(), ints([5, 5]).long()):
+            with pytest.raises(ValueError):
+                tree_attention(q, k, v, lengths)
+    with pytest.raises(UnsupportedCaseError):
+        tree_attention(q.requires_grad_(), k, v, ints([5, 5]))
