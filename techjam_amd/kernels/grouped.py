@@ -19,7 +19,7 @@ import torch.nn.functional as F
 from ..errors import UnsupportedCaseError
 from . import _lib
 from .attention import _ptr, _require_device, _stream_ptr
-from .differential import DTYPES, _empty_heads, _rows_view, _scale, on_device, refuse_tangents
+from .differential import DTYPES, _empty_heads, _rows_view, _scale, refuse_tangents
 
 #: Largest head dim of q and k, and of v.
 MAX_HEAD_DIM = 128
@@ -27,25 +27,36 @@ MAX_HEAD_DIM = 128
 MAX_DRAFTS = 64
 
 
-def _tokens_view(t: torch.Tensor) -> torch.Tensor:
-    """``t`` ``[T, H, D]`` itself when the kernels can read it in place (unit innermost
-    stride, rows and base aligned to 16 bytes, 64 tokens within 2 GiB), else a contiguous copy."""
+def _readable(t: torch.Tensor) -> bool:
+    """Unit innermost stride, rows and base aligned to 16 bytes, 64 tokens within 2 GiB."""
+    st, sh, sd = t.stride()
     size = t.element_size()
+    return sd == 1 and not (st | sh) & (16 // size - 1) and not t.data_ptr() & 15 and st * 64 * size < 1 << 31
 
-    def readable(t):
-        st, sh, sd = t.stride()
-        return sd == 1 and not (st | sh) & (16 // size - 1) and not t.data_ptr() & 15 and st * 64 * size < 1 << 31
 
-    if readable(t):
+def _tokens_view(t: torch.Tensor) -> torch.Tensor:
+    """``t`` ``[T, H, D]`` itself when the kernels can read it in place, else a contiguous copy."""
+    if _readable(t):
         return t
     if min(t.shape[:2]) <= 1:
         # The stride of a dimension of at most one is never used, may be anything,
         # and stays what it is in contiguous(): 0 instead.
         t = t.as_strided(t.shape, [0 if n <= 1 else st for n, st in zip(t.shape[:2], t.stride())] + [t.stride(2)])
-        if readable(t):
+        if _readable(t):
             return t
     t = t.contiguous()
     return t.clone() if t.data_ptr() & 15 else t
+
+
+def _launch(dev: torch.device, entry: str, *args) -> None:
+    """Calls the library with the device current and its current stream as the last argument."""
+    if torch._C._cuda_getDevice() == dev.index:
+        code = getattr(_lib.lib(), entry)(*args, _stream_ptr(dev))
+    else:
+        with torch.cuda.device(dev):
+            code = getattr(_lib.lib(), entry)(*args, _stream_ptr(dev))
+    if code:
+        _lib.check(code, entry)
 
 
 def _check_types(q, k, v, h: int, hk: int) -> None:
@@ -91,16 +102,12 @@ def _forward(q, k, v, offsets, valid_len, scale, causal, stats):
     t, h, d = q.shape
     _, hk, dv = v.shape
     q, k, v = _tokens_view(q), _tokens_view(k), _tokens_view(v)
-    dev = q.device
     out = q.new_empty((t, h, dv))
     lse = q.new_empty((t, h), dtype=torch.float32) if stats else None
     rest = torch.empty_like(out) if stats and q.dtype != torch.float32 else None
-    with on_device(dev):
-        code = _lib.lib().tj_packed_attn_fwd(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), DTYPES[q.dtype], t, offsets.shape[0] - 1, h, hk, d, dv,
-            _lib.strides3(q), _lib.strides3(k), _lib.strides3(v), _lib.strides3(out), scale, int(causal),
-            offsets.data_ptr(), _ptr(valid_len), _ptr(lse), _ptr(rest), _stream_ptr(dev))
-    _lib.check(code, "tj_packed_attn_fwd")
+    _launch(q.device, "tj_packed_attn_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), DTYPES[q.dtype],
+            t, offsets.shape[0] - 1, h, hk, d, dv, _lib.strides3(q), _lib.strides3(k), _lib.strides3(v), _lib.strides3(out),
+            scale, causal, offsets.data_ptr(), _ptr(valid_len), _ptr(lse), _ptr(rest))
     return out, rest, lse
 
 
@@ -110,17 +117,13 @@ def _backward(ctx, dout):
     _, hk, dv = v.shape
     n = offsets.shape[0] - 1
     q, k, v, dout = _tokens_view(q), _tokens_view(k), _tokens_view(v), _tokens_view(dout)
-    dev = q.device
     dq, dk, dvv = q.new_empty((t, h, d)), q.new_empty((t, hk, d)), q.new_empty((t, hk, dv))
     floats = _backward_floats(t, n, h, hk)
     ws = lse.new_empty(floats)
-    with on_device(dev):
-        code = _lib.lib().tj_packed_attn_bwd(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(rest), lse.data_ptr(), dout.data_ptr(),
-            dq.data_ptr(), dk.data_ptr(), dvv.data_ptr(), DTYPES[q.dtype], t, n, h, hk, d, dv,
-            *map(_lib.strides3, (q, k, v, out, dout, dq, dk, dvv)), ctx.scale, int(ctx.causal),
-            offsets.data_ptr(), _ptr(valid_len), ws.data_ptr(), 4 * floats, _stream_ptr(dev))
-    _lib.check(code, "tj_packed_attn_bwd")
+    _launch(q.device, "tj_packed_attn_bwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(rest),
+            lse.data_ptr(), dout.data_ptr(), dq.data_ptr(), dk.data_ptr(), dvv.data_ptr(), DTYPES[q.dtype], t, n, h, hk, d, dv,
+            *map(_lib.strides3, (q, k, v, out, dout, dq, dk, dvv)), ctx.scale, ctx.causal,
+            offsets.data_ptr(), _ptr(valid_len), ws.data_ptr(), 4 * floats)
     return dq, dk, dvv, None, None, None, None
 
 
@@ -287,10 +290,7 @@ def tree_attention(
     out = _empty_heads(b, h, t, wide, q)
     floats = _tree_floats(dtype, b, h, hk, t, c, d, wide)
     ws = q.new_empty(floats, dtype=torch.float32) if floats else None
-    with on_device(dev):
-        code = _lib.lib().tj_tree_attn_fwd(
-            q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dtype, b, h, hk, t, c, d, wide,
+    _launch(dev, "tj_tree_attn_fwd", q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), dtype, b, h, hk, t, c, d, wide,
             _lib.strides4(q), _lib.strides4(k), _lib.strides4(v), _lib.strides4(out), scale,
-            lengths.data_ptr(), _ptr(parents), _ptr(ws), 4 * floats, _stream_ptr(dev))
-    _lib.check(code, "tj_tree_attn_fwd")
+            lengths.data_ptr(), _ptr(parents), _ptr(ws), 4 * floats)
     return out if wide == dv else out[..., :dv]

@@ -301,7 +301,7 @@ int main() {
     expect("tree inner stride", tree(q, TJ_F16, 1, 2, 2, 1, 64, 64, st_bad_inner, len, nullptr, at(8192), 1 << 20), TJ_ERR_ALIGN);
     expect("tree parents alignment", tree(q, TJ_F16, 1, 2, 2, 1, 64, 64, st, len, static_cast<const int32_t*>(at(4098)), at(8192), 1 << 20), TJ_ERR_ALIGN);
     expect("tree workspace", tree(q, TJ_F16, 1, 2, 2, 1, 4096, 64, st, len, nullptr, nullptr, 0), TJ_ERR_WORKSPACE);
-    expect("tree workspace alignment", tree(q, TJ_F16, 1, 2, 2, 1, 64, 64, st, len, nullptr, at(8196), 1 << 20), TJ_ERR_ALIGN);
+    expect("tree workspace alignment", tree(q, TJ_F16, 1, 2, 2, 1, 4096, 64, st, len, nullptr, at(8196), 1 << 30), TJ_ERR_ALIGN);
     expect("tree empty", tree(nullptr, TJ_F16, 0, 2, 2, 1, 64, 64, st, nullptr, nullptr, nullptr, 0), TJ_OK);
     expect_size("tree workspace of huge sizes", tj_tree_attn_workspace_bytes(TJ_F16, kBig, 2, 2, 1, 64, 64, 64), 0);
     expect_size("tree workspace of no type", tj_tree_attn_workspace_bytes(9, 1, 2, 2, 1, 64, 64, 64), 0);

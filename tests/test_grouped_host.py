@@ -181,6 +181,7 @@ def test_entry_points_refuse_before_launching():
                                   parents, ws, nb, None)
 
     assert tree() == _lib.TJ_ERR_WORKSPACE
+    assert L.tj_tree_attn_workspace_bytes(_lib.TJ_F16, 1, 4, 2, 1, 1024, 64, 64) == 0  # swept whole
     assert tree(lengths=None) == tree(h=5) == tree(b=1 << 30) == _lib.TJ_ERR_SHAPE
     assert tree(sq=65, parents=p) == _lib.TJ_ERR_UNSUPPORTED
     assert tree(b=0) == _lib.TJ_OK

@@ -390,6 +390,18 @@ def test_draft_launches(dtype, d, h, t):
     compare_tree(q, k, v, lengths)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("d", [32, 64, 96, 128])
+@pytest.mark.parametrize("h,t", [(2, 3), (4, 12), (8, 15), (8, 40)])
+def test_draft_launches_in_parts(dtype, d, h, t):
+    """The same against caches that are not swept whole."""
+    rng = random.Random(h * t + d)
+    q, k, v = draft_inputs(2, h, 1, t, 1500, d, dtype, seed=d)
+    parents = [[rng.randint(max(-1, i - 5), i - 1) for i in range(t)] for _ in range(2)]
+    compare_tree(q, k, v, [1500, 401], parents)
+    compare_tree(q, k, v, [1500, 401])
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_sequences_that_fill_the_chip_are_swept_whole(dtype):
     b = 300
