@@ -191,7 +191,7 @@ __global__ __launch_bounds__(kThreads, (HD * (int)sizeof(T) <= 256 ? 2 : 1)) voi
       dot();
     }
   }
-  const float del = pair_sum(sum);
+  float del = pair_sum(sum);
   const float lse = row.live ? a.lse[(int64_t)(g.start + row.i) * a.H + hk * a.G + row.g] : __builtin_inff();
   // The row's own lift: its lane (and the one of the other half) has all of its dO.
   const DsLift<T> lifts(a, g, hk, lane);
@@ -203,7 +203,8 @@ __global__ __launch_bounds__(kThreads, (HD * (int)sizeof(T) <= 256 ? 2 : 1)) voi
       for (int j = 0; j < 8; ++j) norm = fmaf((float)of[s][j], (float)of[s][j], norm);
     lift = lifts.of(sqrtf(pair_sum(norm)));
   }
-  const float common = lifts.all() / DsLift<T>::kP, c2 = a.scale * kLog2e, d0 = -del * lift;
+  const float common = lifts.all() / DsLift<T>::kP, c2 = a.scale * kLog2e;
+  float d0 = -del * lift;
   float16_t dq[DB];
 #pragma unroll
   for (int d = 0; d < DB; ++d) dq[d] = zero16();
@@ -220,6 +221,16 @@ __global__ __launch_bounds__(kThreads, (HD * (int)sizeof(T) <= 256 ? 2 : 1)) voi
                            [&](int s, frag_t<T> f) { p = Elem<T>::mma(f, qf[s], p); });
     read_ahead<KS, kDepth>([&](int s) { return Rows::row_frag(tile + vrow, s, 0); },
                            [&](int s, frag_t<T> f) { dp = Elem<T>::mma(f, of[s], dp); });
+    if (own_end <= BN) {
+      // Rows of one tile: delta = sum of P dP, exact to what fp32 sums are. (The output's has the rounding of P in it, which
+      // shows where few keys share a row: sequences of two tokens, dQ 1.4 instead of 1.6 times one rounding from 64 bits.)
+      float exact = 0.f;
+#pragma unroll
+      for (int e = 0; e < 16; ++e)
+        if (kv0 + acc_row(e, hl) <= row.limit) exact = fmaf(fast_exp2(fmaf(p[e], c2, -lse)), dp[e], exact);
+      del = pair_sum(exact);
+      d0 = -del * lift;
+    }
 #pragma unroll
     for (int e = 0; e < 16; ++e) p[e] = fast_exp2(fmaf(p[e], c2, -lse)) * fmaf(dp[e], lift, d0);
     // Selected, not multiplied: what a masked key holds does not matter.

@@ -184,7 +184,8 @@ def packed_attention(
     sequences of ``S`` rows. Rows that hold no token, also those before the first and behind the last
     sequence, come out as zeros; what they hold is not read, and their gradients are zero.
 
-    ``scale`` defaults to ``D ** -0.5``; its magnitude is at most 2^127. A NaN or an infinity
+    ``scale`` defaults to ``D ** -0.5``; its magnitude is at most 2^127. Scores are float32 numbers, exact to
+    2^-24 of their size; rows with one beyond 2^27 may come out as NaN. A NaN or an infinity
     among a sequence's tokens spoils what depends on it; one in ``v`` under ``is_causal`` also
     the up to 31 tokens before it in its tile of 32, as 0 times NaN.
 
