@@ -459,8 +459,8 @@ int tj_diff_attn_bwd(const void* q, const void* k, const void* v, const float* m
  *
  * dtype: TJ_F32, TJ_F16 or TJ_BF16, shared by q, k, v and o, with the products of
  * tj_diff_attn_fwd. D and Dv <= 128, both multiples of 16 bytes. Strides in
- * elements, the innermost 1, the others multiples of 16 bytes; 64 rows of k and v (and
- * of q and dout below) within 2 GiB (TJ_ERR_UNSUPPORTED otherwise).
+ * elements, the innermost 1, the others multiples of 16 bytes and below 2^31; 64 rows of k
+ * and v (and of q and dout below) within 2 GiB (TJ_ERR_UNSUPPORTED otherwise).
  *
  * lse and, with 16-bit types, o_rest: what tj_packed_attn_bwd reads again, or NULL:
  * fp32 [T, H], log2 of the rows' softmax sums (rows without a token are not written), and what
@@ -503,7 +503,8 @@ int tj_packed_attn_bwd(const void* q, const void* k, const void* v, const void* 
  * on whose line it stands and those at a negative position: their rows are written as zeros, and
  * what the cache holds in their place may be anything. What it holds behind lengths[b] is not read.
  * Sizes (TJ_ERR_SHAPE past them): B H Sq below 2^23 - 2^16, B Hk below 2^22, B Sk below 2^35.
- * Types, dims and strides as in tj_packed_attn_fwd (four strides). workspace:
+ * Types, dims and strides as in tj_packed_attn_fwd (four strides, of which those of k's and v's heads and all
+ * batches' may be larger). workspace:
  * tj_tree_attn_workspace_bytes bytes, as above; NULL where that is 0.
  */
 size_t tj_tree_attn_workspace_bytes(int dtype, int64_t B, int64_t H, int64_t Hk, int64_t Sq, int64_t Sk,

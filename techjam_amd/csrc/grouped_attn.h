@@ -14,7 +14,7 @@
 
 namespace tj {
 
-// Strided [rows, heads, dim] view with unit dim stride.
+// Strided [rows, heads, dim] view with unit dim stride, the others below 2^31.
 struct View3 {
   int64_t st, sh;
   __device__ __forceinline__ int64_t row(int64_t t, int h) const { return t * st + h * sh; }
@@ -149,7 +149,8 @@ struct Region {
         const int mid = (lo + hi) / 2;
         int x = 0;
 #pragma unroll
-        for (int c = 0; c < kChunks; ++c) x += a.causal ? max(0, n[c] - mid) : (n[c] > mid ? n[c] : 0);
+        for (int c = 0; c < kChunks; ++c)
+          if (c * kWave < regions(a)) x += a.causal ? max(0, n[c] - mid) : (n[c] > mid ? n[c] : 0);
         x = over_wave(x, sum);
         if (x > at) lo = mid;
         else {
@@ -200,10 +201,29 @@ struct Region {
     return false;
   }
 
-  // The tile of workgroup `at`, of as many slots as the launch has.
-  __device__ __forceinline__ bool take(const PackedArgs& a, int at, int per, int unit, bool down, int lane) {
-    if (regions(a) <= kRanked) return ranked(a, at, per, unit, down, lane);
-    return find(a, down ? at : a.n_slots - 1 - at, per, unit, lane);
+  // The tile of workgroup `at`, of as many slots as the launch has, for all of its waves: the first one looks, as the
+  // others would take the vector unit's time for the same numbers. `told`: six integers of LDS.
+  __device__ __forceinline__ bool take(const PackedArgs& a, int at, int per, int unit, bool down, int tid, int* told) {
+    const int lane = tid % kWave;
+    if (tid < kWave) {
+      const bool any = regions(a) <= kRanked ? ranked(a, at, per, unit, down, lane)
+                                             : find(a, down ? at : a.n_slots - 1 - at, per, unit, lane);
+      if (lane == 0) {
+        told[0] = any;
+        told[1] = index;
+        told[2] = start;
+        told[3] = rows;
+        told[4] = len;
+        told[5] = tile;
+      }
+    }
+    __syncthreads();
+    index = __builtin_amdgcn_readfirstlane(told[1]);
+    start = __builtin_amdgcn_readfirstlane(told[2]);
+    rows = __builtin_amdgcn_readfirstlane(told[3]);
+    len = __builtin_amdgcn_readfirstlane(told[4]);
+    tile = __builtin_amdgcn_readfirstlane(told[5]);
+    return __builtin_amdgcn_readfirstlane(told[0]) != 0;
   }
 };
 
@@ -262,16 +282,40 @@ struct WaveRows {
   template <typename V>
   __device__ __forceinline__ static void put(uint32_t at, V x) { *(__attribute__((address_space(3))) V*)(uintptr_t)at = x; }
 
-  // The lane's chunks of the rows; row(n): a pointer to row n's elements, or null where it is not there.
-  template <typename F>
-  __device__ __forceinline__ static void read(vec_t x[N], int width, int lane, F&& row) {
+  // The tokens and heads of the rows that the lane moves, from row `first` of the (region or sequence, key head)
+  // on: tokens from that of row `first`, heads from the group's first. Counted up rather than divided.
+  struct Places {
+    int row, i[N], g[N];
+    __device__ __forceinline__ Places(int first, Divisor group, int lane) : row(first + lane / Rows::kChunks) {
+      const int q = kPer / group, rest = kPer - q * group.n, token = first / group;
+      int at = row / group, head = row - at * group.n;
+#pragma unroll
+      for (int n = 0; n < N; ++n) {
+        i[n] = at - token;
+        g[n] = head;
+        at += q;
+        head += rest;
+        if (head >= group.n) {
+          head -= group.n;
+          ++at;
+        }
+      }
+    }
+    __device__ __forceinline__ int64_t offset(int n, int st, int sh) const { return (int64_t)i[n] * st + (int64_t)g[n] * sh; }
+    __device__ __forceinline__ bool before(int n, int end) const { return row + n * kPer < end; }
+  };
+
+  // The lane's chunks of the rows before `end`; p: the first row's token and the group's first head, whose
+  // tokens are st and heads sh elements apart.
+  __device__ __forceinline__ static void read(vec_t x[N], const T* p, int64_t st, int64_t sh, int width, const Places& places,
+                                              int end, int lane) {
     const int col = lane % Rows::kChunks * Rows::kVec;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-      const T* p = row(n * kPer + lane / Rows::kChunks);
 #pragma unroll
       for (int j = 0; j < Rows::kVec; ++j) x[n][j] = (T)0.f;
-      if (p != nullptr && col < width) x[n] = *reinterpret_cast<const vec_t*>(p + col);
+      if (places.before(n, end) && col < width)
+        x[n] = *reinterpret_cast<const vec_t*>(p + col + places.offset(n, (int)st, (int)sh));
     }
   }
   // They, as the wave's fragments.
@@ -289,8 +333,9 @@ struct WaveRows {
 
   // Accumulators of a transposed product to rows of memory: value(d, c): the four values of the lane's row from
   // column 32 d + 8 c + 4 (lane / 32) on.
-  template <typename V, typename F>
-  __device__ __forceinline__ static void write(uint32_t tile, int width, int lane, V&& value, F&& row) {
+  template <typename V>
+  __device__ __forceinline__ static void write(T* p, int64_t st, int64_t sh, int width, const Places& places, int end,
+                                               uint32_t tile, int lane, V&& value) {
     typedef T t4 __attribute__((ext_vector_type(4)));
     const int r = lane % 32;
 #pragma unroll
@@ -308,8 +353,7 @@ struct WaveRows {
     for (int n = 0; n < N; ++n) {
       const int r = n * kPer + lane / Rows::kChunks;
       const vec_t x = lds_at<vec_t>(tile + r * Rows::kRowBytes + (((lane % Rows::kChunks) ^ Rows::swizzle(r)) << 4));
-      T* p = row(r);
-      if (p != nullptr && col < width) *reinterpret_cast<vec_t*>(p + col) = x;
+      if (places.before(n, end) && col < width) *reinterpret_cast<vec_t*>(p + col + places.offset(n, (int)st, (int)sh)) = x;
     }
   }
 };

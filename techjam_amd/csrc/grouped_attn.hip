@@ -29,6 +29,14 @@ bool view_ok(const void* p, const int64_t* st, int n, int dtype) {
 // Rows that the tile copies reach by 31-bit byte offsets, up to 64 at a time.
 bool rows_ok(int64_t stride, int dtype) { return stride >= 0 && stride < (int64_t(1) << 31) / (64 * elem_bytes(dtype)); }
 
+// The kernels multiply strides as 32-bit numbers, other than a batch's; n strides.
+bool near_ok(std::initializer_list<const int64_t*> views, int n) {
+  for (const int64_t* st : views)
+    for (int i = n - 3; i < n - 1; ++i)
+      if (st[i] >= int64_t(1) << 31 || st[i] <= -(int64_t(1) << 31)) return false;
+  return true;
+}
+
 bool aligned4(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 3u) == 0; }
 
 // Sizes that the kernels' 32-bit row and slot numbers and the grids (workgroups of up to 512
@@ -97,7 +105,9 @@ extern "C" int tj_packed_attn_fwd(const void* q, const void* k, const void* v, v
   if (!view_ok(q, q_strides, 3, dtype) || !view_ok(k, k_strides, 3, dtype) || !view_ok(v, v_strides, 3, dtype) ||
       !view_ok(o, o_strides, 3, dtype) || !tjh::aligned16(o_rest) || !aligned4(offsets) || !aligned4(lengths) || !aligned4(lse))
     return TJ_ERR_ALIGN;
-  if (!rows_ok(k_strides[0], dtype) || !rows_ok(v_strides[0], dtype)) return TJ_ERR_UNSUPPORTED;
+  if (!rows_ok(k_strides[0], dtype) || !rows_ok(v_strides[0], dtype) ||
+      !near_ok({q_strides, k_strides, v_strides, o_strides}, 3))
+    return TJ_ERR_UNSUPPORTED;
   PackedArgs a = packed_args(q, k, v, T, N, H, Hk, D, Dv, q_strides, k_strides, v_strides, o_strides, scale, causal, offsets,
                              lengths);
   a.o = o;
@@ -133,6 +143,8 @@ extern "C" int tj_packed_attn_bwd(const void* q, const void* k, const void* v, c
     return TJ_ERR_ALIGN;
   for (const int64_t* st : {q_strides, k_strides, v_strides, do_strides})
     if (!rows_ok(st[0], dtype)) return TJ_ERR_UNSUPPORTED;
+  if (!near_ok({q_strides, k_strides, v_strides, o_strides, do_strides, dq_strides, dk_strides, dv_strides}, 3))
+    return TJ_ERR_UNSUPPORTED;
   if (workspace == nullptr || workspace_bytes < tj_packed_attn_bwd_workspace_bytes(T, N, H, Hk)) return TJ_ERR_WORKSPACE;
   if (!tjh::aligned16(workspace)) return TJ_ERR_ALIGN;
   PackedArgs a = packed_args(q, k, v, T, N, H, Hk, D, Dv, q_strides, k_strides, v_strides, o_strides, scale, causal, offsets,
@@ -167,7 +179,8 @@ extern "C" int tj_tree_attn_fwd(const void* q, const void* k, const void* v, voi
   if (!view_ok(q, q_strides, 4, dtype) || !view_ok(k, k_strides, 4, dtype) || !view_ok(v, v_strides, 4, dtype) ||
       !view_ok(o, o_strides, 4, dtype) || !aligned4(lengths) || !aligned4(parents))
     return TJ_ERR_ALIGN;
-  if (!rows_ok(k_strides[2], dtype) || !rows_ok(v_strides[2], dtype)) return TJ_ERR_UNSUPPORTED;
+  if (!rows_ok(k_strides[2], dtype) || !rows_ok(v_strides[2], dtype) || !near_ok({q_strides, o_strides}, 4))
+    return TJ_ERR_UNSUPPORTED;
   TreeArgs a = tree_sizes(B, H, Hk, Sq, Sk, D, Dv);
   a.q = q; a.k = k; a.v = v; a.o = o;
   a.vq = View4{q_strides[0], q_strides[1], q_strides[2]}; a.vk = View4{k_strides[0], k_strides[1], k_strides[2]};

@@ -141,8 +141,9 @@ __global__ __launch_bounds__(kThreads, (HD * (int)sizeof(T) <= 256 ? 2 : 1)) voi
   __shared__ __attribute__((aligned(1024))) unsigned char smem[QS::kBytes];
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave, hl = lane / 32;
   const int kg = w / RB, rb = w % RB, hk = blockIdx.x % a.Hk;
+  __shared__ int told[6];
   Region g;
-  if (!g.take(a, blockIdx.x / a.Hk, a.G, ROWS, false, lane)) return;
+  if (!g.take(a, blockIdx.x / a.Hk, a.G, ROWS, false, tid, told)) return;
   const int L = g.len, R = g.rows * a.G, r0 = g.tile * ROWS, rw0 = r0 + 32 * rb;
   auto span = [&](int row, int last) {
     return row >= R || row / a.by_group >= L ? 0 : (a.causal ? min(L, min(last, R - 1) / a.by_group + 1) : L);
@@ -160,20 +161,18 @@ __global__ __launch_bounds__(kThreads, (HD * (int)sizeof(T) <= 256 ? 2 : 1)) voi
   SweepRow row{r, r / a.by_group, r % a.by_group, 0, r < R && r / a.by_group < L};
   row.limit = a.causal ? row.i : L - 1;
   const int free = a.causal ? rw0 / a.by_group : L - 1;  // the last key that all of the wave's rows see
+  const typename Wave::Places places(rw0, a.by_group, lane);
+  const int64_t token0 = g.start + rw0 / a.by_group;
   frag_t<T> qf[KS], of[KS];
   float sum = 0.f, norm = 0.f;
   {
     typename Wave::vec_t xq[Wave::N], xo[Wave::N], xy[Wave::N], xz[Wave::N];
-    auto rows = [&](const void* p, const View3& v) {
-      return [&, p](int n) -> const T* {
-        const int r = rw0 + n, i = r / a.by_group;
-        return r < R && i < L ? reinterpret_cast<const T*>(p) + v.row(g.start + i, hk * a.G + r - i * a.G) : nullptr;
-      };
-    };
-    Wave::read(xq, a.D, lane, rows(a.q, a.vq));
-    Wave::read(xo, a.Dv, lane, rows(a.dout, a.vdo));
-    Wave::read(xy, a.Dv, lane, rows(a.out, a.vo));
-    if constexpr (sizeof(T) == 2) Wave::read(xz, a.Dv, lane, rows(a.rest, a.vo));
+    const int end = L * a.G;
+    const int64_t at = a.vo.row(token0, hk * a.G);
+    Wave::read(xq, reinterpret_cast<const T*>(a.q) + a.vq.row(token0, hk * a.G), a.vq.st, a.vq.sh, a.D, places, end, lane);
+    Wave::read(xo, reinterpret_cast<const T*>(a.dout) + a.vdo.row(token0, hk * a.G), a.vdo.st, a.vdo.sh, a.Dv, places, end, lane);
+    Wave::read(xy, reinterpret_cast<const T*>(a.out) + at, a.vo.st, a.vo.sh, a.Dv, places, end, lane);
+    if constexpr (sizeof(T) == 2) Wave::read(xz, reinterpret_cast<const T*>(a.rest) + at, a.vo.st, a.vo.sh, a.Dv, places, end, lane);
     const uint32_t turn = QS::kOwn ? lds_offset(smem) + QS::kTiles + rb * Wave::kBytes : tiles + SH::kBytes + rb * Wave::kBytes;
     frag_t<T> y[KS];
     auto dot = [&] {
@@ -280,15 +279,11 @@ __global__ __launch_bounds__(kThreads, (HD * (int)sizeof(T) <= 256 ? 2 : 1)) voi
     st[32] = -del * common;
   }
   const float out = a.scale / lift;
-  Wave::write(lds_offset(smem) + rb * Wave::kBytes, a.D, lane,
-              [&](int d, int c) {
+  Wave::write(reinterpret_cast<T*>(a.dq) + a.vdq.row(token0, hk * a.G), a.vdq.st, a.vdq.sh, a.D, places, R,
+              lds_offset(smem) + rb * Wave::kBytes, lane, [&](int d, int c) {
                 float4_t y = {0.f, 0.f, 0.f, 0.f};
                 if (row.live) y = float4_t{dq[d][4 * c], dq[d][4 * c + 1], dq[d][4 * c + 2], dq[d][4 * c + 3]} * out;
                 return y;
-              },
-              [&](int n) -> T* {
-                const int r = rw0 + n, i = r / a.by_group;
-                return r < R ? reinterpret_cast<T*>(a.dq) + a.vdq.row(g.start + i, hk * a.G + r - i * a.G) : nullptr;
               });
 }
 
@@ -321,8 +316,9 @@ packed_bwd_kv_kernel(PackedArgs a) {
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave, hl = lane / 32,
             ln = lane % 32;
   const int kb = w % KB, rg = w / KB, hk = blockIdx.x % a.Hk;
+  __shared__ int told[6];
   Region g;
-  if (!g.take(a, blockIdx.x / a.Hk, 1, KV::KEYS, true, lane)) return;
+  if (!g.take(a, blockIdx.x / a.Hk, 1, KV::KEYS, true, tid, told)) return;
   const int L = g.len, k0 = g.tile * KV::KEYS, kw0 = k0 + 32 * kb, key = kw0 + ln;
 
   // The group's KB waves bring its tiles.
@@ -363,12 +359,9 @@ packed_bwd_kv_kernel(PackedArgs a) {
     using Wave = WaveRows<T, HD>;
     static_assert(KB * Wave::kBytes <= SH::kBytes, "room for the keys");
     typename Wave::vec_t xk[Wave::N], xv[Wave::N];
-    Wave::read(xk, a.D, lane, [&](int n) -> const T* {
-      return kw0 + n < L ? reinterpret_cast<const T*>(a.k) + a.vk.row(g.start + kw0 + n, hk) : nullptr;
-    });
-    Wave::read(xv, a.Dv, lane, [&](int n) -> const T* {
-      return kw0 + n < L ? reinterpret_cast<const T*>(a.v) + a.vv.row(g.start + kw0 + n, hk) : nullptr;
-    });
+    const typename Wave::Places places(kw0, Divisor{1u << 31, 0, 1}, lane);  // a group of one
+    Wave::read(xk, reinterpret_cast<const T*>(a.k) + a.vk.row(g.start + kw0, hk), a.vk.st, 0, a.D, places, L, lane);
+    Wave::read(xv, reinterpret_cast<const T*>(a.v) + a.vv.row(g.start + kw0, hk), a.vv.st, 0, a.Dv, places, L, lane);
     Wave::turn(xk, group + SH::kBytes + kb * Wave::kBytes, lane, kf);
     Wave::turn(xv, group + SH::kBytes + kb * Wave::kBytes, lane, vf);
   }

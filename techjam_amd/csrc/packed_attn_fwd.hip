@@ -44,8 +44,9 @@ __global__ __launch_bounds__(kThreads, (HD * (int)sizeof(T) <= 256 ? 2 : 1)) voi
   // Consecutive ids run on the XCDs in turn, so the key head varies fastest: the tiles that share
   // K and V also share an XCD's L2.
   const int hk = blockIdx.x % a.Hk;
+  __shared__ int told[6];
   Region g;
-  if (!g.take(a, blockIdx.x / a.Hk, a.G, ROWS, false, lane)) return;
+  if (!g.take(a, blockIdx.x / a.Hk, a.G, ROWS, false, tid, told)) return;
   const int L = g.len, R = g.rows * a.G, r0 = g.tile * ROWS, rw0 = r0 + 32 * rb;
   // Keys needed by rows row .. last (clipped to the region's).
   auto span = [&](int row, int last) {
@@ -58,13 +59,12 @@ __global__ __launch_bounds__(kThreads, (HD * (int)sizeof(T) <= 256 ? 2 : 1)) voi
             a.vk.st, a.vv.st, a.D, a.Dv, rb, lane);
   int kv0 = BN * kg;
   if (!FS::kBefore && kv0 < kv_end) keys.issue(kv0, L, tiles, rb);
+  const typename Wave::Places places(rw0, a.by_group, lane);
+  const int64_t token0 = g.start + rw0 / a.by_group;
   State st;
   {
     typename Wave::vec_t x[Wave::N];
-    Wave::read(x, a.D, lane, [&](int n) -> const T* {
-      const int r = rw0 + n, i = r / a.by_group;
-      return r < R && i < L ? reinterpret_cast<const T*>(a.q) + a.vq.row(g.start + i, hk * a.G + r - i * a.G) : nullptr;
-    });
+    Wave::read(x, reinterpret_cast<const T*>(a.q) + a.vq.row(token0, hk * a.G), a.vq.st, a.vq.sh, a.D, places, L * a.G, lane);
     Wave::turn(x, tiles + (FS::kBefore ? 0 : SH::kBytes) + rb * Wave::kBytes, lane, st.q);
   }
   if constexpr (FS::kBefore) {
@@ -113,21 +113,16 @@ __global__ __launch_bounds__(kThreads, (HD * (int)sizeof(T) <= 256 ? 2 : 1)) voi
   }
   const uint32_t turn = lds_offset(smem) + rb * Wave::kBytes;
   auto value = [&](int d, int c) { return row.live ? st.four(d, c) * inv : float4_t{0.f, 0.f, 0.f, 0.f}; };
-  auto place = [&](void* p) {
-    return [&, p](int n) -> T* {
-      const int r = rw0 + n, i = r / a.by_group;
-      return r < R ? reinterpret_cast<T*>(p) + a.vo.row(g.start + i, hk * a.G + r - i * a.G) : nullptr;
-    };
-  };
-  Wave::write(turn, a.Dv, lane, value, place(a.o));
+  const int64_t at = a.vo.row(token0, hk * a.G);
+  Wave::write(reinterpret_cast<T*>(a.o) + at, a.vo.st, a.vo.sh, a.Dv, places, R, turn, lane, value);
   if constexpr (STATS && sizeof(T) == 2) {
     wait_lds();
-    Wave::write(turn, a.Dv, lane, [&](int d, int c) {
+    Wave::write(reinterpret_cast<T*>(a.rest) + at, a.vo.st, a.vo.sh, a.Dv, places, R, turn, lane, [&](int d, int c) {
       float4_t y = value(d, c);
 #pragma unroll
       for (int j = 0; j < 4; ++j) y[j] -= (float)(T)y[j];
       return y;
-    }, place(a.rest));
+    });
   }
 }
 

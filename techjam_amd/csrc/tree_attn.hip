@@ -110,12 +110,11 @@ __global__ __launch_bounds__((TreeShape<T, HD, BLOCKS>::THREADS), (TreeShape<T, 
     row.live = row.live && !(gone >> t & 1);
   }
   State st;
+  const typename Wave::Places places(rw0, a.by_group, lane);
+  const int token0 = rw0 / a.by_group;
   {
     typename Wave::vec_t x[Wave::N];
-    Wave::read(x, a.D, lane, [&](int n) -> const T* {
-      const int r = rw0 + n, i = r / a.by_group;
-      return r < a.R ? reinterpret_cast<const T*>(a.q) + a.vq.row(b, hk * a.G + r - i * a.G, i) : nullptr;
-    });
+    Wave::read(x, reinterpret_cast<const T*>(a.q) + a.vq.row(b, hk * a.G, token0), a.vq.ss, a.vq.sh, a.D, places, a.R, lane);
     Wave::turn(x, tiles + (TS::kBefore ? 0 : SH::kBytes) + rb * Wave::kBytes, lane, st.q);
   }
   if constexpr (TS::kBefore) {
@@ -180,12 +179,9 @@ __global__ __launch_bounds__((TreeShape<T, HD, BLOCKS>::THREADS), (TreeShape<T, 
   if (kg != 0) return;
   if (whole) {
     const float inv = 1.f / sum;
-    Wave::write(lds_offset(smem) + rb * Wave::kBytes, a.Dv, lane,
-                [&](int d, int c) { return row.live ? st.four(d, c) * inv : float4_t{0.f, 0.f, 0.f, 0.f}; },
-                [&](int n) -> T* {
-                  const int r = rw0 + n, i = r / a.by_group;
-                  return r < a.R ? reinterpret_cast<T*>(a.o) + a.vo.row(b, hk * a.G + r - i * a.G, i) : nullptr;
-                });
+    Wave::write(reinterpret_cast<T*>(a.o) + a.vo.row(b, hk * a.G, token0), a.vo.ss, a.vo.sh, a.Dv, places, a.R,
+                lds_offset(smem) + rb * Wave::kBytes, lane,
+                [&](int d, int c) { return row.live ? st.four(d, c) * inv : float4_t{0.f, 0.f, 0.f, 0.f}; });
     return;
   }
   if (r >= a.R) return;

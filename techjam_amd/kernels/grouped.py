@@ -28,10 +28,11 @@ MAX_DRAFTS = 64
 
 
 def _readable(t: torch.Tensor) -> bool:
-    """Unit innermost stride, rows and base aligned to 16 bytes, 64 tokens within 2 GiB."""
+    """Unit innermost stride, rows and base aligned to 16 bytes, 64 tokens within 2 GiB, heads within 2^31 elements."""
     st, sh, sd = t.stride()
     size = t.element_size()
-    return sd == 1 and not (st | sh) & (16 // size - 1) and not t.data_ptr() & 15 and st * 64 * size < 1 << 31
+    return (sd == 1 and not (st | sh) & (16 // size - 1) and not t.data_ptr() & 15 and st * 64 * size < 1 << 31
+            and sh < 1 << 31)
 
 
 def _tokens_view(t: torch.Tensor) -> torch.Tensor:
