@@ -113,13 +113,14 @@ __device__ __forceinline__ float* stat_at(const PackedArgs& a, const Region& g, 
 }
 
 // A workgroup = RB waves of 32 rows times KG groups, keys through LDS in
-// tiles of 32 dealt to the groups in turn, whose sums meet in LDS at the end. Scores
+// tiles of 32 or 64 dealt to the groups in turn, whose sums meet in LDS at the end. Scores
 // transposed as in the forward kernel: a row's sums are its lane's own numbers, and
 // dS turns into the B operand of dQ^T = K^T dS^T.
 template <typename T, int HD, int BLOCKS>
 struct QShape {
   static constexpr int RB = BLOCKS, KG = 4 / RB, ROWS = 32 * RB;
-  using SH = SweepShape<T, HD, 32>;
+  static constexpr int BN = KG == 1 && HD * (int)sizeof(T) <= 256 ? 64 : 32;  // half the meetings: 1170 -> 1145 us (128 dims), 143 -> 132 (64)
+  using SH = SweepShape<T, HD, BN>;
   using Wave = WaveRows<T, HD>;
   // Two tiles a group, afterwards the groups' sums. The rows come through the second tile while the first keys are on
   // their way, or through a place of their own where it has no room for them.
@@ -132,12 +133,12 @@ template <typename T, int HD>
 constexpr bool groups_fit(int groups) { return groups * SweepShape<T, HD, 32>::W * (int)sizeof(T) <= 1024; }
 
 template <typename T, int HD, int BLOCKS>
-__global__ __launch_bounds__(kThreads, (HD * (int)sizeof(T) <= 256 ? 2 : 1)) void packed_bwd_q_kernel(PackedArgs a) {
+__global__ __launch_bounds__(kThreads, (sizeof(T) == 2 && HD <= 64 ? 3 : (HD * (int)sizeof(T) <= 256 ? 2 : 1))) void packed_bwd_q_kernel(PackedArgs a) {
   using QS = QShape<T, HD, BLOCKS>;
   using SH = typename QS::SH;
   using Wave = typename QS::Wave;
   using Rows = typename SH::Rows;
-  constexpr int KS = SH::KS, DB = SH::DB, BN = 32, RB = QS::RB, KG = QS::KG, ROWS = QS::ROWS, kDepth = SH::kDepth;
+  constexpr int KS = SH::KS, DB = SH::DB, BN = QS::BN, RB = QS::RB, KG = QS::KG, ROWS = QS::ROWS, kDepth = SH::kDepth;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[QS::kBytes];
   const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid / kWave), lane = tid % kWave, hl = lane / 32;
   const int kg = w / RB, rb = w % RB, hk = blockIdx.x % a.Hk;
@@ -213,37 +214,44 @@ __global__ __launch_bounds__(kThreads, (HD * (int)sizeof(T) <= 256 ? 2 : 1)) voi
     wait_copies();
     lds_barrier();
     if (kv0 + KG * BN < kv_end) keys.issue(kv0 + KG * BN, L, tiles + (cur ^ 1) * SH::kBytes, rb);
-    if (kv0 >= own_end) continue;
     const uint32_t tile = tiles + cur * SH::kBytes;
-    float16_t p = zero16(), dp = zero16();
-    read_ahead<KS, kDepth>([&](int s) { return Rows::row_frag(tile + krow, s, 0); },
-                           [&](int s, frag_t<T> f) { p = Elem<T>::mma(f, qf[s], p); });
-    read_ahead<KS, kDepth>([&](int s) { return Rows::row_frag(tile + vrow, s, 0); },
-                           [&](int s, frag_t<T> f) { dp = Elem<T>::mma(f, of[s], dp); });
-    if (own_end <= BN) {
-      // Rows of one tile: delta = sum of P dP, exact to what fp32 sums are. (The output's has the rounding of P in it, which
-      // shows where few keys share a row: sequences of two tokens, dQ 1.4 instead of 1.6 times one rounding from 64 bits.)
-      float exact = 0.f;
 #pragma unroll
-      for (int e = 0; e < 16; ++e)
-        if (kv0 + acc_row(e, hl) <= row.limit) exact = fmaf(fast_exp2(fmaf(p[e], c2, -lse)), dp[e], exact);
-      del = pair_sum(exact);
-      d0 = -del * lift;
+    for (int kb = 0; kb < BN / 32; ++kb) {
+      const int at = kv0 + 32 * kb;
+      if (at < own_end) {
+        const int rows = kb * 32 * Rows::kRowBytes;
+        float16_t p = zero16(), dp = zero16();
+        read_ahead<KS, kDepth>([&](int s) { return Rows::row_frag(tile + krow, s, rows); },
+                               [&](int s, frag_t<T> f) { p = Elem<T>::mma(f, qf[s], p); });
+        read_ahead<KS, kDepth>([&](int s) { return Rows::row_frag(tile + vrow, s, rows); },
+                               [&](int s, frag_t<T> f) { dp = Elem<T>::mma(f, of[s], dp); });
+        if (own_end <= 32) {
+          // Rows of 32 keys: delta = sum of P dP, exact to what fp32 sums are. (The output's has the rounding of P in it, which
+          // shows where few keys share a row: sequences of two tokens, dQ 1.4 instead of 1.6 times one rounding from 64 bits.)
+          float exact = 0.f;
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (at + acc_row(e, hl) <= row.limit) exact = fmaf(fast_exp2(fmaf(p[e], c2, -lse)), dp[e], exact);
+          del = pair_sum(exact);
+          d0 = -del * lift;
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) p[e] = fast_exp2(fmaf(p[e], c2, -lse)) * fmaf(dp[e], lift, d0);
+        // Selected, not multiplied: what a masked key holds does not matter.
+        if (at + 31 > free) {
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if (at + acc_row(e, hl) > row.limit) p[e] = 0.f;
+        }
+        frag_t<T> fs[2];
+#pragma unroll
+        for (int s = 0; s < 2; ++s) fs[s] = acc_frag<T>(p, s);
+        if constexpr (kDepth > 0) __builtin_amdgcn_sched_barrier(0);
+        read_ahead<2 * DB, kDepth>(
+            [&](int j) { return Rows::col_frag(tile + kcol, j % DB, rows + 16 * (j / DB) * Rows::kRowBytes); },
+            [&](int j, frag_t<T> f) { dq[j % DB] = Elem<T>::mma(f, fs[j / DB], dq[j % DB]); });
+      }
     }
-#pragma unroll
-    for (int e = 0; e < 16; ++e) p[e] = fast_exp2(fmaf(p[e], c2, -lse)) * fmaf(dp[e], lift, d0);
-    // Selected, not multiplied: what a masked key holds does not matter.
-    if (kv0 + BN - 1 > free) {
-#pragma unroll
-      for (int e = 0; e < 16; ++e)
-        if (kv0 + acc_row(e, hl) > row.limit) p[e] = 0.f;
-    }
-    frag_t<T> fs[2];
-#pragma unroll
-    for (int s = 0; s < 2; ++s) fs[s] = acc_frag<T>(p, s);
-    if constexpr (kDepth > 0) __builtin_amdgcn_sched_barrier(0);
-    read_ahead<2 * DB, kDepth>([&](int j) { return Rows::col_frag(tile + kcol, j % DB, 16 * (j / DB) * Rows::kRowBytes); },
-                               [&](int j, frag_t<T> f) { dq[j % DB] = Elem<T>::mma(f, fs[j / DB], dq[j % DB]); });
   }
 
   // The groups' sums, the upper half's added to the lower half's.
