@@ -15,7 +15,13 @@
 //
 // The dQ kernel goes over the keys of its rows and leaves each row's lse and delta
 // as the dK, dV kernel wants them; that one goes over the rows of its keys. So
-// nothing is added up across workgroups, and the result does not depend on their order.
+// nothing is added up across workgroups, and the result does not depend on their order; seven
+// products a pair are formed where five would do (the others need dQ by atomics).
+//
+// 1904 and 14480 tokens, 16 heads on 8, 128 dims, bf16, causal: dQ 1140 us, 1150 TFLOP/s of its three
+// products (the forward kernel 810), dK and dV 1590 us, 1100 TFLOP/s of its four; matrix units 59 and 55 %
+// busy, vector units 49 and 37, at 1.74 and 1.82 of 2.4 GHz: power, as in the forward kernel. 96 sequences of about 340
+// tokens, 16 heads on 4, 64 dims: dQ 126 us (of which 79 move rows: 335 MB), dK and dV 145.
 #include "grouped_attn.h"
 
 namespace tj {
@@ -307,7 +313,8 @@ struct KvShape {
   using SH = SweepShape<T, HD, 32>;
   static constexpr int KB = BLOCKS, RG = GROUPS, WAVES = KB * RG, KEYS = 32 * KB;
   static constexpr int kDepth = HD == 32 ? 0 : sizeof(T) == 2 ? 2 : 1;
-  // Waves of a SIMD, by the registers.
+  // Waves of a SIMD, by the registers: with one at 128 dims (310 registers) 2534 us instead of 1600, with two at 64
+  // dims 37 instead of 28.
   static constexpr int kMin = sizeof(T) == 2 ? (HD <= 64 && KB > 1 ? 3 : 2) : (HD == 32 ? 2 : 1);
 };
 
@@ -510,6 +517,8 @@ int packed_bwd(const PackedArgs& a, int dtype, hipStream_t stream) {
     using T = decltype(t);
     constexpr int HD = decltype(hd)::value;
     const int64_t rows = (int64_t)a.T * a.G;  // of one key head
+    // us with 128 / 64 rows a workgroup: 512 tiles of 128 rows, 64 dims 31 / 22; 4260 tiles 137 / 187; 2056 tiles of 128 dims
+    // 1142 / 1248.
     int rc;
     if constexpr (groups_fit<T, HD>(4)) {
       if ((rows + 63) / 64 * a.Hk <= kCus / 2) rc = launch_q<T, HD, 1>(a, stream);
@@ -520,6 +529,8 @@ int packed_bwd(const PackedArgs& a, int dtype, hipStream_t stream) {
       else rc = launch_q<T, HD, 4>(a, stream);
     }
     if (rc != TJ_OK) return rc;
+    // 64 keys, or 32 where those leave half of the CUs idle. us with 128 / 64 / 32 keys a workgroup: short sequences of 64 dims
+    // 298 / 234 / 266, long ones of 128 dims 1589 / 1601 / 2439.
     if ((int64_t)(a.T + 63) / 64 * a.Hk <= kCus / 2) return launch_kv<T, HD, 1, groups_fit<T, HD>(4) ? 4 : 2>(a, stream);
     return launch_kv<T, HD, 2, 2>(a, stream);
   });

@@ -4,6 +4,14 @@
 // A workgroup = RB waves of 32 rows of one (sequence, key head) times KG
 // groups; key tiles of 32 or 64 stream through LDS, dealt to the groups in turn,
 // and the groups' sums meet in LDS at the end.
+//
+// Long sequences are bound by power: 32768 tokens, 8 heads on 2, 128 dims, bf16, causal take
+// 1924 us, 1143 TFLOP/s of 2D + 2Dv operations a pair (a large library product of that type
+// 1218), the matrix unit 63 % and the vector unit 55 % busy at a clock of 1.46 of 2.4 GHz. Short ones are
+// bound by what stands before and after their few key tiles: 96 sequences of about 340
+// tokens, 16 heads on 4, 64 dims take 92 us, of which looking for the tile, q, and the results
+// take 47 without any keys (235 MB, 5 TB/s), the vector unit 63 % busy. A batch of 24 prompts of up to
+// 2935 tokens, 16384 in all, 16 heads on 2, 128 dims: 117 us, of which the longest tile takes 90.
 #include "grouped_attn.h"
 
 namespace tj {
@@ -11,8 +19,9 @@ namespace {
 
 constexpr int kThreads = 256;
 
-// Four waves: 128 rows where those fill the chip, else 64 with two groups or 32 with four, if two
-// tiles for each fit.
+// Four waves: 128 rows where those fill the chip (two workgroups a CU past 64 dims, by the LDS, else
+// four), else 64 with two groups or 32 with four, if two tiles for each fit. us with 128 / 64 rows: 512 tiles of 128 rows, 64
+// dims 24 / 19, 4260 tiles 92 / 121; 423 tiles of 96 dims 24 / 28, 2068 of 128 dims 120 / 163.
 template <typename T, int HD, int BLOCKS>
 struct FwdShape {
   static constexpr int RB = BLOCKS, KG = 4 / RB, ROWS = 32 * RB;
