@@ -15,7 +15,7 @@ from typing import List, Optional
 import torch
 import torch.nn as nn
 
-from ..kernels.grouped import packed_attention, tree_attention
+from ..kernels.grouped import check_parents, packed_attention, tree_attention
 from ..model import Linear, prefix_lengths
 
 
@@ -45,6 +45,9 @@ class GroupedState:
         self.lengths = torch.zeros(batch, dtype=torch.int32, device=device)
         self.longest = 0
         self.drafts = 0
+
+    def check_drafts(self, parents, tokens: int) -> None:
+        check_parents(parents, self.lengths.shape[0], tokens, self.lengths.device)
 
     def reserve(self, tokens: int) -> None:
         if self.longest + tokens > self.capacity:

@@ -187,8 +187,9 @@ def packed_attention(
 
     ``scale`` defaults to ``D ** -0.5``; its magnitude is at most 2^127. Scores are float32 numbers, exact to
     2^-24 of their size; rows with one beyond 2^27 may come out as NaN. A NaN or an infinity
-    among a sequence's tokens spoils what depends on it; one in ``v`` under ``is_causal`` also
-    the up to 31 tokens before it in its tile of 32, as 0 times NaN.
+    among a sequence's tokens spoils what depends on it, and under ``is_causal``, as 0 times NaN,
+    up to 31 neighbours that do not: one in ``v`` the outputs of tokens before it, one in ``k`` their
+    gradients, one in ``q`` or the output gradient the gradients of keys behind it.
 
     Gradients come for q, k and v; their sums have a fixed order, so equal calls give equal
     bits. In float16 the gradient of ``k`` sums its rows at one scale: beside an output gradient 1e6
@@ -223,6 +224,13 @@ def packed_attention(
 
 
 # -- drafted tokens against a cache ---------------------------------------------
+
+def check_parents(parents: torch.Tensor, b: int, t: int, dev: torch.device) -> None:
+    """Refuses what cannot be the parents of ``t`` drafts of each of ``b`` sequences."""
+    if t > MAX_DRAFTS:
+        raise UnsupportedCaseError(f"trees of {t} drafts are not supported (at most {MAX_DRAFTS})")
+    _check_ints("parents", parents, (b, t), dev)
+
 
 @lru_cache(maxsize=256)
 def _tree_floats(dtype: int, b: int, h: int, hk: int, t: int, c: int, d: int, dv: int) -> int:
@@ -275,8 +283,8 @@ def tree_attention(
                          f"v_cache {tuple(v_cache.shape)}")
     _check_types(q, k_cache, v_cache, h, hk)
     scale = _scale(scale, d)
-    if parents is not None and t > MAX_DRAFTS:
-        raise UnsupportedCaseError(f"trees of {t} drafts are not supported (at most {MAX_DRAFTS})")
+    if parents is not None:
+        check_parents(parents, b, t, q.device)
     if lengths is None:
         raise ValueError("lengths must be given: a cache's capacity is not its sequences' length")
     refuse_tangents(q, k_cache, v_cache)
@@ -284,8 +292,6 @@ def tree_attention(
         raise UnsupportedCaseError("tree_attention has no gradients; call it under torch.no_grad()")
     dev = _require_device(q, k_cache, v_cache)
     _check_ints("lengths", lengths, (b,), dev)
-    if parents is not None:
-        _check_ints("parents", parents, (b, t), dev)
     q, k, v = map(_rows_view, _padded(q, k_cache, v_cache))
     dtype = DTYPES[q.dtype]
     d, wide = q.shape[-1], v.shape[-1]

@@ -619,12 +619,16 @@ class TransformerEncoder(nn.Module):
         tokens = x.shape[1]
         if tokens == 0:
             raise ValueError("a step has at least one token")
+        if parents is not None:
+            state.check_drafts(parents, tokens)
         state.reserve(tokens)
         place = state.lengths[:, None].long() + torch.arange(tokens, device=x.device)
         # The state counts the tokens when all layers have them: a refused call
         # leaves it as it was.
         lengths = state.lengths + tokens
         drafts = () if parents is None else (parents,)
+        if hasattr(state, "drafts"):
+            state.drafts = 0  # their places are written over, also by a call that fails on its way
         for layer, cache in zip(self.layers, state.layers):
             x = x + layer.attention.step(layer.norm1(x), cache, lengths, place, *drafts)
             x = layer.ffn(x)
@@ -632,8 +636,8 @@ class TransformerEncoder(nn.Module):
         if parents is None:
             state.lengths.copy_(lengths)
             state.longest += tokens
-        if hasattr(state, "drafts"):
-            state.drafts = 0 if parents is None else tokens
+        else:
+            state.drafts = tokens
         return x
 
     def _check_state(self, x, state) -> None:

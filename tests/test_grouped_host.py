@@ -277,3 +277,29 @@ def test_accepted_drafts_move_behind_what_is_settled():
     state.longest = 99
     state.recount()
     assert state.longest == 7
+
+
+def test_a_refused_tree_leaves_the_drafts_before_it():
+    m = model()
+    state = m.new_state(2, 100)
+    state.lengths.fill_(6)
+    state.longest = 6
+    state.drafts = 2
+    before = [(c.k.normal_().clone(), c.v.normal_().clone()) for c in state.layers]
+    for parents in (torch.full((2, 2), -1), torch.full((2, 3), -1, dtype=torch.int32), torch.full((1, 2), -1, dtype=torch.int32),
+                    [[-1, 0]] * 2, torch.full((2, 2), -1, dtype=torch.int32, device="meta")):
+        with pytest.raises(ValueError, match="parents"):
+            m.step(torch.zeros(2, 2, 32), state, parents)
+    with pytest.raises(UnsupportedCaseError, match="65 drafts"):
+        m.step(torch.zeros(2, 65, 32), state, torch.full((2, 65), -1, dtype=torch.int32))
+    assert state.drafts == 2 and state.longest == 6
+    assert all(torch.equal(c.k, k) and torch.equal(c.v, v) for c, (k, v) in zip(state.layers, before))
+
+
+def test_a_call_that_fails_on_its_way_leaves_no_drafts():
+    m = model()
+    state = m.new_state(2, 100)
+    state.drafts = 2
+    with pytest.raises(UnsupportedCaseError):  # no kernels for CPU tensors
+        m.step(torch.zeros(2, 2, 32), state, torch.full((2, 2), -1, dtype=torch.int32))
+    assert state.drafts == 0
