@@ -121,8 +121,8 @@ struct Region {
   // The at-th tile of all when those that take longest come first, so that no long one is left
   // for the end: a causal sequence of n tiles has one of each length from 1 to n (the
   // last the longest, or with `down` the first), another n of length n. Tiles without tokens
-  // come last. Every wave counts for itself, by halving the range of lengths: half a
-  // microsecond, where a launch that sorts would take several. For up to kRanked regions.
+  // come last. One wave counts, by halving the range of lengths: half a microsecond, where a
+  // launch that sorts would take several. For up to kRanked regions.
   static constexpr int kChunks = 4, kRanked = kChunks * kWave;
   __device__ __forceinline__ bool ranked(const PackedArgs& a, int at, int per, int unit, bool down, int lane) {
     int n[kChunks], from_[kChunks], rows_[kChunks], len_[kChunks], count = 0, top = 0;
@@ -262,10 +262,10 @@ struct SweepShape {
   static constexpr int kTensor = BN * W * (int)sizeof(T), kBytes = 2 * kTensor;  // K's tile, then V's
 };
 
-// A lane's row: r of the tile's (region or sequence, key head): its token, head, and
+// A lane's row of the tile's (region or sequence, key head): its token, head, and
 // the last key it sees.
 struct SweepRow {
-  int r, i, g, limit;
+  int i, g, limit;
   bool live;
 };
 

@@ -165,7 +165,7 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 && HD <= 64 ? 3 : (HD * (
   if (kv0 < kv_end) keys.issue(kv0, L, tiles, rb);
 
   const int r = rw0 + lane % 32;
-  SweepRow row{r, r / a.by_group, r % a.by_group, 0, r < R && r / a.by_group < L};
+  SweepRow row{r / a.by_group, r % a.by_group, 0, r < R && r / a.by_group < L};
   row.limit = a.causal ? row.i : L - 1;
   const int free = a.causal ? rw0 / a.by_group : L - 1;  // the last key that all of the wave's rows see
   const typename Wave::Places places(rw0, a.by_group, lane);

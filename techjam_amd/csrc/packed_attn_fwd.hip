@@ -82,7 +82,7 @@ __global__ __launch_bounds__(kThreads, (HD * (int)sizeof(T) <= 256 ? 2 : 1)) voi
   }
   st.init(a.scale, lane);
   const int r = rw0 + lane % 32;
-  SweepRow row{r, r / a.by_group, r % a.by_group, 0, r < R && r / a.by_group < L};
+  SweepRow row{r / a.by_group, r % a.by_group, 0, r < R && r / a.by_group < L};
   row.limit = a.causal ? row.i : L - 1;
   const int free = a.causal ? rw0 / a.by_group : L - 1;  // the last key that all of the wave's rows see
   // The workgroup goes round together, the last round maybe without a tile for every group.

@@ -103,7 +103,7 @@ __global__ __launch_bounds__((TreeShape<T, HD, BLOCKS>::THREADS), (TreeShape<T, 
   int kv0 = kv_begin + BN * kg;
   if (!TS::kBefore && kv0 < kv_end) keys.issue(kv0, L, tiles, rb);
   const int r = rw0 + lane % 32;
-  SweepRow row{r, r / a.by_group, r % a.by_group, 0, false};
+  SweepRow row{r / a.by_group, r % a.by_group, 0, false};
   row.limit = ctx + row.i;
   row.live = r < a.R && row.limit >= 0;
   uint64_t seen = 0, gone = 0;
