@@ -246,3 +246,32 @@ def test_steps_are_not_captured():
         graph = torch.cuda.CUDAGraph()
         with torch.inference_mode(), torch.cuda.graph(graph), pytest.raises(UnsupportedCaseError, match="captured"):
             model.step(x[:, :1], state, parents)
+
+
+def test_empty_prompts_and_prompts_that_fill_the_cache():
+    model, x, _ = encoder(seq=40)
+    with torch.no_grad():
+        state = model.new_state(3, 40)
+        none = torch.zeros(4, dtype=torch.int32, device="cuda")
+        assert model.prefill_packed(x.new_zeros(0, x.shape[2]).cuda(), none, state).shape == (0, x.shape[2])
+        out = model.prefill_packed(x[0, :5].cuda(), none + 2, state)  # rows of no prompt
+        assert out.shape == (5, x.shape[2]) and not out.any()
+        assert state.lengths.tolist() == [0, 0, 0] and state.longest == 0
+        near(model.step(x[:, :1].cuda(), state)[:, 0], model(x[:, :1].cuda())[:, 0].cpu().double())
+        buffer, offsets = packed_rows(x, torch.tensor([40, 39, 0]))
+        model.prefill_packed(buffer, offsets, state)
+        assert state.lengths.tolist() == [40, 39, 0] and state.longest == 40
+        with pytest.raises(ValueError, match="capacity"):
+            model.step(x[:, :1].cuda(), state)
+
+
+def test_packed_sequences_under_autocast():
+    model, x, lengths = encoder(seq=40)
+    buffer, offsets = packed_rows(x, lengths)
+    want = model.forward_packed(buffer, offsets).detach()
+    with torch.autocast("cuda", torch.bfloat16):
+        out = model.forward_packed(buffer, offsets)
+    out.float().square().mean().backward()
+    assert all(p.grad is not None and torch.isfinite(p.grad).all() for p in model.parameters())
+    # Two layers whose products round inputs and results to bf16, 2^-8 each: about twenty roundings.
+    assert (out.float() - want).abs().max() < 20 * 2 ** -8 * want.abs().max()

@@ -583,3 +583,46 @@ def test_refusals_on_the_gpu():
                 tree_attention(q, k, v, lengths)
     with pytest.raises(UnsupportedCaseError):
         tree_attention(q.requires_grad_(), k, v, ints([5, 5]))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("t,c", [(70, 40), (300, 33), (5, 1), (3, 0), (2100, 2100)])
+def test_chains_longer_than_the_cache(dtype, t, c):
+    """Tokens at negative positions are not there, the others see what the cache holds of them."""
+    q, k, v = draft_inputs(2, 4, 2, t, c, 64, dtype)
+    compare_tree(q, k, v, [c, c // 2])
+
+
+def test_graphs_of_training_and_drafts_replay_in_turn():
+    """Two training steps and a tree of the same tensors, captured one after the other and replayed
+    in turn with eager calls between: no graph's workspace is another's."""
+    from techjam_amd.kernels import packed_attention, tree_attention
+
+    first = [inputs(300, 4, 2, 64, 64, torch.float16, seed=n)[:3] for n in range(2)]
+    offsets = [ints([0, 120, 300]), ints([5, 6, 200])]
+    dout = torch.randn(300, 4, 64, device="cuda", dtype=torch.float16)
+
+    def step(n):
+        leaves = [x.detach().requires_grad_() for x in first[n]]
+        out = packed_attention(*leaves, offsets[n], is_causal=True)
+        return (out.detach(), *torch.autograd.grad(out, leaves, dout))
+
+    q, k, v = draft_inputs(2, 4, 2, 6, 3000, 64, torch.float16)
+    lengths, parents = ints([3000, 1100]), ints([[-1, 0, 0, 1, 1, 4]] * 2)
+
+    def drafts():
+        with torch.no_grad():
+            return (tree_attention(q, k, v, lengths, parents),)
+
+    calls = [lambda: step(0), drafts, lambda: step(1)]
+    graphs = [captured(call) for call in calls]
+    for _ in range(4):
+        dout.normal_()
+        q.normal_()
+        for x in first:
+            for y in x:
+                y.data.normal_()
+        for n in (2, 0, 1, 0):
+            replay(graphs[n][0])
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(graphs[n][1], calls[n]()))
