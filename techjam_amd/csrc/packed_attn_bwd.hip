@@ -227,10 +227,11 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 && HD <= 64 ? 3 : (HD * (
       if (at < own_end) {
         const int rows = kb * 32 * Rows::kRowBytes;
         float16_t p = zero16(), dp = zero16();
-        read_ahead<KS, kDepth>([&](int s) { return Rows::row_frag(tile + krow, s, rows); },
-                               [&](int s, frag_t<T> f) { p = Elem<T>::mma(f, qf[s], p); });
-        read_ahead<KS, kDepth>([&](int s) { return Rows::row_frag(tile + vrow, s, rows); },
-                               [&](int s, frag_t<T> f) { dp = Elem<T>::mma(f, of[s], dp); });
+        read_ahead<2 * KS, kDepth>([&](int s) { return Rows::row_frag(tile + (s < KS ? krow : vrow), s % KS, rows); },
+                                   [&](int s, frag_t<T> f) {
+                                     if (s < KS) p = Elem<T>::mma(f, qf[s % KS], p);
+                                     else dp = Elem<T>::mma(f, of[s % KS], dp);
+                                   });
         if (own_end <= 32) {
           // Rows of 32 keys: delta = sum of P dP, exact to what fp32 sums are. (The output's has the rounding of P in it, which
           // shows where few keys share a row: sequences of two tokens, dQ 1.4 instead of 1.6 times one rounding from 64 bits.)
@@ -312,7 +313,8 @@ template <typename T, int HD, int BLOCKS, int GROUPS>
 struct KvShape {
   using SH = SweepShape<T, HD, 32>;
   static constexpr int KB = BLOCKS, RG = GROUPS, WAVES = KB * RG, KEYS = 32 * KB;
-  static constexpr int kDepth = HD == 32 ? 0 : sizeof(T) == 2 ? 2 : 1;
+  // 64 dims: 142 us with two, 139 with three; 128 dims: 1629 and 1669.
+  static constexpr int kDepth = HD == 32 ? 0 : sizeof(T) == 2 ? (HD == 64 ? 3 : 2) : 1;
   // Waves of a SIMD, by the registers: with one at 128 dims (310 registers) 2534 us instead of 1600, with two at 64
   // dims 37 instead of 28.
   static constexpr int kMin = sizeof(T) == 2 ? (HD <= 64 && KB > 1 ? 3 : 2) : (HD == 32 ? 2 : 1);
@@ -401,10 +403,11 @@ packed_bwd_kv_kernel(PackedArgs a) {
     }
     if (!busy) continue;
     float16_t p = zero16(), dp = zero16();
-    read_ahead<KS, kDepth>([&](int s) { return Rows::row_frag(tile + qrow, s, 0); },
-                           [&](int s, frag_t<T> f) { p = Elem<T>::mma(f, kf[s], p); });
-    read_ahead<KS, kDepth>([&](int s) { return Rows::row_frag(tile + orow, s, 0); },
-                           [&](int s, frag_t<T> f) { dp = Elem<T>::mma(f, vf[s], dp); });
+    read_ahead<2 * KS, kDepth>([&](int s) { return Rows::row_frag(tile + (s < KS ? qrow : orow), s % KS, 0); },
+                               [&](int s, frag_t<T> f) {
+                                 if (s < KS) p = Elem<T>::mma(f, kf[s % KS], p);
+                                 else dp = Elem<T>::mma(f, vf[s % KS], dp);
+                               });
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const float4_t ls = lds_at<float4_t>(srow + q * 32), d0 = lds_at<float4_t>(srow + 128 + q * 32);
@@ -430,10 +433,12 @@ packed_bwd_kv_kernel(PackedArgs a) {
       fs[s] = acc_frag<T>(dp, s);
     }
     if constexpr (kDepth > 0) __builtin_amdgcn_sched_barrier(0);
-    read_ahead<2 * DB, kDepth>([&](int j) { return Rows::col_frag(tile + ocol, j % DB, 16 * (j / DB) * Rows::kRowBytes); },
-                               [&](int j, frag_t<T> f) { dv[j % DB] = Elem<T>::mma(fp[j / DB], f, dv[j % DB]); });
-    read_ahead<2 * DB, kDepth>([&](int j) { return Rows::col_frag(tile + qcol, j % DB, 16 * (j / DB) * Rows::kRowBytes); },
-                               [&](int j, frag_t<T> f) { dk[j % DB] = Elem<T>::mma(fs[j / DB], f, dk[j % DB]); });
+    read_ahead<4 * DB, kDepth>(
+        [&](int j) { return Rows::col_frag(tile + (j < 2 * DB ? ocol : qcol), j % DB, 16 * (j / DB % 2) * Rows::kRowBytes); },
+        [&](int j, frag_t<T> f) {
+          if (j < 2 * DB) dv[j % DB] = Elem<T>::mma(fp[j / DB % 2], f, dv[j % DB]);
+          else dk[j % DB] = Elem<T>::mma(fs[j / DB % 2], f, dk[j % DB]);
+        });
   }
 
   // The groups' sums, the upper half's added to the lower half's.
