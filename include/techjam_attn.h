@@ -477,7 +477,8 @@ int tj_packed_attn_fwd(const void* q, const void* k, const void* v, void* o, int
  * The gradients of tj_packed_attn_fwd for the output gradient dout [T, H, Dv]: dq, dk, dv
  * (shaped and typed like q, k, v). o, o_rest and lse come from the forward call. Rows without a token
  * get zeros and their dout is not read. The sums' order is fixed: the same call gives the
- * same bits. workspace: tj_packed_attn_bwd_workspace_bytes bytes, 16-byte aligned, contents
+ * same bits. workspace: tj_packed_attn_bwd_workspace_bytes bytes (up to 64 MiB more than the rows'
+ * numbers where few key heads' gradients are summed in parts), 16-byte aligned, contents
  * irrelevant, calls sharing one ordered on one stream.
  */
 size_t tj_packed_attn_bwd_workspace_bytes(int64_t T, int64_t N, int64_t H, int64_t Hk);

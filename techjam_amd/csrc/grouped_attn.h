@@ -54,6 +54,8 @@ struct PackedArgs {
   void *dq, *dk, *dv;
   float* stat;             // [slots of 32 tokens, H, 2, 32] what the dK, dV kernel reads of a row
   float* peak;             // [slots of 64 tokens, Hk, 2] largest norms of dO and V rows (fp16 operands)
+  int shares;              // workgroups that share the rows of a key tile
+  float* part;             // [shares, T, Hk, Dv + D] their sums for dV and dK; used where there are several
 };
 
 // The rows fall into regions: what lies before the first sequence, the sequences,
@@ -530,6 +532,7 @@ TreePlan tree_plan(const TreeArgs& a, int dtype);
 int tree_fwd(const TreeArgs& a, const TreePlan& p, int dtype, hipStream_t stream);
 
 int packed_fwd(const PackedArgs& a, int dtype, hipStream_t stream);
+int packed_bwd_shares(int64_t T, int64_t N, int64_t H, int64_t Hk);
 int packed_bwd(const PackedArgs& a, int dtype, hipStream_t stream);
 
 }  // namespace tj

@@ -62,6 +62,12 @@ PackedArgs packed_args(const void* q, const void* k, const void* v, int64_t T, i
 // The numbers of 32 tokens, then the peaks of 64.
 size_t stat_floats(int64_t T, int64_t N, int64_t H) { return size_t(region_slots(T, N, 1, 32)) * size_t(H) * 64; }
 size_t peak_floats(int64_t T, int64_t N, int64_t Hk) { return size_t(region_slots(T, N, 1, 64)) * size_t(Hk) * 2; }
+// Behind them, from a whole 16 bytes on, the sums of shared key tiles, of the largest dims.
+size_t part_first(int64_t T, int64_t N, int64_t H, int64_t Hk) { return (stat_floats(T, N, H) + peak_floats(T, N, Hk) + 3) / 4 * 4; }
+size_t part_floats(int64_t T, int64_t N, int64_t H, int64_t Hk) {
+  const int shares = packed_bwd_shares(T, N, H, Hk);
+  return shares == 1 ? 0 : size_t(shares) * size_t(T) * size_t(Hk) * 256;
+}
 
 // A cache's capacity is no part of a grid, but its blocks of 32 keys are counted.
 bool tree_sizes_ok(int64_t B, int64_t H, int64_t Hk, int64_t Sq, int64_t Sk) {
@@ -118,7 +124,7 @@ extern "C" int tj_packed_attn_fwd(const void* q, const void* k, const void* v, v
 
 extern "C" size_t tj_packed_attn_bwd_workspace_bytes(int64_t T, int64_t N, int64_t H, int64_t Hk) {
   if (!packed_sizes_ok(T, N, H, Hk)) return 0;
-  return (stat_floats(T, N, H) + peak_floats(T, N, Hk)) * sizeof(float);
+  return (part_first(T, N, H, Hk) + part_floats(T, N, H, Hk)) * sizeof(float);
 }
 
 extern "C" int tj_packed_attn_bwd(const void* q, const void* k, const void* v, const void* o,
@@ -155,6 +161,8 @@ extern "C" int tj_packed_attn_bwd(const void* q, const void* k, const void* v, c
   a.vdk = View3{dk_strides[0], dk_strides[1]}; a.vdv = View3{dv_strides[0], dv_strides[1]};
   a.stat = static_cast<float*>(workspace);
   a.peak = a.stat + stat_floats(T, N, H);
+  a.shares = packed_bwd_shares(T, N, H, Hk);
+  a.part = a.stat + part_first(T, N, H, Hk);
   return packed_bwd(a, dtype, stream);
 }
 

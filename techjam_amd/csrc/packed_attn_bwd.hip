@@ -15,13 +15,16 @@
 //
 // The dQ kernel goes over the keys of its rows and leaves each row's lse and delta
 // as the dK, dV kernel wants them; that one goes over the rows of its keys. So
-// nothing is added up across workgroups, and the result does not depend on their order; seven
+// no atomics are needed, and the result does not depend on the workgroups' order (where several
+// share the rows of few keys, their sums are joined in a fixed one); seven
 // products a pair are formed where five would do (the others need dQ by atomics).
 //
 // 1904 and 14480 tokens, 16 heads on 8, 128 dims, bf16, causal: dQ 1140 us, 1150 TFLOP/s of its three
 // products (the forward kernel 810), dK and dV 1590 us, 1100 TFLOP/s of its four; matrix units 59 and 55 %
 // busy, vector units 49 and 37, at 1.74 and 1.82 of 2.4 GHz: power, as in the forward kernel. 96 sequences of about 340
 // tokens, 16 heads on 4, 64 dims: dQ 126 us (of which 79 move rows: 335 MB), dK and dV 145.
+#include <algorithm>
+
 #include "grouped_attn.h"
 
 namespace tj {
@@ -335,7 +338,8 @@ packed_bwd_kv_kernel(PackedArgs a) {
   const int kb = w % KB, rg = w / KB, hk = blockIdx.x % a.Hk;
   __shared__ int told[6];
   Region g;
-  if (!g.take(a, blockIdx.x / a.Hk, 1, KV::KEYS, true, tid, told)) return;
+  const int share = blockIdx.x / a.Hk % a.shares;
+  if (!g.take(a, blockIdx.x / a.Hk / a.shares, 1, KV::KEYS, true, tid, told)) return;
   const int L = g.len, k0 = g.tile * KV::KEYS, kw0 = k0 + 32 * kb, key = kw0 + ln;
 
   // The group's KB waves bring its tiles.
@@ -345,7 +349,8 @@ packed_bwd_kv_kernel(PackedArgs a) {
   const T* op = reinterpret_cast<const T*>(a.dout) + a.vdo.row(g.start, hk * a.G);
   const uint32_t group = lds_offset(smem) + rg * 2 * SH::kBytes, stat0 = lds_offset(stat[rg]);
   const uint32_t qrow = Rows::lane_row(lane), qcol = Rows::lane_col(lane), orow = qrow + SH::kTensor, ocol = qcol + SH::kTensor;
-  // Tile n: head n / tiles of the group, tokens i_begin + 32 (n % tiles) on.
+  // Tile n: head n / tiles of the group, tokens i_begin + 32 (n % tiles) on. They are dealt to the groups of all
+  // workgroups that share the keys.
   const int i_begin = a.causal ? k0 : 0;
   const int tiles = k0 < L ? (L - i_begin + BM - 1) / BM : 0, n_end = tiles * a.G;
   // `n` tiles further on: the head and the token (no division in the loop).
@@ -366,8 +371,9 @@ packed_bwd_kv_kernel(PackedArgs a) {
   };
 
   int h = 0, i0 = i_begin;  // this round's tile
-  if (rg < n_end) {
-    advance(h, i0, rg);
+  const int n0 = share * RG + rg, step = a.shares * RG;
+  if (n0 < n_end) {
+    advance(h, i0, n0);
     issue(h, i0, 0);
   }
   frag_t<T> kf[KS], vf[KS];
@@ -388,8 +394,8 @@ packed_bwd_kv_kernel(PackedArgs a) {
 
   const float dl = DsLift<T>(a, g, hk, lane).all(), lift = dl / DsLift<T>::kP, c2 = a.scale * kLog2e;
   // The workgroup goes round together, the last round maybe without a tile for every group.
-  const int rounds = (n_end + RG - 1) / RG;
-  for (int round = 0, n = rg, cur = 0; round < rounds; ++round, n += RG, cur ^= 1) {
+  const int rounds = (n_end - share * RG + step - 1) / step;
+  for (int round = 0, n = n0, cur = 0; round < rounds; ++round, n += step, cur ^= 1) {
     // The tile is there, and the group's other one has been read by its waves.
     wait_copies();
     lds_barrier();
@@ -397,8 +403,8 @@ packed_bwd_kv_kernel(PackedArgs a) {
     // Else there is no tile, or every token stands before the wave's keys.
     const bool busy = n < n_end && (!a.causal || i0 + BM > kw0);
     const int at = i0;
-    if (n + RG < n_end) {
-      advance(h, i0, RG);
+    if (n + step < n_end) {
+      advance(h, i0, step);
       issue(h, i0, cur ^ 1);
     }
     if (!busy) continue;
@@ -480,6 +486,15 @@ packed_bwd_kv_kernel(PackedArgs a) {
     const int j = kw0 + acc_row(r, hl);
     if (j >= g.rows) continue;
     const bool in = j < L;
+    if (a.shares > 1) {
+      float* x = a.part + (((int64_t)share * a.T + g.start + j) * a.Hk + hk) * (a.Dv + a.D);
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        if (32 * d + ln < a.Dv) x[32 * d + ln] = in ? dv[d][r] * dv_scale : 0.f;
+        if (32 * d + ln < a.D) x[a.Dv + 32 * d + ln] = in ? dk[d][r] * dk_scale : 0.f;
+      }
+      continue;
+    }
     T* pv = reinterpret_cast<T*>(a.dv) + a.vdv.row(g.start + j, hk);
     T* pk = reinterpret_cast<T*>(a.dk) + a.vdk.row(g.start + j, hk);
 #pragma unroll
@@ -488,6 +503,22 @@ packed_bwd_kv_kernel(PackedArgs a) {
       if (32 * d + ln < a.D) pk[32 * d + ln] = (T)(in ? dk[d][r] * dk_scale : 0.f);
     }
   }
+}
+
+// dV and dK of the workgroups that shared the rows of a key tile, summed in their order; four columns a thread.
+template <typename T>
+__global__ __launch_bounds__(kThreads) void packed_bwd_join_kernel(PackedArgs a) {
+  const int width = a.Dv + a.D, chunks = width / 4;
+  const int64_t at = (int64_t)blockIdx.x * kThreads + threadIdx.x, row = at / chunks;
+  if (row >= (int64_t)a.T * a.Hk) return;
+  const int col = (int)(at - row * chunks) * 4, hk = (int)(row % a.Hk);
+  const int64_t t = row / a.Hk, step = (int64_t)a.T * a.Hk * width;
+  const float* x = a.part + row * width + col;
+  float4_t y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+  for (int s = 0; s < a.shares; ++s) y += *reinterpret_cast<const float4_t*>(x + s * step);
+  T* p = col < a.Dv ? reinterpret_cast<T*>(a.dv) + a.vdv.row(t, hk) + col : reinterpret_cast<T*>(a.dk) + a.vdk.row(t, hk) + col - a.Dv;
+  store4t<T>(p, y[0], y[1], y[2], y[3]);
 }
 
 template <typename T, int HD, int BLOCKS>
@@ -503,12 +534,29 @@ int launch_kv(PackedArgs a, hipStream_t stream) {
   using KV = KvShape<T, HD, BLOCKS, GROUPS>;
   const int64_t slots = region_slots(a.T, a.N, 1, KV::KEYS);
   a.n_slots = (int)slots;
-  hipLaunchKernelGGL((packed_bwd_kv_kernel<T, HD, BLOCKS, GROUPS>), dim3(uint32_t(slots * a.Hk)), dim3(64 * KV::WAVES), 0,
+  hipLaunchKernelGGL((packed_bwd_kv_kernel<T, HD, BLOCKS, GROUPS>), dim3(uint32_t(slots * a.Hk * a.shares)), dim3(64 * KV::WAVES), 0,
                      stream, a);
+  const int rc = tjh::launch_status();
+  if (rc != TJ_OK || a.shares == 1) return rc;
+  const int64_t chunks = (int64_t)a.T * a.Hk * ((a.Dv + a.D) / 4);
+  hipLaunchKernelGGL((packed_bwd_join_kernel<T>), dim3(uint32_t((chunks + kThreads - 1) / kThreads)), dim3(kThreads), 0, stream, a);
   return tjh::launch_status();
 }
 
 }  // namespace
+
+// Key tiles are few where few key heads serve many query heads, and each then has many rounds, 0.85 us apiece at 64
+// dims whatever else runs: with 256 workgroups of them the dK, dV kernel took 437 us beside 115 of dQ (4096 tokens, 32
+// heads on 4). So several workgroups share a tile's rows, up to 1024 in all and 16 rounds each or more of a sequence of
+// ordinary length; their sums go through memory. us with one / two / four / eight, joining included, bf16: 4096 tokens, 32
+// heads on 4, 64 dims (256 tiles) 440 / 262 / 169 / 181; 4 x 2048, 16 on 2, 128 dims (256) 319 / 202 / 177 / 202; 4096,
+// 32 on 8, 128 dims (512) 356 / 313 / 332 / 411; 8192, 32 on 8, 128 dims (1024) 1091 / 1065 / 1120 / 1267; 2048, 16 on 2, 64
+// dims (64) with four / twelve / sixteen 70 / 40 / 42 instead of 120.
+int packed_bwd_shares(int64_t T, int64_t N, int64_t H, int64_t Hk) {
+  const int64_t tiles = std::max<int64_t>(1, (T + 63) / 64 * Hk);
+  const int64_t rounds = (T / std::max<int64_t>(N, 1) + 31) / 32 * (H / Hk) / 2;
+  return (int)std::max<int64_t>(1, std::min<int64_t>({16, 1024 / tiles, rounds / 16}));
+}
 
 int packed_bwd(const PackedArgs& a, int dtype, hipStream_t stream) {
   if (dtype == TJ_F16) {
@@ -536,7 +584,7 @@ int packed_bwd(const PackedArgs& a, int dtype, hipStream_t stream) {
     if (rc != TJ_OK) return rc;
     // 64 keys, or 32 where those leave half of the CUs idle. us with 128 / 64 / 32 keys a workgroup: short sequences of 64 dims
     // 298 / 234 / 266, long ones of 128 dims 1589 / 1601 / 2439.
-    if ((int64_t)(a.T + 63) / 64 * a.Hk <= kCus / 2) return launch_kv<T, HD, 1, groups_fit<T, HD>(4) ? 4 : 2>(a, stream);
+    if (a.shares == 1 && (int64_t)(a.T + 63) / 64 * a.Hk <= kCus / 2) return launch_kv<T, HD, 1, groups_fit<T, HD>(4) ? 4 : 2>(a, stream);
     return launch_kv<T, HD, 2, 2>(a, stream);
   });
 }

@@ -626,3 +626,55 @@ def test_graphs_of_training_and_drafts_replay_in_turn():
             replay(graphs[n][0])
             torch.cuda.synchronize()
             assert all(torch.equal(a, b) for a, b in zip(graphs[n][1], calls[n]()))
+
+
+# -- key tiles whose rows several workgroups share ---------------------------------
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lengths,h,hk,d,dv,shares", [
+    ([700, 0, 1321, 33], 8, 1, 64, 64, 4),
+    ([1100], 32, 1, 32, 16, 16),
+    ([900, 1, 1030], 12, 2, 128, 40, 3),
+    ([1500], 10, 2, 80, 96, 7),
+])
+def test_shared_key_tiles(dtype, causal, lengths, h, hk, d, dv, shares):
+    from techjam_amd.kernels.grouped import _backward_floats
+
+    t = 5 + sum(lengths) + 70
+    assert 0 <= _backward_floats(t, len(lengths), h, hk) - shares * t * hk * 256 < 2 * t * hk * 256
+    q, k, v, dout = inputs(t, h, hk, d, dv, dtype, seed=h)
+    offsets = offsets_of(lengths, 5)
+    got = compare_packed(q, k, v, offsets, causal, dout)
+    assert not got["dk"][:5].any() and not got["dv"][-70:].any()
+    assert same(got, run_packed(q, k, v, offsets, causal, dout))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_shared_key_tiles_of_a_padded_batch(dtype):
+    q, k, v, dout = inputs(2400, 16, 2, 64, 64, dtype, seed=3)
+    compare_packed(q, k, v, [0, 1200, 2400], True, dout, valid_len=[1200, 417])
+
+
+def test_shared_key_tiles_in_a_graph():
+    from techjam_amd.kernels import packed_attention
+
+    q, k, v, dout = inputs(1300, 8, 1, 64, 64, torch.bfloat16, seed=5)
+    leaves, offsets = [x.detach().clone().requires_grad_() for x in (q, k, v)], ints([0, 600, 1300])
+
+    def call():
+        out = packed_attention(*leaves, offsets, is_causal=True)
+        return [out, *torch.autograd.grad(out, leaves, dout)]
+
+    graph, held = captured(call)
+    for n in range(4):
+        with torch.no_grad():
+            for x in (*leaves, dout):
+                x.normal_()
+            offsets.copy_(ints([n, 600 + 50 * n, 1300 - n]))
+        torch.cuda.synchronize()
+        replay(graph)
+        torch.cuda.synchronize()
+        got = [x.detach().clone() for x in held]
+        want = run_packed(*leaves, offsets.tolist(), True, dout)
+        assert same(dict(enumerate(got)), dict(enumerate(want.values())))
