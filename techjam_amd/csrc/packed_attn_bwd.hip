@@ -571,14 +571,15 @@ int packed_bwd(const PackedArgs& a, int dtype, hipStream_t stream) {
     constexpr int HD = decltype(hd)::value;
     const int64_t rows = (int64_t)a.T * a.G;  // of one key head
     // us with 128 / 64 rows a workgroup: 512 tiles of 128 rows, 64 dims 31 / 22; 4260 tiles 137 / 187; 2056 tiles of 128 dims
-    // 1142 / 1248.
+    // 1142 / 1248; 768 tiles of 64 dims of a causal sequence of 16384 382 / 347, 1024 of 512 tokens 37 / 41.
+    const int64_t most = (HD <= 64 && sizeof(T) == 2 && long_triangles(a) ? 3 : 2) * kCus;
     int rc;
     if constexpr (groups_fit<T, HD>(4)) {
       if ((rows + 63) / 64 * a.Hk <= kCus / 2) rc = launch_q<T, HD, 1>(a, stream);
-      else if ((rows + 127) / 128 * a.Hk <= 2 * kCus) rc = launch_q<T, HD, 2>(a, stream);
+      else if ((rows + 127) / 128 * a.Hk <= most) rc = launch_q<T, HD, 2>(a, stream);
       else rc = launch_q<T, HD, 4>(a, stream);
     } else {
-      if ((rows + 127) / 128 * a.Hk <= 2 * kCus) rc = launch_q<T, HD, 2>(a, stream);
+      if ((rows + 127) / 128 * a.Hk <= most) rc = launch_q<T, HD, 2>(a, stream);
       else rc = launch_q<T, HD, 4>(a, stream);
     }
     if (rc != TJ_OK) return rc;

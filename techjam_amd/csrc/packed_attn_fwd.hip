@@ -21,7 +21,9 @@ constexpr int kThreads = 256;
 
 // Four waves: 128 rows where those fill the chip (two workgroups a CU past 64 dims, by the LDS, else
 // four), else 64 with two groups or 32 with four, if two tiles for each fit. us with 128 / 64 rows: 512 tiles of 128 rows, 64
-// dims 24 / 19, 4260 tiles 92 / 121; 423 tiles of 96 dims 24 / 28, 2068 of 128 dims 120 / 163.
+// dims 24 / 19, 4260 tiles 92 / 121; 423 tiles of 96 dims 24 / 28, 2068 of 128 dims 120 / 163. Long causal sequences want them
+// up to twice as far, as tiles that all run at once end when the longest does: 512 tiles of 128 dims of 16384 tokens
+// 463 / 356, of 4096 112 / 97, but of 1024 37 / 40 and of 256 20 / 27; 768 of 64 dims of 16384 316 / 288.
 template <typename T, int HD, int BLOCKS>
 struct FwdShape {
   static constexpr int RB = BLOCKS, KG = 4 / RB, ROWS = 32 * RB;
@@ -156,7 +158,7 @@ int packed_fwd(const PackedArgs& a, int dtype, hipStream_t stream) {
     if constexpr (groups_fit<T, HD>(4))
       if ((rows + 63) / 64 * a.Hk <= kCus / 2) return launch<T, HD, 1>(a, stream);
     if constexpr (groups_fit<T, HD>(2))
-      if ((rows + 127) / 128 * a.Hk <= (HD <= 64 ? 2 : 1) * kCus) return launch<T, HD, 2>(a, stream);
+      if ((rows + 127) / 128 * a.Hk <= (HD <= 64 ? 2 : 1) * (long_triangles(a) ? 2 : 1) * kCus) return launch<T, HD, 2>(a, stream);
     return launch<T, HD, 4>(a, stream);
   });
 }
