@@ -535,7 +535,7 @@ int tree_fwd(const TreeArgs& a, const TreePlan& p, int dtype, hipStream_t stream
 inline bool long_triangles(const PackedArgs& a) { return a.causal && a.T / (a.N > 0 ? a.N : 1) >= 2048; }
 
 int packed_fwd(const PackedArgs& a, int dtype, hipStream_t stream);
-int packed_bwd_shares(int64_t T, int64_t N, int64_t H, int64_t Hk);
+int packed_bwd_shares(int dtype, int64_t T, int64_t N, int64_t H, int64_t Hk);
 int packed_bwd(const PackedArgs& a, int dtype, hipStream_t stream);
 
 }  // namespace tj

@@ -1,6 +1,8 @@
 // Attention with grouped heads, packed sequences and drafted tokens: the C ABI entry
 // points and their argument checks. The kernels are in packed_attn_fwd.hip,
 // packed_attn_bwd.hip and tree_attn.hip.
+#include <algorithm>
+
 #include "grouped_attn.h"
 
 namespace tj {
@@ -62,10 +64,10 @@ PackedArgs packed_args(const void* q, const void* k, const void* v, int64_t T, i
 // The numbers of 32 tokens, then the peaks of 64.
 size_t stat_floats(int64_t T, int64_t N, int64_t H) { return size_t(region_slots(T, N, 1, 32)) * size_t(H) * 64; }
 size_t peak_floats(int64_t T, int64_t N, int64_t Hk) { return size_t(region_slots(T, N, 1, 64)) * size_t(Hk) * 2; }
-// Behind them, from a whole 16 bytes on, the sums of shared key tiles, of the largest dims.
+// Behind them, from a whole 16 bytes on, the sums of shared key tiles, of the type with most of them and the largest dims.
 size_t part_first(int64_t T, int64_t N, int64_t H, int64_t Hk) { return (stat_floats(T, N, H) + peak_floats(T, N, Hk) + 3) / 4 * 4; }
 size_t part_floats(int64_t T, int64_t N, int64_t H, int64_t Hk) {
-  const int shares = packed_bwd_shares(T, N, H, Hk);
+  const int shares = std::max(packed_bwd_shares(TJ_F32, T, N, H, Hk), packed_bwd_shares(TJ_BF16, T, N, H, Hk));
   return shares == 1 ? 0 : size_t(shares) * size_t(T) * size_t(Hk) * 256;
 }
 
@@ -161,7 +163,7 @@ extern "C" int tj_packed_attn_bwd(const void* q, const void* k, const void* v, c
   a.vdk = View3{dk_strides[0], dk_strides[1]}; a.vdv = View3{dv_strides[0], dv_strides[1]};
   a.stat = static_cast<float*>(workspace);
   a.peak = a.stat + stat_floats(T, N, H);
-  a.shares = packed_bwd_shares(T, N, H, Hk);
+  a.shares = packed_bwd_shares(dtype, T, N, H, Hk);
   a.part = a.stat + part_first(T, N, H, Hk);
   return packed_bwd(a, dtype, stream);
 }

@@ -552,11 +552,17 @@ int launch_kv(PackedArgs a, hipStream_t stream) {
 // ordinary length; their sums go through memory. us with one / two / four / eight, joining included, bf16: 4096 tokens, 32
 // heads on 4, 64 dims (256 tiles) 440 / 262 / 169 / 181; 4 x 2048, 16 on 2, 128 dims (256) 319 / 202 / 177 / 202; 4096,
 // 32 on 8, 128 dims (512) 356 / 313 / 332 / 411; 8192, 32 on 8, 128 dims (1024) 1091 / 1065 / 1120 / 1267; 2048, 16 on 2, 64
-// dims (64) with four / twelve / sixteen 70 / 40 / 42 instead of 120.
-int packed_bwd_shares(int64_t T, int64_t N, int64_t H, int64_t Hk) {
+// dims (64) with four / twelve / sixteen 70 / 40 / 42 instead of 120. Rounds of fp32 take about six times as long and half as many
+// workgroups fill the chip: 512 and four rounds. us with one / two / four / eight: 2000 tokens, 2 on 2, 96 dims (64
+// tiles) 212 / 120 / 71 / 66; 2 x 700, 8 on 8, 64 dims (176) 62 / 53 / 75 / 116; 2 x 2000, 16 on 4, 128 dims (252)
+// 1056 / 621 / 651 / 729; 1024, 4 on 4, 64 dims (64) 51 / 54 / 38 / 47.
+int packed_bwd_shares(int dtype, int64_t T, int64_t N, int64_t H, int64_t Hk) {
   const int64_t tiles = std::max<int64_t>(1, (T + 63) / 64 * Hk);
   const int64_t rounds = (T / std::max<int64_t>(N, 1) + 31) / 32 * (H / Hk) / 2;
-  return (int)std::max<int64_t>(1, std::min<int64_t>({16, 1024 / tiles, rounds / 16}));
+  const bool wide = dtype == TJ_F32;
+  const int64_t shares = std::max<int64_t>(1, std::min<int64_t>({16, (wide ? 512 : 1024) / tiles, rounds / (wide ? 4 : 16)}));
+  // Four groups of a workgroup with 32 keys do what two workgroups would: 120 us and 116 + 4.
+  return shares == 2 && !wide && tiles <= kCus / 2 ? 1 : (int)shares;
 }
 
 int packed_bwd(const PackedArgs& a, int dtype, hipStream_t stream) {
