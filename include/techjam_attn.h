@@ -464,7 +464,7 @@ int tj_diff_attn_bwd(const void* q, const void* k, const void* v, const float* m
  *
  * lse and, with 16-bit types, o_rest: what tj_packed_attn_bwd reads again, or NULL:
  * fp32 [T, H], log2 of the rows' softmax sums (rows without a token are not written), and what
- * rounding took from o, in o's type, shape and strides (NULL for fp32).
+ * rounding took from o (in fp16 times 2^11), in o's type, shape and strides (NULL for fp32).
  */
 int tj_packed_attn_fwd(const void* q, const void* k, const void* v, void* o, int dtype,
                        int64_t T, int64_t N, int64_t H, int64_t Hk, int64_t D, int64_t Dv,

@@ -46,7 +46,7 @@ struct PackedArgs {
   const int32_t* off;      // [N + 1]
   const int32_t* len;      // [N] valid tokens of each sequence's rows, or null: all
   float* lse;              // [T, H] log2 of a row's sum of 2^(score log2 e); or null
-  void* rest;              // what rounding took from o, in o's type and layout (16-bit types); or null
+  void* rest;              // kRestLift times what rounding took from o, in o's type and layout (16-bit types); or null
   int n_slots;             // of the launch, see Region
   // Backward.
   const void *out, *dout;
@@ -249,6 +249,12 @@ struct TreeArgs {
   float *part_o, *part_ml;
   int32_t* plan;           // [B, 2] a sequence's first part, the keys of each
 };
+
+// What rounding took from the output (PackedArgs::rest) is kept times this. fp16: 2^11, as the rest is 2^-11 of the output
+// and would lose its bits below 2^-24 where the output is small; with it the two are off by 2^-22 of the output, and by
+// 2^-36 at the most below 2^-14. The largest, 16 of 65504, becomes 2^15. bf16 has fp32's exponents.
+template <typename T>
+constexpr float kRestLift = std::is_same<T, half_t>::value ? 2048.f : 1.f;
 
 constexpr float kLazy = 8.f;  // the running maximum moves when a row's maximum grows by more than 2^8
 

@@ -7,7 +7,8 @@
 //
 // the last two summed over the group's rows. delta comes from the output as it was
 // returned plus what its rounding took away, which the forward pass keeps (in bf16
-// and fp16; together the two have 16 and 22 bits): from the rounded output alone dQ and dK
+// and fp16; together the two have 16 and 22 bits, in fp16 down to outputs of 2^-14, kRestLift in
+// grouped_attn.h): from the rounded output alone dQ and dK
 // are 1.55 to 2.4 times as far from 64 bits as one rounding of the result (the most
 // for sequences of a few tokens), so 1.45 times. 16-bit inputs have P and dS rounded to
 // their type for these products, one rounding more than the result's own (fp32
@@ -186,19 +187,20 @@ __global__ __launch_bounds__(kThreads, (sizeof(T) == 2 && HD <= 64 ? 3 : (HD * (
     if constexpr (sizeof(T) == 2) Wave::read(xz, reinterpret_cast<const T*>(a.rest) + at, a.vo.st, a.vo.sh, a.Dv, places, end, lane);
     const uint32_t turn = QS::kOwn ? lds_offset(smem) + QS::kTiles + rb * Wave::kBytes : tiles + SH::kBytes + rb * Wave::kBytes;
     frag_t<T> y[KS];
-    auto dot = [&] {
+    auto dot = [&](float x) {
 #pragma unroll
       for (int s = 0; s < KS; ++s)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sum = fmaf((float)of[s][j], (float)y[s][j], sum);
+        for (int j = 0; j < 8; ++j) x = fmaf((float)of[s][j], (float)y[s][j], x);
+      return x;
     };
     Wave::turn(xq, turn, lane, qf);
     Wave::turn(xo, turn, lane, of);
     Wave::turn(xy, turn, lane, y);
-    dot();
+    sum = dot(0.f);
     if constexpr (sizeof(T) == 2) {
       Wave::turn(xz, turn, lane, y);
-      dot();
+      sum = kRestLift<T> == 1.f ? dot(sum) : fmaf(dot(0.f), 1.f / kRestLift<T>, sum);
     }
   }
   float del = pair_sum(sum);

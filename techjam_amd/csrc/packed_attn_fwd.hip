@@ -131,7 +131,7 @@ __global__ __launch_bounds__(kThreads, (HD * (int)sizeof(T) <= 256 ? 2 : 1)) voi
     Wave::write(reinterpret_cast<T*>(a.rest) + at, a.vo.st, a.vo.sh, a.Dv, places, R, turn, lane, [&](int d, int c) {
       float4_t y = value(d, c);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) y[j] -= (float)(T)y[j];
+      for (int j = 0; j < 4; ++j) y[j] = (y[j] - (float)(T)y[j]) * kRestLift<T>;
       return y;
     });
   }
