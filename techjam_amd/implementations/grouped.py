@@ -16,7 +16,7 @@ import torch
 import torch.nn as nn
 
 from ..kernels.grouped import check_parents, packed_attention, tree_attention
-from ..model import Linear, prefix_lengths
+from ..model import Linear, not_captured, prefix_lengths
 
 
 class GroupedCache:
@@ -61,8 +61,10 @@ class GroupedState:
         move to the places behind what was settled; the other drafts are dropped.
 
         ``counts`` on the host say how long the longest sequence is now; on the device they are not
-        waited for, and the bound grows by ``M``, until :meth:`recount`.
+        waited for, and the bound grows by ``M``, until :meth:`recount`. Not for graphs: a replay would
+        settle tokens that the bound does not count.
         """
+        not_captured()
         if self.drafts == 0:
             raise ValueError("there are no drafts to accept: the last call was no step over a tree")
         b = self.lengths.shape[0]
@@ -87,6 +89,7 @@ class GroupedState:
 
     def recount(self) -> None:
         """Asks the device (and waits for it) how long the longest sequence is."""
+        not_captured()
         self.longest = int(self.lengths.max())
 
 

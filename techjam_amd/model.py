@@ -437,12 +437,12 @@ class EncoderBlock(nn.Module):
                                              norm_dtype=f16 if fp16_operands and not last else f32))
 
 
-def _not_captured() -> None:
+def not_captured() -> None:
     """A replay would not count its tokens against the caches' capacity."""
     if torch.cuda.is_available() and torch.cuda.is_current_stream_capturing():
         from .errors import UnsupportedCaseError
 
-        raise UnsupportedCaseError("prefill and step keep count on the host and cannot be captured into a graph")
+        raise UnsupportedCaseError("prefill, step and accept keep count on the host and cannot be captured into a graph")
 
 
 def _must(t):
@@ -538,7 +538,7 @@ class TransformerEncoder(nn.Module):
     def prefill(self, x, state, valid_token_mask: Optional[torch.Tensor] = None):
         """The forward pass of each sequence's first tokens (``x`` ``[B, S, D]``,
         right-padded by the mask) that leaves their keys and values in ``state``."""
-        _not_captured()
+        not_captured()
         self._check_state(x, state)
         if x.shape[1] > state.capacity:
             raise ValueError(f"{x.shape[1]} tokens exceed the cache's capacity of {state.capacity}")
@@ -561,7 +561,7 @@ class TransformerEncoder(nn.Module):
         """:meth:`prefill` of prompts laid end to end (grouped attention; ``x`` and ``offsets`` as in
         :meth:`forward_packed`, one sequence for each of ``state``): their outputs, ``[T, D]``. Waits for the
         device once, to look at the offsets."""
-        _not_captured()
+        not_captured()
         self._check_packed(x)
         batch = state.lengths.shape[0]
         if offsets.shape != (batch + 1,):
@@ -610,7 +610,7 @@ class TransformerEncoder(nn.Module):
         ``kernels.tree_attention``) the tokens are drafts that form trees: each sees the settled tokens
         and its own line of parents. Nothing is settled by that: ``state.accept`` makes one line of them
         the sequence's next tokens, and the next step drops the others."""
-        _not_captured()
+        not_captured()
         self._check_state(x, state)
         if parents is not None and self.attention != "grouped":
             from .errors import UnsupportedCaseError

@@ -27,3 +27,24 @@ def test_gradients_of_small_values(dtype, causal, size, loss_scale):
     for name, (value, bound) in packed(q, k, v, [0, 200, 500], causal, None, None, dout).items():
         # The output of fp16 is as far off as its steps of 2^-24 are wide: check adds them to its bound.
         check(name, got[name], value, bound, None if name == "out" else norm_of(dtype))
+
+
+# -- states ----------------------------------------------------------------------
+
+def test_accepting_is_not_captured():
+    from techjam_amd import UnsupportedCaseError
+    from test_grouped_model_gpu import encoder
+
+    model, x, _ = encoder()
+    state = model.new_state(3, 12)
+    x = x.cuda()
+    path, counts = torch.tensor([[0, 1]] * 3).cuda(), torch.tensor([2, 1, 0]).cuda()
+    with torch.no_grad():
+        model.prefill(x[:, :8], state)
+        model.step(x[:, :2], state, torch.tensor([[-1, 0]] * 3, dtype=torch.int32).cuda())
+        graph = torch.cuda.CUDAGraph()
+        with torch.inference_mode(), torch.cuda.graph(graph), pytest.raises(UnsupportedCaseError, match="captured"):
+            state.accept(path, counts)
+        assert state.lengths.tolist() == [8, 8, 8] and state.longest == 8 and state.drafts == 2
+        state.accept(path, counts)
+        assert state.lengths.tolist() == [10, 9, 8] and state.longest == 10 and state.drafts == 0
