@@ -26,6 +26,12 @@ class GroupedCache:
         self.k = torch.zeros(batch, kv_heads, capacity, head_dim, dtype=dtype, device=device)
         self.v = torch.zeros(batch, kv_heads, capacity, head_dim, dtype=dtype, device=device)
 
+    def check_type(self, dtype: torch.dtype) -> None:
+        """Refuses keys and values of another type, which a copy would round in silence."""
+        if dtype != self.k.dtype:
+            raise ValueError(f"the cache holds {self.k.dtype}, the call's keys and values are {dtype}: "
+                             "create the state in that dtype")
+
 
 class GroupedState:
     """Every layer's cache and the sequences' settled lengths (int32 ``[B]`` on the device).
@@ -139,6 +145,7 @@ class GroupedSelfAttention(nn.Module):
         b, s, _ = x.shape
         q, k, v = self.qkv(x)
         if cache is not None:
+            cache.check_type(k.dtype)
             cache.k[:, :, :s] = k.transpose(1, 2)
             cache.v[:, :, :s] = v.transpose(1, 2)
         offsets = torch.arange(0, b * s + 1, s, dtype=torch.int32, device=x.device) if s else x.new_zeros(b + 1, dtype=torch.int32)
@@ -165,9 +172,7 @@ class GroupedSelfAttention(nn.Module):
         ``parents``, the last of ``lengths`` (these included), whose places in the cache are ``place``
         (int64 ``[B, T]``)."""
         q, k, v = self.qkv(x)
-        if k.dtype != cache.k.dtype:
-            raise ValueError(f"the cache holds {cache.k.dtype}, the step's keys and values are {k.dtype}: "
-                             "create the state in that dtype")
+        cache.check_type(k.dtype)
         rows = torch.arange(x.shape[0], device=x.device)[:, None]
         cache.k[rows, :, place] = k
         cache.v[rows, :, place] = v

@@ -523,7 +523,8 @@ class TransformerEncoder(nn.Module):
     def new_state(self, batch: int, capacity: int, dtype: Optional[torch.dtype] = None):
         """Empty caches for ``batch`` sequences of up to ``capacity`` tokens. Their
         type is that of the steps' projections: the parameters' (the default),
-        or autocast's for steps under it; a step whose type differs is refused."""
+        or autocast's for steps under it; a step whose type differs is refused, and with
+        grouped attention a prefill too."""
         from .errors import UnsupportedCaseError
         from .implementations.differential import DifferentialState
         from .implementations.grouped import GroupedState
@@ -582,9 +583,7 @@ class TransformerEncoder(nn.Module):
         place = (row - offsets[sequence]).long()
         for layer, cache in zip(self.layers, state.layers):
             def keep(k, v):
-                if k.dtype != cache.k.dtype:
-                    raise ValueError(f"the cache holds {cache.k.dtype}, the prompts' keys and values are {k.dtype}: "
-                                     "create the state in that dtype")
+                cache.check_type(k.dtype)
                 cache.k[sequence, :, place] = k
                 cache.v[sequence, :, place] = v
             x = layer.forward_packed(x, offsets, True, keep)

@@ -48,3 +48,20 @@ def test_accepting_is_not_captured():
         assert state.lengths.tolist() == [8, 8, 8] and state.longest == 8 and state.drafts == 2
         state.accept(path, counts)
         assert state.lengths.tolist() == [10, 9, 8] and state.longest == 10 and state.drafts == 0
+
+
+def test_prompts_are_not_rounded_into_a_cache_of_another_type():
+    from test_grouped_model_gpu import encoder
+
+    model, x, lengths = encoder()
+    mask = (torch.arange(x.shape[1])[None, :] < lengths[:, None]).cuda()
+    with torch.no_grad():
+        for dtype in (torch.float16, torch.bfloat16):
+            state = model.new_state(3, 50, dtype)
+            with pytest.raises(ValueError, match="create the state in that dtype"):
+                model.prefill(x.cuda(), state, mask)
+            assert not state.lengths.any() and state.longest == 0
+            with torch.autocast("cuda", dtype):  # whose projections have that type
+                model.prefill(x.cuda(), state, mask)
+                assert model.step(x.cuda()[:, :1], state).isfinite().all()
+            assert state.lengths.tolist() == [n + 1 for n in lengths.tolist()]

@@ -29,3 +29,20 @@ def test_accept_and_recount_are_not_captured(monkeypatch):
     state.accept(torch.zeros(2, 1, dtype=torch.long), torch.ones(2, dtype=torch.long))
     state.recount()
     assert state.lengths.tolist() == [5, 5] and state.longest == 5
+
+
+# -- caches of another type --------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16, torch.float64])
+def test_first_tokens_are_not_rounded_into_a_cache_of_another_type(dtype):
+    """The step that follows would be refused, with the prompts already rounded."""
+    m = model()
+    cache = m.new_state(2, 8, dtype).layers[0]
+    cache.k.fill_(7)
+    cache.v.fill_(7)
+    attention, lengths = m.layers[0].attention, torch.full((2,), 4, dtype=torch.int32)
+    with pytest.raises(ValueError, match="create the state in that dtype"):
+        attention(torch.randn(2, 4, 32), None, True, lengths, cache)
+    with pytest.raises(ValueError, match="create the state in that dtype"):
+        attention.step(torch.randn(2, 1, 32), cache, lengths, torch.full((2, 1), 3))
+    assert (cache.k == 7).all() and (cache.v == 7).all()
