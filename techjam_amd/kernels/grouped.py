@@ -225,6 +225,14 @@ def packed_attention(
 
 # -- drafted tokens against a cache ---------------------------------------------
 
+def _queries_view(t: torch.Tensor) -> torch.Tensor:
+    """``_rows_view`` of the new tokens, whose heads the kernels reach by 32-bit numbers of elements."""
+    if t.stride(1) >= 1 << 31:
+        # One head's stride is never used.
+        t = t.contiguous() if t.shape[1] > 1 else t.as_strided(t.shape, (t.stride(0), 0, *t.stride()[2:]))
+    return _rows_view(t)
+
+
 def check_parents(parents: torch.Tensor, b: int, t: int, dev: torch.device) -> None:
     """Refuses what cannot be the parents of ``t`` drafts of each of ``b`` sequences."""
     if t > MAX_DRAFTS:
@@ -292,7 +300,8 @@ def tree_attention(
         raise UnsupportedCaseError("tree_attention has no gradients; call it under torch.no_grad()")
     dev = _require_device(q, k_cache, v_cache)
     _check_ints("lengths", lengths, (b,), dev)
-    q, k, v = map(_rows_view, _padded(q, k_cache, v_cache))
+    q, k, v = _padded(q, k_cache, v_cache)
+    q, k, v = _queries_view(q), _rows_view(k), _rows_view(v)
     dtype = DTYPES[q.dtype]
     d, wide = q.shape[-1], v.shape[-1]
     out = _empty_heads(b, h, t, wide, q)

@@ -7,6 +7,7 @@ import torch
 
 from grouped_reference import check, packed
 from test_grouped_gpu import inputs, norm_of, run_packed
+from test_grouped_use_gpu import draft_inputs, run_tree
 
 pytestmark = pytest.mark.gpu
 
@@ -27,6 +28,21 @@ def test_gradients_of_small_values(dtype, causal, size, loss_scale):
     for name, (value, bound) in packed(q, k, v, [0, 200, 500], causal, None, None, dout).items():
         # The output of fp16 is as far off as its steps of 2^-24 are wide: check adds them to its bound.
         check(name, got[name], value, bound, None if name == "out" else norm_of(dtype))
+
+
+# -- strides -----------------------------------------------------------------------
+
+def test_new_tokens_whose_heads_are_far_apart():
+    """Heads 2^31 elements apart, and one head with such a stride, give what the same tokens side by side give."""
+    b, h, t, d = 2, 2, 3, 64
+    q, k, v = draft_inputs(b, h, 1, t, 300, d, torch.float16)
+    parents = [[-1, 0, 0]] * b
+    want = run_tree(q, k, v, [300, 120], parents)
+    big = torch.empty((1 << 31) + 64 + b * t * d, dtype=torch.float16, device="cuda")
+    far = big.as_strided((b, h, t, d), (t * d, (1 << 31) + 64, d, 1)).copy_(q)
+    assert torch.equal(run_tree(far, k, v, [300, 120], parents), want)
+    one = big.as_strided((b, 1, t, d), (t * d, 1 << 33, d, 1))
+    assert torch.equal(run_tree(one, k, v, [300, 120], parents), run_tree(q[:, :1].contiguous(), k, v, [300, 120], parents))
 
 
 # -- states ----------------------------------------------------------------------

@@ -2,11 +2,15 @@
 
 from __future__ import annotations
 
+import sys
+
 import pytest
 import torch
 
 from techjam_amd import UnsupportedCaseError
 from test_grouped_host import model
+
+kernels = sys.modules["techjam_amd.kernels.grouped"]
 
 
 # -- what a graph's replay would not count ----------------------------------------
@@ -46,3 +50,28 @@ def test_first_tokens_are_not_rounded_into_a_cache_of_another_type(dtype):
     with pytest.raises(ValueError, match="create the state in that dtype"):
         attention.step(torch.randn(2, 1, 32), cache, lengths, torch.full((2, 1), 3))
     assert (cache.k == 7).all() and (cache.v == 7).all()
+
+
+# -- strides past what the kernels multiply ------------------------------------------
+
+def _far(shape, strides):
+    n = sum((a - 1) * b for a, b in zip(shape, strides)) + 1
+    t = torch.empty(n, dtype=torch.float16).as_strided(shape, strides)  # memory that is never touched takes none
+    t.copy_(torch.randn(shape, generator=torch.Generator().manual_seed(0)))
+    return t
+
+
+@pytest.mark.parametrize("shape,strides,in_place", [
+    ((2, 4, 3, 64), (768, 64, 256, 1), True),                    # a projection's
+    ((1, 2, 3, 64), (64, (1 << 31) + 64, 64, 1), False),         # heads too far apart for 32 bits
+    ((1, 2, 3, 64), (64, (1 << 31) - 64, 64, 1), True),
+    ((2, 1, 3, 64), (192, (1 << 33) + 1, 64, 1), True),          # one head: its stride is never used
+    ((2, 1, 3, 64), (192, 1 << 33, 64, 1), True),
+    ((2, 2, 1, 64), ((1 << 31) + 64, 64, 1 << 33, 1), True),     # sequences may be as far apart as they like
+])
+def test_new_tokens_are_read_in_place_where_they_can_be(shape, strides, in_place):
+    t = _far(shape, strides)
+    seen = kernels._queries_view(t)
+    assert torch.equal(seen, t) and (seen.data_ptr() == t.data_ptr()) == in_place
+    sb, sh, ss, sd = seen.stride()
+    assert sd == 1 and not (sb | sh | ss) % 8 and seen.data_ptr() % 16 == 0 and sh < 1 << 31 and ss * 64 * 2 < 1 << 31
