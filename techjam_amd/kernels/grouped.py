@@ -78,6 +78,13 @@ def _check_ints(name: str, t, shape, dev: torch.device) -> None:
         raise ValueError(f"{name} must be a contiguous int32 tensor of shape {tuple(shape)} on {dev}")
 
 
+def check_offsets(offsets, dev: torch.device) -> None:
+    """Refuses what cannot be the offsets of sequences laid end to end."""
+    if not isinstance(offsets, torch.Tensor) or offsets.ndim != 1 or offsets.shape[0] == 0:
+        raise ValueError("offsets must be an int32 tensor of one element more than there are sequences")
+    _check_ints("offsets", offsets, offsets.shape, dev)
+
+
 def _padded(q, k, v):
     """Head dims that fill no whole 16 bytes are zero-padded to the next that
     does: zeros add nothing to a score and give columns that are cut off."""
@@ -210,9 +217,7 @@ def packed_attention(
     scale = _scale(scale, d)
     refuse_tangents(q, k, v)
     dev = _require_device(q, k, v)
-    if not isinstance(offsets, torch.Tensor) or offsets.ndim != 1 or offsets.shape[0] == 0:
-        raise ValueError("offsets must be an int32 tensor of one element more than there are sequences")
-    _check_ints("offsets", offsets, offsets.shape, dev)
+    check_offsets(offsets, dev)
     if valid_len is not None:
         _check_ints("valid_len", valid_len, (offsets.shape[0] - 1,), dev)
     q, k, v = _padded(q, k, v)

@@ -503,7 +503,7 @@ class TransformerEncoder(nn.Module):
         """Sequences laid end to end, ``x`` ``[T, D]`` (grouped attention): tokens ``offsets[n] .. offsets[n + 1] - 1``
         (int32 ``[N + 1]`` on the device) are sequence ``n``. Rows before the first and behind the last sequence are not
         read and come out as zeros. Runs unfused, with gradients where they are enabled."""
-        self._check_packed(x)
+        self._check_packed(x, offsets)
         rows = torch.arange(x.shape[0], device=x.device)
         outside = ((rows < offsets[0]) | (rows >= offsets[-1]))[:, None]
         x = x.masked_fill(outside, 0)
@@ -511,13 +511,15 @@ class TransformerEncoder(nn.Module):
             x = layer.forward_packed(x, offsets, self.config.causal)
         return self.final_norm(x).masked_fill(outside, 0)
 
-    def _check_packed(self, x) -> None:
+    def _check_packed(self, x, offsets) -> None:
         from .errors import UnsupportedCaseError
+        from .kernels.grouped import check_offsets
 
         if self.attention != "grouped":
             raise UnsupportedCaseError("sequences laid end to end: encoders of grouped attention only")
         if x.ndim != 2 or x.shape[1] != self.config.d_model:
             raise ValueError(f"x must be [T, {self.config.d_model}], not {tuple(x.shape)}")
+        check_offsets(offsets, x.device)
 
     # -- token by token (causal differential or grouped attention) -----------
     def new_state(self, batch: int, capacity: int, dtype: Optional[torch.dtype] = None):
@@ -563,7 +565,7 @@ class TransformerEncoder(nn.Module):
         :meth:`forward_packed`, one sequence for each of ``state``): their outputs, ``[T, D]``. Waits for the
         device once, to look at the offsets."""
         not_captured()
-        self._check_packed(x)
+        self._check_packed(x, offsets)
         batch = state.lengths.shape[0]
         if offsets.shape != (batch + 1,):
             raise ValueError(f"offsets must be [{batch + 1}], one sequence for each of the state, not {tuple(offsets.shape)}")

@@ -75,3 +75,29 @@ def test_new_tokens_are_read_in_place_where_they_can_be(shape, strides, in_place
     assert torch.equal(seen, t) and (seen.data_ptr() == t.data_ptr()) == in_place
     sb, sh, ss, sd = seen.stride()
     assert sd == 1 and not (sb | sh | ss) % 8 and seen.data_ptr() % 16 == 0 and sh < 1 << 31 and ss * 64 * 2 < 1 << 31
+
+
+# -- packed prompts ------------------------------------------------------------------
+
+@pytest.mark.parametrize("offsets", [
+    torch.tensor([0, 3, 8]),                                    # int64
+    torch.tensor([0.0, 3.0, 8.0]), torch.tensor([0, 9, 3, 9, 8, 9], dtype=torch.int32)[::2], [0, 3, 8], None])
+def test_offsets_of_another_kind_leave_the_state_as_it_was(offsets):
+    """They are refused before the state is emptied, as offsets of the wrong values are."""
+    m = model()
+    state = m.new_state(2, 8)
+    state.lengths.fill_(6)
+    state.longest, state.drafts = 6, 2
+    with pytest.raises(ValueError, match="offsets"):
+        m.prefill_packed(torch.zeros(8, 32), offsets, state)
+    assert state.lengths.tolist() == [6, 6] and state.longest == 6 and state.drafts == 2
+    with pytest.raises(ValueError, match="offsets"):
+        m.forward_packed(torch.zeros(8, 32), offsets)
+
+
+@pytest.mark.parametrize("offsets", [torch.zeros(0, dtype=torch.int32), torch.zeros(1, 3, dtype=torch.int32),
+                                     torch.tensor(0, dtype=torch.int32), torch.zeros(3, dtype=torch.int32, device="meta")])
+def test_offsets_of_another_shape_or_place_are_refused(offsets):
+    for m in (model(), model(layers=0)):
+        with pytest.raises(ValueError, match="offsets"):
+            m.forward_packed(torch.zeros(8, 32), offsets)
