@@ -456,7 +456,8 @@ class TransformerEncoder(nn.Module):
 
     #: "fp32" (default): float32 GEMMs under torch's matmul precision setting.
     #: "fp16": GEMM operands rounded to fp16 with fp32 accumulation (the
-    #: mantissa of TF32); fused GPU path only, other paths raise.
+    #: mantissa of TF32); fused GPU path only, other paths raise (prefill and step
+    #: of differential attention take float32 ones whatever it says).
     gemm_operands = "fp32"
 
     def __init__(self, config: TransformerConfig) -> None:
@@ -477,13 +478,7 @@ class TransformerEncoder(nn.Module):
     def forward_layers(self, x, valid_token_mask=None, valid_len=None, gemm_operands=None):
         """The layer stack and final norm; ``gemm_operands`` overrides the
         model's setting for this call."""
-        operands = self.gemm_operands if gemm_operands is None else gemm_operands
-        if operands not in ("fp32", "fp16"):
-            raise ValueError(f"gemm_operands must be 'fp32' or 'fp16', not {operands!r}")
-        if operands == "fp16" and self.attention != "softmax":
-            from .errors import UnsupportedCaseError
-
-            raise UnsupportedCaseError(f"fp16 GEMM operands are not implemented for {self.attention} attention")
+        operands = self._operands(gemm_operands)
         if self._can_fuse_norms(x, valid_token_mask, valid_len):
             return self._forward_layers_fused(x, valid_token_mask, valid_len, operands)
         if operands == "fp16":
@@ -498,6 +493,17 @@ class TransformerEncoder(nn.Module):
         if valid_token_mask is not None:
             x.masked_fill_(~valid_token_mask[..., None], 0)  # x is the norm's fresh output
         return x
+
+    def _operands(self, gemm_operands: Optional[str] = None) -> str:
+        """The GEMM operands of a call, refused where its attention does not have them."""
+        operands = self.gemm_operands if gemm_operands is None else gemm_operands
+        if operands not in ("fp32", "fp16"):
+            raise ValueError(f"gemm_operands must be 'fp32' or 'fp16', not {operands!r}")
+        if operands == "fp16" and self.attention != "softmax":
+            from .errors import UnsupportedCaseError
+
+            raise UnsupportedCaseError(f"fp16 GEMM operands are not implemented for {self.attention} attention")
+        return operands
 
     def forward_packed(self, x, offsets):
         """Sequences laid end to end, ``x`` ``[T, D]`` (grouped attention): tokens ``offsets[n] .. offsets[n + 1] - 1``
@@ -520,6 +526,7 @@ class TransformerEncoder(nn.Module):
         if x.ndim != 2 or x.shape[1] != self.config.d_model:
             raise ValueError(f"x must be [T, {self.config.d_model}], not {tuple(x.shape)}")
         check_offsets(offsets, x.device)
+        self._operands()
 
     # -- token by token (causal differential or grouped attention) -----------
     def new_state(self, batch: int, capacity: int, dtype: Optional[torch.dtype] = None):
@@ -648,6 +655,7 @@ class TransformerEncoder(nn.Module):
         if self.attention == "grouped":
             from .implementations.grouped import grouped_heads
 
+            self._operands()
             head = grouped_heads(self.config)
         else:
             head = (2 * self.config.num_heads, d // self.config.num_heads // 2)

@@ -101,3 +101,25 @@ def test_offsets_of_another_shape_or_place_are_refused(offsets):
     for m in (model(), model(layers=0)):
         with pytest.raises(ValueError, match="offsets"):
             m.forward_packed(torch.zeros(8, 32), offsets)
+
+
+# -- operands ------------------------------------------------------------------------
+
+def test_fp16_operands_are_refused_everywhere():
+    """They are the fused softmax encoder's; the padded forward pass says so, and the others would take float32."""
+    m = model()
+    state = m.new_state(2, 8)
+    state.lengths.fill_(6)
+    state.longest, state.drafts = 6, 2
+    m.gemm_operands = "fp16"
+    offsets = torch.tensor([0, 3, 8], dtype=torch.int32)
+    for call in (lambda: m(torch.zeros(2, 8, 32)), lambda: m.forward_packed(torch.zeros(8, 32), offsets),
+                 lambda: m.prefill_packed(torch.zeros(8, 32), offsets, state), lambda: m.prefill(torch.zeros(2, 4, 32), state),
+                 lambda: m.step(torch.zeros(2, 1, 32), state),
+                 lambda: m.step(torch.zeros(2, 1, 32), state, torch.full((2, 1), -1, dtype=torch.int32))):
+        with pytest.raises(UnsupportedCaseError, match="fp16 GEMM operands"):
+            call()
+    assert state.lengths.tolist() == [6, 6] and state.longest == 6 and state.drafts == 2
+    m.gemm_operands = "bf16"
+    with pytest.raises(ValueError, match="gemm_operands"):
+        m.forward_packed(torch.zeros(8, 32), offsets)
