@@ -2,14 +2,72 @@
 
 from __future__ import annotations
 
+import random
+
 import pytest
 import torch
 
-from grouped_reference import check, packed
-from test_grouped_gpu import inputs, norm_of, run_packed
+from grouped_reference import check, packed, tree
+from test_grouped_gpu import DTYPES, inputs, ints, norm_of, offsets_of, run_packed
 from test_grouped_use_gpu import draft_inputs, run_tree
 
+from techjam_amd.kernels import _lib
+from techjam_amd.kernels.differential import DTYPES as CODES
+
 pytestmark = pytest.mark.gpu
+
+
+class Guarded:
+    """Tensors carved out of one buffer, 4 KiB of known bytes before, between and behind them."""
+
+    ROOM, BYTE = 4096, 0xA5
+
+    def __init__(self, **wanted):
+        sizes = {name: torch.empty(shape, dtype=dtype, device="meta").nbytes for name, (shape, dtype) in wanted.items()}
+        self.buffer = torch.full((self.ROOM + sum(-(-n // 256) * 256 + self.ROOM for n in sizes.values()),), self.BYTE,
+                                 dtype=torch.uint8, device="cuda")
+        self.guards, at, end = [], 0, 0
+        for name, (shape, dtype) in wanted.items():
+            at = -(-end // 256) * 256 + self.ROOM
+            self.guards.append((end, at))
+            end = at + sizes[name]
+            setattr(self, name, self.buffer[at:end].view(dtype).view(shape))
+        self.guards.append((end, self.buffer.numel()))
+
+    def check(self, what):
+        for a, b in self.guards:
+            assert (self.buffer[a:b] == self.BYTE).all(), f"{what}: bytes outside of a tensor were written"
+
+
+def strides(t):
+    return (_lib.strides3 if t.ndim == 3 else _lib.strides4)(t)
+
+
+def stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
+def packed_calls(q, k, v, dout, offsets, causal=True, valid_len=None, fill=None):
+    """Forward and backward through the C entry points, into guarded tensors."""
+    (t, h, d), (_, hk, dv) = q.shape, v.shape
+    n, lib, wide = offsets.shape[0] - 1, _lib.lib(), q.dtype == torch.float32
+    f32 = torch.float32
+    floats = lib.tj_packed_attn_bwd_workspace_bytes(t, n, h, hk) // 4
+    g = Guarded(o=((t, h, dv), q.dtype), rest=((t, h, dv), q.dtype), lse=((t, h), f32), dq=((t, h, d), q.dtype),
+                dk=((t, hk, d), q.dtype), dv=((t, hk, dv), q.dtype), ws=((floats,), f32))
+    if fill is not None:
+        g.ws.fill_(fill)
+    rest = None if wide else g.rest.data_ptr()
+    valid = None if valid_len is None else valid_len.data_ptr()
+    sizes, scale = (CODES[q.dtype], t, n, h, hk, d, dv), d ** -0.5
+    assert lib.tj_packed_attn_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), g.o.data_ptr(), *sizes, *map(strides, (q, k, v, g.o)),
+                                  scale, causal, offsets.data_ptr(), valid, g.lse.data_ptr(), rest, stream()) == _lib.TJ_OK
+    assert lib.tj_packed_attn_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), g.o.data_ptr(), rest, g.lse.data_ptr(),
+                                  dout.data_ptr(), g.dq.data_ptr(), g.dk.data_ptr(), g.dv.data_ptr(), *sizes,
+                                  *map(strides, (q, k, v, g.o, dout, g.dq, g.dk, g.dv)), scale, causal, offsets.data_ptr(),
+                                  valid, g.ws.data_ptr(), 4 * floats, stream()) == _lib.TJ_OK
+    torch.cuda.synchronize()
+    return g
 
 
 # -- values at the lower end of a type -------------------------------------------
@@ -28,6 +86,52 @@ def test_gradients_of_small_values(dtype, causal, size, loss_scale):
     for name, (value, bound) in packed(q, k, v, [0, 200, 500], causal, None, None, dout).items():
         # The output of fp16 is as far off as its steps of 2^-24 are wide: check adds them to its bound.
         check(name, got[name], value, bound, None if name == "out" else norm_of(dtype))
+
+
+# -- nothing outside of the tensors is written ---------------------------------------
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("t,h,hk,d", [(200, 4, 2, 64), (2100, 8, 1, 32), (5000, 8, 4, 64), (150, 6, 2, 80)])
+def test_bytes_around_packed_tensors_stay(dtype, t, h, hk, d):
+    """Offsets in order and out of it, up to 256 regions and beyond, key tiles that are shared and not."""
+    rng = random.Random(t)
+    q, k, v, dout = (x.contiguous() for x in inputs(t, h, hk, d, d, dtype, seed=t))
+    kept = [x.clone() for x in (q, k, v, dout)]
+    for offsets in ([0, t], offsets_of([t // 3, 0, t // 2], 3), [0, 500, 100, 200], [-50, 20, 10, 1 << 30], [t - 50, 100, 50, 0],
+                    [t, 0, t, 0, t], [-5, -4], [rng.randint(-300, t + 300) for _ in range(40)], [(1 << 31) - 1, -(1 << 31), 7] * 30,
+                    [rng.randint(0, t) for _ in range(400)], sorted(rng.randint(0, t) for _ in range(400))):
+        for causal in (True, False):
+            g = packed_calls(q, k, v, dout, ints(offsets), causal)
+            g.check(f"offsets {offsets[:6]}, causal {causal}")
+            if offsets == sorted(offsets) and 0 <= offsets[0] and offsets[-1] <= t:
+                got = dict(out=g.o, dq=g.dq, dk=g.dk, dv=g.dv)
+                want = run_packed(q, k, v, offsets, causal, dout)
+                assert all(torch.equal(got[n], want[n]) for n in got)
+    assert all(torch.equal(a, b) for a, b in zip((q, k, v, dout), kept))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("b,h,hk,t,c,d", [(3, 4, 2, 6, 300, 64), (2, 8, 1, 40, 1500, 32), (5, 3, 3, 1, 2000, 128), (2, 8, 2, 64, 900, 80)])
+def test_bytes_around_drafts_stay(dtype, b, h, hk, t, c, d):
+    """Whatever the lengths and parents are."""
+    lib, rng = _lib.lib(), random.Random(c)
+    q, k, v = (x.contiguous() for x in draft_inputs(b, h, hk, t, c, d, dtype, seed=c))
+    sizes = (CODES[dtype], b, h, hk, t, c, d, d)
+    floats = lib.tj_tree_attn_workspace_bytes(*sizes) // 4
+    wild = [(1 << 31) - 1, -(1 << 31), -1, t, t - 1, c, 1 << 20]
+    for form in ("chain", "tree", "wild"):
+        lengths = [rng.choice(wild) for _ in range(b)] if form == "wild" else [rng.randint(0, c) for _ in range(b)]
+        parents = None if form == "chain" else [
+            [rng.choice(wild) if form == "wild" and rng.random() < 0.3 else rng.randint(-1, i - 1) for i in range(t)] for _ in range(b)]
+        g = Guarded(o=((b, h, t, d), dtype), ws=((floats,), torch.float32))
+        held = [ints(lengths), None if parents is None else ints(parents)]
+        assert lib.tj_tree_attn_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), g.o.data_ptr(), *sizes, *map(strides, (q, k, v, g.o)),
+                                    d ** -0.5, held[0].data_ptr(), None if parents is None else held[1].data_ptr(),
+                                    g.ws.data_ptr() if floats else None, 4 * floats, stream()) == _lib.TJ_OK
+        torch.cuda.synchronize()
+        g.check(f"{form}, lengths {lengths}")
+        value, bound = tree(q, k, v, lengths, parents)
+        check(form, g.o, value, bound, norm_of(dtype))
 
 
 # -- strides -----------------------------------------------------------------------

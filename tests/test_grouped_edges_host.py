@@ -2,6 +2,7 @@
 
 from __future__ import annotations
 
+import random
 import sys
 
 import pytest
@@ -123,3 +124,25 @@ def test_fp16_operands_are_refused_everywhere():
     m.gemm_operands = "bf16"
     with pytest.raises(ValueError, match="gemm_operands"):
         m.forward_packed(torch.zeros(8, 32), offsets)
+
+
+# -- offsets out of order ----------------------------------------------------------------
+
+def test_offsets_out_of_order_reach_nothing_outside():
+    """Whatever region and tile a workgroup finds: with offsets clipped to 0 .. T and the tile's rows checked against the
+    region's, as the kernels do both, its rows, their numbers and their peaks lie within what is allocated."""
+    rng = random.Random(2)
+    lists = [[0, 500, 100, 200], [-50, 20, 10, 1 << 30], [150, 100, 50, 0], [(1 << 31) - 1, -(1 << 31), 7] * 30]
+    lists += [[rng.randint(-300, 700) for _ in range(rng.randint(1, 60))] for _ in range(200)]
+    for offsets in lists:
+        t, n = rng.choice((1, 63, 64, 200, 500)), len(offsets) - 1
+        edges = [0] + [min(t, max(0, x)) for x in offsets] + [t]
+        for j in range(n + 2):
+            start, rows = edges[j], max(0, edges[j + 1] - edges[j])
+            assert 0 <= start and start + rows <= t
+            for unit in (32, 64):  # the numbers of 32 tokens, the peaks of 64
+                assert rows == 0 or start // unit + j + (rows - 1) // unit < t // unit + n + 2
+            for per, unit in ((1, 64), (2, 32), (3, 128), (8, 64)):
+                for tile in range(-(-rows * per // unit)):  # those that there() lets through
+                    first, last = tile * unit // per, min(rows * per, (tile + 1) * unit) - 1
+                    assert first < rows and last // per < rows
