@@ -185,3 +185,36 @@ def test_prompts_are_not_rounded_into_a_cache_of_another_type():
                 model.prefill(x.cuda(), state, mask)
                 assert model.step(x.cuda()[:, :1], state).isfinite().all()
             assert state.lengths.tolist() == [n + 1 for n in lengths.tolist()]
+
+
+# -- gradients against differences -------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("causal", [True, False])
+def test_gradients_against_differences_along_them(dtype, causal):
+    """The slope along the gradient itself, of unit size an element, and a tenth of a random direction: <g, way> is nearly
+    |g| |way|, so that a gradient of another size or without a term shows.
+
+    Central differences in 64 bits with steps h = 2^-12: with way's largest element below 6, a score moves by
+    d <= 6 h (sum |k|) / sqrt(32) < 2^-5 a row, and the third-order term (d^2 / 6, times the fourth cumulants' factor of
+    at most 26) is below 0.5 % of the slope. The kernels' own error is what their gradients are held to."""
+    q, k, v, dout = inputs(90, 4, 2, 32, 32, dtype)
+    dout = (dout.float() * 10).to(dtype)
+    offsets = [0, 33, 90]
+    got = run_packed(q, k, v, offsets, causal, dout)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    for name, x in (("dq", q), ("dk", k), ("dv", v)):
+        grad = got[name].double()
+        noise = torch.randn(x.shape, generator=g, device="cuda").double()
+        way = (grad / grad.square().mean().sqrt()).clamp(-5, 5) + 0.1 * noise
+        step = 2.0 ** -12
+        ends = []
+        for sign in (1, -1):
+            moved = {"dq": q.double(), "dk": k.double(), "dv": v.double()}
+            moved[name] = moved[name] + sign * step * way
+            out = packed(moved["dq"], moved["dk"], moved["dv"], offsets, causal)["out"][0]
+            ends.append((out * dout.double()).sum())
+        slope = (ends[0] - ends[1]) / (2 * step)
+        err = ((grad * way).sum() - slope).abs()
+        assert slope > 0.8 * grad.norm() * way.norm(), name
+        assert err <= 0.005 * slope + norm_of(dtype) * grad.norm() * way.norm(), name
