@@ -218,3 +218,49 @@ def test_gradients_against_differences_along_them(dtype, causal):
         err = ((grad * way).sum() - slope).abs()
         assert slope > 0.8 * grad.norm() * way.norm(), name
         assert err <= 0.005 * slope + norm_of(dtype) * grad.norm() * way.norm(), name
+
+
+# -- how many workgroups share a key tile's rows -------------------------------------------
+
+def expected_shares(dtype, t, n, h, hk):
+    """The rule beside packed_bwd_shares: up to 1024 workgroups (float32: 512) and 16 rounds each or more (four)."""
+    tiles = max(1, (t + 63) // 64 * hk)
+    rounds = (t // max(n, 1) + 31) // 32 * (h // hk) // 2
+    most, least = (512, 4) if dtype == torch.float32 else (1024, 16)
+    shares = max(1, min(16, most // tiles, rounds // least))
+    return 1 if shares == 2 and dtype != torch.float32 and tiles <= 128 else shares
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lengths,first,tail,h,hk,d,dv,shares,shares32", [
+    ([700, 0, 1321, 33], 5, 70, 8, 1, 64, 64, 4, 15),
+    ([1100], 5, 70, 32, 1, 32, 16, 16, 16),
+    ([900, 1, 1030], 5, 70, 12, 2, 128, 40, 3, 8),
+    ([1500], 5, 70, 10, 2, 80, 96, 7, 10),
+    ([700, 680], 1, 2, 8, 8, 64, 64, 1, 2),
+    ([1024], 1, 2, 4, 4, 32, 32, 1, 4),
+    ([600, 400], 1, 2, 3, 1, 96, 96, 1, 6),
+    ([1000], 1, 2, 8, 4, 128, 128, 1, 8),
+])
+def test_key_tiles_are_shared_among_as_many_as_the_rule_says(dtype, lengths, first, tail, h, hk, d, dv, shares, shares32):
+    """Counted in the workspace: every sharing workgroup leaves a slab of sums there, behind the rows' numbers."""
+    t, n, offsets = first + sum(lengths) + tail, len(lengths), offsets_of(lengths, first)
+    wide = dtype == torch.float32
+    want = shares32 if wide else shares
+    assert expected_shares(dtype, t, n, h, hk) == want
+    q, k, v, dout = (x.contiguous() for x in inputs(t, h, hk, d, dv, dtype, seed=h))
+    mark = -1.2345e30
+    g = packed_calls(q, k, v, dout, ints(offsets), fill=mark)
+    g.check("shared key tiles")
+    numbers = (t // 32 + n + 2) * h * 64 + (t // 64 + n + 2) * hk * 2
+    sums, slab = g.ws[-(-numbers // 4) * 4:], t * hk * (d + dv)
+    written = (sums != mark).nonzero()
+    most = max(expected_shares(x, t, n, h, hk) for x in DTYPES)
+    assert g.ws.numel() == -(-numbers // 4) * 4 + (0 if most == 1 else most * t * hk * 256)
+    if want == 1:
+        assert written.numel() == 0
+    else:
+        assert (sums[:want * slab] != mark).all() and (sums[want * slab:] == mark).all()
+    # Any number of them gives the gradients.
+    for name, (value, bound) in packed(q, k, v, offsets, True, None, None, dout).items():
+        check(name, getattr(g, {"out": "o"}.get(name, name)), value, bound, norm_of(dtype))
