@@ -264,3 +264,47 @@ def test_key_tiles_are_shared_among_as_many_as_the_rule_says(dtype, lengths, fir
     # Any number of them gives the gradients.
     for name, (value, bound) in packed(q, k, v, offsets, True, None, None, dout).items():
         check(name, getattr(g, {"out": "o"}.get(name, name)), value, bound, norm_of(dtype))
+
+
+# -- encoders of 16-bit parameters ----------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_sixteen_bit_encoders_against_64_bits(dtype):
+    """Values and gradients of an encoder of rounded parameters, and of its prefill and step.
+
+    Two layers of about a dozen operators and the last norm round their results 25 times on a value's way, each by at
+    most half a step of it: together at most 25 half steps of the 2-norm (a norm or a softmax that raises an error is
+    made up for by signs that differ). Gradients pass as many again, of operands as far off: 60."""
+    from test_grouped_model_gpu import encoder, params_of, plain_forward
+
+    u = torch.finfo(dtype).eps / 2
+
+    def near(got, want, roundings, size=None):
+        err = (got.detach().cpu().double() - want.detach()).norm().item()
+        assert err <= roundings * u * (want.norm().item() if size is None else size), err / want.norm().item()
+
+    model, x, lengths = encoder()
+    model = model.to(dtype)
+    x = x.to(dtype)
+    mask = torch.arange(x.shape[1])[None, :] < lengths[:, None]
+    params = params_of(model)
+    want = plain_forward(params, x.double(), lengths, 4, 2, 2, True)
+    out = model(x.cuda(), mask.cuda())
+    assert out.dtype == dtype and not out[~mask.cuda()].any()
+    near(out, want, 25)
+    weight = torch.randn(x.shape, generator=torch.Generator().manual_seed(2)).to(dtype)
+    names, leaves = zip(*model.named_parameters())
+    got = torch.autograd.grad(out, leaves, weight.cuda())
+    ref = torch.autograd.grad(want, list(params.values()), weight.double())
+    largest = max(r.norm().item() for r in ref)
+    for name, g, r in zip(names, got, ref):
+        # A key bias moves every score of a row alike: its gradient is zero but for rounding.
+        near(g, r, 60, largest if name.endswith("k_proj.bias") else None)
+    new = torch.randn(3, 3, x.shape[2], generator=torch.Generator().manual_seed(3)).to(dtype)
+    with torch.no_grad():
+        state = model.new_state(3, 50)
+        near(model.prefill(x.cuda(), state, mask.cuda()), want, 25)
+        steps = torch.cat((model.step(new[:, :1].cuda(), state), model.step(new[:, 1:].cuda(), state)), 1)
+        for b, n in enumerate(lengths.tolist()):
+            whole = torch.cat((x[b, :n], new[b])).double()[None]
+            near(steps[b], plain_forward(params, whole, torch.tensor([n + 3]), 4, 2, 2, True)[0, n:], 25)
