@@ -20,10 +20,11 @@
 // share the rows of few keys, their sums are joined in a fixed one); seven
 // products a pair are formed where five would do (the others need dQ by atomics).
 //
-// 1904 and 14480 tokens, 16 heads on 8, 128 dims, bf16, causal: dQ 1090 to 1120 us, 1190 TFLOP/s of its three
-// products (the forward kernel 820), dK and dV 1560 to 1620 us, 1100 TFLOP/s of its four; matrix units 64 and 57 %
-// busy, vector units 46 and 38, at 1.7 of 2.4 GHz: power, as in the forward kernel. 96 sequences of about 340
-// tokens, 16 heads on 4, 64 dims: dQ 126 us (of which 79 move rows: 335 MB), dK and dV 140: the first
+// Medians of a hundred calls after two hundred others. 1904 and 14480 tokens, 16 heads on 8, 128 dims, bf16, causal: dQ
+// 1137 us, 1153 TFLOP/s of its three products (the forward kernel 859 us), dK and dV 1648 us, 1060 TFLOP/s of its
+// four; matrix units 63 and 56 % busy, vector units 46 and 37, at 1.73 and 1.81 of 2.4 GHz: power, as in the forward kernel (4 % less
+// time on another card). 96 sequences of about 340
+// tokens, 16 heads on 4, 64 dims: dQ 124 us (of which 79 move rows: 335 MB), dK and dV 138: the first
 // 64 keys of the longest, 1870 tokens, have 118 rounds one after the other, 98 us if nothing else runs.
 #include <algorithm>
 

@@ -5,13 +5,15 @@
 // groups; key tiles of 32 or 64 stream through LDS, dealt to the groups in turn,
 // and the groups' sums meet in LDS at the end.
 //
-// Long sequences are bound by power: 32768 tokens, 8 heads on 2, 128 dims, bf16, causal take
-// 1924 us, 1143 TFLOP/s of 2D + 2Dv operations a pair (a large library product of that type
-// 1218), the matrix unit 63 % and the vector unit 55 % busy at a clock of 1.46 of 2.4 GHz. Short ones are
-// bound by what stands before and after their few key tiles: 96 sequences of about 340
-// tokens, 16 heads on 4, 64 dims take 92 us, of which looking for the tile, q, and the results
-// take 47 without any keys (235 MB, 5 TB/s), the vector unit 63 % busy. A batch of 24 prompts of up to
-// 2935 tokens, 16384 in all, 16 heads on 2, 128 dims: 117 us, of which the longest tile takes 90.
+// Medians of a hundred calls after two hundred others. Long sequences are bound by power: 32768 tokens, 8 heads on 2,
+// 128 dims, bf16, causal take 2032 us (1906 on another card), 1082 TFLOP/s of 2D + 2Dv operations a pair (a large
+// library product of that type 1218), the matrix unit 59 % and the vector unit 52 % busy at a clock of 1.72 of 2.4 GHz.
+// Short ones are bound by what stands before and after their few key tiles: 96 sequences of about 340
+// tokens, 16 heads on 4, 64 dims take 86 us, of which looking for the tile, q, and the results
+// take 47 without any keys (235 MB, 5 TB/s), the vector unit 61 % busy. A batch of 24 prompts of up to
+// 2935 tokens, 16384 in all, 16 heads on 2, 128 dims: 115 us. It is balanced (dealt to the 512 places of two workgroups
+// a CU, the 2068 tiles end after 47 rounds of 64 keys where the mean is 46), so a pair of rounds takes 2.4 us of a CU whose
+// matrix units need 0.9: with two waves a SIMD a wave's scores, exponentials and values follow each other.
 #include "grouped_attn.h"
 
 namespace tj {

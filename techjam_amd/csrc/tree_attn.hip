@@ -7,10 +7,10 @@
 // part of the keys, so that up to 256 rows read a key from memory once; the tiles are dealt to the
 // groups, whose sums meet in LDS at the end. Parts are joined by tree_join_kernel.
 //
-// Bound by the cache's bytes: 8 sequences of 22528 to 65536 keys, 16 drafts, 16 heads on 4, 128 dims, bf16: 130 us
-// + 6 of joining, 5.5 TB/s (a copy of 1 GiB: 5.1); 64 sequences of 1072 to 4096 keys, one token, 64 dims, fp16: 31 us + 4,
-// 5.4 TB/s. 256 rows a key head (64 drafts, 16 sequences of up to 8192 keys) take 56 us, 3.3 TB/s: every part
-// leaves 128 KB of sums, 34 MB in all, written in 7 us and joined in 9.
+// Medians of a hundred calls after two hundred others. Bound by the cache's bytes: 8 sequences of 22528 to 65536 keys, 16
+// drafts, 16 heads on 4, 128 dims, bf16: 132 us + 6 of joining, 5.5 TB/s (a copy of 1 GiB: 5.1); 64 sequences of 1072 to 4096
+// keys, one token, 64 dims, fp16: 31 us + 4, 5.5 TB/s. 256 rows a key head (64 drafts, 16 sequences of up to 8192 keys) take
+// 58 us, 3.2 TB/s: every part leaves 128 KB of sums, 34 MB in all, written in 7 us and joined in 9.
 #include "grouped_attn.h"
 
 namespace tj {
