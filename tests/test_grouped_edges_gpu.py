@@ -308,3 +308,21 @@ def test_sixteen_bit_encoders_against_64_bits(dtype):
         for b, n in enumerate(lengths.tolist()):
             whole = torch.cat((x[b, :n], new[b])).double()[None]
             near(steps[b], plain_forward(params, whole, torch.tensor([n + 3]), 4, 2, 2, True)[0, n:], 25)
+
+
+def test_packed_encoder_replays_in_a_graph():
+    """Inference over packed sequences, replayed with other rows and other offsets, eager calls between."""
+    from graph_capture import captured, replay
+    from test_grouped_model_gpu import encoder
+
+    model, x, _ = encoder()
+    rows, offsets = x[0].cuda().clone(), ints([0, 13, 40])
+    with torch.no_grad():
+        graph, held = captured(lambda: model.forward_packed(rows, offsets))
+        for n in range(4):
+            rows.normal_()
+            offsets.copy_(ints([n, 20 - 6 * n, 40 - 2 * n]))
+            torch.cuda.synchronize()
+            replay(graph)
+            torch.cuda.synchronize()
+            assert torch.equal(held, model.forward_packed(rows, offsets))
